@@ -1,0 +1,362 @@
+// AdamW over many variables in one launch, with both moments in 32 bits or in 8 bits, and the global norm of their gradients.
+//
+// A step t = 1, 2, ... with a variable's gradient g (the pieces `g`, `side[s] * side_scale[s]` and the constant l1 added up):
+//     g <- g * c,  c = 1 or clipnorm / norm over all variables
+//     m <- m + (g - m) (1 - beta_1)          v <- v + (g g - v) (1 - beta_2)          r = sqrt(v)
+//     w <- clip(w - w (lr decay) - m alpha / (r + epsilon), lo, hi),   alpha = lr sqrt(1 - beta_2^t) / (1 - beta_1^t)
+// in fp32 whatever the type of w and g; w is rounded to its type once, at the end.
+//
+// Moments in 8 bits.  m and r (not v: the square root halves the exponents a block spans) are E4M3 codes times a power of two
+// 2^(s - 127) per 256 elements, s = max(exponent field of the block's largest magnitude - 7, 1), so the largest lies in [128, 256).
+// The step of a slow average is far below half a code (1 - beta_2 = 0.001 against code distances of 1/16 to 1/8), so rounding
+// to the nearest code would never move it: codes are rounded stochastically, which keeps the average unbiased.  The 16-bit numbers
+// come from Philox4x32-7 (seven rounds: the fewest that pass the statistical tests of Salmon et al., SC'11; the rounding
+// draws 32 bits per element): word e % 4 of counter (e / 4, t), low half for m and high half for r.  As fp32 numbers scaled by
+// 2^-120, E4M3 values have their code, normal and subnormal, in bits 20 to 27, so rounding is one addition to the bits below and a shift.
+// An r above zero keeps at least the smallest code: a zero would let epsilon alone divide the next step.
+#include "hgq_device.h"
+#include "hgq_host.h"
+
+namespace hgq {
+
+constexpr int ADAMW_ITEMS = 28, ADAMW_PIECES = 32;
+constexpr int ADAMW_CHUNK = 2048;  // elements a workgroup takes at a time: eight blocks of 256
+constexpr int ADAMW_GRID = 2048;
+
+struct AdamwItem {
+    void *w;
+    const void *g;
+    void *m, *v;
+    uint8_t *m_scale, *v_scale;
+    int64_t n, first;
+    float l1, lo, hi, decay;
+    int type;
+    short piece, pieces;  // its entries of the launch's list of further gradient pieces
+};
+struct AdamwLaunch {
+    AdamwItem item[ADAMW_ITEMS];
+    const float *side[ADAMW_PIECES], *side_scale[ADAMW_PIECES];
+    uint32_t start[ADAMW_ITEMS + 1];  // first chunk of each item; the last entry: their number
+};
+struct AdamwSum {
+    const float *term[HGQ_SUM_BATCH];
+    int n;
+    float *out;
+};
+
+__device__ __forceinline__ float load_as_f32(const void *p, int64_t e, int type) {
+    if (type == HGQ_TYPE_F32) return ((const float *)p)[e];
+    const uint16_t h = ((const uint16_t *)p)[e];
+    if (type == HGQ_TYPE_BF16) return __uint_as_float((uint32_t)h << 16);
+    _Float16 f;
+    __builtin_memcpy(&f, &h, 2);
+    return (float)f;
+}
+
+__device__ __forceinline__ void store_f32_as(void *p, int64_t e, int type, float v) {
+    if (type == HGQ_TYPE_F32) {
+        ((float *)p)[e] = v;
+    } else if (type == HGQ_TYPE_BF16) {  // to the nearest, ties to even; a NaN stays one
+        const uint32_t b = __float_as_uint(v);
+        ((uint16_t *)p)[e] = v != v ? (uint16_t)((b >> 16) | 0x40) : (uint16_t)((b + 0x7fff + ((b >> 16) & 1)) >> 16);
+    } else {
+        ((_Float16 *)p)[e] = (_Float16)v;
+    }
+}
+
+// the gradient of element e: its pieces in the order of the descriptor, then the regularizer's constant
+__device__ __forceinline__ float gradient(const AdamwLaunch &a, const AdamwItem &it, int64_t e) {
+    float g = it.g ? load_as_f32(it.g, e, it.type) : 0.0f;
+    for (int s = 0; s < it.pieces; ++s) {
+        const float *scale = a.side_scale[it.piece + s], d = a.side[it.piece + s][e];
+        g = __fadd_rn(g, scale ? __fmul_rn(scale[0], d) : d);
+    }
+    return __fadd_rn(g, it.l1);
+}
+
+__device__ __forceinline__ void philox4x32_7(uint64_t counter, uint64_t step, uint64_t seed, uint32_t (&out)[4]) {
+    uint32_t c0 = (uint32_t)counter, c1 = (uint32_t)(counter >> 32), c2 = (uint32_t)step, c3 = (uint32_t)(step >> 32);
+    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 7; ++r) {
+        const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
+        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0, c1 = (uint32_t)p1, c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1, c3 = (uint32_t)p0;
+        k0 += 0x9E3779B9u, k1 += 0xBB67AE85u;
+    }
+    out[0] = c0, out[1] = c1, out[2] = c2, out[3] = c3;
+}
+
+// E4M3 code (0x7f: not a number) of a magnitude under the block's scale byte s, rounded by the 16-bit number h
+__device__ __forceinline__ uint32_t e4m3_code(float a, int s, uint32_t h) {
+    const uint32_t c = (__float_as_uint(ldexpf(a, 7 - s)) + (h << 4)) >> 20;
+    return a < __builtin_inff() ? c : 0x7fu;
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t code, int s) {
+    return ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)code, 0), s - 127);
+}
+
+__device__ __forceinline__ uint32_t exponent_field(float v) {  // of finite magnitudes; the others do not count
+    const uint32_t e = (__float_as_uint(v) >> 23) & 0xff;
+    return e == 255 ? 0 : e;
+}
+
+struct AdamwStep {
+    float c, alpha, lr, one_minus_b1, one_minus_b2, eps;
+    uint64_t t, seed;
+};
+
+// w <- the updated weight; m and r already hold the new moments
+__device__ __forceinline__ float adamw_weight(float w, float m, float r, const AdamwItem &it, const AdamwStep &k) {
+    w = __fsub_rn(w, __fmul_rn(w, __fmul_rn(k.lr, it.decay)));
+    w = __fsub_rn(w, __fdiv_rn(__fmul_rn(m, k.alpha), __fadd_rn(r, k.eps)));
+    return w < it.lo ? it.lo : w > it.hi ? it.hi : w;  // (not a number stays that)
+}
+
+// one variable's elements [e0, e0 + ADAMW_CHUNK): a lane takes four neighbours, a wavefront 256 - the block that shares a scale
+template <int BITS>
+__device__ __forceinline__ void adamw_chunk(const AdamwLaunch &a, const AdamwItem &it, const AdamwStep &k, int64_t e0) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t b = e0 + wave * 256; b < e0 + ADAMW_CHUNK && b < it.n; b += 1024) {
+        const int64_t e = b + lane * 4;
+        float m[4], r[4];
+        int sm = 0, sr = 0;
+        if (BITS == 8) sm = it.m_scale[b >> 8], sr = it.v_scale[b >> 8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m[j] = r[j] = 0.0f;
+            if (e + j < it.n) {
+                const float g = __fmul_rn(gradient(a, it, e + j), k.c);
+                float v;
+                if (BITS == 8) {
+                    m[j] = e4m3_value(((const uint8_t *)it.m)[e + j], sm);
+                    v = e4m3_value(((const uint8_t *)it.v)[e + j], sr);
+                    v = __fmul_rn(v, v);
+                } else {
+                    m[j] = ((const float *)it.m)[e + j], v = ((const float *)it.v)[e + j];
+                }
+                m[j] = __fadd_rn(m[j], __fmul_rn(__fsub_rn(g, m[j]), k.one_minus_b1));
+                v = __fadd_rn(v, __fmul_rn(__fsub_rn(__fmul_rn(g, g), v), k.one_minus_b2));
+                r[j] = __fsqrt_rn(v);
+                store_f32_as(it.w, e + j, it.type, adamw_weight(load_as_f32(it.w, e + j, it.type), m[j], r[j], it, k));
+                if (BITS == 32) ((float *)it.m)[e + j] = m[j], ((float *)it.v)[e + j] = v;
+            }
+        }
+        if (BITS == 8) {
+            uint32_t em = 8, er = 8;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) em = max(em, exponent_field(m[j])), er = max(er, exponent_field(r[j]));
+#pragma unroll
+            for (int d = 32; d; d >>= 1) em = max(em, (uint32_t)__shfl_xor((int)em, d)), er = max(er, (uint32_t)__shfl_xor((int)er, d));
+            sm = (int)em - 7, sr = (int)er - 7;
+            uint32_t h[4];
+            philox4x32_7((uint64_t)(it.first + e) >> 2, k.t, k.seed, h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (e + j < it.n) {
+                    uint32_t cr = e4m3_code(r[j], sr, h[j] >> 16);
+                    if (cr == 0 && r[j] > 0.0f) cr = 1;
+                    ((uint8_t *)it.m)[e + j] = (uint8_t)(e4m3_code(fabsf(m[j]), sm, h[j] & 0xffff) | (signbit(m[j]) ? 0x80u : 0u));
+                    ((uint8_t *)it.v)[e + j] = (uint8_t)cr;
+                }
+            if (lane == 0) it.m_scale[b >> 8] = (uint8_t)sm, it.v_scale[b >> 8] = (uint8_t)sr;
+        }
+    }
+}
+
+// sum of the workgroup's values, in a fixed order, returned to every thread
+__device__ __forceinline__ double block_sum(double v, double *lds) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < (int)blockDim.x >> 6; ++w) v += lds[w];
+    __syncthreads();
+    return v;
+}
+
+__device__ __forceinline__ float norm_of_parts(const double *parts, int n, double *lds) {
+    double v = 0;
+    for (int p = threadIdx.x; p < n; p += 256) v += parts[p];
+    return (float)sqrt(block_sum(v, lds));
+}
+
+// The step's number, the powers of the decay rates and the learning rate live in device memory (hgq_adamw_state), so a recorded launch
+// moves on at every replay.  All workgroups read them; the last one to finish the step's last launch writes the next step's.
+template <int BITS>
+__global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum, hgq_adamw_state *state, double b1, double b2, float eps,
+                                                    float clipnorm, const double *parts, int n_parts, float *norm_out, uint64_t seed, int items,
+                                                    int last) {
+    __shared__ double lds[4];
+    if (sum.n > 0 && blockIdx.x == 0 && threadIdx.x == 0) {  // the step's loss terms, which the update does not read
+        float v = sum.term[0][0];
+        for (int t = 1; t < sum.n; ++t) v = __fadd_rn(v, sum.term[t][0]);
+        sum.out[0] = v;
+    }
+    AdamwStep k;
+    const int64_t t = state->step + 1;
+    const double p1 = state->beta_1_power * b1, p2 = state->beta_2_power * b2, lr = state->lr;
+    k.alpha = (float)(lr * sqrt(1.0 - p2) / (1.0 - p1)), k.lr = (float)lr, k.t = (uint64_t)t, k.seed = seed;
+    k.one_minus_b1 = (float)(1.0 - b1), k.one_minus_b2 = (float)(1.0 - b2), k.eps = eps;
+    k.c = 1.0f;
+    if (n_parts > 0) {
+        const float norm = norm_of_parts(parts, n_parts, lds);
+        // no clipping up to the bound; a norm that is not finite makes every step not a number
+        k.c = norm <= clipnorm ? 1.0f : norm < __builtin_inff() ? __fdiv_rn(clipnorm, norm) : __builtin_nanf("");
+        if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
+    }
+    int i = 0;
+    for (uint32_t c = blockIdx.x; c < a.start[items]; c += gridDim.x) {
+        while (c >= a.start[i + 1]) ++i;
+        adamw_chunk<BITS>(a, a.item[i], k, (int64_t)(c - a.start[i]) * ADAMW_CHUNK);
+    }
+    if (!last) return;
+    __syncthreads();  // (every thread has used what it read of the state)
+    if (threadIdx.x == 0 && atomicAdd(&state->ticket, 1u) == gridDim.x - 1)
+        state->step = t, state->beta_1_power = p1, state->beta_2_power = p2, state->ticket = 0;
+}
+
+// sums of squares, one per workgroup: in fp64, so that no finite gradient overflows and their order does not show
+__global__ __launch_bounds__(256) void norm_parts_kernel(AdamwLaunch a, int items, double *parts) {
+    __shared__ double lds[4];
+    double v = 0;
+    int i = 0;
+    for (uint32_t c = blockIdx.x; c < a.start[items]; c += gridDim.x) {
+        while (c >= a.start[i + 1]) ++i;
+        const AdamwItem &it = a.item[i];
+        const int64_t e0 = (int64_t)(c - a.start[i]) * ADAMW_CHUNK, end = e0 + ADAMW_CHUNK < it.n ? e0 + ADAMW_CHUNK : it.n;
+        for (int64_t e = e0 + threadIdx.x; e < end; e += 256) {
+            const double g = gradient(a, it, e);
+            v += g * g;
+        }
+    }
+    v = block_sum(v, lds);
+    if (threadIdx.x == 0) parts[blockIdx.x] = v;
+}
+
+__global__ __launch_bounds__(256) void norm_finish_kernel(const double *parts, int n, float *out) {
+    __shared__ double lds[4];
+    const float norm = norm_of_parts(parts, n, lds);
+    if (threadIdx.x == 0) out[0] = norm;
+}
+
+}  // namespace hgq
+
+using namespace hgq;
+
+namespace {
+
+// Goes over `items` in launches of up to ADAMW_ITEMS variables and ADAMW_PIECES further gradient pieces: fn(launch, variables, last).
+// Descriptors travel as launch arguments (4 KB at most), so the calls are safe under HIP graph capture.
+template <class F>
+int for_launches(const hgq_adamw_item *items, int count, F fn) {
+    int at = 0;
+    bool done = false;
+    while (!done) {
+        AdamwLaunch a = {};
+        int n = 0, pieces = 0;
+        uint64_t chunks = 0;
+        for (; at < count && n < ADAMW_ITEMS; ++at) {
+            const hgq_adamw_item &s = items[at];
+            if (s.n == 0) continue;
+            int own = 0;
+            for (int k = 0; k < HGQ_SGD_SIDES; ++k) own += s.side[k] != nullptr;
+            const uint64_t own_chunks = ((uint64_t)s.n + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
+            if (pieces + own > ADAMW_PIECES || (n > 0 && chunks + own_chunks > 0x7fffffffu)) break;
+            AdamwItem &d = a.item[n];
+            d.w = s.w, d.g = s.g, d.m = s.m, d.v = s.v, d.m_scale = s.m_scale, d.v_scale = s.v_scale, d.n = s.n, d.first = s.first;
+            d.l1 = s.l1, d.lo = s.lo, d.hi = s.hi, d.decay = s.decay, d.type = s.type, d.piece = (short)pieces, d.pieces = (short)own;
+            for (int k = 0; k < HGQ_SGD_SIDES; ++k)
+                if (s.side[k]) a.side[pieces] = s.side[k], a.side_scale[pieces] = s.side_scale[k], ++pieces;
+            a.start[n] = (uint32_t)chunks;
+            chunks += own_chunks;
+            a.start[++n] = (uint32_t)chunks;
+        }
+        while (at < count && items[at].n == 0) ++at;
+        done = at >= count;
+        const int rc = fn(a, n, done);
+        if (rc) return rc;
+    }
+    return HGQ_OK;
+}
+
+int check_items(const char *what, const hgq_adamw_item *items, int count, int bits) {
+    if (count < 0 || (count > 0 && !items)) return fail(HGQ_ERR_ARG, "%s: bad arguments", what);
+    for (int t = 0; t < count; ++t) {
+        const hgq_adamw_item &s = items[t];
+        if (s.n < 0 || s.n > (int64_t)1 << 40) return fail(HGQ_ERR_ARG, "%s: bad number of elements in item %d", what, t);
+        if (s.n == 0) continue;
+        bool any = s.g != nullptr;
+        for (int k = 0; k < HGQ_SGD_SIDES; ++k) any = any || s.side[k];
+        if (!any || (bits && (!s.w || !s.m || !s.v))) return fail(HGQ_ERR_ARG, "%s: null pointer in item %d", what, t);
+        if (s.type != HGQ_TYPE_F32 && s.type != HGQ_TYPE_BF16 && s.type != HGQ_TYPE_F16) return fail(HGQ_ERR_ARG, "%s: unknown type in item %d", what, t);
+        if (bits == 8 && (!s.m_scale || !s.v_scale || s.first < 0 || s.first % HGQ_ADAMW_BLOCK))
+            return fail(HGQ_ERR_ARG, "%s: item %d has no scales, or its first element is not a multiple of %d", what, t, HGQ_ADAMW_BLOCK);
+    }
+    return HGQ_OK;
+}
+
+constexpr int NORM_GRID = 512;
+
+int norm_grid(const AdamwLaunch &a, int n) {
+    const uint32_t chunks = n ? a.start[n] : 0;
+    return (int)(chunks < NORM_GRID ? chunks : NORM_GRID);
+}
+
+}  // namespace
+
+extern "C" int64_t hgq_global_norm_parts(const hgq_adamw_item *items, int count) {
+    if (check_items("hgq_global_norm_parts", items, count, 0)) return -1;
+    int64_t parts = 0;
+    for_launches(items, count, [&](const AdamwLaunch &a, int n, bool) {
+        parts += norm_grid(a, n);
+        return HGQ_OK;
+    });
+    return parts;
+}
+
+extern "C" int hgq_global_norm(const hgq_adamw_item *items, int count, double *parts, float *out, void *stream) {
+    int rc = check_items("hgq_global_norm", items, count, 0);
+    if (rc) return rc;
+    int64_t at = 0;
+    rc = for_launches(items, count, [&](const AdamwLaunch &a, int n, bool) {
+        const int grid = norm_grid(a, n);
+        if (!grid) return HGQ_OK;
+        if (!parts) return fail(HGQ_ERR_ARG, "hgq_global_norm: null workspace");
+        hipLaunchKernelGGL(norm_parts_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a, n, parts + at);
+        at += grid;
+        return check_launch("hgq_global_norm");
+    });
+    if (rc || !out) return rc;
+    hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, parts, (int)at, out);
+    return check_launch("hgq_global_norm");
+}
+
+extern "C" int hgq_adamw_update_multi(const hgq_adamw_item *items, int count, int state_bits, hgq_adamw_state *state, double beta_1,
+                                      double beta_2, float epsilon, float clipnorm, const double *norm_parts, int64_t n_parts, float *norm_out,
+                                      uint64_t seed, const float *const *terms, int n_terms, float *sum_out, void *stream) {
+    if (state_bits != 8 && state_bits != 32) return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: moments have 8 or 32 bits, not %d", state_bits);
+    int rc = check_items("hgq_adamw_update_multi", items, count, state_bits);
+    if (rc) return rc;
+    if (!state) return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: null state");
+    if (!(beta_1 >= 0 && beta_1 < 1 && beta_2 >= 0 && beta_2 < 1 && epsilon >= 0))
+        return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: 0 <= beta < 1 and epsilon >= 0 are expected");
+    if (n_parts < 0 || n_parts > 0x7fffffff || (n_parts > 0 && (!norm_parts || !(clipnorm > 0))))
+        return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: a positive clipnorm and the parts of the norm go together");
+    if (n_terms < 0 || n_terms > HGQ_SUM_BATCH || (n_terms > 0 && (!terms || !sum_out)))
+        return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: up to %d terms and an output are expected", HGQ_SUM_BATCH);
+    AdamwSum sum = {};
+    sum.n = n_terms, sum.out = sum_out;
+    for (int t = 0; t < n_terms; ++t)
+        if (!(sum.term[t] = terms[t])) return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: null term %d", t);
+    return for_launches(items, count, [&](const AdamwLaunch &a, int n, bool last) {
+        const uint32_t chunks = n ? a.start[n] : 0;
+        const int grid = chunks < 1 ? 1 : chunks < ADAMW_GRID ? (int)chunks : ADAMW_GRID;  // (no element at all: the step still counts)
+        auto kernel = state_bits == 8 ? adamw_kernel<8> : adamw_kernel<32>;
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a, sum, state, beta_1, beta_2, epsilon, clipnorm, norm_parts,
+                           (int)n_parts, norm_out, seed, n, (int)last);
+        sum.n = 0, norm_out = nullptr;
+        return check_launch("hgq_adamw_update_multi");
+    });
+}

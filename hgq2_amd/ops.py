@@ -10,7 +10,9 @@ raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
+from array import array
 from typing import Sequence
 
 import torch
@@ -18,7 +20,7 @@ from torch import Tensor
 
 from . import _lib
 
-__all__ = ['quantize', 'wrap_track_i_', 'qdense', 'dense_ebops', 'sparse_ce', 'sgd_update_', 'sgd_update_multi_', 'qsoftmax', 'conv2d', 'matmul_bias_act', 'col_moments', 'attn_scores', 'attn_combine', 'ATTN_MAX', 'pool2d', 'conv2d_ebops', 'conv_geometry', 'conv2d_ebops_supported', 'mse', 'dense_moments', 'dense_moments_supported', 'bn_fold', 'qbits', 'ebops_finish', 'qattention', 'qattention_supported', 'bits_ebops', 'gdense', 'gdense_supported', 'affine_rows']
+__all__ = ['quantize', 'wrap_track_i_', 'qdense', 'dense_ebops', 'sparse_ce', 'sgd_update_', 'sgd_update_multi_', 'qsoftmax', 'conv2d', 'matmul_bias_act', 'col_moments', 'attn_scores', 'attn_combine', 'ATTN_MAX', 'pool2d', 'conv2d_ebops', 'conv_geometry', 'conv2d_ebops_supported', 'mse', 'dense_moments', 'dense_moments_supported', 'bn_fold', 'qbits', 'ebops_finish', 'qattention', 'qattention_supported', 'bits_ebops', 'gdense', 'gdense_supported', 'affine_rows', 'global_norm', 'adamw_update_multi_', 'adamw_state', 'adamw_moments']
 
 
 def _ptr(t: Tensor | None):
@@ -3363,6 +3365,223 @@ def sgd_update_multi_(ws, gs, l1, lo, hi, lr, sides=None, sum_terms=None, sum_ou
     sgd_update_multi_op(list(ws), [g.contiguous() if g is not None else empty for g in gs], [float(v) for v in l1],
                         [float(v) for v in lo], [float(v) for v in hi], float(lr), flat_s, flat_c,
                         [t.detach() for t in sum_terms] if sum_terms else [], sum_out if sum_terms else empty)
+
+
+# ---- AdamW and the global norm of gradients
+ADAMW_BLOCK = 256  # HGQ_ADAMW_BLOCK of include/hgq_hip.h: elements that share the scale of a moment in 8 bits
+_TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ADAMW_WORDS = 19  # hgq_adamw_item as 64-bit words
+_NO_SIDES = (0,) * (2 * SGD_SIDES)
+_adamw_limits = {}
+
+
+class _AdamwItem(ctypes.Structure):
+    """``hgq_adamw_item`` of include/hgq_hip.h (what :func:`_adamw_item` writes word by word)."""
+
+    _fields_ = [('w', ctypes.c_void_p), ('g', ctypes.c_void_p), ('m', ctypes.c_void_p), ('v', ctypes.c_void_p), ('m_scale', ctypes.c_void_p),
+                ('v_scale', ctypes.c_void_p), ('n', ctypes.c_int64), ('first', ctypes.c_int64), ('l1', ctypes.c_float), ('lo', ctypes.c_float),
+                ('hi', ctypes.c_float), ('decay', ctypes.c_float), ('type', ctypes.c_int), ('side', ctypes.c_void_p * SGD_SIDES),
+                ('side_scale', ctypes.c_void_p * SGD_SIDES)]
+
+
+class _AdamwState(ctypes.Structure):
+    """``hgq_adamw_state`` of include/hgq_hip.h."""
+
+    _fields_ = [('step', ctypes.c_int64), ('beta_1_power', ctypes.c_double), ('beta_2_power', ctypes.c_double), ('lr', ctypes.c_double),
+                ('ticket', ctypes.c_uint32), ('unused', ctypes.c_uint32)]
+
+
+def _adamw_limits_words(l1: float, lo: float, hi: float, decay: float):
+    """The four floats of a descriptor as two words (the same few combinations come back at every step)."""
+    key = (l1, lo, hi, decay)
+    got = _adamw_limits.get(key)
+    if got is None:
+        if len(_adamw_limits) > 4096:
+            _adamw_limits.clear()
+        got = _adamw_limits[key] = struct.unpack('qq', struct.pack('ffff', l1, lo, hi, decay))
+    return got
+
+
+def _check_gradient(name: str, t: Tensor, device, dtype, numel: int):
+    if t.device == device and t.dtype is dtype and t.numel() == numel and t.layout is torch.strided:
+        return
+    _need(t.layout is torch.strided, f'{name} must be dense')
+    _need(t.device == device, f'{name} must be on {device}, got {t.device}')
+    _need(t.dtype == dtype, f'{name} must be {dtype}, got {t.dtype}')
+    _need(t.numel() == numel, f'{name} has {t.numel()} elements, not {numel}')
+
+
+def _side_words(pairs, device, numel: int, held: list):
+    """The words of a descriptor's further gradient pieces: ``(scale or None, gradient)`` pairs."""
+    _need(len(pairs) <= SGD_SIDES, f'at most {SGD_SIDES} side gradients per variable')
+    ptrs, scales = [0] * SGD_SIDES, [0] * SGD_SIDES
+    for s, (sc, sd) in enumerate(pairs):
+        _check_gradient('side gradient', sd, device, _F32, numel)
+        sd = sd.contiguous()
+        held.append(sd)
+        ptrs[s] = sd.data_ptr()
+        if sc is not None:
+            _need(sc.device == device and sc.dtype == torch.float32 and sc.numel() == 1, 'a side-gradient scale is one float32 on the GPU')
+            held.append(sc)
+            scales[s] = sc.data_ptr()
+    return (*ptrs, *scales)
+
+
+class _device_of:
+    """Launches go to the current stream of the device that the tensors are on, whichever device is the current one."""
+
+    def __init__(self, device):
+        self.device, self.guard = device, None
+
+    def __enter__(self):
+        if self.device.index is not None and self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+@torch.library.custom_op('hgq::global_norm', mutates_args=())
+def global_norm_op(tensors: Sequence[Tensor]) -> Tensor:
+    _need(len(tensors) >= 1, 'at least one tensor is expected')
+    device = tensors[0].device
+    _need(device.type == 'cuda', f'tensors must be on a GPU (there is no CPU implementation), got device {device}')
+    words, held = [], []
+    for t in tensors:
+        _need(t.device == device and t.layout is torch.strided, f'tensors must be dense and on one device, got {t.device}')
+        code = _TYPE_CODES.get(t.dtype)
+        _need(code is not None, f'tensors must be float32, bfloat16 or float16, got {t.dtype}')
+        if not t.is_contiguous():
+            t = t.contiguous()
+            held.append(t)
+        words += (0, t.data_ptr(), 0, 0, 0, 0, t.numel(), 0, 0, 0, code, *_NO_SIDES)
+    items = array('q', words)
+    out = torch.empty((), dtype=torch.float32, device=device)
+    lib, at, n = _lib.load(), items.buffer_info()[0], len(tensors)
+    with _device_of(device):
+        parts = torch.empty(lib.hgq_global_norm_parts(at, n), dtype=torch.float64, device=device)
+        rc = lib.hgq_global_norm(at, n, parts.data_ptr(), out.data_ptr(), _stream())
+    _lib.check(rc, 'hgq_global_norm')
+    return out
+
+
+@global_norm_op.register_fake
+def _(tensors):
+    return tensors[0].new_empty((), dtype=torch.float32)
+
+
+def global_norm(tensors: Sequence[Tensor]) -> Tensor:
+    """``sqrt(sum of squares of all elements)`` of float32, bfloat16 or float16 GPU tensors, as ``keras.ops`` users write
+    ``global_norm`` of their gradients (``None`` entries are left out): one float32, summed in fp64 in a fixed order, so it neither
+    overflows before its result does nor depends on the order in which workgroups end.  Not differentiable."""
+    return global_norm_op([t.detach() for t in tensors if t is not None])
+
+
+def adamw_state(device, lr: float, iterations: int = 0, beta_1: float = 0.9, beta_2: float = 0.999) -> Tensor:
+    """The device-side state of an AdamW run after ``iterations`` steps (``hgq_adamw_state``), as five int64 words."""
+    raw = struct.pack('qdddq', int(iterations), float(beta_1)**int(iterations), float(beta_2)**int(iterations), float(lr), 0)
+    return torch.tensor(struct.unpack('5q', raw), dtype=torch.int64).to(device)
+
+
+def adamw_moments(n: int, device, state_bits: int = 32) -> list[Tensor]:
+    """Moments of ``n`` elements before the first step: ``[m, v]`` in float32, or with 8 bits ``[codes of m, scales of m, codes of
+    sqrt(v), scales of sqrt(v)]`` - E4M3 codes and one power of two (E8M0) per 256 elements."""
+    _need(state_bits in (8, 32), f'moments have 8 or 32 bits, not {state_bits}')
+    if state_bits == 32:
+        return [torch.zeros(n, dtype=torch.float32, device=device) for _ in range(2)]
+    made = []
+    for _ in range(2):
+        made.append(torch.zeros(n, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn))
+        made.append(torch.ones(-(-n // ADAMW_BLOCK), dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu))
+    return made
+
+
+def _adamw_launch(items, count: int, state_bits: int, state: Tensor, beta_1: float, beta_2: float, epsilon: float, clipnorm, norm_out,
+                  seed: int, sum_terms, sum_out):
+    """``items``: hgq_adamw_item words of ``count`` variables in an ``array('q')``; ``clipnorm`` None: no clipping."""
+    lib, at = _lib.load(), items.buffer_info()[0]
+    device = state.device
+    with _device_of(device):
+        stream = _stream()
+        n_parts = 0
+        if clipnorm is not None:
+            n_parts = lib.hgq_global_norm_parts(at, count)
+            # this call's own: in a captured step it belongs to that graph
+            parts = torch.empty(n_parts, dtype=torch.float64, device=device)
+            if n_parts:
+                _lib.check(lib.hgq_global_norm(at, count, parts.data_ptr(), None, stream), 'hgq_global_norm')
+        ptrs, n_terms = None, len(sum_terms) if sum_terms else 0
+        if n_terms:
+            _need(n_terms <= SUM_BATCH, f'at most {SUM_BATCH} terms ride along with the update')
+            ptrs = (ctypes.c_void_p * n_terms)()
+            for t, term in enumerate(sum_terms):
+                _check_f32('term', term)
+                _need(term.numel() == 1, 'every term must hold one element')
+                ptrs[t] = term.data_ptr()
+            _check_f32('sum_out', sum_out)
+        rc = lib.hgq_adamw_update_multi(at, count, state_bits, state.data_ptr(), beta_1, beta_2, epsilon, clipnorm if n_parts else 0.0,
+                                        parts.data_ptr() if n_parts else None, n_parts, norm_out.data_ptr() if norm_out is not None else None,
+                                        seed, ptrs, n_terms, sum_out.data_ptr() if n_terms else None, stream)
+    _lib.check(rc, 'hgq_adamw_update_multi')
+
+
+@torch.library.custom_op('hgq::adamw_update_multi', mutates_args=('ws', 'moments', 'state', 'norm_out'))
+def adamw_update_multi_op(ws: Sequence[Tensor], gs: Sequence[Tensor], moments: Sequence[Tensor], l1: Sequence[float], lo: Sequence[float],
+                          hi: Sequence[float], decay: Sequence[float], state_bits: int, state: Tensor, beta_1: float, beta_2: float,
+                          epsilon: float, clipnorm: float, norm_out: Tensor, seed: int) -> None:
+    """``moments``: two tensors per variable (four with 8 bits); ``clipnorm`` 0: no clipping."""
+    n, per = len(ws), 2 if state_bits == 32 else 4
+    _need(state_bits in (8, 32), f'moments have 8 or 32 bits, not {state_bits}')
+    _need(n >= 1 and all(len(v) == n for v in (gs, l1, lo, hi, decay)) and len(moments) == per * n, 'per-variable lists differ in length')
+    device = ws[0].device
+    _need(device.type == 'cuda', f'variables must be GPU tensors (there is no CPU implementation), got device {device}')
+    _need(state.dtype == torch.int64 and state.numel() == 5 and state.device == device, 'state: what adamw_state makes, on the variables\' device')
+    _need(len({w.data_ptr() for w in ws if w.numel()}) == sum(1 for w in ws if w.numel()), 'a variable is listed twice')
+    _need(clipnorm >= 0, 'clipnorm must not be negative')
+    words, first = [], 0
+    for t, (w, g) in enumerate(zip(ws, gs)):
+        code, num = _TYPE_CODES.get(w.dtype), w.numel()
+        _need(code is not None, f'variables must be float32, bfloat16 or float16, got {w.dtype}')
+        _check_gradient('variable', w, device, w.dtype, num)
+        _check_gradient('gradient', g, device, w.dtype, num)
+        mom = moments[per * t:per * t + per]
+        kinds = (_F32, _F32) if per == 2 else (torch.float8_e4m3fn, torch.float8_e8m0fnu) * 2
+        sizes = (num, num) if per == 2 else (num, -(-num // ADAMW_BLOCK)) * 2
+        for name, mt, kind, size in zip(('m', 'v') if per == 2 else ('m', 'm scale', 'v', 'v scale'), mom, kinds, sizes):
+            _check_gradient(name, mt, device, kind, size)
+        _need(all(k.is_contiguous() for k in (w, g, *mom)), 'variables, gradients and moments must be contiguous')
+        p = [k.data_ptr() for k in mom]
+        words += (w.data_ptr(), g.data_ptr(), *((p[0], p[1], 0, 0) if per == 2 else (p[0], p[2], p[1], p[3])), num, first,
+                  *_adamw_limits_words(l1[t], lo[t], hi[t], decay[t]), code, *_NO_SIDES)
+        first += -(-num // ADAMW_BLOCK) * ADAMW_BLOCK
+    if norm_out.numel():
+        _check_f32('norm_out', norm_out)
+        _need(norm_out.numel() == 1 and norm_out.device == device, 'norm_out is one float32')
+    _adamw_launch(array('q', words), n, state_bits, state, beta_1, beta_2, epsilon, clipnorm or None,
+                  norm_out if norm_out.numel() else None, seed, None, None)
+
+
+def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: float = 0.999, epsilon: float = 1e-7, decay=None, l1=None,
+                        lo=None, hi=None, clipnorm: float | None = None, norm_out: Tensor | None = None, seed: int = 0):
+    """One AdamW step of the variables ``ws`` (float32, bfloat16 or float16, contiguous) with the gradients ``gs`` of the same types, in
+    place.  ``moments[t]``: what :func:`adamw_moments` makes for variable ``t`` (its length says whether they have 32 or 8 bits);
+    ``state``: :func:`adamw_state`, which the launch moves on (recorded in a HIP graph, every replay is the next step).  Per variable:
+    weight ``decay``, an ``l1`` added to the gradient, and bounds ``lo``, ``hi`` of the result.  ``clipnorm``: gradients are scaled down
+    to this global norm; a norm that is not finite makes every variable not a number.  :class:`hgq2_amd.train.AdamW` is this with
+    the moments, regularizers and constraints of a model's variables."""
+    n, inf = len(ws), float('inf')
+    _need(len(moments) == n and n >= 1, 'per-variable lists differ in length')
+    _need(clipnorm is None or clipnorm > 0, 'clipnorm must be positive')
+    bits = 32 if len(moments[0]) == 2 else 8
+    each = lambda v, d: [d] * n if v is None else [float(k) for k in v]  # noqa: E731
+    empty = torch.empty(0, dtype=torch.float32, device=state.device)
+    adamw_update_multi_op([w.detach() for w in ws], [g.detach().contiguous() for g in gs], [k for m in moments for k in m], each(l1, 0.0),
+                          each(lo, -inf), each(hi, inf), each(decay, 0.0), bits, state, float(beta_1), float(beta_2), float(epsilon),
+                          float(clipnorm or 0.0), norm_out if norm_out is not None else empty, int(seed) & (2**63 - 1))
+    touch_state()
 
 
 # ======================================================================================

@@ -9,6 +9,7 @@ propagate; ``w <- w - lr * g``; apply each variable's constraint.
 from __future__ import annotations
 
 import operator
+from array import array
 
 import torch
 
@@ -136,6 +137,167 @@ class SGD:
             p.copy_(c(p))
 
 
+class AdamW(SGD):
+    """AdamW as ``keras.optimizers.AdamW`` defines it (same argument names and defaults; ``weight_decay=0`` is Adam), with the
+    regularizers and constraints handled as in :class:`SGD` and the same ``zero_grad`` / ``backward`` / ``step``: all variables are
+    updated in one launch per 28 of them.
+
+    ``state_bits=8`` keeps both moments in 8 bits with one scale per 256 elements (2 bytes per weight instead of 8; a layer with a
+    bit-width per weight has three variables of its kernel's size), rounded stochastically from ``seed``.  Variables and gradients
+    are float32, or bfloat16 / float16 with the arithmetic in fp32.  ``global_clipnorm`` scales the gradients - regularizers and
+    EBOPs pieces included - down to that global norm; ``grad_norm`` then holds the last step's norm (a 0-dim GPU tensor).
+
+    The number of steps and the learning rate live in device memory: a step recorded in a HIP graph (:class:`GraphedTrainStep`)
+    counts on at every replay, and setting ``lr`` between replays takes effect in the next one.  The moments of all variables lie in
+    one buffer each (``momentum`` and ``velocity``, or ``momentum``, ``momentum_scale``, ``velocity_root`` and ``velocity_scale``), every
+    variable at a multiple of 256 elements.  Variables must stay contiguous, on their device, and of their size and type."""
+
+    def __init__(self, params, lr: float = 0.001, weight_decay: float = 0.004, beta_1: float = 0.9, beta_2: float = 0.999,
+                 epsilon: float = 1e-7, global_clipnorm: float | None = None, state_bits: int = 32, seed: int = 0,
+                 fold_regularizers: bool = False):
+        super().__init__(params, 0.0, fold_regularizers)
+        if not self.params:
+            raise ValueError('AdamW needs at least one trainable variable')
+        if state_bits not in (8, 32):
+            raise ValueError(f'moments have 8 or 32 bits, not {state_bits}')
+        if not (0 <= beta_1 < 1 and 0 <= beta_2 < 1 and epsilon >= 0 and weight_decay >= 0):
+            raise ValueError('0 <= beta < 1, epsilon >= 0 and weight_decay >= 0 are expected')
+        if global_clipnorm is not None and not global_clipnorm > 0:
+            raise ValueError('global_clipnorm must be positive')
+        self.device = self.params[0].device
+        if self.device.type != 'cuda':
+            raise ValueError(f'variables must be GPU tensors (there is no CPU implementation), got device {self.device}')
+        for p in self.params:
+            if p.dtype not in ops._TYPE_CODES:
+                raise ValueError(f'variables must be float32, bfloat16 or float16, got {p.dtype}')
+            if p.device != self.device:
+                raise ValueError(f'variables must be on one device, got {self.device} and {p.device}')
+        if len(self._owner_ids) != len(self.params):
+            raise ValueError('a variable is listed twice')
+        self.weight_decay, self.beta_1, self.beta_2 = float(weight_decay), float(beta_1), float(beta_2)
+        self.epsilon, self.global_clipnorm = float(epsilon), None if global_clipnorm is None else float(global_clipnorm)
+        self.state_bits, self.seed = int(state_bits), int(seed) & (2**63 - 1)
+        self._no_decay = set()
+        self._numel, self._at, n = [p.numel() for p in self.params], [], 0
+        for k in self._numel:
+            self._at.append(n)
+            n += -(-k // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
+        moments = ops.adamw_moments(n, self.device, self.state_bits)
+        if self.state_bits == 32:
+            self._names = ('momentum', 'velocity')
+        else:
+            self._names = ('momentum', 'momentum_scale', 'velocity_root', 'velocity_scale')
+        for name, t in zip(self._names, moments):
+            setattr(self, name, t)
+        self.grad_norm = torch.zeros((), dtype=torch.float32, device=self.device) if self.global_clipnorm is not None else None
+        self._state = ops.adamw_state(self.device, lr, 0, self.beta_1, self.beta_2)
+        self.lr = lr
+
+    # ---- learning rate and step number: in device memory, where a recorded step reads them
+    @property
+    def lr(self):
+        return self._lr
+
+    @lr.setter
+    def lr(self, value):
+        self._lr = float(value)
+        state = getattr(self, '_state', None)  # (the base class sets it before there is one)
+        if state is not None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('AdamW.lr cannot be set inside a capture: every replay would set it again')
+            state[3:4].view(torch.float64).fill_(self._lr)
+
+    @property
+    def iterations(self) -> int:
+        """Steps done, replayed ones included (waits for the GPU)."""
+        return int(self._state[0])
+
+    def exclude_from_weight_decay(self, var_list=None, var_names=None):
+        """Variables, or parts of variables' names (``var_name``), that are not decayed."""
+        ids = {id(v) for v in var_list or ()}
+        names = tuple(var_names or ())
+        for p in self.params:
+            if id(p) in ids or any(n in (getattr(p, 'var_name', None) or '') for n in names):
+                self._no_decay.add(id(p))
+
+    def state_dict(self) -> dict:
+        """The number of steps and copies of the moments (read back by :meth:`load_state_dict`)."""
+        return {'iterations': self.iterations, **{k: getattr(self, k).clone() for k in self._names}}
+
+    def load_state_dict(self, state: dict):
+        """Continue from another run's :meth:`state_dict` over variables of the same sizes and the same ``state_bits``."""
+        if set(state) != {'iterations', *self._names}:
+            raise ValueError(f'expected the entries iterations, {", ".join(self._names)}; got {", ".join(sorted(state))}')
+        if int(state['iterations']) < 0:
+            raise ValueError('iterations must not be negative')
+        for k in self._names:
+            have, new = getattr(self, k), state[k]
+            if new.shape != have.shape or new.dtype != have.dtype:
+                raise ValueError(f'{k}: expected {have.dtype} {tuple(have.shape)}, got {new.dtype} {tuple(new.shape)}')
+        with torch.no_grad():
+            for k in self._names:
+                have, new = getattr(self, k), state[k]
+                if have.element_size() == 1:  # (bit for bit, whatever conversions a type has)
+                    have, new = have.view(torch.uint8), new.view(torch.uint8)
+                have.copy_(new)
+            self._state.copy_(ops.adamw_state('cpu', self._lr, state['iterations'], self.beta_1, self.beta_2))
+
+    @torch.no_grad()
+    def step(self):
+        sums = ops.join_side(hand_over_sums=True)  # the loss terms' sum rides along with the update launch
+        words, held, post = [], [], []
+        dev, inf = self.device, float('inf')
+        mom = [getattr(self, k).data_ptr() for k in self._names]
+        wide = self.state_bits == 32
+        count = 0
+        for p, n, at in zip(self.params, self._numel, self._at):
+            g = p.grad
+            side = getattr(p, '_hgq_side', None)
+            if (g is None and not side) or n == 0:
+                continue
+            ops._check_gradient('variable', p, dev, p.dtype, n)
+            if not p.is_contiguous():
+                raise ValueError('variables must be contiguous')
+            if g is not None:
+                ops._check_gradient('gradient', g, dev, p.dtype, n)
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    held.append(g)
+            if side:
+                side = list(side)
+                while len(side) > ops.SGD_SIDES:  # more pieces than the kernel takes: fold the surplus into one
+                    (s1, d1), (s2, d2) = side.pop(), side.pop()
+                    side.append((None, (d1 if s1 is None else s1 * d1) + (d2 if s2 is None else s2 * d2)))
+            c = getattr(p, 'constraint', None)
+            r = getattr(p, 'regularizer', None)
+            lo, hi = -inf, inf
+            if c is not None:
+                bounds = c.bounds()
+                if bounds is None:  # a constraint that is not a clip: applied after the update
+                    post.append((p, c))
+                else:
+                    lo, hi = bounds
+            l1 = r.l1 if (self.fold_regularizers and isinstance(r, MonoL1)) else 0.0
+            decay = 0.0 if id(p) in self._no_decay else self.weight_decay
+            if wide:
+                m = (mom[0] + 4 * at, mom[1] + 4 * at, 0, 0)
+            else:
+                b = at // ops.ADAMW_BLOCK
+                m = (mom[0] + at, mom[2] + at, mom[1] + b, mom[3] + b)
+            words += (p.data_ptr(), g.data_ptr() if g is not None else 0, *m, n, at, *ops._adamw_limits_words(l1, lo, hi, decay),
+                      ops._TYPE_CODES[p.dtype], *(ops._side_words(side, dev, n, held) if side else ops._NO_SIDES))
+            count += 1
+        ride = sums.pop(0) if (count and sums) else (None, None)
+        for terms, out in sums:
+            ops.sum_scalars_into(terms, out)
+        if count:
+            ops.touch_state()  # written through pointers: the version counters do not move
+            ops._adamw_launch(array('q', words), count, self.state_bits, self._state, self.beta_1, self.beta_2, self.epsilon, self.global_clipnorm,
+                              self.grad_norm, self.seed, ride[0], ride[1])
+        for p, c in post:
+            p.copy_(c(p))
+
+
 class GraphedTrainStep:
     """One training step (forward, loss, backward, optimizer update) captured in a HIP graph.
 
@@ -144,7 +306,7 @@ class GraphedTrainStep:
     static buffers before each replay.  ``loss_fn(outputs, labels)`` must be built from capturable
     operations (``hgq2_amd.ops.sparse_ce`` is)."""
 
-    def __init__(self, model, loss_fn, optimizer: SGD, example_x, example_y, warmup: int = 3, overlap: bool = True,
+    def __init__(self, model, loss_fn, optimizer: 'SGD | AdamW', example_x, example_y, warmup: int = 3, overlap: bool = True,
                  warmup_data=None, feed: 'ResidentBatches | None' = None):
         """The recording is preceded by ``warmup`` real training steps on the example batch (operators create their
         per-stream scratch there, not inside the graph) - or, with ``warmup_data`` (a sequence of ``(x, y)`` of the
@@ -409,8 +571,8 @@ class _FusedStep:
 
 
 def train_step_for(model, example_x, example_y, lr: float = 0.01, loss: str = 'sparse_ce', fused: bool | None = None,
-                   warmup_data=None, feed=None, warmup: int = 3):
-    """A callable ``step(x, y) -> loss`` that runs one SGD training step of ``model`` on the fastest path that covers it.
+                   warmup_data=None, feed=None, warmup: int = 3, optimizer='sgd'):
+    """A callable ``step(x, y) -> loss`` that runs one training step of ``model`` on the fastest path that covers it.
 
     A built stack of :class:`QDense` layers trained with mean sparse categorical cross-entropy and within what
     :class:`FusedQDenseStack` checks (widths up to 64, the default quantizer kinds, an LDS plan that fits) runs on the
@@ -420,12 +582,19 @@ def train_step_for(model, example_x, example_y, lr: float = 0.01, loss: str = 's
     the time per step and nothing else.  ``fused=False`` forces the per-layer path, ``fused=True`` raises where the
     whole-step path does not apply.  The returned object's ``path`` is ``'fused'`` or ``'layers_graph'``.
     ``warmup_data``, ``feed``, ``warmup``: see :class:`GraphedTrainStep` (the whole-step path needs no steps before it and
-    takes none: ``warmup_losses`` is then empty; it does not use a ``feed`` either)."""
+    takes none: ``warmup_losses`` is then empty; it does not use a ``feed`` either).  ``optimizer``: ``'sgd'``, ``'adamw'``
+    (:class:`AdamW` with ``lr`` and Keras' other defaults) or a callable that makes one of the model's variables, for
+    instance ``lambda v: AdamW(v, lr=1e-3, global_clipnorm=1.0, state_bits=8, fold_regularizers=True)``; anything but
+    ``'sgd'`` runs the per-layer path, and the returned object's ``opt`` is the optimizer (its ``lr`` may change between steps)."""
     if loss not in ('sparse_ce', 'mse'):
         raise ValueError(f"loss must be 'sparse_ce' or 'mse', got {loss!r}")
+    if not callable(optimizer) and optimizer not in ('sgd', 'adamw'):
+        raise ValueError(f"optimizer must be 'sgd', 'adamw' or a callable that makes one of the variables, got {optimizer!r}")
+    if fused and optimizer != 'sgd':
+        raise ValueError('the fused QDense step updates with SGD only')
     if not model.built:
         model(example_x, training=False)  # creates the variables; an inference call leaves the integer-bit trackers alone
-    if fused is not False and loss == 'sparse_ce':
+    if fused is not False and loss == 'sparse_ce' and optimizer == 'sgd':
         try:
             stack = FusedQDenseStack(model, lr=lr)
             if example_x.dim() != 2 or example_x.shape[1] != stack._arr[0].K:
@@ -442,8 +611,9 @@ def train_step_for(model, example_x, example_y, lr: float = 0.01, loss: str = 's
     elif fused:
         raise ValueError('the fused QDense step computes sparse categorical cross-entropy only')
     loss_fn = ops.sparse_ce if loss == 'sparse_ce' else ops.mse
-    step = GraphedTrainStep(model, loss_fn, SGD(model.parameters(), lr=lr, fold_regularizers=True), example_x, example_y,
-                            warmup=warmup, warmup_data=warmup_data, feed=feed)
+    opt = optimizer(model.parameters()) if callable(optimizer) else (AdamW if optimizer == 'adamw' else SGD)(
+        model.parameters(), lr=lr, fold_regularizers=True)
+    step = GraphedTrainStep(model, loss_fn, opt, example_x, example_y, warmup=warmup, warmup_data=warmup_data, feed=feed)
     step.path = 'layers_graph'
     return step
 
@@ -460,8 +630,9 @@ def folded_regularizer_loss(model) -> float:
 
 
 def fit(model, x, y, *, loss: str = 'sparse_ce', lr: float = 0.01, batch_size: int = 1024, epochs: int = 1, callbacks=(),
-        shuffle: bool = True, seed: int | None = None, fused: bool | None = None):
-    """Train ``model`` on the resident tensors ``x`` / ``y`` (first axis: samples) with plain SGD, the way the reference's
+        shuffle: bool = True, seed: int | None = None, fused: bool | None = None, optimizer='sgd'):
+    """Train ``model`` on the resident tensors ``x`` / ``y`` (first axis: samples) with plain SGD - or with the ``optimizer`` that
+    :func:`train_step_for` is given, which makes it once, before the first batch - the way the reference's
     users call ``model.fit`` (reference tests/base.py:313-331; the epoch hooks of src/hgq/utils/sugar/ drive beta from it):
     per epoch the callbacks' ``on_epoch_begin``, the batches in order (shuffled anew per epoch with ``shuffle``; the last
     one may be shorter), ``on_epoch_end`` with ``logs['loss']`` = the mean of the epoch's step losses.  Returns the list
@@ -514,7 +685,8 @@ def fit(model, x, y, *, loss: str = 'sparse_ce', lr: float = 0.01, batch_size: i
         if step is None:
             # the steps before the recording are this epoch's first batches
             warm = [batch(b) for b in range(min(3, n_full))]
-            step = train_step_for(model, *warm[0], lr=lr, loss=loss, fused=fused, warmup_data=warm, feed=feed, warmup=len(warm))
+            step = train_step_for(model, *warm[0], lr=lr, loss=loss, fused=fused, warmup_data=warm, feed=feed, warmup=len(warm),
+                                  optimizer=optimizer)
             if isinstance(step, _FusedStep):
                 feed = None  # the whole-step kernels read the batch where it lies
             done = getattr(step, 'warmup_losses', [])

@@ -552,6 +552,55 @@ int hgq_sgd_update_multi_sum(const hgq_sgd_item *items, int count, float lr, con
                              void *stream);
 
 /*
+ * AdamW (decoupled weight decay) over many variables, and the global norm of their gradients.  The reference's users train
+ * with keras.optimizers.Adam / AdamW (its published jet-tagging runs do); per step t = 1, 2, ... and element, in fp32:
+ *     grad = c (g + sum_s side_scale[s] side[s] + l1)
+ *     m <- m + (grad - m) (1 - beta_1);   v <- v + (grad grad - v) (1 - beta_2)
+ *     w <- clip(w - w lr decay - m alpha / (sqrt(v) + epsilon), lo, hi),   alpha = lr sqrt(1 - beta_2^t) / (1 - beta_1^t)
+ * c = min(1, clipnorm / norm) where parts of the norm are handed over (not a number if the norm is not finite), else 1.
+ *
+ * state_bits 32: `m`, `v` are fp32 [n].  state_bits 8: `m` and `v` are OCP E4M3 codes [n] of m and of sqrt(v), times the powers of
+ * two 2^(scale - 127) (OCP E8M0) of each HGQ_ADAMW_BLOCK elements, `m_scale` and `v_scale` [ceil(n / HGQ_ADAMW_BLOCK)]; rounded
+ * stochastically with 16-bit numbers of Philox4x32-7: element e takes word e % 4 of counter ((first + e) / 4, t) under key `seed`.
+ * `first` (a multiple of HGQ_ADAMW_BLOCK) keeps the numbers of different variables apart.
+ *
+ * `w` and `g` have the type `type`; `g` NULL: none (then at least one side).  Descriptors are read on the host and travel as
+ * launch arguments.  `state` is device memory: step, beta_1^step, beta_2^step and lr, of the steps done (0, 1, 1 at the start);
+ * the call moves them on, so a recorded call is the next step at every replay.  `ticket` is 0 between calls.  Calls that share
+ * `state` or variables must not overlap in time.  Two items must not name the same memory.
+ *
+ * hgq_global_norm: sqrt(sum of squares of all gradients) (`w`, `m`, `v`, `lo`, `hi`, `decay` are not read), in fp64, to `out` (fp32).
+ * `parts`: hgq_global_norm_parts(items, count) doubles, which hgq_adamw_update_multi takes as `norm_parts` (n_parts > 0: clip); with
+ * `out` NULL only they are written.  norm_out (may be NULL) receives the norm.
+ * `terms`, `n_terms`, `sum_out`: hgq_sum_scalars riding along (n_terms 0: none).
+ */
+#define HGQ_TYPE_F32 0
+#define HGQ_TYPE_BF16 1
+#define HGQ_TYPE_F16 2
+#define HGQ_ADAMW_BLOCK 256
+typedef struct {
+    void *w;
+    const void *g;
+    void *m, *v;
+    uint8_t *m_scale, *v_scale;
+    int64_t n, first;
+    float l1, lo, hi, decay;
+    int type;
+    const float *side[HGQ_SGD_SIDES];
+    const float *side_scale[HGQ_SGD_SIDES];
+} hgq_adamw_item;
+typedef struct {
+    int64_t step;
+    double beta_1_power, beta_2_power, lr;
+    uint32_t ticket, unused;
+} hgq_adamw_state;
+int64_t hgq_global_norm_parts(const hgq_adamw_item *items, int count);
+int hgq_global_norm(const hgq_adamw_item *items, int count, double *parts, float *out, void *stream);
+int hgq_adamw_update_multi(const hgq_adamw_item *items, int count, int state_bits, hgq_adamw_state *state, double beta_1, double beta_2,
+                           float epsilon, float clipnorm, const double *norm_parts, int64_t n_parts, float *norm_out, uint64_t seed,
+                           const float *const *terms, int n_terms, float *sum_out, void *stream);
+
+/*
  * One training step (forward, mean sparse categorical cross-entropy from logits, backward, SGD)
  * of a stack of QDense layers in two launches (three when the quantized weight image is rebuilt).  It performs, in the same order and with the
  * same arithmetic, what the per-layer entry points above do when the reference's call stack
