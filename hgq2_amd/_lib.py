@@ -23,7 +23,7 @@ MODE_K_U8 = 1 << 11
 MODE_SYMMETRIC = 1 << 12
 MODE_TRACING = 1 << 13
 MODE_TRACK_INPUT = 1 << 14
-ACT_NONE, ACT_RELU = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
 
 ROUND_MODES = {'TRN': TRN, 'RND': RND, 'RND_CONV': RND_CONV}
 OVERFLOW_MODES = {'WRAP': WRAP, 'SAT': SAT, 'SAT_SYM': SAT_SYM}
@@ -95,6 +95,10 @@ SIGNATURES = {
     'hgq_global_norm': (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     'hgq_adamw_update_multi': (c_int, [c_void_p, c_int, c_int, c_void_p, ctypes.c_double, ctypes.c_double, c_float, c_float, c_void_p, c_int64,
                                        c_void_p, ctypes.c_uint64, c_void_p, c_int, c_void_p, c_void_p]),
+    'hgq_group_norm_fwd_workspace': (c_int64, [c_int64, c_int64, c_int, c_int, c_int]),
+    'hgq_group_norm_fwd': (c_int, [c_void_p] * 7 + [c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p]),
+    'hgq_group_norm_bwd_workspace': (c_int64, [c_int64, c_int64, c_int, c_int, c_int]),
+    'hgq_group_norm_bwd': (c_int, [c_void_p] * 10 + [c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     'hgq_quantize_bwd_workspace': (c_int64, [c_int64, c_int64, c_int64]),
     'hgq_quantize_bwd_sliced': (c_int, [c_void_p] * 9 + [c_int64, c_int64, c_int64, c_int, c_void_p]),
     'hgq_quantize_bwd_slice_count': (c_int64, [c_int64, c_int64, c_int64]),

@@ -10,7 +10,7 @@ from types import SimpleNamespace
 import torch
 
 from . import ops
-from .core import Layer, Sequential  # noqa: F401  (Sequential is part of this module's surface)
+from .core import Layer, Sequential, get_initializer  # noqa: F401  (Sequential is part of this module's surface)
 
 
 def _pair(v):
@@ -98,5 +98,62 @@ class GlobalAveragePooling1D(Layer):
     host_fn = staticmethod(lambda x: torch.mean(x, dim=1))
 
 
-layers = SimpleNamespace(MaxPooling2D=MaxPooling2D, AveragePooling2D=AveragePooling2D, Flatten=Flatten,
+class GroupNormalization(Layer):
+    """``keras.layers.GroupNormalization`` over the trailing channel axis (same argument names and defaults; ``groups=-1``: each
+    channel by itself), with an activation in the same launch.  Full precision, not quantized: what a network trained on small batches
+    puts between its layers in the place of a batch normalisation, whose moments such batches do not give.  Variables ``gamma`` and
+    ``beta`` are float32; inputs are float32, bfloat16 or float16 GPU tensors ``[batch, ..., channels]``."""
+
+    def __init__(self, groups=32, axis=-1, epsilon=1e-3, center=True, scale=True, beta_initializer='zeros', gamma_initializer='ones',
+                 beta_regularizer=None, gamma_regularizer=None, beta_constraint=None, gamma_constraint=None, activation=None, **kwargs):
+        super().__init__(**kwargs)
+        if activation not in ops.GROUP_ACTIVATIONS:
+            raise ValueError(f'GroupNormalization: activation must be one of linear, relu, silu; got {activation!r}')
+        if int(groups) < 1 and int(groups) != -1:
+            raise ValueError(f'GroupNormalization: groups must be positive, or -1 for as many as channels; got {groups}')
+        if not float(epsilon) >= 0:
+            raise ValueError('GroupNormalization: epsilon must not be negative')
+        self.groups, self.axis, self.epsilon = int(groups), int(axis), float(epsilon)
+        self.center, self.scale, self.activation = bool(center), bool(scale), activation
+        self.beta_initializer, self.gamma_initializer = get_initializer(beta_initializer), get_initializer(gamma_initializer)
+        self.beta_regularizer, self.gamma_regularizer = beta_regularizer, gamma_regularizer
+        self.beta_constraint, self.gamma_constraint = beta_constraint, gamma_constraint
+        self.gamma = self.beta = None
+
+    def build(self, input_shape):
+        input_shape = tuple(input_shape)
+        if len(input_shape) < 2 or self.axis % len(input_shape) != len(input_shape) - 1:
+            raise NotImplementedError('GroupNormalization: the trailing axis of [batch, ..., channels] only')
+        channels = int(input_shape[-1])
+        if self.groups == -1:
+            self.groups = channels
+        if channels % self.groups:
+            raise ValueError(f'GroupNormalization: {channels} channels do not fall into {self.groups} groups of one size')
+        if self.scale:
+            self.gamma = self.add_weight(shape=(channels,), name='gamma', initializer=self.gamma_initializer, regularizer=self.gamma_regularizer,
+                                         constraint=self.gamma_constraint)
+        if self.center:
+            self.beta = self.add_weight(shape=(channels,), name='beta', initializer=self.beta_initializer, regularizer=self.beta_regularizer,
+                                        constraint=self.beta_constraint)
+        super().build(input_shape)
+
+    def call(self, x, training=None):
+        return ops.group_norm(x, self.groups, self.gamma, self.beta, self.epsilon, self.activation)
+
+    def get_config(self):
+        return {'name': self.name, 'groups': self.groups, 'axis': self.axis, 'epsilon': self.epsilon, 'center': self.center, 'scale': self.scale,
+                'beta_initializer': self.beta_initializer, 'gamma_initializer': self.gamma_initializer, 'beta_regularizer': self.beta_regularizer,
+                'gamma_regularizer': self.gamma_regularizer, 'beta_constraint': self.beta_constraint, 'gamma_constraint': self.gamma_constraint,
+                'activation': self.activation}
+
+    def host_fn(self, x):
+        """The same on a CPU tensor with library routines (for checks against a CPU model)."""
+        import torch.nn.functional as F
+
+        vec = [None if t is None else t.detach().to(x.device, x.dtype) for t in (self.gamma, self.beta)]
+        y = F.group_norm(x.movedim(-1, 1), self.groups, *vec, self.epsilon).movedim(1, -1)
+        return torch.relu(y) if self.activation == 'relu' else F.silu(y) if self.activation in ('silu', 'swish') else y
+
+
+layers = SimpleNamespace(GroupNormalization=GroupNormalization, MaxPooling2D=MaxPooling2D, AveragePooling2D=AveragePooling2D, Flatten=Flatten,
                          GlobalAveragePooling1D=GlobalAveragePooling1D, Layer=Layer)

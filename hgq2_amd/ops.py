@@ -20,7 +20,7 @@ from torch import Tensor
 
 from . import _lib
 
-__all__ = ['quantize', 'wrap_track_i_', 'qdense', 'dense_ebops', 'sparse_ce', 'sgd_update_', 'sgd_update_multi_', 'qsoftmax', 'conv2d', 'matmul_bias_act', 'col_moments', 'attn_scores', 'attn_combine', 'ATTN_MAX', 'pool2d', 'conv2d_ebops', 'conv_geometry', 'conv2d_ebops_supported', 'mse', 'dense_moments', 'dense_moments_supported', 'bn_fold', 'qbits', 'ebops_finish', 'qattention', 'qattention_supported', 'bits_ebops', 'gdense', 'gdense_supported', 'affine_rows', 'global_norm', 'adamw_update_multi_', 'adamw_state', 'adamw_moments']
+__all__ = ['quantize', 'wrap_track_i_', 'qdense', 'dense_ebops', 'sparse_ce', 'sgd_update_', 'sgd_update_multi_', 'qsoftmax', 'conv2d', 'matmul_bias_act', 'col_moments', 'attn_scores', 'attn_combine', 'ATTN_MAX', 'pool2d', 'conv2d_ebops', 'conv_geometry', 'conv2d_ebops_supported', 'mse', 'dense_moments', 'dense_moments_supported', 'bn_fold', 'qbits', 'ebops_finish', 'qattention', 'qattention_supported', 'bits_ebops', 'gdense', 'gdense_supported', 'affine_rows', 'global_norm', 'adamw_update_multi_', 'adamw_state', 'adamw_moments', 'group_norm']
 
 
 def _ptr(t: Tensor | None):
@@ -3582,6 +3582,113 @@ def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: flo
                           each(lo, -inf), each(hi, inf), each(decay, 0.0), bits, state, float(beta_1), float(beta_2), float(epsilon),
                           float(clipnorm or 0.0), norm_out if norm_out is not None else empty, int(seed) & (2**63 - 1))
     touch_state()
+
+
+# ---- group normalisation
+GROUP_ACTIVATIONS = {None: _lib.ACT_NONE, 'linear': _lib.ACT_NONE, 'relu': _lib.ACT_RELU, 'silu': _lib.ACT_SILU, 'swish': _lib.ACT_SILU}
+
+
+def _group_shape(x: Tensor, groups: int):
+    _need(x.is_cuda, f'x must be a GPU tensor (there is no CPU implementation), got device {x.device}')
+    code = _TYPE_CODES.get(x.dtype)
+    _need(code is not None, f'x must be float32, bfloat16 or float16, got {x.dtype}')
+    _need(x.dim() >= 2 and x.shape[-1] >= 1, 'x must be [batch, ..., channels]')
+    _need(x.is_contiguous(), 'x must be contiguous')
+    B, C = x.shape[0], x.shape[-1]
+    _need(groups >= 1 and C % groups == 0, f'{C} channels do not fall into {groups} groups of one size')
+    S = 1
+    for d in x.shape[1:-1]:
+        S *= d
+    return B, S, C, code
+
+
+def _channel_vector(name: str, t: Tensor, x: Tensor):
+    """A per-channel operand, or an empty tensor in the place of none."""
+    if t.numel():
+        _need(t.device == x.device and t.dtype is _F32 and t.is_contiguous() and t.numel() == x.shape[-1],
+              f'{name} must be a contiguous float32 tensor of {x.shape[-1]} elements on {x.device}')
+
+
+@torch.library.custom_op('hgq::group_norm_fwd', mutates_args=())
+def group_norm_fwd(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon: float, act: int) -> tuple[Tensor, Tensor, Tensor]:
+    """``gamma``, ``beta`` empty: none.  Returns y and, per sample and group, the mean and 1 / sqrt(var + epsilon)."""
+    B, S, C, code = _group_shape(x, groups)
+    _channel_vector('gamma', gamma, x), _channel_vector('beta', beta, x)
+    y = torch.empty_like(x)
+    stats = torch.empty(2, B, groups, dtype=torch.float32, device=x.device)
+    mean, rstd = stats.unbind(0)
+    lib = _lib.load()
+    with _device_of(x.device):
+        need = lib.hgq_group_norm_fwd_workspace(B, S, C, groups, code)
+        ws = torch.empty(need, dtype=torch.float32, device=x.device) if need > 0 else None
+        rc = lib.hgq_group_norm_fwd(_ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean), _ptr(rstd), _ptr(ws), B, S, C, groups, epsilon, act, code,
+                                    _stream())
+    _lib.check(rc, 'hgq_group_norm_fwd')
+    return y, mean, rstd
+
+
+@group_norm_fwd.register_fake
+def _(x, gamma, beta, groups, epsilon, act):
+    stats = x.new_empty((2, x.shape[0], groups), dtype=torch.float32)
+    return torch.empty_like(x), stats[0], stats[1]
+
+
+@torch.library.custom_op('hgq::group_norm_bwd', mutates_args=())
+def group_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, beta: Tensor, mean: Tensor, rstd: Tensor, groups: int, act: int, need_dx: bool,
+                   need_dgamma: bool, need_dbeta: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """Gradients that are not needed come back empty."""
+    B, S, C, code = _group_shape(x, groups)
+    _channel_vector('gamma', gamma, x), _channel_vector('beta', beta, x)
+    _need(dy.device == x.device and dy.dtype == x.dtype and dy.shape == x.shape and dy.is_contiguous(), 'dy must be like x')
+    _check_f32('mean', mean), _check_f32('rstd', rstd)
+    _need(mean.numel() == B * groups and rstd.numel() == B * groups, 'mean and rstd are what the forward call left')
+    dx = torch.empty_like(x) if need_dx else x.new_empty(0)
+    dgamma, dbeta = (torch.empty(C if want else 0, dtype=torch.float32, device=x.device) for want in (need_dgamma, need_dbeta))
+    lib = _lib.load()
+    with _device_of(x.device):
+        need = lib.hgq_group_norm_bwd_workspace(B, S, C, groups, code)
+        ws = torch.empty(need, dtype=torch.float32, device=x.device) if need > 0 else None
+        rc = lib.hgq_group_norm_bwd(_ptr(dy), _ptr(x), _ptr(gamma), _ptr(beta), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dgamma), _ptr(dbeta), _ptr(ws),
+                                    B, S, C, groups, act, code, _stream())
+    _lib.check(rc, 'hgq_group_norm_bwd')
+    return dx, dgamma, dbeta
+
+
+@group_norm_bwd.register_fake
+def _(dy, x, gamma, beta, mean, rstd, groups, act, need_dx, need_dgamma, need_dbeta):
+    C = x.shape[-1]
+    return (torch.empty_like(x) if need_dx else x.new_empty(0), x.new_empty(C if need_dgamma else 0, dtype=torch.float32),
+            x.new_empty(C if need_dbeta else 0, dtype=torch.float32))
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, groups, epsilon, act):
+        empty = torch.empty(0, dtype=torch.float32, device=x.device)
+        ga, be = (t if t is not None else empty for t in (gamma, beta))
+        y, mean, rstd = group_norm_fwd(x, ga, be, groups, epsilon, act)
+        ctx.save_for_backward(x, ga, be, mean, rstd)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, ga, be, mean, rstd = ctx.saved_tensors
+        want = ctx.needs_input_grad[:3]
+        grads = group_norm_bwd(gy.contiguous(), x, ga, be, mean, rstd, ctx.groups, ctx.act, *want)
+        return (*(g if w else None for g, w in zip(grads, want)), None, None, None)
+
+
+def group_norm(x: Tensor, groups: int, gamma: Tensor | None = None, beta: Tensor | None = None, epsilon: float = 1e-3,
+               activation: str | None = None) -> Tensor:
+    """Group normalisation of ``x`` ``[batch, ..., channels]`` (float32, bfloat16 or float16, any number of axes between) over each
+    sample's groups of adjacent channels and all its positions, times ``gamma`` plus ``beta`` (float32 ``[channels]``, or ``None``),
+    and an activation (``None`` / ``'linear'``, ``'relu'``, ``'silu'`` / ``'swish'``); differentiable in x, gamma and beta.  ``groups=1``
+    normalises whole samples, ``groups=channels`` each channel by itself."""
+    _need(activation in GROUP_ACTIVATIONS, f'activation must be one of linear, relu, silu; got {activation!r}')
+    _need(epsilon >= 0, 'epsilon must not be negative')
+    return _GroupNorm.apply(x.contiguous(), gamma, beta, int(groups), float(epsilon), GROUP_ACTIVATIONS[activation])
 
 
 # ======================================================================================

@@ -119,7 +119,8 @@ def _registry():
 
     reg = {name: getattr(layers, name) for name in layers.__all__ if isinstance(getattr(layers, name), type)}
     reg.update({'Sequential': _core.Sequential, 'Quantizer': Quantizer, 'MaxPooling2D': host.MaxPooling2D,
-                'AveragePooling2D': host.AveragePooling2D, 'Flatten': host.Flatten, 'GlobalAveragePooling1D': host.GlobalAveragePooling1D})
+                'AveragePooling2D': host.AveragePooling2D, 'Flatten': host.Flatten, 'GlobalAveragePooling1D': host.GlobalAveragePooling1D,
+                'GroupNormalization': host.GroupNormalization})
     return reg
 
 

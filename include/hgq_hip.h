@@ -62,6 +62,7 @@ extern "C" {
 
 #define HGQ_ACT_NONE 0
 #define HGQ_ACT_RELU 1
+#define HGQ_ACT_SILU 2 /* z / (1 + exp(-z)); hgq_group_norm_* alone */
 
 int hgq_version(void);
 const char *hgq_last_error(void);
@@ -1071,6 +1072,21 @@ int hgq_conv2d_ebops(const float *bits_in, const float *bits_ker, const hgq_conv
 
 /* Fill kernel (graph-capture safe replacement for a memset). */
 int hgq_fill_u32(uint32_t *p, uint32_t value, int64_t n, void *stream);
+
+/*
+ * Group normalisation with an activation over channels-last tensors (keras.layers.GroupNormalization beside the reference's
+ * layers; src/hgq/layers/batch_normalization.py normalises over the batch instead), x [B, S, C] with S positions and C channels in G groups:
+ *     xhat = (x - mean) / sqrt(var + eps) over a sample's group;   z = xhat gamma[c] + beta[c];   y = act(z)
+ * x, y, dy, dx: `type` (HGQ_TYPE_*), all else fp32.  gamma, beta [C] or NULL (1, 0); mean, rstd [B, G] are written by the forward
+ * call and read by the backward one; act HGQ_ACT_NONE, _RELU or _SILU.  dx, dgamma [C], dbeta [C]: NULL = not wanted; the latter are sums
+ * over B and S in an order that depends on the shape alone.  workspace: *_workspace(...) floats (0: NULL will do; -1: bad arguments).
+ */
+int64_t hgq_group_norm_fwd_workspace(int64_t B, int64_t S, int C, int G, int type);
+int hgq_group_norm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, float *workspace, int64_t B,
+                       int64_t S, int C, int G, float eps, int act, int type, void *stream);
+int64_t hgq_group_norm_bwd_workspace(int64_t B, int64_t S, int C, int G, int type);
+int hgq_group_norm_bwd(const void *dy, const void *x, const float *gamma, const float *beta, const float *mean, const float *rstd, void *dx,
+                       float *dgamma, float *dbeta, float *workspace, int64_t B, int64_t S, int C, int G, int act, int type, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,323 @@
+"""Group normalisation against a plain implementation in 64 bits.
+
+Tolerances, u = 2^-24 (half a step of fp32) and L = 96: no sum of the kernels adds more than 64 terms one after the other before it goes
+on pairwise, in at most 32 further levels, so a sum is off by at most L u times the sum of magnitudes.  The mean is then off by L u
+mean|x| and the variance, formed about that mean, relatively by 2 L u; xhat by rstd L u mean|x| + L u |xhat|.  z adds three roundings, an
+activation at most 1.1 times what z is off (the largest slope of z / (1 + exp(-z))) and 8 u of its own.  The backward formulas are carried through term by
+term below (a second derivative is at most 1/2).  A 16-bit type adds half a step.  Where |z| is within its tolerance of zero the slope of
+a relu may be either: such elements are left out, and counted into the sums' tolerances."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U, L = 2.0**-24, 96
+HALF = {torch.float32: 0.0, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+
+
+def _definition(x, dy, gamma, beta, G, eps, act):
+    """Values and tolerances of y, dx, dgamma, dbeta in 64 bits on the CPU; x [B, S, C]."""
+    x, dy = x.double().cpu(), dy.double().cpu()
+    B, S, C = x.shape
+    ga = gamma.double().cpu() if gamma is not None else torch.ones(C, dtype=torch.float64)
+    be = beta.double().cpu() if beta is not None else torch.zeros(C, dtype=torch.float64)
+    per = lambda t: t.view(B, S, G, C // G)  # noqa: E731
+    gmean = lambda t: per(t).mean(dim=(1, 3), keepdim=True)  # noqa: E731
+    whole = lambda t: t.expand(B, S, G, C // G).reshape(B, S, C)  # noqa: E731
+    mean = gmean(x)
+    var = ((per(x) - mean) ** 2).mean(dim=(1, 3), keepdim=True)
+    rstd = whole(1 / torch.sqrt(var + eps))
+    xh = (x - whole(mean)) * rstd
+    t_xh = rstd * L * U * whole(gmean(x.abs())) + (L + 4) * U * xh.abs()
+    z = xh * ga + be
+    t_z = t_xh * ga.abs() + 3 * U * ((xh * ga).abs() + be.abs())
+    p = torch.sigmoid(z)
+    if act == 'relu':
+        y, slope, unsure = z.clamp(min=0), (z > 0).double(), z.abs() <= t_z
+    elif act == 'silu':
+        y, slope, unsure = z * p, p * (1 + z * (1 - p)), torch.zeros_like(z, dtype=torch.bool)
+    else:
+        y, slope, unsure = z, torch.ones_like(z), torch.zeros_like(z, dtype=torch.bool)
+    curved = 1.0 if act == 'silu' else 0.0
+    t_y = 1.1 * t_z + curved * 8 * U * y.abs() * (1 + z.abs())
+    dz = dy * slope
+    t_dz = dy.abs() * (curved * (0.5 * t_z + 16 * U * (1 + z.abs())) + U) + torch.where(unsure, dy.abs(), 0.0)
+    d, t_d = dz * ga, t_dz * ga.abs() + U * (dz * ga).abs()
+    m1, m2 = whole(gmean(d)), whole(gmean(d * xh))
+    t_m1 = whole(gmean(t_d)) + L * U * whole(gmean(d.abs()))
+    t_m2 = whole(gmean(t_d * xh.abs() + d.abs() * t_xh)) + L * U * whole(gmean((d * xh).abs()))
+    dx = (d - m1 - xh * m2) * rstd
+    t_dx = rstd * (t_d + t_m1 + xh.abs() * t_m2 + m2.abs() * t_xh + 4 * U * (d.abs() + m1.abs() + (xh * m2).abs())) + (L + 4) * U * dx.abs()
+    t_dx = torch.where(unsure, math.inf, t_dx)
+    dgamma, dbeta = (dz * xh).sum(dim=(0, 1)), dz.sum(dim=(0, 1))
+    t_dg = (t_dz * xh.abs() + dz.abs() * t_xh).sum(dim=(0, 1)) + 2 * L * U * (dz * xh).abs().sum(dim=(0, 1))
+    t_db = t_dz.sum(dim=(0, 1)) + 2 * L * U * dz.abs().sum(dim=(0, 1))  # (twice: within a sample, and over the samples)
+    return (y, dx, dgamma, dbeta), (t_y, t_dx, t_dg, t_db)
+
+
+def _check(got, want, tol, dtype, what):
+    got = got.detach().double().cpu().reshape(want.shape)
+    tol = tol + HALF[dtype] * (want.abs() + tol).clamp(max=1e300) + (2.0**-25 if dtype == torch.float16 else 0.0)
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()}, worst {float(((got - want).abs() / tol.clamp(min=1e-300)).max()):.3g} times the tolerance'
+
+
+def _run(dev, shape, G, dtype, act, seed, eps=1e-3, scale=True, center=True, offset=0.5):
+    from hgq2_amd import ops
+
+    g = torch.Generator().manual_seed(seed)
+    C = shape[-1]
+    x = (torch.randn(shape, generator=g) + offset * torch.randn(C, generator=g)).to(dtype).to(dev).requires_grad_(True)
+    dy = torch.randn(shape, generator=g).to(dtype).to(dev)
+    gamma = (1 + 0.3 * torch.randn(C, generator=g)).to(dev).requires_grad_(True) if scale else None
+    beta = (0.3 * torch.randn(C, generator=g)).to(dev).requires_grad_(True) if center else None
+    y = ops.group_norm(x, G, gamma, beta, eps, act)
+    assert y.dtype == dtype and y.shape == x.shape
+    leaves = [t for t in (x, gamma, beta) if t is not None]
+    grads = list(torch.autograd.grad(y, leaves, dy))
+    flat = (shape[0], -1, C)
+    want, tol = _definition(x.detach().reshape(flat), dy.reshape(flat), None if gamma is None else gamma.detach(), None if beta is None else beta.detach(), G, eps, act)
+    _check(y, want[0], tol[0], dtype, 'y')
+    _check(grads.pop(0), want[1], tol[1], dtype, 'dx')
+    if scale:
+        _check(grads.pop(0), want[2], tol[2], torch.float32, 'dgamma')
+    if center:
+        _check(grads.pop(0), want[3], tol[3], torch.float32, 'dbeta')
+
+
+# a row of one channel; channels by themselves; whole samples; rows of odd width; groups narrower and wider than 16 bytes; few long and many short samples
+SHAPES = [((3, 1, 1), 1), ((1, 7), 7), ((5, 24), 4), ((4, 1, 64), 1), ((2, 9, 33), 3), ((2, 5, 7, 35), 5), ((3, 17, 40), 40), ((2, 6, 6, 32), 8),
+          ((2, 1, 30, 48), 6), ((97, 30, 48), 6), ((1, 28, 28, 32), 8), ((2, 64, 64, 64), 1), ((1, 61, 67, 96), 4), ((3, 2, 3, 4, 16), 2),
+          ((2, 3, 5000), 1), ((1, 4, 9000), 2), ((2, 100, 1000), 250), ((1, 20000, 8), 2), ((1, 130, 130, 24), 3), ((700, 3, 6), 2), ((2, 300, 512), 32),
+          ((1, 5, 8192), 1), ((1, 3, 12288), 3), ((2, 40, 1028), 257), ((1, 70000, 4), 4), ((40, 49, 256), 32), ((1, 1, 100000), 1)]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('shape,G', SHAPES)
+def test_against_64_bits(dev, shape, G, dtype):
+    act = ('linear', 'relu', 'silu')[(sum(shape) + G) % 3]
+    _run(dev, shape, G, dtype, act, sum(shape) * 7 + G)
+
+
+@pytest.mark.parametrize('act', ['linear', 'relu', 'silu', 'swish', None])
+@pytest.mark.parametrize('scale,center', [(True, True), (False, True), (True, False), (False, False)])
+def test_activations_and_missing_variables(dev, act, scale, center):
+    _run(dev, (6, 10, 10, 20), 5, torch.float32, act if act != 'swish' else 'silu', 5, scale=scale, center=center)
+    from hgq2_amd import ops
+
+    x = torch.randn(3, 4, 8, device=dev)
+    if act in ('swish', None):
+        assert torch.equal(ops.group_norm(x, 2, activation=act), ops.group_norm(x, 2, activation={'swish': 'silu', None: 'linear'}[act]))
+
+
+@pytest.mark.parametrize('shape,G', [((2, 50, 32), 4), ((1, 40000, 16), 2), ((2, 3, 5000), 1)])
+def test_far_from_zero(dev, shape, G):
+    """A mean of 3000 standard deviations: mean(x^2) - mean(x)^2 would be noise."""
+    from hgq2_amd import ops
+
+    g = torch.Generator().manual_seed(2)
+    x = (torch.randn(shape, generator=g) + 3000.0).to(dev)
+    y = ops.group_norm(x, G, epsilon=0.0)
+    # (fp32 holds x to 2^-13 of the standard deviation; the kernel starts from what is held)
+    want, tol = _definition(x, torch.zeros(shape), None, None, G, 0.0, 'linear')
+    _check(y, want[0], tol[0], torch.float32, 'y')
+    assert abs(float(y.double().square().mean()) - 1) < 0.01
+
+
+def test_what_is_not_finite_stays_in_its_group(dev):
+    from hgq2_amd import ops
+
+    for shape, G in (((4, 20, 12), 3), ((2, 50000, 8), 2), ((3, 2, 6000), 2)):
+        g = torch.Generator().manual_seed(3)
+        x = torch.randn(shape, generator=g).to(dev)
+        dy = torch.randn(shape, generator=g).to(dev)
+        for bad in (float('nan'), float('inf')):
+            for act in ('linear', 'relu', 'silu'):
+                outs = []
+                for poison in (False, True):
+                    xp = x.clone()
+                    if poison:
+                        xp[1, 1, 0] = bad
+                    xp.requires_grad_(True)
+                    y = ops.group_norm(xp, G, activation=act)
+                    outs.append((y.detach(), *torch.autograd.grad(y, xp, dy)))
+                D = shape[-1] // G
+                for a, b in zip(*outs):
+                    keep = torch.ones(shape, dtype=torch.bool, device=dev)
+                    keep[1, :, :D] = False
+                    assert torch.equal(a[keep], b[keep]) and torch.isfinite(a).all()
+                    assert torch.isnan(b[~keep]).all()
+
+
+def test_empty_batches(dev):
+    from hgq2_amd import ops
+
+    for shape in ((0, 5, 8), (3, 0, 8)):
+        x = torch.zeros(shape, device=dev, requires_grad=True)
+        gamma, beta = torch.ones(8, device=dev, requires_grad=True), torch.zeros(8, device=dev, requires_grad=True)
+        y = ops.group_norm(x, 2, gamma, beta)
+        dx, dg, db = torch.autograd.grad(y, [x, gamma, beta], torch.zeros(shape, device=dev))
+        assert y.shape == dx.shape == shape and not dg.any() and not db.any()
+
+
+def test_strides_offsets_and_partial_gradients(dev):
+    """Views that begin off an aligned address, transposed inputs and gradients, and gradients of some operands only."""
+    from hgq2_amd import ops
+
+    g = torch.Generator().manual_seed(4)
+    for dtype in (torch.float32, torch.bfloat16):
+        for C, G, S in ((32, 8, 50), (32, 8, 20000), (48, 6, 30)):
+            buf = torch.randn(1 + 2 * S * C, generator=g).to(dtype).to(dev)
+            x = buf[1:].view(2, S, C)
+            dy = torch.randn(2, C, S, generator=g).to(dtype).to(dev).transpose(1, 2)
+            gamma = torch.randn(1 + C, generator=g).to(dev)[1:]
+            xs, ga = x.clone().requires_grad_(True), gamma.clone().requires_grad_(True)
+            xt = x.transpose(1, 2).contiguous().transpose(1, 2).requires_grad_(True)
+            base = ops.group_norm(xs, G, ga, activation='silu')
+            wx, wg = torch.autograd.grad(base, [xs, ga], dy.contiguous())
+            xv = x.detach().requires_grad_(True)
+            gv = gamma.detach().requires_grad_(True)
+            y = ops.group_norm(xv, G, gv, activation='silu')
+            vx, vg = torch.autograd.grad(y, [xv, gv], dy)
+            tol = 2.0**-7 if dtype == torch.bfloat16 else 1e-5  # (another order of the same sums)
+            for a, b in ((y, base), (vx, wx)):
+                assert float((a.float() - b.float()).abs().max()) <= tol * float(b.float().abs().max())
+            assert float((vg - wg).abs().max()) <= 1e-4 * float(wg.abs().max())
+            yt = ops.group_norm(xt, G, ga, activation='silu')
+            assert torch.equal(yt, base)
+            only_gamma, = torch.autograd.grad(ops.group_norm(x.clone(), G, ga, activation='silu'), [ga], dy.contiguous())
+            assert torch.equal(only_gamma, wg)
+            only_x, = torch.autograd.grad(ops.group_norm(xs, G, ga.detach(), activation='silu'), [xs], dy.contiguous())
+            assert torch.equal(only_x, wx)
+
+
+def test_gradients_against_differences(dev):
+    """Directional differences of the definition in 64 bits at the same point: the error of a central difference of step h is of order
+    h^2, 1e-8 here, and the fp32 gradients are within 1e-5 of their scale."""
+    from hgq2_amd import ops
+
+    g = torch.Generator().manual_seed(5)
+    x0, dy = torch.randn(3, 11, 12, generator=g), torch.randn(3, 11, 12, generator=g)
+    ga0, be0 = 1 + 0.3 * torch.randn(12, generator=g), 0.3 * torch.randn(12, generator=g)
+
+    def value(x, ga, be):
+        t = x.view(3, 11, 4, 3)
+        m = t.mean(dim=(1, 3), keepdim=True)
+        v = ((t - m) ** 2).mean(dim=(1, 3), keepdim=True)
+        z = ((t - m) / torch.sqrt(v + 1e-3)).reshape(3, 11, 12) * ga + be
+        return float((z * torch.sigmoid(z) * dy.double()).sum())
+
+    ops_in = [t.to(dev).requires_grad_(True) for t in (x0, ga0, be0)]
+    grads = torch.autograd.grad(ops.group_norm(ops_in[0], 4, ops_in[1], ops_in[2], 1e-3, 'silu'), ops_in, dy.to(dev))
+    for k in range(3):
+        for trial in range(4):
+            at = [t.double() for t in (x0, ga0, be0)]
+            way = torch.randn(at[k].shape, generator=g, dtype=torch.float64)
+            h = 1e-4
+            lo, hi = list(at), list(at)
+            lo[k], hi[k] = at[k] - h * way, at[k] + h * way
+            diff = (value(*hi) - value(*lo)) / (2 * h)
+            have = float((grads[k].double().cpu() * way).sum())
+            assert abs(have - diff) <= 1e-5 * float((grads[k].double().cpu() * way).abs().sum()) + 1e-6
+
+
+@pytest.mark.parametrize('shape,G', [((64, 13, 13, 32), 8), ((2, 128, 128, 32), 4), ((2, 5, 6000), 2)])
+def test_recorded_and_repeated(dev, shape, G):
+    """Forward and backward recorded together: every replay gives the eager bits for the inputs of its time, and two recordings that are
+    replayed in turn do not disturb each other; repeated calls give the same bits."""
+    from hgq2_amd import ops
+
+    gen = torch.Generator().manual_seed(6)
+    C = shape[-1]
+    feeds = [(torch.randn(shape, generator=gen).to(dev), torch.randn(shape, generator=gen).to(dev)) for _ in range(3)]
+    gamma, beta = torch.randn(C, generator=gen).to(dev).requires_grad_(True), torch.randn(C, generator=gen).to(dev).requires_grad_(True)
+
+    def both(x, dy):
+        y = ops.group_norm(x, G, gamma, beta, activation='relu')
+        return (y.detach(), *torch.autograd.grad(y, [x, gamma, beta], dy))
+
+    eager = [both(x.clone().requires_grad_(True), dy) for x, dy in feeds]
+    again = both(feeds[0][0].clone().requires_grad_(True), feeds[0][1])
+    assert all(torch.equal(a, b) for a, b in zip(eager[0], again))
+    side = torch.cuda.Stream()
+    recorded = []
+    for _ in range(2):
+        x, dy = feeds[0][0].clone().requires_grad_(True), feeds[0][1].clone()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            both(x, dy)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = both(x, dy)
+        recorded.append((graph, x, dy, out))
+    for k in (0, 1, 2, 1, 0):
+        for graph, x, dy, _ in recorded:
+            with torch.no_grad():
+                x.copy_(feeds[k][0]), dy.copy_(feeds[k][1])
+        for graph, *_ in recorded:
+            graph.replay()
+        both(feeds[2][0].clone().requires_grad_(True), feeds[2][1])  # eager work between the replays
+        torch.cuda.synchronize()
+        for _, _, _, out in recorded:
+            assert all(torch.equal(a, b) for a, b in zip(out, eager[k])), k
+
+
+def test_layer_against_its_host_form(dev):
+    from hgq2_amd.host import GroupNormalization
+
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(4, 9, 9, 24, generator=g)
+    for act in (None, 'relu', 'silu'):
+        layer = GroupNormalization(6, activation=act)
+        layer(x.to(dev))
+        with torch.no_grad():
+            layer.gamma.copy_(torch.rand(24, generator=g) + 0.5), layer.beta.copy_(torch.randn(24, generator=g))
+        got, want = layer(x.to(dev), training=True).detach().cpu().double(), layer.host_fn(x.double())
+        assert float((got - want).abs().max()) <= 1e-5 * float(want.abs().max())
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_normalised_network_trained_with_adamw(dev, bits):
+    """The operators together as they are used: a quantized convolution, group normalisation with its activation, a quantized dense layer; loss,
+    clipped AdamW step; recorded, against the same steps run eagerly."""
+    from hgq2_amd import ops
+    from hgq2_amd.config import LayerConfigScope, QuantizerConfigScope
+    from hgq2_amd.host import Flatten, GroupNormalization, MaxPooling2D, Sequential
+    from hgq2_amd.layers import QConv2D, QDense
+    from hgq2_amd.train import AdamW, model_loss, train_step_for
+
+    g = torch.Generator().manual_seed(8)
+    x, y = torch.rand(12, 14, 14, 1, generator=g).to(dev), torch.randint(0, 10, (12,), generator=g).to(dev)
+
+    def net():
+        with QuantizerConfigScope(place='all', default_q_type='kbi', overflow_mode='SAT_SYM'), \
+             QuantizerConfigScope(place='datalane', default_q_type='kif', overflow_mode='WRAP'), LayerConfigScope(enable_ebops=True, beta0=1e-6):
+            model = Sequential([QConv2D(16, 3), GroupNormalization(4, activation='relu'), MaxPooling2D((2, 2)), QConv2D(8, 3), GroupNormalization(1, activation='silu'),
+                                Flatten(), QDense(10)])
+        model(x, training=False)
+        return model
+
+    make = lambda v: AdamW(v, lr=0.003, global_clipnorm=2.0, state_bits=bits, seed=3, fold_regularizers=True)  # noqa: E731
+    a, b = net(), net()
+    with torch.no_grad():
+        for p, q in zip(a.parameters(), b.parameters()):
+            q.copy_(p)
+    names = [p.var_name for p in a.parameters() if p.requires_grad]
+    assert names.count('gamma') == 2 and names.count('beta') >= 2
+    step = train_step_for(a, x, y, optimizer=make, warmup=1)
+    losses = [float(step()) for _ in range(3)]
+    opt = make(b.parameters())
+    for k in range(4):
+        opt.zero_grad()
+        loss = model_loss(b, ops.sparse_ce(b(x, training=True), y), True)
+        opt.backward(loss)
+        opt.step()
+        if k:
+            assert float(loss) == losses[k - 1]  # the same launches
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert torch.equal(p, q) and torch.isfinite(p).all()
+    assert step.opt.iterations == opt.iterations == 4
