@@ -30,7 +30,7 @@ struct AdamwItem {
     uint8_t *m_scale, *v_scale;
     int64_t n, first;
     float l1, lo, hi, decay;
-    int type;
+    short type, vec;      // vec: a plain gradient and aligned memory, four elements per access
     short piece, pieces;  // its entries of the launch's list of further gradient pieces
 };
 struct AdamwLaunch {
@@ -113,55 +113,149 @@ __device__ __forceinline__ float adamw_weight(float w, float m, float r, const A
     return w < it.lo ? it.lo : w > it.hi ? it.hi : w;  // (not a number stays that)
 }
 
+// the new moments of one element with gradient g: m, v and r = sqrt(v)
+__device__ __forceinline__ void adamw_moments(float g, float &m, float &v, float &r, const AdamwStep &k) {
+    g = __fmul_rn(g, k.c);
+    m = __fadd_rn(m, __fmul_rn(__fsub_rn(g, m), k.one_minus_b1));
+    v = __fadd_rn(v, __fmul_rn(__fsub_rn(__fmul_rn(g, g), v), k.one_minus_b2));
+    r = __fsqrt_rn(v);
+}
+
+// Codes of a wavefront's block, four neighbours per lane (those behind the last element: zeros): m and r go in, the scale bytes
+// and a word of four codes each come out.
+__device__ __forceinline__ void encode_block(const float (&m)[4], const float (&r)[4], uint64_t element, const AdamwStep &k, int &sm, int &sr,
+                                             uint32_t &cm, uint32_t &cr) {
+    uint32_t em = 8, er = 8;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) em = max(em, exponent_field(m[j])), er = max(er, exponent_field(r[j]));
+#pragma unroll
+    for (int d = 32; d; d >>= 1) em = max(em, (uint32_t)__shfl_xor((int)em, d)), er = max(er, (uint32_t)__shfl_xor((int)er, d));
+    sm = (int)em - 7, sr = (int)er - 7;
+    uint32_t h[4];
+    philox4x32_7(element >> 2, k.t, k.seed, h);
+    cm = cr = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t a = e4m3_code(fabsf(m[j]), sm, h[j] & 0xffff) | ((__float_as_uint(m[j]) >> 24) & 0x80u);
+        uint32_t b = e4m3_code(r[j], sr, h[j] >> 16);
+        if (b == 0 && r[j] > 0.0f) b = 1;
+        cm |= a << (8 * j), cr |= b << (8 * j);
+    }
+}
+
+// a wavefront's block of 256 elements at b, element by element: any alignment, any gradient pieces, any end
+template <int BITS>
+__device__ __forceinline__ void adamw_block_any(const AdamwLaunch &a, const AdamwItem &it, const AdamwStep &k, int64_t b) {
+    const int lane = threadIdx.x & 63;
+    const int64_t e = b + lane * 4;
+    float m[4], r[4];
+    int sm = 0, sr = 0;
+    if (BITS == 8) sm = it.m_scale[b >> 8], sr = it.v_scale[b >> 8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        m[j] = r[j] = 0.0f;
+        if (e + j < it.n) {
+            float v;
+            if (BITS == 8) {
+                m[j] = e4m3_value(((const uint8_t *)it.m)[e + j], sm);
+                v = e4m3_value(((const uint8_t *)it.v)[e + j], sr);
+                v = __fmul_rn(v, v);
+            } else {
+                m[j] = ((const float *)it.m)[e + j], v = ((const float *)it.v)[e + j];
+            }
+            adamw_moments(gradient(a, it, e + j), m[j], v, r[j], k);
+            store_f32_as(it.w, e + j, it.type, adamw_weight(load_as_f32(it.w, e + j, it.type), m[j], r[j], it, k));
+            if (BITS == 32) ((float *)it.m)[e + j] = m[j], ((float *)it.v)[e + j] = v;
+        }
+    }
+    if (BITS == 8) {
+        uint32_t cm, cr;
+        encode_block(m, r, (uint64_t)(it.first + e), k, sm, sr, cm, cr);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (e + j < it.n) ((uint8_t *)it.m)[e + j] = (uint8_t)(cm >> (8 * j)), ((uint8_t *)it.v)[e + j] = (uint8_t)(cr >> (8 * j));
+        if (lane == 0) it.m_scale[b >> 8] = (uint8_t)sm, it.v_scale[b >> 8] = (uint8_t)sr;
+    }
+}
+
+typedef uint32_t words2_t __attribute__((ext_vector_type(2)));
+typedef float floats4_t __attribute__((ext_vector_type(4)));
+
+// four neighbours of an aligned array as they lie in memory
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+    typedef floats4_t raw;
+};
+template <>
+struct Four<__bf16> {
+    typedef __bf16 raw __attribute__((ext_vector_type(4)));
+};
+template <>
+struct Four<_Float16> {
+    typedef _Float16 raw __attribute__((ext_vector_type(4)));
+};
+
+// N of a wavefront's whole blocks, at b and every 1024 elements on: four elements per access, all loads before the first use
+template <int BITS, typename T, int N>
+__device__ __forceinline__ void adamw_blocks(const AdamwItem &it, const AdamwStep &k, int64_t b) {
+    typedef typename Four<T>::raw raw;
+    const int lane = threadIdx.x & 63;
+    const int64_t e = b + lane * 4;
+    raw w[N], g[N];
+    floats4_t m[N], v[N];
+    uint32_t cm[N], cr[N];
+    int sm[N], sr[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        g[n] = *(const raw *)((const T *)it.g + e + 1024 * n);
+        w[n] = *(const raw *)((const T *)it.w + e + 1024 * n);
+        if (BITS == 32) {
+            m[n] = *(const floats4_t *)((const float *)it.m + e + 1024 * n), v[n] = *(const floats4_t *)((const float *)it.v + e + 1024 * n);
+        } else {
+            cm[n] = *(const uint32_t *)((const uint8_t *)it.m + e + 1024 * n), cr[n] = *(const uint32_t *)((const uint8_t *)it.v + e + 1024 * n);
+            sm[n] = it.m_scale[(b >> 8) + 4 * n], sr[n] = it.v_scale[(b >> 8) + 4 * n];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        float mm[4], rr[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float vv;
+            if (BITS == 32) {
+                mm[j] = m[n][j], vv = v[n][j];
+            } else {
+                mm[j] = e4m3_value((cm[n] >> (8 * j)) & 0xff, sm[n]), vv = e4m3_value((cr[n] >> (8 * j)) & 0xff, sr[n]);
+                vv = __fmul_rn(vv, vv);
+            }
+            adamw_moments(__fadd_rn((float)g[n][j], it.l1), mm[j], vv, rr[j], k);
+            w[n][j] = (T)adamw_weight((float)w[n][j], mm[j], rr[j], it, k);
+            m[n][j] = mm[j], v[n][j] = vv;
+        }
+        *(raw *)((T *)it.w + e + 1024 * n) = w[n];
+        if (BITS == 32) {
+            *(floats4_t *)((float *)it.m + e + 1024 * n) = m[n], *(floats4_t *)((float *)it.v + e + 1024 * n) = v[n];
+        } else {
+            encode_block(mm, rr, (uint64_t)(it.first + e + 1024 * n), k, sm[n], sr[n], cm[n], cr[n]);
+            *(uint32_t *)((uint8_t *)it.m + e + 1024 * n) = cm[n], *(uint32_t *)((uint8_t *)it.v + e + 1024 * n) = cr[n];
+            if (lane == 0) it.m_scale[(b >> 8) + 4 * n] = (uint8_t)sm[n], it.v_scale[(b >> 8) + 4 * n] = (uint8_t)sr[n];
+        }
+    }
+}
+
 // one variable's elements [e0, e0 + ADAMW_CHUNK): a lane takes four neighbours, a wavefront 256 - the block that shares a scale
 template <int BITS>
 __device__ __forceinline__ void adamw_chunk(const AdamwLaunch &a, const AdamwItem &it, const AdamwStep &k, int64_t e0) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t b = e0 + wave * 256; b < e0 + ADAMW_CHUNK && b < it.n; b += 1024) {
-        const int64_t e = b + lane * 4;
-        float m[4], r[4];
-        int sm = 0, sr = 0;
-        if (BITS == 8) sm = it.m_scale[b >> 8], sr = it.v_scale[b >> 8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            m[j] = r[j] = 0.0f;
-            if (e + j < it.n) {
-                const float g = __fmul_rn(gradient(a, it, e + j), k.c);
-                float v;
-                if (BITS == 8) {
-                    m[j] = e4m3_value(((const uint8_t *)it.m)[e + j], sm);
-                    v = e4m3_value(((const uint8_t *)it.v)[e + j], sr);
-                    v = __fmul_rn(v, v);
-                } else {
-                    m[j] = ((const float *)it.m)[e + j], v = ((const float *)it.v)[e + j];
-                }
-                m[j] = __fadd_rn(m[j], __fmul_rn(__fsub_rn(g, m[j]), k.one_minus_b1));
-                v = __fadd_rn(v, __fmul_rn(__fsub_rn(__fmul_rn(g, g), v), k.one_minus_b2));
-                r[j] = __fsqrt_rn(v);
-                store_f32_as(it.w, e + j, it.type, adamw_weight(load_as_f32(it.w, e + j, it.type), m[j], r[j], it, k));
-                if (BITS == 32) ((float *)it.m)[e + j] = m[j], ((float *)it.v)[e + j] = v;
-            }
-        }
-        if (BITS == 8) {
-            uint32_t em = 8, er = 8;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) em = max(em, exponent_field(m[j])), er = max(er, exponent_field(r[j]));
-#pragma unroll
-            for (int d = 32; d; d >>= 1) em = max(em, (uint32_t)__shfl_xor((int)em, d)), er = max(er, (uint32_t)__shfl_xor((int)er, d));
-            sm = (int)em - 7, sr = (int)er - 7;
-            uint32_t h[4];
-            philox4x32_7((uint64_t)(it.first + e) >> 2, k.t, k.seed, h);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (e + j < it.n) {
-                    uint32_t cr = e4m3_code(r[j], sr, h[j] >> 16);
-                    if (cr == 0 && r[j] > 0.0f) cr = 1;
-                    ((uint8_t *)it.m)[e + j] = (uint8_t)(e4m3_code(fabsf(m[j]), sm, h[j] & 0xffff) | (signbit(m[j]) ? 0x80u : 0u));
-                    ((uint8_t *)it.v)[e + j] = (uint8_t)cr;
-                }
-            if (lane == 0) it.m_scale[b >> 8] = (uint8_t)sm, it.v_scale[b >> 8] = (uint8_t)sr;
-        }
+    const int64_t b0 = e0 + (threadIdx.x >> 6) * 256;
+    if (it.vec && e0 + ADAMW_CHUNK <= it.n) {
+        if (it.type == HGQ_TYPE_F32) adamw_blocks<BITS, float, 2>(it, k, b0);
+        else if (it.type == HGQ_TYPE_BF16) adamw_blocks<BITS, __bf16, 2>(it, k, b0);
+        else adamw_blocks<BITS, _Float16, 2>(it, k, b0);
+        return;
     }
+    for (int64_t b = b0; b < e0 + ADAMW_CHUNK && b < it.n; b += 1024) adamw_block_any<BITS>(a, it, k, b);
 }
 
 // sum of the workgroup's values, in a fixed order, returned to every thread
@@ -266,7 +360,9 @@ int for_launches(const hgq_adamw_item *items, int count, F fn) {
             if (pieces + own > ADAMW_PIECES || (n > 0 && chunks + own_chunks > 0x7fffffffu)) break;
             AdamwItem &d = a.item[n];
             d.w = s.w, d.g = s.g, d.m = s.m, d.v = s.v, d.m_scale = s.m_scale, d.v_scale = s.v_scale, d.n = s.n, d.first = s.first;
-            d.l1 = s.l1, d.lo = s.lo, d.hi = s.hi, d.decay = s.decay, d.type = s.type, d.piece = (short)pieces, d.pieces = (short)own;
+            d.l1 = s.l1, d.lo = s.lo, d.hi = s.hi, d.decay = s.decay, d.type = (short)s.type, d.piece = (short)pieces, d.pieces = (short)own;
+            const uintptr_t size = s.type == HGQ_TYPE_F32 ? 4 : 2, moment = s.m_scale ? 1 : 4;
+            d.vec = own == 0 && (((uintptr_t)s.w | (uintptr_t)s.g) & (4 * size - 1)) == 0 && (((uintptr_t)s.m | (uintptr_t)s.v) & (4 * moment - 1)) == 0;
             for (int k = 0; k < HGQ_SGD_SIDES; ++k)
                 if (s.side[k]) a.side[pieces] = s.side[k], a.side_scale[pieces] = s.side_scale[k], ++pieces;
             a.start[n] = (uint32_t)chunks;
