@@ -22,6 +22,7 @@ namespace hgq {
 constexpr int ADAMW_ITEMS = 28, ADAMW_PIECES = 32;
 constexpr int ADAMW_CHUNK = 2048;  // elements a workgroup takes at a time: eight blocks of 256
 constexpr int ADAMW_GRID = 2048;
+constexpr int NORM_LOADS = 8, NORM_GRID = 1024;
 
 struct AdamwItem {
     void *w;
@@ -311,15 +312,44 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
         state->step = t, state->beta_1_power = p1, state->beta_2_power = p2, state->ticket = 0;
 }
 
+// squares of four neighbours; (v ^ 2 of fp32 has 48 bits and stays exact in fp64)
+template <typename T>
+__device__ __forceinline__ double squares(const typename Four<T>::raw &g, float l1) {
+    double v = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const double d = __fadd_rn((float)g[j], l1);
+        v += d * d;
+    }
+    return v;
+}
+
+// one variable's elements [e0, e0 + NORM_LOADS * 1024), whole and aligned: all loads before the first use
+template <typename T>
+__device__ __forceinline__ double norm_chunk(const AdamwItem &it, int64_t e0) {
+    typedef typename Four<T>::raw raw;
+    raw g[NORM_LOADS];
+#pragma unroll
+    for (int n = 0; n < NORM_LOADS; ++n) g[n] = *(const raw *)((const T *)it.g + e0 + 1024 * n + 4 * threadIdx.x);
+    double v = 0;
+#pragma unroll
+    for (int n = 0; n < NORM_LOADS; ++n) v += squares<T>(g[n], it.l1);
+    return v;
+}
+
 // sums of squares, one per workgroup: in fp64, so that no finite gradient overflows and their order does not show
-__global__ __launch_bounds__(256) void norm_parts_kernel(AdamwLaunch a, int items, double *parts) {
+__global__ __launch_bounds__(256) void norm_parts_kernel(AdamwLaunch a, int items, int chunk, double *parts) {
     __shared__ double lds[4];
     double v = 0;
     int i = 0;
     for (uint32_t c = blockIdx.x; c < a.start[items]; c += gridDim.x) {
         while (c >= a.start[i + 1]) ++i;
         const AdamwItem &it = a.item[i];
-        const int64_t e0 = (int64_t)(c - a.start[i]) * ADAMW_CHUNK, end = e0 + ADAMW_CHUNK < it.n ? e0 + ADAMW_CHUNK : it.n;
+        const int64_t e0 = (int64_t)(c - a.start[i]) * chunk, end = e0 + chunk < it.n ? e0 + chunk : it.n;
+        if (it.vec && end - e0 == NORM_LOADS * 1024) {
+            v += it.type == HGQ_TYPE_F32 ? norm_chunk<float>(it, e0) : it.type == HGQ_TYPE_BF16 ? norm_chunk<__bf16>(it, e0) : norm_chunk<_Float16>(it, e0);
+            continue;
+        }
         for (int64_t e = e0 + threadIdx.x; e < end; e += 256) {
             const double g = gradient(a, it, e);
             v += g * g;
@@ -344,7 +374,7 @@ namespace {
 // Goes over `items` in launches of up to ADAMW_ITEMS variables and ADAMW_PIECES further gradient pieces: fn(launch, variables, last).
 // Descriptors travel as launch arguments (4 KB at most), so the calls are safe under HIP graph capture.
 template <class F>
-int for_launches(const hgq_adamw_item *items, int count, F fn) {
+int for_launches(const hgq_adamw_item *items, int count, int chunk, F fn) {
     int at = 0;
     bool done = false;
     while (!done) {
@@ -356,7 +386,7 @@ int for_launches(const hgq_adamw_item *items, int count, F fn) {
             if (s.n == 0) continue;
             int own = 0;
             for (int k = 0; k < HGQ_SGD_SIDES; ++k) own += s.side[k] != nullptr;
-            const uint64_t own_chunks = ((uint64_t)s.n + ADAMW_CHUNK - 1) / ADAMW_CHUNK;
+            const uint64_t own_chunks = ((uint64_t)s.n + chunk - 1) / chunk;
             if (pieces + own > ADAMW_PIECES || (n > 0 && chunks + own_chunks > 0x7fffffffu)) break;
             AdamwItem &d = a.item[n];
             d.w = s.w, d.g = s.g, d.m = s.m, d.v = s.v, d.m_scale = s.m_scale, d.v_scale = s.v_scale, d.n = s.n, d.first = s.first;
@@ -393,8 +423,6 @@ int check_items(const char *what, const hgq_adamw_item *items, int count, int bi
     return HGQ_OK;
 }
 
-constexpr int NORM_GRID = 512;
-
 int norm_grid(const AdamwLaunch &a, int n) {
     const uint32_t chunks = n ? a.start[n] : 0;
     return (int)(chunks < NORM_GRID ? chunks : NORM_GRID);
@@ -405,7 +433,8 @@ int norm_grid(const AdamwLaunch &a, int n) {
 extern "C" int64_t hgq_global_norm_parts(const hgq_adamw_item *items, int count) {
     if (check_items("hgq_global_norm_parts", items, count, 0)) return -1;
     int64_t parts = 0;
-    for_launches(items, count, [&](const AdamwLaunch &a, int n, bool) {
+    const int chunk = NORM_LOADS * 1024;
+    for_launches(items, count, chunk, [&](const AdamwLaunch &a, int n, bool) {
         parts += norm_grid(a, n);
         return HGQ_OK;
     });
@@ -416,11 +445,12 @@ extern "C" int hgq_global_norm(const hgq_adamw_item *items, int count, double *p
     int rc = check_items("hgq_global_norm", items, count, 0);
     if (rc) return rc;
     int64_t at = 0;
-    rc = for_launches(items, count, [&](const AdamwLaunch &a, int n, bool) {
+    const int chunk = NORM_LOADS * 1024;
+    rc = for_launches(items, count, chunk, [&](const AdamwLaunch &a, int n, bool) {
         const int grid = norm_grid(a, n);
         if (!grid) return HGQ_OK;
         if (!parts) return fail(HGQ_ERR_ARG, "hgq_global_norm: null workspace");
-        hipLaunchKernelGGL(norm_parts_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a, n, parts + at);
+        hipLaunchKernelGGL(norm_parts_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a, n, chunk, parts + at);
         at += grid;
         return check_launch("hgq_global_norm");
     });
@@ -446,7 +476,7 @@ extern "C" int hgq_adamw_update_multi(const hgq_adamw_item *items, int count, in
     sum.n = n_terms, sum.out = sum_out;
     for (int t = 0; t < n_terms; ++t)
         if (!(sum.term[t] = terms[t])) return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: null term %d", t);
-    return for_launches(items, count, [&](const AdamwLaunch &a, int n, bool last) {
+    return for_launches(items, count, ADAMW_CHUNK, [&](const AdamwLaunch &a, int n, bool last) {
         const uint32_t chunks = n ? a.start[n] : 0;
         const int grid = chunks < 1 ? 1 : chunks < ADAMW_GRID ? (int)chunks : ADAMW_GRID;  // (no element at all: the step still counts)
         auto kernel = state_bits == 8 ? adamw_kernel<8> : adamw_kernel<32>;

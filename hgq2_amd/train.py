@@ -150,7 +150,7 @@ class AdamW(SGD):
     The number of steps and the learning rate live in device memory: a step recorded in a HIP graph (:class:`GraphedTrainStep`)
     counts on at every replay, and setting ``lr`` between replays takes effect in the next one.  The moments of all variables lie in
     one buffer each (``momentum`` and ``velocity``, or ``momentum``, ``momentum_scale``, ``velocity_root`` and ``velocity_scale``), every
-    variable at a multiple of 256 elements.  Variables must stay contiguous, on their device, and of their size and type."""
+    variable at a multiple of 256 elements (``offsets``).  Variables must stay contiguous, on their device, and of their size and type."""
 
     def __init__(self, params, lr: float = 0.001, weight_decay: float = 0.004, beta_1: float = 0.9, beta_2: float = 0.999,
                  epsilon: float = 1e-7, global_clipnorm: float | None = None, state_bits: int = 32, seed: int = 0,
@@ -178,20 +178,40 @@ class AdamW(SGD):
         self.epsilon, self.global_clipnorm = float(epsilon), None if global_clipnorm is None else float(global_clipnorm)
         self.state_bits, self.seed = int(state_bits), int(seed) & (2**63 - 1)
         self._no_decay = set()
-        self._numel, self._at, n = [p.numel() for p in self.params], [], 0
-        for k in self._numel:
-            self._at.append(n)
-            n += -(-k // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
-        moments = ops.adamw_moments(n, self.device, self.state_bits)
+        self._layout, self.offsets, n = [], [], 0  # where each variable's moments begin
+        for p in self.params:
+            self._layout.append((p, p.numel(), p.nbytes, p.dtype))
+            self.offsets.append(n)
+            n += -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
+        self._moments = ops.adamw_moments(n, self.device, self.state_bits)
         if self.state_bits == 32:
             self._names = ('momentum', 'velocity')
         else:
             self._names = ('momentum', 'momentum_scale', 'velocity_root', 'velocity_scale')
-        for name, t in zip(self._names, moments):
-            setattr(self, name, t)
+        # the variables' descriptors (hgq_adamw_item): moments, place and type now, the other words at every step
+        words, mom = [], [t.data_ptr() for t in self._moments]
+        for (p, _, _, dtype), at in zip(self._layout, self.offsets):
+            if self.state_bits == 32:
+                m = (mom[0] + 4 * at, mom[1] + 4 * at, 0, 0)
+            else:
+                m = (mom[0] + at, mom[2] + at, mom[1] + at // ops.ADAMW_BLOCK, mom[3] + at // ops.ADAMW_BLOCK)
+            words += (0, 0, *m, 0, at, 0, 0, ops._TYPE_CODES[dtype], *ops._NO_SIDES)
+        self._items = array('q', words)
         self.grad_norm = torch.zeros((), dtype=torch.float32, device=self.device) if self.global_clipnorm is not None else None
         self._state = ops.adamw_state(self.device, lr, 0, self.beta_1, self.beta_2)
         self.lr = lr
+
+    # ---- the moments, all variables' in one buffer each
+    def _moment(self, name):
+        if name not in self._names:
+            raise AttributeError(f'moments with {self.state_bits} bits have no {name}')
+        return self._moments[self._names.index(name)]
+
+    momentum = property(lambda self: self._moment('momentum'))
+    velocity = property(lambda self: self._moment('velocity'))
+    momentum_scale = property(lambda self: self._moment('momentum_scale'))
+    velocity_root = property(lambda self: self._moment('velocity_root'))
+    velocity_scale = property(lambda self: self._moment('velocity_scale'))
 
     # ---- learning rate and step number: in device memory, where a recorded step reads them
     @property
@@ -245,54 +265,60 @@ class AdamW(SGD):
     @torch.no_grad()
     def step(self):
         sums = ops.join_side(hand_over_sums=True)  # the loss terms' sum rides along with the update launch
-        words, held, post = [], [], []
+        items, held, post = self._items, [], []
         dev, inf = self.device, float('inf')
-        mom = [getattr(self, k).data_ptr() for k in self._names]
-        wide = self.state_bits == 32
+        index, fold, no_decay, decays = dev.index, self.fold_regularizers, self._no_decay, self.weight_decay
+        plain = ops._adamw_limits_words(0.0, -inf, inf, decays)
         count = 0
-        for p, n, at in zip(self.params, self._numel, self._at):
-            g = p.grad
-            side = getattr(p, '_hgq_side', None)
-            if (g is None and not side) or n == 0:
+        # (the host's share of a small step: a variable is asked for each thing once, its own attributes come from one dictionary, and
+        # only the words of its descriptor that can change are written)
+        for at, (p, n, size, dtype) in enumerate(self._layout):
+            at *= ops._ADAMW_WORDS
+            g, extra = p.grad, p.__dict__
+            side = extra.get('_hgq_side')
+            if n == 0 or (g is None and not side):
+                items[at + 6] = 0  # (an item without elements is passed over)
                 continue
-            ops._check_gradient('variable', p, dev, p.dtype, n)
-            if not p.is_contiguous():
-                raise ValueError('variables must be contiguous')
+            if p.get_device() != index or p.dtype is not dtype or p.nbytes != size or not p.is_contiguous():
+                raise ValueError(f'variables must stay contiguous, on {dev}, and of their size and type')
+            gradient = 0
             if g is not None:
-                ops._check_gradient('gradient', g, dev, p.dtype, n)
+                if g.get_device() != index or g.dtype is not dtype or g.nbytes != size or g.layout is not torch.strided:
+                    ops._check_gradient('gradient', g, dev, dtype, n)
                 if not g.is_contiguous():
                     g = g.contiguous()
                     held.append(g)
+                gradient = g.data_ptr()
+            items[at], items[at + 1], items[at + 6] = p.data_ptr(), gradient, n
+            c, r = extra.get('constraint'), extra.get('regularizer')
+            if c is None and r is None and not no_decay:
+                bounds = plain
+            else:
+                lo, hi = -inf, inf
+                if c is not None:
+                    clip = c.bounds()
+                    if clip is None:  # a constraint that is not a clip: applied after the update
+                        post.append((p, c))
+                    else:
+                        lo, hi = clip
+                l1 = r.l1 if (fold and isinstance(r, MonoL1)) else 0.0
+                bounds = ops._adamw_limits_words(l1, lo, hi, 0.0 if id(p) in no_decay else decays)
+            items[at + 8], items[at + 9] = bounds
             if side:
                 side = list(side)
                 while len(side) > ops.SGD_SIDES:  # more pieces than the kernel takes: fold the surplus into one
                     (s1, d1), (s2, d2) = side.pop(), side.pop()
                     side.append((None, (d1 if s1 is None else s1 * d1) + (d2 if s2 is None else s2 * d2)))
-            c = getattr(p, 'constraint', None)
-            r = getattr(p, 'regularizer', None)
-            lo, hi = -inf, inf
-            if c is not None:
-                bounds = c.bounds()
-                if bounds is None:  # a constraint that is not a clip: applied after the update
-                    post.append((p, c))
-                else:
-                    lo, hi = bounds
-            l1 = r.l1 if (self.fold_regularizers and isinstance(r, MonoL1)) else 0.0
-            decay = 0.0 if id(p) in self._no_decay else self.weight_decay
-            if wide:
-                m = (mom[0] + 4 * at, mom[1] + 4 * at, 0, 0)
-            else:
-                b = at // ops.ADAMW_BLOCK
-                m = (mom[0] + at, mom[2] + at, mom[1] + b, mom[3] + b)
-            words += (p.data_ptr(), g.data_ptr() if g is not None else 0, *m, n, at, *ops._adamw_limits_words(l1, lo, hi, decay),
-                      ops._TYPE_CODES[p.dtype], *(ops._side_words(side, dev, n, held) if side else ops._NO_SIDES))
+                items[at + 11:at + 19] = array('q', ops._side_words(side, dev, n, held))
+            elif items[at + 11]:
+                items[at + 11:at + 19] = array('q', ops._NO_SIDES)
             count += 1
         ride = sums.pop(0) if (count and sums) else (None, None)
         for terms, out in sums:
             ops.sum_scalars_into(terms, out)
         if count:
             ops.touch_state()  # written through pointers: the version counters do not move
-            ops._adamw_launch(array('q', words), count, self.state_bits, self._state, self.beta_1, self.beta_2, self.epsilon, self.global_clipnorm,
+            ops._adamw_launch(items, len(self._layout), self.state_bits, self._state, self.beta_1, self.beta_2, self.epsilon, self.global_clipnorm,
                               self.grad_norm, self.seed, ride[0], ride[1])
         for p, c in post:
             p.copy_(c(p))

@@ -138,7 +138,7 @@ def test_two_steps_against_64_bits(dev, sizes, odd, clip, dtype, bits):
         if clip is not None:
             assert abs(float(opt.grad_norm) - total) <= 2 * U * total
         for k, (p, w0) in enumerate(zip(params, old)):
-            n, at = p.numel(), opt._at[k]
+            n, at = p.numel(), opt.offsets[k]
             if not n:
                 continue
             part = slice(at, at + n)
