@@ -13,7 +13,6 @@ struct GroupShape {
     int64_t B, S;
     int C, G, D;
     float eps;
-    int act;
 };
 
 template <typename T>
@@ -31,18 +30,23 @@ __device__ __forceinline__ float to_f32<__bf16>(__bf16 v) {
     return (float)v;
 }
 
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == HGQ_ACT_RELU) return z > 0.0f || z != z ? z : 0.0f;
-    if (act == HGQ_ACT_SILU) return z / (1.0f + expf(-z));
+// 1 / (1 + exp(-z)).  The product z / ln 2 is off by half a unit, so exp(-z) relatively by |z| 2^-24; 1 / inf = 0 where it overflows.
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269502f)); }
+
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if (ACT == HGQ_ACT_RELU) return z > 0.0f || z != z ? z : 0.0f;
+    if (ACT == HGQ_ACT_SILU) return z * sigmoid(z);
     return z;
 }
 
 // dy act'(z)
-__device__ __forceinline__ float through_activation(float dy, float z, int act) {
-    if (act == HGQ_ACT_RELU) return z > 0.0f ? dy : z != z ? z : 0.0f;
-    if (act == HGQ_ACT_SILU) {
-        const float p = 1.0f / (1.0f + expf(-z));
-        return dy * (p * (1.0f + z * (1.0f - p)));
+template <int ACT>
+__device__ __forceinline__ float through_activation(float dy, float z) {
+    if (ACT == HGQ_ACT_RELU) return z > 0.0f ? dy : z != z ? z : 0.0f;
+    if (ACT == HGQ_ACT_SILU) {
+        const float p = sigmoid(z);
+        return dy * (p * fmaf(z, 1.0f - p, 1.0f));
     }
     return dy;
 }
@@ -60,7 +64,7 @@ __device__ __forceinline__ double group_sum(double v, double *lds) {
 }
 
 // One workgroup per sample and group, any shape: the group is read three times, its sums are formed in fp64.
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void group_norm_fwd_any(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
                                                           T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, GroupShape s) {
     __shared__ double lds[4];
@@ -81,12 +85,12 @@ __global__ __launch_bounds__(256) void group_norm_fwd_any(const T *__restrict__ 
         const int c = g * s.D + (int)(e % s.D);
         const int64_t at = base + e / s.D * s.C + e % s.D;
         const float z = (to_f32(x[at]) - mean) * rstd * (gamma ? gamma[c] : 1.0f) + (beta ? beta[c] : 0.0f);
-        y[at] = (T)activate(z, s.act);
+        y[at] = (T)activate<ACT>(z);
     }
 }
 
 // One workgroup per sample and group, any shape.  part [B][2 C]: each sample's terms of dgamma, then of dbeta.
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ gamma,
                                                           const float *__restrict__ beta, const float *__restrict__ mean_in,
                                                           const float *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ part, GroupShape s) {
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ 
             for (int64_t p = py; p < s.S; p += ty) {
                 const int64_t at = base + p * s.C + d;
                 const float xh = (to_f32(x[at]) - mean) * rstd;
-                const float dz = through_activation(to_f32(dy[at]), xh * ga + be, s.act);
+                const float dz = through_activation<ACT>(to_f32(dy[at]), xh * ga + be);
                 a += dz, h += (double)dz * xh;
             }
         s1 += a * ga, s2 += h * ga;
@@ -126,9 +130,382 @@ __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ 
         const int c = g * s.D + (int)(e % s.D);
         const int64_t at = base + e / s.D * s.C + e % s.D;
         const float ga = gamma ? gamma[c] : 1.0f, xh = (to_f32(x[at]) - mean) * rstd;
-        const float dz = through_activation(to_f32(dy[at]), xh * ga + (beta ? beta[c] : 0.0f), s.act);
+        const float dz = through_activation<ACT>(to_f32(dy[at]), xh * ga + (beta ? beta[c] : 0.0f));
         dx[at] = (T)((dz * ga - m1 - xh * m2) * rstd);
     }
+}
+
+
+// ---- tiles held in registers -----------------------------------------------------------------------------------------
+// A workgroup holds a tile - the positions (or a run of them) of K whole groups of one sample, or of several small samples - in
+// registers, four neighbours per access, so x (and dy) are read once and the variance is formed about the mean in a second
+// pass over registers.  A thread keeps its four columns in all its rows, and with them its scales and its sums per channel.
+// Rows: positions (K < G: rows of C channels of which K D are the tile's); with all groups, q = 4 / gcd(C, 4) positions are one
+// row, so rows are whole accesses for every C; the last row may be short.  A sample that is too long for one tile is cut into
+// `splits` runs of rows: one launch leaves their sums, the next one joins them and applies them.
+struct GroupTile {
+    int64_t B;
+    int n, C, G, D, K, stride;       // n: elements of a sample; stride: of a row
+    int fold;                        // positions per row
+    int TX, TY, NS;                  // threads across a row; rows of a sample side by side; samples
+    int rows, split_rows, splits;    // rows of a sample; of a split
+    int chunks, tiles;               // G / K; runs of rows (or sets of samples) of all samples
+    int team;                        // threads that add up a group's sums
+    float eps, inv;                  // 1 / elements of a group
+};
+
+// four neighbours as they lie in memory: sizeof(T) words
+template <typename T>
+struct Four {
+    typedef uint32_t words __attribute__((ext_vector_type(sizeof(T))));
+    words w;
+
+    __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(&w, p, sizeof(w)); }  // (rows of any width: aligned to an element only)
+    __device__ __forceinline__ void store(T *p) const { __builtin_memcpy(p, &w, sizeof(w)); }
+    __device__ __forceinline__ float get(int j) const {
+        T v[4];
+        __builtin_memcpy(v, &w, sizeof(w));
+        return to_f32(v[j]);
+    }
+    __device__ __forceinline__ void set(const float (&f)[4]) {
+        T v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (T)f[j];
+        __builtin_memcpy(&w, v, sizeof(w));
+    }
+    // What is cheap to form again is not carried in registers from one pass over the tile to the next: the compiler forgets what it knows.
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(w)); }
+};
+
+// where a thread works: its sample in the tile, row and columns
+struct GroupThread {
+    int s, ty, col;
+    bool on;
+    __device__ __forceinline__ explicit GroupThread(const GroupTile &p) {
+        const int tx = threadIdx.x % p.TX, rr = threadIdx.x / p.TX;
+        s = rr / p.TY, ty = rr - s * p.TY, col = tx * 4, on = s < p.NS;
+    }
+};
+
+// A thread's accesses of a run of rows [r0, r1): `full` whole ones from element `at` of the sample on, `step` apart, then `rest` elements
+struct GroupRows {
+    int full, rest, at, step;
+    __device__ __forceinline__ GroupRows(const GroupTile &p, const GroupThread &t, bool on, int c0, int r0, int r1) {
+        const int r = r0 + t.ty, rows = on && r < r1 ? (r1 - r + p.TY - 1) / p.TY : 0;
+        at = r * p.stride + c0, step = p.TY * p.stride, full = rows, rest = 0;
+        if (rows > 0) {
+            const int behind = at + (rows - 1) * step + 4 - p.n;  // (only a sample's last row is short)
+            if (behind > 0) full = rows - 1, rest = behind < 4 ? 4 - behind : 0;
+        }
+    }
+};
+
+// Sums of one value per column (v[4] of each thread) over the rows and the columns of every group in the tile: total[NS * K] in LDS, to
+// all threads, in a fixed order.  ONE: a thread's columns are of one group, and it adds them first.  red: blockDim.x * (ONE ? 1 : 4).
+template <bool ONE>
+__device__ __forceinline__ void sum_groups(const GroupTile &p, const GroupThread &t, const float (&v)[4], float *red, float *total) {
+    if (t.on) {
+        if (ONE) {
+            red[threadIdx.x] = (v[0] + v[1]) + (v[2] + v[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) red[threadIdx.x * 4 + j] = v[j];
+        }
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & (p.team - 1);
+    const int across = ONE ? p.D / 4 : p.D, width = ONE ? p.TX : p.TX * 4, cols = ONE ? across : across * p.fold;
+    const int r0 = lane / cols, first = lane - r0 * cols, step = p.team / cols, rest = p.team - step * cols;
+    for (int g = threadIdx.x / p.team; g < p.NS * p.K; g += blockDim.x / p.team) {
+        const float *mine = red + (g / p.K) * p.TY * width + (g % p.K) * across;
+        float sum = 0;
+        for (int r = r0, c = first; r < p.TY;) {
+            const int f = !ONE && p.fold > 1 ? c / across : 0;
+            sum += mine[r * width + f * p.C + (c - f * across)];
+            r += step, c += rest;
+            if (c >= cols) c -= cols, ++r;
+        }
+        for (int d = p.team / 2; d; d >>= 1) sum += __shfl_xor(sum, d);
+        if (lane == 0) total[g] = sum;
+    }
+    __syncthreads();
+}
+
+// the group of a thread's column j within the tile
+template <bool ONE>
+__device__ __forceinline__ int group_of(const GroupTile &p, const GroupThread &t, int j) {
+    const int c = t.col + (ONE ? 0 : j);
+    return t.s * p.K + (!ONE && p.fold > 1 ? c % p.C : c) / p.D;
+}
+
+// phase 0: whole tiles; 1: mean and sum of squares about it of every split, parts [B][splits][G][2]; 2: join those, apply
+template <typename T, int ACT, bool ONE, int NV>
+__global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                            T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out,
+                                                            float *__restrict__ parts, GroupTile p, int phase) {
+    extern __shared__ float lds[];
+    const int groups = p.NS * p.K;
+    float *total = lds, *stat = lds + groups, *red = lds + 2 * groups;
+    const GroupThread t(p);
+    // the chunks of one sample share cache lines: their workgroups follow each other on one of the eight dies (blocks go round them)
+    const int64_t blk = blockIdx.x;
+    const int64_t z = blk / (8 * p.chunks) * 8 + blk % 8;
+    const int chunk = (int)(blk / 8 % p.chunks);
+    if (z >= p.tiles) return;
+    const int split = (int)(z % p.splits);
+    const int64_t b = z / p.splits * p.NS + t.s;
+    const bool on = t.on && b < p.B;
+    const int c0 = chunk * p.K * p.D + t.col;  // (with fold: the column in the row)
+    const int r0 = split * p.split_rows, r1 = min(p.rows, r0 + p.split_rows);
+    const T *xs = x + b * p.n;
+    const GroupRows rows(p, t, on, c0, r0, r1);
+    Four<T> v[NV];
+    float last[3] = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i < rows.full) v[i].load(xs + rows.at + i * rows.step);
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+        if (j < rows.rest) last[j] = to_f32(xs[rows.at + rows.full * rows.step + j]);
+    constexpr int N = ONE ? 1 : 4;  // means of a thread's columns
+    float mean[N], rstd[N];
+    if (phase < 2) {
+        float acc[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < rows.full)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] += v[i].get(j);
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < rows.rest) acc[j] += last[j];
+        sum_groups<ONE>(p, t, acc, red, total);
+        // elements of a group in this tile
+        const float inv = p.splits == 1 ? p.inv : 1.0f / (float)((min(p.n / p.C, r1 * p.fold) - r0 * p.fold) * p.D);
+#pragma unroll
+        for (int j = 0; j < N; ++j) mean[j] = t.on ? total[group_of<ONE>(p, t, j)] * inv : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < rows.full) {
+                v[i].forget();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float d = v[i].get(j) - mean[j % N];
+                    acc[j] = fmaf(d, d, acc[j]);
+                }
+            }
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < rows.rest) {
+                const float d = last[j] - mean[j % N];
+                acc[j] = fmaf(d, d, acc[j]);
+            }
+        sum_groups<ONE>(p, t, acc, red, stat);
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+            const int64_t bg = z / p.splits * p.NS + g / p.K;
+            if (bg >= p.B) break;
+            const int64_t at = bg * p.G + chunk * p.K + g % p.K;
+            if (phase == 1) {
+                float *out = parts + ((bg * p.splits + split) * p.G + chunk * p.K + g % p.K) * 2;
+                out[0] = total[g] * inv, out[1] = stat[g];
+            } else {
+                mean_out[at] = total[g] * inv, rstd_out[at] = 1.0f / sqrtf(stat[g] * p.inv + p.eps);
+            }
+        }
+        if (phase == 1) return;
+#pragma unroll
+        for (int j = 0; j < N; ++j) rstd[j] = t.on ? 1.0f / sqrtf(stat[group_of<ONE>(p, t, j)] * p.inv + p.eps) : 0.0f;
+    } else {
+        // the splits' means about the first one's, and their squares about the joint mean
+        const int lane = threadIdx.x & (p.team - 1);
+        for (int g = threadIdx.x / p.team; g < groups; g += blockDim.x / p.team) {
+            const float *in = parts + (b - t.s) * p.splits * p.G * 2 + (chunk * p.K + g) * 2;  // (one sample: NS = 1)
+            const float first = in[0];
+            float m = 0, q = 0;
+            for (int k = lane; k < p.splits; k += p.team) {
+                const float w = (float)((min(p.n / p.C, (k + 1) * p.split_rows * p.fold) - k * p.split_rows * p.fold) * p.D) * p.inv;
+                m += w * (in[(int64_t)k * p.G * 2] - first);
+            }
+            for (int d = p.team / 2; d; d >>= 1) m += __shfl_xor(m, d);
+            for (int k = lane; k < p.splits; k += p.team) {
+                const float w = (float)((min(p.n / p.C, (k + 1) * p.split_rows * p.fold) - k * p.split_rows * p.fold) * p.D) * p.inv;
+                const float d = in[(int64_t)k * p.G * 2] - first - m;
+                q += in[(int64_t)k * p.G * 2 + 1] * p.inv + w * d * d;
+            }
+            for (int d = p.team / 2; d; d >>= 1) q += __shfl_xor(q, d);
+            if (lane == 0) {
+                total[g] = first + m, stat[g] = 1.0f / sqrtf(q + p.eps);
+                if (split == 0) mean_out[(b - t.s) * p.G + chunk * p.K + g] = total[g], rstd_out[(b - t.s) * p.G + chunk * p.K + g] = stat[g];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < N; ++j) mean[j] = t.on ? total[group_of<ONE>(p, t, j)] : 0.0f, rstd[j] = t.on ? stat[group_of<ONE>(p, t, j)] : 0.0f;
+    }
+    if (!on) return;
+    float scale[4], be[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int c = p.fold > 1 ? (c0 + j) % p.C : c0 + j;
+        scale[j] = rstd[j % N] * (gamma ? gamma[c] : 1.0f), be[j] = beta ? beta[c] : 0.0f;
+    }
+    T *ys = y + b * p.n;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i < rows.full) {
+            v[i].forget();
+            float out[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[j] = activate<ACT>(fmaf(v[i].get(j) - mean[j % N], scale[j], be[j]));
+            v[i].set(out);
+            v[i].store(ys + rows.at + i * rows.step);
+        }
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+        if (j < rows.rest) ys[rows.at + rows.full * rows.step + j] = (T)activate<ACT>(fmaf(last[j] - mean[j % N], scale[j], be[j]));
+}
+
+// phase 0: whole tiles; 1: sums of d rstd and d xhat rstd of every split, parts [B][splits][G][2], and the channels' sums; 2: join them, dx.
+// Every tile leaves its terms of dgamma and dbeta, slices [tiles][2 C] (NULL: not wanted).
+template <typename T, int ACT, bool ONE, int NV>
+__global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ gamma,
+                                                            const float *__restrict__ beta, const float *__restrict__ mean_in,
+                                                            const float *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ slices,
+                                                            float *__restrict__ parts, GroupTile p, int phase) {
+    extern __shared__ float lds[];
+    const int groups = p.NS * p.K;
+    float *total = lds, *stat = lds + groups, *red = lds + 2 * groups;
+    const GroupThread t(p);
+    const int64_t blk = blockIdx.x;
+    const int64_t z = blk / (8 * p.chunks) * 8 + blk % 8;
+    const int chunk = (int)(blk / 8 % p.chunks);
+    if (z >= p.tiles) return;
+    const int c0 = chunk * p.K * p.D + t.col;
+    const int split = (int)(z % p.splits);
+    const int64_t b = z / p.splits * p.NS + t.s;
+    const bool on = t.on && b < p.B;
+    const int r0 = split * p.split_rows, r1 = min(p.rows, r0 + p.split_rows);
+    const T *xs = x + b * p.n, *ds = dy + b * p.n;
+    const GroupRows rows(p, t, on, c0, r0, r1);
+    Four<T> v[NV], w[NV];
+    float last[3] = {0, 0, 0}, dlast[3] = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i < rows.full) v[i].load(xs + rows.at + i * rows.step), w[i].load(ds + rows.at + i * rows.step);
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+        if (j < rows.rest) last[j] = to_f32(xs[rows.at + rows.full * rows.step + j]), dlast[j] = to_f32(ds[rows.at + rows.full * rows.step + j]);
+    constexpr int N = ONE ? 1 : 4;  // groups of a thread's columns
+    float mean[N], rstd[N], scale[4], be[4];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int64_t g = b * p.G + chunk * p.K + group_of<ONE>(p, t, j) - t.s * p.K;
+        mean[j] = on ? mean_in[g] : 0.0f, rstd[j] = on ? rstd_in[g] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int c = p.fold > 1 ? (c0 + j) % p.C : c0 + j;
+        scale[j] = rstd[j % N] * (t.on && gamma ? gamma[c] : 1.0f), be[j] = t.on && beta ? beta[c] : 0.0f;
+    }
+    float h[4] = {0, 0, 0, 0}, a[4] = {0, 0, 0, 0};  // of dz (x - mean) and of dz
+    if (phase < 2) {
+        float mine[2][4];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < rows.full)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float d = v[i].get(j) - mean[j % N], dz = through_activation<ACT>(w[i].get(j), fmaf(d, scale[j], be[j]));
+                    a[j] += dz, h[j] = fmaf(dz, d, h[j]);
+                }
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < rows.rest) {
+                const float d = last[j] - mean[j % N], dz = through_activation<ACT>(dlast[j], fmaf(d, scale[j], be[j]));
+                a[j] += dz, h[j] = fmaf(dz, d, h[j]);
+            }
+        // sums of d rstd and of d xhat rstd: gamma rstd is what is at hand
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] *= rstd[j % N], mine[0][j] = a[j] * scale[j], mine[1][j] = h[j] * scale[j];
+        if (phase == 1 || dx) {
+            sum_groups<ONE>(p, t, mine[0], red, total);
+            sum_groups<ONE>(p, t, mine[1], red, stat);
+        }
+        if (phase == 1) {
+            for (int g = threadIdx.x; g < groups; g += blockDim.x) {  // (one sample: NS = 1)
+                float *out = parts + (((b - t.s) * p.splits + split) * p.G + chunk * p.K + g) * 2;
+                out[0] = total[g], out[1] = stat[g];
+            }
+        }
+    } else {
+        const int lane = threadIdx.x & (p.team - 1);
+        for (int g = threadIdx.x / p.team; g < groups; g += blockDim.x / p.team) {
+            const float *in = parts + (b - t.s) * p.splits * p.G * 2 + (chunk * p.K + g) * 2;
+            float m1 = 0, m2 = 0;
+            for (int k = lane; k < p.splits; k += p.team) m1 += in[(int64_t)k * p.G * 2], m2 += in[(int64_t)k * p.G * 2 + 1];
+            for (int d = p.team / 2; d; d >>= 1) m1 += __shfl_xor(m1, d), m2 += __shfl_xor(m2, d);
+            if (lane == 0) total[g] = m1, stat[g] = m2;
+        }
+        __syncthreads();
+    }
+    if (phase != 1 && dx && on) {
+        // dx = dz gamma rstd - mean(d) rstd - (x - mean) rstd mean(d xhat) rstd
+        float m1[N], m2[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) m1[j] = -total[group_of<ONE>(p, t, j)] * p.inv, m2[j] = -stat[group_of<ONE>(p, t, j)] * p.inv * rstd[j];
+        T *out = dx + b * p.n;
+        auto one = [&](float xv, float dv, int j) {
+            const float d = xv - mean[j % N], dz = through_activation<ACT>(dv, fmaf(d, scale[j], be[j]));
+            return fmaf(dz, scale[j], fmaf(d, m2[j % N], m1[j % N]));
+        };
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < rows.full) {
+                v[i].forget(), w[i].forget();
+                float o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = one(v[i].get(j), w[i].get(j), j);
+                v[i].set(o);
+                v[i].store(out + rows.at + i * rows.step);
+            }
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < rows.rest) out[rows.at + rows.full * rows.step + j] = (T)one(last[j], dlast[j], j);
+    }
+    if (!slices || phase == 2) return;
+    // this tile's sums per channel: over its rows and samples, the folded positions with them
+    const int width = p.TX * 4, cols = p.K * p.D, folds = p.fold == 4 ? 2 : p.fold - 1, count = (p.NS * p.TY) << folds;  // (fold = 1, 2 or 4)
+    int team = 1;
+    while (team < 64 && team * 2 * cols <= (int)blockDim.x) team *= 2;
+    const int lane = threadIdx.x & (team - 1);
+    for (int k = 0; k < 2; ++k) {
+        if (t.on)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) red[threadIdx.x * 4 + j] = k ? a[j] : h[j];
+        __syncthreads();
+        for (int c = threadIdx.x / team; c < cols; c += blockDim.x / team) {
+            float sum = 0;
+            for (int e = lane; e < count; e += team) sum += red[(e >> folds) * width + (e & (p.fold - 1)) * p.C + c];
+            for (int d = team / 2; d; d >>= 1) sum += __shfl_xor(sum, d);
+            if (lane == 0) slices[z * 2 * p.C + k * p.C + chunk * cols + c] = sum;
+        }
+        __syncthreads();
+    }
+}
+
+// Adds up runs of SLICE_RUN slices of M entries: where a batch leaves more slices than the last reduction takes well
+constexpr int SLICE_RUN = 64;
+__global__ __launch_bounds__(64) void group_norm_join_slices(const float *__restrict__ slices, int64_t n, int64_t M, float *__restrict__ out) {
+    const int64_t e = (int64_t)blockIdx.x * 64 + threadIdx.x, first = (int64_t)blockIdx.y * SLICE_RUN;
+    if (e >= M) return;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int64_t k = first; k < first + SLICE_RUN && k < n; k += 8)
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (k + u < n) v[u] += slices[(k + u) * M + e];
+    out[blockIdx.y * M + e] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
 }
 
 }  // namespace hgq
@@ -146,31 +523,166 @@ int check_shape(const char *what, int64_t B, int64_t S, int C, int G, int act, i
     return HGQ_OK;
 }
 
+constexpr int GROUP_THREADS = 1024;  // most threads of a workgroup
+constexpr int64_t MOST_SLICES = 2048;
+
+// accesses of four that a thread can hold of one tensor: 128 bytes
 template <typename T>
-int fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, const GroupShape &s, hipStream_t st) {
-    hipLaunchKernelGGL(group_norm_fwd_any<T>, dim3((unsigned)(s.B * s.G)), dim3(256), 0, st, (const T *)x, gamma, beta, (T *)y, mean, rstd, s);
-    return check_launch("hgq_group_norm_fwd");
+constexpr int MOST_HELD = 32 / sizeof(T);
+int most_held(int type) { return type == HGQ_TYPE_F32 ? MOST_HELD<float> : MOST_HELD<__bf16>; }
+
+// The tile's width for K of the groups; false: it is none (more than GROUP_THREADS accesses, or not whole ones)
+bool widen(GroupTile &p, int K) {
+    p.K = K;
+    p.fold = K < p.G ? 1 : p.C % 4 == 0 ? 1 : p.C % 2 == 0 ? 2 : 4;
+    if (K < p.G && (int64_t)K * p.D % 4) return false;
+    const int64_t width = K < p.G ? (int64_t)K * p.D : (int64_t)p.fold * p.C;
+    if (width > 4 * GROUP_THREADS) return false;
+    p.TX = (int)(width / 4);
+    p.stride = K < p.G ? p.C : (int)width;
+    const int S = p.n / p.C;
+    p.rows = (S + p.fold - 1) / p.fold;
+    p.chunks = p.G / K;
+    return true;
+}
+
+// Lays out the tiles; false: the shape is left to the kernels for any shape.  held: accesses per thread (the kernel's NV).
+bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, int G, int type, bool backward) {
+    if (B == 0 || S == 0 || S > (1 << 29) / C || C > 65536) return false;  // (offsets within a sample, and a tile behind it, in 32 bits)
+    p = {};
+    p.B = B, p.n = (int)(S * C), p.C = C, p.G = G, p.D = C / G, p.inv = 1.0f / (float)(S * (C / G)), p.NS = 1;
+    const int most = most_held(type);
+    // the most groups that fit and still leave two workgroups for every compute unit; else the fewest that fit
+    int best = 0;
+    for (int K = 1; K <= G; K = K < G && (K + 1) * p.D > 4 * GROUP_THREADS ? G : K + 1) {
+        if (G % K || !widen(p, K) || p.rows > GROUP_THREADS / p.TX * most) continue;
+        if (!best || B * (G / K) >= 512) best = K;
+        if (K == G) break;
+    }
+    if (best) {
+        widen(p, best);
+        held = 4;
+        while ((p.rows + held - 1) / held * p.TX > GROUP_THREADS) held *= 2;
+        p.TY = (p.rows + held - 1) / held;
+        p.splits = 1, p.split_rows = p.rows;
+        const int one = p.TY * p.TX;  // small samples share a workgroup while there are enough of them
+        while ((p.NS + 1) * one <= 256 && B / (p.NS + 1) * p.chunks >= 512) ++p.NS;
+    } else {
+        for (int K = G; K >= 1 && !best; K = K == G && G > 4 * GROUP_THREADS / p.D + 1 ? 4 * GROUP_THREADS / p.D + 1 : K - 1)
+            if (G % K == 0 && widen(p, K)) best = K;
+        if (!best) return false;
+        held = most / 2;
+        p.TY = 512 / p.TX > 1 ? 512 / p.TX : 1;
+        p.split_rows = p.TY * held;
+        p.splits = (p.rows + p.split_rows - 1) / p.split_rows;
+    }
+    threads = (p.NS * p.TY * p.TX + 63) / 64 * 64;
+    p.team = 1;
+    while (p.team < 64 && p.team * 2 * p.NS * p.K <= threads) p.team *= 2;
+    const int64_t tiles = (B + p.NS - 1) / p.NS * p.splits;
+    if (tiles > 65535 * (int64_t)SLICE_RUN || tiles * p.chunks > 0x7fffffff / 16) return false;
+    p.tiles = (int)tiles;
+    return true;
+}
+
+// the tiles' terms of dgamma and dbeta, and runs of them added up where they are many
+int64_t slices_floats(const GroupTile &p) { return 2 * (int64_t)p.C * (p.tiles + (p.tiles > MOST_SLICES ? (p.tiles + SLICE_RUN - 1) / SLICE_RUN : 0)); }
+
+int64_t parts_floats(const GroupTile &p) { return p.splits > 1 ? p.B * p.splits * p.G * 2 : 0; }
+
+int lds_bytes(const GroupTile &p, int threads, bool backward) {
+    return 4 * (2 * p.NS * p.K + threads * (p.D % 4 == 0 && !backward ? 1 : 4));
+}
+
+unsigned blocks(const GroupTile &p) { return (unsigned)(((int64_t)p.tiles + 7) / 8 * 8 * p.chunks); }
+
+template <typename T, int ACT, bool ONE>
+auto fwd_kernel(int held) {
+    return held == 4 ? group_norm_fwd_tile<T, ACT, ONE, 4> : held == 8 ? group_norm_fwd_tile<T, ACT, ONE, 8> : group_norm_fwd_tile<T, ACT, ONE, MOST_HELD<T>>;
+}
+
+template <typename T, int ACT, bool ONE>
+auto bwd_kernel(int held) {
+    return held == 4 ? group_norm_bwd_tile<T, ACT, ONE, 4> : held == 8 ? group_norm_bwd_tile<T, ACT, ONE, 8> : group_norm_bwd_tile<T, ACT, ONE, MOST_HELD<T>>;
+}
+
+template <typename T, int ACT>
+int fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, float *ws, const GroupShape &s, int type,
+        hipStream_t st) {
+    GroupTile p;
+    int held, threads;
+    if (!plan(p, held, threads, s.B, s.S, s.C, s.G, type, false)) {
+        hipLaunchKernelGGL((group_norm_fwd_any<T, ACT>), dim3((unsigned)(s.B * s.G)), dim3(256), 0, st, (const T *)x, gamma, beta, (T *)y, mean, rstd, s);
+        return check_launch("hgq_group_norm_fwd");
+    }
+    p.eps = s.eps;
+    if (p.splits > 1 && !ws) return fail(HGQ_ERR_ARG, "hgq_group_norm_fwd: null workspace");
+    auto kernel = p.D % 4 == 0 ? fwd_kernel<T, ACT, true>(held) : fwd_kernel<T, ACT, false>(held);
+    for (int phase = p.splits > 1 ? 1 : 0; phase < (p.splits > 1 ? 3 : 1); ++phase) {
+        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, false), st, (const T *)x, gamma, beta, (T *)y, mean, rstd, ws, p, phase);
+        const int rc = check_launch("hgq_group_norm_fwd");
+        if (rc) return rc;
+    }
+    return HGQ_OK;
+}
+
+template <typename T, int ACT>
+int bwd(const void *dy, const void *x, const float *gamma, const float *beta, const float *mean, const float *rstd, void *dx, float *dgamma,
+        float *dbeta, float *ws, const GroupShape &s, int type, hipStream_t st) {
+    const bool sums = dgamma || dbeta;
+    GroupTile p;
+    int held, threads;
+    if (!plan(p, held, threads, s.B, s.S, s.C, s.G, type, true)) {
+        hipLaunchKernelGGL((group_norm_bwd_any<T, ACT>), dim3((unsigned)(s.B * s.G)), dim3(256), 0, st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd, (T *)dx,
+                           sums ? ws : nullptr, s);
+        const int rc = check_launch("hgq_group_norm_bwd");
+        if (rc || !sums) return rc;
+        return reduce_parts(ws, (int)s.B, 2 * (int64_t)s.C, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
+    }
+    const int64_t M = 2 * (int64_t)s.C;
+    float *slices = sums ? ws : nullptr, *parts = p.splits > 1 ? ws + slices_floats(p) : nullptr;
+    if (p.splits > 1 && !ws) return fail(HGQ_ERR_ARG, "hgq_group_norm_bwd: null workspace");
+    auto kernel = p.D % 4 == 0 ? bwd_kernel<T, ACT, true>(held) : bwd_kernel<T, ACT, false>(held);
+    for (int phase = p.splits > 1 ? 1 : 0; phase < (p.splits > 1 ? 3 : 1); ++phase) {
+        if (phase == 2 && !dx) break;
+        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, true), st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd,
+                           (T *)dx, slices, parts, p, phase);
+        const int rc = check_launch("hgq_group_norm_bwd");
+        if (rc) return rc;
+    }
+    if (!sums) return HGQ_OK;
+    if (p.tiles <= MOST_SLICES) return reduce_parts(slices, p.tiles, M, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
+    const int runs = (p.tiles + SLICE_RUN - 1) / SLICE_RUN;
+    float *joined = slices + p.tiles * M;
+    hipLaunchKernelGGL(group_norm_join_slices, dim3((unsigned)((M + 63) / 64), (unsigned)runs), dim3(64), 0, st, slices, (int64_t)p.tiles, M, joined);
+    const int rc = check_launch("hgq_group_norm_bwd");
+    return rc ? rc : reduce_parts(joined, runs, M, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
 }
 
 template <typename T>
-int bwd(const void *dy, const void *x, const float *gamma, const float *beta, const float *mean, const float *rstd, void *dx, float *dgamma,
-        float *dbeta, float *ws, const GroupShape &s, hipStream_t st) {
-    const bool sums = dgamma || dbeta;
-    hipLaunchKernelGGL(group_norm_bwd_any<T>, dim3((unsigned)(s.B * s.G)), dim3(256), 0, st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd, (T *)dx,
-                       sums ? ws : nullptr, s);
-    const int rc = check_launch("hgq_group_norm_bwd");
-    if (rc || !sums) return rc;
-    return reduce_parts(ws, (int)s.B, 2 * (int64_t)s.C, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
+auto fwd_of(int act) {
+    return act == HGQ_ACT_RELU ? fwd<T, HGQ_ACT_RELU> : act == HGQ_ACT_SILU ? fwd<T, HGQ_ACT_SILU> : fwd<T, HGQ_ACT_NONE>;
+}
+
+template <typename T>
+auto bwd_of(int act) {
+    return act == HGQ_ACT_RELU ? bwd<T, HGQ_ACT_RELU> : act == HGQ_ACT_SILU ? bwd<T, HGQ_ACT_SILU> : bwd<T, HGQ_ACT_NONE>;
 }
 
 }  // namespace
 
 extern "C" int64_t hgq_group_norm_fwd_workspace(int64_t B, int64_t S, int C, int G, int type) {
-    return check_shape("hgq_group_norm_fwd_workspace", B, S, C, G, HGQ_ACT_NONE, type) ? -1 : 0;
+    if (check_shape("hgq_group_norm_fwd_workspace", B, S, C, G, HGQ_ACT_NONE, type)) return -1;
+    GroupTile p;
+    int held, threads;
+    return plan(p, held, threads, B, S, C, G, type, false) ? parts_floats(p) : 0;
 }
 
 extern "C" int64_t hgq_group_norm_bwd_workspace(int64_t B, int64_t S, int C, int G, int type) {
-    return check_shape("hgq_group_norm_bwd_workspace", B, S, C, G, HGQ_ACT_NONE, type) ? -1 : B * 2 * C;
+    if (check_shape("hgq_group_norm_bwd_workspace", B, S, C, G, HGQ_ACT_NONE, type)) return -1;
+    GroupTile p;
+    int held, threads;
+    return plan(p, held, threads, B, S, C, G, type, true) ? slices_floats(p) + parts_floats(p) : B * 2 * C;
 }
 
 extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, float *workspace,
@@ -180,8 +692,8 @@ extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float
     if (!(eps >= 0)) return fail(HGQ_ERR_ARG, "hgq_group_norm_fwd: epsilon must not be negative");
     if (B == 0 || S == 0) return HGQ_OK;
     if (!x || !y || !mean || !rstd) return fail(HGQ_ERR_ARG, "hgq_group_norm_fwd: null pointer");
-    const GroupShape s = {B, S, C, G, C / G, eps, act};
-    return (type == HGQ_TYPE_F32 ? fwd<float> : type == HGQ_TYPE_BF16 ? fwd<__bf16> : fwd<_Float16>)(x, gamma, beta, y, mean, rstd, s, (hipStream_t)stream);
+    const GroupShape s = {B, S, C, G, C / G, eps};
+    return (type == HGQ_TYPE_F32 ? fwd_of<float>(act) : type == HGQ_TYPE_BF16 ? fwd_of<__bf16>(act) : fwd_of<_Float16>(act))(x, gamma, beta, y, mean, rstd, workspace, s, type, (hipStream_t)stream);
 }
 
 extern "C" int hgq_group_norm_bwd(const void *dy, const void *x, const float *gamma, const float *beta, const float *mean, const float *rstd,
@@ -195,7 +707,7 @@ extern "C" int hgq_group_norm_bwd(const void *dy, const void *x, const float *ga
     }
     if (!dy || !x || !mean || !rstd || ((dgamma || dbeta) && !workspace)) return fail(HGQ_ERR_ARG, "hgq_group_norm_bwd: null pointer");
     if (!dx && !dgamma && !dbeta) return HGQ_OK;
-    const GroupShape s = {B, S, C, G, C / G, 0.0f, act};
-    return (type == HGQ_TYPE_F32 ? bwd<float> : type == HGQ_TYPE_BF16 ? bwd<__bf16> : bwd<_Float16>)(dy, x, gamma, beta, mean, rstd, dx, dgamma, dbeta, workspace, s,
-                                                                                                    (hipStream_t)stream);
+    const GroupShape s = {B, S, C, G, C / G, 0.0f};
+    return (type == HGQ_TYPE_F32 ? bwd_of<float>(act) : type == HGQ_TYPE_BF16 ? bwd_of<__bf16>(act) : bwd_of<_Float16>(act))(dy, x, gamma, beta, mean, rstd, dx, dgamma, dbeta, workspace, s,
+                                                                                                    type, (hipStream_t)stream);
 }
