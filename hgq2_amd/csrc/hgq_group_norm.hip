@@ -551,28 +551,41 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     if (B == 0 || S == 0 || S > (1 << 29) / C || C > 65536) return false;  // (offsets within a sample, and a tile behind it, in 32 bits)
     p = {};
     p.B = B, p.n = (int)(S * C), p.C = C, p.G = G, p.D = C / G, p.inv = 1.0f / (float)(S * (C / G)), p.NS = 1;
-    const int most = most_held(type);
-    // the most groups that fit and still leave two workgroups for every compute unit; else the fewest that fit
+    const int most = most_held(type), size = type == HGQ_TYPE_F32 ? 4 : 2;
+    // How many groups a tile holds.  A workgroup costs about 2 us whatever it holds, so with work for every compute unit the most groups that
+    // stay under 96 KB (1024 x 26 x 26 x 32 fp32 in 8 groups, backward: 86 KB 68 us, 43 KB 74 us, 11 KB 97 us; 256 x 8 x 8 x 512: 64 KB 22 us, 4 KB 29 us).
+    // With little work the fewest groups: one sample of 28 x 28 x 32 in 8 workgroups 5.8 us, in one 7.5 us.  A tile of more than 96 KB
+    // leaves a compute unit with one workgroup that loads, waits and stores in turn, and narrow ones read parts of cache lines: the
+    // sample is cut into runs of rows and read twice (48 x 64 x 64 x 512 bfloat16: held, 32-byte rows 148 us, cut with 128-byte rows 127 us).
     int best = 0;
     for (int K = 1; K <= G; K = K < G && (K + 1) * p.D > 4 * GROUP_THREADS ? G : K + 1) {
-        if (G % K || !widen(p, K) || p.rows > GROUP_THREADS / p.TX * most) continue;
-        if (!best || B * (G / K) >= 512) best = K;
+        if (G % K || !widen(p, K)) continue;
+        if (p.rows <= GROUP_THREADS / p.TX * most && (int64_t)p.rows * p.TX * 4 * size <= 96 << 10 && (!best || B * (G / K) >= 512)) best = K;
         if (K == G) break;
     }
     if (best) {
         widen(p, best);
-        held = 4;
+        // rows per thread: many amortise what a workgroup costs (the first shape in 43 KB tiles, backward: 8 rows 74 us, 4 rows 97 us), few
+        // spread little work over more threads
+        held = B * p.chunks >= 512 ? most : 4;
         while ((p.rows + held - 1) / held * p.TX > GROUP_THREADS) held *= 2;
         p.TY = (p.rows + held - 1) / held;
         p.splits = 1, p.split_rows = p.rows;
         const int one = p.TY * p.TX;  // small samples share a workgroup while there are enough of them
         while ((p.NS + 1) * one <= 256 && B / (p.NS + 1) * p.chunks >= 512) ++p.NS;
     } else {
-        for (int K = G; K >= 1 && !best; K = K == G && G > 4 * GROUP_THREADS / p.D + 1 ? 4 * GROUP_THREADS / p.D + 1 : K - 1)
-            if (G % K == 0 && widen(p, K)) best = K;
+        // rows of 128 bytes or more, whole lines (16 x 128 x 128 x 64 fp32 in 8 groups, backward: 128 bytes 59 us, 32 bytes and less over 63 us)
+        for (int K = 1; K <= G; K = K < G && (K + 1) * p.D > 4 * GROUP_THREADS ? G : K + 1) {
+            if (G % K == 0 && widen(p, K)) {
+                best = K;
+                if (p.TX * 4 * size >= 128) break;
+            }
+            if (K == G) break;
+        }
         if (!best) return false;
-        held = most / 2;
-        p.TY = 512 / p.TX > 1 ? 512 / p.TX : 1;
+        widen(p, best);
+        held = most;
+        p.TY = 256 / p.TX > 1 ? 256 / p.TX : 1;
         p.split_rows = p.TY * held;
         p.splits = (p.rows + p.split_rows - 1) / p.split_rows;
     }
