@@ -10,6 +10,8 @@ raises.
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
 import struct
 import threading
 from array import array
@@ -3598,73 +3600,81 @@ GROUP_ACTIVATIONS = {None: _lib.ACT_NONE, 'linear': _lib.ACT_NONE, 'relu': _lib.
 
 
 def _group_shape(x: Tensor, groups: int):
-    _need(x.is_cuda, f'x must be a GPU tensor (there is no CPU implementation), got device {x.device}')
-    code = _TYPE_CODES.get(x.dtype)
-    _need(code is not None, f'x must be float32, bfloat16 or float16, got {x.dtype}')
-    _need(x.dim() >= 2 and x.shape[-1] >= 1, 'x must be [batch, ..., channels]')
-    _need(x.is_contiguous(), 'x must be contiguous')
-    B, C = x.shape[0], x.shape[-1]
-    _need(groups >= 1 and C % groups == 0, f'{C} channels do not fall into {groups} groups of one size')
-    S = 1
-    for d in x.shape[1:-1]:
-        S *= d
-    return B, S, C, code
+    code, shape = _TYPE_CODES.get(x.dtype), x.shape
+    if code is None or not x.is_cuda or len(shape) < 2 or not x.is_contiguous() or shape[-1] < 1 or groups < 1 or shape[-1] % groups:
+        # (what is wrong is put into words only here: the checks run at every call)
+        _need(x.is_cuda, f'x must be a GPU tensor (there is no CPU implementation), got device {x.device}')
+        _need(code is not None, f'x must be float32, bfloat16 or float16, got {x.dtype}')
+        _need(len(shape) >= 2 and shape[-1] >= 1, f'x must be [batch, ..., channels], got {tuple(shape)}')
+        _need(x.is_contiguous(), 'x must be contiguous')
+        raise ValueError(f'{shape[-1]} channels do not fall into {groups} groups of one size')
+    return shape[0], math.prod(shape[1:-1]), shape[-1], code
 
 
-def _channel_vector(name: str, t: Tensor, x: Tensor):
+def _channel_vector(name: str, t: Tensor, index: int, channels: int):
     """A per-channel operand, or an empty tensor in the place of none."""
-    if t.numel():
-        _need(t.device == x.device and t.dtype is _F32 and t.is_contiguous() and t.numel() == x.shape[-1],
-              f'{name} must be a contiguous float32 tensor of {x.shape[-1]} elements on {x.device}')
+    n = t.numel()
+    if n and (n != channels or t.dtype is not _F32 or t.get_device() != index or not t.is_contiguous()):
+        raise ValueError(f'{name} must be a contiguous float32 tensor of {channels} elements on the same GPU, got {t.dtype} {tuple(t.shape)} on {t.device}')
+
+
+@functools.lru_cache(4096)
+def _group_workspace(backward: bool, *shape) -> int:
+    """Workspace in floats, by the sizes alone."""
+    lib = _lib.load()
+    return (lib.hgq_group_norm_bwd_workspace if backward else lib.hgq_group_norm_fwd_workspace)(*shape)
 
 
 @torch.library.custom_op('hgq::group_norm_fwd', mutates_args=())
-def group_norm_fwd(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon: float, act: int) -> tuple[Tensor, Tensor, Tensor]:
-    """``gamma``, ``beta`` empty: none.  Returns y and, per sample and group, the mean and 1 / sqrt(var + epsilon)."""
+def group_norm_fwd(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon: float, act: int) -> tuple[Tensor, Tensor]:
+    """``gamma``, ``beta`` empty: none.  Returns y and, per sample and group, the mean and 1 / sqrt(var + epsilon) (``[2, batch, groups]``)."""
     B, S, C, code = _group_shape(x, groups)
-    _channel_vector('gamma', gamma, x), _channel_vector('beta', beta, x)
+    device = x.device
+    _channel_vector('gamma', gamma, device.index, C), _channel_vector('beta', beta, device.index, C)
     y = torch.empty_like(x)
-    stats = torch.empty(2, B, groups, dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    lib = _lib.load()
-    with _device_of(x.device) as stream:
-        need = lib.hgq_group_norm_fwd_workspace(B, S, C, groups, code)
-        ws = torch.empty(need, dtype=torch.float32, device=x.device) if need > 0 else None
-        rc = lib.hgq_group_norm_fwd(_ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean), _ptr(rstd), _ptr(ws), B, S, C, groups, epsilon, act, code,
-                                    stream)
-    _lib.check(rc, 'hgq_group_norm_fwd')
-    return y, mean, rstd
+    stats = torch.empty((2, B, groups), dtype=torch.float32, device=device)
+    at, need = stats.data_ptr(), _group_workspace(False, B, S, C, groups, code)
+    with _device_of(device) as stream:
+        ws = torch.empty(need, dtype=torch.float32, device=device) if need > 0 else None
+        rc = _lib.load().hgq_group_norm_fwd(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), at, at + 4 * B * groups if at else None,
+                                            ws.data_ptr() if need > 0 else None, B, S, C, groups, epsilon, act, code, stream)
+    if rc:
+        _lib.check(rc, 'hgq_group_norm_fwd')
+    return y, stats
 
 
 @group_norm_fwd.register_fake
 def _(x, gamma, beta, groups, epsilon, act):
-    stats = x.new_empty((2, x.shape[0], groups), dtype=torch.float32)
-    return torch.empty_like(x), stats[0], stats[1]
+    return torch.empty_like(x), x.new_empty((2, x.shape[0], groups), dtype=torch.float32)
 
 
 @torch.library.custom_op('hgq::group_norm_bwd', mutates_args=())
-def group_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, beta: Tensor, mean: Tensor, rstd: Tensor, groups: int, act: int, need_dx: bool,
+def group_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, beta: Tensor, stats: Tensor, groups: int, act: int, need_dx: bool,
                    need_dgamma: bool, need_dbeta: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """Gradients that are not needed come back empty."""
+    """``stats``: what the forward call left.  Gradients that are not needed come back empty."""
     B, S, C, code = _group_shape(x, groups)
-    _channel_vector('gamma', gamma, x), _channel_vector('beta', beta, x)
-    _need(dy.device == x.device and dy.dtype == x.dtype and dy.shape == x.shape and dy.is_contiguous(), 'dy must be like x')
-    _check_f32('mean', mean), _check_f32('rstd', rstd)
-    _need(mean.numel() == B * groups and rstd.numel() == B * groups, 'mean and rstd are what the forward call left')
+    device = x.device
+    _channel_vector('gamma', gamma, device.index, C), _channel_vector('beta', beta, device.index, C)
+    if not (dy.shape == x.shape and dy.dtype is x.dtype and dy.get_device() == device.index and dy.is_contiguous()):
+        raise ValueError(f'dy must be contiguous and like x, got {dy.dtype} {tuple(dy.shape)} on {dy.device}')
+    if not (stats.numel() == 2 * B * groups and stats.dtype is _F32 and stats.get_device() == device.index and stats.is_contiguous()):
+        raise ValueError('stats must be what the forward call left')
     dx = torch.empty_like(x) if need_dx else x.new_empty(0)
-    dgamma, dbeta = (torch.empty(C if want else 0, dtype=torch.float32, device=x.device) for want in (need_dgamma, need_dbeta))
-    lib = _lib.load()
-    with _device_of(x.device) as stream:
-        need = lib.hgq_group_norm_bwd_workspace(B, S, C, groups, code)
-        ws = torch.empty(need, dtype=torch.float32, device=x.device) if need > 0 else None
-        rc = lib.hgq_group_norm_bwd(_ptr(dy), _ptr(x), _ptr(gamma), _ptr(beta), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dgamma), _ptr(dbeta), _ptr(ws),
-                                    B, S, C, groups, act, code, stream)
-    _lib.check(rc, 'hgq_group_norm_bwd')
+    dgamma = torch.empty(C if need_dgamma else 0, dtype=torch.float32, device=device)
+    dbeta = torch.empty(C if need_dbeta else 0, dtype=torch.float32, device=device)
+    at, need = stats.data_ptr(), _group_workspace(True, B, S, C, groups, code)
+    with _device_of(device) as stream:
+        ws = torch.empty(need, dtype=torch.float32, device=device) if need > 0 else None
+        rc = _lib.load().hgq_group_norm_bwd(dy.data_ptr(), x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), at, at + 4 * B * groups if at else None,
+                                            dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr() if need > 0 else None, B, S, C, groups, act,
+                                            code, stream)
+    if rc:
+        _lib.check(rc, 'hgq_group_norm_bwd')
     return dx, dgamma, dbeta
 
 
 @group_norm_bwd.register_fake
-def _(dy, x, gamma, beta, mean, rstd, groups, act, need_dx, need_dgamma, need_dbeta):
+def _(dy, x, gamma, beta, stats, groups, act, need_dx, need_dgamma, need_dbeta):
     C = x.shape[-1]
     return (torch.empty_like(x) if need_dx else x.new_empty(0), x.new_empty(C if need_dgamma else 0, dtype=torch.float32),
             x.new_empty(C if need_dbeta else 0, dtype=torch.float32))
@@ -3673,20 +3683,35 @@ def _(dy, x, gamma, beta, mean, rstd, groups, act, need_dx, need_dgamma, need_db
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, groups, epsilon, act):
-        empty = torch.empty(0, dtype=torch.float32, device=x.device)
-        ga, be = (t if t is not None else empty for t in (gamma, beta))
-        y, mean, rstd = group_norm_fwd(x, ga, be, groups, epsilon, act)
-        ctx.save_for_backward(x, ga, be, mean, rstd)
+        if gamma is None or beta is None:
+            empty = torch.empty(0, dtype=torch.float32, device=x.device)
+            gamma, beta = (t if t is not None else empty for t in (gamma, beta))
+        y, stats = group_norm_fwd(x, gamma, beta, groups, epsilon, act)
+        ctx.save_for_backward(x, gamma, beta, stats)
         ctx.groups, ctx.act = groups, act
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        x, ga, be, mean, rstd = ctx.saved_tensors
-        want = ctx.needs_input_grad[:3]
-        grads = group_norm_bwd(gy.contiguous(), x, ga, be, mean, rstd, ctx.groups, ctx.act, *want)
-        return (*(g if w else None for g, w in zip(grads, want)), None, None, None)
+        x, gamma, beta, stats = ctx.saved_tensors
+        wx, wg, wb, *_ = ctx.needs_input_grad
+        dx, dg, db = group_norm_bwd(gy.contiguous(), x, gamma, beta, stats, ctx.groups, ctx.act, wx, wg, wb)
+        if torch.is_grad_enabled():  # (create_graph)
+            dx, dg, db = _OnceOnly.apply(dx, dg, db, gy, x, gamma, beta)
+        return dx if wx else None, dg if wg else None, db if wb else None, None, None, None
+
+
+class _OnceOnly(torch.autograd.Function):
+    """Gradients that were asked for with ``create_graph``: usable as they are, and refused where they are to be differentiated again
+    (without this they would pass for constants)."""
+
+    @staticmethod
+    def forward(ctx, dx, dg, db, *inputs):
+        return dx.view_as(dx), dg.view_as(dg), db.view_as(db)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError('group_norm is differentiable once: its gradients have no gradient')
 
 
 def group_norm(x: Tensor, groups: int, gamma: Tensor | None = None, beta: Tensor | None = None, epsilon: float = 1e-3,
@@ -3695,7 +3720,8 @@ def group_norm(x: Tensor, groups: int, gamma: Tensor | None = None, beta: Tensor
     sample's groups of adjacent channels and all its positions, times ``gamma`` plus ``beta`` (float32 ``[channels]``, or ``None``),
     and an activation (``None`` / ``'linear'``, ``'relu'``, ``'silu'`` / ``'swish'``); differentiable in x, gamma and beta.  ``groups=1``
     normalises whole samples, ``groups=channels`` each channel by itself."""
-    _need(activation in GROUP_ACTIVATIONS, f'activation must be one of linear, relu, silu; got {activation!r}')
+    if activation not in GROUP_ACTIVATIONS:
+        raise ValueError(f'activation must be one of linear, relu, silu; got {activation!r}')
     _need(epsilon >= 0, 'epsilon must not be negative')
     return _GroupNorm.apply(x.contiguous(), gamma, beta, int(groups), float(epsilon), GROUP_ACTIVATIONS[activation])
 

@@ -321,3 +321,15 @@ def test_a_normalised_network_trained_with_adamw(dev, bits):
     for p, q in zip(a.parameters(), b.parameters()):
         assert torch.equal(p, q) and torch.isfinite(p).all()
     assert step.opt.iterations == opt.iterations == 4
+
+
+def test_gradients_of_gradients_are_refused(dev):
+    from hgq2_amd import ops
+
+    x = torch.randn(2, 5, 8, device=dev, requires_grad=True)
+    y = ops.group_norm(x, 2, activation='silu')
+    plain, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    once, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    assert torch.equal(once.detach(), plain)
+    with pytest.raises(RuntimeError, match='differentiable once'):
+        once.sum().backward()
