@@ -149,26 +149,30 @@ template <int BITS>
 __device__ __forceinline__ void adamw_block_any(const AdamwLaunch &a, const AdamwItem &it, const AdamwStep &k, int64_t b) {
     const int lane = threadIdx.x & 63;
     const int64_t e = b + lane * 4;
-    float m[4], r[4];
+    float m[4], v[4], r[4], g[4], w[4];
     int sm = 0, sr = 0;
     if (BITS == 8) sm = it.m_scale[b >> 8], sr = it.v_scale[b >> 8];
+    // (all loads before the first store: the compiler cannot know that the arrays do not overlap)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        m[j] = r[j] = 0.0f;
+        m[j] = v[j] = r[j] = g[j] = w[j] = 0.0f;
         if (e + j < it.n) {
-            float v;
+            g[j] = gradient(a, it, e + j), w[j] = load_as_f32(it.w, e + j, it.type);
             if (BITS == 8) {
-                m[j] = e4m3_value(((const uint8_t *)it.m)[e + j], sm);
-                v = e4m3_value(((const uint8_t *)it.v)[e + j], sr);
-                v = __fmul_rn(v, v);
+                m[j] = e4m3_value(((const uint8_t *)it.m)[e + j], sm), v[j] = e4m3_value(((const uint8_t *)it.v)[e + j], sr);
+                v[j] = __fmul_rn(v[j], v[j]);
             } else {
-                m[j] = ((const float *)it.m)[e + j], v = ((const float *)it.v)[e + j];
+                m[j] = ((const float *)it.m)[e + j], v[j] = ((const float *)it.v)[e + j];
             }
-            adamw_moments(gradient(a, it, e + j), m[j], v, r[j], k);
-            store_f32_as(it.w, e + j, it.type, adamw_weight(load_as_f32(it.w, e + j, it.type), m[j], r[j], it, k));
-            if (BITS == 32) ((float *)it.m)[e + j] = m[j], ((float *)it.v)[e + j] = v;
         }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (e + j < it.n) {
+            adamw_moments(g[j], m[j], v[j], r[j], k);
+            store_f32_as(it.w, e + j, it.type, adamw_weight(w[j], m[j], r[j], it, k));
+            if (BITS == 32) ((float *)it.m)[e + j] = m[j], ((float *)it.v)[e + j] = v[j];
+        }
     if (BITS == 8) {
         uint32_t cm, cr;
         encode_block(m, r, (uint64_t)(it.first + e), k, sm, sr, cm, cr);
@@ -256,7 +260,10 @@ __device__ __forceinline__ void adamw_chunk(const AdamwLaunch &a, const AdamwIte
         else adamw_blocks<BITS, _Float16, 2>(it, k, b0);
         return;
     }
-    for (int64_t b = b0; b < e0 + ADAMW_CHUNK && b < it.n; b += 1024) adamw_block_any<BITS>(a, it, k, b);
+    for (int64_t b = b0; b < e0 + ADAMW_CHUNK && b < it.n; b += 1024) {
+        if (it.vec && it.type == HGQ_TYPE_F32 && b + 256 <= it.n) adamw_blocks<BITS, float, 1>(it, k, b);
+        else adamw_block_any<BITS>(a, it, k, b);
+    }
 }
 
 // sum of the workgroup's values, in a fixed order, returned to every thread
