@@ -285,7 +285,10 @@ __device__ __forceinline__ float norm_of_parts(const double *parts, int n, doubl
 }
 
 // The step's number, the powers of the decay rates and the learning rate live in device memory (hgq_adamw_state), so a recorded launch
-// moves on at every replay.  All workgroups read them; the last one to finish the step's last launch writes the next step's.
+// moves on at every replay.  All workgroups read them; in a step's last launch each then takes a ticket, and the one with the last
+// ticket writes the next step's.  Tickets of one counter come one every 27 ns (2048 workgroups: 55 us, more than an update of 4 million
+// elements takes), so there are 32 counters in cache lines of their own, and one for those that finish them; and a workgroup takes
+// its ticket when it begins, so that the answer is there when it ends.
 template <int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum, hgq_adamw_state *state, double b1, double b2, float eps,
                                                     float clipnorm, const double *parts, int n_parts, float *norm_out, uint64_t seed, int items,
@@ -296,11 +299,24 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
         for (int t = 1; t < sum.n; ++t) v = __fadd_rn(v, sum.term[t][0]);
         sum.out[0] = v;
     }
-    AdamwStep k;
-    const int64_t t = state->step + 1;
-    const double p1 = state->beta_1_power * b1, p2 = state->beta_2_power * b2, lr = state->lr;
-    k.alpha = (float)(lr * sqrt(1.0 - p2) / (1.0 - p1)), k.lr = (float)lr, k.t = (uint64_t)t, k.seed = seed;
-    k.one_minus_b1 = (float)(1.0 - b1), k.one_minus_b2 = (float)(1.0 - b2), k.eps = eps;
+    __shared__ AdamwStep shared;
+    uint32_t left = 1;  // tickets not taken before this workgroup's, of its counter
+    int64_t t = 0;
+    double p1 = 0, p2 = 0;
+    const uint32_t counter = gridDim.x > HGQ_ADAMW_TICKETS ? 1 + blockIdx.x % HGQ_ADAMW_TICKETS : HGQ_ADAMW_TICKETS + 1;
+    if (threadIdx.x == 0) {
+        const double lr = state->lr;
+        t = state->step + 1, p1 = state->beta_1_power * b1, p2 = state->beta_2_power * b2;
+        shared.alpha = (float)(lr * sqrt(1.0 - p2) / (1.0 - p1)), shared.lr = (float)lr, shared.t = (uint64_t)t;
+        asm volatile("" ::"v"(t), "v"(p1), "v"(p2), "v"(lr) : "memory");  // (the reads are done before the ticket is taken)
+        if (last) {
+            const uint32_t all = counter <= HGQ_ADAMW_TICKETS ? (gridDim.x - counter) / HGQ_ADAMW_TICKETS + 1 : gridDim.x;
+            left = all - 1 - atomicAdd(&state->ticket[counter][0], 1u);
+        }
+    }
+    __syncthreads();
+    AdamwStep k = shared;
+    k.seed = seed, k.one_minus_b1 = (float)(1.0 - b1), k.one_minus_b2 = (float)(1.0 - b2), k.eps = eps;
     k.c = 1.0f;
     if (n_parts > 0) {
         const float norm = norm_of_parts(parts, n_parts, lds);
@@ -313,10 +329,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
         while (c >= a.start[i + 1]) ++i;
         adamw_chunk<BITS>(a, a.item[i], k, (int64_t)(c - a.start[i]) * ADAMW_CHUNK);
     }
-    if (!last) return;
-    __syncthreads();  // (every thread has used what it read of the state)
-    if (threadIdx.x == 0 && atomicAdd(&state->ticket, 1u) == gridDim.x - 1)
-        state->step = t, state->beta_1_power = p1, state->beta_2_power = p2, state->ticket = 0;
+    if (left) return;
+    state->ticket[counter][0] = 0;
+    if (counter <= HGQ_ADAMW_TICKETS) {
+        if (atomicAdd(&state->ticket[HGQ_ADAMW_TICKETS + 1][0], 1u) != HGQ_ADAMW_TICKETS - 1) return;
+        state->ticket[HGQ_ADAMW_TICKETS + 1][0] = 0;
+    }
+    state->step = t, state->beta_1_power = p1, state->beta_2_power = p2;
 }
 
 // squares of four neighbours; (v ^ 2 of fp32 has 48 bits and stays exact in fp64)

@@ -3371,6 +3371,7 @@ def sgd_update_multi_(ws, gs, l1, lo, hi, lr, sides=None, sum_terms=None, sum_ou
 
 # ---- AdamW and the global norm of gradients
 ADAMW_BLOCK = 256  # HGQ_ADAMW_BLOCK of include/hgq_hip.h: elements that share the scale of a moment in 8 bits
+ADAMW_TICKETS = 32  # HGQ_ADAMW_TICKETS
 _TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ADAMW_WORDS = 19  # hgq_adamw_item as 64-bit words
 _NO_SIDES = (0,) * (2 * SGD_SIDES)
@@ -3390,7 +3391,10 @@ class _AdamwState(ctypes.Structure):
     """``hgq_adamw_state`` of include/hgq_hip.h."""
 
     _fields_ = [('step', ctypes.c_int64), ('beta_1_power', ctypes.c_double), ('beta_2_power', ctypes.c_double), ('lr', ctypes.c_double),
-                ('ticket', ctypes.c_uint32), ('unused', ctypes.c_uint32)]
+                ('ticket', (ctypes.c_uint32 * 32) * (ADAMW_TICKETS + 2))]
+
+
+_ADAMW_STATE_WORDS = ctypes.sizeof(_AdamwState) // 8
 
 
 def _adamw_limits_words(l1: float, lo: float, hi: float, decay: float):
@@ -3493,9 +3497,11 @@ def global_norm(tensors: Sequence[Tensor]) -> Tensor:
 
 
 def adamw_state(device, lr: float, iterations: int = 0, beta_1: float = 0.9, beta_2: float = 0.999) -> Tensor:
-    """The device-side state of an AdamW run after ``iterations`` steps (``hgq_adamw_state``), as five int64 words."""
-    raw = struct.pack('qdddq', int(iterations), float(beta_1)**int(iterations), float(beta_2)**int(iterations), float(lr), 0)
-    return torch.tensor(struct.unpack('5q', raw), dtype=torch.int64).to(device)
+    """The device-side state of an AdamW run after ``iterations`` steps (``hgq_adamw_state``), as int64 words."""
+    raw = struct.pack('qddd', int(iterations), float(beta_1)**int(iterations), float(beta_2)**int(iterations), float(lr))
+    words = torch.zeros(_ADAMW_STATE_WORDS, dtype=torch.int64)
+    words[:4] = torch.tensor(struct.unpack('4q', raw), dtype=torch.int64)
+    return words.to(device)
 
 
 def adamw_moments(n: int, device, state_bits: int = 32) -> list[Tensor]:
@@ -3549,7 +3555,7 @@ def adamw_update_multi_op(ws: Sequence[Tensor], gs: Sequence[Tensor], moments: S
     _need(n >= 1 and all(len(v) == n for v in (gs, l1, lo, hi, decay)) and len(moments) == per * n, 'per-variable lists differ in length')
     device = ws[0].device
     _need(device.type == 'cuda', f'variables must be GPU tensors (there is no CPU implementation), got device {device}')
-    _need(state.dtype == torch.int64 and state.numel() == 5 and state.device == device, 'state: what adamw_state makes, on the variables\' device')
+    _need(state.dtype == torch.int64 and state.numel() == _ADAMW_STATE_WORDS and state.is_contiguous() and state.device == device, 'state: what adamw_state makes, on the variables\' device')
     _need(len({w.data_ptr() for w in ws if w.numel()}) == sum(1 for w in ws if w.numel()), 'a variable is listed twice')
     _need(clipnorm >= 0, 'clipnorm must not be negative')
     words, first = [], 0

@@ -567,7 +567,7 @@ int hgq_sgd_update_multi_sum(const hgq_sgd_item *items, int count, float lr, con
  *
  * `w` and `g` have the type `type`; `g` NULL: none (then at least one side).  Descriptors are read on the host and travel as
  * launch arguments.  `state` is device memory: step, beta_1^step, beta_2^step and lr, of the steps done (0, 1, 1 at the start);
- * the call moves them on, so a recorded call is the next step at every replay.  `ticket` is 0 between calls.  Calls that share
+ * the call moves them on, so a recorded call is the next step at every replay.  Calls that share
  * `state` or variables must not overlap in time.  Two items must not name the same memory.
  *
  * hgq_global_norm: sqrt(sum of squares of all gradients) (`w`, `m`, `v`, `lo`, `hi`, `decay` are not read), in fp64, to `out` (fp32).
@@ -590,10 +590,11 @@ typedef struct {
     const float *side[HGQ_SGD_SIDES];
     const float *side_scale[HGQ_SGD_SIDES];
 } hgq_adamw_item;
+#define HGQ_ADAMW_TICKETS 32
 typedef struct {
     int64_t step;
     double beta_1_power, beta_2_power, lr;
-    uint32_t ticket, unused;
+    uint32_t ticket[HGQ_ADAMW_TICKETS + 2][32]; /* 0 between calls; a cache line each, the first line shared with the above */
 } hgq_adamw_state;
 int64_t hgq_global_norm_parts(const hgq_adamw_item *items, int count);
 int hgq_global_norm(const hgq_adamw_item *items, int count, double *parts, float *out, void *stream);
