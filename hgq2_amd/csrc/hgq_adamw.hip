@@ -20,8 +20,15 @@
 namespace hgq {
 
 constexpr int ADAMW_ITEMS = 28, ADAMW_PIECES = 32;
-constexpr int ADAMW_CHUNK = 2048;  // elements a workgroup takes at a time: eight blocks of 256
+// A step that touches more than the card's 256 MB cache passes through it once: accesses that leave no trace there, four blocks per
+// wavefront in flight, a workgroup per 4096 elements.  150 million elements, 4.2 GB: 851 -> 720 us (5.9 TB/s; the card copies at 5.0), with
+// moments in 8 bits, 2.4 GB: 552 -> 437 us; 37 million bfloat16: 164 -> 137 us.  A smaller step leaves its weights for the next
+// forward pass; two blocks, and up to 2048 workgroups that go over 2048 elements at a time (4 million elements: 22 us either way).
+constexpr int64_t ADAMW_CACHE = (int64_t)256 << 20;
+constexpr int ADAMW_CHUNK = 2048, ADAMW_STREAM_CHUNK = 4096;  // elements a workgroup takes at a time, in blocks of 256
 constexpr int ADAMW_GRID = 2048;
+// Gradients are read around the cache whatever their size: 150 million 145 -> 89 us (6.7 TB/s), 24 million 24 -> 21 us, and the update that
+// follows takes as long to within 3 %.
 constexpr int NORM_LOADS = 8, NORM_GRID = 1024;
 
 struct AdamwItem {
@@ -202,8 +209,19 @@ struct Four<_Float16> {
     typedef _Float16 raw __attribute__((ext_vector_type(4)));
 };
 
+template <bool STREAM, typename V>
+__device__ __forceinline__ V read(const void *p) {
+    return STREAM ? __builtin_nontemporal_load((const V *)p) : *(const V *)p;
+}
+
+template <bool STREAM, typename V>
+__device__ __forceinline__ void write(void *p, V v) {
+    if (STREAM) __builtin_nontemporal_store(v, (V *)p);
+    else *(V *)p = v;
+}
+
 // N of a wavefront's whole blocks, at b and every 1024 elements on: four elements per access, all loads before the first use
-template <int BITS, typename T, int N>
+template <int BITS, typename T, int N, bool STREAM>
 __device__ __forceinline__ void adamw_blocks(const AdamwItem &it, const AdamwStep &k, int64_t b) {
     typedef typename Four<T>::raw raw;
     const int lane = threadIdx.x & 63;
@@ -214,12 +232,12 @@ __device__ __forceinline__ void adamw_blocks(const AdamwItem &it, const AdamwSte
     int sm[N], sr[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        g[n] = *(const raw *)((const T *)it.g + e + 1024 * n);
-        w[n] = *(const raw *)((const T *)it.w + e + 1024 * n);
+        g[n] = read<STREAM, raw>((const T *)it.g + e + 1024 * n);
+        w[n] = read<STREAM, raw>((const T *)it.w + e + 1024 * n);
         if (BITS == 32) {
-            m[n] = *(const floats4_t *)((const float *)it.m + e + 1024 * n), v[n] = *(const floats4_t *)((const float *)it.v + e + 1024 * n);
+            m[n] = read<STREAM, floats4_t>((const float *)it.m + e + 1024 * n), v[n] = read<STREAM, floats4_t>((const float *)it.v + e + 1024 * n);
         } else {
-            cm[n] = *(const uint32_t *)((const uint8_t *)it.m + e + 1024 * n), cr[n] = *(const uint32_t *)((const uint8_t *)it.v + e + 1024 * n);
+            cm[n] = read<STREAM, uint32_t>((const uint8_t *)it.m + e + 1024 * n), cr[n] = read<STREAM, uint32_t>((const uint8_t *)it.v + e + 1024 * n);
             sm[n] = it.m_scale[(b >> 8) + 4 * n], sr[n] = it.v_scale[(b >> 8) + 4 * n];
         }
     }
@@ -239,29 +257,30 @@ __device__ __forceinline__ void adamw_blocks(const AdamwItem &it, const AdamwSte
             w[n][j] = (T)adamw_weight((float)w[n][j], mm[j], rr[j], it, k);
             m[n][j] = mm[j], v[n][j] = vv;
         }
-        *(raw *)((T *)it.w + e + 1024 * n) = w[n];
+        write<STREAM>((T *)it.w + e + 1024 * n, w[n]);
         if (BITS == 32) {
-            *(floats4_t *)((float *)it.m + e + 1024 * n) = m[n], *(floats4_t *)((float *)it.v + e + 1024 * n) = v[n];
+            write<STREAM>((float *)it.m + e + 1024 * n, m[n]), write<STREAM>((float *)it.v + e + 1024 * n, v[n]);
         } else {
             encode_block(mm, rr, (uint64_t)(it.first + e + 1024 * n), k, sm[n], sr[n], cm[n], cr[n]);
-            *(uint32_t *)((uint8_t *)it.m + e + 1024 * n) = cm[n], *(uint32_t *)((uint8_t *)it.v + e + 1024 * n) = cr[n];
+            write<STREAM>((uint8_t *)it.m + e + 1024 * n, cm[n]), write<STREAM>((uint8_t *)it.v + e + 1024 * n, cr[n]);
             if (lane == 0) it.m_scale[(b >> 8) + 4 * n] = (uint8_t)sm[n], it.v_scale[(b >> 8) + 4 * n] = (uint8_t)sr[n];
         }
     }
 }
 
-// one variable's elements [e0, e0 + ADAMW_CHUNK): a lane takes four neighbours, a wavefront 256 - the block that shares a scale
-template <int BITS>
+// one variable's elements [e0, e0 + a chunk): a lane takes four neighbours, a wavefront 256 - the block that shares a scale
+template <int BITS, bool STREAM>
 __device__ __forceinline__ void adamw_chunk(const AdamwLaunch &a, const AdamwItem &it, const AdamwStep &k, int64_t e0) {
+    constexpr int CHUNK = STREAM ? ADAMW_STREAM_CHUNK : ADAMW_CHUNK, N = CHUNK / 1024;
     const int64_t b0 = e0 + (threadIdx.x >> 6) * 256;
-    if (it.vec && e0 + ADAMW_CHUNK <= it.n) {
-        if (it.type == HGQ_TYPE_F32) adamw_blocks<BITS, float, 2>(it, k, b0);
-        else if (it.type == HGQ_TYPE_BF16) adamw_blocks<BITS, __bf16, 2>(it, k, b0);
-        else adamw_blocks<BITS, _Float16, 2>(it, k, b0);
+    if (it.vec && e0 + CHUNK <= it.n) {
+        if (it.type == HGQ_TYPE_F32) adamw_blocks<BITS, float, N, STREAM>(it, k, b0);
+        else if (it.type == HGQ_TYPE_BF16) adamw_blocks<BITS, __bf16, N, STREAM>(it, k, b0);
+        else adamw_blocks<BITS, _Float16, N, STREAM>(it, k, b0);
         return;
     }
-    for (int64_t b = b0; b < e0 + ADAMW_CHUNK && b < it.n; b += 1024) {
-        if (it.vec && it.type == HGQ_TYPE_F32 && b + 256 <= it.n) adamw_blocks<BITS, float, 1>(it, k, b);
+    for (int64_t b = b0; b < e0 + CHUNK && b < it.n; b += 1024) {
+        if (it.vec && it.type == HGQ_TYPE_F32 && b + 256 <= it.n) adamw_blocks<BITS, float, 1, STREAM>(it, k, b);
         else adamw_block_any<BITS>(a, it, k, b);
     }
 }
@@ -289,10 +308,10 @@ __device__ __forceinline__ float norm_of_parts(const double *parts, int n, doubl
 // ticket writes the next step's.  Tickets of one counter come one every 27 ns (2048 workgroups: 55 us, more than an update of 4 million
 // elements takes), so there are 32 counters in cache lines of their own, and one for those that finish them; and a workgroup takes
 // its ticket when it begins, so that the answer is there when it ends.
-template <int BITS>
+template <int BITS, bool STREAM>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum, hgq_adamw_state *state, double b1, double b2, float eps,
-                                                    float clipnorm, const double *parts, int n_parts, float *norm_out, uint64_t seed, int items,
-                                                    int last) {
+                                                    float clipnorm, const double *parts, int n_parts, const float *joined, float *norm_out, uint64_t seed,
+                                                    int items, int last) {
     __shared__ double lds[4];
     if (sum.n > 0 && blockIdx.x == 0 && threadIdx.x == 0) {  // the step's loss terms, which the update does not read
         float v = sum.term[0][0];
@@ -319,7 +338,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
     k.seed = seed, k.one_minus_b1 = (float)(1.0 - b1), k.one_minus_b2 = (float)(1.0 - b2), k.eps = eps;
     k.c = 1.0f;
     if (n_parts > 0) {
-        const float norm = norm_of_parts(parts, n_parts, lds);
+        const float norm = joined ? joined[0] : norm_of_parts(parts, n_parts, lds);
         // no clipping up to the bound; a norm that is not finite makes every step not a number
         k.c = norm <= clipnorm ? 1.0f : norm < __builtin_inff() ? __fdiv_rn(clipnorm, norm) : __builtin_nanf("");
         if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
@@ -327,7 +346,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
     int i = 0;
     for (uint32_t c = blockIdx.x; c < a.start[items]; c += gridDim.x) {
         while (c >= a.start[i + 1]) ++i;
-        adamw_chunk<BITS>(a, a.item[i], k, (int64_t)(c - a.start[i]) * ADAMW_CHUNK);
+        adamw_chunk<BITS, STREAM>(a, a.item[i], k, (int64_t)(c - a.start[i]) * (STREAM ? ADAMW_STREAM_CHUNK : ADAMW_CHUNK));
     }
     if (left) return;
     state->ticket[counter][0] = 0;
@@ -356,7 +375,7 @@ __device__ __forceinline__ double norm_chunk(const AdamwItem &it, int64_t e0) {
     typedef typename Four<T>::raw raw;
     raw g[NORM_LOADS];
 #pragma unroll
-    for (int n = 0; n < NORM_LOADS; ++n) g[n] = *(const raw *)((const T *)it.g + e0 + 1024 * n + 4 * threadIdx.x);
+    for (int n = 0; n < NORM_LOADS; ++n) g[n] = __builtin_nontemporal_load((const raw *)((const T *)it.g + e0 + 1024 * n + 4 * threadIdx.x));
     double v = 0;
 #pragma unroll
     for (int n = 0; n < NORM_LOADS; ++n) v += squares<T>(g[n], it.l1);
@@ -486,7 +505,7 @@ extern "C" int hgq_global_norm(const hgq_adamw_item *items, int count, double *p
 }
 
 extern "C" int hgq_adamw_update_multi(const hgq_adamw_item *items, int count, int state_bits, hgq_adamw_state *state, double beta_1,
-                                      double beta_2, float epsilon, float clipnorm, const double *norm_parts, int64_t n_parts, float *norm_out,
+                                      double beta_2, float epsilon, float clipnorm, double *norm_parts, int64_t n_parts, float *norm_out,
                                       uint64_t seed, const float *const *terms, int n_terms, float *sum_out, void *stream) {
     if (state_bits != 8 && state_bits != 32) return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: moments have 8 or 32 bits, not %d", state_bits);
     int rc = check_items("hgq_adamw_update_multi", items, count, state_bits);
@@ -502,12 +521,24 @@ extern "C" int hgq_adamw_update_multi(const hgq_adamw_item *items, int count, in
     sum.n = n_terms, sum.out = sum_out;
     for (int t = 0; t < n_terms; ++t)
         if (!(sum.term[t] = terms[t])) return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: null term %d", t);
-    return for_launches(items, count, ADAMW_CHUNK, [&](const AdamwLaunch &a, int n, bool last) {
-        const uint32_t chunks = n ? a.start[n] : 0;
-        const int grid = chunks < 1 ? 1 : chunks < ADAMW_GRID ? (int)chunks : ADAMW_GRID;  // (no element at all: the step still counts)
-        auto kernel = state_bits == 8 ? adamw_kernel<8> : adamw_kernel<32>;
+    int64_t bytes = 0;
+    for (int t = 0; t < count; ++t) bytes += items[t].n * ((items[t].type == HGQ_TYPE_F32 ? 12 : 6) + (state_bits == 32 ? 16 : 4));
+    const bool stream_through = bytes > ADAMW_CACHE;
+    // tens of thousands of workgroups take the norm, not its parts
+    float *joined = nullptr;
+    if (stream_through && n_parts > 0) {
+        joined = norm_out ? norm_out : (float *)norm_parts;
+        hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, norm_parts, (int)n_parts, joined);
+        if ((rc = check_launch("hgq_adamw_update_multi"))) return rc;
+        norm_out = nullptr;
+    }
+    return for_launches(items, count, stream_through ? ADAMW_STREAM_CHUNK : ADAMW_CHUNK, [&](const AdamwLaunch &a, int n, bool last) {
+        const uint32_t chunks = n ? a.start[n] : 0, most = stream_through ? chunks : ADAMW_GRID;
+        const int grid = chunks < 1 ? 1 : (int)(chunks < most ? chunks : most);  // (no element at all: the step still counts)
+        auto kernel = state_bits == 8 ? stream_through ? adamw_kernel<8, true> : adamw_kernel<8, false>
+                                      : stream_through ? adamw_kernel<32, true> : adamw_kernel<32, false>;
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a, sum, state, beta_1, beta_2, epsilon, clipnorm, norm_parts,
-                           (int)n_parts, norm_out, seed, n, (int)last);
+                           (int)n_parts, joined, norm_out, seed, n, (int)last);
         sum.n = 0, norm_out = nullptr;
         return check_launch("hgq_adamw_update_multi");
     });

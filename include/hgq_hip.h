@@ -572,7 +572,7 @@ int hgq_sgd_update_multi_sum(const hgq_sgd_item *items, int count, float lr, con
  *
  * hgq_global_norm: sqrt(sum of squares of all gradients) (`w`, `m`, `v`, `lo`, `hi`, `decay` are not read), in fp64, to `out` (fp32).
  * `parts`: hgq_global_norm_parts(items, count) doubles, which hgq_adamw_update_multi takes as `norm_parts` (n_parts > 0: clip); with
- * `out` NULL only they are written.  norm_out (may be NULL) receives the norm.
+ * `out` NULL only they are written; the update may overwrite them.  norm_out (may be NULL) receives the norm.
  * `terms`, `n_terms`, `sum_out`: hgq_sum_scalars riding along (n_terms 0: none).
  */
 #define HGQ_TYPE_F32 0
@@ -599,7 +599,7 @@ typedef struct {
 int64_t hgq_global_norm_parts(const hgq_adamw_item *items, int count);
 int hgq_global_norm(const hgq_adamw_item *items, int count, double *parts, float *out, void *stream);
 int hgq_adamw_update_multi(const hgq_adamw_item *items, int count, int state_bits, hgq_adamw_state *state, double beta_1, double beta_2,
-                           float epsilon, float clipnorm, const double *norm_parts, int64_t n_parts, float *norm_out, uint64_t seed,
+                           float epsilon, float clipnorm, double *norm_parts, int64_t n_parts, float *norm_out, uint64_t seed,
                            const float *const *terms, int n_terms, float *sum_out, void *stream);
 
 /*

@@ -111,7 +111,8 @@ def _variables(sizes, dtype, dev, seed, odd=False):
     return out
 
 
-SIZES = {'few': [1, 3, 255, 256, 257], 'many': [5 + 37 * k for k in range(61)], 'none': [4, 0, 9], 'long': [(1 << 22) + (1 << 20) + 3]}
+SIZES = {'few': [1, 3, 255, 256, 257], 'many': [5 + 37 * k for k in range(61)], 'none': [4, 0, 9], 'long': [(1 << 22) + (1 << 20) + 3],
+         'vast': [17_000_003, 4099, 5]}  # (more than the card's cache holds)
 
 
 @pytest.mark.parametrize('bits', [32, 8])
@@ -119,6 +120,15 @@ SIZES = {'few': [1, 3, 255, 256, 257], 'many': [5 + 37 * k for k in range(61)], 
 @pytest.mark.parametrize('sizes,odd,clip', [('few', False, None), ('few', True, 0.5), ('many', False, 0.5), ('none', False, 1e6), ('long', False, 0.5),
                                             ('long', True, None)])
 def test_two_steps_against_64_bits(dev, sizes, odd, clip, dtype, bits):
+    _two_steps(dev, sizes, odd, clip, dtype, bits)
+
+
+@pytest.mark.parametrize('dtype,bits,clip', [(torch.float32, 32, 0.5), (torch.float32, 8, 0.5), (torch.float32, 8, None), (torch.bfloat16, 32, None)])
+def test_more_than_the_cache_holds(dev, dtype, bits, clip):
+    _two_steps(dev, 'vast', False, clip, dtype, bits)
+
+
+def _two_steps(dev, sizes, odd, clip, dtype, bits):
     from hgq2_amd.train import AdamW
 
     pairs = _variables(SIZES[sizes], dtype, dev, len(sizes) + bits, odd)
