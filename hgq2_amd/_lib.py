@@ -246,6 +246,47 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_native = None
+_NATIVE_CALLS = ('hgq_last_error', 'hgq_global_norm_parts', 'hgq_global_norm', 'hgq_adamw_update_multi', 'hgq_group_norm_fwd_workspace',
+                 'hgq_group_norm_fwd', 'hgq_group_norm_bwd_workspace', 'hgq_group_norm_bwd')
+
+
+def native():
+    """The host code that is compiled against torch (``csrc/hgq_torch.cpp``), bound to the HIP library's entry points; it registers the
+    operators ``hgq::group_norm_fwd``, ``hgq::group_norm_bwd`` and ``hgq::global_norm``."""
+    global _native
+    if _native is not None:
+        return _native
+    import importlib.util
+
+    import torch
+
+    lib, path = load(), os.path.join(_HERE, '_host.so')
+    if not os.path.exists(path):
+        raise HGQLibraryError(f'{path} not found: the host extension is not built. Run `make -C hgq2_amd/csrc` (or __graft_entry__.build()).')
+    spec = importlib.util.spec_from_file_location('hgq2_amd._host', path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in _NATIVE_CALLS}, HGQLibraryError)
+
+    @torch.library.register_fake('hgq::group_norm_fwd')
+    def _(x, gamma, beta, groups, epsilon, act):
+        return torch.empty_like(x), x.new_empty((2, x.shape[0], groups), dtype=torch.float32)
+
+    @torch.library.register_fake('hgq::group_norm_bwd')
+    def _(dy, x, gamma, beta, stats, groups, act, need_dx, need_dgamma, need_dbeta):
+        C = x.shape[-1]
+        return (torch.empty_like(x) if need_dx else x.new_empty(0), x.new_empty(C if need_dgamma else 0, dtype=torch.float32),
+                x.new_empty(C if need_dbeta else 0, dtype=torch.float32))
+
+    @torch.library.register_fake('hgq::global_norm')
+    def _(tensors):
+        return tensors[0].new_empty((), dtype=torch.float32)
+
+    _native = mod
+    return mod
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = load().hgq_last_error()

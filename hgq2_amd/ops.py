@@ -10,8 +10,6 @@ raises.
 from __future__ import annotations
 
 import ctypes
-import functools
-import math
 import struct
 import threading
 from array import array
@@ -3379,7 +3377,7 @@ _adamw_limits = {}
 
 
 class _AdamwItem(ctypes.Structure):
-    """``hgq_adamw_item`` of include/hgq_hip.h (what :func:`_adamw_item` writes word by word)."""
+    """``hgq_adamw_item`` of include/hgq_hip.h (written word by word into an ``array('q')``)."""
 
     _fields_ = [('w', ctypes.c_void_p), ('g', ctypes.c_void_p), ('m', ctypes.c_void_p), ('v', ctypes.c_void_p), ('m_scale', ctypes.c_void_p),
                 ('v_scale', ctypes.c_void_p), ('n', ctypes.c_int64), ('first', ctypes.c_int64), ('l1', ctypes.c_float), ('lo', ctypes.c_float),
@@ -3417,22 +3415,6 @@ def _check_gradient(name: str, t: Tensor, device, dtype, numel: int):
     _need(t.numel() == numel, f'{name} has {t.numel()} elements, not {numel}')
 
 
-def _side_words(pairs, device, numel: int, held: list):
-    """The words of a descriptor's further gradient pieces: ``(scale or None, gradient)`` pairs."""
-    _need(len(pairs) <= SGD_SIDES, f'at most {SGD_SIDES} side gradients per variable')
-    ptrs, scales = [0] * SGD_SIDES, [0] * SGD_SIDES
-    for s, (sc, sd) in enumerate(pairs):
-        _check_gradient('side gradient', sd, device, _F32, numel)
-        sd = sd.contiguous()
-        held.append(sd)
-        ptrs[s] = sd.data_ptr()
-        if sc is not None:
-            _need(sc.device == device and sc.dtype == torch.float32 and sc.numel() == 1, 'a side-gradient scale is one float32 on the GPU')
-            held.append(sc)
-            scales[s] = sc.data_ptr()
-    return (*ptrs, *scales)
-
-
 class _device_of:
     """Launches go to the current stream of the device that the tensors are on, whichever device is the current one: ``with
     _device_of(device) as stream``."""
@@ -3458,42 +3440,11 @@ _current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.curre
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-@torch.library.custom_op('hgq::global_norm', mutates_args=())
-def global_norm_op(tensors: Sequence[Tensor]) -> Tensor:
-    _need(len(tensors) >= 1, 'at least one tensor is expected')
-    device = tensors[0].device
-    _need(device.type == 'cuda', f'tensors must be on a GPU (there is no CPU implementation), got device {device}')
-    n, held, index, at = len(tensors), [], tensors[0].get_device(), 0
-    items = array('q', bytes(8 * _ADAMW_WORDS * n))  # (hgq_adamw_item: gradient, number of elements and type)
-    for t in tensors:
-        code = _TYPE_CODES.get(t.dtype)
-        if code is None or t.get_device() != index or t.layout is not torch.strided:
-            _need(code is not None, f'tensors must be float32, bfloat16 or float16, got {t.dtype}')
-            raise ValueError(f'tensors must be dense and on one device, got {t.layout} on {t.device}')
-        if not t.is_contiguous():
-            t = t.detach().contiguous()
-            held.append(t)
-        items[at + 1], items[at + 6], items[at + 10] = t.data_ptr(), t.numel(), code
-        at += _ADAMW_WORDS
-    out = torch.empty((), dtype=torch.float32, device=device)
-    lib, at = _lib.load(), items.buffer_info()[0]
-    with _device_of(device) as stream:
-        parts = torch.empty(lib.hgq_global_norm_parts(at, n), dtype=torch.float64, device=device)
-        rc = lib.hgq_global_norm(at, n, parts.data_ptr(), out.data_ptr(), stream)
-    _lib.check(rc, 'hgq_global_norm')
-    return out
-
-
-@global_norm_op.register_fake
-def _(tensors):
-    return tensors[0].new_empty((), dtype=torch.float32)
-
-
 def global_norm(tensors: Sequence[Tensor]) -> Tensor:
     """``sqrt(sum of squares of all elements)`` of float32, bfloat16 or float16 GPU tensors, as ``keras.ops`` users write
     ``global_norm`` of their gradients (``None`` entries are left out): one float32, summed in fp64 in a fixed order, so it neither
     overflows before its result does nor depends on the order in which workgroups end.  Not differentiable."""
-    return global_norm_op([t for t in tensors if t is not None])
+    return _lib.native().global_norm(tensors)
 
 
 def adamw_state(device, lr: float, iterations: int = 0, beta_1: float = 0.9, beta_2: float = 0.999) -> Tensor:
@@ -3518,7 +3469,7 @@ def adamw_moments(n: int, device, state_bits: int = 32) -> list[Tensor]:
 
 
 def _adamw_launch(items, count: int, state_bits: int, state: Tensor, beta_1: float, beta_2: float, epsilon: float, clipnorm, norm_out,
-                  seed: int, sum_terms, sum_out):
+                  seed: int):
     """``items``: hgq_adamw_item words of ``count`` variables in an ``array('q')``; ``clipnorm`` None: no clipping."""
     lib, at = _lib.load(), items.buffer_info()[0]
     device = state.device
@@ -3530,18 +3481,9 @@ def _adamw_launch(items, count: int, state_bits: int, state: Tensor, beta_1: flo
             parts = torch.empty(n_parts, dtype=torch.float64, device=device)
             if n_parts:
                 _lib.check(lib.hgq_global_norm(at, count, parts.data_ptr(), None, stream), 'hgq_global_norm')
-        ptrs, n_terms = None, len(sum_terms) if sum_terms else 0
-        if n_terms:
-            _need(n_terms <= SUM_BATCH, f'at most {SUM_BATCH} terms ride along with the update')
-            ptrs = (ctypes.c_void_p * n_terms)()
-            for t, term in enumerate(sum_terms):
-                _check_f32('term', term)
-                _need(term.numel() == 1, 'every term must hold one element')
-                ptrs[t] = term.data_ptr()
-            _check_f32('sum_out', sum_out)
         rc = lib.hgq_adamw_update_multi(at, count, state_bits, state.data_ptr(), beta_1, beta_2, epsilon, clipnorm if n_parts else 0.0,
                                         parts.data_ptr() if n_parts else None, n_parts, norm_out.data_ptr() if norm_out is not None else None,
-                                        seed, ptrs, n_terms, sum_out.data_ptr() if n_terms else None, stream)
+                                        seed, None, 0, None, stream)
     _lib.check(rc, 'hgq_adamw_update_multi')
 
 
@@ -3578,7 +3520,7 @@ def adamw_update_multi_op(ws: Sequence[Tensor], gs: Sequence[Tensor], moments: S
         _check_f32('norm_out', norm_out)
         _need(norm_out.numel() == 1 and norm_out.device == device, 'norm_out is one float32')
     _adamw_launch(array('q', words), n, state_bits, state, beta_1, beta_2, epsilon, clipnorm or None,
-                  norm_out if norm_out.numel() else None, seed, None, None)
+                  norm_out if norm_out.numel() else None, seed)
 
 
 def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: float = 0.999, epsilon: float = 1e-7, decay=None, l1=None,
@@ -3605,121 +3547,6 @@ def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: flo
 GROUP_ACTIVATIONS = {None: _lib.ACT_NONE, 'linear': _lib.ACT_NONE, 'relu': _lib.ACT_RELU, 'silu': _lib.ACT_SILU, 'swish': _lib.ACT_SILU}
 
 
-def _group_shape(x: Tensor, groups: int):
-    code, shape = _TYPE_CODES.get(x.dtype), x.shape
-    if code is None or not x.is_cuda or len(shape) < 2 or not x.is_contiguous() or shape[-1] < 1 or groups < 1 or shape[-1] % groups:
-        # (what is wrong is put into words only here: the checks run at every call)
-        _need(x.is_cuda, f'x must be a GPU tensor (there is no CPU implementation), got device {x.device}')
-        _need(code is not None, f'x must be float32, bfloat16 or float16, got {x.dtype}')
-        _need(len(shape) >= 2 and shape[-1] >= 1, f'x must be [batch, ..., channels], got {tuple(shape)}')
-        _need(x.is_contiguous(), 'x must be contiguous')
-        raise ValueError(f'{shape[-1]} channels do not fall into {groups} groups of one size')
-    return shape[0], math.prod(shape[1:-1]), shape[-1], code
-
-
-def _channel_vector(name: str, t: Tensor, index: int, channels: int):
-    """A per-channel operand, or an empty tensor in the place of none."""
-    n = t.numel()
-    if n and (n != channels or t.dtype is not _F32 or t.get_device() != index or not t.is_contiguous()):
-        raise ValueError(f'{name} must be a contiguous float32 tensor of {channels} elements on the same GPU, got {t.dtype} {tuple(t.shape)} on {t.device}')
-
-
-@functools.lru_cache(4096)
-def _group_workspace(backward: bool, *shape) -> int:
-    """Workspace in floats, by the sizes alone."""
-    lib = _lib.load()
-    return (lib.hgq_group_norm_bwd_workspace if backward else lib.hgq_group_norm_fwd_workspace)(*shape)
-
-
-@torch.library.custom_op('hgq::group_norm_fwd', mutates_args=())
-def group_norm_fwd(x: Tensor, gamma: Tensor, beta: Tensor, groups: int, epsilon: float, act: int) -> tuple[Tensor, Tensor]:
-    """``gamma``, ``beta`` empty: none.  Returns y and, per sample and group, the mean and 1 / sqrt(var + epsilon) (``[2, batch, groups]``)."""
-    B, S, C, code = _group_shape(x, groups)
-    device = x.device
-    _channel_vector('gamma', gamma, device.index, C), _channel_vector('beta', beta, device.index, C)
-    y = torch.empty_like(x)
-    stats = torch.empty((2, B, groups), dtype=torch.float32, device=device)
-    at, need = stats.data_ptr(), _group_workspace(False, B, S, C, groups, code)
-    with _device_of(device) as stream:
-        ws = torch.empty(need, dtype=torch.float32, device=device) if need > 0 else None
-        rc = _lib.load().hgq_group_norm_fwd(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), at, at + 4 * B * groups if at else None,
-                                            ws.data_ptr() if need > 0 else None, B, S, C, groups, epsilon, act, code, stream)
-    if rc:
-        _lib.check(rc, 'hgq_group_norm_fwd')
-    return y, stats
-
-
-@group_norm_fwd.register_fake
-def _(x, gamma, beta, groups, epsilon, act):
-    return torch.empty_like(x), x.new_empty((2, x.shape[0], groups), dtype=torch.float32)
-
-
-@torch.library.custom_op('hgq::group_norm_bwd', mutates_args=())
-def group_norm_bwd(dy: Tensor, x: Tensor, gamma: Tensor, beta: Tensor, stats: Tensor, groups: int, act: int, need_dx: bool,
-                   need_dgamma: bool, need_dbeta: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """``stats``: what the forward call left.  Gradients that are not needed come back empty."""
-    B, S, C, code = _group_shape(x, groups)
-    device = x.device
-    _channel_vector('gamma', gamma, device.index, C), _channel_vector('beta', beta, device.index, C)
-    if not (dy.shape == x.shape and dy.dtype is x.dtype and dy.get_device() == device.index and dy.is_contiguous()):
-        raise ValueError(f'dy must be contiguous and like x, got {dy.dtype} {tuple(dy.shape)} on {dy.device}')
-    if not (stats.numel() == 2 * B * groups and stats.dtype is _F32 and stats.get_device() == device.index and stats.is_contiguous()):
-        raise ValueError('stats must be what the forward call left')
-    dx = torch.empty_like(x) if need_dx else x.new_empty(0)
-    dgamma = torch.empty(C if need_dgamma else 0, dtype=torch.float32, device=device)
-    dbeta = torch.empty(C if need_dbeta else 0, dtype=torch.float32, device=device)
-    at, need = stats.data_ptr(), _group_workspace(True, B, S, C, groups, code)
-    with _device_of(device) as stream:
-        ws = torch.empty(need, dtype=torch.float32, device=device) if need > 0 else None
-        rc = _lib.load().hgq_group_norm_bwd(dy.data_ptr(), x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), at, at + 4 * B * groups if at else None,
-                                            dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr() if need > 0 else None, B, S, C, groups, act,
-                                            code, stream)
-    if rc:
-        _lib.check(rc, 'hgq_group_norm_bwd')
-    return dx, dgamma, dbeta
-
-
-@group_norm_bwd.register_fake
-def _(dy, x, gamma, beta, stats, groups, act, need_dx, need_dgamma, need_dbeta):
-    C = x.shape[-1]
-    return (torch.empty_like(x) if need_dx else x.new_empty(0), x.new_empty(C if need_dgamma else 0, dtype=torch.float32),
-            x.new_empty(C if need_dbeta else 0, dtype=torch.float32))
-
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gamma, beta, groups, epsilon, act):
-        if gamma is None or beta is None:
-            empty = torch.empty(0, dtype=torch.float32, device=x.device)
-            gamma, beta = (t if t is not None else empty for t in (gamma, beta))
-        y, stats = group_norm_fwd(x, gamma, beta, groups, epsilon, act)
-        ctx.save_for_backward(x, gamma, beta, stats)
-        ctx.groups, ctx.act = groups, act
-        return y
-
-    @staticmethod
-    def backward(ctx, gy):
-        x, gamma, beta, stats = ctx.saved_tensors
-        wx, wg, wb, *_ = ctx.needs_input_grad
-        dx, dg, db = group_norm_bwd(gy.contiguous(), x, gamma, beta, stats, ctx.groups, ctx.act, wx, wg, wb)
-        if torch.is_grad_enabled():  # (create_graph)
-            dx, dg, db = _OnceOnly.apply(dx, dg, db, gy, x, gamma, beta)
-        return dx if wx else None, dg if wg else None, db if wb else None, None, None, None
-
-
-class _OnceOnly(torch.autograd.Function):
-    """Gradients that were asked for with ``create_graph``: usable as they are, and refused where they are to be differentiated again
-    (without this they would pass for constants)."""
-
-    @staticmethod
-    def forward(ctx, dx, dg, db, *inputs):
-        return dx.view_as(dx), dg.view_as(dg), db.view_as(db)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise RuntimeError('group_norm is differentiable once: its gradients have no gradient')
-
-
 def group_norm(x: Tensor, groups: int, gamma: Tensor | None = None, beta: Tensor | None = None, epsilon: float = 1e-3,
                activation: str | None = None) -> Tensor:
     """Group normalisation of ``x`` ``[batch, ..., channels]`` (float32, bfloat16 or float16, any number of axes between) over each
@@ -3729,7 +3556,7 @@ def group_norm(x: Tensor, groups: int, gamma: Tensor | None = None, beta: Tensor
     if activation not in GROUP_ACTIVATIONS:
         raise ValueError(f'activation must be one of linear, relu, silu; got {activation!r}')
     _need(epsilon >= 0, 'epsilon must not be negative')
-    return _GroupNorm.apply(x.contiguous(), gamma, beta, int(groups), float(epsilon), GROUP_ACTIVATIONS[activation])
+    return _lib.native().group_norm(x, int(groups), gamma, beta, float(epsilon), GROUP_ACTIVATIONS[activation])
 
 
 # ======================================================================================

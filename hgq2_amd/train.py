@@ -9,11 +9,10 @@ propagate; ``w <- w - lr * g``; apply each variable's constraint.
 from __future__ import annotations
 
 import operator
-from array import array
 
 import torch
 
-from . import ops
+from . import _lib, ops
 from .core import Layer, tree_cache
 from .regularizers import MonoL1
 
@@ -177,10 +176,8 @@ class AdamW(SGD):
         self.weight_decay, self.beta_1, self.beta_2 = float(weight_decay), float(beta_1), float(beta_2)
         self.epsilon, self.global_clipnorm = float(epsilon), None if global_clipnorm is None else float(global_clipnorm)
         self.state_bits, self.seed = int(state_bits), int(seed) & (2**63 - 1)
-        self._no_decay = set()
-        self._layout, self.offsets, n = [], [], 0  # where each variable's moments begin
+        self.offsets, n = [], 0  # where each variable's moments begin
         for p in self.params:
-            self._layout.append((p, p.numel(), p.nbytes, p.dtype))
             self.offsets.append(n)
             n += -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
         self._moments = ops.adamw_moments(n, self.device, self.state_bits)
@@ -188,15 +185,9 @@ class AdamW(SGD):
             self._names = ('momentum', 'velocity')
         else:
             self._names = ('momentum', 'momentum_scale', 'velocity_root', 'velocity_scale')
-        # the variables' descriptors (hgq_adamw_item): moments, place and type now, the other words at every step
-        words, mom = [], [t.data_ptr() for t in self._moments]
-        for (p, _, _, dtype), at in zip(self._layout, self.offsets):
-            if self.state_bits == 32:
-                m = (mom[0] + 4 * at, mom[1] + 4 * at, 0, 0)
-            else:
-                m = (mom[0] + at, mom[2] + at, mom[1] + at // ops.ADAMW_BLOCK, mom[3] + at // ops.ADAMW_BLOCK)
-            words += (0, 0, *m, 0, at, 0, 0, ops._TYPE_CODES[dtype], *ops._NO_SIDES)
-        self._items = array('q', words)
+        self._variables = _lib.native().AdamwVariables(list(self.params), self._moments, self.state_bits)
+        for k in range(len(self.params)):
+            self._variables.set_decay(k, self.weight_decay)
         self.grad_norm = torch.zeros((), dtype=torch.float32, device=self.device) if self.global_clipnorm is not None else None
         self._state = ops.adamw_state(self.device, lr, 0, self.beta_1, self.beta_2)
         self.lr = lr
@@ -236,9 +227,9 @@ class AdamW(SGD):
         """Variables, or parts of variables' names (``var_name``), that are not decayed."""
         ids = {id(v) for v in var_list or ()}
         names = tuple(var_names or ())
-        for p in self.params:
+        for k, p in enumerate(self.params):
             if id(p) in ids or any(n in (getattr(p, 'var_name', None) or '') for n in names):
-                self._no_decay.add(id(p))
+                self._variables.set_decay(k, 0.0)
 
     def state_dict(self) -> dict:
         """The number of steps and copies of the moments (read back by :meth:`load_state_dict`)."""
@@ -265,61 +256,29 @@ class AdamW(SGD):
     @torch.no_grad()
     def step(self):
         sums = ops.join_side(hand_over_sums=True)  # the loss terms' sum rides along with the update launch
-        items, held, post = self._items, [], []
-        dev, inf = self.device, float('inf')
-        index, fold, no_decay, decays = dev.index, self.fold_regularizers, self._no_decay, self.weight_decay
-        plain = ops._adamw_limits_words(0.0, -inf, inf, decays)
-        count = 0
-        # (the host's share of a small step: a variable is asked for each thing once, its own attributes come from one dictionary, and
-        # only the words of its descriptor that can change are written)
-        for at, (p, n, size, dtype) in enumerate(self._layout):
-            at *= ops._ADAMW_WORDS
-            g, extra = p.grad, p.__dict__
-            side = extra.get('_hgq_side')
-            if n == 0 or (g is None and not side):
-                items[at + 6] = 0  # (an item without elements is passed over)
-                continue
-            if p.get_device() != index or p.dtype is not dtype or p.nbytes != size or not p.is_contiguous():
-                raise ValueError(f'variables must stay contiguous, on {dev}, and of their size and type')
-            gradient = 0
-            if g is not None:
-                if g.get_device() != index or g.dtype is not dtype or g.nbytes != size or g.layout is not torch.strided:
-                    ops._check_gradient('gradient', g, dev, dtype, n)
-                if not g.is_contiguous():
-                    g = g.contiguous()
-                    held.append(g)
-                gradient = g.data_ptr()
-            items[at], items[at + 1], items[at + 6] = p.data_ptr(), gradient, n
-            c, r = extra.get('constraint'), extra.get('regularizer')
-            if c is None and r is None and not no_decay:
-                bounds = plain
-            else:
-                lo, hi = -inf, inf
-                if c is not None:
-                    clip = c.bounds()
-                    if clip is None:  # a constraint that is not a clip: applied after the update
-                        post.append((p, c))
-                    else:
-                        lo, hi = clip
-                l1 = r.l1 if (fold and isinstance(r, MonoL1)) else 0.0
-                bounds = ops._adamw_limits_words(l1, lo, hi, 0.0 if id(p) in no_decay else decays)
-            items[at + 8], items[at + 9] = bounds
+        variables, post, inf = self._variables, [], float('inf')
+        special = variables.gather()  # variables with gradient pieces, constraints or regularizers; None: no gradient at all
+        for k in special or ():
+            p = self.params[k]
+            side = list(getattr(p, '_hgq_side', None) or ())
+            while len(side) > ops.SGD_SIDES:  # more pieces than the kernel takes: fold the surplus into one
+                (s1, d1), (s2, d2) = side.pop(), side.pop()
+                side.append((None, (d1 if s1 is None else s1 * d1) + (d2 if s2 is None else s2 * d2)))
             if side:
-                side = list(side)
-                while len(side) > ops.SGD_SIDES:  # more pieces than the kernel takes: fold the surplus into one
-                    (s1, d1), (s2, d2) = side.pop(), side.pop()
-                    side.append((None, (d1 if s1 is None else s1 * d1) + (d2 if s2 is None else s2 * d2)))
-                items[at + 11:at + 19] = array('q', ops._side_words(side, dev, n, held))
-            elif items[at + 11]:
-                items[at + 11:at + 19] = array('q', ops._NO_SIDES)
-            count += 1
-        ride = sums.pop(0) if (count and sums) else (None, None)
+                variables.pieces(k, side)
+            c, r = getattr(p, 'constraint', None), getattr(p, 'regularizer', None)
+            bounds = c.bounds() if c is not None else (-inf, inf)
+            if bounds is None:  # a constraint that is not a clip: applied after the update
+                bounds = (-inf, inf)
+                post.append((p, c))
+            variables.limits(k, r.l1 if (self.fold_regularizers and isinstance(r, MonoL1)) else 0.0, *bounds)
+        ride = sums.pop(0) if (special is not None and sums) else ((), None)
         for terms, out in sums:
             ops.sum_scalars_into(terms, out)
-        if count:
+        if special is not None:
             ops.touch_state()  # written through pointers: the version counters do not move
-            ops._adamw_launch(items, len(self._layout), self.state_bits, self._state, self.beta_1, self.beta_2, self.epsilon, self.global_clipnorm,
-                              self.grad_norm, self.seed, ride[0], ride[1])
+            variables.step(self._state, self.beta_1, self.beta_2, self.epsilon, self.global_clipnorm or 0.0, self.grad_norm, self.seed,
+                           [t.detach() for t in ride[0]], ride[1])
         for p, c in post:
             p.copy_(c(p))
 

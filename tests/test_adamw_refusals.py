@@ -121,3 +121,31 @@ def test_moments_before_the_first_step():
     assert m.dtype == v.dtype == torch.float32 and m.numel() == v.numel() == 300 and not m.any() and not v.any()
     for t, (dtype, n) in zip(ops.adamw_moments(300, 'cpu', 8), ((torch.float8_e4m3fn, 300), (torch.float8_e8m0fnu, 2)) * 2):
         assert t.dtype == dtype and t.numel() == n
+
+
+def test_missing_host_extension_fails_loudly(monkeypatch):
+    monkeypatch.setattr(_lib, '_native', None)
+    monkeypatch.setattr(_lib, '_HERE', '/nonexistent')
+    with pytest.raises(_lib.HGQLibraryError, match='not built'):
+        _lib.native()
+
+
+def test_operators_without_data():
+    """Shapes and types on fake tensors, as tracing sees the operators; CPU tensors reach the check that refuses them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    _lib.native()
+    with FakeTensorMode():
+        x, c = torch.empty(2, 5, 8, dtype=torch.bfloat16, device='cuda'), torch.empty(8, device='cuda')
+        y, stats = torch.ops.hgq.group_norm_fwd(x, c, c, 4, 1e-3, 0)
+        assert y.shape == x.shape and y.dtype == x.dtype and stats.shape == (2, 2, 4) and stats.dtype == torch.float32
+        dx, dg, db = torch.ops.hgq.group_norm_bwd(y, x, c, c, stats, 4, 0, True, True, False)
+        assert dx.shape == x.shape and dg.shape == (8,) and db.numel() == 0
+        assert torch.ops.hgq.global_norm([x, c]).shape == ()
+        out = ops.group_norm(x, 4, c, c, activation='silu')
+        assert out.shape == x.shape and ops.global_norm([x]).dtype == torch.float32
+    z = torch.zeros(2, 5, 8)
+    with pytest.raises(ValueError, match='GPU'):
+        torch.ops.hgq.group_norm_fwd(z, z[0, 0], z[0, 0], 4, 1e-3, 0)
+    with pytest.raises(TypeError, match='tensor'):
+        ops.group_norm(3.0, 4)
