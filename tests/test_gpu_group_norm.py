@@ -19,11 +19,11 @@ HALF = {torch.float32: 0.0, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
 
 
 def _definition(x, dy, gamma, beta, G, eps, act):
-    """Values and tolerances of y, dx, dgamma, dbeta in 64 bits on the CPU; x [B, S, C]."""
-    x, dy = x.double().cpu(), dy.double().cpu()
+    """Values and tolerances of y, dx, dgamma, dbeta in 64 bits; x [B, S, C]."""
+    x, dy = x.double(), dy.double().to(x.device)
     B, S, C = x.shape
-    ga = gamma.double().cpu() if gamma is not None else torch.ones(C, dtype=torch.float64)
-    be = beta.double().cpu() if beta is not None else torch.zeros(C, dtype=torch.float64)
+    ga = gamma.double() if gamma is not None else torch.ones(C, dtype=torch.float64, device=x.device)
+    be = beta.double() if beta is not None else torch.zeros(C, dtype=torch.float64, device=x.device)
     per = lambda t: t.view(B, S, G, C // G)  # noqa: E731
     gmean = lambda t: per(t).mean(dim=(1, 3), keepdim=True)  # noqa: E731
     whole = lambda t: t.expand(B, S, G, C // G).reshape(B, S, C)  # noqa: E731
@@ -59,7 +59,7 @@ def _definition(x, dy, gamma, beta, G, eps, act):
 
 
 def _check(got, want, tol, dtype, what):
-    got = got.detach().double().cpu().reshape(want.shape)
+    got = got.detach().double().reshape(want.shape)
     tol = tol + HALF[dtype] * (want.abs() + tol).clamp(max=1e300) + (2.0**-25 if dtype == torch.float16 else 0.0)
     bad = ~((got - want).abs() <= tol)
     assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()}, worst {float(((got - want).abs() / tol.clamp(min=1e-300)).max()):.3g} times the tolerance'
@@ -333,3 +333,31 @@ def test_gradients_of_gradients_are_refused(dev):
     assert torch.equal(once.detach(), plain)
     with pytest.raises(RuntimeError, match='differentiable once'):
         once.sum().backward()
+
+
+@pytest.mark.parametrize('shape,G,dtype,act', [((1100, 26, 26, 32), 8, torch.float32, 'silu'), ((20, 61, 64, 1024), 32, torch.bfloat16, 'linear')])
+def test_more_than_the_cache_holds(dev, shape, G, dtype, act):
+    """Tensors whose pass exceeds the card's cache (outputs written past it), by their first and last samples and by the sums over all."""
+    from hgq2_amd import ops
+
+    g = torch.Generator(device=dev).manual_seed(9)
+    C = shape[-1]
+    x = torch.randn(shape, generator=g, device=dev).to(dtype).requires_grad_(True)
+    dy = torch.randn(shape, generator=g, device=dev).to(dtype)
+    gamma, beta = (1 + 0.3 * torch.randn(C, generator=g, device=dev)).requires_grad_(True), torch.randn(C, generator=g, device=dev).requires_grad_(True)
+    y = ops.group_norm(x, G, gamma, beta, 1e-3, act)
+    dx, dgamma, dbeta = torch.autograd.grad(y, [x, gamma, beta], dy)
+    for part in (slice(0, 3), slice(shape[0] - 3, shape[0])):
+        flat = (3, -1, C)
+        want, tol = _definition(x[part].detach().reshape(flat), dy[part].reshape(flat), gamma.detach(), beta.detach(), G, 1e-3, act)
+        _check(y[part], want[0], tol[0], dtype, 'y')
+        _check(dx[part], want[1], tol[1], dtype, 'dx')
+    sums, tols = [0, 0], [0, 0]
+    for at in range(0, shape[0], 50):
+        part = slice(at, at + 50)
+        flat = (len(x[part]), -1, C)
+        want, tol = _definition(x[part].detach().reshape(flat), dy[part].reshape(flat), gamma.detach(), beta.detach(), G, 1e-3, act)
+        for k in range(2):
+            sums[k], tols[k] = sums[k] + want[2 + k], tols[k] + tol[2 + k]
+    _check(dgamma, sums[0], tols[0], torch.float32, 'dgamma')
+    _check(dbeta, sums[1], tols[1], torch.float32, 'dbeta')
