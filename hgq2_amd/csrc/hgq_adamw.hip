@@ -14,6 +14,8 @@
 // draws 32 bits per element): word e % 4 of counter (e / 4, t), low half for m and high half for r.  As fp32 numbers scaled by
 // 2^-120, E4M3 values have their code, normal and subnormal, in bits 20 to 27, so rounding is one addition to the bits below and a shift.
 // An r above zero keeps at least the smallest code: a zero would let epsilon alone divide the next step.
+#include <math.h>
+
 #include "hgq_device.h"
 #include "hgq_host.h"
 
@@ -38,7 +40,8 @@ struct AdamwItem {
     uint8_t *m_scale, *v_scale;
     int64_t n, first;
     float l1, lo, hi, decay;
-    short type, vec;      // vec: a plain gradient and aligned memory, four elements per access
+    char type, vec;       // vec: a plain gradient and aligned memory, four elements per access
+    char bounded;         // lo or hi is finite
     short piece, pieces;  // its entries of the launch's list of further gradient pieces
 };
 struct AdamwLaunch {
@@ -94,14 +97,12 @@ __device__ __forceinline__ void philox4x32_7(uint64_t counter, uint64_t step, ui
     out[0] = c0, out[1] = c1, out[2] = c2, out[3] = c3;
 }
 
-// E4M3 code (0x7f: not a number) of a magnitude under the block's scale byte s, rounded by the 16-bit number h
-__device__ __forceinline__ uint32_t e4m3_code(float a, int s, uint32_t h) {
-    const uint32_t c = (__float_as_uint(ldexpf(a, 7 - s)) + (h << 4)) >> 20;
-    return a < __builtin_inff() ? c : 0x7fu;
-}
+// E4M3 code of a finite magnitude under the block's scale byte s, rounded by the 16-bit number h
+__device__ __forceinline__ uint32_t e4m3_code(float a, int s, uint32_t h) { return (__float_as_uint(ldexpf(a, 7 - s)) + (h << 4)) >> 20; }
 
-__device__ __forceinline__ float e4m3_value(uint32_t code, int s) {
-    return ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)code, 0), s - 127);
+template <int J>
+__device__ __forceinline__ float e4m3_value(uint32_t codes, int s) {  // of byte J
+    return ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)codes, J), s - 127);
 }
 
 __device__ __forceinline__ uint32_t exponent_field(float v) {  // of finite magnitudes; the others do not count
@@ -114,10 +115,14 @@ struct AdamwStep {
     uint64_t t, seed;
 };
 
-// w <- the updated weight; m and r already hold the new moments
+// w <- the updated weight; m and r already hold the new moments.  The quotient is a product with the hardware's reciprocal (one unit in
+// the last place; r + eps lies in [2^-75, 2^65] or is zero): the step is far smaller than w, and a rounded division takes ten instructions.
 __device__ __forceinline__ float adamw_weight(float w, float m, float r, const AdamwItem &it, const AdamwStep &k) {
     w = __fsub_rn(w, __fmul_rn(w, __fmul_rn(k.lr, it.decay)));
-    w = __fsub_rn(w, __fdiv_rn(__fmul_rn(m, k.alpha), __fadd_rn(r, k.eps)));
+    return __fsub_rn(w, __fmul_rn(__fmul_rn(m, k.alpha), __builtin_amdgcn_rcpf(__fadd_rn(r, k.eps))));
+}
+
+__device__ __forceinline__ float adamw_clip(float w, const AdamwItem &it) {
     return w < it.lo ? it.lo : w > it.hi ? it.hi : w;  // (not a number stays that)
 }
 
@@ -129,25 +134,45 @@ __device__ __forceinline__ void adamw_moments(float g, float &m, float &v, float
     r = __fsqrt_rn(v);
 }
 
+typedef uint16_t halves_t __attribute__((ext_vector_type(2)));
+
 // Codes of a wavefront's block, four neighbours per lane (those behind the last element: zeros): m and r go in, the scale bytes
 // and a word of four codes each come out.
 __device__ __forceinline__ void encode_block(const float (&m)[4], const float (&r)[4], uint64_t element, const AdamwStep &k, int &sm, int &sr,
                                              uint32_t &cm, uint32_t &cr) {
-    uint32_t em = 8, er = 8;
+    // magnitudes by their bits: in the order of the numbers, infinities and what is not a number behind them
+    uint32_t mm = 0, rm = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) em = max(em, exponent_field(m[j])), er = max(er, exponent_field(r[j]));
+    for (int j = 0; j < 4; ++j) mm = max(mm, __float_as_uint(m[j]) & 0x7fffffffu), rm = max(rm, __float_as_uint(r[j]));
+    const bool plain = __all(max(mm, rm) < 0x7f800000u);
+    uint32_t both = mm >> 23 << 16 | rm >> 23;  // both exponent fields in the halves of one word: one exchange for the two maxima
+    if (!plain) {                               // what is not finite does not count
+        uint32_t em = 0, er = 0;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) em = max(em, (uint32_t)__shfl_xor((int)em, d)), er = max(er, (uint32_t)__shfl_xor((int)er, d));
-    sm = (int)em - 7, sr = (int)er - 7;
+        for (int j = 0; j < 4; ++j) em = max(em, exponent_field(m[j])), er = max(er, exponent_field(r[j]));
+        both = em << 16 | er;
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const uint32_t other = (uint32_t)__shfl_xor((int)both, d);
+        halves_t a, b;
+        __builtin_memcpy(&a, &both, 4), __builtin_memcpy(&b, &other, 4);
+        a = __builtin_elementwise_max(a, b);
+        __builtin_memcpy(&both, &a, 4);
+    }
+    sm = max((int)(both >> 16), 8) - 7, sr = max((int)(both & 0xffff), 8) - 7;
     uint32_t h[4];
     philox4x32_7(element >> 2, k.t, k.seed, h);
     cm = cr = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint32_t a = e4m3_code(fabsf(m[j]), sm, h[j] & 0xffff) | ((__float_as_uint(m[j]) >> 24) & 0x80u);
-        uint32_t b = e4m3_code(r[j], sr, h[j] >> 16);
-        if (b == 0 && r[j] > 0.0f) b = 1;
-        cm |= a << (8 * j), cr |= b << (8 * j);
+        uint32_t a = e4m3_code(fabsf(m[j]), sm, h[j] & 0xffff), b = e4m3_code(r[j], sr, h[j] >> 16);
+        b = max(b, min(__float_as_uint(r[j]), 1u));  // (above zero: the smallest code at least)
+        if (!plain) {
+            if (exponent_field(m[j]) == 0 && !(fabsf(m[j]) < 1.0f)) a = 0x7f;
+            if (exponent_field(r[j]) == 0 && !(r[j] < 1.0f)) b = 0x7f;
+        }
+        cm |= (a | ((__float_as_uint(m[j]) >> 24) & 0x80u)) << (8 * j), cr |= b << (8 * j);
     }
 }
 
@@ -166,7 +191,7 @@ __device__ __forceinline__ void adamw_block_any(const AdamwLaunch &a, const Adam
         if (e + j < it.n) {
             g[j] = gradient(a, it, e + j), w[j] = load_as_f32(it.w, e + j, it.type);
             if (BITS == 8) {
-                m[j] = e4m3_value(((const uint8_t *)it.m)[e + j], sm), v[j] = e4m3_value(((const uint8_t *)it.v)[e + j], sr);
+                m[j] = e4m3_value<0>(((const uint8_t *)it.m)[e + j], sm), v[j] = e4m3_value<0>(((const uint8_t *)it.v)[e + j], sr);
                 v[j] = __fmul_rn(v[j], v[j]);
             } else {
                 m[j] = ((const float *)it.m)[e + j], v[j] = ((const float *)it.v)[e + j];
@@ -177,7 +202,7 @@ __device__ __forceinline__ void adamw_block_any(const AdamwLaunch &a, const Adam
     for (int j = 0; j < 4; ++j)
         if (e + j < it.n) {
             adamw_moments(g[j], m[j], v[j], r[j], k);
-            store_f32_as(it.w, e + j, it.type, adamw_weight(w[j], m[j], r[j], it, k));
+            store_f32_as(it.w, e + j, it.type, adamw_clip(adamw_weight(w[j], m[j], r[j], it, k), it));
             if (BITS == 32) ((float *)it.m)[e + j] = m[j], ((float *)it.v)[e + j] = v[j];
         }
     if (BITS == 8) {
@@ -243,20 +268,27 @@ __device__ __forceinline__ void adamw_blocks(const AdamwItem &it, const AdamwSte
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        float mm[4], rr[4];
+        float mm[4], vv[4], rr[4], ww[4];
+        if (BITS == 32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mm[j] = m[n][j], vv[j] = v[n][j];
+        } else {
+            mm[0] = e4m3_value<0>(cm[n], sm[n]), mm[1] = e4m3_value<1>(cm[n], sm[n]), mm[2] = e4m3_value<2>(cm[n], sm[n]), mm[3] = e4m3_value<3>(cm[n], sm[n]);
+            vv[0] = e4m3_value<0>(cr[n], sr[n]), vv[1] = e4m3_value<1>(cr[n], sr[n]), vv[2] = e4m3_value<2>(cr[n], sr[n]), vv[3] = e4m3_value<3>(cr[n], sr[n]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vv[j] = __fmul_rn(vv[j], vv[j]);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float vv;
-            if (BITS == 32) {
-                mm[j] = m[n][j], vv = v[n][j];
-            } else {
-                mm[j] = e4m3_value((cm[n] >> (8 * j)) & 0xff, sm[n]), vv = e4m3_value((cr[n] >> (8 * j)) & 0xff, sr[n]);
-                vv = __fmul_rn(vv, vv);
-            }
-            adamw_moments(__fadd_rn((float)g[n][j], it.l1), mm[j], vv, rr[j], k);
-            w[n][j] = (T)adamw_weight((float)w[n][j], mm[j], rr[j], it, k);
-            m[n][j] = mm[j], v[n][j] = vv;
+            adamw_moments(__fadd_rn((float)g[n][j], it.l1), mm[j], vv[j], rr[j], k);
+            ww[j] = adamw_weight((float)w[n][j], mm[j], rr[j], it, k);
+            m[n][j] = mm[j], v[n][j] = vv[j];
         }
+        if (it.bounded)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ww[j] = adamw_clip(ww[j], it);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[n][j] = (T)ww[j];
         write<STREAM>((T *)it.w + e + 1024 * n, w[n]);
         if (BITS == 32) {
             write<STREAM>((float *)it.m + e + 1024 * n, m[n]), write<STREAM>((float *)it.v + e + 1024 * n, v[n]);
@@ -435,7 +467,7 @@ int for_launches(const hgq_adamw_item *items, int count, int chunk, F fn) {
             if (pieces + own > ADAMW_PIECES || (n > 0 && chunks + own_chunks > 0x7fffffffu)) break;
             AdamwItem &d = a.item[n];
             d.w = s.w, d.g = s.g, d.m = s.m, d.v = s.v, d.m_scale = s.m_scale, d.v_scale = s.v_scale, d.n = s.n, d.first = s.first;
-            d.l1 = s.l1, d.lo = s.lo, d.hi = s.hi, d.decay = s.decay, d.type = (short)s.type, d.piece = (short)pieces, d.pieces = (short)own;
+            d.l1 = s.l1, d.lo = s.lo, d.hi = s.hi, d.decay = s.decay, d.type = (char)s.type, d.bounded = !(s.lo == -INFINITY && s.hi == INFINITY), d.piece = (short)pieces, d.pieces = (short)own;
             const uintptr_t size = s.type == HGQ_TYPE_F32 ? 4 : 2, moment = s.m_scale ? 1 : 4;
             d.vec = own == 0 && (((uintptr_t)s.w | (uintptr_t)s.g) & (4 * size - 1)) == 0 && (((uintptr_t)s.m | (uintptr_t)s.v) & (4 * moment - 1)) == 0;
             for (int k = 0; k < HGQ_SGD_SIDES; ++k)

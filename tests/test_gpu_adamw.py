@@ -4,7 +4,7 @@ Tolerances follow the arithmetic of one step from exact inputs, u = 2^-24 (half 
 most 2 u (the norm's rounding and the division's), so the gradient by 3 u.  m: the gradient and three roundings of the difference, times
 1 - beta_1, and one of the sum: 6 u (1 - beta_1) (|g| + |m|) + u |m'|.  v: g g is off by 7 u, then the same: 10 u (1 - beta_2) (g^2 + v) +
 u v'.  The step m alpha / (r + eps): what m and half of what v are off
-by, relatively, and six roundings (root, sum, alpha, product, quotient, conversion).  w: that, and three roundings of w; a 16-bit
+by, relatively, and seven roundings: root, sum, alpha and two products u each, the reciprocal a unit in the last place, 2 u.  w: that, and three roundings of w; a 16-bit
 type adds half a step of its own."""
 
 import math
@@ -52,7 +52,7 @@ def _plain(w, g, m, v, t, lr=0.001, b1=0.9, b2=0.999, eps=1e-7, decay=0.004, c=1
     r = v.sqrt()
     step = m * alpha / (r + eps)
     new = w * (1 - lr * decay) - step
-    tw = 3 * U * w.abs() + alpha * tm / (r + eps) + step.abs() * (tv / (2 * v).clamp(min=1e-300) + 6 * U)
+    tw = 3 * U * w.abs() + alpha * tm / (r + eps) + step.abs() * (tv / (2 * v).clamp(min=1e-300) + 7 * U)
     tw = torch.where(v == 0, 3 * U * w.abs(), tw)
     return new.clamp(lo, hi), m, v, tw, tm, tv
 
