@@ -154,6 +154,8 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 };
 
 Tensor group_norm(const Tensor &x, int64_t groups, const std::optional<Tensor> &gamma, const std::optional<Tensor> &beta, double epsilon, int64_t act) {
+    for (const auto &[name, t] : {std::make_pair("gamma", &gamma), std::make_pair("beta", &beta)})
+        TORCH_CHECK_VALUE(!*t || ((*t)->dim() == 1 && x.dim() >= 1 && (*t)->numel() == x.size(-1)), name, " must be a vector with an element per channel");
     const Tensor none = gamma && beta ? Tensor() : at::empty({0}, x.options().dtype(at::kFloat).requires_grad(false));
     return GroupNorm::apply(x.contiguous(), gamma ? *gamma : none, beta ? *beta : none, groups, epsilon, act);
 }
@@ -286,22 +288,26 @@ public:
               const py::list &terms, const py::handle &sum_out) {
         HANDLE_TH_ERRORS
         const Tensor &st = THPVariable_Unpack(state.ptr());
-        const c10::DeviceGuard guard(device_);
-        void *stream = stream_of(st);
-        Tensor parts;
-        int64_t n = 0;
-        if (clipnorm > 0 && (n = library().global_norm_parts(items_.data(), (int)items_.size())) > 0) {
-            parts = workspace(n, st, at::kDouble);  // this call's own: in a captured step it belongs to that graph
-            check(lib.global_norm(items_.data(), (int)items_.size(), parts.data_ptr<double>(), nullptr, stream), "hgq_global_norm");
-        }
         const float *ptrs[HGQ_SUM_BATCH];
         TORCH_CHECK_VALUE(terms.size() <= HGQ_SUM_BATCH, "at most ", HGQ_SUM_BATCH, " terms ride along with the update");
         for (size_t t = 0; t < terms.size(); ++t) ptrs[t] = scalar(terms[t], "every term");
-        check(library().adamw_update_multi(items_.data(), (int)items_.size(), bits_, (hgq_adamw_state *)st.data_ptr(), beta_1, beta_2, (float)epsilon,
-                                     n > 0 ? (float)clipnorm : 0.0f, n > 0 ? parts.data_ptr<double>() : nullptr, n,
-                                     norm_out.is_none() ? nullptr : scalar(norm_out, "norm_out"), seed, ptrs, (int)terms.size(),
-                                     terms.size() ? scalar(sum_out, "sum_out") : nullptr, stream),
-              "hgq_adamw_update_multi");
+        float *norm = norm_out.is_none() ? nullptr : scalar(norm_out, "norm_out"), *sum = terms.size() ? scalar(sum_out, "sum_out") : nullptr;
+        const int n_terms = (int)terms.size(), count = (int)items_.size();
+        {
+            const py::gil_scoped_release others;
+            const c10::DeviceGuard guard(device_);
+            void *stream = stream_of(st);
+            Tensor parts;
+            int64_t n = 0;
+            if (clipnorm > 0 && (n = library().global_norm_parts(items_.data(), count)) > 0) {
+                parts = workspace(n, st, at::kDouble);  // this call's own: in a captured step it belongs to that graph
+                check(lib.global_norm(items_.data(), count, parts.data_ptr<double>(), nullptr, stream), "hgq_global_norm");
+            }
+            check(library().adamw_update_multi(items_.data(), count, bits_, (hgq_adamw_state *)st.data_ptr(), beta_1, beta_2, (float)epsilon,
+                                               n > 0 ? (float)clipnorm : 0.0f, n > 0 ? parts.data_ptr<double>() : nullptr, n, norm, seed, ptrs, n_terms, sum,
+                                               stream),
+                  "hgq_adamw_update_multi");
+        }
         held_.clear();  // (the allocator hands this memory to later work of the same stream only)
         END_HANDLE_TH_ERRORS_PYBIND
     }
@@ -370,7 +376,13 @@ PYBIND11_MODULE(_host, m) {
         std::optional<Tensor> ga, be;
         if (!gamma.is_none()) ga = tensor_of(gamma, "gamma");
         if (!beta.is_none()) be = tensor_of(beta, "beta");
-        return py::reinterpret_steal<py::object>(THPVariable_Wrap(group_norm(tensor_of(x, "x"), groups, ga, be, epsilon, act)));
+        const Tensor input = tensor_of(x, "x");
+        Tensor y;
+        {
+            const py::gil_scoped_release others;
+            y = group_norm(input, groups, ga, be, epsilon, act);
+        }
+        return py::reinterpret_steal<py::object>(THPVariable_Wrap(y));
         END_HANDLE_TH_ERRORS_PYBIND
     });
     m.def("global_norm", [](const py::sequence &tensors) {
@@ -381,8 +393,13 @@ PYBIND11_MODULE(_host, m) {
             if (!t.is_none()) list.push_back(tensor_of(t, "every entry"));
         static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::global_norm", "").typed<Tensor(at::TensorList)>();
         TORCH_CHECK_VALUE(!list.empty(), "at least one tensor is expected");
-        at::AutoDispatchBelowADInplaceOrView below;  // (a number: not differentiable)
-        return py::reinterpret_steal<py::object>(THPVariable_Wrap(op.call(list)));
+        Tensor norm;
+        {
+            const py::gil_scoped_release others;
+            at::AutoDispatchBelowADInplaceOrView below;  // (a number: not differentiable)
+            norm = op.call(list);
+        }
+        return py::reinterpret_steal<py::object>(THPVariable_Wrap(norm));
         END_HANDLE_TH_ERRORS_PYBIND
     });
     py::class_<AdamwVariables>(m, "AdamwVariables")

@@ -3532,7 +3532,8 @@ def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: flo
     to this global norm; a norm that is not finite makes every variable not a number.  :class:`hgq2_amd.train.AdamW` is this with
     the moments, regularizers and constraints of a model's variables."""
     n, inf = len(ws), float('inf')
-    _need(len(moments) == n and n >= 1, 'per-variable lists differ in length')
+    _need(n >= 1 and len(gs) == n and len(moments) == n, 'per-variable lists differ in length')
+    _need(all(g is not None for g in gs), 'every variable needs a gradient')
     _need(clipnorm is None or clipnorm > 0, 'clipnorm must be positive')
     bits = 32 if len(moments[0]) == 2 else 8
     each = lambda v, d: [d] * n if v is None else [float(k) for k in v]  # noqa: E731

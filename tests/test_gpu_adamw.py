@@ -444,3 +444,68 @@ def test_fit_with_adamw(dev):
     assert len(made) == 1 and made[0].iterations == 16  # 8 batches an epoch, the last one shorter
     hist = fit(_model(dev), x, y, batch_size=500, epochs=1, lr=0.001, optimizer='adamw', seed=1)
     assert math.isfinite(hist[0]['loss'])
+
+
+def test_what_the_class_refuses(dev):
+    from hgq2_amd.train import AdamW
+
+    p = torch.nn.Parameter(torch.ones(10, device=dev))
+    with pytest.raises(ValueError, match='twice'):
+        AdamW([p, p])
+    with pytest.raises(ValueError, match='float32'):
+        AdamW([torch.nn.Parameter(torch.ones(3, device=dev, dtype=torch.float64))])
+    with pytest.raises(ValueError, match='one device'):
+        AdamW([p, torch.nn.Parameter(torch.ones(3))])
+    for data in (torch.ones(9, device=dev), torch.ones(10, device=dev, dtype=torch.bfloat16), torch.ones(10), torch.ones(20, device=dev)[::2]):
+        q = torch.nn.Parameter(torch.ones(10, device=dev))
+        opt = AdamW([q])
+        q.data = data
+        q.grad = torch.ones_like(q)
+        before = q.detach().clone()
+        with pytest.raises(ValueError, match='stay contiguous'):
+            opt.step()
+        assert torch.equal(q, before) and opt.iterations == 0
+    q = torch.nn.Parameter(torch.ones(10, device=dev))
+    opt = AdamW([q])
+    q._hgq_side = [(None, torch.ones(9, device=dev))]
+    with pytest.raises(ValueError, match='side gradient'):
+        opt.step()
+    with pytest.raises(AttributeError, match='32 bits'):
+        opt.velocity_root
+    with pytest.raises(AttributeError, match='8 bits'):
+        AdamW([q], state_bits=8).velocity
+
+
+def test_streams_and_a_sparse_gradient(dev):
+    """Two optimizers that step on two streams at once do what they do one after the other; a sparse gradient is refused."""
+    from hgq2_amd.train import AdamW
+
+    gen = torch.Generator().manual_seed(14)
+    data = [(torch.randn(200_000, generator=gen).to(dev), torch.randn(200_000, generator=gen).to(dev)) for _ in range(2)]
+
+    def make():
+        out = []
+        for w, g in data:
+            p = torch.nn.Parameter(w.clone())
+            p.grad = g
+            out.append((p, AdamW([p], global_clipnorm=1.0, state_bits=8, seed=2)))
+        return out
+
+    one, two = make(), make()
+    for _ in range(4):
+        for _, opt in one:
+            opt.step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in two]
+    for _ in range(4):
+        for (_, opt), s in zip(two, streams):
+            with torch.cuda.stream(s):
+                opt.step()
+    torch.cuda.synchronize()
+    for (a, x), (b, y) in zip(one, two):
+        assert torch.equal(a, b) and torch.equal(x.momentum.view(torch.uint8), y.momentum.view(torch.uint8)) and torch.equal(x.grad_norm, y.grad_norm)
+    p = torch.nn.Parameter(torch.ones(4, 3, device=dev))
+    opt = AdamW([p])
+    p.grad = torch.sparse_coo_tensor(torch.tensor([[1]]), torch.ones(1, 3), (4, 3)).to(dev)
+    with pytest.raises(ValueError, match='dense'):
+        opt.step()

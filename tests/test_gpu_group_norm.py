@@ -361,3 +361,52 @@ def test_more_than_the_cache_holds(dev, shape, G, dtype, act):
             sums[k], tols[k] = sums[k] + want[2 + k], tols[k] + tol[2 + k]
     _check(dgamma, sums[0], tols[0], torch.float32, 'dgamma')
     _check(dbeta, sums[1], tols[1], torch.float32, 'dbeta')
+
+
+def test_what_is_refused_on_the_gpu(dev):
+    from hgq2_amd import ops
+
+    x = torch.randn(2, 5, 8, device=dev)
+    one = torch.ones(8, device=dev)
+    for kw in (dict(groups=3), dict(groups=0), dict(groups=-1), dict(groups=16)):
+        with pytest.raises(ValueError, match='groups of one size'):
+            ops.group_norm(x, **kw)
+    for gamma in (one[:4], one.view(1, 8), torch.empty(0, device=dev), one.cpu(), one.double(), one.bfloat16(), torch.ones(16, device=dev)[::2]):
+        with pytest.raises(ValueError, match='gamma'):
+            ops.group_norm(x, 2, gamma)
+        with pytest.raises(ValueError, match='beta'):
+            ops.group_norm(x, 2, one, gamma)
+    with pytest.raises(ValueError, match='float32'):
+        ops.group_norm(x.double(), 2)
+    with pytest.raises(ValueError, match='batch'):
+        ops.group_norm(one, 2)
+    y, stats = torch.ops.hgq.group_norm_fwd(x, one, one, 2, 1e-3, 0)
+    for args in ((x[:1], x, one, one, stats), (x.bfloat16(), x, one, one, stats), (x, x, one, one, stats[:1]), (x.transpose(0, 1), x, one, one, stats)):
+        with pytest.raises(ValueError):
+            torch.ops.hgq.group_norm_bwd(*args, 2, 0, True, True, True)
+
+
+def test_two_backward_passes_and_another_stream(dev):
+    from hgq2_amd import ops
+
+    g = torch.Generator().manual_seed(10)
+    x = torch.randn(40, 300, 64, generator=g).to(dev).requires_grad_(True)
+    gamma = torch.randn(64, generator=g).to(dev).requires_grad_(True)
+    dy = torch.randn(40, 300, 64, generator=g).to(dev)
+    y = ops.group_norm(x, 8, gamma, activation='silu')
+    first = torch.autograd.grad(y, [x, gamma], dy, retain_graph=True)
+    again = torch.autograd.grad(y, [x, gamma], dy)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        z = ops.group_norm(x, 8, gamma, activation='silu')
+        there = torch.autograd.grad(z, [x, gamma], dy)
+    s.synchronize()
+    assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(first, there))
+    with pytest.raises(RuntimeError, match='modified'):
+        w = torch.randn(2, 5, 8, device=dev, requires_grad=True)
+        v = w * 1.0
+        out = ops.group_norm(v, 2)
+        v.add_(1.0)
+        out.sum().backward()
