@@ -543,8 +543,8 @@ extern "C" int hgq_adamw_update_multi(const hgq_adamw_item *items, int count, in
     int rc = check_items("hgq_adamw_update_multi", items, count, state_bits);
     if (rc) return rc;
     if (!state) return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: null state");
-    if (!(beta_1 >= 0 && beta_1 < 1 && beta_2 >= 0 && beta_2 < 1 && epsilon >= 0))
-        return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: 0 <= beta < 1 and epsilon >= 0 are expected");
+    if (!(beta_1 >= 0 && beta_1 < 1 && beta_2 >= 0 && beta_2 < 1 && (epsilon == 0 || epsilon >= 0x1p-126f)))
+        return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: 0 <= beta < 1 and an epsilon of 0 or at least 2^-126 are expected");
     if (n_parts < 0 || n_parts > 0x7fffffff || (n_parts > 0 && (!norm_parts || !(clipnorm > 0))))
         return fail(HGQ_ERR_ARG, "hgq_adamw_update_multi: a positive clipnorm and the parts of the norm go together");
     if (n_terms < 0 || n_terms > HGQ_SUM_BATCH || (n_terms > 0 && (!terms || !sum_out)))

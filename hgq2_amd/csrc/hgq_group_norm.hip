@@ -72,75 +72,79 @@ __device__ __forceinline__ double group_sum(double v, double *lds) {
     return v;
 }
 
-// One workgroup per sample and group, any shape: the group is read three times, its sums are formed in fp64.
+// A workgroup takes one sample's group after another, any shape: the group is read three times, its sums are formed in fp64.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void group_norm_fwd_any(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
                                                           T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, GroupShape s) {
     __shared__ double lds[4];
-    const int64_t b = blockIdx.x / s.G;
-    const int g = (int)(blockIdx.x % s.G);
-    const int64_t base = b * s.S * s.C + (int64_t)g * s.D, n = s.S * s.D;
-    double sum = 0;
-    for (int64_t e = threadIdx.x; e < n; e += 256) sum += to_f32(x[base + e / s.D * s.C + e % s.D]);
-    const float mean = (float)(group_sum(sum, lds) / (double)n);
-    double sq = 0;
-    for (int64_t e = threadIdx.x; e < n; e += 256) {
-        const float d = to_f32(x[base + e / s.D * s.C + e % s.D]) - mean;
-        sq += (double)d * d;
-    }
-    const float rstd = 1.0f / sqrtf((float)(group_sum(sq, lds) / (double)n) + s.eps);
-    if (threadIdx.x == 0) mean_out[blockIdx.x] = mean, rstd_out[blockIdx.x] = rstd;
-    for (int64_t e = threadIdx.x; e < n; e += 256) {
-        const int c = g * s.D + (int)(e % s.D);
-        const int64_t at = base + e / s.D * s.C + e % s.D;
-        const float ga = gamma ? gamma[c] : 1.0f, z = affine<ACT>(to_f32(x[at]) - mean, rstd, ga, rstd * ga, beta ? beta[c] : 0.0f);
-        y[at] = (T)activate<ACT>(z);
+    for (int64_t bg = blockIdx.x; bg < s.B * s.G; bg += gridDim.x) {
+        const int64_t b = bg / s.G;
+        const int g = (int)(bg - b * s.G);
+        const int64_t base = b * s.S * s.C + (int64_t)g * s.D, n = s.S * s.D;
+        double sum = 0;
+        for (int64_t e = threadIdx.x; e < n; e += 256) sum += to_f32(x[base + e / s.D * s.C + e % s.D]);
+        const float mean = (float)(group_sum(sum, lds) / (double)n);
+        double sq = 0;
+        for (int64_t e = threadIdx.x; e < n; e += 256) {
+            const float d = to_f32(x[base + e / s.D * s.C + e % s.D]) - mean;
+            sq += (double)d * d;
+        }
+        const float rstd = 1.0f / sqrtf((float)(group_sum(sq, lds) / (double)n) + s.eps);
+        if (threadIdx.x == 0) mean_out[bg] = mean, rstd_out[bg] = rstd;
+        for (int64_t e = threadIdx.x; e < n; e += 256) {
+            const int c = g * s.D + (int)(e % s.D);
+            const int64_t at = base + e / s.D * s.C + e % s.D;
+            const float ga = gamma ? gamma[c] : 1.0f, z = affine<ACT>(to_f32(x[at]) - mean, rstd, ga, rstd * ga, beta ? beta[c] : 0.0f);
+            y[at] = (T)activate<ACT>(z);
+        }
     }
 }
 
-// One workgroup per sample and group, any shape.  part [B][2 C]: each sample's terms of dgamma, then of dbeta.
+// A workgroup takes one sample's group after another, any shape.  part [B][2 C]: each sample's terms of dgamma, then of dbeta.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ gamma,
                                                           const float *__restrict__ beta, const float *__restrict__ mean_in,
                                                           const float *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ part, GroupShape s) {
     __shared__ double lds[4];
     __shared__ double col[2][256];
-    const int64_t b = blockIdx.x / s.G;
-    const int g = (int)(blockIdx.x % s.G);
-    const int64_t base = b * s.S * s.C + (int64_t)g * s.D, n = s.S * s.D;
-    const float mean = mean_in[blockIdx.x], rstd = rstd_in[blockIdx.x];
     int tx = 1;  // threads side by side over channels, the others over positions
     while (tx < s.D && tx < 256) tx *= 2;
     const int ty = 256 / tx, cx = threadIdx.x % tx, py = threadIdx.x / tx;
-    double s1 = 0, s2 = 0;  // of d and d xhat, over the group
-    for (int c0 = 0; c0 < s.D; c0 += tx) {
-        const int d = c0 + cx, c = g * s.D + d;
-        double a = 0, h = 0;
-        const float ga = d < s.D && gamma ? gamma[c] : 1.0f, be = d < s.D && beta ? beta[c] : 0.0f;
-        if (d < s.D)
-            for (int64_t p = py; p < s.S; p += ty) {
-                const int64_t at = base + p * s.C + d;
-                const float xh = (to_f32(x[at]) - mean) * rstd;
-                const float dz = through_activation<ACT>(to_f32(dy[at]), xh * ga + be);
-                a += dz, h += (double)dz * xh;
+    for (int64_t bg = blockIdx.x; bg < s.B * s.G; bg += gridDim.x) {
+        const int64_t b = bg / s.G;
+        const int g = (int)(bg - b * s.G);
+        const int64_t base = b * s.S * s.C + (int64_t)g * s.D, n = s.S * s.D;
+        const float mean = mean_in[bg], rstd = rstd_in[bg];
+        double s1 = 0, s2 = 0;  // of d and d xhat, over the group
+        for (int c0 = 0; c0 < s.D; c0 += tx) {
+            const int d = c0 + cx, c = g * s.D + d;
+            double a = 0, h = 0;
+            const float ga = d < s.D && gamma ? gamma[c] : 1.0f, be = d < s.D && beta ? beta[c] : 0.0f;
+            if (d < s.D)
+                for (int64_t p = py; p < s.S; p += ty) {
+                    const int64_t at = base + p * s.C + d;
+                    const float xh = (to_f32(x[at]) - mean) * rstd;
+                    const float dz = through_activation<ACT>(to_f32(dy[at]), xh * ga + be);
+                    a += dz, h += (double)dz * xh;
+                }
+            s1 += a * ga, s2 += h * ga;
+            col[0][threadIdx.x] = h, col[1][threadIdx.x] = a;
+            __syncthreads();
+            if (py == 0 && d < s.D && part) {
+                for (int r = 1; r < ty; ++r) h += col[0][r * tx + cx], a += col[1][r * tx + cx];
+                part[b * 2 * s.C + c] = (float)h, part[b * 2 * s.C + s.C + c] = (float)a;
             }
-        s1 += a * ga, s2 += h * ga;
-        col[0][threadIdx.x] = h, col[1][threadIdx.x] = a;
-        __syncthreads();
-        if (py == 0 && d < s.D && part) {
-            for (int r = 1; r < ty; ++r) h += col[0][r * tx + cx], a += col[1][r * tx + cx];
-            part[b * 2 * s.C + c] = (float)h, part[b * 2 * s.C + s.C + c] = (float)a;
+            __syncthreads();
         }
-        __syncthreads();
-    }
-    const float m1 = (float)(group_sum(s1, lds) / (double)n), m2 = (float)(group_sum(s2, lds) / (double)n);
-    if (!dx) return;
-    for (int64_t e = threadIdx.x; e < n; e += 256) {
-        const int c = g * s.D + (int)(e % s.D);
-        const int64_t at = base + e / s.D * s.C + e % s.D;
-        const float ga = gamma ? gamma[c] : 1.0f, xh = (to_f32(x[at]) - mean) * rstd;
-        const float dz = through_activation<ACT>(to_f32(dy[at]), xh * ga + (beta ? beta[c] : 0.0f));
-        dx[at] = (T)((dz * ga - m1 - xh * m2) * rstd);
+        const float m1 = (float)(group_sum(s1, lds) / (double)n), m2 = (float)(group_sum(s2, lds) / (double)n);
+        if (!dx) continue;
+        for (int64_t e = threadIdx.x; e < n; e += 256) {
+            const int c = g * s.D + (int)(e % s.D);
+            const int64_t at = base + e / s.D * s.C + e % s.D;
+            const float ga = gamma ? gamma[c] : 1.0f, xh = (to_f32(x[at]) - mean) * rstd;
+            const float dz = through_activation<ACT>(to_f32(dy[at]), xh * ga + (beta ? beta[c] : 0.0f));
+            dx[at] = (T)((dz * ga - m1 - xh * m2) * rstd);
+        }
     }
 }
 
@@ -607,7 +611,7 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     p.team = 1;
     while (p.team < 64 && p.team * 2 * p.NS * p.K <= threads) p.team *= 2;
     const int64_t tiles = (B + p.NS - 1) / p.NS * p.splits;
-    if (tiles > 65535 * (int64_t)SLICE_RUN || tiles * p.chunks > 0x7fffffff / 16) return false;
+    if (tiles > 65535 * (int64_t)SLICE_RUN || (tiles + 7) * p.chunks * threads > 0xffffffff) return false;  // (a launch has less than 2^32 threads)
     p.tiles = (int)tiles;
     // What a pass reads and writes against the card's 256 MB cache, and rows of whole lines: 48 x 64 x 64 x 512 bfloat16, forward 131 -> 110 us,
     // backward 206 -> 196 us; 1024 x 26 x 26 x 32 fp32, backward 67 -> 58 us.  Half lines are slower that way (64 x 32 x 32 x 256 fp32 in
@@ -624,6 +628,8 @@ int64_t parts_floats(const GroupTile &p) { return p.splits > 1 ? p.B * p.splits 
 int lds_bytes(const GroupTile &p, int threads, bool backward) {
     return 4 * (2 * p.NS * p.K + threads * (p.D % 4 == 0 && !backward ? 1 : 4));
 }
+
+unsigned any_grid(const GroupShape &s) { return (unsigned)(s.B * s.G < 1 << 20 ? s.B * s.G : 1 << 20); }
 
 unsigned blocks(const GroupTile &p) { return (unsigned)(((int64_t)p.tiles + 7) / 8 * 8 * p.chunks); }
 
@@ -643,7 +649,7 @@ int fwd(const void *x, const float *gamma, const float *beta, void *y, float *me
     GroupTile p;
     int held, threads;
     if (!plan(p, held, threads, s.B, s.S, s.C, s.G, type, false)) {
-        hipLaunchKernelGGL((group_norm_fwd_any<T, ACT>), dim3((unsigned)(s.B * s.G)), dim3(256), 0, st, (const T *)x, gamma, beta, (T *)y, mean, rstd, s);
+        hipLaunchKernelGGL((group_norm_fwd_any<T, ACT>), dim3(any_grid(s)), dim3(256), 0, st, (const T *)x, gamma, beta, (T *)y, mean, rstd, s);
         return check_launch("hgq_group_norm_fwd");
     }
     p.eps = s.eps;
@@ -664,7 +670,7 @@ int bwd(const void *dy, const void *x, const float *gamma, const float *beta, co
     GroupTile p;
     int held, threads;
     if (!plan(p, held, threads, s.B, s.S, s.C, s.G, type, true)) {
-        hipLaunchKernelGGL((group_norm_bwd_any<T, ACT>), dim3((unsigned)(s.B * s.G)), dim3(256), 0, st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd, (T *)dx,
+        hipLaunchKernelGGL((group_norm_bwd_any<T, ACT>), dim3(any_grid(s)), dim3(256), 0, st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd, (T *)dx,
                            sums ? ws : nullptr, s);
         const int rc = check_launch("hgq_group_norm_bwd");
         if (rc || !sums) return rc;

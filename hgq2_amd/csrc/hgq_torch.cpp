@@ -4,6 +4,7 @@
 // called through the C ABI of libhgq_hip.so (bind()), outputs and workspaces are torch tensors on the current stream of their device.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
@@ -153,9 +154,26 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     }
 };
 
+// A recorded backward pass hands the gradient of a leaf to the leaf's one accumulating node, on the stream that the node was made on.  One that
+// an earlier graph made on another stream, and keeps alive, would pull that stream into the recording, which ends the process.
+void accumulates_here(const char *name, const Tensor &t) {
+    if (!t.defined() || !t.requires_grad() || t.grad_fn()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (!stream || stream->id() == c10::hip::getCurrentHIPStream(t.device().index()).id()) return;
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, name,
+                " belongs to a graph of another stream that is still alive: its backward pass cannot be recorded here (release what that graph gave, or "
+                "make it on this stream)");
+}
+
 Tensor group_norm(const Tensor &x, int64_t groups, const std::optional<Tensor> &gamma, const std::optional<Tensor> &beta, double epsilon, int64_t act) {
     for (const auto &[name, t] : {std::make_pair("gamma", &gamma), std::make_pair("beta", &beta)})
         TORCH_CHECK_VALUE(!*t || ((*t)->dim() == 1 && x.dim() >= 1 && (*t)->numel() == x.size(-1)), name, " must be a vector with an element per channel");
+    if (at::GradMode::is_enabled()) {
+        accumulates_here("x", x);
+        if (gamma) accumulates_here("gamma", *gamma);
+        if (beta) accumulates_here("beta", *beta);
+    }
     const Tensor none = gamma && beta ? Tensor() : at::empty({0}, x.options().dtype(at::kFloat).requires_grad(false));
     return GroupNorm::apply(x.contiguous(), gamma ? *gamma : none, beta ? *beta : none, groups, epsilon, act);
 }
@@ -189,7 +207,7 @@ constexpr float INF = std::numeric_limits<float>::infinity();
 // The descriptors of an optimizer's variables: moments, place and type once; variable, gradient and limits at every step.
 class AdamwVariables {
 public:
-    AdamwVariables(const py::list &params, const py::list &moments, int state_bits) : params_(params), bits_(state_bits) {
+    AdamwVariables(const py::sequence &params, const py::list &moments, int state_bits) : params_(params), bits_(state_bits) {  // (a copy of the list)
         for (const auto &m : moments) moments_.push_back(THPVariable_Unpack(m.ptr()));
         int64_t at = 0;
         for (const auto &p : params) {
@@ -223,7 +241,7 @@ public:
         bool any = false;
         for (size_t k = 0; k < items_.size(); ++k) {
             hgq_adamw_item &it = items_[k];
-            PyObject *p = PyList_GET_ITEM(params_.ptr(), (Py_ssize_t)k);
+            PyObject *p = PyTuple_GET_ITEM(params_.ptr(), (Py_ssize_t)k);
             const Tensor &t = THPVariable_Unpack(p);
             const Tensor &g = t.grad();
             PyObject **dict = _PyObject_GetDictPtr(p);
@@ -319,7 +337,7 @@ private:
         return t.data_ptr<float>();
     }
 
-    py::list params_;
+    const py::tuple params_;
     std::vector<Tensor> moments_, held_;
     std::vector<hgq_adamw_item> items_;
     std::vector<int64_t> sizes_;
@@ -403,7 +421,7 @@ PYBIND11_MODULE(_host, m) {
         END_HANDLE_TH_ERRORS_PYBIND
     });
     py::class_<AdamwVariables>(m, "AdamwVariables")
-        .def(py::init<const py::list &, const py::list &, int>())
+        .def(py::init<const py::sequence &, const py::list &, int>())
         .def("set_decay", &AdamwVariables::set_decay)
         .def("gather", &AdamwVariables::gather)
         .def("limits", &AdamwVariables::limits)

@@ -3415,6 +3415,14 @@ def _check_gradient(name: str, t: Tensor, device, dtype, numel: int):
     _need(t.numel() == numel, f'{name} has {t.numel()} elements, not {numel}')
 
 
+def _need_apart(what: str, tensors):
+    """The elements of contiguous tensors must not share memory: two threads would write them at once."""
+    end = -1
+    for start, size in sorted((t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel()):
+        _need(start >= end, f'{what} share memory')
+        end = start + size
+
+
 class _device_of:
     """Launches go to the current stream of the device that the tensors are on, whichever device is the current one: ``with
     _device_of(device) as stream``."""
@@ -3516,6 +3524,7 @@ def adamw_update_multi_op(ws: Sequence[Tensor], gs: Sequence[Tensor], moments: S
         words += (w.data_ptr(), g.data_ptr(), *((p[0], p[1], 0, 0) if per == 2 else (p[0], p[2], p[1], p[3])), num, first,
                   *_adamw_limits_words(l1[t], lo[t], hi[t], decay[t]), code, *_NO_SIDES)
         first += -(-num // ADAMW_BLOCK) * ADAMW_BLOCK
+    _need_apart('variables', ws), _need_apart('moments', moments)
     if norm_out.numel():
         _check_f32('norm_out', norm_out)
         _need(norm_out.numel() == 1 and norm_out.device == device, 'norm_out is one float32')

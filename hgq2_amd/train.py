@@ -149,7 +149,8 @@ class AdamW(SGD):
     The number of steps and the learning rate live in device memory: a step recorded in a HIP graph (:class:`GraphedTrainStep`)
     counts on at every replay, and setting ``lr`` between replays takes effect in the next one.  The moments of all variables lie in
     one buffer each (``momentum`` and ``velocity``, or ``momentum``, ``momentum_scale``, ``velocity_root`` and ``velocity_scale``), every
-    variable at a multiple of 256 elements (``offsets``).  Variables must stay contiguous, on their device, and of their size and type."""
+    variable at a multiple of 256 elements (``offsets``).  Variables must stay contiguous, apart from each other, on their device, and of
+    their size and type."""
 
     def __init__(self, params, lr: float = 0.001, weight_decay: float = 0.004, beta_1: float = 0.9, beta_2: float = 0.999,
                  epsilon: float = 1e-7, global_clipnorm: float | None = None, state_bits: int = 32, seed: int = 0,
@@ -161,6 +162,8 @@ class AdamW(SGD):
             raise ValueError(f'moments have 8 or 32 bits, not {state_bits}')
         if not (0 <= beta_1 < 1 and 0 <= beta_2 < 1 and epsilon >= 0 and weight_decay >= 0):
             raise ValueError('0 <= beta < 1, epsilon >= 0 and weight_decay >= 0 are expected')
+        if 0 < epsilon < 2.0**-126:
+            raise ValueError('an epsilon below 2^-126, the smallest normal float32, is not zero and not one either')
         if global_clipnorm is not None and not global_clipnorm > 0:
             raise ValueError('global_clipnorm must be positive')
         self.device = self.params[0].device
@@ -173,7 +176,8 @@ class AdamW(SGD):
                 raise ValueError(f'variables must be on one device, got {self.device} and {p.device}')
         if len(self._owner_ids) != len(self.params):
             raise ValueError('a variable is listed twice')
-        self.weight_decay, self.beta_1, self.beta_2 = float(weight_decay), float(beta_1), float(beta_2)
+        ops._need_apart('variables', self.params)
+        self.beta_1, self.beta_2 = float(beta_1), float(beta_2)
         self.epsilon, self.global_clipnorm = float(epsilon), None if global_clipnorm is None else float(global_clipnorm)
         self.state_bits, self.seed = int(state_bits), int(seed) & (2**63 - 1)
         self.offsets, n = [], 0  # where each variable's moments begin
@@ -186,8 +190,8 @@ class AdamW(SGD):
         else:
             self._names = ('momentum', 'momentum_scale', 'velocity_root', 'velocity_scale')
         self._variables = _lib.native().AdamwVariables(list(self.params), self._moments, self.state_bits)
-        for k in range(len(self.params)):
-            self._variables.set_decay(k, self.weight_decay)
+        self._not_decayed = set()
+        self.weight_decay = weight_decay
         self.grad_norm = torch.zeros((), dtype=torch.float32, device=self.device) if self.global_clipnorm is not None else None
         self._state = ops.adamw_state(self.device, lr, 0, self.beta_1, self.beta_2)
         self.lr = lr
@@ -219,6 +223,18 @@ class AdamW(SGD):
             state[3:4].view(torch.float64).fill_(self._lr)
 
     @property
+    def weight_decay(self):
+        return self._weight_decay
+
+    @weight_decay.setter
+    def weight_decay(self, value):  # (a recorded step keeps the one it was recorded with)
+        if not value >= 0:
+            raise ValueError('weight_decay must not be negative')
+        self._weight_decay = float(value)
+        for k in range(len(self.params)):
+            self._variables.set_decay(k, 0.0 if k in self._not_decayed else self._weight_decay)
+
+    @property
     def iterations(self) -> int:
         """Steps done, replayed ones included (waits for the GPU)."""
         return int(self._state[0])
@@ -229,6 +245,7 @@ class AdamW(SGD):
         names = tuple(var_names or ())
         for k, p in enumerate(self.params):
             if id(p) in ids or any(n in (getattr(p, 'var_name', None) or '') for n in names):
+                self._not_decayed.add(k)
                 self._variables.set_decay(k, 0.0)
 
     def state_dict(self) -> dict:
@@ -693,7 +710,7 @@ def fit(model, x, y, *, loss: str = 'sparse_ce', lr: float = 0.01, batch_size: i
             else:
                 total += step.eager(bx, by).reshape(())
         logs['loss'] = float(total) / (n_full + (1 if tail else 0))
-        if not isinstance(step, _FusedStep):
+        if not isinstance(step, _FusedStep) and step.opt.fold_regularizers:
             logs['loss'] += folded_regularizer_loss(model)
         for cb in callbacks:
             cb.on_epoch_end(epoch, logs)

@@ -149,3 +149,16 @@ def test_operators_without_data():
         torch.ops.hgq.group_norm_fwd(z, z[0, 0], z[0, 0], 4, 1e-3, 0)
     with pytest.raises(TypeError, match='tensor'):
         ops.group_norm(3.0, 4)
+
+
+def test_an_epsilon_that_is_no_normal_number_and_memory_that_is_shared():
+    p = torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(ValueError, match='2\\^-126'):
+        AdamW([p], epsilon=1e-40)
+    assert _update(_item(), eps=1e-40) == _lib.ERR_ARG
+    buf = torch.zeros(10)
+    ops._need_apart('variables', [buf[5:], buf[:5], buf[3:3]])
+    with pytest.raises(ValueError, match='variables share memory'):
+        ops._need_apart('variables', [buf[4:], buf[:5]])
+    with pytest.raises(ValueError, match='variables share memory'):
+        ops._need_apart('variables', [buf[2:3], buf[:5]])

@@ -509,3 +509,56 @@ def test_streams_and_a_sparse_gradient(dev):
     p.grad = torch.sparse_coo_tensor(torch.tensor([[1]]), torch.ones(1, 3), (4, 3)).to(dev)
     with pytest.raises(ValueError, match='dense'):
         opt.step()
+
+
+def test_memory_that_is_shared_and_decay_that_changes(dev):
+    from hgq2_amd import ops
+    from hgq2_amd.train import AdamW
+
+    buf = torch.zeros(12, device=dev)
+    with pytest.raises(ValueError, match='share memory'):
+        AdamW([torch.nn.Parameter(buf[:8]), torch.nn.Parameter(buf[4:])])
+    ws, state = [buf[:4], buf[4:]], ops.adamw_state(dev, 0.1)
+    moments = [ops.adamw_moments(8, dev) for _ in ws]
+    with pytest.raises(ValueError, match='moments share memory'):
+        ops.adamw_update_multi_([buf[:8], torch.zeros(8, device=dev)], [torch.ones(8, device=dev)] * 2, [moments[0], moments[0]], state)
+    assert not buf.any() and int(state[0]) == 0
+
+    a, b = (torch.nn.Parameter(torch.ones(5, device=dev)) for _ in range(2))
+    opt = AdamW([a, b], lr=0.5, weight_decay=0.25)
+    opt.exclude_from_weight_decay([b])
+    a.grad, b.grad = torch.zeros_like(a), torch.zeros_like(b)
+    opt.step()  # gradients of zero: the decay alone moves
+    assert torch.equal(a, torch.full_like(a, 0.875)) and torch.equal(b, torch.ones_like(b))
+    opt.weight_decay = 0.5
+    opt.step()
+    assert torch.equal(a, torch.full_like(a, 0.875 * 0.75)) and torch.equal(b, torch.ones_like(b)) and opt.weight_decay == 0.5
+    with pytest.raises(ValueError, match='negative'):
+        opt.weight_decay = -0.1
+
+
+def test_more_elements_than_32_bits_count(dev):
+    """2^32 + 1077 elements: the first and the last ones against 64 bits, and the norm (all other gradients are zero)."""
+    from hgq2_amd import ops
+
+    n, edge = 2**32 + 1077, 1077 + 3 * BLOCK
+    gen = torch.Generator().manual_seed(15)
+    w, g = (torch.zeros(n, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    ends = (slice(0, edge), slice(n - edge, n))  # (both begin with a block)
+    assert (n - edge) % BLOCK == 0
+    for e in ends:
+        w[e], g[e] = torch.randn(edge, generator=gen).to(dev), torch.randn(edge, generator=gen).to(dev)
+    assert abs(float(ops.global_norm([g])) - math.sqrt(sum(float((g[e].double()**2).sum()) for e in ends))) <= 2 * U * 100
+    moments, state = ops.adamw_moments(n, dev, 8), ops.adamw_state(dev, 0.001)
+    before = [w[e].clone() for e in ends]
+    ops.adamw_update_multi_([w], [g], [moments], state, decay=[0.004], seed=9)
+    for e, old in zip(ends, before):
+        zero = torch.zeros(edge)
+        nw, nm, nv, tw, tm, tv = _plain(old, g[e], zero, zero, 1)
+        _near(w[e], nw, tw, torch.bfloat16, 'w')
+        h = _philox(np.arange(e.start // 4, -(-e.stop // 4), dtype=np.uint64), 1, 9)[:edge]
+        scales = slice(e.start // BLOCK, -(-e.stop // BLOCK))
+        _codes_near(moments[0][e], moments[1][scales], nm, tm, h & np.uint64(0xFFFF), False, 'm')
+        r = nv.sqrt()
+        _codes_near(moments[2][e], moments[3][scales], r, tv / (2 * r).clamp(min=1e-300) + 2 * U * r, h >> np.uint64(16), True, 'r')
+    assert not w[edge:n - edge].any()

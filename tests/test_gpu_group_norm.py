@@ -410,3 +410,50 @@ def test_two_backward_passes_and_another_stream(dev):
         out = ops.group_norm(v, 2)
         v.add_(1.0)
         out.sum().backward()
+
+
+# more groups than a launch has workgroups of 256 threads; 67 million groups of one access per row; more than 2^31 elements
+@pytest.mark.parametrize('shape,G,dtype', [((129, 2, 131072), 131072, torch.float32), ((16400, 2, 16396), 4099, torch.bfloat16),
+                                           ((33, 1 << 16, 1024), 8, torch.bfloat16)])
+def test_very_many_groups_and_elements(dev, shape, G, dtype):
+    from hgq2_amd import ops
+
+    g = torch.Generator(device=dev).manual_seed(12)
+    x = torch.randn(shape, generator=g, device=dev, dtype=dtype).requires_grad_(True)
+    dy = torch.randn(shape, generator=g, device=dev, dtype=dtype)
+    gamma, beta = (torch.randn(shape[-1], generator=g, device=dev) for _ in range(2))
+    y = ops.group_norm(x, G, gamma, beta, activation='silu')
+    dx, = torch.autograd.grad(y, x, dy)
+    for b in (0, shape[0] // 2, shape[0] - 1):
+        part = slice(b, b + 1)
+        want, tol = _definition(x[part].detach(), dy[part], gamma, beta, G, 1e-3, 'silu')
+        _check(y[part], want[0], tol[0], dtype, f'y of sample {b}')
+        _check(dx[part], want[1], tol[1], dtype, f'dx of sample {b}')
+
+
+def test_recording_while_another_streams_graph_lives(dev):
+    """A leaf whose gradients an earlier, living graph of another stream accumulates is refused in a recording, and taken once that is gone."""
+    from hgq2_amd import ops
+
+    g = torch.Generator().manual_seed(13)
+    x = torch.randn(4, 20, 16, generator=g).to(dev)
+    gamma = torch.nn.Parameter(torch.randn(16, generator=g).to(dev))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # outside a recording either stream will do
+        want = torch.autograd.grad(ops.group_norm(x, 4, gamma).square().sum(), gamma)[0]
+    torch.cuda.synchronize()
+    living = ops.group_norm(x, 4, gamma)
+    with pytest.raises(RuntimeError, match='gamma belongs to a graph of another stream'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            ops.group_norm(x, 4, gamma)
+    del living
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ops.group_norm(x, 4, gamma).backward(2 * ops.group_norm(x, 4, gamma.detach()))
+    got = gamma.grad
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.allclose(got, want, rtol=1e-5, atol=1e-5)
