@@ -562,3 +562,29 @@ def test_more_elements_than_32_bits_count(dev):
         r = nv.sqrt()
         _codes_near(moments[2][e], moments[3][scales], r, tv / (2 * r).clamp(min=1e-300) + 2 * U * r, h >> np.uint64(16), True, 'r')
     assert not w[edge:n - edge].any()
+
+
+def test_fit_counts_regularizers_once(dev):
+    """An epoch's loss is the same whether the optimizer folds the regularizers into its launch or they are terms of the loss."""
+    from hgq2_amd.regularizers import MonoL1
+    from hgq2_amd.train import AdamW, fit
+
+    gen = torch.Generator().manual_seed(16)
+    x, y = torch.randn(512, 16, generator=gen).to(dev), torch.randint(0, 5, (512,), generator=gen).to(dev)
+    nets, losses = [_model(dev) for _ in range(2)], []
+    for net in nets:
+        net(x, training=False)
+    with torch.no_grad():
+        for a, b in zip(nets[1].parameters(), nets[0].parameters()):
+            a.copy_(b)
+    for fold, net in zip((True, False), nets):
+        regularised = [p for p in net.parameters() if p.requires_grad and isinstance(getattr(p, 'regularizer', None), MonoL1)]
+        assert regularised
+        for p in regularised:
+            p.regularizer = MonoL1(1e-4)
+        hist = fit(net, x, y, batch_size=128, lr=0.0, shuffle=False,
+                   optimizer=lambda v: AdamW(v, lr=0.0, weight_decay=0.0, fold_regularizers=fold))  # noqa: B023
+        losses.append(hist[0]['loss'])
+        total = sum(float(p.regularizer(p)) for p in regularised)
+        assert total > 0.01
+    assert abs(losses[0] - losses[1]) <= 1e-5 * abs(losses[0])
