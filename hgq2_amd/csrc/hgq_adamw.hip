@@ -47,13 +47,22 @@ struct AdamwItem {
 struct AdamwLaunch {
     AdamwItem item[ADAMW_ITEMS];
     const float *side[ADAMW_PIECES], *side_scale[ADAMW_PIECES];
-    uint32_t start[ADAMW_ITEMS + 1];  // first chunk of each item; the last entry: their number
+    uint32_t start[ADAMW_ITEMS + 1];  // first chunk of each item, then their number in all further entries
 };
 struct AdamwSum {
     const float *term[HGQ_SUM_BATCH];
     int n;
     float *out;
 };
+
+// The item of a chunk: comparisons with all starts, not one load after the other.  A step of 28 variables with 13 thousand elements: 6.5 ->
+// 5.4 us; 150 million elements past the cache 730 -> 722 us.
+__device__ __forceinline__ int item_of(const AdamwLaunch &a, uint32_t chunk) {
+    int i = 0;
+#pragma unroll
+    for (int k = 1; k < ADAMW_ITEMS; ++k) i += chunk >= a.start[k];
+    return i;
+}
 
 __device__ __forceinline__ float load_as_f32(const void *p, int64_t e, int type) {
     if (type == HGQ_TYPE_F32) return ((const float *)p)[e];
@@ -343,7 +352,7 @@ __device__ __forceinline__ float norm_of_parts(const double *parts, int n, doubl
 template <int BITS, bool STREAM>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum, hgq_adamw_state *state, double b1, double b2, float eps,
                                                     float clipnorm, const double *parts, int n_parts, const float *joined, float *norm_out, uint64_t seed,
-                                                    int items, int last) {
+                                                    int last) {
     __shared__ double lds[4];
     if (sum.n > 0 && blockIdx.x == 0 && threadIdx.x == 0) {  // the step's loss terms, which the update does not read
         float v = sum.term[0][0];
@@ -375,9 +384,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
         k.c = norm <= clipnorm ? 1.0f : norm < __builtin_inff() ? __fdiv_rn(clipnorm, norm) : __builtin_nanf("");
         if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
     }
-    int i = 0;
-    for (uint32_t c = blockIdx.x; c < a.start[items]; c += gridDim.x) {
-        while (c >= a.start[i + 1]) ++i;
+    for (uint32_t c = blockIdx.x; c < a.start[ADAMW_ITEMS]; c += gridDim.x) {
+        const int i = item_of(a, c);
         adamw_chunk<BITS, STREAM>(a, a.item[i], k, (int64_t)(c - a.start[i]) * (STREAM ? ADAMW_STREAM_CHUNK : ADAMW_CHUNK));
     }
     if (left) return;
@@ -415,11 +423,11 @@ __device__ __forceinline__ double norm_chunk(const AdamwItem &it, int64_t e0) {
 }
 
 // sums of squares, one per workgroup: in fp64, so that no finite gradient overflows and their order does not show
-__global__ __launch_bounds__(256) void norm_parts_kernel(AdamwLaunch a, int items, int chunk, double *parts) {
+__global__ __launch_bounds__(256) void norm_parts_kernel(AdamwLaunch a, int chunk, double *parts) {
     __shared__ double lds[4];
     double v = 0;
-    int i = 0;
-    for (uint32_t c = blockIdx.x; c < a.start[items]; c += gridDim.x) {
+    int i = item_of(a, blockIdx.x);
+    for (uint32_t c = blockIdx.x; c < a.start[ADAMW_ITEMS]; c += gridDim.x) {
         while (c >= a.start[i + 1]) ++i;
         const AdamwItem &it = a.item[i];
         const int64_t e0 = (int64_t)(c - a.start[i]) * chunk, end = e0 + chunk < it.n ? e0 + chunk : it.n;
@@ -448,7 +456,7 @@ using namespace hgq;
 
 namespace {
 
-// Goes over `items` in launches of up to ADAMW_ITEMS variables and ADAMW_PIECES further gradient pieces: fn(launch, variables, last).
+// Goes over `items` in launches of up to ADAMW_ITEMS variables and ADAMW_PIECES further gradient pieces: fn(launch, last).
 // Descriptors travel as launch arguments (4 KB at most), so the calls are safe under HIP graph capture.
 template <class F>
 int for_launches(const hgq_adamw_item *items, int count, int chunk, F fn) {
@@ -472,13 +480,13 @@ int for_launches(const hgq_adamw_item *items, int count, int chunk, F fn) {
             d.vec = own == 0 && (((uintptr_t)s.w | (uintptr_t)s.g) & (4 * size - 1)) == 0 && (((uintptr_t)s.m | (uintptr_t)s.v) & (4 * moment - 1)) == 0;
             for (int k = 0; k < HGQ_SGD_SIDES; ++k)
                 if (s.side[k]) a.side[pieces] = s.side[k], a.side_scale[pieces] = s.side_scale[k], ++pieces;
-            a.start[n] = (uint32_t)chunks;
+            a.start[n++] = (uint32_t)chunks;
             chunks += own_chunks;
-            a.start[++n] = (uint32_t)chunks;
         }
+        for (int k = n; k <= ADAMW_ITEMS; ++k) a.start[k] = (uint32_t)chunks;
         while (at < count && items[at].n == 0) ++at;
         done = at >= count;
-        const int rc = fn(a, n, done);
+        const int rc = fn(a, done);
         if (rc) return rc;
     }
     return HGQ_OK;
@@ -500,8 +508,8 @@ int check_items(const char *what, const hgq_adamw_item *items, int count, int bi
     return HGQ_OK;
 }
 
-int norm_grid(const AdamwLaunch &a, int n) {
-    const uint32_t chunks = n ? a.start[n] : 0;
+int norm_grid(const AdamwLaunch &a) {
+    const uint32_t chunks = a.start[ADAMW_ITEMS];
     return (int)(chunks < NORM_GRID ? chunks : NORM_GRID);
 }
 
@@ -511,8 +519,8 @@ extern "C" int64_t hgq_global_norm_parts(const hgq_adamw_item *items, int count)
     if (check_items("hgq_global_norm_parts", items, count, 0)) return -1;
     int64_t parts = 0;
     const int chunk = NORM_LOADS * 1024;
-    for_launches(items, count, chunk, [&](const AdamwLaunch &a, int n, bool) {
-        parts += norm_grid(a, n);
+    for_launches(items, count, chunk, [&](const AdamwLaunch &a, bool) {
+        parts += norm_grid(a);
         return HGQ_OK;
     });
     return parts;
@@ -523,11 +531,11 @@ extern "C" int hgq_global_norm(const hgq_adamw_item *items, int count, double *p
     if (rc) return rc;
     int64_t at = 0;
     const int chunk = NORM_LOADS * 1024;
-    rc = for_launches(items, count, chunk, [&](const AdamwLaunch &a, int n, bool) {
-        const int grid = norm_grid(a, n);
+    rc = for_launches(items, count, chunk, [&](const AdamwLaunch &a, bool) {
+        const int grid = norm_grid(a);
         if (!grid) return HGQ_OK;
         if (!parts) return fail(HGQ_ERR_ARG, "hgq_global_norm: null workspace");
-        hipLaunchKernelGGL(norm_parts_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a, n, chunk, parts + at);
+        hipLaunchKernelGGL(norm_parts_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a, chunk, parts + at);
         at += grid;
         return check_launch("hgq_global_norm");
     });
@@ -564,13 +572,13 @@ extern "C" int hgq_adamw_update_multi(const hgq_adamw_item *items, int count, in
         if ((rc = check_launch("hgq_adamw_update_multi"))) return rc;
         norm_out = nullptr;
     }
-    return for_launches(items, count, stream_through ? ADAMW_STREAM_CHUNK : ADAMW_CHUNK, [&](const AdamwLaunch &a, int n, bool last) {
-        const uint32_t chunks = n ? a.start[n] : 0, most = stream_through ? chunks : ADAMW_GRID;
+    return for_launches(items, count, stream_through ? ADAMW_STREAM_CHUNK : ADAMW_CHUNK, [&](const AdamwLaunch &a, bool last) {
+        const uint32_t chunks = a.start[ADAMW_ITEMS], most = stream_through ? chunks : ADAMW_GRID;
         const int grid = chunks < 1 ? 1 : (int)(chunks < most ? chunks : most);  // (no element at all: the step still counts)
         auto kernel = state_bits == 8 ? stream_through ? adamw_kernel<8, true> : adamw_kernel<8, false>
                                       : stream_through ? adamw_kernel<32, true> : adamw_kernel<32, false>;
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a, sum, state, beta_1, beta_2, epsilon, clipnorm, norm_parts,
-                           (int)n_parts, joined, norm_out, seed, n, (int)last);
+                           (int)n_parts, joined, norm_out, seed, (int)last);
         sum.n = 0, norm_out = nullptr;
         return check_launch("hgq_adamw_update_multi");
     });

@@ -126,12 +126,16 @@ struct OnceOnly : torch::autograd::Function<OnceOnly> {
 };
 
 // (through the dispatcher, so that fake tensors and tracing see the two operators)
+const auto &forward_op() {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::group_norm_fwd", "").typed<decltype(group_norm_fwd)>();
+    return op;
+}
+
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
     static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &gamma, const Tensor &beta, int64_t groups, double epsilon,
                           int64_t act) {
-        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::group_norm_fwd", "").typed<decltype(group_norm_fwd)>();
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [y, stats] = op.call(x, gamma, beta, groups, epsilon, act);
+        auto [y, stats] = forward_op().call(x, gamma, beta, groups, epsilon, act);
         ctx->save_for_backward({x, gamma, beta, stats});
         ctx->saved_data["groups"] = groups, ctx->saved_data["act"] = act;
         return y;
@@ -169,13 +173,18 @@ void accumulates_here(const char *name, const Tensor &t) {
 Tensor group_norm(const Tensor &x, int64_t groups, const std::optional<Tensor> &gamma, const std::optional<Tensor> &beta, double epsilon, int64_t act) {
     for (const auto &[name, t] : {std::make_pair("gamma", &gamma), std::make_pair("beta", &beta)})
         TORCH_CHECK_VALUE(!*t || ((*t)->dim() == 1 && x.dim() >= 1 && (*t)->numel() == x.size(-1)), name, " must be a vector with an element per channel");
-    if (at::GradMode::is_enabled()) {
+    const auto differentiated = [](const Tensor &t) { return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined(); };
+    const bool graph = differentiated(x) || (gamma && differentiated(*gamma)) || (beta && differentiated(*beta));
+    if (graph) {
         accumulates_here("x", x);
         if (gamma) accumulates_here("gamma", *gamma);
         if (beta) accumulates_here("beta", *beta);
     }
     const Tensor none = gamma && beta ? Tensor() : at::empty({0}, x.options().dtype(at::kFloat).requires_grad(false));
-    return GroupNorm::apply(x.contiguous(), gamma ? *gamma : none, beta ? *beta : none, groups, epsilon, act);
+    const Tensor &ga = gamma ? *gamma : none, &be = beta ? *beta : none;
+    if (graph) return GroupNorm::apply(x.contiguous(), ga, be, groups, epsilon, act);
+    at::AutoDispatchBelowADInplaceOrView below;  // (no node to make)
+    return std::get<0>(forward_op().call(x.contiguous(), ga, be, groups, epsilon, act));
 }
 
 // ---- the global norm -------------------------------------------------------------------------------------------------
@@ -236,6 +245,7 @@ public:
     // regularizer - which the caller sets by `limits` and `pieces`; None: there is no gradient at all.
     py::object gather() {
         HANDLE_TH_ERRORS
+        const at::NoGradGuard no_grad;
         held_.clear();
         py::list special;
         bool any = false;
@@ -283,6 +293,7 @@ public:
     // further gradient pieces of variable k: (scale or None, gradient) pairs
     void pieces(int64_t k, const py::list &pairs) {
         HANDLE_TH_ERRORS
+        const at::NoGradGuard no_grad;
         hgq_adamw_item &it = items_.at(k);
         TORCH_CHECK_VALUE(pairs.size() <= HGQ_SGD_SIDES, "at most ", HGQ_SGD_SIDES, " side gradients per variable");
         for (size_t s = 0; s < pairs.size(); ++s) {

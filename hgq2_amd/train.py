@@ -270,34 +270,45 @@ class AdamW(SGD):
                 have.copy_(new)
             self._state.copy_(ops.adamw_state('cpu', self._lr, state['iterations'], self.beta_1, self.beta_2))
 
-    @torch.no_grad()
     def step(self):
         sums = ops.join_side(hand_over_sums=True)  # the loss terms' sum rides along with the update launch
-        variables, post, inf = self._variables, [], float('inf')
+        variables, post = self._variables, ()
         special = variables.gather()  # variables with gradient pieces, constraints or regularizers; None: no gradient at all
-        for k in special or ():
+        if special or len(sums) > 1 or (special is None and sums):
+            with torch.no_grad():
+                post = self._specials(special or ())
+                ride = sums.pop(0) if (special is not None and sums) else ((), None)
+                for terms, out in sums:
+                    ops.sum_scalars_into(terms, out)
+        else:
+            ride = sums[0] if sums else ((), None)
+        if special is not None:
+            ops.touch_state()  # written through pointers: the version counters do not move
+            variables.step(self._state, self.beta_1, self.beta_2, self.epsilon, self.global_clipnorm or 0.0, self.grad_norm, self.seed,
+                           [t.detach() for t in ride[0]], ride[1])
+        if post:
+            with torch.no_grad():
+                for p, c in post:
+                    p.copy_(c(p))
+
+    def _specials(self, indices):
+        """Hands over the gradient pieces, bounds and folded regularizers of these variables; the constraints to apply after the update."""
+        post, inf = [], float('inf')
+        for k in indices:
             p = self.params[k]
             side = list(getattr(p, '_hgq_side', None) or ())
             while len(side) > ops.SGD_SIDES:  # more pieces than the kernel takes: fold the surplus into one
                 (s1, d1), (s2, d2) = side.pop(), side.pop()
                 side.append((None, (d1 if s1 is None else s1 * d1) + (d2 if s2 is None else s2 * d2)))
             if side:
-                variables.pieces(k, side)
+                self._variables.pieces(k, side)
             c, r = getattr(p, 'constraint', None), getattr(p, 'regularizer', None)
             bounds = c.bounds() if c is not None else (-inf, inf)
             if bounds is None:  # a constraint that is not a clip: applied after the update
                 bounds = (-inf, inf)
                 post.append((p, c))
-            variables.limits(k, r.l1 if (self.fold_regularizers and isinstance(r, MonoL1)) else 0.0, *bounds)
-        ride = sums.pop(0) if (special is not None and sums) else ((), None)
-        for terms, out in sums:
-            ops.sum_scalars_into(terms, out)
-        if special is not None:
-            ops.touch_state()  # written through pointers: the version counters do not move
-            variables.step(self._state, self.beta_1, self.beta_2, self.epsilon, self.global_clipnorm or 0.0, self.grad_norm, self.seed,
-                           [t.detach() for t in ride[0]], ride[1])
-        for p, c in post:
-            p.copy_(c(p))
+            self._variables.limits(k, r.l1 if (self.fold_regularizers and isinstance(r, MonoL1)) else 0.0, *bounds)
+        return post
 
 
 class GraphedTrainStep:

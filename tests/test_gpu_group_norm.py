@@ -457,3 +457,18 @@ def test_recording_while_another_streams_graph_lives(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.allclose(got, want, rtol=1e-5, atol=1e-5)
+
+
+def test_tangents_are_refused_and_a_call_without_gradients_makes_no_node(dev):
+    import torch.autograd.forward_ad as fw
+
+    from hgq2_amd import ops
+
+    x = torch.randn(2, 5, 8, device=dev)
+    gamma = torch.nn.Parameter(torch.ones(8, device=dev))
+    y = ops.group_norm(x, 2, gamma)
+    with torch.no_grad():
+        z = ops.group_norm(x, 2, gamma)
+    assert y.requires_grad and not z.requires_grad and torch.equal(y, z) and not ops.group_norm(x, 2).requires_grad
+    with fw.dual_level(), pytest.raises(Exception, match='jvp|forward'):
+        ops.group_norm(fw.make_dual(x, torch.ones_like(x)), 2)
