@@ -172,10 +172,13 @@ struct GroupTile {
 template <typename T>
 struct Four {
     typedef uint32_t words __attribute__((ext_vector_type(sizeof(T))));
+    typedef words unaligned __attribute__((aligned(sizeof(T))));
     words w;
 
     __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(&w, p, sizeof(w)); }  // (rows of any width: aligned to an element only)
-    typedef words unaligned __attribute__((aligned(sizeof(T))));
+    __device__ __forceinline__ void load_last(const T *p) {  // past the cache
+        w = __builtin_nontemporal_load((const unaligned *)p);
+    }
     __device__ __forceinline__ void store(T *p, bool through) const {  // through: past the cache
         if (through) __builtin_nontemporal_store(w, (unaligned *)p);
         else __builtin_memcpy(p, &w, sizeof(w));
@@ -279,9 +282,15 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
     const GroupRows rows(p, t, on, c0, r0, r1);
     Four<T> v[NV];
     float last[3] = {0, 0, 0};
+    if (phase == 2 && p.through) {  // (the last read of what the cache does not keep)
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (i < rows.full) v[i].load(xs + rows.at + i * rows.step);
+        for (int i = 0; i < NV; ++i)
+            if (i < rows.full) v[i].load_last(xs + rows.at + i * rows.step);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < rows.full) v[i].load(xs + rows.at + i * rows.step);
+    }
 #pragma unroll
     for (int j = 0; j < 3; ++j)
         if (j < rows.rest) last[j] = to_f32(xs[rows.at + rows.full * rows.step + j]);
@@ -409,9 +418,15 @@ __global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict_
     const GroupRows rows(p, t, on, c0, r0, r1);
     Four<T> v[NV], w[NV];
     float last[3] = {0, 0, 0}, dlast[3] = {0, 0, 0};
+    if (phase == 2 && p.through) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (i < rows.full) v[i].load(xs + rows.at + i * rows.step), w[i].load(ds + rows.at + i * rows.step);
+        for (int i = 0; i < NV; ++i)
+            if (i < rows.full) v[i].load_last(xs + rows.at + i * rows.step), w[i].load_last(ds + rows.at + i * rows.step);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < rows.full) v[i].load(xs + rows.at + i * rows.step), w[i].load(ds + rows.at + i * rows.step);
+    }
 #pragma unroll
     for (int j = 0; j < 3; ++j)
         if (j < rows.rest) last[j] = to_f32(xs[rows.at + rows.full * rows.step + j]), dlast[j] = to_f32(ds[rows.at + rows.full * rows.step + j]);
@@ -614,7 +629,8 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     if (tiles > 65535 * (int64_t)SLICE_RUN || (tiles + 7) * p.chunks * threads > 0xffffffff) return false;  // (a launch has less than 2^32 threads)
     p.tiles = (int)tiles;
     // What a pass reads and writes against the card's 256 MB cache, and rows of whole lines: 48 x 64 x 64 x 512 bfloat16, forward 131 -> 110 us,
-    // backward 206 -> 196 us; 1024 x 26 x 26 x 32 fp32, backward 67 -> 58 us.  Half lines are slower that way (64 x 32 x 32 x 256 fp32 in
+    // backward 206 -> 196 us, and 8 and 6 us less with the second read of its cut samples past the cache as well; 1024 x 26 x 26 x 32 fp32,
+    // backward 67 -> 58 us.  Half lines are slower that way (64 x 32 x 32 x 256 fp32 in
     // rows of 64 bytes, backward 50 -> 54 us), and a smaller output is still there for the layer that reads it next.
     p.through = B * S * C * size * (backward ? 3 : 2) > (int64_t)256 << 20 && p.TX * 4 * size % 128 == 0;
     return true;
