@@ -528,17 +528,23 @@ __global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict_
     }
 }
 
-// Adds up runs of SLICE_RUN slices of M entries: where a batch leaves more slices than the last reduction takes well
-constexpr int SLICE_RUN = 64;
+// Adds up runs of SLICE_RUN slices of M entries: where a batch leaves more slices than the last reduction takes well.  All loads of a run are in
+// flight at once (20000 x 30 x 48 in 6 groups, 10000 slices: runs of 64 by eight loads 22 us, of 32 by 32 loads 4.3 us).
+constexpr int SLICE_RUN = 32;
 __global__ __launch_bounds__(64) void group_norm_join_slices(const float *__restrict__ slices, int64_t n, int64_t M, float *__restrict__ out) {
-    const int64_t e = (int64_t)blockIdx.x * 64 + threadIdx.x, first = (int64_t)blockIdx.y * SLICE_RUN;
+    const int64_t e = (int64_t)blockIdx.x * 64 + threadIdx.x;
     if (e >= M) return;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int64_t k = first; k < first + SLICE_RUN && k < n; k += 8)
+    for (int64_t run = blockIdx.y; run * SLICE_RUN < n; run += gridDim.y) {
+        const int64_t first = run * SLICE_RUN, behind = n - first;
+        float v[SLICE_RUN];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (k + u < n) v[u] += slices[(k + u) * M + e];
-    out[blockIdx.y * M + e] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        for (int k = 0; k < SLICE_RUN; ++k) v[k] = k < behind ? slices[(first + k) * M + e] : 0.0f;
+#pragma unroll
+        for (int d = SLICE_RUN / 2; d; d /= 2)
+#pragma unroll
+            for (int k = 0; k < d; ++k) v[k] += v[k + d];
+        out[run * M + e] = v[0];
+    }
 }
 
 }  // namespace hgq
@@ -626,11 +632,10 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     p.team = 1;
     while (p.team < 64 && p.team * 2 * p.NS * p.K <= threads) p.team *= 2;
     const int64_t tiles = (B + p.NS - 1) / p.NS * p.splits;
-    if (tiles > 65535 * (int64_t)SLICE_RUN || (tiles + 7) * p.chunks * threads > 0xffffffff) return false;  // (a launch has less than 2^32 threads)
+    if ((tiles + 7) * p.chunks * threads > 0xffffffff) return false;  // (a launch has less than 2^32 threads)
     p.tiles = (int)tiles;
     // What a pass reads and writes against the card's 256 MB cache, and rows of whole lines: 48 x 64 x 64 x 512 bfloat16, forward 131 -> 110 us,
-    // backward 206 -> 196 us, and 8 and 6 us less with the second read of its cut samples past the cache as well; 1024 x 26 x 26 x 32 fp32,
-    // backward 67 -> 58 us.  Half lines are slower that way (64 x 32 x 32 x 256 fp32 in
+    // backward 206 -> 196 us, and 7 and 6 us less with the second read of its cut samples past the cache as well.  Half lines are slower that way (64 x 32 x 32 x 256 fp32 in
     // rows of 64 bytes, backward 50 -> 54 us), and a smaller output is still there for the layer that reads it next.
     p.through = B * S * C * size * (backward ? 3 : 2) > (int64_t)256 << 20 && p.TX * 4 * size % 128 == 0;
     return true;
@@ -707,7 +712,7 @@ int bwd(const void *dy, const void *x, const float *gamma, const float *beta, co
     if (p.tiles <= MOST_SLICES) return reduce_parts(slices, p.tiles, M, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
     const int runs = (p.tiles + SLICE_RUN - 1) / SLICE_RUN;
     float *joined = slices + p.tiles * M;
-    hipLaunchKernelGGL(group_norm_join_slices, dim3((unsigned)((M + 63) / 64), (unsigned)runs), dim3(64), 0, st, slices, (int64_t)p.tiles, M, joined);
+    hipLaunchKernelGGL(group_norm_join_slices, dim3((unsigned)((M + 63) / 64), (unsigned)(runs < 65535 ? runs : 65535)), dim3(64), 0, st, slices, (int64_t)p.tiles, M, joined);
     const int rc = check_launch("hgq_group_norm_bwd");
     return rc ? rc : reduce_parts(joined, runs, M, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
 }
