@@ -635,8 +635,9 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     if ((tiles + 7) * p.chunks * threads > 0xffffffff) return false;  // (a launch has less than 2^32 threads)
     p.tiles = (int)tiles;
     // What a pass reads and writes against the card's 256 MB cache, and rows of whole lines: 48 x 64 x 64 x 512 bfloat16, forward 131 -> 110 us,
-    // backward 206 -> 196 us, and 7 and 6 us less with the second read of its cut samples past the cache as well.  Half lines are slower that way (64 x 32 x 32 x 256 fp32 in
-    // rows of 64 bytes, backward 50 -> 54 us), and a smaller output is still there for the layer that reads it next.
+    // backward 206 -> 196 us, and 7 and 6 us less with the second read of its cut samples past the cache as well.  Half lines are slower
+    // that way (64 x 32 x 32 x 256 fp32 in rows of 64 bytes, backward 50 -> 54 us), and a smaller output is still there for the layer
+    // that reads it next.
     p.through = B * S * C * size * (backward ? 3 : 2) > (int64_t)256 << 20 && p.TX * 4 * size % 128 == 0;
     return true;
 }

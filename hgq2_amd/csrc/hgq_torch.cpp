@@ -4,6 +4,7 @@
 // called through the C ABI of libhgq_hip.so (bind()), outputs and workspaces are torch tensors on the current stream of their device.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
@@ -54,7 +55,18 @@ float *floats(const Tensor &t) { return t.numel() ? t.data_ptr<float>() : nullpt
 
 void *memory(const Tensor &t) { return t.numel() ? t.data_ptr() : nullptr; }
 
-Tensor workspace(int64_t n, const Tensor &like, at::ScalarType type = at::kFloat) { return at::empty({n}, like.options().dtype(type)); }
+Tensor vector_like(int64_t n, const Tensor &like) { return at::empty({n}, like.options().dtype(at::kFloat)); }
+
+// A call's scratch memory on the current stream of the current device: the allocator hands it to later work of that stream only, and
+// under capture it belongs to the graph.  (A tensor takes 1 us to make, this a quarter of that.)
+template <typename T>
+struct Workspace {
+    c10::DataPtr memory;
+    explicit Workspace(int64_t n) {
+        if (n > 0) memory = c10::hip::HIPCachingAllocator::get()->allocate((size_t)n * sizeof(T));
+    }
+    T *get() const { return (T *)memory.get(); }
+};
 
 // ---- group normalisation ---------------------------------------------------------------------------------------------
 struct GroupSizes {
@@ -83,11 +95,10 @@ std::tuple<Tensor, Tensor> group_norm_fwd(const Tensor &x, const Tensor &gamma, 
     const GroupSizes s = group_sizes(x, groups);
     channel_vector("gamma", gamma, x), channel_vector("beta", beta, x);
     const c10::DeviceGuard guard(x.device());
-    Tensor y = at::empty_like(x), stats = at::empty({2, s.B, s.G}, x.options().dtype(at::kFloat)), ws;
-    const int64_t need = library().group_norm_fwd_workspace(s.B, s.S, (int)s.C, s.G, s.type);
-    if (need > 0) ws = workspace(need, x);
+    Tensor y = at::empty_like(x), stats = at::empty({2, s.B, s.G}, x.options().dtype(at::kFloat));
+    const Workspace<float> ws(library().group_norm_fwd_workspace(s.B, s.S, (int)s.C, s.G, s.type));
     float *mean = floats(stats);
-    check(lib.group_norm_fwd(memory(x), floats(gamma), floats(beta), memory(y), mean, mean ? mean + s.B * s.G : nullptr, need > 0 ? floats(ws) : nullptr,
+    check(lib.group_norm_fwd(memory(x), floats(gamma), floats(beta), memory(y), mean, mean ? mean + s.B * s.G : nullptr, ws.get(),
                              s.B, s.S, (int)s.C, s.G, (float)epsilon, (int)act, s.type, stream_of(x)),
           "hgq_group_norm_fwd");
     return {y, stats};
@@ -102,13 +113,12 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor &dy, const Tensor
     TORCH_CHECK_VALUE(stats.numel() == 2 * s.B * s.G && stats.scalar_type() == at::kFloat && stats.device() == x.device() && stats.is_contiguous(),
                       "stats must be what the forward call left");
     const c10::DeviceGuard guard(x.device());
-    Tensor dx = need_dx ? at::empty_like(x) : at::empty({0}, x.options()), dgamma = workspace(need_dgamma ? s.C : 0, x),
-           dbeta = workspace(need_dbeta ? s.C : 0, x), ws;
-    const int64_t need = library().group_norm_bwd_workspace(s.B, s.S, (int)s.C, s.G, s.type);
-    if (need > 0) ws = workspace(need, x);
+    Tensor dx = need_dx ? at::empty_like(x) : at::empty({0}, x.options()), dgamma = vector_like(need_dgamma ? s.C : 0, x),
+           dbeta = vector_like(need_dbeta ? s.C : 0, x);
+    const Workspace<float> ws(library().group_norm_bwd_workspace(s.B, s.S, (int)s.C, s.G, s.type));
     const float *mean = floats(stats);
     check(lib.group_norm_bwd(memory(dy), memory(x), floats(gamma), floats(beta), mean, mean ? mean + s.B * s.G : nullptr, memory(dx), floats(dgamma),
-                             floats(dbeta), need > 0 ? floats(ws) : nullptr, s.B, s.S, (int)s.C, s.G, (int)act, s.type, stream_of(x)),
+                             floats(dbeta), ws.get(), s.B, s.S, (int)s.C, s.G, (int)act, s.type, stream_of(x)),
           "hgq_group_norm_bwd");
     return {dx, dgamma, dbeta};
 }
@@ -188,25 +198,26 @@ Tensor group_norm(const Tensor &x, int64_t groups, const std::optional<Tensor> &
 }
 
 // ---- the global norm -------------------------------------------------------------------------------------------------
-Tensor global_norm(const std::vector<Tensor> &tensors) {
+Tensor global_norm(at::TensorList tensors) {
     TORCH_CHECK_VALUE(!tensors.empty(), "at least one tensor is expected");
     const Tensor &first = tensors[0];
     TORCH_CHECK_VALUE(first.is_cuda(), "tensors must be on a GPU (there is no CPU implementation), got device ", first.device());
     const c10::DeviceGuard guard(first.device());
-    std::vector<hgq_adamw_item> items(tensors.size());
+    std::vector<hgq_adamw_item> items(tensors.size());  // (zeros)
     std::vector<Tensor> held;
     for (size_t k = 0; k < tensors.size(); ++k) {
-        Tensor t = tensors[k];
+        const Tensor &t = tensors[k];
         const int type = type_code(t.scalar_type());
         TORCH_CHECK_VALUE(type >= 0, "tensors must be float32, bfloat16 or float16, got ", t.scalar_type());
         TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.device() == first.device(), "tensors must be dense and on one device, got ", t.layout(), " on ", t.device());
-        if (!t.is_contiguous()) held.push_back(t = t.detach().contiguous());
-        items[k] = {};
-        items[k].g = memory(t), items[k].n = t.numel(), items[k].type = type;
+        items[k].n = t.numel(), items[k].type = type;
+        if (!items[k].n) continue;
+        if (!t.is_contiguous()) held.push_back(t.detach().contiguous());
+        items[k].g = t.is_contiguous() ? t.const_data_ptr() : held.back().const_data_ptr();
     }
     Tensor out = at::empty({}, first.options().dtype(at::kFloat));
-    Tensor parts = workspace(library().global_norm_parts(items.data(), (int)items.size()), first, at::kDouble);
-    check(lib.global_norm(items.data(), (int)items.size(), (double *)memory(parts), out.data_ptr<float>(), stream_of(first)), "hgq_global_norm");
+    const Workspace<double> parts(library().global_norm_parts(items.data(), (int)items.size()));
+    check(lib.global_norm(items.data(), (int)items.size(), parts.get(), out.data_ptr<float>(), stream_of(first)), "hgq_global_norm");
     return out;
 }
 
@@ -326,14 +337,11 @@ public:
             const py::gil_scoped_release others;
             const c10::DeviceGuard guard(device_);
             void *stream = stream_of(st);
-            Tensor parts;
-            int64_t n = 0;
-            if (clipnorm > 0 && (n = library().global_norm_parts(items_.data(), count)) > 0) {
-                parts = workspace(n, st, at::kDouble);  // this call's own: in a captured step it belongs to that graph
-                check(lib.global_norm(items_.data(), count, parts.data_ptr<double>(), nullptr, stream), "hgq_global_norm");
-            }
+            const int64_t n = clipnorm > 0 ? library().global_norm_parts(items_.data(), count) : 0;
+            const Workspace<double> parts(n);
+            if (n > 0) check(lib.global_norm(items_.data(), count, parts.get(), nullptr, stream), "hgq_global_norm");
             check(library().adamw_update_multi(items_.data(), count, bits_, (hgq_adamw_state *)st.data_ptr(), beta_1, beta_2, (float)epsilon,
-                                               n > 0 ? (float)clipnorm : 0.0f, n > 0 ? parts.data_ptr<double>() : nullptr, n, norm, seed, ptrs, n_terms, sum,
+                                               n > 0 ? (float)clipnorm : 0.0f, parts.get(), n, norm, seed, ptrs, n_terms, sum,
                                                stream),
                   "hgq_adamw_update_multi");
         }
@@ -390,12 +398,12 @@ TORCH_LIBRARY_FRAGMENT(hgq, m) {
 TORCH_LIBRARY_IMPL(hgq, CUDA, m) {
     m.impl("group_norm_fwd", group_norm_fwd);
     m.impl("group_norm_bwd", group_norm_bwd);
-    m.impl("global_norm", [](at::TensorList t) { return global_norm(t.vec()); });
+    m.impl("global_norm", global_norm);
 }
 TORCH_LIBRARY_IMPL(hgq, CPU, m) {
     m.impl("group_norm_fwd", group_norm_fwd);
     m.impl("group_norm_bwd", group_norm_bwd);
-    m.impl("global_norm", [](at::TensorList t) { return global_norm(t.vec()); });
+    m.impl("global_norm", global_norm);
 }
 
 PYBIND11_MODULE(_host, m) {
