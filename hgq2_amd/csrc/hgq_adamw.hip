@@ -24,8 +24,9 @@ namespace hgq {
 constexpr int ADAMW_ITEMS = 28, ADAMW_PIECES = 32;
 // A step that touches more than the card's 256 MB cache passes through it once: accesses that leave no trace there, four blocks per
 // wavefront in flight, a workgroup per 4096 elements.  150 million elements, 4.2 GB: 851 -> 720 us (5.9 TB/s; the card copies at 5.0), with
-// moments in 8 bits, 2.4 GB: 552 -> 437 us; 37 million bfloat16: 164 -> 137 us.  A smaller step leaves its weights for the next
-// forward pass; two blocks, and up to 2048 workgroups that go over 2048 elements at a time (4 million elements: 22 us either way).
+// moments in 8 bits, 2.4 GB: 552 -> 437 us (now 409, its 79 vector instructions per element close behind); 37 million bfloat16: 164 ->
+// 137 us.  A smaller step leaves its weights for the next forward pass; two blocks, and up to 2048 workgroups that go over 2048
+// elements at a time (4 million elements: 22 us either way).
 constexpr int64_t ADAMW_CACHE = (int64_t)256 << 20;
 constexpr int ADAMW_CHUNK = 2048, ADAMW_STREAM_CHUNK = 4096;  // elements a workgroup takes at a time, in blocks of 256
 constexpr int ADAMW_GRID = 2048;
