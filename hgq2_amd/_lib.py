@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -246,7 +247,7 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-_native = None
+_native, _native_lock = None, threading.Lock()
 _NATIVE_CALLS = ('hgq_last_error', 'hgq_global_norm_parts', 'hgq_global_norm', 'hgq_adamw_update_multi', 'hgq_group_norm_fwd_workspace',
                  'hgq_group_norm_fwd', 'hgq_group_norm_bwd_workspace', 'hgq_group_norm_bwd')
 
@@ -254,9 +255,14 @@ _NATIVE_CALLS = ('hgq_last_error', 'hgq_global_norm_parts', 'hgq_global_norm', '
 def native():
     """The host code that is compiled against torch (``csrc/hgq_torch.cpp``), bound to the HIP library's entry points; it registers the
     operators ``hgq::group_norm_fwd``, ``hgq::group_norm_bwd`` and ``hgq::global_norm``."""
-    global _native
     if _native is not None:
         return _native
+    with _native_lock:
+        return _native if _native is not None else _load_native()
+
+
+def _load_native():
+    global _native
     import importlib.util
 
     import torch

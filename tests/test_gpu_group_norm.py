@@ -472,3 +472,36 @@ def test_tangents_are_refused_and_a_call_without_gradients_makes_no_node(dev):
     assert y.requires_grad and not z.requires_grad and torch.equal(y, z) and not ops.group_norm(x, 2).requires_grad
     with fw.dual_level(), pytest.raises(Exception, match='jvp|forward'):
         ops.group_norm(fw.make_dual(x, torch.ones_like(x)), 2)
+
+
+def test_two_threads(dev):
+    """Two threads, each on a stream of its own, get what one gets alone."""
+    import threading
+
+    from hgq2_amd import ops
+
+    g = torch.Generator().manual_seed(17)
+    data = []
+    for shape, G in (((50, 100, 48), 6), ((3, 5000, 32), 4)):
+        data.append((torch.randn(shape, generator=g).to(dev).requires_grad_(True), torch.randn(shape[-1], generator=g).to(dev).requires_grad_(True), G,
+                     torch.randn(shape, generator=g).to(dev)))
+
+    def work(x, gamma, G, dy):
+        y = ops.group_norm(x, G, gamma, activation='silu')
+        return [y.detach(), *torch.autograd.grad(y, [x, gamma], dy), ops.global_norm([y.detach(), dy])]
+
+    want, got = [work(*d) for d in data], [None, None]
+    torch.cuda.synchronize()
+
+    def run(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                out = work(*data[k])
+            torch.cuda.current_stream().synchronize()
+            got[k] = out
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for a, b in zip(want, got):
+        assert b is not None and all(torch.equal(p, q) for p, q in zip(a, b))

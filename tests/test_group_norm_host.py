@@ -92,3 +92,28 @@ def test_layer_is_saved_with_its_model(cpu_build, tmp_path):
     assert (other.groups, other.epsilon, other.activation, other.name) == (3, 1e-5, 'silu', 'norm')
     assert torch.equal(other.gamma, model.layers[0].gamma) and torch.equal(other.beta, model.layers[0].beta)
     assert other.gamma.constraint.bounds() == (0.0, 2.0) and other.beta.constraint is None
+
+
+def test_first_use_from_several_threads():
+    """Whichever thread asks first loads the host extension; the others wait for it."""
+    import os
+    import subprocess
+    import sys
+
+    code = '''
+import threading
+import torch
+from hgq2_amd import _lib
+_lib.load()
+gate, got = threading.Barrier(8), []
+def ask():
+    gate.wait()
+    got.append(_lib.native())
+threads = [threading.Thread(target=ask) for _ in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert len(got) == 8 and len({id(m) for m in got}) == 1, len(got)
+'''
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
