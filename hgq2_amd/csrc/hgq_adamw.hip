@@ -339,12 +339,6 @@ __device__ __forceinline__ double block_sum(double v, double *lds) {
     return v;
 }
 
-__device__ __forceinline__ float norm_of_parts(const double *parts, int n, double *lds) {
-    double v = 0;
-    for (int p = threadIdx.x; p < n; p += 256) v += parts[p];
-    return (float)sqrt(block_sum(v, lds));
-}
-
 // The step's number, the powers of the decay rates and the learning rate live in device memory (hgq_adamw_state), so a recorded launch
 // moves on at every replay.  All workgroups read them; in a step's last launch each then takes a ticket, and the one with the last
 // ticket writes the next step's.  Tickets of one counter come one every 27 ns (2048 workgroups: 55 us, more than an update of 4 million
@@ -360,14 +354,21 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
         for (int t = 1; t < sum.n; ++t) v = __fadd_rn(v, sum.term[t][0]);
         sum.out[0] = v;
     }
+    // What the memory has to answer first - the state, the parts of the norm, the descriptor of the first chunk - is asked for at once, and only then
+    // waited for (0.88 million elements: 8.1 -> 7.6 us).
+    const double lr = state->lr, power_1 = state->beta_1_power, power_2 = state->beta_2_power;
+    const int64_t steps = state->step;
+    double squares = 0;
+    if (n_parts > 0 && !joined)
+        for (int p = threadIdx.x; p < n_parts; p += 256) squares += parts[p];
+    const int first = item_of(a, blockIdx.x);
     __shared__ AdamwStep shared;
     uint32_t left = 1;  // tickets not taken before this workgroup's, of its counter
     int64_t t = 0;
     double p1 = 0, p2 = 0;
     const uint32_t counter = gridDim.x > HGQ_ADAMW_TICKETS ? 1 + blockIdx.x % HGQ_ADAMW_TICKETS : HGQ_ADAMW_TICKETS + 1;
     if (threadIdx.x == 0) {
-        const double lr = state->lr;
-        t = state->step + 1, p1 = state->beta_1_power * b1, p2 = state->beta_2_power * b2;
+        t = steps + 1, p1 = power_1 * b1, p2 = power_2 * b2;
         shared.alpha = (float)(lr * sqrt(1.0 - p2) / (1.0 - p1)), shared.lr = (float)lr, shared.t = (uint64_t)t;
         asm volatile("" ::"v"(t), "v"(p1), "v"(p2), "v"(lr) : "memory");  // (the reads are done before the ticket is taken)
         if (last) {
@@ -380,13 +381,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
     k.seed = seed, k.one_minus_b1 = (float)(1.0 - b1), k.one_minus_b2 = (float)(1.0 - b2), k.eps = eps;
     k.c = 1.0f;
     if (n_parts > 0) {
-        const float norm = joined ? joined[0] : norm_of_parts(parts, n_parts, lds);
+        const float norm = joined ? joined[0] : (float)sqrt(block_sum(squares, lds));
         // no clipping up to the bound; a norm that is not finite makes every step not a number
         k.c = norm <= clipnorm ? 1.0f : norm < __builtin_inff() ? __fdiv_rn(clipnorm, norm) : __builtin_nanf("");
         if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
     }
     for (uint32_t c = blockIdx.x; c < a.start[ADAMW_ITEMS]; c += gridDim.x) {
-        const int i = item_of(a, c);
+        const int i = c == blockIdx.x ? first : item_of(a, c);
         adamw_chunk<BITS, STREAM>(a, a.item[i], k, (int64_t)(c - a.start[i]) * (STREAM ? ADAMW_STREAM_CHUNK : ADAMW_CHUNK));
     }
     if (left) return;
@@ -447,8 +448,10 @@ __global__ __launch_bounds__(256) void norm_parts_kernel(AdamwLaunch a, int chun
 
 __global__ __launch_bounds__(256) void norm_finish_kernel(const double *parts, int n, float *out) {
     __shared__ double lds[4];
-    const float norm = norm_of_parts(parts, n, lds);
-    if (threadIdx.x == 0) out[0] = norm;
+    double v = 0;
+    for (int p = threadIdx.x; p < n; p += 256) v += parts[p];
+    v = block_sum(v, lds);
+    if (threadIdx.x == 0) out[0] = (float)sqrt(v);
 }
 
 }  // namespace hgq
