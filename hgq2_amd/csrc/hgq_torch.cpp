@@ -271,17 +271,17 @@ public:
             const bool pieces = side && PyObject_IsTrue(side) == 1;
             it.n = 0;
             if (sizes_[k] == 0 || (!g.defined() && !pieces)) continue;
-            TORCH_CHECK_VALUE(t.device() == device_ && t.scalar_type() == types_[k] && t.numel() == sizes_[k] && t.is_contiguous(),
+            TORCH_CHECK_VALUE(t.device() == device_ && t.scalar_type() == types_[k] && t.numel() == sizes_[k] && t.is_contiguous() && !t.is_neg(),
                               "variables must stay contiguous, on ", device_, ", and of their size and type");
             it.w = t.data_ptr(), it.g = nullptr;
             if (g.defined()) {
                 TORCH_CHECK_VALUE(g.layout() == at::kStrided, "gradient must be dense");
                 TORCH_CHECK_VALUE(g.device() == device_ && g.scalar_type() == types_[k] && g.numel() == sizes_[k], "gradient must be like its variable, got ",
                                   g.scalar_type(), " ", g.sizes(), " on ", g.device());
-                if (g.is_contiguous()) {
+                if (g.is_contiguous() && !g.is_neg()) {
                     it.g = g.data_ptr();
                 } else {
-                    held_.push_back(g.contiguous());
+                    held_.push_back(g.contiguous().resolve_neg());
                     it.g = held_.back().data_ptr();
                 }
             }
@@ -312,7 +312,7 @@ public:
             const Tensor &d = THPVariable_Unpack(pair[1].ptr());
             TORCH_CHECK_VALUE(d.device() == device_ && d.scalar_type() == at::kFloat && d.numel() == sizes_[k] && d.layout() == at::kStrided,
                               "a side gradient must be a dense float32 tensor of its variable's size on ", device_);
-            held_.push_back(d.contiguous());
+            held_.push_back(d.contiguous().resolve_neg());
             it.side[s] = held_.back().data_ptr<float>();
             if (pair[0].is_none()) continue;
             const Tensor &c = THPVariable_Unpack(pair[0].ptr());

@@ -3547,7 +3547,7 @@ def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: flo
     bits = 32 if len(moments[0]) == 2 else 8
     each = lambda v, d: [d] * n if v is None else [float(k) for k in v]  # noqa: E731
     empty = torch.empty(0, dtype=torch.float32, device=state.device)
-    adamw_update_multi_op([w.detach() for w in ws], [g.detach().contiguous() for g in gs], [k for m in moments for k in m], each(l1, 0.0),
+    adamw_update_multi_op([w.detach() for w in ws], [g.detach().contiguous().resolve_neg() for g in gs], [k for m in moments for k in m], each(l1, 0.0),
                           each(lo, -inf), each(hi, inf), each(decay, 0.0), bits, state, float(beta_1), float(beta_2), float(epsilon),
                           float(clipnorm or 0.0), norm_out if norm_out is not None else empty, int(seed) & (2**63 - 1))
     touch_state()

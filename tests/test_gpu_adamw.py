@@ -588,3 +588,29 @@ def test_fit_counts_regularizers_once(dev):
         total = sum(float(p.regularizer(p)) for p in regularised)
         assert total > 0.01
     assert abs(losses[0] - losses[1]) <= 1e-5 * abs(losses[0])
+
+
+def test_gradients_that_are_views(dev):
+    """Gradients that are lazily negated, expanded or transposed count as what they stand for."""
+    from hgq2_amd import ops
+    from hgq2_amd.train import AdamW
+
+    gen = torch.Generator().manual_seed(18)
+    base = torch.randn(6, 40, generator=gen).to(dev)
+    views = [torch._neg_view(base), base[:1].expand(6, 40), base.t().contiguous().t(), torch.view_as_complex(base.view(6, 20, 2)).conj().imag.repeat(1, 2)]
+    for g in views:
+        a, b = (torch.nn.Parameter(torch.ones(6, 40, device=dev)) for _ in range(2))
+        a.grad, b.grad = g, g.clone(memory_format=torch.contiguous_format).resolve_neg()
+        one, two = AdamW([a], global_clipnorm=1.0), AdamW([b], global_clipnorm=1.0)
+        one.step(), two.step()
+        assert torch.equal(a, b) and torch.equal(one.momentum, two.momentum) and torch.equal(one.grad_norm, two.grad_norm)
+        assert torch.equal(ops.global_norm([g]), one.grad_norm)
+        c, state = torch.ones(6, 40, device=dev), ops.adamw_state(dev, 0.001)
+        ops.adamw_update_multi_([c], [g], [ops.adamw_moments(240, dev)], state, decay=[0.004], clipnorm=1.0)
+        assert torch.equal(c, a)
+    p = torch.nn.Parameter(torch.ones(6, 40, device=dev))
+    opt = AdamW([p])
+    p.data = torch._neg_view(p.data)
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match='stay contiguous'):
+        opt.step()
