@@ -170,11 +170,15 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 // A recorded backward pass hands the gradient of a leaf to the leaf's one accumulating node, on the stream that the node was made on.  One that
 // an earlier graph made on another stream, and keeps alive, would pull that stream into the recording, which ends the process.
-void accumulates_here(const char *name, const Tensor &t) {
-    if (!t.defined() || !t.requires_grad() || t.grad_fn()) return;
+bool accumulates_elsewhere(const Tensor &t) {
+    if (!t.defined() || !t.requires_grad() || t.grad_fn()) return false;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
     const auto stream = node ? node->stream() : std::nullopt;
-    if (!stream || stream->id() == c10::hip::getCurrentHIPStream(t.device().index()).id()) return;
+    return stream && stream->id() != c10::hip::getCurrentHIPStream(t.device().index()).id();
+}
+
+void accumulates_here(const char *name, const Tensor &t) {
+    if (!accumulates_elsewhere(t)) return;
     TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, name,
                 " belongs to a graph of another stream that is still alive: its backward pass cannot be recorded here (release what that graph gave, or "
                 "make it on this stream)");
@@ -408,6 +412,7 @@ TORCH_LIBRARY_IMPL(hgq, CPU, m) {
 
 PYBIND11_MODULE(_host, m) {
     m.def("bind", &bind);
+    m.def("accumulates_elsewhere", [](const py::handle &t) { return accumulates_elsewhere(tensor_of(t, "a variable")); });
     m.def("group_norm", [](const py::handle &x, int64_t groups, const py::handle &gamma, const py::handle &beta, double epsilon, int64_t act) {
         HANDLE_TH_ERRORS
         std::optional<Tensor> ga, be;

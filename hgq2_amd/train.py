@@ -291,6 +291,15 @@ class AdamW(SGD):
                 for p, c in post:
                     p.copy_(c(p))
 
+    def refuse_other_graphs(self, stream):
+        """Raises where a variable's gradients are accumulated by a living graph of another stream: a backward pass recorded on ``stream``
+        would pull that stream into the recording, which ends the process."""
+        with torch.cuda.stream(stream):
+            for p in self.params:
+                if _lib.native().accumulates_elsewhere(p):
+                    raise RuntimeError(f"{getattr(p, 'var_name', None) or 'a variable'} belongs to a graph of another stream that is still alive: the step "
+                                       'cannot be recorded (release what that graph gave, the loss of an eager step for instance)')
+
     def _specials(self, indices):
         """Hands over the gradient pieces, bounds and folded regularizers of these variables; the constraints to apply after the update."""
         post, inf = [], float('inf')
@@ -355,6 +364,8 @@ class GraphedTrainStep:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         self.opt.zero_grad(set_to_none=True)
+        if isinstance(self.opt, AdamW):
+            self.opt.refuse_other_graphs(side)
         self.graph = torch.cuda.CUDAGraph()
         # captured on the stream the warm-up ran on: scratch that operators keep per stream (allocated and cleared once,
         # during the warm-up) is found again instead of being created, and cleared, inside the graph

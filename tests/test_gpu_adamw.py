@@ -614,3 +614,24 @@ def test_gradients_that_are_views(dev):
     p.grad = torch.ones_like(p)
     with pytest.raises(ValueError, match='stay contiguous'):
         opt.step()
+
+
+def test_recording_beside_a_living_loss_is_refused(dev):
+    from hgq2_amd import ops
+    from hgq2_amd.train import AdamW, model_loss, train_step_for
+
+    gen = torch.Generator().manual_seed(20)
+    x, y = torch.randn(128, 16, generator=gen).to(dev), torch.randint(0, 5, (128,), generator=gen).to(dev)
+    net = _model(dev)
+    net(x, training=False)
+    opt = AdamW(net.parameters(), fold_regularizers=True)
+    for _ in range(2):
+        opt.zero_grad()
+        loss = model_loss(net, ops.sparse_ce(net(x, training=True), y), True)
+        opt.backward(loss)
+        opt.step()
+    with pytest.raises(RuntimeError, match='another stream that is still alive'):
+        train_step_for(net, x, y, optimizer='adamw')
+    del loss
+    step = train_step_for(net, x, y, optimizer='adamw')
+    assert math.isfinite(float(step())) and step.opt.iterations == 4

@@ -505,3 +505,31 @@ def test_two_threads(dev):
     [t.join() for t in threads]
     for a, b in zip(want, got):
         assert b is not None and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_recording_again_and_beside_a_living_loss(dev):
+    """A second recording of one model works; one beside the living loss of an eager step is refused and leaves everything usable."""
+    from hgq2_amd import ops
+    from hgq2_amd.config import LayerConfigScope, QuantizerConfigScope
+    from hgq2_amd.host import GroupNormalization, Sequential
+    from hgq2_amd.layers import QDense
+    from hgq2_amd.train import AdamW, model_loss, train_step_for
+
+    g = torch.Generator().manual_seed(19)
+    x, y = torch.rand(64, 12, generator=g).to(dev), torch.randint(0, 5, (64,), generator=g).to(dev)
+    with QuantizerConfigScope(place='all', default_q_type='kbi', overflow_mode='SAT_SYM'), \
+         QuantizerConfigScope(place='datalane', default_q_type='kif', overflow_mode='WRAP'), LayerConfigScope(enable_ebops=True, beta0=1e-6):
+        model = Sequential([QDense(24), GroupNormalization(3, activation='relu'), QDense(5)])
+    make = lambda v: AdamW(v, lr=0.003, fold_regularizers=True)  # noqa: E731
+    for _ in range(2):
+        step = train_step_for(model, x, y, optimizer=make)
+        assert all(math.isfinite(float(step())) for _ in range(3)) and step.opt.iterations == 6
+    opt = make(model.parameters())
+    loss = model_loss(model, ops.sparse_ce(model(x, training=True), y), True)
+    opt.backward(loss)
+    opt.step()
+    with pytest.raises(RuntimeError, match='belongs to a graph of another stream'):
+        train_step_for(model, x, y, optimizer=make)
+    del loss
+    step = train_step_for(model, x, y, optimizer=make)
+    assert all(math.isfinite(float(step())) for _ in range(3)) and step.opt.iterations == 6
