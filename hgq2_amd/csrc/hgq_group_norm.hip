@@ -395,9 +395,10 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
 }
 
 // phase 0: whole tiles; 1: sums of d rstd and d xhat rstd of every split, parts [B][splits][G][2], and the channels' sums; 2: join them, dx.
-// Every tile leaves its terms of dgamma and dbeta, slices [tiles][2 C] (NULL: not wanted).
-template <typename T, int ACT, bool ONE, int NV>
-__global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ gamma,
+// Every tile leaves its terms of dgamma and dbeta, slices [tiles][2 C] (NULL: not wanted).  MORE: rows of a thread beyond those in its registers, which it
+// keeps in LDS.
+template <typename T, int ACT, bool ONE, int NV, int MORE>
+__global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ gamma,
                                                             const float *__restrict__ beta, const float *__restrict__ mean_in,
                                                             const float *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ slices,
                                                             float *__restrict__ parts, GroupTile p, int phase) {
@@ -416,7 +417,11 @@ __global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict_
     const int r0 = split * p.split_rows, r1 = min(p.rows, r0 + p.split_rows);
     const T *xs = x + b * p.n, *ds = dy + b * p.n;
     const GroupRows rows(p, t, on, c0, r0, r1);
-    Four<T> v[NV], w[NV];
+    Four<T> v[NV], w[NV], more_v[MORE ? MORE : 1], more_w[MORE ? MORE : 1];
+    auto *const kept = (typename Four<T>::words *)(lds + ((2 * groups + 4 * blockDim.x + 3) & ~3u)) + threadIdx.x;  // [MORE][x, dy][threads]
+#pragma unroll
+    for (int i = 0; i < MORE; ++i)
+        if (NV + i < rows.full) more_v[i].load(xs + rows.at + (NV + i) * rows.step), more_w[i].load(ds + rows.at + (NV + i) * rows.step);
     float last[3] = {0, 0, 0}, dlast[3] = {0, 0, 0};
     if (phase == 2 && p.through) {
 #pragma unroll
@@ -430,6 +435,9 @@ __global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict_
 #pragma unroll
     for (int j = 0; j < 3; ++j)
         if (j < rows.rest) last[j] = to_f32(xs[rows.at + rows.full * rows.step + j]), dlast[j] = to_f32(ds[rows.at + rows.full * rows.step + j]);
+#pragma unroll
+    for (int i = 0; i < MORE; ++i)
+        if (NV + i < rows.full) kept[2 * i * blockDim.x] = more_v[i].w, kept[(2 * i + 1) * blockDim.x] = more_w[i].w;
     constexpr int N = ONE ? 1 : 4;  // groups of a thread's columns
     float mean[N], rstd[N], ga[4], scale[4], be[4];
 #pragma unroll
@@ -442,26 +450,31 @@ __global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict_
         const int c = p.fold > 1 ? (c0 + j) % p.C : c0 + j;
         ga[j] = t.on && gamma ? gamma[c] : 1.0f, scale[j] = rstd[j % N] * ga[j], be[j] = t.on && beta ? beta[c] : 0.0f;
     }
+    // rstd gamma: before a relu the two are needed by themselves, and their product is not kept beside them
+    auto times = [&](int j) { return ACT == HGQ_ACT_RELU ? rstd[j % N] * ga[j] : scale[j]; };
     float h[4] = {0, 0, 0, 0}, a[4] = {0, 0, 0, 0};  // of dz (x - mean) and of dz
     if (phase < 2) {
         float mine[2][4];
+        auto add = [&](float xv, float dv, int j) {
+            const float d = xv - mean[j % N], dz = through_activation<ACT>(dv, affine<ACT>(d, rstd[j % N], ga[j], scale[j], be[j]));
+            a[j] += dz, h[j] = fmaf(dz, d, h[j]);
+        };
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (i < rows.full)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float d = v[i].get(j) - mean[j % N], dz = through_activation<ACT>(w[i].get(j), affine<ACT>(d, rstd[j % N], ga[j], scale[j], be[j]));
-                    a[j] += dz, h[j] = fmaf(dz, d, h[j]);
-                }
+                for (int j = 0; j < 4; ++j) add(v[i].get(j), w[i].get(j), j);
+        for (int i = 0; i < MORE && NV + i < rows.full; ++i) {
+            const Four<T> x4 = {kept[2 * i * blockDim.x]}, d4 = {kept[(2 * i + 1) * blockDim.x]};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) add(x4.get(j), d4.get(j), j);
+        }
 #pragma unroll
         for (int j = 0; j < 3; ++j)
-            if (j < rows.rest) {
-                const float d = last[j] - mean[j % N], dz = through_activation<ACT>(dlast[j], affine<ACT>(d, rstd[j % N], ga[j], scale[j], be[j]));
-                a[j] += dz, h[j] = fmaf(dz, d, h[j]);
-            }
+            if (j < rows.rest) add(last[j], dlast[j], j);
         // sums of d rstd and of d xhat rstd: gamma rstd is what is at hand
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] *= rstd[j % N], mine[0][j] = a[j] * scale[j], mine[1][j] = h[j] * scale[j];
+        for (int j = 0; j < 4; ++j) h[j] *= rstd[j % N], mine[0][j] = a[j] * times(j), mine[1][j] = h[j] * times(j);
         if (phase == 1 || dx) {
             sum_groups<ONE>(p, t, mine[0], red, total);
             sum_groups<ONE>(p, t, mine[1], red, stat);
@@ -491,7 +504,7 @@ __global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict_
         T *out = dx + b * p.n;
         auto one = [&](float xv, float dv, int j) {
             const float d = xv - mean[j % N], dz = through_activation<ACT>(dv, affine<ACT>(d, rstd[j % N], ga[j], scale[j], be[j]));
-            return fmaf(dz, scale[j], fmaf(d, m2[j % N], m1[j % N]));
+            return fmaf(dz, times(j), fmaf(d, m2[j % N], m1[j % N]));
         };
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -503,6 +516,15 @@ __global__ __launch_bounds__(1024) void group_norm_bwd_tile(const T *__restrict_
                 v[i].set(o);
                 v[i].store(out + rows.at + i * rows.step, p.through);
             }
+        for (int i = 0; i < MORE && NV + i < rows.full; ++i) {
+            Four<T> x4 = {kept[2 * i * blockDim.x]};
+            const Four<T> d4 = {kept[(2 * i + 1) * blockDim.x]};
+            float o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = one(x4.get(j), d4.get(j), j);
+            x4.set(o);
+            x4.store(out + rows.at + (NV + i) * rows.step, p.through);
+        }
 #pragma unroll
         for (int j = 0; j < 3; ++j)
             if (j < rows.rest) out[rows.at + rows.full * rows.step + j] = (T)one(last[j], dlast[j], j);
@@ -569,6 +591,8 @@ constexpr int64_t MOST_SLICES = 2048;
 template <typename T>
 constexpr int MOST_HELD = 32 / sizeof(T);
 int most_held(int type) { return type == HGQ_TYPE_F32 ? MOST_HELD<float> : MOST_HELD<__bf16>; }
+// and further ones in LDS (backward, both tensors): 48 KB of a workgroup of 512 threads
+constexpr int in_lds(int most) { return 3 * most / 8; }
 
 // The tile's width for K of the groups; false: it is none (more than GROUP_THREADS accesses, or not whole ones)
 bool widen(GroupTile &p, int K) {
@@ -585,7 +609,7 @@ bool widen(GroupTile &p, int K) {
     return true;
 }
 
-// Lays out the tiles; false: the shape is left to the kernels for any shape.  held: accesses per thread (the kernel's NV).
+// Lays out the tiles; false: the shape is left to the kernels for any shape.  held: accesses per thread.
 bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, int G, int type, bool backward) {
     if (B == 0 || S == 0 || S > (1 << 29) / C || C > 65536) return false;  // (offsets within a sample, and a tile behind it, in 32 bits)
     p = {};
@@ -608,6 +632,13 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
         // spread little work over more threads
         held = B * p.chunks >= 512 ? most : 4;
         while ((p.rows + held - 1) / held * p.TX > GROUP_THREADS) held *= 2;
+        // The backward pass takes 120 registers: 16 wavefronts per compute unit.  A workgroup of 9 to 11 leaves it no second one to load
+        // while the first computes, one of 5 leaves four places empty: where rows kept in LDS bring it down to 8 or 4, two or four
+        // fit (1024 x 26 x 26 x 32 in 8 groups: fp32, 11 -> 8, 70 -> 54 us; bfloat16, 2048 samples in 4 groups, 6 -> 4, 98 -> 63 us).  Elsewhere they only
+        // cost (1024 x 20 x 20 x 32, 7 -> 5: 38 -> 48 us).
+        const int more = most + in_lds(most);
+        for (int fits = 512; backward && held == most && fits >= 256; fits /= 2)
+            if ((p.rows + most - 1) / most * p.TX > fits && (p.rows + more - 1) / more * p.TX <= fits) held = more;
         p.TY = (p.rows + held - 1) / held;
         p.splits = 1, p.split_rows = p.rows;
         const int one = p.TY * p.TX;  // small samples share a workgroup while there are enough of them
@@ -647,8 +678,9 @@ int64_t slices_floats(const GroupTile &p) { return 2 * (int64_t)p.C * (p.tiles +
 
 int64_t parts_floats(const GroupTile &p) { return p.splits > 1 ? p.B * p.splits * p.G * 2 : 0; }
 
-int lds_bytes(const GroupTile &p, int threads, bool backward) {
-    return 4 * (2 * p.NS * p.K + threads * (p.D % 4 == 0 && !backward ? 1 : 4));
+int lds_bytes(const GroupTile &p, int threads, int held, int type, bool backward) {
+    const int most = most_held(type), kept = held > most ? 16 + in_lds(most) * 2 * threads * (type == HGQ_TYPE_F32 ? 16 : 8) : 0;
+    return 4 * (2 * p.NS * p.K + threads * (p.D % 4 == 0 && !backward ? 1 : 4)) + kept;
 }
 
 unsigned any_grid(const GroupShape &s) { return (unsigned)(s.B * s.G < 1 << 20 ? s.B * s.G : 1 << 20); }
@@ -662,7 +694,11 @@ auto fwd_kernel(int held) {
 
 template <typename T, int ACT, bool ONE>
 auto bwd_kernel(int held) {
-    return held == 4 ? group_norm_bwd_tile<T, ACT, ONE, 4> : held == 8 ? group_norm_bwd_tile<T, ACT, ONE, 8> : group_norm_bwd_tile<T, ACT, ONE, MOST_HELD<T>>;
+    constexpr int most = MOST_HELD<T>;
+    return held > most ? group_norm_bwd_tile<T, ACT, ONE, most, in_lds(most)>
+           : held == 4 ? group_norm_bwd_tile<T, ACT, ONE, 4, 0>
+           : held == 8 ? group_norm_bwd_tile<T, ACT, ONE, 8, 0>
+                       : group_norm_bwd_tile<T, ACT, ONE, most, 0>;
 }
 
 template <typename T, int ACT>
@@ -678,7 +714,7 @@ int fwd(const void *x, const float *gamma, const float *beta, void *y, float *me
     if (p.splits > 1 && !ws) return fail(HGQ_ERR_ARG, "hgq_group_norm_fwd: null workspace");
     auto kernel = p.D % 4 == 0 ? fwd_kernel<T, ACT, true>(held) : fwd_kernel<T, ACT, false>(held);
     for (int phase = p.splits > 1 ? 1 : 0; phase < (p.splits > 1 ? 3 : 1); ++phase) {
-        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, false), st, (const T *)x, gamma, beta, (T *)y, mean, rstd, ws, p, phase);
+        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, held, type, false), st, (const T *)x, gamma, beta, (T *)y, mean, rstd, ws, p, phase);
         const int rc = check_launch("hgq_group_norm_fwd");
         if (rc) return rc;
     }
@@ -704,7 +740,7 @@ int bwd(const void *dy, const void *x, const float *gamma, const float *beta, co
     auto kernel = p.D % 4 == 0 ? bwd_kernel<T, ACT, true>(held) : bwd_kernel<T, ACT, false>(held);
     for (int phase = p.splits > 1 ? 1 : 0; phase < (p.splits > 1 ? 3 : 1); ++phase) {
         if (phase == 2 && !dx) break;
-        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, true), st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd,
+        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, held, type, true), st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd,
                            (T *)dx, slices, parts, p, phase);
         const int rc = check_launch("hgq_group_norm_bwd");
         if (rc) return rc;
