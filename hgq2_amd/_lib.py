@@ -277,7 +277,7 @@ def _load_native():
 
     @torch.library.register_fake('hgq::group_norm_fwd')
     def _(x, gamma, beta, groups, epsilon, act):
-        return torch.empty_like(x), x.new_empty((2, x.shape[0], groups), dtype=torch.float32)
+        return torch.empty_like(x), x.new_empty((2, x.shape[0], groups), dtype=torch.float64)
 
     @torch.library.register_fake('hgq::group_norm_bwd')
     def _(dy, x, gamma, beta, stats, groups, act, need_dx, need_dgamma, need_dbeta):

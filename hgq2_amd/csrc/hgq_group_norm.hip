@@ -4,6 +4,13 @@
 // Backward, with dz = dy act'(z) and d = dz gamma:
 //     dx = (d - mean(d) - xhat mean(d xhat)) / sqrt(var + eps);   dgamma[c] = sum dz xhat,  dbeta[c] = sum dz  over B and S
 // x, y, dy and dx have one of three types; everything between is fp32, the variance about the mean (not a difference of squares).
+//
+// The border of a relu.  Which side of zero z falls on decides whether a whole dy passes, and z within fp32's rounding of zero (one element in
+// some ten million) decides it by chance, for every evaluation in fp32 its own.  So before a relu mean and 1 / sqrt(var + eps) are formed in 64 bits
+// and handed to the backward pass as such; there z > 0 is x > t (x < t where gamma is negative) with t = mean - beta / (gamma rstd),
+// rounded to fp32 towards the side that changes no comparison with an fp32 x: the exact decision takes fewer instructions than z.
+#include <type_traits>
+
 #include "hgq_device.h"
 #include "hgq_host.h"
 
@@ -40,19 +47,29 @@ __device__ __forceinline__ float activate(float z) {
     return z;
 }
 
-// z of d = x - mean.  Before a relu the roundings follow the formula's order, (d rstd) gamma + beta: which side of zero a value falls on that
-// lies within rounding of it is then the same for every program that does so with the same mean (11 of 160 tensors of 22 million elements held
-// one that fell differently from an fp32 evaluation by elementary operations; 13 of 120 with d (rstd gamma) + beta in one rounding).
-template <int ACT>
-__device__ __forceinline__ float affine(float d, float rstd, float gamma, float scale, float beta) {
-    if (ACT == HGQ_ACT_RELU) return __fadd_rn(__fmul_rn(__fmul_rn(d, rstd), gamma), beta);
-    return fmaf(d, scale, beta);  // scale: rstd gamma
-}
+// Before a relu: (x - t) scale > 0 is z > 0, scale: gamma rstd.  A gamma of zero leaves beta alone to decide, by the sign of an infinite t; the
+// scale is then the smallest number, so that the product has that sign.
+struct ReluBorder {
+    float t, scale;
+    __device__ __forceinline__ void set(double mean, double rstd, float gamma, float beta) {
+        const double a = rstd * gamma;
+        scale = a == 0.0 ? 0x1p-149f : (float)a;
+        double inv = __builtin_amdgcn_rcp(a);  // and two steps of Newton's: a rounded division and rounding by library calls took 1 us a wavefront
+        inv = fma(fma(-a, inv, 1.0), inv, inv), inv = fma(fma(-a, inv, 1.0), inv, inv);
+        const double at = fma(-(double)beta, inv, mean);
+        t = (float)at;
+        if (((double)t - at) * a > 0.0) {  // rounded to the wrong side: the neighbour
+            const int bits = __float_as_int(t);
+            t = t == 0.0f ? (a > 0.0 ? -0x1p-149f : 0x1p-149f) : __int_as_float((t > 0.0f) == (a > 0.0) ? bits - 1 : bits + 1);
+        }
+        if (a == 0.0) t = beta > 0.0f ? -INFINITY : INFINITY;
+    }
+    __device__ __forceinline__ float through(float dy, float x) const { return (x - t) * scale > 0.0f ? dy : 0.0f; }
+};
 
-// dy act'(z)
+// dy act'(z), of silu and of no activation
 template <int ACT>
 __device__ __forceinline__ float through_activation(float dy, float z) {
-    if (ACT == HGQ_ACT_RELU) return z > 0.0f ? dy : z != z ? z : 0.0f;
     if (ACT == HGQ_ACT_SILU) {
         const float p = sigmoid(z);
         return dy * (p * fmaf(z, 1.0f - p, 1.0f));
@@ -75,7 +92,7 @@ __device__ __forceinline__ double group_sum(double v, double *lds) {
 // A workgroup takes one sample's group after another, any shape: the group is read three times, its sums are formed in fp64.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void group_norm_fwd_any(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
-                                                          T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, GroupShape s) {
+                                                          T *__restrict__ y, double *__restrict__ mean_out, double *__restrict__ rstd_out, GroupShape s) {
     __shared__ double lds[4];
     for (int64_t bg = blockIdx.x; bg < s.B * s.G; bg += gridDim.x) {
         const int64_t b = bg / s.G;
@@ -83,18 +100,20 @@ __global__ __launch_bounds__(256) void group_norm_fwd_any(const T *__restrict__ 
         const int64_t base = b * s.S * s.C + (int64_t)g * s.D, n = s.S * s.D;
         double sum = 0;
         for (int64_t e = threadIdx.x; e < n; e += 256) sum += to_f32(x[base + e / s.D * s.C + e % s.D]);
-        const float mean = (float)(group_sum(sum, lds) / (double)n);
+        const double mean64 = group_sum(sum, lds) / (double)n;
+        const float mean = (float)mean64;
         double sq = 0;
         for (int64_t e = threadIdx.x; e < n; e += 256) {
-            const float d = to_f32(x[base + e / s.D * s.C + e % s.D]) - mean;
-            sq += (double)d * d;
+            const double d = to_f32(x[base + e / s.D * s.C + e % s.D]) - mean64;
+            sq += d * d;
         }
-        const float rstd = 1.0f / sqrtf((float)(group_sum(sq, lds) / (double)n) + s.eps);
-        if (threadIdx.x == 0) mean_out[bg] = mean, rstd_out[bg] = rstd;
+        const double rstd64 = 1.0 / sqrt(group_sum(sq, lds) / (double)n + s.eps);
+        const float rstd = (float)rstd64;
+        if (threadIdx.x == 0) mean_out[bg] = mean64, rstd_out[bg] = rstd64;
         for (int64_t e = threadIdx.x; e < n; e += 256) {
             const int c = g * s.D + (int)(e % s.D);
             const int64_t at = base + e / s.D * s.C + e % s.D;
-            const float ga = gamma ? gamma[c] : 1.0f, z = affine<ACT>(to_f32(x[at]) - mean, rstd, ga, rstd * ga, beta ? beta[c] : 0.0f);
+            const float z = fmaf(to_f32(x[at]) - mean, rstd * (gamma ? gamma[c] : 1.0f), beta ? beta[c] : 0.0f);
             y[at] = (T)activate<ACT>(z);
         }
     }
@@ -103,8 +122,8 @@ __global__ __launch_bounds__(256) void group_norm_fwd_any(const T *__restrict__ 
 // A workgroup takes one sample's group after another, any shape.  part [B][2 C]: each sample's terms of dgamma, then of dbeta.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ gamma,
-                                                          const float *__restrict__ beta, const float *__restrict__ mean_in,
-                                                          const float *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ part, GroupShape s) {
+                                                          const float *__restrict__ beta, const double *__restrict__ mean_in,
+                                                          const double *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ part, GroupShape s) {
     __shared__ double lds[4];
     __shared__ double col[2][256];
     int tx = 1;  // threads side by side over channels, the others over positions
@@ -114,7 +133,13 @@ __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ 
         const int64_t b = bg / s.G;
         const int g = (int)(bg - b * s.G);
         const int64_t base = b * s.S * s.C + (int64_t)g * s.D, n = s.S * s.D;
-        const float mean = mean_in[bg], rstd = rstd_in[bg];
+        const float mean = (float)mean_in[bg], rstd = (float)rstd_in[bg];
+        auto through = [&](float dv, float xv, float xh, float ga, float be) {  // dz
+            if (ACT != HGQ_ACT_RELU) return through_activation<ACT>(dv, xh * ga + be);
+            ReluBorder border;
+            border.set(mean_in[bg], rstd_in[bg], ga, be);
+            return xh == xh ? border.through(dv, xv) : xh;
+        };
         double s1 = 0, s2 = 0;  // of d and d xhat, over the group
         for (int c0 = 0; c0 < s.D; c0 += tx) {
             const int d = c0 + cx, c = g * s.D + d;
@@ -123,8 +148,8 @@ __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ 
             if (d < s.D)
                 for (int64_t p = py; p < s.S; p += ty) {
                     const int64_t at = base + p * s.C + d;
-                    const float xh = (to_f32(x[at]) - mean) * rstd;
-                    const float dz = through_activation<ACT>(to_f32(dy[at]), xh * ga + be);
+                    const float xv = to_f32(x[at]), xh = (xv - mean) * rstd;
+                    const float dz = through(to_f32(dy[at]), xv, xh, ga, be);
                     a += dz, h += (double)dz * xh;
                 }
             s1 += a * ga, s2 += h * ga;
@@ -141,8 +166,8 @@ __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ 
         for (int64_t e = threadIdx.x; e < n; e += 256) {
             const int c = g * s.D + (int)(e % s.D);
             const int64_t at = base + e / s.D * s.C + e % s.D;
-            const float ga = gamma ? gamma[c] : 1.0f, xh = (to_f32(x[at]) - mean) * rstd;
-            const float dz = through_activation<ACT>(to_f32(dy[at]), xh * ga + (beta ? beta[c] : 0.0f));
+            const float ga = gamma ? gamma[c] : 1.0f, be = beta ? beta[c] : 0.0f, xv = to_f32(x[at]), xh = (xv - mean) * rstd;
+            const float dz = through(to_f32(dy[at]), xv, xh, ga, be);
             dx[at] = (T)((dz * ga - m1 - xh * m2) * rstd);
         }
     }
@@ -223,8 +248,8 @@ struct GroupRows {
 
 // Sums of one value per column (v[4] of each thread) over the rows and the columns of every group in the tile: total[NS * K] in LDS, to
 // all threads, in a fixed order.  ONE: a thread's columns are of one group, and it adds them first.  red: blockDim.x * (ONE ? 1 : 4).
-template <bool ONE>
-__device__ __forceinline__ void sum_groups(const GroupTile &p, const GroupThread &t, const float (&v)[4], float *red, float *total) {
+template <bool ONE, typename V>
+__device__ __forceinline__ void sum_groups(const GroupTile &p, const GroupThread &t, const V (&v)[4], V *red, V *total) {
     if (t.on) {
         if (ONE) {
             red[threadIdx.x] = (v[0] + v[1]) + (v[2] + v[3]);
@@ -238,8 +263,8 @@ __device__ __forceinline__ void sum_groups(const GroupTile &p, const GroupThread
     const int across = ONE ? p.D / 4 : p.D, width = ONE ? p.TX : p.TX * 4, cols = ONE ? across : across * p.fold;
     const int r0 = lane / cols, first = lane - r0 * cols, step = p.team / cols, rest = p.team - step * cols;
     for (int g = threadIdx.x / p.team; g < p.NS * p.K; g += blockDim.x / p.team) {
-        const float *mine = red + (g / p.K) * p.TY * width + (g % p.K) * across;
-        float sum = 0;
+        const V *mine = red + (g / p.K) * p.TY * width + (g % p.K) * across;
+        V sum = 0;
         for (int r = r0, c = first; r < p.TY;) {
             const int f = !ONE && p.fold > 1 ? c / across : 0;
             sum += mine[r * width + f * p.C + (c - f * across)];
@@ -262,11 +287,12 @@ __device__ __forceinline__ int group_of(const GroupTile &p, const GroupThread &t
 // phase 0: whole tiles; 1: mean and sum of squares about it of every split, parts [B][splits][G][2]; 2: join those, apply
 template <typename T, int ACT, bool ONE, int NV>
 __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
-                                                            T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out,
-                                                            float *__restrict__ parts, GroupTile p, int phase) {
+                                                            T *__restrict__ y, double *__restrict__ mean_out, double *__restrict__ rstd_out,
+                                                            double *__restrict__ parts, GroupTile p, int phase) {
+    typedef std::conditional_t<ACT == HGQ_ACT_RELU, double, float> V;  // of the sums and what they give
     extern __shared__ float lds[];
     const int groups = p.NS * p.K;
-    float *total = lds, *stat = lds + groups, *red = lds + 2 * groups;
+    V *total = (V *)lds, *stat = total + groups, *red = stat + groups;
     const GroupThread t(p);
     // the chunks of one sample share cache lines: their workgroups follow each other on one of the eight dies (blocks go round them)
     const int64_t blk = blockIdx.x;
@@ -296,8 +322,9 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
         if (j < rows.rest) last[j] = to_f32(xs[rows.at + rows.full * rows.step + j]);
     constexpr int N = ONE ? 1 : 4;  // means of a thread's columns
     float mean[N], rstd[N];
+    const V one = 1, eps = p.eps;
     if (phase < 2) {
-        float acc[4] = {0, 0, 0, 0};
+        V acc[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (i < rows.full)
@@ -308,9 +335,13 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
             if (j < rows.rest) acc[j] += last[j];
         sum_groups<ONE>(p, t, acc, red, total);
         // elements of a group in this tile
-        const float inv = p.splits == 1 ? p.inv : 1.0f / (float)((min(p.n / p.C, r1 * p.fold) - r0 * p.fold) * p.D);
+        const V inv = one / (V)(p.splits == 1 ? p.n / p.G : (min(p.n / p.C, r1 * p.fold) - r0 * p.fold) * p.D);
 #pragma unroll
-        for (int j = 0; j < N; ++j) mean[j] = t.on ? total[group_of<ONE>(p, t, j)] * inv : 0.0f;
+        for (int j = 0; j < N; ++j) mean[j] = t.on ? (float)(total[group_of<ONE>(p, t, j)] * inv) : 0.0f;
+        auto square = [&](float x, int j) {  // (about the mean's fp32 value: within 2^-24 of it, whose square is nothing)
+            const V d = x - mean[j % N];
+            acc[j] = fma(d, d, acc[j]);
+        };
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] = 0;
 #pragma unroll
@@ -318,65 +349,57 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
             if (i < rows.full) {
                 v[i].forget();
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float d = v[i].get(j) - mean[j % N];
-                    acc[j] = fmaf(d, d, acc[j]);
-                }
+                for (int j = 0; j < 4; ++j) square(v[i].get(j), j);
             }
 #pragma unroll
         for (int j = 0; j < 3; ++j)
-            if (j < rows.rest) {
-                const float d = last[j] - mean[j % N];
-                acc[j] = fmaf(d, d, acc[j]);
-            }
+            if (j < rows.rest) square(last[j], j);
         sum_groups<ONE>(p, t, acc, red, stat);
         for (int g = threadIdx.x; g < groups; g += blockDim.x) {
             const int64_t bg = z / p.splits * p.NS + g / p.K;
             if (bg >= p.B) break;
             const int64_t at = bg * p.G + chunk * p.K + g % p.K;
             if (phase == 1) {
-                float *out = parts + ((bg * p.splits + split) * p.G + chunk * p.K + g % p.K) * 2;
+                double *out = parts + ((bg * p.splits + split) * p.G + chunk * p.K + g % p.K) * 2;
                 out[0] = total[g] * inv, out[1] = stat[g];
             } else {
-                mean_out[at] = total[g] * inv, rstd_out[at] = 1.0f / sqrtf(stat[g] * p.inv + p.eps);
+                mean_out[at] = total[g] * inv, rstd_out[at] = one / sqrt(stat[g] * inv + eps);
             }
         }
         if (phase == 1) return;
 #pragma unroll
-        for (int j = 0; j < N; ++j) rstd[j] = t.on ? 1.0f / sqrtf(stat[group_of<ONE>(p, t, j)] * p.inv + p.eps) : 0.0f;
+        for (int j = 0; j < N; ++j) rstd[j] = t.on ? (float)(one / sqrt(stat[group_of<ONE>(p, t, j)] * inv + eps)) : 0.0f;
     } else {
-        // the splits' means about the first one's, and their squares about the joint mean
+        // the splits' means, and their squares about the joint one
         const int lane = threadIdx.x & (p.team - 1);
         for (int g = threadIdx.x / p.team; g < groups; g += blockDim.x / p.team) {
-            const float *in = parts + (b - t.s) * p.splits * p.G * 2 + (chunk * p.K + g) * 2;  // (one sample: NS = 1)
-            const float first = in[0];
-            float m = 0, q = 0;
-            for (int k = lane; k < p.splits; k += p.team) {
-                const float w = (float)((min(p.n / p.C, (k + 1) * p.split_rows * p.fold) - k * p.split_rows * p.fold) * p.D) * p.inv;
-                m += w * (in[(int64_t)k * p.G * 2] - first);
-            }
+            const double *in = parts + (b - t.s) * p.splits * p.G * 2 + (chunk * p.K + g) * 2;  // (one sample: NS = 1)
+            const double all = 1.0 / (double)(p.n / p.G);
+            auto share = [&](int k) { return (double)((min(p.n / p.C, (k + 1) * p.split_rows * p.fold) - k * p.split_rows * p.fold) * p.D) * all; };
+            double m = 0, q = 0;
+            for (int k = lane; k < p.splits; k += p.team) m += share(k) * in[(int64_t)k * p.G * 2];
             for (int d = p.team / 2; d; d >>= 1) m += __shfl_xor(m, d);
             for (int k = lane; k < p.splits; k += p.team) {
-                const float w = (float)((min(p.n / p.C, (k + 1) * p.split_rows * p.fold) - k * p.split_rows * p.fold) * p.D) * p.inv;
-                const float d = in[(int64_t)k * p.G * 2] - first - m;
-                q += in[(int64_t)k * p.G * 2 + 1] * p.inv + w * d * d;
+                const double d = in[(int64_t)k * p.G * 2] - m;
+                q += in[(int64_t)k * p.G * 2 + 1] * all + share(k) * d * d;
             }
             for (int d = p.team / 2; d; d >>= 1) q += __shfl_xor(q, d);
             if (lane == 0) {
-                total[g] = first + m, stat[g] = 1.0f / sqrtf(q + p.eps);
-                if (split == 0) mean_out[(b - t.s) * p.G + chunk * p.K + g] = total[g], rstd_out[(b - t.s) * p.G + chunk * p.K + g] = stat[g];
+                const double r = 1.0 / sqrt(q + (double)p.eps);
+                total[g] = (V)m, stat[g] = (V)r;
+                if (split == 0) mean_out[(b - t.s) * p.G + chunk * p.K + g] = m, rstd_out[(b - t.s) * p.G + chunk * p.K + g] = r;
             }
         }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < N; ++j) mean[j] = t.on ? total[group_of<ONE>(p, t, j)] : 0.0f, rstd[j] = t.on ? stat[group_of<ONE>(p, t, j)] : 0.0f;
+        for (int j = 0; j < N; ++j) mean[j] = t.on ? (float)total[group_of<ONE>(p, t, j)] : 0.0f, rstd[j] = t.on ? (float)stat[group_of<ONE>(p, t, j)] : 0.0f;
     }
     if (!on) return;
-    float ga[4], scale[4], be[4];
+    float scale[4], be[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = p.fold > 1 ? (c0 + j) % p.C : c0 + j;
-        ga[j] = gamma ? gamma[c] : 1.0f, scale[j] = rstd[j % N] * ga[j], be[j] = beta ? beta[c] : 0.0f;
+        scale[j] = rstd[j % N] * (gamma ? gamma[c] : 1.0f), be[j] = beta ? beta[c] : 0.0f;
     }
     T *ys = y + b * p.n;
 #pragma unroll
@@ -385,13 +408,13 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
             v[i].forget();
             float out[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) out[j] = activate<ACT>(affine<ACT>(v[i].get(j) - mean[j % N], rstd[j % N], ga[j], scale[j], be[j]));
+            for (int j = 0; j < 4; ++j) out[j] = activate<ACT>(fmaf(v[i].get(j) - mean[j % N], scale[j], be[j]));
             v[i].set(out);
             v[i].store(ys + rows.at + i * rows.step, p.through);
         }
 #pragma unroll
     for (int j = 0; j < 3; ++j)
-        if (j < rows.rest) ys[rows.at + rows.full * rows.step + j] = (T)activate<ACT>(affine<ACT>(last[j] - mean[j % N], rstd[j % N], ga[j], scale[j], be[j]));
+        if (j < rows.rest) ys[rows.at + rows.full * rows.step + j] = (T)activate<ACT>(fmaf(last[j] - mean[j % N], scale[j], be[j]));
 }
 
 // phase 0: whole tiles; 1: sums of d rstd and d xhat rstd of every split, parts [B][splits][G][2], and the channels' sums; 2: join them, dx.
@@ -399,8 +422,8 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
 // keeps in LDS.
 template <typename T, int ACT, bool ONE, int NV, int MORE>
 __global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ gamma,
-                                                            const float *__restrict__ beta, const float *__restrict__ mean_in,
-                                                            const float *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ slices,
+                                                            const float *__restrict__ beta, const double *__restrict__ mean_in,
+                                                            const double *__restrict__ rstd_in, T *__restrict__ dx, float *__restrict__ slices,
                                                             float *__restrict__ parts, GroupTile p, int phase) {
     extern __shared__ float lds[];
     const int groups = p.NS * p.K;
@@ -417,6 +440,23 @@ __global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(cons
     const int r0 = split * p.split_rows, r1 = min(p.rows, r0 + p.split_rows);
     const T *xs = x + b * p.n, *ds = dy + b * p.n;
     const GroupRows rows(p, t, on, c0, r0, r1);
+    // A relu's borders, one per column and sample: shared out over the threads and handed on through LDS (every thread for its own four columns:
+    // 1024 x 26 x 26 x 32, 57 us for 53); asked for ahead of the tile.
+    const int width = p.TX * 4, borders = ACT == HGQ_ACT_RELU && p.TY > 1 ? p.NS * width : 0;
+    struct {
+        double mean = 0, rstd = 0;
+        float gamma = 1, beta = 0;
+    } its;
+    auto ask = [&](int k) {
+        const int col = k % width, c = p.fold > 1 ? col % p.C : chunk * p.K * p.D + col;
+        const int64_t of = z / p.splits * p.NS + k / width;
+        if (of >= p.B) return;
+        const int64_t g = of * p.G + c / p.D;
+        its.mean = mean_in[g], its.rstd = rstd_in[g];
+        if (gamma) its.gamma = gamma[c];
+        if (beta) its.beta = beta[c];
+    };
+    if ((int)threadIdx.x < borders) ask(threadIdx.x);
     Four<T> v[NV], w[NV], more_v[MORE ? MORE : 1], more_w[MORE ? MORE : 1];
     auto *const kept = (typename Four<T>::words *)(lds + ((2 * groups + 4 * blockDim.x + 3) & ~3u)) + threadIdx.x;  // [MORE][x, dy][threads]
 #pragma unroll
@@ -439,24 +479,47 @@ __global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(cons
     for (int i = 0; i < MORE; ++i)
         if (NV + i < rows.full) kept[2 * i * blockDim.x] = more_v[i].w, kept[(2 * i + 1) * blockDim.x] = more_w[i].w;
     constexpr int N = ONE ? 1 : 4;  // groups of a thread's columns
-    float mean[N], rstd[N], ga[4], scale[4], be[4];
+    float mean[N], rstd[N], scale[4], be[4];
+    ReluBorder relu[4];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         const int64_t g = b * p.G + chunk * p.K + group_of<ONE>(p, t, j) - t.s * p.K;
-        mean[j] = on ? mean_in[g] : 0.0f, rstd[j] = on ? rstd_in[g] : 0.0f;
+        mean[j] = on ? (float)mean_in[g] : 0.0f, rstd[j] = on ? (float)rstd_in[g] : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = p.fold > 1 ? (c0 + j) % p.C : c0 + j;
-        ga[j] = t.on && gamma ? gamma[c] : 1.0f, scale[j] = rstd[j % N] * ga[j], be[j] = t.on && beta ? beta[c] : 0.0f;
+        const float ga = t.on && gamma ? gamma[c] : 1.0f;
+        be[j] = t.on && beta ? beta[c] : 0.0f, scale[j] = rstd[j % N] * ga;
+        relu[j].t = relu[j].scale = 0;
+        if (ACT == HGQ_ACT_RELU && on && !borders) {
+            const int64_t g = b * p.G + chunk * p.K + group_of<ONE>(p, t, j) - t.s * p.K;
+            relu[j].set(mean_in[g], rstd_in[g], ga, be[j]);
+        }
     }
-    // rstd gamma: before a relu the two are needed by themselves, and their product is not kept beside them
-    auto times = [&](int j) { return ACT == HGQ_ACT_RELU ? rstd[j % N] * ga[j] : scale[j]; };
+    if (borders) {
+        for (int k = threadIdx.x; k < borders; k += blockDim.x) {
+            if (k != (int)threadIdx.x) ask(k);
+            ReluBorder it;
+            it.set(its.mean, its.rstd, its.gamma, its.beta);
+            red[2 * k] = it.t, red[2 * k + 1] = it.scale;
+        }
+        __syncthreads();
+        if (on)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) relu[j] = {red[2 * (t.s * width + t.col + j)], red[2 * (t.s * width + t.col + j) + 1]};
+        __syncthreads();
+    }
+    auto times = [&](int j) { return ACT == HGQ_ACT_RELU ? relu[j].scale : scale[j]; };  // rstd gamma
+    auto through = [&](float dv, float xv, float d, int j) {  // dz
+        if (ACT == HGQ_ACT_RELU) return relu[j].through(dv, xv);
+        return through_activation<ACT>(dv, fmaf(d, scale[j], be[j]));
+    };
     float h[4] = {0, 0, 0, 0}, a[4] = {0, 0, 0, 0};  // of dz (x - mean) and of dz
     if (phase < 2) {
         float mine[2][4];
         auto add = [&](float xv, float dv, int j) {
-            const float d = xv - mean[j % N], dz = through_activation<ACT>(dv, affine<ACT>(d, rstd[j % N], ga[j], scale[j], be[j]));
+            const float d = xv - mean[j % N], dz = through(dv, xv, d, j);
             a[j] += dz, h[j] = fmaf(dz, d, h[j]);
         };
 #pragma unroll
@@ -472,6 +535,9 @@ __global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(cons
 #pragma unroll
         for (int j = 0; j < 3; ++j)
             if (j < rows.rest) add(last[j], dlast[j], j);
+        if (ACT == HGQ_ACT_RELU)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = fmaf(0.0f, mean[j % N], a[j]);  // (a sample that is not finite)
         // sums of d rstd and of d xhat rstd: gamma rstd is what is at hand
 #pragma unroll
         for (int j = 0; j < 4; ++j) h[j] *= rstd[j % N], mine[0][j] = a[j] * times(j), mine[1][j] = h[j] * times(j);
@@ -503,8 +569,8 @@ __global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(cons
         for (int j = 0; j < N; ++j) m1[j] = -total[group_of<ONE>(p, t, j)] * p.inv, m2[j] = -stat[group_of<ONE>(p, t, j)] * p.inv * rstd[j];
         T *out = dx + b * p.n;
         auto one = [&](float xv, float dv, int j) {
-            const float d = xv - mean[j % N], dz = through_activation<ACT>(dv, affine<ACT>(d, rstd[j % N], ga[j], scale[j], be[j]));
-            return fmaf(dz, times(j), fmaf(d, m2[j % N], m1[j % N]));
+            const float d = xv - mean[j % N];
+            return fmaf(through(dv, xv, d, j), times(j), fmaf(d, m2[j % N], m1[j % N]));
         };
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -531,7 +597,7 @@ __global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(cons
     }
     if (!slices || phase == 2) return;
     // this tile's sums per channel: over its rows and samples, the folded positions with them
-    const int width = p.TX * 4, cols = p.K * p.D, folds = p.fold == 4 ? 2 : p.fold - 1, count = (p.NS * p.TY) << folds;  // (fold = 1, 2 or 4)
+    const int cols = p.K * p.D, folds = p.fold == 4 ? 2 : p.fold - 1, count = (p.NS * p.TY) << folds;  // (fold = 1, 2 or 4)
     int team = 1;
     while (team < 64 && team * 2 * cols <= (int)blockDim.x) team *= 2;
     const int lane = threadIdx.x & (team - 1);
@@ -596,6 +662,7 @@ constexpr int in_lds(int most) { return 3 * most / 8; }
 
 // The tile's width for K of the groups; false: it is none (more than GROUP_THREADS accesses, or not whole ones)
 bool widen(GroupTile &p, int K) {
+    if (K > 1024) return false;  // (their sums lie in LDS)
     p.K = K;
     p.fold = K < p.G ? 1 : p.C % 4 == 0 ? 1 : p.C % 2 == 0 ? 2 : 4;
     if (K < p.G && (int64_t)K * p.D % 4) return false;
@@ -676,11 +743,12 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
 // the tiles' terms of dgamma and dbeta, and runs of them added up where they are many
 int64_t slices_floats(const GroupTile &p) { return 2 * (int64_t)p.C * (p.tiles + (p.tiles > MOST_SLICES ? (p.tiles + SLICE_RUN - 1) / SLICE_RUN : 0)); }
 
-int64_t parts_floats(const GroupTile &p) { return p.splits > 1 ? p.B * p.splits * p.G * 2 : 0; }
+int64_t parts_floats(const GroupTile &p, bool backward) { return p.splits > 1 ? p.B * p.splits * p.G * (backward ? 2 : 4) : 0; }
 
-int lds_bytes(const GroupTile &p, int threads, int held, int type, bool backward) {
+int lds_bytes(const GroupTile &p, int threads, int held, int type, int act, bool backward) {
     const int most = most_held(type), kept = held > most ? 16 + in_lds(most) * 2 * threads * (type == HGQ_TYPE_F32 ? 16 : 8) : 0;
-    return 4 * (2 * p.NS * p.K + threads * (p.D % 4 == 0 && !backward ? 1 : 4)) + kept;
+    const int size = act == HGQ_ACT_RELU && !backward ? 8 : 4;
+    return size * (2 * p.NS * p.K + threads * (p.D % 4 == 0 && !backward ? 1 : 4)) + kept;
 }
 
 unsigned any_grid(const GroupShape &s) { return (unsigned)(s.B * s.G < 1 << 20 ? s.B * s.G : 1 << 20); }
@@ -702,7 +770,7 @@ auto bwd_kernel(int held) {
 }
 
 template <typename T, int ACT>
-int fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, float *ws, const GroupShape &s, int type,
+int fwd(const void *x, const float *gamma, const float *beta, void *y, double *mean, double *rstd, float *ws, const GroupShape &s, int type,
         hipStream_t st) {
     GroupTile p;
     int held, threads;
@@ -714,7 +782,7 @@ int fwd(const void *x, const float *gamma, const float *beta, void *y, float *me
     if (p.splits > 1 && !ws) return fail(HGQ_ERR_ARG, "hgq_group_norm_fwd: null workspace");
     auto kernel = p.D % 4 == 0 ? fwd_kernel<T, ACT, true>(held) : fwd_kernel<T, ACT, false>(held);
     for (int phase = p.splits > 1 ? 1 : 0; phase < (p.splits > 1 ? 3 : 1); ++phase) {
-        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, held, type, false), st, (const T *)x, gamma, beta, (T *)y, mean, rstd, ws, p, phase);
+        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, held, type, ACT, false), st, (const T *)x, gamma, beta, (T *)y, mean, rstd, (double *)ws, p, phase);
         const int rc = check_launch("hgq_group_norm_fwd");
         if (rc) return rc;
     }
@@ -722,7 +790,7 @@ int fwd(const void *x, const float *gamma, const float *beta, void *y, float *me
 }
 
 template <typename T, int ACT>
-int bwd(const void *dy, const void *x, const float *gamma, const float *beta, const float *mean, const float *rstd, void *dx, float *dgamma,
+int bwd(const void *dy, const void *x, const float *gamma, const float *beta, const double *mean, const double *rstd, void *dx, float *dgamma,
         float *dbeta, float *ws, const GroupShape &s, int type, hipStream_t st) {
     const bool sums = dgamma || dbeta;
     GroupTile p;
@@ -740,7 +808,7 @@ int bwd(const void *dy, const void *x, const float *gamma, const float *beta, co
     auto kernel = p.D % 4 == 0 ? bwd_kernel<T, ACT, true>(held) : bwd_kernel<T, ACT, false>(held);
     for (int phase = p.splits > 1 ? 1 : 0; phase < (p.splits > 1 ? 3 : 1); ++phase) {
         if (phase == 2 && !dx) break;
-        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, held, type, true), st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd,
+        hipLaunchKernelGGL(kernel, dim3(blocks(p)), dim3(threads), lds_bytes(p, threads, held, type, ACT, true), st, (const T *)dy, (const T *)x, gamma, beta, mean, rstd,
                            (T *)dx, slices, parts, p, phase);
         const int rc = check_launch("hgq_group_norm_bwd");
         if (rc) return rc;
@@ -770,17 +838,17 @@ extern "C" int64_t hgq_group_norm_fwd_workspace(int64_t B, int64_t S, int C, int
     if (check_shape("hgq_group_norm_fwd_workspace", B, S, C, G, HGQ_ACT_NONE, type)) return -1;
     GroupTile p;
     int held, threads;
-    return plan(p, held, threads, B, S, C, G, type, false) ? parts_floats(p) : 0;
+    return plan(p, held, threads, B, S, C, G, type, false) ? parts_floats(p, false) : 0;
 }
 
 extern "C" int64_t hgq_group_norm_bwd_workspace(int64_t B, int64_t S, int C, int G, int type) {
     if (check_shape("hgq_group_norm_bwd_workspace", B, S, C, G, HGQ_ACT_NONE, type)) return -1;
     GroupTile p;
     int held, threads;
-    return plan(p, held, threads, B, S, C, G, type, true) ? slices_floats(p) + parts_floats(p) : B * 2 * C;
+    return plan(p, held, threads, B, S, C, G, type, true) ? slices_floats(p) + parts_floats(p, true) : B * 2 * C;
 }
 
-extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, float *workspace,
+extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float *beta, void *y, double *mean, double *rstd, float *workspace,
                                   int64_t B, int64_t S, int C, int G, float eps, int act, int type, void *stream) {
     int rc = check_shape("hgq_group_norm_fwd", B, S, C, G, act, type);
     if (rc) return rc;
@@ -791,7 +859,7 @@ extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float
     return (type == HGQ_TYPE_F32 ? fwd_of<float>(act) : type == HGQ_TYPE_BF16 ? fwd_of<__bf16>(act) : fwd_of<_Float16>(act))(x, gamma, beta, y, mean, rstd, workspace, s, type, (hipStream_t)stream);
 }
 
-extern "C" int hgq_group_norm_bwd(const void *dy, const void *x, const float *gamma, const float *beta, const float *mean, const float *rstd,
+extern "C" int hgq_group_norm_bwd(const void *dy, const void *x, const float *gamma, const float *beta, const double *mean, const double *rstd,
                                   void *dx, float *dgamma, float *dbeta, float *workspace, int64_t B, int64_t S, int C, int G, int act, int type,
                                   void *stream) {
     int rc = check_shape("hgq_group_norm_bwd", B, S, C, G, act, type);

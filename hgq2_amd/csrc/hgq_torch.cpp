@@ -95,9 +95,9 @@ std::tuple<Tensor, Tensor> group_norm_fwd(const Tensor &x, const Tensor &gamma, 
     const GroupSizes s = group_sizes(x, groups);
     channel_vector("gamma", gamma, x), channel_vector("beta", beta, x);
     const c10::DeviceGuard guard(x.device());
-    Tensor y = at::empty_like(x), stats = at::empty({2, s.B, s.G}, x.options().dtype(at::kFloat));
+    Tensor y = at::empty_like(x), stats = at::empty({2, s.B, s.G}, x.options().dtype(at::kDouble));
     const Workspace<float> ws(library().group_norm_fwd_workspace(s.B, s.S, (int)s.C, s.G, s.type));
-    float *mean = floats(stats);
+    double *mean = (double *)memory(stats);
     check(lib.group_norm_fwd(memory(x), floats(gamma), floats(beta), memory(y), mean, mean ? mean + s.B * s.G : nullptr, ws.get(),
                              s.B, s.S, (int)s.C, s.G, (float)epsilon, (int)act, s.type, stream_of(x)),
           "hgq_group_norm_fwd");
@@ -110,13 +110,13 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_bwd(const Tensor &dy, const Tensor
     channel_vector("gamma", gamma, x), channel_vector("beta", beta, x);
     TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && dy.device() == x.device() && dy.is_contiguous(),
                       "dy must be contiguous and like x, got ", dy.scalar_type(), " ", dy.sizes(), " on ", dy.device());
-    TORCH_CHECK_VALUE(stats.numel() == 2 * s.B * s.G && stats.scalar_type() == at::kFloat && stats.device() == x.device() && stats.is_contiguous(),
+    TORCH_CHECK_VALUE(stats.numel() == 2 * s.B * s.G && stats.scalar_type() == at::kDouble && stats.device() == x.device() && stats.is_contiguous(),
                       "stats must be what the forward call left");
     const c10::DeviceGuard guard(x.device());
     Tensor dx = need_dx ? at::empty_like(x) : at::empty({0}, x.options()), dgamma = vector_like(need_dgamma ? s.C : 0, x),
            dbeta = vector_like(need_dbeta ? s.C : 0, x);
     const Workspace<float> ws(library().group_norm_bwd_workspace(s.B, s.S, (int)s.C, s.G, s.type));
-    const float *mean = floats(stats);
+    const double *mean = (const double *)memory(stats);
     check(lib.group_norm_bwd(memory(dy), memory(x), floats(gamma), floats(beta), mean, mean ? mean + s.B * s.G : nullptr, memory(dx), floats(dgamma),
                              floats(dbeta), ws.get(), s.B, s.S, (int)s.C, s.G, (int)act, s.type, stream_of(x)),
           "hgq_group_norm_bwd");

@@ -1078,15 +1078,15 @@ int hgq_fill_u32(uint32_t *p, uint32_t value, int64_t n, void *stream);
  * Group normalisation with an activation over channels-last tensors (keras.layers.GroupNormalization beside the reference's
  * layers; src/hgq/layers/batch_normalization.py normalises over the batch instead), x [B, S, C] with S positions and C channels in G groups:
  *     xhat = (x - mean) / sqrt(var + eps) over a sample's group;   z = xhat gamma[c] + beta[c];   y = act(z)
- * x, y, dy, dx: `type` (HGQ_TYPE_*), all else fp32.  gamma, beta [C] or NULL (1, 0); mean, rstd [B, G] are written by the forward
- * call and read by the backward one; act HGQ_ACT_NONE, _RELU or _SILU.  dx, dgamma [C], dbeta [C]: NULL = not wanted; the latter are sums
- * over B and S in an order that depends on the shape alone.  workspace: *_workspace(...) floats (0: NULL will do; -1: bad arguments).
+ * x, y, dy, dx: `type` (HGQ_TYPE_*), all else fp32.  gamma, beta [C] or NULL (1, 0); mean, rstd [B, G] (fp64: before a relu the backward
+ * call decides in 64 bits what lies within fp32's rounding of its border) are written by the forward call and read by the backward one; act HGQ_ACT_NONE, _RELU or _SILU.  dx, dgamma [C], dbeta [C]: NULL = not wanted; the latter are sums
+ * over B and S in an order that depends on the shape alone.  workspace: *_workspace(...) floats at a multiple of 8 bytes (0: NULL will do; -1: bad arguments).
  */
 int64_t hgq_group_norm_fwd_workspace(int64_t B, int64_t S, int C, int G, int type);
-int hgq_group_norm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, float *workspace, int64_t B,
+int hgq_group_norm_fwd(const void *x, const float *gamma, const float *beta, void *y, double *mean, double *rstd, float *workspace, int64_t B,
                        int64_t S, int C, int G, float eps, int act, int type, void *stream);
 int64_t hgq_group_norm_bwd_workspace(int64_t B, int64_t S, int C, int G, int type);
-int hgq_group_norm_bwd(const void *dy, const void *x, const float *gamma, const float *beta, const float *mean, const float *rstd, void *dx,
+int hgq_group_norm_bwd(const void *dy, const void *x, const float *gamma, const float *beta, const double *mean, const double *rstd, void *dx,
                        float *dgamma, float *dbeta, float *workspace, int64_t B, int64_t S, int C, int G, int act, int type, void *stream);
 
 #ifdef __cplusplus

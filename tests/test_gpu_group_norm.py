@@ -541,3 +541,32 @@ def test_recording_again_and_beside_a_living_loss(dev):
                                            ((520, 681, 27), 9, torch.float16), ((520, 26, 26, 64), 8, torch.float16), ((512, 360, 32), 4, torch.float32)])
 def test_rows_in_lds(dev, shape, G, dtype, act):
     _run(dev, shape, G, dtype, act, sum(shape) + G)
+
+
+@pytest.mark.parametrize('shape,dtype', [((1024, 26, 26, 32), torch.float32), ((2, 30000, 32), torch.float32), ((40, 30, 48), torch.float16), ((2, 3, 5000), torch.float32)])
+def test_the_side_of_a_relus_border(dev, shape, dtype):
+    """x next to where z is zero, to both sides, for gammas of both signs and zero: with dy = 1, dx shows what passes.  In 64 bits from the statistics
+    that the operator reports, so no rounding but theirs counts."""
+    g = torch.Generator().manual_seed(21)
+    C, G = shape[-1], 2
+    from hgq2_amd import _lib
+
+    _lib.native()
+    x = torch.randn(shape, generator=g).to(dtype).to(dev)
+    gamma, beta = torch.randn(C, generator=g).to(dev), 0.5 * torch.randn(C, generator=g).to(dev)
+    gamma[3], gamma[4], beta[3], beta[4] = 0.0, 0.0, 0.7, -0.7
+    for _ in range(3):  # (moving elements to the border moves the statistics a little: again)
+        y, stats = torch.ops.hgq.group_norm_fwd(x, gamma, beta, G, 1e-3, 1)
+        flat = x.view(shape[0], -1, C)
+        mean, rstd = (t.view(shape[0], 1, G).repeat_interleave(C // G, dim=2) for t in stats)
+        at = (mean - beta.double() / (gamma.double() * rstd)).to(dtype)
+        for k in range(min(3, flat.shape[1])):
+            row = at[:, 0] if k == 0 else torch.nextafter(at[:, 0].float(), torch.full_like(at[:, 0].float(), math.inf if k == 1 else -math.inf)).to(dtype)
+            flat[:, k] = torch.where(torch.isfinite(row), row, flat[:, k])
+    y, stats = torch.ops.hgq.group_norm_fwd(x, gamma, beta, G, 1e-3, 1)
+    mean, rstd = (t.view(shape[0], 1, G).repeat_interleave(C // G, dim=2) for t in stats)
+    passes = (x.view(shape[0], -1, C).double() - mean) * rstd * gamma.double() + beta.double() > 0
+    assert passes[..., 3].all() and not passes[..., 4].any()
+    dy = torch.ones_like(x)
+    _, _, dbeta = torch.ops.hgq.group_norm_bwd(dy, x, gamma, beta, stats, G, 1, True, True, True)
+    assert torch.equal(dbeta.double(), passes.sum(dim=(0, 1)).double())  # (counts below 2^24 are exact)
