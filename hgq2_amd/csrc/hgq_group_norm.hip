@@ -704,7 +704,7 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
         // fit (1024 x 26 x 26 x 32 in 8 groups: fp32, 11 -> 8, 70 -> 54 us; bfloat16, 2048 samples in 4 groups, 6 -> 4, 98 -> 63 us).  Elsewhere they only
         // cost (1024 x 20 x 20 x 32, 7 -> 5: 38 -> 48 us).
         const int more = most + in_lds(most);
-        for (int fits = 512; backward && held == most && fits >= 256; fits /= 2)
+        for (int fits = 512; backward && held == most && p.K <= 512 && fits >= 256; fits /= 2)  // (K: 64 KB hold the rows and the groups' sums)
             if ((p.rows + most - 1) / most * p.TX > fits && (p.rows + more - 1) / more * p.TX <= fits) held = more;
         p.TY = (p.rows + held - 1) / held;
         p.splits = 1, p.split_rows = p.rows;

@@ -538,7 +538,8 @@ def test_recording_again_and_beside_a_living_loss(dev):
 # tiles of which some rows lie in LDS: groups of whole accesses and others, rows of two and four positions with a short last one, 8 and 4 wavefronts
 @pytest.mark.parametrize('act', ['linear', 'relu', 'silu'])
 @pytest.mark.parametrize('shape,G,dtype', [((600, 26, 26, 32), 8, torch.float32), ((520, 551, 30), 10, torch.float32), ((513, 26, 26, 32), 4, torch.bfloat16),
-                                           ((520, 681, 27), 9, torch.float16), ((520, 26, 26, 64), 8, torch.float16), ((512, 360, 32), 4, torch.float32)])
+                                           ((520, 681, 27), 9, torch.float16), ((520, 26, 26, 64), 8, torch.float16), ((512, 360, 32), 4, torch.float32),
+                                           ((512, 20, 1024), 1024, torch.float32), ((512, 20, 1024), 512, torch.float32)])
 def test_rows_in_lds(dev, shape, G, dtype, act):
     _run(dev, shape, G, dtype, act, sum(shape) + G)
 
