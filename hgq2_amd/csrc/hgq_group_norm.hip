@@ -47,24 +47,28 @@ __device__ __forceinline__ float activate(float z) {
     return z;
 }
 
-// Before a relu: (x - t) scale > 0 is z > 0, scale: gamma rstd.  A gamma of zero leaves beta alone to decide, by the sign of an infinite t; the
-// scale is then the smallest number, so that the product has that sign.
+// Before a relu: z > 0 where x - t has the sign of scale = gamma rstd; a difference of zero counts as positive, so t is the smallest number that passes
+// for a positive scale, and the last one that does not below a negative one, -0 where it is zero (x - t is then +0 for both zeros).  Signs, not
+// their product: that may underflow.  A gamma of zero leaves beta alone to decide, by the sign of an infinite t; what is not a number does not pass.
 struct ReluBorder {
     float t, scale;
     __device__ __forceinline__ void set(double mean, double rstd, float gamma, float beta) {
         const double a = rstd * gamma;
-        scale = a == 0.0 ? 0x1p-149f : (float)a;
+        scale = (float)a;
+        if (scale == 0.0f) scale = a < 0.0 ? -0x1p-149f : 0x1p-149f;  // (of the sign that fp32 would lose)
         double inv = __builtin_amdgcn_rcp(a);  // and two steps of Newton's: a rounded division and rounding by library calls took 1 us a wavefront
         inv = fma(fma(-a, inv, 1.0), inv, inv), inv = fma(fma(-a, inv, 1.0), inv, inv);
         const double at = fma(-(double)beta, inv, mean);
         t = (float)at;
-        if (((double)t - at) * a > 0.0) {  // rounded to the wrong side: the neighbour
+        if (a > 0.0 ? (double)t <= at : (double)t < at) {  // the next one up
             const int bits = __float_as_int(t);
-            t = t == 0.0f ? (a > 0.0 ? -0x1p-149f : 0x1p-149f) : __int_as_float((t > 0.0f) == (a > 0.0) ? bits - 1 : bits + 1);
+            if (t < INFINITY) t = t == 0.0f ? 0x1p-149f : __int_as_float(t > 0.0f ? bits + 1 : bits - 1);
         }
         if (a == 0.0) t = beta > 0.0f ? -INFINITY : INFINITY;
+        if (!(t == t && a == a)) t = a < 0.0 ? -INFINITY : INFINITY, scale = fabsf(scale) >= 0.0f ? scale : __builtin_nanf("");
+        if (t == 0.0f) t = -0.0f;
     }
-    __device__ __forceinline__ float through(float dy, float x) const { return (x - t) * scale > 0.0f ? dy : 0.0f; }
+    __device__ __forceinline__ float through(float dy, float x) const { return (__float_as_int(x - t) ^ __float_as_int(scale)) >= 0 ? dy : 0.0f; }
 };
 
 // dy act'(z), of silu and of no activation
