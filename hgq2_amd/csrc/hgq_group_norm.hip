@@ -7,7 +7,8 @@
 //
 // The border of a relu.  Which side of zero z falls on decides whether a whole dy passes, and z within fp32's rounding of zero (one element in
 // some ten million) decides it by chance, for every evaluation in fp32 its own.  So before a relu mean and 1 / sqrt(var + eps) are formed in 64 bits
-// and handed to the backward pass as such; there z > 0 is x > t (x < t where gamma is negative) with t = mean - beta / (gamma rstd),
+// and handed to the backward pass as such, and what the mean's rounding to fp32 left out goes into the forward pass's beta (far from zero it would move
+// the border: at a mean of 3000 standard deviations by 1e-4 of one); backward z > 0 is x > t (x < t where gamma is negative) with t = mean - beta / (gamma rstd),
 // rounded to fp32 towards the side that changes no comparison with an fp32 x: the exact decision takes fewer instructions than z.
 #include <type_traits>
 
@@ -117,8 +118,10 @@ __global__ __launch_bounds__(256) void group_norm_fwd_any(const T *__restrict__ 
         for (int64_t e = threadIdx.x; e < n; e += 256) {
             const int c = g * s.D + (int)(e % s.D);
             const int64_t at = base + e / s.D * s.C + e % s.D;
-            const float z = fmaf(to_f32(x[at]) - mean, rstd * (gamma ? gamma[c] : 1.0f), beta ? beta[c] : 0.0f);
-            y[at] = (T)activate<ACT>(z);
+            const float scale = rstd * (gamma ? gamma[c] : 1.0f);
+            float be = beta ? beta[c] : 0.0f;
+            if (ACT == HGQ_ACT_RELU) be = fmaf(-(float)(mean64 - mean), scale, be);
+            y[at] = (T)activate<ACT>(fmaf(to_f32(x[at]) - mean, scale, be));
         }
     }
 }
@@ -327,6 +330,8 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
     constexpr int N = ONE ? 1 : 4;  // means of a thread's columns
     float mean[N], rstd[N];
     const V one = 1, eps = p.eps;
+    // elements of a group in this tile
+    const V inv = one / (V)(p.splits == 1 ? p.n / p.G : (min(p.n / p.C, r1 * p.fold) - r0 * p.fold) * p.D);
     if (phase < 2) {
         V acc[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -338,8 +343,6 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
         for (int j = 0; j < 3; ++j)
             if (j < rows.rest) acc[j] += last[j];
         sum_groups<ONE>(p, t, acc, red, total);
-        // elements of a group in this tile
-        const V inv = one / (V)(p.splits == 1 ? p.n / p.G : (min(p.n / p.C, r1 * p.fold) - r0 * p.fold) * p.D);
 #pragma unroll
         for (int j = 0; j < N; ++j) mean[j] = t.on ? (float)(total[group_of<ONE>(p, t, j)] * inv) : 0.0f;
         auto square = [&](float x, int j) {  // (about the mean's fp32 value: within 2^-24 of it, whose square is nothing)
@@ -404,6 +407,10 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
     for (int j = 0; j < 4; ++j) {
         const int c = p.fold > 1 ? (c0 + j) % p.C : c0 + j;
         scale[j] = rstd[j % N] * (gamma ? gamma[c] : 1.0f), be[j] = beta ? beta[c] : 0.0f;
+        if (ACT == HGQ_ACT_RELU) {  // (the 64-bit mean again from LDS: kept, it took up to eight registers)
+            const V m = total[group_of<ONE>(p, t, j)];
+            be[j] = fmaf(-(float)((phase < 2 ? m * inv : m) - mean[j % N]), scale[j], be[j]);
+        }
     }
     T *ys = y + b * p.n;
 #pragma unroll
