@@ -102,6 +102,15 @@ class SGD:
             else:
                 loss.backward(self._unit)
 
+    def refuse_other_graphs(self, stream):
+        """Raises where a variable's gradients are accumulated by a living graph of another stream: a backward pass recorded on ``stream``
+        would pull that stream into the recording, which ends the process."""
+        with torch.cuda.stream(stream):
+            for p in self.params:
+                if _lib.native().accumulates_elsewhere(p):
+                    raise RuntimeError(f"{getattr(p, 'var_name', None) or 'a variable'} belongs to a graph of another stream that is still alive: the step "
+                                       'cannot be recorded (release what that graph gave, the loss of an eager step for instance)')
+
     @torch.no_grad()
     def step(self):
         sums = ops.join_side(hand_over_sums=True)  # the loss terms' sum rides along with the update launch
@@ -291,15 +300,6 @@ class AdamW(SGD):
                 for p, c in post:
                     p.copy_(c(p))
 
-    def refuse_other_graphs(self, stream):
-        """Raises where a variable's gradients are accumulated by a living graph of another stream: a backward pass recorded on ``stream``
-        would pull that stream into the recording, which ends the process."""
-        with torch.cuda.stream(stream):
-            for p in self.params:
-                if _lib.native().accumulates_elsewhere(p):
-                    raise RuntimeError(f"{getattr(p, 'var_name', None) or 'a variable'} belongs to a graph of another stream that is still alive: the step "
-                                       'cannot be recorded (release what that graph gave, the loss of an eager step for instance)')
-
     def _specials(self, indices):
         """Hands over the gradient pieces, bounds and folded regularizers of these variables; the constraints to apply after the update."""
         post, inf = [], float('inf')
@@ -347,6 +347,7 @@ class GraphedTrainStep:
         self.loss = None
         self.warmup_losses = []
         side = torch.cuda.Stream()
+        self._refuse_other_graphs(side)  # before the warm-up trains the variables and draws from the feed
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             if feed is not None:
@@ -364,13 +365,29 @@ class GraphedTrainStep:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         self.opt.zero_grad(set_to_none=True)
-        if isinstance(self.opt, AdamW):
-            self.opt.refuse_other_graphs(side)
+        self._refuse_other_graphs(side)  # (and what the warm-up left alive)
         self.graph = torch.cuda.CUDAGraph()
         # captured on the stream the warm-up ran on: scratch that operators keep per stream (allocated and cleared once,
         # during the warm-up) is found again instead of being created, and cleared, inside the graph
         with torch.cuda.graph(self.graph, stream=side):
             self.loss = self._step()
+
+    def _refuse_other_graphs(self, side):
+        import gc
+
+        refuse = getattr(self.opt, 'refuse_other_graphs', None)
+        if refuse is None:  # (an optimizer of the caller's own)
+            return
+        try:
+            refuse(side)
+        except RuntimeError:
+            # what no caller holds does not count: the terms of the model's last call, which its next call replaces, and unreachable cycles
+            if isinstance(self.model, torch.nn.Module):
+                for m in self.model.modules():
+                    if isinstance(m, Layer):
+                        m._losses = []
+            gc.collect()
+            refuse(side)
 
     def _step(self):
         import contextlib
