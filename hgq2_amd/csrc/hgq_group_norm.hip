@@ -751,8 +751,25 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     return true;
 }
 
-// the tiles' terms of dgamma and dbeta, and runs of them added up where they are many
-int64_t slices_floats(const GroupTile &p) { return 2 * (int64_t)p.C * (p.tiles + (p.tiles > MOST_SLICES ? (p.tiles + SLICE_RUN - 1) / SLICE_RUN : 0)); }
+// n slices of terms of dgamma and dbeta, and runs of them added up - runs of runs - until the last reduction takes them: it adds n / 128 in a row
+int64_t slices_floats(int64_t n, int C) {
+    int64_t all = n;
+    for (; n > MOST_SLICES; all += n) n = (n + SLICE_RUN - 1) / SLICE_RUN;
+    return 2 * (int64_t)C * all;
+}
+
+int sum_slices(float *slices, int64_t n, int C, float *dgamma, float *dbeta, hipStream_t st) {
+    const int64_t M = 2 * (int64_t)C;
+    while (n > MOST_SLICES) {
+        const int64_t runs = (n + SLICE_RUN - 1) / SLICE_RUN;
+        float *joined = slices + n * M;
+        hipLaunchKernelGGL(group_norm_join_slices, dim3((unsigned)((M + 63) / 64), (unsigned)(runs < 65535 ? runs : 65535)), dim3(64), 0, st, slices, n, M, joined);
+        const int rc = check_launch("hgq_group_norm_bwd");
+        if (rc) return rc;
+        slices = joined, n = runs;
+    }
+    return reduce_parts(slices, (int)n, M, dgamma, C, dbeta, C, nullptr, 0, st);
+}
 
 int64_t parts_floats(const GroupTile &p, bool backward) { return p.splits > 1 ? p.B * p.splits * p.G * (backward ? 2 : 4) : 0; }
 
@@ -811,10 +828,9 @@ int bwd(const void *dy, const void *x, const float *gamma, const float *beta, co
                            sums ? ws : nullptr, s);
         const int rc = check_launch("hgq_group_norm_bwd");
         if (rc || !sums) return rc;
-        return reduce_parts(ws, (int)s.B, 2 * (int64_t)s.C, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
+        return sum_slices(ws, s.B, s.C, dgamma, dbeta, st);
     }
-    const int64_t M = 2 * (int64_t)s.C;
-    float *slices = sums ? ws : nullptr, *parts = p.splits > 1 ? ws + slices_floats(p) : nullptr;
+    float *slices = sums ? ws : nullptr, *parts = p.splits > 1 ? ws + slices_floats(p.tiles, s.C) : nullptr;
     if (p.splits > 1 && !ws) return fail(HGQ_ERR_ARG, "hgq_group_norm_bwd: null workspace");
     auto kernel = p.D % 4 == 0 ? bwd_kernel<T, ACT, true>(held) : bwd_kernel<T, ACT, false>(held);
     for (int phase = p.splits > 1 ? 1 : 0; phase < (p.splits > 1 ? 3 : 1); ++phase) {
@@ -824,13 +840,7 @@ int bwd(const void *dy, const void *x, const float *gamma, const float *beta, co
         const int rc = check_launch("hgq_group_norm_bwd");
         if (rc) return rc;
     }
-    if (!sums) return HGQ_OK;
-    if (p.tiles <= MOST_SLICES) return reduce_parts(slices, p.tiles, M, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
-    const int runs = (p.tiles + SLICE_RUN - 1) / SLICE_RUN;
-    float *joined = slices + p.tiles * M;
-    hipLaunchKernelGGL(group_norm_join_slices, dim3((unsigned)((M + 63) / 64), (unsigned)(runs < 65535 ? runs : 65535)), dim3(64), 0, st, slices, (int64_t)p.tiles, M, joined);
-    const int rc = check_launch("hgq_group_norm_bwd");
-    return rc ? rc : reduce_parts(joined, runs, M, dgamma, s.C, dbeta, s.C, nullptr, 0, st);
+    return sums ? sum_slices(slices, p.tiles, s.C, dgamma, dbeta, st) : HGQ_OK;
 }
 
 template <typename T>
@@ -856,7 +866,7 @@ extern "C" int64_t hgq_group_norm_bwd_workspace(int64_t B, int64_t S, int C, int
     if (check_shape("hgq_group_norm_bwd_workspace", B, S, C, G, HGQ_ACT_NONE, type)) return -1;
     GroupTile p;
     int held, threads;
-    return plan(p, held, threads, B, S, C, G, type, true) ? slices_floats(p) + parts_floats(p, true) : B * 2 * C;
+    return plan(p, held, threads, B, S, C, G, type, true) ? slices_floats(p.tiles, C) + parts_floats(p, true) : slices_floats(B, C);
 }
 
 extern "C" int hgq_group_norm_fwd(const void *x, const float *gamma, const float *beta, void *y, double *mean, double *rstd, float *workspace,
