@@ -566,10 +566,10 @@ __global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(cons
         const int lane = threadIdx.x & (p.team - 1);
         for (int g = threadIdx.x / p.team; g < groups; g += blockDim.x / p.team) {
             const float *in = parts + (b - t.s) * p.splits * p.G * 2 + (chunk * p.K + g) * 2;
-            float m1 = 0, m2 = 0;
+            double m1 = 0, m2 = 0;  // (thousands of splits in a row: in fp32 they drift by hundreds of its roundings)
             for (int k = lane; k < p.splits; k += p.team) m1 += in[(int64_t)k * p.G * 2], m2 += in[(int64_t)k * p.G * 2 + 1];
             for (int d = p.team / 2; d; d >>= 1) m1 += __shfl_xor(m1, d), m2 += __shfl_xor(m2, d);
-            if (lane == 0) total[g] = m1, stat[g] = m2;
+            if (lane == 0) total[g] = (float)m1, stat[g] = (float)m2;
         }
         __syncthreads();
     }

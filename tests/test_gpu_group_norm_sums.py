@@ -34,3 +34,18 @@ def test_many_samples_without_a_tile(dev, B, C, dtype):
             sums[k], tols[k] = sums[k] + want[2 + k], tols[k] + tol[2 + k]
     _check(dbeta, sums[1], tols[1], torch.float32, 'dbeta')
     _check(dgamma, sums[0], tols[0], torch.float32, 'dgamma')
+
+
+@pytest.mark.parametrize('C,G,dtype', [(32, 32, torch.float32), (32, 8, torch.float32), (32, 32, torch.bfloat16)])
+def test_one_long_sample(dev, C, G, dtype):
+    """A sample cut into thousands of runs, with dy = 1 and one gamma per group: d is its own mean, dx zero but for the rounding of the two means."""
+    from hgq2_amd import ops
+
+    S = (1 << 21) + 77
+    g = torch.Generator(device=dev).manual_seed(29)
+    x = torch.randn(1, S, C, generator=g, device=dev).to(dtype).requires_grad_(True)
+    gamma = (torch.rand(G, generator=g, device=dev) + 0.5).repeat_interleave(C // G)
+    y = ops.group_norm(x, G, gamma)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    want, tol = _definition(x.detach(), torch.ones_like(y), gamma, None, G, 1e-3, 'linear')
+    _check(dx, want[1], tol[1], dtype, 'dx')
