@@ -141,22 +141,26 @@ __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ 
         const int g = (int)(bg - b * s.G);
         const int64_t base = b * s.S * s.C + (int64_t)g * s.D, n = s.S * s.D;
         const float mean = (float)mean_in[bg], rstd = (float)rstd_in[bg];
-        auto through = [&](float dv, float xv, float xh, float ga, float be) {  // dz
+        auto border = [&](float ga, float be) {
+            ReluBorder r = {0, 0};
+            if (ACT == HGQ_ACT_RELU) r.set(mean_in[bg], rstd_in[bg], ga, be);
+            return r;
+        };
+        auto through = [&](float dv, float xv, float xh, float ga, float be, const ReluBorder &edge) {  // dz
             if (ACT != HGQ_ACT_RELU) return through_activation<ACT>(dv, xh * ga + be);
-            ReluBorder border;
-            border.set(mean_in[bg], rstd_in[bg], ga, be);
-            return xh == xh ? border.through(dv, xv) : xh;
+            return xh == xh ? edge.through(dv, xv) : xh;
         };
         double s1 = 0, s2 = 0;  // of d and d xhat, over the group
         for (int c0 = 0; c0 < s.D; c0 += tx) {
             const int d = c0 + cx, c = g * s.D + d;
             double a = 0, h = 0;
             const float ga = d < s.D && gamma ? gamma[c] : 1.0f, be = d < s.D && beta ? beta[c] : 0.0f;
+            const ReluBorder edge = border(ga, be);
             if (d < s.D)
                 for (int64_t p = py; p < s.S; p += ty) {
                     const int64_t at = base + p * s.C + d;
                     const float xv = to_f32(x[at]), xh = (xv - mean) * rstd;
-                    const float dz = through(to_f32(dy[at]), xv, xh, ga, be);
+                    const float dz = through(to_f32(dy[at]), xv, xh, ga, be, edge);
                     a += dz, h += (double)dz * xh;
                 }
             s1 += a * ga, s2 += h * ga;
@@ -174,7 +178,7 @@ __global__ __launch_bounds__(256) void group_norm_bwd_any(const T *__restrict__ 
             const int c = g * s.D + (int)(e % s.D);
             const int64_t at = base + e / s.D * s.C + e % s.D;
             const float ga = gamma ? gamma[c] : 1.0f, be = beta ? beta[c] : 0.0f, xv = to_f32(x[at]), xh = (xv - mean) * rstd;
-            const float dz = through(to_f32(dy[at]), xv, xh, ga, be);
+            const float dz = through(to_f32(dy[at]), xv, xh, ga, be, border(ga, be));
             dx[at] = (T)((dz * ga - m1 - xh * m2) * rstd);
         }
     }
