@@ -269,7 +269,7 @@ def _load_native():
 
     lib, path = load(), os.path.join(_HERE, '_host.so')
     if not os.path.exists(path):
-        raise HGQLibraryError(f'{path} not found: the host extension is not built. Run `make -C hgq2_amd/csrc` (or __graft_entry__.build()).')
+        raise HGQLibraryError(f'{path} not found: the host extension is not built. Run `make -C hgq2_amd/csrc` (or __graft_entry__.build()) where g++ and PyTorch-ROCm are installed.')
     spec = importlib.util.spec_from_file_location('hgq2_amd._host', path)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
