@@ -247,33 +247,52 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-_native, _native_lock = None, threading.Lock()
+_host, _native, _native_lock = None, None, threading.RLock()
 _NATIVE_CALLS = ('hgq_last_error', 'hgq_global_norm_parts', 'hgq_global_norm', 'hgq_adamw_update_multi', 'hgq_group_norm_fwd_workspace',
                  'hgq_group_norm_fwd', 'hgq_group_norm_bwd_workspace', 'hgq_group_norm_bwd')
 
 
 def native():
-    """The host code that is compiled against torch (``csrc/hgq_torch.cpp``), bound to the HIP library's entry points; it registers the
-    operators ``hgq::group_norm_fwd``, ``hgq::group_norm_bwd`` and ``hgq::global_norm``."""
+    """The host code that is compiled against torch (``csrc/hgq_torch.cpp``), bound to the HIP library's entry points."""
+    global _native
     if _native is not None:
         return _native
     with _native_lock:
-        return _native if _native is not None else _load_native()
+        if _native is None:
+            lib, mod = load(), host_extension()
+            mod.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in _NATIVE_CALLS}, HGQLibraryError)
+            _native = mod
+    return _native
 
 
-def _load_native():
-    global _native
+def register_operators():
+    """Makes the operators ``hgq::group_norm_fwd``, ``hgq::group_norm_bwd`` and ``hgq::global_norm`` known, like those of ``ops.py``; the HIP library
+    is loaded when one is first called.  Where the extension is missing, or does not load, the first use says so."""
+    try:
+        host_extension()
+    except (HGQLibraryError, ImportError):
+        pass
+
+
+def host_extension():
+    global _host
+    path = os.path.join(_HERE, '_host.so')
+    if not os.path.exists(path):
+        raise HGQLibraryError(f'{path} not found: the host extension is not built. Run `make -C hgq2_amd/csrc` (or __graft_entry__.build()) where g++ and PyTorch-ROCm are installed.')
+    with _native_lock:
+        if _host is None:
+            _host = _load_host(path)
+    return _host
+
+
+def _load_host(path):
     import importlib.util
 
     import torch
 
-    lib, path = load(), os.path.join(_HERE, '_host.so')
-    if not os.path.exists(path):
-        raise HGQLibraryError(f'{path} not found: the host extension is not built. Run `make -C hgq2_amd/csrc` (or __graft_entry__.build()) where g++ and PyTorch-ROCm are installed.')
     spec = importlib.util.spec_from_file_location('hgq2_amd._host', path)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
-    mod.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in _NATIVE_CALLS}, HGQLibraryError)
 
     @torch.library.register_fake('hgq::group_norm_fwd')
     def _(x, gamma, beta, groups, epsilon, act):
@@ -289,7 +308,6 @@ def _load_native():
     def _(tensors):
         return tensors[0].new_empty((), dtype=torch.float32)
 
-    _native = mod
     return mod
 
 

@@ -13,6 +13,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <atomic>
+
 #include "../../include/hgq_hip.h"
 
 namespace py = pybind11;
@@ -32,8 +34,24 @@ struct Library {  // the entry points that are called from here
 } lib;
 PyObject *library_error = nullptr;  // hgq2_amd._lib.HGQLibraryError
 
+std::atomic<bool> bound{false};
+
+[[noreturn]] void rethrow(py::error_already_set &error) {  // as the Python exception that it is
+    error.restore();
+    python_error e;
+    e.persist();
+    throw e;
+}
+
 const Library &library() {
-    TORCH_CHECK(lib.last_error, "the HIP library is not bound (hgq2_amd._lib.native())");
+    if (!bound) {  // an operator called by its name alone, before anything else asked for the library
+        const py::gil_scoped_acquire gil;
+        try {
+            py::module_::import("hgq2_amd._lib").attr("native")();
+        } catch (py::error_already_set &e) {
+            rethrow(e);
+        }
+    }
     return lib;
 }
 
@@ -382,6 +400,7 @@ void bind(const py::dict &entries, const py::object &error) {
     lib.group_norm_fwd = (decltype(lib.group_norm_fwd))at("hgq_group_norm_fwd");
     lib.group_norm_bwd_workspace = (decltype(lib.group_norm_bwd_workspace))at("hgq_group_norm_bwd_workspace");
     lib.group_norm_bwd = (decltype(lib.group_norm_bwd))at("hgq_group_norm_bwd");
+    bound = true;
 }
 
 Tensor tensor_of(const py::handle &h, const char *what) {

@@ -3553,6 +3553,9 @@ def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: flo
     touch_state()
 
 
+_lib.register_operators()  # `hgq::global_norm` and those of group normalisation, which are compiled
+
+
 # ---- group normalisation
 GROUP_ACTIVATIONS = {None: _lib.ACT_NONE, 'linear': _lib.ACT_NONE, 'relu': _lib.ACT_RELU, 'silu': _lib.ACT_SILU, 'swish': _lib.ACT_SILU}
 
