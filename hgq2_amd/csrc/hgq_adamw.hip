@@ -24,7 +24,7 @@ namespace hgq {
 constexpr int ADAMW_ITEMS = 28, ADAMW_PIECES = 32;
 // A step that touches more than the card's 256 MB cache passes through it once: accesses that leave no trace there, four blocks per
 // wavefront in flight, a workgroup per 4096 elements.  150 million elements, 4.2 GB: 851 -> 720 us (5.9 TB/s; the card copies at 5.0), with
-// moments in 8 bits, 2.4 GB: 552 -> 437 us (now 409, its 79 vector instructions per element close behind); 37 million bfloat16: 164 ->
+// moments in 8 bits, 2.4 GB: 552 -> 437 us (now 401 - 415, its 88 vector instructions per element close behind); 37 million bfloat16: 164 ->
 // 137 us.  A smaller step leaves its weights for the next forward pass; two blocks, and up to 2048 workgroups that go over 2048
 // elements at a time (4 million elements: 22 us either way).
 constexpr int64_t ADAMW_CACHE = (int64_t)256 << 20;
@@ -142,7 +142,7 @@ __device__ __forceinline__ void adamw_moments(float g, float &m, float &v, float
     m = __fadd_rn(m, __fmul_rn(__fsub_rn(g, m), k.one_minus_b1));
     v = __fadd_rn(v, __fmul_rn(__fsub_rn(__fmul_rn(g, g), v), k.one_minus_b2));
     // The rounded root: __fsqrt_rn is the hardware's here, a unit in the last place off, which moves a code where r lies on a border of its
-    // rounding (150 million elements: 17 codes of r).  Some ten vector instructions more: with 8-bit moments 401 -> 415 us there, 821 -> 823 with 32-bit ones.
+    // rounding (150 million elements: 17 codes of r).  Nine vector instructions more: with 8-bit moments 401 -> 415 us there, 821 -> 823 with 32-bit ones.
     r = sqrtf(v);
 }
 

@@ -434,7 +434,8 @@ __global__ __launch_bounds__(1024) void group_norm_fwd_tile(const T *__restrict_
 
 // phase 0: whole tiles; 1: sums of d rstd and d xhat rstd of every split, parts [B][splits][G][2], and the channels' sums; 2: join them, dx.
 // Every tile leaves its terms of dgamma and dbeta, slices [tiles][2 C] (NULL: not wanted).  MORE: rows of a thread beyond those in its registers, which it
-// keeps in LDS.
+// keeps in LDS.  The 16-bit forms with 16 rows before a relu, for groups that are not whole accesses, spill 8 of 128 registers (2048 x 26 x 26 x 30
+// bfloat16 in 5 groups, backward 75 us; x 32 in 4 groups, without a spill, 65 us).
 template <typename T, int ACT, bool ONE, int NV, int MORE>
 __global__ __launch_bounds__(MORE ? 512 : 1024, 4) void group_norm_bwd_tile(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ gamma,
                                                             const float *__restrict__ beta, const double *__restrict__ mean_in,
@@ -697,11 +698,12 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     p = {};
     p.B = B, p.n = (int)(S * C), p.C = C, p.G = G, p.D = C / G, p.inv = 1.0f / (float)(S * (C / G)), p.NS = 1;
     const int most = most_held(type), size = type == HGQ_TYPE_F32 ? 4 : 2;
-    // How many groups a tile holds.  A workgroup costs about 2 us whatever it holds, so with work for every compute unit the most groups that
-    // stay under 96 KB (1024 x 26 x 26 x 32 fp32 in 8 groups, backward: 86 KB 68 us, 43 KB 74 us, 11 KB 97 us; 256 x 8 x 8 x 512: 64 KB 22 us, 4 KB 29 us).
-    // With little work the fewest groups: one sample of 28 x 28 x 32 in 8 workgroups 5.8 us, in one 7.5 us.  A tile of more than 96 KB
-    // leaves a compute unit with one workgroup that loads, waits and stores in turn, and narrow ones read parts of cache lines: the
-    // sample is cut into runs of rows and read twice (48 x 64 x 64 x 512 bfloat16: held, 32-byte rows 148 us, cut with 128-byte rows 127 us).
+    // How many groups a tile holds.  A workgroup costs about 2 us whatever it holds, and narrow ones read parts of cache lines, so with work for
+    // every compute unit the most groups that stay under 96 KB (dx with silu: 1024 x 26 x 26 x 32 fp32 in 8 groups, 86 KB 50 us, 43 KB 52 us, 11 KB
+    // 97 us; 64 x 32 x 32 x 256 in 32 groups, 64 KB 38 us, 32 KB 41 us, 8 KB 60 us).  With little work the fewest groups: one sample of 28 x 28 x 32 in 8
+    // workgroups 5.8 us, in one 7.5 us.  A tile of more than 96 KB leaves a compute unit with one workgroup that loads, waits and stores in
+    // turn: the sample is cut into runs of rows and read twice (48 x 64 x 64 x 512 bfloat16 with silu, held in 32-byte rows: forward 148 us, dx
+    // 224 us; cut, with 128-byte rows: 116 and 188 us).
     int best = 0;
     for (int K = 1; K <= G; K = K < G && (K + 1) * p.D > 4 * GROUP_THREADS ? G : K + 1) {
         if (G % K || !widen(p, K)) continue;
@@ -710,13 +712,13 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     }
     if (best) {
         widen(p, best);
-        // rows per thread: many amortise what a workgroup costs (the first shape in 43 KB tiles, backward: 8 rows 74 us, 4 rows 97 us), few
+        // rows per thread: many amortise what a workgroup costs (the first shape in 43 KB tiles, dx with silu: 8 rows 52 us, 4 rows 72 us), few
         // spread little work over more threads
         held = B * p.chunks >= 512 ? most : 4;
         while ((p.rows + held - 1) / held * p.TX > GROUP_THREADS) held *= 2;
         // The backward pass takes 120 registers: 16 wavefronts per compute unit.  A workgroup of 9 to 11 leaves it no second one to load
         // while the first computes, one of 5 leaves four places empty: where rows kept in LDS bring it down to 8 or 4, two or four
-        // fit (1024 x 26 x 26 x 32 in 8 groups: fp32, 11 -> 8, 70 -> 54 us; bfloat16, 2048 samples in 4 groups, 6 -> 4, 98 -> 63 us).  Elsewhere they only
+        // fit (1024 x 26 x 26 x 32 in 8 groups, dx with silu: fp32, 11 -> 8, 61 -> 50 us; bfloat16, 2048 samples in 4 groups, 6 -> 4, 86 -> 64 us).  Elsewhere they only
         // cost (1024 x 20 x 20 x 32, 7 -> 5: 38 -> 48 us).
         const int more = most + in_lds(most);
         for (int fits = 512; backward && held == most && p.K <= 512 && fits >= 256; fits /= 2)  // (K: 64 KB hold the rows and the groups' sums)
@@ -726,7 +728,8 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
         const int one = p.TY * p.TX;  // small samples share a workgroup while there are enough of them
         while ((p.NS + 1) * one <= 256 && B / (p.NS + 1) * p.chunks >= 512) ++p.NS;
     } else {
-        // rows of 128 bytes or more, whole lines (16 x 128 x 128 x 64 fp32 in 8 groups, backward: 128 bytes 59 us, 32 bytes and less over 63 us)
+        // rows of 128 bytes or more, whole lines (dx with silu: 48 x 64 x 64 x 512 bfloat16 in 32 groups, 128 bytes 188 us, 64 bytes 213 us, 32 bytes
+        // 271 us; 16 x 128 x 128 x 64 fp32 in 8 groups 58, 57 and 61 us)
         for (int K = 1; K <= G; K = K < G && (K + 1) * p.D > 4 * GROUP_THREADS ? G : K + 1) {
             if (G % K == 0 && widen(p, K)) {
                 best = K;
@@ -747,8 +750,8 @@ bool plan(GroupTile &p, int &held, int &threads, int64_t B, int64_t S, int C, in
     const int64_t tiles = (B + p.NS - 1) / p.NS * p.splits;
     if ((tiles + 7) * p.chunks * threads > 0xffffffff) return false;  // (a launch has less than 2^32 threads)
     p.tiles = (int)tiles;
-    // What a pass reads and writes against the card's 256 MB cache, and rows of whole lines: 48 x 64 x 64 x 512 bfloat16, forward 131 -> 110 us,
-    // backward 206 -> 196 us, and 7 and 6 us less with the second read of its cut samples past the cache as well.  Half lines are slower
+    // What a pass reads and writes against the card's 256 MB cache, and rows of whole lines: 48 x 64 x 64 x 512 bfloat16 with silu, forward 119 -> 116
+    // us, dx 192 -> 188 us, before a relu 120 -> 118 and 241 -> 237 us (without an activation 114 -> 122 and 184 -> 183 us).  Half lines are slower
     // that way (64 x 32 x 32 x 256 fp32 in rows of 64 bytes, backward 50 -> 54 us), and a smaller output is still there for the layer
     // that reads it next.
     p.through = B * S * C * size * (backward ? 3 : 2) > (int64_t)256 << 20 && p.TX * 4 * size % 128 == 0;
