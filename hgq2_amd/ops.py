@@ -3520,11 +3520,12 @@ def adamw_update_multi_op(ws: Sequence[Tensor], gs: Sequence[Tensor], moments: S
         for name, mt, kind, size in zip(('m', 'v') if per == 2 else ('m', 'm scale', 'v', 'v scale'), mom, kinds, sizes):
             _check_gradient(name, mt, device, kind, size)
         _need(all(k.is_contiguous() for k in (w, g, *mom)), 'variables, gradients and moments must be contiguous')
+        _need(not any(k.is_neg() for k in (w, g, *mom)), 'variables, gradients and moments must not be lazily negated views')
         p = [k.data_ptr() for k in mom]
         words += (w.data_ptr(), g.data_ptr(), *((p[0], p[1], 0, 0) if per == 2 else (p[0], p[2], p[1], p[3])), num, first,
                   *_adamw_limits_words(l1[t], lo[t], hi[t], decay[t]), code, *_NO_SIDES)
         first += -(-num // ADAMW_BLOCK) * ADAMW_BLOCK
-    _need_apart('variables', ws), _need_apart('moments', moments)
+    _need_apart('variables', ws), _need_apart('moments', moments), _need_apart('variables and moments', [*ws, *moments])
     if norm_out.numel():
         _check_f32('norm_out', norm_out)
         _need(norm_out.numel() == 1 and norm_out.device == device, 'norm_out is one float32')
@@ -3535,7 +3536,8 @@ def adamw_update_multi_op(ws: Sequence[Tensor], gs: Sequence[Tensor], moments: S
 def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: float = 0.999, epsilon: float = 1e-7, decay=None, l1=None,
                         lo=None, hi=None, clipnorm: float | None = None, norm_out: Tensor | None = None, seed: int = 0):
     """One AdamW step of the variables ``ws`` (float32, bfloat16 or float16, contiguous) with the gradients ``gs`` of the same types, in
-    place.  ``moments[t]``: what :func:`adamw_moments` makes for variable ``t`` (its length says whether they have 32 or 8 bits);
+    place.  ``moments[t]``: what :func:`adamw_moments` makes for variable ``t`` (its length says whether they have 32 or 8 bits); variables and
+    moments lie apart from each other, and none is a lazily negated view;
     ``state``: :func:`adamw_state`, which the launch moves on (recorded in a HIP graph, every replay is the next step).  Per variable:
     weight ``decay``, an ``l1`` added to the gradient, and bounds ``lo``, ``hi`` of the result.  ``clipnorm``: gradients are scaled down
     to this global norm; a norm that is not finite makes every variable not a number.  :class:`hgq2_amd.train.AdamW` is this with
@@ -3544,6 +3546,7 @@ def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: flo
     _need(n >= 1 and len(gs) == n and len(moments) == n, 'per-variable lists differ in length')
     _need(all(g is not None for g in gs), 'every variable needs a gradient')
     _need(clipnorm is None or clipnorm > 0, 'clipnorm must be positive')
+    _need(not any(k.is_neg() for k in (*ws, *(k for m in moments for k in m))), 'variables and moments must not be lazily negated views')
     bits = 32 if len(moments[0]) == 2 else 8
     each = lambda v, d: [d] * n if v is None else [float(k) for k in v]  # noqa: E731
     empty = torch.empty(0, dtype=torch.float32, device=state.device)
