@@ -384,8 +384,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwLaunch a, AdamwSum sum,
     k.c = 1.0f;
     if (n_parts > 0) {
         const float norm = joined ? joined[0] : (float)sqrt(block_sum(squares, lds));
-        // no clipping up to the bound; a norm that is not finite makes every step not a number
-        k.c = norm <= clipnorm ? 1.0f : norm < __builtin_inff() ? __fdiv_rn(clipnorm, norm) : __builtin_nanf("");
+        // No clipping up to the bound; a norm that is not finite makes every step not a number.  The product with the rounded reciprocal is
+        // Keras' order of operations, a rounding more than the quotient, which stands in where the reciprocal is no normal number.
+        const float inverse = __fdiv_rn(1.0f, norm);
+        const bool normal = inverse >= 0x1p-126f && inverse < __builtin_inff();
+        k.c = norm <= clipnorm ? 1.0f : !(norm < __builtin_inff()) ? __builtin_nanf("") : normal ? fminf(__fmul_rn(clipnorm, inverse), 1.0f) : __fdiv_rn(clipnorm, norm);
         if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
     }
     for (uint32_t c = blockIdx.x; c < a.start[ADAMW_ITEMS]; c += gridDim.x) {

@@ -38,3 +38,34 @@ def test_the_root_is_rounded(dev):
     bad = (got != want * 16 * scale) & inside
     assert not bad.any(), f'{int(bad.sum())} of {n} codes'
     assert torch.equal(got[::BLOCK], (15 * 16 * scale)[::BLOCK])
+
+
+def test_the_clipping_factor_is_keras(dev):
+    """clipnorm times the rounded reciprocal of the rounded norm.  With beta_1 = 0 the first moment is the clipped gradient, and of a gradient of
+    one that is the factor itself."""
+    from hgq2_amd import ops
+
+    gen = torch.Generator().manual_seed(32)
+    other = 30 * torch.rand(200, generator=gen)
+    clips = (0.9 * torch.rand(200, generator=gen) + 0.05).tolist()
+    clips[:4] = [0.1, 0.3, 0.7, 1.0]
+    got, want = [], []
+    for a, clip in zip(other.tolist(), clips):
+        g = torch.tensor([1.0, a])
+        m, norm = ops.adamw_moments(2, dev), torch.zeros((), device=dev)
+        ops.adamw_update_multi_([torch.zeros(2, device=dev)], [g.to(dev)], [m], ops.adamw_state(dev, 0.001), beta_1=0.0, clipnorm=clip, norm_out=norm)
+        n = np.float32(np.sqrt(np.sum(g.double().numpy() ** 2)))
+        assert np.float32(norm.item()) == n
+        got.append(m[0][0].item())
+        want.append(float(np.float32(clip) * (np.float32(1) / n)) if n > np.float32(clip) else 1.0)
+    assert got == want
+
+
+@pytest.mark.parametrize('norm,clip', [(2.0**-130, 2.0**-133), (2.0**-130, 2.0**-126), (2.0**127, 2.0**100), (1.5 * 2.0**127, 3 * 2.0**80), (2.0**-126, 2.0**-128)])
+def test_clipping_at_the_ends_of_the_range(dev, norm, clip):
+    """Where the reciprocal overflows or is no normal number the factor is the quotient, here a power of two."""
+    from hgq2_amd import ops
+
+    m = ops.adamw_moments(1, dev)
+    ops.adamw_update_multi_([torch.zeros(1, device=dev)], [torch.tensor([norm], device=dev)], [m], ops.adamw_state(dev, 0.001), beta_1=0.0, clipnorm=clip)
+    assert m[0].item() == min(norm, clip)
