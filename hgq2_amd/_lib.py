@@ -100,6 +100,15 @@ SIGNATURES = {
     'hgq_group_norm_fwd': (c_int, [c_void_p] * 7 + [c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p]),
     'hgq_group_norm_bwd_workspace': (c_int64, [c_int64, c_int64, c_int, c_int, c_int]),
     'hgq_group_norm_bwd': (c_int, [c_void_p] * 10 + [c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    'hgq_distill_topk_workspace': (c_int64, [c_int64] * 3 + [c_int]),
+    'hgq_distill_topk_fwd': (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int] + [c_void_p] * 6 + [c_int64] * 3 + [ctypes.c_double, c_int, c_void_p]),
+    'hgq_distill_topk_bwd': (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int] + [c_void_p] * 5 + [c_int] + [c_int64] * 3 + [ctypes.c_double, c_int, c_void_p]),
+    'hgq_relative_bias_fwd': (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p] + [c_int64] * 4 + [c_void_p, c_int, c_int, c_int64, c_void_p, c_int, c_int, c_void_p]),
+    'hgq_relative_bias_bwd_workspace': (c_int64, [c_int64] * 4 + [c_int] * 2),
+    'hgq_relative_bias_bwd': (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p] + [c_int64] * 4 + [c_void_p, c_int, c_int, c_int64, c_void_p, c_int, c_int, c_void_p]),
+    'hgq_residual_norm_fwd': (c_int, [c_void_p] * 9 + [c_int64] * 3 + [c_float, c_float, c_int, c_int, c_void_p]),
+    'hgq_residual_norm_bwd_workspace': (c_int64, [c_int64] * 3 + [c_int]),
+    'hgq_residual_norm_bwd': (c_int, [c_void_p] * 15 + [c_int64] * 3 + [c_float, c_float, c_int, c_int, c_void_p]),
     'hgq_quantize_bwd_workspace': (c_int64, [c_int64, c_int64, c_int64]),
     'hgq_quantize_bwd_sliced': (c_int, [c_void_p] * 9 + [c_int64, c_int64, c_int64, c_int, c_void_p]),
     'hgq_quantize_bwd_slice_count': (c_int64, [c_int64, c_int64, c_int64]),
@@ -249,7 +258,9 @@ def load() -> ctypes.CDLL:
 
 _host, _native, _native_lock = None, None, threading.RLock()
 _NATIVE_CALLS = ('hgq_last_error', 'hgq_global_norm_parts', 'hgq_global_norm', 'hgq_adamw_update_multi', 'hgq_group_norm_fwd_workspace',
-                 'hgq_group_norm_fwd', 'hgq_group_norm_bwd_workspace', 'hgq_group_norm_bwd')
+                 'hgq_group_norm_fwd', 'hgq_group_norm_bwd_workspace', 'hgq_group_norm_bwd', 'hgq_distill_topk_workspace', 'hgq_distill_topk_fwd',
+                 'hgq_distill_topk_bwd', 'hgq_relative_bias_fwd', 'hgq_relative_bias_bwd_workspace', 'hgq_relative_bias_bwd', 'hgq_residual_norm_fwd',
+                 'hgq_residual_norm_bwd_workspace', 'hgq_residual_norm_bwd')
 
 
 def native():
@@ -266,7 +277,7 @@ def native():
 
 
 def register_operators():
-    """Makes the operators ``hgq::group_norm_fwd``, ``hgq::group_norm_bwd`` and ``hgq::global_norm`` known, like those of ``ops.py``; the HIP library
+    """Makes the operators of ``csrc/hgq_torch.cpp`` (``hgq::global_norm``, ``hgq::group_norm_fwd`` and so on) known, like those of ``ops.py``; the HIP library
     is loaded when one is first called.  Where the extension is missing, or does not load, the first use says so."""
     try:
         host_extension()
@@ -307,6 +318,40 @@ def _load_host(path):
     @torch.library.register_fake('hgq::global_norm')
     def _(tensors):
         return tensors[0].new_empty((), dtype=torch.float32)
+
+    @torch.library.register_fake('hgq::distill_topk_fwd')
+    def _(logits, teacher_logits, teacher_indices, teacher_lse, sample_weight, temperature, gradient):
+        rows = logits.shape[0] if gradient else 0
+        number = torch.float32
+        return logits.new_empty((), dtype=number), logits.new_empty((rows, 4), dtype=number), logits.new_empty((rows, logits.shape[1]))
+
+    @torch.library.register_fake('hgq::distill_topk_bwd')
+    def _(upstream, logits, teacher_logits, teacher_indices, teacher_lse, sample_weight, stats, temperature):
+        return logits.new_empty(logits.shape)
+
+    @torch.library.register_fake('hgq::distill_topk_bwd_')
+    def _(upstream, logits, teacher_logits, teacher_indices, teacher_lse, sample_weight, stats, temperature, dlogits):
+        return None
+
+    @torch.library.register_fake('hgq::relative_bias_fwd')
+    def _(scores, table, offsets, offset, first, both):
+        return scores.new_empty(scores.shape)
+
+    @torch.library.register_fake('hgq::relative_bias_bwd')
+    def _(dout, offsets, offset, first, both):
+        return dout.new_empty(((len(first) + 1) * (2 if both else 1), dout.shape[1]), dtype=torch.float32)
+
+    @torch.library.register_fake('hgq::residual_norm_fwd')
+    def _(x, update, gate, post_gamma, pre_gamma, gate_rows, scale, epsilon, act, keep):
+        has = update.shape == x.shape
+        rows = x.numel() // x.shape[-1]
+        return (torch.empty_like(x) if has else x.new_empty(0), torch.empty_like(x), x.new_empty((2 if has else 1) * rows if keep else 0, dtype=torch.float32))
+
+    @torch.library.register_fake('hgq::residual_norm_bwd')
+    def _(dy, dh, x, update, gate, post_gamma, pre_gamma, r, gate_rows, scale, epsilon, act, need_dx, need_dupdate, need_dgate, need_dpost, need_dpre):
+        like = lambda t, need: torch.empty_like(t) if need else x.new_empty(0)  # noqa: E731
+        vector = lambda need: x.new_empty(x.shape[-1] if need else 0, dtype=torch.float32)  # noqa: E731
+        return like(x, need_dx), like(x, need_dupdate and update.shape == x.shape), like(gate, need_dgate), vector(need_dpost), vector(need_dpre)
 
     return mod
 

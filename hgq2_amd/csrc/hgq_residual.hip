@@ -1,0 +1,497 @@
+// What stands between two blocks of a network: the norm behind the first, its gate, the residual sum and the norm ahead of the second.
+// Rows of C channels, norm(v) = v / sqrt(mean(v^2) + eps):
+//     n = norm(u);   b = scale act(gate) n post;   y = x + b;   h = norm(y) pre               (act: none, or 1 / (1 + exp(-gate)))
+// Backward, given dy and dh, with m = norm(y), e = dh pre and r_u, r_y the factors of both norms:
+//     dx = dy + r_y (e - m mean(e m));   dn = dx scale act(gate) post;   du = r_u (dn - n mean(dn n))
+//     dpre = sum dh m,  dpost = sum dx scale act(gate) n  over rows;   dgate = dx scale n post act'(gate)
+// A gate has an element for each of x, or one row for P rows (a sample's positions): its gradient is then a sum over them.  Without u: y = x.
+//
+// Bound by memory.  One pass each way: a row's elements stay in registers, eight a thread, while a team of as many threads as the row needs
+// forms both means; the backward pass forms y again from x (which costs the bytes that y would, and keeps what y's rounding drops).  Sums over rows stay
+// in registers while a workgroup goes from row to row, and leave as one slice per workgroup, added in a fixed order.
+#include <type_traits>
+
+#include "hgq_host.h"
+#include "hgq_vector.h"
+
+namespace hgq {
+
+constexpr int RES_HELD = 8;     // elements of a row in a thread
+constexpr int RES_WIDEST = 8192;  // channels up to which 1024 threads hold a row
+
+struct ResidualRows {
+    const void *x, *u, *gate, *dy, *dh;
+    const float *post, *pre;
+    void *y, *h, *dx, *du, *dgate;
+    float *r_u, *r_y;
+    float *slices;       // [workgroups][2][C]: dpost, dpre
+    float *gate_slices;  // [units][C], or null: dgate is written as it is formed
+    int64_t rows, P, units, per_unit, cuts;  // rows; of a gate's row; what a workgroup takes at a time, its rows; units of a sample
+    int C, tpr, act, by_sample;
+    float scale, eps;
+};
+
+// the threads of a row: neighbouring lanes of a wavefront, or (WIDE) a workgroup
+template <bool WIDE>
+__device__ __forceinline__ float row_sum(float v, int tpr, float *lds) {
+    if (!WIDE) return team_sum(v, tpr);
+    v = team_sum(v, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const int waves = tpr >> 6;
+    v = team_sum(lds[threadIdx.x & (waves - 1)], waves);
+    __syncthreads();
+    return v;
+}
+
+__device__ __forceinline__ float norm_factor(float sum, int C, float eps) { return 1.0f / sqrtf(sum / (float)C + eps); }
+
+__device__ __forceinline__ float opened(float g, int act) { return act ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269502f)) : g; }
+
+template <typename T>
+struct Held {
+    static constexpr int N = Vec<T>::N, NV = RES_HELD / N;
+    int at[NV], n[NV];  // this thread's columns
+    __device__ __forceinline__ Held(int lane, int tpr, int C) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) at[v] = (v * tpr + lane) * N, n[v] = max(0, min(N, C - at[v]));
+    }
+    __device__ __forceinline__ void load(float *f, const T *row) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const Vec<T> r = n[v] == N ? load_vec(row + at[v]) : load_part(row + at[v], n[v], (T)0.0f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[v * N + e] = (float)r.v[e];
+        }
+    }
+    __device__ __forceinline__ void store(T *row, const float *f) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            Vec<T> r;
+#pragma unroll
+            for (int e = 0; e < N; ++e) r.v[e] = (T)f[v * N + e];
+            if (n[v] == N) store_vec(row + at[v], r);
+            else store_part(row + at[v], r, n[v]);
+        }
+    }
+    __device__ __forceinline__ void vector(float *f, const float *p, float scale) const {  // of channels, times `scale`
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[v * N + e] = e < n[v] ? (p ? p[at[v] + e] : 1.0f) * scale : 0.0f;
+    }
+};
+
+enum { NO_UPDATE, NO_GATE, GATED };
+
+template <typename T, int KIND, bool WIDE>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void residual_fwd(const ResidualRows a) {
+    __shared__ float lds[16];
+    const int teams = WIDE ? 1 : 256 / a.tpr, slot = WIDE ? 0 : threadIdx.x / a.tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (a.tpr - 1);
+    const Held<T> held(lane, a.tpr, a.C);
+    float post[RES_HELD], pre[RES_HELD];
+    if (KIND != NO_UPDATE) held.vector(post, a.post, a.scale);
+    held.vector(pre, a.pre, 1.0f);
+    for (int64_t row = (int64_t)blockIdx.x * teams + slot; row < a.rows; row += (int64_t)gridDim.x * teams) {
+        const int64_t base = row * a.C;
+        float y[RES_HELD], u[RES_HELD], g[RES_HELD], s = 0;
+        held.load(y, (const T *)a.x + base);
+        if (KIND != NO_UPDATE) {
+            held.load(u, (const T *)a.u + base);
+            if (KIND == GATED) held.load(g, (const T *)a.gate + (a.by_sample ? row / a.P * a.C : base));
+#pragma unroll
+            for (int e = 0; e < RES_HELD; ++e) s += u[e] * u[e];
+            const float r_u = norm_factor(row_sum<WIDE>(s, a.tpr, lds), a.C, a.eps);
+            s = 0;
+#pragma unroll
+            for (int e = 0; e < RES_HELD; ++e) {
+                float b = u[e] * r_u * post[e];
+                if (KIND == GATED) b *= opened(g[e], a.act);
+                y[e] += b;
+            }
+            if (a.r_u && lane == 0) a.r_u[row] = r_u;
+            held.store((T *)a.y + base, y);
+        }
+#pragma unroll
+        for (int e = 0; e < RES_HELD; ++e) s += y[e] * y[e];
+        const float r_y = norm_factor(row_sum<WIDE>(s, a.tpr, lds), a.C, a.eps);
+        if (a.r_y && lane == 0) a.r_y[row] = r_y;
+#pragma unroll
+        for (int e = 0; e < RES_HELD; ++e) y[e] *= r_y * pre[e];
+        held.store((T *)a.h + base, y);
+    }
+}
+
+template <typename T, int KIND, bool WIDE>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void residual_bwd(const ResidualRows a) {
+    __shared__ float lds[16];
+    __shared__ float joined[WIDE ? 1 : 256 * RES_HELD];
+    const int teams = WIDE ? 1 : 256 / a.tpr, slot = WIDE ? 0 : threadIdx.x / a.tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (a.tpr - 1);
+    const Held<T> held(lane, a.tpr, a.C);
+    float post[RES_HELD], pre[RES_HELD], dpost[RES_HELD] = {}, dpre[RES_HELD] = {}, dgate[RES_HELD] = {};
+    if (KIND != NO_UPDATE) held.vector(post, a.post, a.scale);
+    held.vector(pre, a.pre, 1.0f);
+
+    // one row of channels from the teams' sums, in order
+    auto leave = [&](const float *f, auto *out) {
+        if (WIDE) {
+#pragma unroll
+            for (int v = 0; v < Held<T>::NV; ++v)
+#pragma unroll
+                for (int e = 0; e < Held<T>::N; ++e)
+                    if (e < held.n[v]) out[held.at[v] + e] = (std::remove_reference_t<decltype(*out)>)f[v * Held<T>::N + e];
+            return;
+        }
+        __syncthreads();
+        const int width = a.tpr * RES_HELD;
+#pragma unroll
+        for (int v = 0; v < Held<T>::NV; ++v)
+#pragma unroll
+            for (int e = 0; e < Held<T>::N; ++e) joined[slot * width + held.at[v] + e] = f[v * Held<T>::N + e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.C; c += 256) {
+            float s = 0;
+            for (int t = 0; t < teams; ++t) s += joined[t * width + c];
+            out[c] = (std::remove_reference_t<decltype(*out)>)s;
+        }
+    };
+
+    for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        const int64_t sample = unit / a.cuts, r0 = sample * a.P + (unit - sample * a.cuts) * a.per_unit, r1 = min(min(r0 + a.per_unit, (sample + 1) * a.P), a.rows);
+        float g[RES_HELD], open[RES_HELD];
+        if (KIND == GATED && a.by_sample) held.load(g, (const T *)a.gate + sample * a.C);
+        for (int64_t row = r0 + slot; row < r1; row += teams) {
+            const int64_t base = row * a.C;
+            float x[RES_HELD], n[RES_HELD], dy[RES_HELD], dh[RES_HELD];
+            held.load(x, (const T *)a.x + base);
+            if (KIND != NO_UPDATE) held.load(n, (const T *)a.u + base);
+            if (KIND == GATED && !a.by_sample) held.load(g, (const T *)a.gate + base);
+            if (a.dy) held.load(dy, (const T *)a.dy + base);
+            if (a.dh) held.load(dh, (const T *)a.dh + base);
+            const float r_u = KIND != NO_UPDATE ? a.r_u[row] : 0.0f, r_y = a.r_y[row];
+            if (KIND != NO_UPDATE) {
+#pragma unroll
+                for (int e = 0; e < RES_HELD; ++e) {
+                    n[e] *= r_u;
+                    float b = n[e] * post[e];
+                    if (KIND == GATED) open[e] = opened(g[e], a.act), b *= open[e];
+                    x[e] += b;
+                }
+            }
+            if (a.dh) {
+                float s = 0;
+#pragma unroll
+                for (int e = 0; e < RES_HELD; ++e) {
+                    x[e] *= r_y;  // m
+                    dpre[e] += dh[e] * x[e];
+                    dh[e] *= pre[e];
+                    s += dh[e] * x[e];
+                }
+                s = row_sum<WIDE>(s, a.tpr, lds) / (float)a.C;
+#pragma unroll
+                for (int e = 0; e < RES_HELD; ++e) {
+                    const float d = r_y * (dh[e] - x[e] * s);
+                    dy[e] = a.dy ? dy[e] + d : d;
+                }
+            }
+            if (a.dx) held.store((T *)a.dx + base, dy);
+            if (KIND == NO_UPDATE) continue;
+            float s = 0, dn[RES_HELD];
+#pragma unroll
+            for (int e = 0; e < RES_HELD; ++e) {
+                const float db = KIND == GATED ? dy[e] * open[e] : dy[e];
+                dpost[e] += db * n[e];
+                dn[e] = db * post[e];
+                s += dn[e] * n[e];
+                if (KIND == GATED) {
+                    float dg = dy[e] * (n[e] * post[e]);
+                    if (a.act) dg *= open[e] * (1.0f - open[e]);
+                    if (a.by_sample) dgate[e] += dg;
+                    else open[e] = dg;
+                }
+            }
+            if (KIND == GATED && !a.by_sample && a.dgate) held.store((T *)a.dgate + base, open);
+            if (a.du) {
+                s = row_sum<WIDE>(s, a.tpr, lds) / (float)a.C;
+#pragma unroll
+                for (int e = 0; e < RES_HELD; ++e) dn[e] = r_u * (dn[e] - n[e] * s);
+                held.store((T *)a.du + base, dn);
+            }
+        }
+        if (KIND == GATED && a.by_sample && a.dgate) {
+            if (a.gate_slices) leave(dgate, a.gate_slices + unit * a.C);
+            else leave(dgate, (T *)a.dgate + sample * a.C);
+#pragma unroll
+            for (int e = 0; e < RES_HELD; ++e) dgate[e] = 0;
+        }
+    }
+    if (a.slices) {
+        float *out = a.slices + (int64_t)blockIdx.x * 2 * a.C;
+        if (KIND != NO_UPDATE) {
+#pragma unroll
+            for (int e = 0; e < RES_HELD; ++e) dpost[e] *= a.scale;
+            leave(dpost, out);
+        }
+        leave(dpre, out + a.C);
+    }
+}
+
+// Rows of more channels than a workgroup holds: read again for each of the means, sums over rows in the workgroup's own slice.
+template <typename T>
+__device__ __forceinline__ float residual_sum_element(const ResidualRows &a, int64_t base, int64_t gate_base, int c, float r_u) {
+    float y = (float)((const T *)a.x)[base + c];
+    if (a.u) {
+        float b = (float)((const T *)a.u)[base + c] * r_u * ((a.post ? a.post[c] : 1.0f) * a.scale);
+        if (a.gate) b *= opened((float)((const T *)a.gate)[gate_base + c], a.act);
+        y += b;
+    }
+    return y;
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
+    __shared__ float lds[16];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int64_t base = row * a.C, gate_base = a.by_sample ? row / a.P * a.C : base;
+        float r_u = 0, s = 0;
+        if (a.u) {
+            for (int c = threadIdx.x; c < a.C; c += 1024) {
+                const float u = (float)((const T *)a.u)[base + c];
+                s += u * u;
+            }
+            r_u = norm_factor(row_sum<true>(s, 1024, lds), a.C, a.eps);
+            s = 0;
+        }
+        for (int c = threadIdx.x; c < a.C; c += 1024) {
+            const float y = residual_sum_element<T>(a, base, gate_base, c, r_u);
+            s += y * y;
+        }
+        const float r_y = norm_factor(row_sum<true>(s, 1024, lds), a.C, a.eps);
+        for (int c = threadIdx.x; c < a.C; c += 1024) {
+            const float y = residual_sum_element<T>(a, base, gate_base, c, r_u);
+            if (a.u) ((T *)a.y)[base + c] = (T)y;
+            ((T *)a.h)[base + c] = (T)(y * (r_y * (a.pre ? a.pre[c] : 1.0f)));
+        }
+        if (threadIdx.x == 0) {
+            if (a.r_u) a.r_u[row] = r_u;
+            if (a.r_y) a.r_y[row] = r_y;
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
+    __shared__ float lds[16];
+    float *dpost = a.slices ? a.slices + (int64_t)blockIdx.x * 2 * a.C : nullptr, *dpre = dpost ? dpost + a.C : nullptr;
+    if (dpost)
+        for (int c = threadIdx.x; c < 2 * a.C; c += 1024) dpost[c] = 0;
+    __syncthreads();
+    for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        const int64_t sample = unit / a.cuts, r0 = sample * a.P + (unit - sample * a.cuts) * a.per_unit, r1 = min(min(r0 + a.per_unit, (sample + 1) * a.P), a.rows);
+        float *dgate = a.by_sample && a.dgate ? a.gate_slices + unit * a.C : nullptr;
+        for (int64_t row = r0; row < r1; ++row) {
+            const int64_t base = row * a.C, gate_base = a.by_sample ? sample * a.C : base;
+            const float r_u = a.u ? a.r_u[row] : 0.0f, r_y = a.r_y[row];
+            float s1 = 0, s2 = 0;
+            if (a.dh) {
+                for (int c = threadIdx.x; c < a.C; c += 1024)
+                    s1 += (float)((const T *)a.dh)[base + c] * (a.pre ? a.pre[c] : 1.0f) * (residual_sum_element<T>(a, base, gate_base, c, r_u) * r_y);
+                s1 = row_sum<true>(s1, 1024, lds) / (float)a.C;
+            }
+            auto through = [&](int c, float &dh_m) {  // dx of channel c
+                float d = a.dy ? (float)((const T *)a.dy)[base + c] : 0.0f;
+                if (a.dh) {
+                    const float m = residual_sum_element<T>(a, base, gate_base, c, r_u) * r_y, dh = (float)((const T *)a.dh)[base + c];
+                    dh_m = dh * m;
+                    d += r_y * (dh * (a.pre ? a.pre[c] : 1.0f) - m * s1);
+                }
+                return d;
+            };
+            for (int c = threadIdx.x; c < a.C; c += 1024) {
+                float dh_m = 0;
+                const float d = through(c, dh_m);
+                if (dpre) dpre[c] += dh_m;
+                if (a.dx) ((T *)a.dx)[base + c] = (T)d;
+                if (!a.u) continue;
+                const float n = (float)((const T *)a.u)[base + c] * r_u, post = (a.post ? a.post[c] : 1.0f) * a.scale;
+                const float open = a.gate ? opened((float)((const T *)a.gate)[gate_base + c], a.act) : 1.0f, db = d * open;
+                if (dpost) dpost[c] += db * n * a.scale;
+                s2 += db * post * n;
+                if (a.dgate) {
+                    float dg = d * (n * post);
+                    if (a.act) dg *= open * (1.0f - open);
+                    if (dgate) dgate[c] = row == r0 ? dg : dgate[c] + dg;
+                    else ((T *)a.dgate)[base + c] = (T)dg;
+                }
+            }
+            if (!a.du) continue;
+            s2 = row_sum<true>(s2, 1024, lds) / (float)a.C;
+            for (int c = threadIdx.x; c < a.C; c += 1024) {
+                float unused;
+                const float n = (float)((const T *)a.u)[base + c] * r_u, post = (a.post ? a.post[c] : 1.0f) * a.scale;
+                const float open = a.gate ? opened((float)((const T *)a.gate)[gate_base + c], a.act) : 1.0f;
+                ((T *)a.du)[base + c] = (T)(r_u * (through(c, unused) * open * post - n * s2));
+            }
+        }
+    }
+}
+
+// out[b][c] = sum over n of in[b][n][c] (rows of `stride` floats), 32 columns and 32 runs of rows a workgroup, joined in fp64
+template <typename T>
+__global__ __launch_bounds__(1024) void residual_join(const float *__restrict__ in, int64_t n, int C, int64_t stride, T *__restrict__ out) {
+    __shared__ double sums[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5;
+    const float *from = in + (int64_t)blockIdx.y * n * stride;
+    double s = 0;
+    if (c < C)
+        for (int64_t k = run; k < n; k += 32) s += from[k * stride + c];
+    sums[run][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (run == 0 && c < C) {
+        s = 0;
+        for (int r = 0; r < 32; ++r) s += sums[r][threadIdx.x & 31];
+        out[(int64_t)blockIdx.y * C + c] = (T)(float)s;
+    }
+}
+
+namespace {
+
+int check_residual(const char *what, int64_t rows, int64_t P, int64_t C, float scale, float eps, int act, int type) {
+    if (rows < 0 || P < 1 || C < 1 || !(eps >= 0) || scale != scale || rows % P) return fail(HGQ_ERR_ARG, "%s: rows %lld (%lld a gate), channels %lld, epsilon %g, scale %g", what, (long long)rows, (long long)P, (long long)C, eps, scale);
+    if (type < HGQ_TYPE_F32 || type > HGQ_TYPE_F16 || act < 0 || act > 1) return fail(HGQ_ERR_ARG, "%s: unknown type or activation", what);
+    if (C > 1 << 28 || rows > (int64_t)1 << 40) return fail(HGQ_ERR_UNSUPPORTED, "%s: %lld rows of %lld channels", what, (long long)rows, (long long)C);
+    return HGQ_OK;
+}
+
+struct ResidualPlan {
+    int tpr, threads, grid;
+    int64_t units, per_unit, cuts;
+};
+
+// by_sample: a unit has rows of one sample, whose gate's gradient it adds up
+ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample) {
+    ResidualPlan p;
+    p.tpr = 1;
+    while (p.tpr * RES_HELD < C && p.tpr < 1024) p.tpr *= 2;
+    p.threads = p.tpr > 256 ? p.tpr : 256;
+    if (p.tpr > 64) p.threads = p.tpr;
+    const int teams = p.tpr > 64 ? 1 : 256 / p.tpr;
+    const int64_t most = 256 * (p.threads >= 1024 ? 1 : 1024 / p.threads);
+    if (by_sample) {
+        const int64_t samples = rows / P;
+        p.cuts = samples < most ? (most + samples - 1) / samples : 1;
+        int64_t fewest = 8 * teams;  // rows that pay for a slice
+        if (p.cuts > (P + fewest - 1) / fewest) p.cuts = (P + fewest - 1) / fewest;
+        p.per_unit = (P + p.cuts - 1) / p.cuts;
+        p.cuts = (P + p.per_unit - 1) / p.per_unit;
+        p.units = samples * p.cuts;
+    } else {
+        p.per_unit = (rows + most - 1) / most;
+        p.per_unit = (p.per_unit + teams - 1) / teams * teams;
+        p.cuts = p.units = (rows + p.per_unit - 1) / p.per_unit;
+    }
+    p.grid = (int)(p.units < most ? p.units : most);
+    return p;
+}
+
+template <typename T, int KIND>
+int forward(const ResidualRows &a, const ResidualPlan &p, hipStream_t st) {
+    const int64_t most = 256 * 2048 / p.threads;
+    if (a.C > RES_WIDEST) {
+        hipLaunchKernelGGL((residual_fwd_any<T>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(1024), 0, st, a);
+    } else if (p.tpr > 64) {
+        hipLaunchKernelGGL((residual_fwd<T, KIND, true>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(p.tpr), 0, st, a);
+    } else {
+        const int64_t blocks = (a.rows + 256 / p.tpr - 1) / (256 / p.tpr);
+        hipLaunchKernelGGL((residual_fwd<T, KIND, false>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, a);
+    }
+    return check_launch("hgq_residual_norm_fwd");
+}
+
+template <typename T, int KIND>
+int backward(const ResidualRows &a, const ResidualPlan &p, float *dpost, float *dpre, hipStream_t st) {
+    const char *what = "hgq_residual_norm_bwd";
+    if (a.C > RES_WIDEST) hipLaunchKernelGGL((residual_bwd_any<T>), dim3(p.grid), dim3(1024), 0, st, a);
+    else if (p.tpr > 64) hipLaunchKernelGGL((residual_bwd<T, KIND, true>), dim3(p.grid), dim3(p.tpr), 0, st, a);
+    else hipLaunchKernelGGL((residual_bwd<T, KIND, false>), dim3(p.grid), dim3(256), 0, st, a);
+    int rc = check_launch(what);
+    const unsigned columns = (unsigned)((a.C + 31) / 32);
+    if (!rc && dpost) {
+        hipLaunchKernelGGL(residual_join<float>, dim3(columns), dim3(1024), 0, st, (const float *)a.slices, (int64_t)p.grid, a.C, (int64_t)2 * a.C, dpost);
+        rc = check_launch(what);
+    }
+    if (!rc && dpre) {
+        hipLaunchKernelGGL(residual_join<float>, dim3(columns), dim3(1024), 0, st, (const float *)a.slices + a.C, (int64_t)p.grid, a.C, (int64_t)2 * a.C, dpre);
+        rc = check_launch(what);
+    }
+    if (!rc && a.gate_slices) {
+        const int64_t samples = a.rows / a.P;
+        for (int64_t b = 0; b < samples && !rc; b += 65535) {
+            const unsigned many = (unsigned)(samples - b < 65535 ? samples - b : 65535);
+            hipLaunchKernelGGL(residual_join<T>, dim3(columns, many), dim3(1024), 0, st, (const float *)a.gate_slices + b * p.cuts * a.C, p.cuts, a.C, (int64_t)a.C, (T *)a.dgate + b * a.C);
+            rc = check_launch(what);
+        }
+    }
+    return rc;
+}
+
+bool slices_of_gate(const ResidualPlan &p, int C) { return p.cuts > 1 || C > RES_WIDEST; }
+
+template <typename T>
+auto forward_of(int kind) {
+    return kind == NO_UPDATE ? forward<T, NO_UPDATE> : kind == NO_GATE ? forward<T, NO_GATE> : forward<T, GATED>;
+}
+
+template <typename T>
+auto backward_of(int kind) {
+    return kind == NO_UPDATE ? backward<T, NO_UPDATE> : kind == NO_GATE ? backward<T, NO_GATE> : backward<T, GATED>;
+}
+
+}  // namespace
+}  // namespace hgq
+
+using namespace hgq;
+
+extern "C" int hgq_residual_norm_fwd(const void *x, const void *u, const void *gate, const float *post, const float *pre, void *y, void *h, float *r_u, float *r_y,
+                                     int64_t rows, int64_t P, int64_t C, float scale, float eps, int act, int type, void *stream) {
+    const char *what = "hgq_residual_norm_fwd";
+    int rc = check_residual(what, rows, P, C, scale, eps, act, type);
+    if (rc || rows == 0) return rc;
+    if (!x || !h || (u && !y) || (gate && !u)) return fail(HGQ_ERR_ARG, "%s: null pointer", what);
+    ResidualRows a = {};
+    a.x = x, a.u = u, a.gate = gate, a.post = post, a.pre = pre, a.y = y, a.h = h, a.r_u = u ? r_u : nullptr, a.r_y = r_y;
+    const ResidualPlan p = residual_plan(rows, P, (int)C, false);
+    a.rows = rows, a.P = P, a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.scale = scale, a.eps = eps;
+    const int kind = !u ? NO_UPDATE : gate ? GATED : NO_GATE;
+    return (type == HGQ_TYPE_F32 ? forward_of<float>(kind) : type == HGQ_TYPE_BF16 ? forward_of<__bf16>(kind) : forward_of<_Float16>(kind))(a, p, (hipStream_t)stream);
+}
+
+extern "C" int64_t hgq_residual_norm_bwd_workspace(int64_t rows, int64_t P, int64_t C, int type) {
+    if (check_residual("hgq_residual_norm_bwd_workspace", rows, P, C, 1.0f, 0.0f, 0, type)) return -1;
+    if (rows == 0) return 0;
+    const ResidualPlan p = residual_plan(rows, P, (int)C, P > 1);
+    return 2 * p.grid * C + (P > 1 && slices_of_gate(p, (int)C) ? p.units * C : 0);
+}
+
+extern "C" int hgq_residual_norm_bwd(const void *dy, const void *dh, const void *x, const void *u, const void *gate, const float *post, const float *pre,
+                                     const float *r_u, const float *r_y, void *dx, void *du, void *dgate, float *dpost, float *dpre, float *workspace,
+                                     int64_t rows, int64_t P, int64_t C, float scale, float eps, int act, int type, void *stream) {
+    const char *what = "hgq_residual_norm_bwd";
+    int rc = check_residual(what, rows, P, C, scale, eps, act, type);
+    if (rc) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (rows == 0) {
+        if (dpost && (rc = fill_f32(dpost, 0.0f, C, st))) return rc;
+        return dpre ? fill_f32(dpre, 0.0f, C, st) : HGQ_OK;
+    }
+    if (!x || !r_y || (u && !r_u) || (!dy && !dh) || !workspace || (gate && !u) || (dgate && !gate) || (!u && (du || dpost))) return fail(HGQ_ERR_ARG, "%s: null pointer", what);
+    const ResidualPlan p = residual_plan(rows, P, (int)C, P > 1);
+    ResidualRows a = {};
+    a.x = x, a.u = u, a.gate = gate, a.dy = dy, a.dh = dh, a.post = post, a.pre = pre, a.dx = dx, a.du = du, a.dgate = dgate;
+    a.r_u = (float *)r_u, a.r_y = (float *)r_y, a.slices = dpost || dpre ? workspace : nullptr;
+    a.gate_slices = dgate && P > 1 && slices_of_gate(p, (int)C) ? workspace + 2 * p.grid * C : nullptr;
+    a.rows = rows, a.P = P > 1 ? P : rows, a.units = p.units, a.per_unit = p.per_unit, a.cuts = p.cuts;
+    a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1 && gate, a.scale = scale, a.eps = eps;
+    const int kind = !u ? NO_UPDATE : gate ? GATED : NO_GATE;
+    return (type == HGQ_TYPE_F32 ? backward_of<float>(kind) : type == HGQ_TYPE_BF16 ? backward_of<__bf16>(kind) : backward_of<_Float16>(kind))(a, p, dpost, dpre, st);
+}

@@ -1,5 +1,6 @@
-// The host side of the operators whose calls are short beside what Python costs around them: group normalisation with its autograd
-// node (a backward pass in Python waits for the interpreter on the engine's thread: 118 us for two launches of 10 us each), the
+// The host side of the operators whose calls are short beside what Python costs around them: group normalisation, distillation, the
+// relative position bias and the norms around a residual sum with their autograd
+// nodes (a backward pass in Python waits for the interpreter on the engine's thread: 118 us for two launches of 10 us each), the
 // global norm, and the walk over an optimizer's variables (28 variables: 34 us in Python).  Arguments are checked here, the kernels are
 // called through the C ABI of libhgq_hip.so (bind()), outputs and workspaces are torch tensors on the current stream of their device.
 #include <ATen/ATen.h>
@@ -10,6 +11,7 @@
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
@@ -31,6 +33,15 @@ struct Library {  // the entry points that are called from here
     decltype(&hgq_group_norm_fwd) group_norm_fwd;
     decltype(&hgq_group_norm_bwd_workspace) group_norm_bwd_workspace;
     decltype(&hgq_group_norm_bwd) group_norm_bwd;
+    decltype(&hgq_distill_topk_workspace) distill_topk_workspace;
+    decltype(&hgq_distill_topk_fwd) distill_topk_fwd;
+    decltype(&hgq_distill_topk_bwd) distill_topk_bwd;
+    decltype(&hgq_relative_bias_fwd) relative_bias_fwd;
+    decltype(&hgq_relative_bias_bwd_workspace) relative_bias_bwd_workspace;
+    decltype(&hgq_relative_bias_bwd) relative_bias_bwd;
+    decltype(&hgq_residual_norm_fwd) residual_norm_fwd;
+    decltype(&hgq_residual_norm_bwd_workspace) residual_norm_bwd_workspace;
+    decltype(&hgq_residual_norm_bwd) residual_norm_bwd;
 } lib;
 PyObject *library_error = nullptr;  // hgq2_amd._lib.HGQLibraryError
 
@@ -219,6 +230,392 @@ Tensor group_norm(const Tensor &x, int64_t groups, const std::optional<Tensor> &
     return std::get<0>(forward_op().call(x.contiguous(), ga, be, groups, epsilon, act));
 }
 
+// ---- what the three operators below share --------------------------------------------------------------------------------
+void on_gpu(const char *name, const Tensor &t) {
+    TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a GPU tensor (there is no CPU implementation), got device ", t.device());
+    TORCH_CHECK_VALUE(type_code(t.scalar_type()) >= 0, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+}
+
+// float32 numbers, `n` of them (empty: none)
+void numbers(const char *name, const Tensor &t, int64_t n, const Tensor &like) {
+    TORCH_CHECK_VALUE(t.numel() == 0 || (t.numel() == n && t.scalar_type() == at::kFloat && t.device() == like.device() && t.is_contiguous()), name,
+                      " must be a contiguous float32 tensor of ", n, " elements on ", like.device(), ", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+}
+
+bool differentiated(const Tensor &t) { return t.defined() && ((t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined()); }
+
+Tensor plain(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+// Gradients asked for with create_graph, of any operator: see OnceOnly.
+struct AllOnceOnly : torch::autograd::Function<AllOnceOnly> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, at::TensorList grads, at::TensorList inputs, std::string what) {
+        ctx->saved_data["what"] = what;
+        torch::autograd::variable_list out;
+        for (const Tensor &g : grads) out.push_back(g.view_as(g));
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &) {
+        TORCH_CHECK(false, ctx->saved_data["what"].toStringRef(), " is differentiable once: its gradients have no gradient");
+    }
+};
+
+void once_only(torch::autograd::variable_list &grads, const std::vector<Tensor> &inputs, const char *what) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::variable_list there, from;
+    for (const Tensor &g : grads)
+        if (g.defined()) there.push_back(g);
+    for (const Tensor &t : inputs)
+        if (t.defined()) from.push_back(t);
+    if (there.empty()) return;
+    const auto out = AllOnceOnly::apply(at::TensorList(there), at::TensorList(from), std::string(what));
+    size_t k = 0;
+    for (Tensor &g : grads)
+        if (g.defined()) g = out[k++];
+}
+
+// ---- distillation from a teacher's top logits --------------------------------------------------------------------------
+struct DistillSizes {
+    int64_t rows, V, K;
+    int type, t_type, index_bytes;
+};
+
+DistillSizes distill_sizes(const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, double T) {
+    on_gpu("logits", z), on_gpu("teacher_logits", t);
+    TORCH_CHECK_VALUE(z.dim() == 2 && t.dim() == 2 && t.size(0) == z.size(0), "logits [rows, vocabulary] and teacher_logits [rows, entries] expected, got ", z.sizes(), " and ", t.sizes());
+    TORCH_CHECK_VALUE(z.size(1) >= 1 && t.size(1) >= 1, "logits and teacher_logits must have entries, got ", z.sizes(), " and ", t.sizes());
+    TORCH_CHECK_VALUE((z.stride(1) == 1 || z.size(1) == 1) && z.stride(0) >= 0, "rows of logits must be contiguous");
+    TORCH_CHECK_VALUE(index.sizes() == t.sizes() && (index.scalar_type() == at::kInt || index.scalar_type() == at::kLong), "teacher_indices must be int32 or int64 and like teacher_logits, got ",
+                      index.scalar_type(), " ", index.sizes());
+    TORCH_CHECK_VALUE(t.device() == z.device() && index.device() == z.device(), "logits and the teacher's list must be on one device");
+    TORCH_CHECK_VALUE(t.is_contiguous() && index.is_contiguous(), "the teacher's list must be contiguous");
+    numbers("teacher_lse", lse, z.size(0), z), numbers("sample_weight", weight, z.size(0), z);
+    TORCH_CHECK_VALUE(T > 0 && std::isfinite(T), "temperature must be positive, got ", T);
+    return {z.size(0), z.size(1), t.size(1), type_code(z.scalar_type()), type_code(t.scalar_type()), index.scalar_type() == at::kLong ? 8 : 4};
+}
+
+std::tuple<Tensor, Tensor, Tensor> distill_topk_fwd(const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, double T, bool gradient) {
+    const DistillSizes s = distill_sizes(z, t, index, lse, weight, T);
+    const c10::DeviceGuard guard(z.device());
+    const auto options = z.options().dtype(at::kFloat);
+    Tensor loss = at::empty({}, options), stats = at::empty({gradient ? s.rows : 0, 4}, options), dz = at::empty({gradient ? s.rows : 0, s.V}, z.options());
+    const Workspace<float> ws(library().distill_topk_workspace(s.rows, s.V, s.K, lse.numel() > 0));
+    check(lib.distill_topk_fwd(memory(z), z.stride(0), memory(t), s.t_type, memory(index), s.index_bytes, floats(lse), floats(weight), loss.data_ptr<float>(), floats(stats),
+                               memory(dz), ws.get(), s.rows, s.V, s.K, T, s.type, stream_of(z)),
+          "hgq_distill_topk_fwd");
+    return {loss, stats, dz};
+}
+
+void distill_backward(const Tensor &up, const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, const Tensor &stats, const Tensor &dz, bool holds_unit,
+                      double T) {
+    const DistillSizes s = distill_sizes(z, t, index, lse, weight, T);
+    TORCH_CHECK_VALUE(up.numel() == 1 && up.scalar_type() == at::kFloat && up.device() == z.device(), "the loss' gradient must be one float32 on ", z.device());
+    TORCH_CHECK_VALUE(stats.numel() == 4 * s.rows && stats.scalar_type() == at::kFloat && stats.device() == z.device() && stats.is_contiguous(), "stats must be what the forward call left");
+    TORCH_CHECK_VALUE(dz.sizes() == z.sizes() && dz.scalar_type() == z.scalar_type() && dz.device() == z.device() && dz.is_contiguous(), "the logits' gradient must be contiguous and like them");
+    const c10::DeviceGuard guard(z.device());
+    check(library().distill_topk_bwd(memory(z), z.stride(0), memory(t), s.t_type, memory(index), s.index_bytes, floats(lse), floats(weight), up.data_ptr<float>(), floats(stats), memory(dz),
+                                     holds_unit, s.rows, s.V, s.K, T, s.type, stream_of(z)),
+          "hgq_distill_topk_bwd");
+}
+
+Tensor distill_topk_bwd(const Tensor &up, const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, const Tensor &stats, double T) {
+    on_gpu("logits", z);
+    Tensor dz = at::empty(z.sizes(), z.options());
+    distill_backward(up, z, t, index, lse, weight, stats, dz, false, T);
+    return dz;
+}
+
+// `dz`: the gradient for an upstream of one, which is left as it is where the upstream is one
+void distill_topk_bwd_(const Tensor &up, const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, const Tensor &stats, double T, Tensor dz) {
+    distill_backward(up, z, t, index, lse, weight, stats, dz, true, T);
+}
+
+const auto &distill_op() {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::distill_topk_fwd", "").typed<decltype(distill_topk_fwd)>();
+    return op;
+}
+
+// The forward pass writes the gradient for an upstream of one while the row is at hand.  The backward pass hands it on where the upstream is one - the
+// kernel that looks at it ends at once - and forms it anew elsewhere, so there is one rounding whatever the upstream (a loss scaled
+// for float16 gets the gradients it was scaled for).  A graph that is kept may be asked again: it gets a tensor of its own each time.
+struct DistillTopk : torch::autograd::Function<DistillTopk> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, double T) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [loss, stats, dz] = distill_op().call(z, t, index, lse, weight, T, true);
+        ctx->save_for_backward({z, t, index, lse, weight, stats, dz});
+        ctx->saved_data["T"] = T;
+        return loss;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
+        static const auto anew = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::distill_topk_bwd", "").typed<decltype(distill_topk_bwd)>();
+        static const auto over = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::distill_topk_bwd_", "").typed<decltype(distill_topk_bwd_)>();
+        const auto saved = ctx->get_saved_variables();
+        torch::autograd::variable_list out(6);
+        if (!ctx->needs_input_grad(0)) return out;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const Tensor up = plain(grads[0]).to(at::kFloat);
+            if (torch::autograd::get_current_graph_task_keep_graph()) {
+                out[0] = anew.call(up, saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["T"].toDouble());
+            } else {
+                out[0] = saved[6];
+                over.call(up, saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["T"].toDouble(), out[0]);
+            }
+        }
+        once_only(out, {grads[0], saved[0]}, "distill_topk");
+        return out;
+    }
+};
+
+Tensor distill_topk(const Tensor &logits, const Tensor &teacher, const Tensor &indices, double T, const std::optional<Tensor> &lse, const std::optional<Tensor> &weight) {
+    const auto lead = [](const Tensor &t) { return t.sizes().slice(0, t.dim() - 1); };
+    TORCH_CHECK_VALUE(logits.dim() >= 1 && teacher.dim() == logits.dim() && lead(teacher) == lead(logits), "teacher_logits must have the logits' leading axes, got ", teacher.sizes(), " for ", logits.sizes());
+    TORCH_CHECK_VALUE(indices.sizes() == teacher.sizes(), "teacher_indices must be like teacher_logits, got ", indices.sizes(), " for ", teacher.sizes());
+    for (const auto &[name, t] : {std::make_pair("teacher_lse", &lse), std::make_pair("sample_weight", &weight)})
+        TORCH_CHECK_VALUE(!*t || (*t)->sizes() == lead(logits), name, " must have an element per row of logits, got ", (*t)->sizes(), " for ", logits.sizes());
+    TORCH_CHECK_VALUE(!differentiated(teacher) && !(lse && differentiated(*lse)) && !(weight && differentiated(*weight)), "distill_topk is differentiable in the logits alone: detach the teacher's tensors and the weights");
+    const bool graph = differentiated(logits);
+    if (graph) accumulates_here("logits", logits);
+    const int64_t V = logits.size(-1), K = teacher.size(-1);
+    int64_t rows = 1;
+    for (const int64_t n : lead(logits)) rows *= n;
+    Tensor z = logits.dim() == 2 ? logits : logits.reshape({rows, V});
+    if ((V > 1 && z.stride(1) != 1) || z.stride(0) < 0 || z.is_neg()) z = z.contiguous().resolve_neg();
+    const auto flat = [rows](const Tensor &t, int64_t n) { return plain(t.detach()).reshape({rows, n}).contiguous(); };
+    const Tensor none = lse && weight ? Tensor() : at::empty({0}, logits.options().dtype(at::kFloat).requires_grad(false));
+    const Tensor t = flat(teacher, K), i = flat(indices, K), l = lse ? flat(*lse, 1) : none, w = weight ? flat(*weight, 1) : none;
+    // an empty tensor stands for none: with no rows there is nothing that a lse could change
+    if (graph) return DistillTopk::apply(z, t, i, l, w, T);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return std::get<0>(distill_op().call(z, t, i, l, w, T, false));
+}
+
+// ---- relative position bias ----------------------------------------------------------------------------------------------
+struct BiasSizes {
+    int64_t B, H, T, S;
+    int type, m;
+    std::vector<int> first;
+};
+
+bool whole_planes(const Tensor &t) {
+    return t.numel() == 0 || ((t.size(3) == 1 || t.stride(3) == 1) && (t.size(2) == 1 || t.stride(2) == t.size(3)) && t.stride(0) >= 0 && t.stride(1) >= 0);
+}
+
+BiasSizes bias_sizes(const char *name, const Tensor &x, const Tensor &offsets, at::IntArrayRef first) {
+    on_gpu(name, x);
+    TORCH_CHECK_VALUE(x.dim() == 4, name, " must be [batch, heads, queries, keys], got ", x.sizes());
+    TORCH_CHECK_VALUE(whole_planes(x), name, ": a head's queries and keys must be contiguous");
+    TORCH_CHECK_VALUE(offsets.numel() == 0 || (offsets.dim() == 1 && offsets.numel() == x.size(0) && offsets.device() == x.device() && offsets.is_contiguous() &&
+                                               (offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong)),
+                      "offset must be a number, or a contiguous int32 or int64 tensor with one for each of the batch on ", x.device(), ", got ", offsets.scalar_type(), " ", offsets.sizes());
+    BiasSizes s = {x.size(0), x.size(1), x.size(2), x.size(3), type_code(x.scalar_type()), (int)first.size() + 1, {}};
+    for (const int64_t f : first) s.first.push_back(f > INT32_MAX ? INT32_MAX : (int)f);
+    return s;
+}
+
+// `first`: the first distances of the buckets of a direction but the nearest
+Tensor relative_bias_fwd(const Tensor &scores, const Tensor &table, const Tensor &offsets, int64_t offset, at::IntArrayRef first, bool both) {
+    const BiasSizes s = bias_sizes("scores", scores, offsets, first);
+    TORCH_CHECK_VALUE(table.scalar_type() == at::kFloat && table.device() == scores.device() && table.is_contiguous() && table.dim() == 2 && table.size(0) == (both ? 2 : 1) * s.m && table.size(1) == s.H,
+                      "table must be a contiguous float32 tensor [", (both ? 2 : 1) * s.m, ", ", s.H, "] on ", scores.device(), ", got ", table.scalar_type(), " ", table.sizes(), " on ", table.device());
+    const c10::DeviceGuard guard(scores.device());
+    Tensor out = at::empty(scores.sizes(), scores.options());
+    check(library().relative_bias_fwd(memory(scores), scores.stride(0), scores.stride(1), floats(table), memory(out), s.B, s.H, s.T, s.S, s.first.data(), s.m, both, offset, memory(offsets),
+                                      offsets.scalar_type() == at::kInt ? 4 : 8, s.type, stream_of(scores)),
+          "hgq_relative_bias_fwd");
+    return out;
+}
+
+Tensor relative_bias_bwd(const Tensor &dy, const Tensor &offsets, int64_t offset, at::IntArrayRef first, bool both) {
+    const BiasSizes s = bias_sizes("the scores' gradient", dy, offsets, first);
+    const c10::DeviceGuard guard(dy.device());
+    Tensor dtable = at::empty({(both ? 2 : 1) * s.m, s.H}, dy.options().dtype(at::kFloat));
+    const Workspace<float> ws(library().relative_bias_bwd_workspace(s.B, s.H, s.T, s.S, s.m, both));
+    check(lib.relative_bias_bwd(memory(dy), dy.stride(0), dy.stride(1), floats(dtable), ws.get(), s.B, s.H, s.T, s.S, s.first.data(), s.m, both, offset, memory(offsets),
+                                offsets.scalar_type() == at::kInt ? 4 : 8, s.type, stream_of(dy)),
+          "hgq_relative_bias_bwd");
+    return dtable;
+}
+
+const auto &bias_op() {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::relative_bias_fwd", "").typed<decltype(relative_bias_fwd)>();
+    return op;
+}
+
+// with a head's queries and keys in one piece
+Tensor planes(const Tensor &t) {
+    if (t.dim() == 4 && whole_planes(t) && !t.is_neg()) return t;
+    return t.contiguous().resolve_neg();
+}
+
+struct RelativeBias : torch::autograd::Function<RelativeBias> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &scores, const Tensor &table, const Tensor &offsets, int64_t offset, std::vector<int64_t> first, bool both) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({offsets});
+        ctx->saved_data["offset"] = offset, ctx->saved_data["first"] = first, ctx->saved_data["both"] = both;
+        return bias_op().call(scores, table, offsets, offset, first, both);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::relative_bias_bwd", "").typed<decltype(relative_bias_bwd)>();
+        torch::autograd::variable_list out(6), table(1);
+        if (ctx->needs_input_grad(0)) out[0] = grads[0];
+        if (ctx->needs_input_grad(1)) {
+            {
+                at::AutoDispatchBelowADInplaceOrView below;
+                table[0] = op.call(planes(grads[0]), ctx->get_saved_variables()[0], ctx->saved_data["offset"].toInt(), ctx->saved_data["first"].toIntVector(), ctx->saved_data["both"].toBool());
+            }
+            once_only(table, {grads[0]}, "relative_bias");
+            out[1] = table[0];
+        }
+        return out;
+    }
+};
+
+Tensor relative_bias(const Tensor &scores, const Tensor &table, std::vector<int64_t> first, bool both, int64_t offset, const std::optional<Tensor> &offsets) {
+    TORCH_CHECK_VALUE(scores.dim() == 3 || scores.dim() == 4, "scores must be [heads, queries, keys] or [batch, heads, queries, keys], got ", scores.sizes());
+    const bool graph = differentiated(scores) || differentiated(table);
+    if (graph) accumulates_here("scores", scores), accumulates_here("table", table);
+    const Tensor x = planes(scores.dim() == 3 ? scores.unsqueeze(0) : scores), none = offsets ? *offsets : at::empty({0}, scores.options().dtype(at::kLong).requires_grad(false));
+    Tensor out;
+    if (graph) {
+        out = RelativeBias::apply(x, plain(table.contiguous()), none, offset, first, both);
+    } else {
+        at::AutoDispatchBelowADInplaceOrView below;
+        out = bias_op().call(x, plain(table.contiguous()), none, offset, first, both);
+    }
+    return scores.dim() == 3 ? out.squeeze(0) : out;
+}
+
+// ---- norms around a residual sum -----------------------------------------------------------------------------------------
+struct ResidualSizes {
+    int64_t rows, C;
+    int type;
+};
+
+ResidualSizes residual_sizes(const Tensor &x, const Tensor &u, const Tensor &gate, const Tensor &post, const Tensor &pre, int64_t P) {
+    on_gpu("x", x);
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must be [..., channels], got ", x.sizes());
+    TORCH_CHECK_VALUE(x.is_contiguous(), "x must be contiguous");
+    const int64_t C = x.size(-1), rows = x.numel() / C;
+    TORCH_CHECK_VALUE((u.dim() == 1 && u.numel() == 0) || (u.sizes() == x.sizes() && u.scalar_type() == x.scalar_type() && u.device() == x.device() && u.is_contiguous()), "update must be contiguous and like x, got ",
+                      u.scalar_type(), " ", u.sizes(), " on ", u.device());
+    TORCH_CHECK_VALUE(P >= 1 && rows % P == 0, "rows of a gate");
+    TORCH_CHECK_VALUE(gate.numel() == 0 || ((rows == 0 || gate.numel() == rows / P * C) && gate.scalar_type() == x.scalar_type() && gate.device() == x.device() && gate.is_contiguous()),
+                      "gate must be contiguous, of x's type, and have an element for each of x or each of a sample's channels, got ", gate.scalar_type(), " ", gate.sizes(), " on ", gate.device());
+    numbers("post_gamma", post, C, x), numbers("pre_gamma", pre, C, x);
+    return {rows, C, type_code(x.scalar_type())};
+}
+
+std::tuple<Tensor, Tensor, Tensor> residual_norm_fwd(const Tensor &x, const Tensor &u, const Tensor &gate, const Tensor &post, const Tensor &pre, int64_t P, double scale, double epsilon,
+                                                     int64_t act, bool keep) {
+    const ResidualSizes s = residual_sizes(x, u, gate, post, pre, P);
+    const c10::DeviceGuard guard(x.device());
+    const bool update = u.sizes() == x.sizes();
+    Tensor y = update ? at::empty_like(x) : at::empty({0}, x.options()), h = at::empty_like(x), r = vector_like(keep ? (update ? 2 : 1) * s.rows : 0, x);
+    float *r_y = floats(r), *r_u = r_y && update ? r_y + s.rows : nullptr;
+    check(library().residual_norm_fwd(memory(x), memory(u), memory(gate), floats(post), floats(pre), memory(y), memory(h), r_u, r_y, s.rows, P, s.C, (float)scale, (float)epsilon, (int)act,
+                                      s.type, stream_of(x)),
+          "hgq_residual_norm_fwd");
+    return {y, h, r};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> residual_norm_bwd(const Tensor &dy, const Tensor &dh, const Tensor &x, const Tensor &u, const Tensor &gate, const Tensor &post, const Tensor &pre,
+                                                                     const Tensor &r, int64_t P, double scale, double epsilon, int64_t act, bool need_dx, bool need_du, bool need_dgate,
+                                                                     bool need_dpost, bool need_dpre) {
+    const ResidualSizes s = residual_sizes(x, u, gate, post, pre, P);
+    for (const Tensor *g : {&dy, &dh})
+        TORCH_CHECK_VALUE(g->numel() == 0 || (g->sizes() == x.sizes() && g->scalar_type() == x.scalar_type() && g->device() == x.device() && g->is_contiguous()), "gradients must be contiguous and like x");
+    const bool update = u.sizes() == x.sizes();
+    TORCH_CHECK_VALUE(r.numel() == (update ? 2 : 1) * s.rows && r.scalar_type() == at::kFloat && r.device() == x.device() && r.is_contiguous(), "r must be what the forward call left");
+    const c10::DeviceGuard guard(x.device());
+    const Tensor none = at::empty({0}, x.options());
+    Tensor dx = need_dx ? at::empty_like(x) : none, du = need_du && update ? at::empty_like(x) : none, dgate = !need_dgate ? none : s.rows ? at::empty_like(gate) : at::zeros_like(gate), dpost = vector_like(need_dpost ? s.C : 0, x),
+           dpre = vector_like(need_dpre ? s.C : 0, x);
+    const Workspace<float> ws(library().residual_norm_bwd_workspace(s.rows, P, s.C, s.type));
+    const float *r_y = floats(r), *r_u = r_y && update ? r_y + s.rows : nullptr;
+    check(lib.residual_norm_bwd(memory(dy), memory(dh), memory(x), memory(u), s.rows ? memory(gate) : nullptr, floats(post), floats(pre), r_u, r_y, memory(dx), memory(du), s.rows ? memory(dgate) : nullptr, floats(dpost), floats(dpre),
+                                ws.get(), s.rows, P, s.C, (float)scale, (float)epsilon, (int)act, s.type, stream_of(x)),
+          "hgq_residual_norm_bwd");
+    return {dx, du, dgate, dpost, dpre};
+}
+
+const auto &residual_op() {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::residual_norm_fwd", "").typed<decltype(residual_norm_fwd)>();
+    return op;
+}
+
+struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &u, const Tensor &gate, const Tensor &post, const Tensor &pre, int64_t P,
+                                                  double scale, double epsilon, int64_t act) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [y, h, r] = residual_op().call(x, u, gate, post, pre, P, scale, epsilon, act, true);
+        ctx->save_for_backward({x, u, gate, post, pre, r});
+        ctx->saved_data["P"] = P, ctx->saved_data["scale"] = scale, ctx->saved_data["epsilon"] = epsilon, ctx->saved_data["act"] = act;
+        ctx->set_materialize_grads(false);
+        if (u.sizes() != x.sizes()) return {h};
+        return {y, h};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::residual_norm_bwd", "").typed<decltype(residual_norm_bwd)>();
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0];
+        const bool update = grads.size() == 2;
+        torch::autograd::variable_list out(9);
+        const Tensor &gy = update ? grads[0] : Tensor(), &gh = grads[update ? 1 : 0];
+        if (!gy.defined() && !gh.defined()) return out;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            const Tensor none = at::empty({0}, x.options().requires_grad(false));
+            const auto given = [&](const Tensor &g) { return g.defined() ? plain(g.contiguous()) : none; };
+            const auto [dx, du, dgate, dpost, dpre] = op.call(given(gy), given(gh), x, saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["P"].toInt(),
+                                                              ctx->saved_data["scale"].toDouble(), ctx->saved_data["epsilon"].toDouble(), ctx->saved_data["act"].toInt(),
+                                                              ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3), ctx->needs_input_grad(4));
+            const Tensor *all[] = {&dx, &du, &dgate, &dpost, &dpre};
+            for (int k = 0; k < 5; ++k)
+                if (ctx->needs_input_grad(k)) out[k] = *all[k];
+        }
+        once_only(out, {gy, gh, saved[0], saved[1], saved[2], saved[3], saved[4]}, "residual_norm");
+        return out;
+    }
+};
+
+// {y, h}; without an update {h}
+std::vector<Tensor> residual_norm(const Tensor &x, const std::optional<Tensor> &u, const std::optional<Tensor> &gate, const std::optional<Tensor> &post, const std::optional<Tensor> &pre,
+                                  double scale, double epsilon, int64_t act) {
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must be [..., channels], got ", x.sizes());
+    const int64_t C = x.size(-1), rows = x.numel() / C;
+    for (const auto &[name, t] : {std::make_pair("post_gamma", &post), std::make_pair("pre_gamma", &pre)})
+        TORCH_CHECK_VALUE(!*t || ((*t)->dim() == 1 && (*t)->numel() == C), name, " must be a vector with an element per channel");
+    TORCH_CHECK_VALUE(!u || u->sizes() == x.sizes(), "update must be like x, got ", u->sizes(), " for ", x.sizes());
+    int64_t P = 1;
+    if (gate && gate->sizes() != x.sizes()) {
+        bool fits = gate->dim() >= 1 && gate->size(-1) == C;
+        if (gate->dim() == 1) {  // one row for all
+            P = rows;
+        } else {  // one for each sample
+            fits = fits && x.dim() >= 2 && gate->size(0) == x.size(0) && (gate->dim() == 2 || gate->dim() == x.dim());
+            for (int64_t d = 1; d + 1 < gate->dim() && fits; ++d) fits = gate->size(d) == 1;
+            P = x.dim() >= 2 && x.size(0) ? rows / x.size(0) : 1;
+        }
+        TORCH_CHECK_VALUE(fits, "gate must be like x, [batch, channels] or [channels], got ", gate->sizes(), " for ", x.sizes());
+        if (P < 1) P = 1;
+    }
+    std::vector<Tensor> inputs = {x};
+    const char *names[] = {"x", "update", "gate", "post_gamma", "pre_gamma"};
+    const std::optional<Tensor> *rest[] = {&u, &gate, &post, &pre};
+    bool graph = differentiated(x), missing = false;
+    for (const auto *t : rest) graph = graph || (*t && differentiated(**t)), missing = missing || !*t;
+    const Tensor none = missing ? at::empty({0}, x.options().dtype(at::kFloat).requires_grad(false)) : Tensor();
+    for (const auto *t : rest) inputs.push_back(*t ? **t : none);
+    if (graph)
+        for (int k = 0; k < 5; ++k) accumulates_here(names[k], inputs[k]);
+    for (Tensor &t : inputs) t = plain(t.contiguous());
+    if (graph) return ResidualNorm::apply(inputs[0], inputs[1], inputs[2], inputs[3], inputs[4], P, scale, epsilon, act);
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, h, r] = residual_op().call(inputs[0], inputs[1], inputs[2], inputs[3], inputs[4], P, scale, epsilon, act, false);
+    if (!u) return {h};
+    return {y, h};
+}
+
 // ---- the global norm -------------------------------------------------------------------------------------------------
 Tensor global_norm(at::TensorList tensors) {
     TORCH_CHECK_VALUE(!tensors.empty(), "at least one tensor is expected");
@@ -400,12 +797,26 @@ void bind(const py::dict &entries, const py::object &error) {
     lib.group_norm_fwd = (decltype(lib.group_norm_fwd))at("hgq_group_norm_fwd");
     lib.group_norm_bwd_workspace = (decltype(lib.group_norm_bwd_workspace))at("hgq_group_norm_bwd_workspace");
     lib.group_norm_bwd = (decltype(lib.group_norm_bwd))at("hgq_group_norm_bwd");
+    lib.distill_topk_workspace = (decltype(lib.distill_topk_workspace))at("hgq_distill_topk_workspace");
+    lib.distill_topk_fwd = (decltype(lib.distill_topk_fwd))at("hgq_distill_topk_fwd");
+    lib.distill_topk_bwd = (decltype(lib.distill_topk_bwd))at("hgq_distill_topk_bwd");
+    lib.relative_bias_fwd = (decltype(lib.relative_bias_fwd))at("hgq_relative_bias_fwd");
+    lib.relative_bias_bwd_workspace = (decltype(lib.relative_bias_bwd_workspace))at("hgq_relative_bias_bwd_workspace");
+    lib.relative_bias_bwd = (decltype(lib.relative_bias_bwd))at("hgq_relative_bias_bwd");
+    lib.residual_norm_fwd = (decltype(lib.residual_norm_fwd))at("hgq_residual_norm_fwd");
+    lib.residual_norm_bwd_workspace = (decltype(lib.residual_norm_bwd_workspace))at("hgq_residual_norm_bwd_workspace");
+    lib.residual_norm_bwd = (decltype(lib.residual_norm_bwd))at("hgq_residual_norm_bwd");
     bound = true;
 }
 
 Tensor tensor_of(const py::handle &h, const char *what) {
     TORCH_CHECK_TYPE(THPVariable_Check(h.ptr()), what, " must be a tensor, got ", py::str(py::type::of(h)).cast<std::string>());
     return THPVariable_Unpack(h.ptr());
+}
+
+std::optional<Tensor> tensor_or_none(const py::handle &h, const char *what) {
+    if (h.is_none()) return std::nullopt;
+    return tensor_of(h, what);
 }
 
 }  // namespace
@@ -415,6 +826,18 @@ TORCH_LIBRARY_FRAGMENT(hgq, m) {
     m.def("group_norm_bwd(Tensor dy, Tensor x, Tensor gamma, Tensor beta, Tensor stats, int groups, int act, bool need_dx, bool need_dgamma, bool need_dbeta) "
           "-> (Tensor, Tensor, Tensor)");
     m.def("global_norm(Tensor[] tensors) -> Tensor");
+    m.def("distill_topk_fwd(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor teacher_lse, Tensor sample_weight, float temperature, bool gradient) "
+          "-> (Tensor, Tensor, Tensor)");
+    m.def("distill_topk_bwd(Tensor upstream, Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor teacher_lse, Tensor sample_weight, Tensor stats, float temperature) "
+          "-> Tensor");
+    m.def("distill_topk_bwd_(Tensor upstream, Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor teacher_lse, Tensor sample_weight, Tensor stats, float temperature, "
+          "Tensor(a!) dlogits) -> ()");
+    m.def("relative_bias_fwd(Tensor scores, Tensor table, Tensor offsets, int offset, int[] first, bool both) -> Tensor");
+    m.def("relative_bias_bwd(Tensor dout, Tensor offsets, int offset, int[] first, bool both) -> Tensor");
+    m.def("residual_norm_fwd(Tensor x, Tensor update, Tensor gate, Tensor post_gamma, Tensor pre_gamma, int gate_rows, float scale, float epsilon, int act, bool keep) "
+          "-> (Tensor, Tensor, Tensor)");
+    m.def("residual_norm_bwd(Tensor dy, Tensor dh, Tensor x, Tensor update, Tensor gate, Tensor post_gamma, Tensor pre_gamma, Tensor r, int gate_rows, float scale, float epsilon, int act, "
+          "bool need_dx, bool need_dupdate, bool need_dgate, bool need_dpost, bool need_dpre) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 // (CPU tensors reach the checks, which say that there is no CPU implementation)
@@ -422,11 +845,25 @@ TORCH_LIBRARY_IMPL(hgq, CUDA, m) {
     m.impl("group_norm_fwd", group_norm_fwd);
     m.impl("group_norm_bwd", group_norm_bwd);
     m.impl("global_norm", global_norm);
+    m.impl("distill_topk_fwd", distill_topk_fwd);
+    m.impl("distill_topk_bwd", distill_topk_bwd);
+    m.impl("distill_topk_bwd_", distill_topk_bwd_);
+    m.impl("relative_bias_fwd", relative_bias_fwd);
+    m.impl("relative_bias_bwd", relative_bias_bwd);
+    m.impl("residual_norm_fwd", residual_norm_fwd);
+    m.impl("residual_norm_bwd", residual_norm_bwd);
 }
 TORCH_LIBRARY_IMPL(hgq, CPU, m) {
     m.impl("group_norm_fwd", group_norm_fwd);
     m.impl("group_norm_bwd", group_norm_bwd);
     m.impl("global_norm", global_norm);
+    m.impl("distill_topk_fwd", distill_topk_fwd);
+    m.impl("distill_topk_bwd", distill_topk_bwd);
+    m.impl("distill_topk_bwd_", distill_topk_bwd_);
+    m.impl("relative_bias_fwd", relative_bias_fwd);
+    m.impl("relative_bias_bwd", relative_bias_bwd);
+    m.impl("residual_norm_fwd", residual_norm_fwd);
+    m.impl("residual_norm_bwd", residual_norm_bwd);
 }
 
 PYBIND11_MODULE(_host, m) {
@@ -461,6 +898,44 @@ PYBIND11_MODULE(_host, m) {
             norm = op.call(list);
         }
         return py::reinterpret_steal<py::object>(THPVariable_Wrap(norm));
+        END_HANDLE_TH_ERRORS_PYBIND
+    });
+    m.def("distill_topk", [](const py::handle &logits, const py::handle &teacher, const py::handle &indices, double T, const py::handle &lse, const py::handle &weight) {
+        HANDLE_TH_ERRORS
+        const Tensor z = tensor_of(logits, "logits"), t = tensor_of(teacher, "teacher_logits"), i = tensor_of(indices, "teacher_indices");
+        const auto l = tensor_or_none(lse, "teacher_lse"), w = tensor_or_none(weight, "sample_weight");
+        Tensor loss;
+        {
+            const py::gil_scoped_release others;
+            loss = distill_topk(z, t, i, T, l, w);
+        }
+        return py::reinterpret_steal<py::object>(THPVariable_Wrap(loss));
+        END_HANDLE_TH_ERRORS_PYBIND
+    });
+    m.def("relative_bias", [](const py::handle &scores, const py::handle &table, const std::vector<int64_t> &first, bool both, int64_t offset, const py::handle &offsets) {
+        HANDLE_TH_ERRORS
+        const Tensor x = tensor_of(scores, "scores"), t = tensor_of(table, "table");
+        const auto o = tensor_or_none(offsets, "offset");
+        Tensor out;
+        {
+            const py::gil_scoped_release others;
+            out = relative_bias(x, t, first, both, offset, o);
+        }
+        return py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
+        END_HANDLE_TH_ERRORS_PYBIND
+    });
+    m.def("residual_norm", [](const py::handle &x, const py::handle &update, const py::handle &gate, const py::handle &post, const py::handle &pre, double scale, double epsilon, int64_t act) {
+        HANDLE_TH_ERRORS
+        const Tensor input = tensor_of(x, "x");
+        const auto u = tensor_or_none(update, "update"), g = tensor_or_none(gate, "gate"), po = tensor_or_none(post, "post_gamma"), pr = tensor_or_none(pre, "pre_gamma");
+        std::vector<Tensor> out;
+        {
+            const py::gil_scoped_release others;
+            out = residual_norm(input, u, g, po, pr, scale, epsilon, act);
+        }
+        py::tuple t(out.size());
+        for (size_t k = 0; k < out.size(); ++k) t[k] = py::reinterpret_steal<py::object>(THPVariable_Wrap(out[k]));
+        return py::object(t);
         END_HANDLE_TH_ERRORS_PYBIND
     });
     py::class_<AdamwVariables>(m, "AdamwVariables")

@@ -10,6 +10,7 @@ raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 import threading
 from array import array
@@ -20,7 +21,7 @@ from torch import Tensor
 
 from . import _lib
 
-__all__ = ['quantize', 'wrap_track_i_', 'qdense', 'dense_ebops', 'sparse_ce', 'sgd_update_', 'sgd_update_multi_', 'qsoftmax', 'conv2d', 'matmul_bias_act', 'col_moments', 'attn_scores', 'attn_combine', 'ATTN_MAX', 'pool2d', 'conv2d_ebops', 'conv_geometry', 'conv2d_ebops_supported', 'mse', 'dense_moments', 'dense_moments_supported', 'bn_fold', 'qbits', 'ebops_finish', 'qattention', 'qattention_supported', 'bits_ebops', 'gdense', 'gdense_supported', 'affine_rows', 'global_norm', 'adamw_update_multi_', 'adamw_state', 'adamw_moments', 'group_norm']
+__all__ = ['quantize', 'wrap_track_i_', 'qdense', 'dense_ebops', 'sparse_ce', 'sgd_update_', 'sgd_update_multi_', 'qsoftmax', 'conv2d', 'matmul_bias_act', 'col_moments', 'attn_scores', 'attn_combine', 'ATTN_MAX', 'pool2d', 'conv2d_ebops', 'conv_geometry', 'conv2d_ebops_supported', 'mse', 'dense_moments', 'dense_moments_supported', 'bn_fold', 'qbits', 'ebops_finish', 'qattention', 'qattention_supported', 'bits_ebops', 'gdense', 'gdense_supported', 'affine_rows', 'global_norm', 'adamw_update_multi_', 'adamw_state', 'adamw_moments', 'group_norm', 'distill_topk', 'relative_bias', 'relative_buckets', 'residual_norm', 'rms_norm']
 
 
 def _ptr(t: Tensor | None):
@@ -3556,7 +3557,7 @@ def adamw_update_multi_(ws, gs, moments, state, beta_1: float = 0.9, beta_2: flo
     touch_state()
 
 
-_lib.register_operators()  # `hgq::global_norm` and those of group normalisation, which are compiled
+_lib.register_operators()  # `hgq::global_norm`, group normalisation and those further down, which are compiled
 
 
 # ---- group normalisation
@@ -3573,6 +3574,90 @@ def group_norm(x: Tensor, groups: int, gamma: Tensor | None = None, beta: Tensor
         raise ValueError(f'activation must be one of linear, relu, silu; got {activation!r}')
     _need(epsilon >= 0, 'epsilon must not be negative')
     return _lib.native().group_norm(x, int(groups), gamma, beta, float(epsilon), GROUP_ACTIVATIONS[activation])
+
+
+# ---- distillation, relative position bias, norms around a residual sum
+def distill_topk(logits: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, temperature: float = 1.0, teacher_lse: Tensor | None = None,
+                 sample_weight: Tensor | None = None) -> Tensor:
+    """Mean loss of a student's ``logits`` ``[..., vocabulary]`` against the ``K`` largest logits that a teacher gave for the same rows:
+    ``teacher_logits`` and ``teacher_indices`` ``[..., K]`` (int32 or int64; K up to 1024).  With ``q = softmax(logits / T)`` a row's loss is
+    ``T^2 sum_k p_k (log p_k - log q[i_k])``, the divergence of the student from the teacher times the square of the ``temperature`` T, which keeps the
+    gradient's size.  ``p`` is the softmax over the list, or, with ``teacher_lse`` ``[...]`` (float32: the teacher's own ``logsumexp(logits / T)`` over
+    everything), its true probabilities; what both have outside the list is then one more entry, ``T^2 p' log(p' / q')``, which counts
+    nothing where the student has nothing there.
+
+    Entries whose index is not in ``0 .. vocabulary - 1`` (-1, say) are missing: lists may be of different lengths; an index that comes twice counts with both.
+    ``sample_weight`` ``[...]`` (float32) multiplies the rows' losses, and their sum is divided by the number of rows, as Keras does.  A row without
+    entries, or with the weight 0, has no loss and no gradient, whatever its logits hold; without rows the loss is 0.
+
+    Logits and teacher's logits are float32, bfloat16 or float16 GPU tensors; rows of a wider buffer (``buffer[:, :vocabulary]``) are read where they
+    lie.  Differentiable once, in the logits.  The gradient for an upstream gradient of one is written by the forward call, so ``loss.backward()``
+    costs no second pass; another upstream gradient (a factor on the loss) makes the backward pass form it anew."""
+    return _lib.native().distill_topk(logits, teacher_logits, teacher_indices, float(temperature), teacher_lse, sample_weight)
+
+
+@functools.lru_cache(maxsize=64)
+def relative_buckets(buckets: int, max_distance: int) -> tuple[int, ...]:
+    """The first distances of buckets 1 .. ``buckets`` - 1 of one direction.  Half of them, h = ``buckets // 2``, have one distance each; bucket b beyond begins
+    where ``h + log(n / h) / log(max_distance / h) (buckets - h)`` reaches b - decided in whole numbers, no logarithm is rounded."""
+    h = buckets // 2
+    _need(h >= 1, f'a direction needs at least two buckets, got {buckets}')
+    _need(h < max_distance <= 1 << 30, f'max_distance must lie above the {h} distances that have a bucket each, and not above 2^30; got {max_distance}')
+    first, width = list(range(1, h + 1)), buckets - h
+    for b in range(1, width):
+        lo, hi = h, max_distance  # (n / h)^width >= (max_distance / h)^b first holds in (lo, hi]
+        while hi - lo > 1:
+            n = (lo + hi) // 2
+            if n**width * h**b >= max_distance**b * h**width:
+                hi = n
+            else:
+                lo = n
+        first.append(hi)
+    return tuple(first)
+
+
+def relative_bias(scores: Tensor, table: Tensor, max_distance: int = 128, bidirectional: bool = True, offset: int | Tensor = 0) -> Tensor:
+    """Attention ``scores`` ``[batch, heads, queries, keys]`` (or without the batch; float32, bfloat16 or float16) plus a learned bias by relative
+    position: ``table[bucket(j - (i + offset)), head]`` with ``table`` ``[buckets, heads]`` in float32.  Near distances have a bucket each, farther ones share
+    buckets that grow with the logarithm of the distance up to ``max_distance``, beyond which all are one (:func:`relative_buckets`).
+    ``bidirectional``: half of the buckets are for keys behind the query's position (j > i + offset), else those count as distance 0.  ``offset``: the position of
+    the first query among the keys - a number, or an int32 / int64 tensor ``[batch]`` on the GPU, one for each sequence (single tokens
+    of sequences of different lengths).  At most 128 buckets.  Masked scores (-inf) stay what they are.  Differentiable once in scores and table."""
+    _need(isinstance(table, Tensor) and table.dim() == 2, 'table must be [buckets, heads]')
+    n = table.shape[0]
+    _need(n <= 128, f'at most 128 buckets, got {n}')
+    _need(not bidirectional or n % 2 == 0, f'both directions have as many buckets: an even number, got {n}')
+    first = relative_buckets(n // 2 if bidirectional else n, int(max_distance))
+    at, each = (0, offset) if isinstance(offset, Tensor) else (int(offset), None)
+    _need(-(1 << 62) < at < 1 << 62, 'offset is out of range')
+    return _lib.native().relative_bias(scores, table, first, bool(bidirectional), at, each)
+
+
+GATE_ACTIVATIONS = {None: 0, 'linear': 0, 'sigmoid': 1}
+
+
+def residual_norm(x: Tensor, update: Tensor, post_gamma: Tensor | None = None, pre_gamma: Tensor | None = None, gate: Tensor | None = None,
+                  gate_activation: str | None = None, scale: float = 1.0, epsilon: float = 1e-6) -> tuple[Tensor, Tensor]:
+    """What stands between two blocks of a network, in one pass: the norm of a block's output ``update`` (like ``x``), its ``gate`` and the residual sum
+    with its ``scale``, and the norm ahead of the next block.  Returns ``(y, h)``:
+
+        y = x + scale * act(gate) * norm(update) * post_gamma;    h = norm(y) * pre_gamma;    norm(v) = v / sqrt(mean(v^2) + epsilon)
+
+    over the trailing axis of ``x`` ``[..., channels]`` (float32, bfloat16 or float16; everything between is float32, h is formed of y before y is
+    rounded).  The gammas are float32 ``[channels]`` or ``None``.  ``gate`` (x's type): like ``x``, ``[batch, channels]`` for each sample's positions alike, or
+    ``[channels]``; ``gate_activation`` ``None`` / ``'linear'`` or ``'sigmoid'``.  Differentiable once in all of them."""
+    if gate_activation not in GATE_ACTIVATIONS:
+        raise ValueError(f'gate_activation must be one of linear, sigmoid; got {gate_activation!r}')
+    _need(epsilon >= 0, 'epsilon must not be negative')
+    _need(isinstance(update, Tensor), 'update must be a tensor like x')
+    return _lib.native().residual_norm(x, update, gate, post_gamma, pre_gamma, float(scale), float(epsilon), GATE_ACTIVATIONS[gate_activation])
+
+
+def rms_norm(x: Tensor, gamma: Tensor | None = None, epsilon: float = 1e-6) -> Tensor:
+    """``x / sqrt(mean(x^2) + epsilon) * gamma`` over the trailing axis (``keras.layers.RMSNormalization``): the norm ahead of a network's first block,
+    with the types and rules of :func:`residual_norm`."""
+    _need(epsilon >= 0, 'epsilon must not be negative')
+    return _lib.native().residual_norm(x, None, None, None, gamma, 1.0, float(epsilon), 0)[0]
 
 
 # ======================================================================================

@@ -1089,6 +1089,52 @@ int64_t hgq_group_norm_bwd_workspace(int64_t B, int64_t S, int C, int G, int typ
 int hgq_group_norm_bwd(const void *dy, const void *x, const float *gamma, const float *beta, const double *mean, const double *rstd, void *dx,
                        float *dgamma, float *dbeta, float *workspace, int64_t B, int64_t S, int C, int G, int act, int type, void *stream);
 
+/*
+ * Loss of a student's logits against a teacher's top logits (beside the Keras losses that the reference's users train with), row r of
+ * z [rows, V] against entries t [rows, K] at indices i [rows, K], temperature T > 0:
+ *     q = softmax(z / T);   p_k = softmax(t / T) over the list, or with lse [rows] exp(t_k / T - lse), lse = the teacher's log sum exp(t / T) over its whole vocabulary
+ *     loss = (1 / rows) sum_r weight_r T^2 (sum_k p_k log(p_k / q[i_k]) + p' log(p' / q'));   p' = max(0, 1 - sum p), q' outside the list (only with lse, and where q' > 0)
+ * z, dz: `type`, t: `t_type` (HGQ_TYPE_*), rows of z `z_stride` elements apart, all else contiguous; indices of 4 or 8 bytes, those that are not in 0 .. V - 1 are
+ * missing entries, one that comes twice counts with the sum of both.  lse, weight: NULL for none.  A row without entries, or with the weight 0, has no
+ * loss and the gradient 0 (1 / rows stays).  _fwd: loss [1]; stats [rows][4] and dz [rows, V], the gradient for an upstream gradient of one, NULL = not wanted.
+ * _bwd: dz for the upstream gradient upstream[0], from stats; holds_unit: dz is what _fwd left, and stays as it is where upstream[0] is 1.
+ * workspace: *_workspace(...) floats at a multiple of 8 bytes (-1: bad arguments).  K up to 1024, V up to 2^30.
+ */
+int64_t hgq_distill_topk_workspace(int64_t rows, int64_t V, int64_t K, int rest);
+int hgq_distill_topk_fwd(const void *z, int64_t z_stride, const void *t, int t_type, const void *index, int index_bytes, const float *lse, const float *weight,
+                         float *loss, float *stats, void *dz, float *workspace, int64_t rows, int64_t V, int64_t K, double T, int type, void *stream);
+int hgq_distill_topk_bwd(const void *z, int64_t z_stride, const void *t, int t_type, const void *index, int index_bytes, const float *lse, const float *weight,
+                         const float *upstream, const float *stats, void *dz, int holds_unit, int64_t rows, int64_t V, int64_t K, double T, int type, void *stream);
+
+/*
+ * Learned bias by relative position on attention scores [B, H, T, S] (beside the score contractions of src/hgq/layers/attn/mha.py):
+ *     out[b, h, i, j] = scores[b, h, i, j] + table[bucket(d), h],   d = j - (i + offset);   table [n, H] fp32, n = both ? 2 m : m <= 128
+ *     bucket(d) = how many of first[0 .. m - 2] (HOST memory, rising from 1 on) are <= |d| (both = 0: <= max(-d, 0)), plus m for d > 0 with both
+ *     dtable[k, h] = sum of dy over all positions of bucket k (the gradient of the scores is dy itself)
+ * scores, dy: batch and heads stride_b, stride_h elements apart, a head's T x S contiguous; out contiguous; both of `type` (HGQ_TYPE_*).  offset: a
+ * number, or offsets [B] of 4 or 8 bytes on the device.  Sums in an order that depends on the shape alone.  workspace: floats at a multiple of 8 bytes.
+ */
+int hgq_relative_bias_fwd(const void *scores, int64_t stride_b, int64_t stride_h, const float *table, void *out, int64_t B, int64_t H, int64_t T, int64_t S,
+                          const int *first, int m, int both, int64_t offset, const void *offsets, int offset_bytes, int type, void *stream);
+int64_t hgq_relative_bias_bwd_workspace(int64_t B, int64_t H, int64_t T, int64_t S, int m, int both);
+int hgq_relative_bias_bwd(const void *dy, int64_t stride_b, int64_t stride_h, float *dtable, float *workspace, int64_t B, int64_t H, int64_t T, int64_t S,
+                          const int *first, int m, int both, int64_t offset, const void *offsets, int offset_bytes, int type, void *stream);
+
+/*
+ * The norms around a residual sum (beside the reference's layers; src/hgq/layers/batch_normalization.py normalises over the batch instead), rows of C channels:
+ *     norm(v) = v / sqrt(mean(v^2) + eps);   y = x + scale act(gate) norm(u) post;   h = norm(y) pre
+ * x, u, gate, y, h and their gradients: `type` (HGQ_TYPE_*); post, pre [C] fp32 or NULL (1); act 0: none, 1: 1 / (1 + exp(-gate)).  u NULL: y = x (not written) and
+ * h = norm(x) pre.  gate [rows, C] (P = 1) or [rows / P, C], one row for P rows each; NULL: none.  r_u, r_y [rows]: written by _fwd (NULL: not wanted), read
+ * by _bwd.  _bwd: dy or dh may be NULL (zero); dx, du, dgate (like gate), dpost, dpre [C]: NULL = not wanted; sums over rows in an order that depends on the shape
+ * alone.  workspace: *_workspace(...) floats.
+ */
+int hgq_residual_norm_fwd(const void *x, const void *u, const void *gate, const float *post, const float *pre, void *y, void *h, float *r_u, float *r_y, int64_t rows,
+                          int64_t P, int64_t C, float scale, float eps, int act, int type, void *stream);
+int64_t hgq_residual_norm_bwd_workspace(int64_t rows, int64_t P, int64_t C, int type);
+int hgq_residual_norm_bwd(const void *dy, const void *dh, const void *x, const void *u, const void *gate, const float *post, const float *pre, const float *r_u,
+                          const float *r_y, void *dx, void *du, void *dgate, float *dpost, float *dpre, float *workspace, int64_t rows, int64_t P, int64_t C, float scale,
+                          float eps, int act, int type, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,183 @@
+"""Distillation, relative position bias and the norms around a residual sum: what is refused before any GPU is touched (CPU)."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from hgq2_amd import _lib, ops
+
+
+def _refused(rc, name, code=None):
+    assert rc == (_lib.ERR_ARG if code is None else code) and name in _lib.load().hgq_last_error(), rc
+
+
+def _distill(fwd=True, z=256, z_stride=9, t=256, t_type=0, index=256, index_bytes=4, loss=256, ws=256, up=256, stats=256, dz=256, rows=3, V=9, K=2, T=1.0, type=0):
+    """Calls that a check turns down: the addresses are never read."""
+    lib = _lib.load()
+    if fwd:
+        return lib.hgq_distill_topk_fwd(z, z_stride, t, t_type, index, index_bytes, None, None, loss, None, None, ws, rows, V, K, T, type, None)
+    return lib.hgq_distill_topk_bwd(z, z_stride, t, t_type, index, index_bytes, None, None, up, stats, dz, 0, rows, V, K, T, type, None)
+
+
+@pytest.mark.parametrize('kw', [dict(rows=-1), dict(V=0), dict(K=0), dict(T=0.0), dict(T=-1.0), dict(T=math.nan), dict(T=math.inf), dict(type=3), dict(t_type=-1), dict(index_bytes=2),
+                                dict(z=None), dict(t=None), dict(index=None), dict(z_stride=-9)])
+def test_distillation_entry_points(kw):
+    _refused(_distill(**kw), b'hgq_distill_topk_fwd')
+    _refused(_distill(fwd=False, **kw), b'hgq_distill_topk_bwd')
+
+
+def test_distillation_limits():
+    _refused(_distill(loss=None), b'null')
+    _refused(_distill(ws=None), b'null')
+    for k in ('up', 'stats', 'dz'):
+        _refused(_distill(fwd=False, **{k: None}), b'null')
+    for kw in (dict(K=1025), dict(V=(1 << 30) + 1), dict(rows=1 << 41)):
+        _refused(_distill(**kw), b'hgq_distill_topk_fwd', _lib.ERR_UNSUPPORTED)
+        _refused(_distill(fwd=False, **kw), b'hgq_distill_topk_bwd', _lib.ERR_UNSUPPORTED)
+        assert _lib.load().hgq_distill_topk_workspace(kw.get('rows', 3), kw.get('V', 9), kw.get('K', 2), 0) == -1
+    assert _distill(fwd=False, rows=0, z=None) == 0
+
+
+@pytest.mark.parametrize('rows,V,K', [(1, 5, 5), (16384, 5, 5), (7, 64, 65), (1, 32000, 64), (300, 32000, 64), (2, 300000, 1000), (4096, 131072, 100), (4096, 1 << 20, 100)])
+def test_distillation_workspace(rows, V, K):
+    """A sum for each workgroup, and two numbers for each part of a row where rows are cut: never more than a small part of the logits."""
+    for rest in (0, 1):
+        n = _lib.load().hgq_distill_topk_workspace(rows, V, K, rest)
+        assert 2 <= n <= 2 * rows + max(2 * rows * V // 4096, 0) + 2 * rows
+
+
+def _bias(fwd=True, x=256, table=256, out=256, ws=256, B=2, H=2, T=3, S=4, first=(1, 2, 5), m=None, both=1, offset_bytes=8, type=0):
+    lib, n = _lib.load(), len(first) + 1 if m is None else m
+    first = (ctypes.c_int * max(1, len(first)))(*first) if first is not None else None
+    if fwd:
+        return lib.hgq_relative_bias_fwd(x, 24, 12, table, out, B, H, T, S, first, n, both, 0, None, offset_bytes, type, None)
+    return lib.hgq_relative_bias_bwd(x, 24, 12, table, ws, B, H, T, S, first, n, both, 0, None, offset_bytes, type, None)
+
+
+@pytest.mark.parametrize('kw', [dict(B=-1), dict(H=-1), dict(T=-1), dict(S=-1), dict(type=3), dict(offset_bytes=2), dict(first=(0, 2)), dict(first=(3, 2)), dict(first=(1, (1 << 30) + 1)),
+                                dict(first=(), m=1), dict(x=None), dict(table=None)])
+def test_bias_entry_points(kw):
+    _refused(_bias(**kw), b'hgq_relative_bias_fwd')
+    _refused(_bias(fwd=False, **kw), b'hgq_relative_bias_bwd')
+
+
+def test_bias_limits():
+    for kw in (dict(first=tuple(range(1, 65))), dict(first=tuple(range(1, 129)), both=0), dict(T=1 << 16, S=1 << 16), dict(B=1 << 31), dict(H=1 << 21)):
+        _refused(_bias(**kw), b'hgq_relative_bias_fwd', _lib.ERR_UNSUPPORTED)
+        _refused(_bias(fwd=False, **kw), b'hgq_relative_bias_bwd', _lib.ERR_UNSUPPORTED)
+    _refused(_bias(out=None), b'null')
+    _refused(_bias(fwd=False, ws=None), b'null')
+    assert _bias(B=0, x=None) == _bias(S=0, x=None) == _bias(fwd=False, H=0, x=None) == 0
+    assert _lib.load().hgq_relative_bias_bwd_workspace(2, 2, 3, 4, 65, 1) == _lib.load().hgq_relative_bias_bwd_workspace(2, 2, -3, 4, 4, 1) == -1
+
+
+def _residual(fwd=True, x=256, u=256, gate=None, y=256, h=256, dy=256, dh=256, r_u=256, r_y=256, ws=256, rows=6, P=1, C=8, scale=1.0, eps=1e-6, act=0, type=0, du=256, dgate=None, dpost=256):
+    lib = _lib.load()
+    if fwd:
+        return lib.hgq_residual_norm_fwd(x, u, gate, None, None, y, h, r_u, r_y, rows, P, C, scale, eps, act, type, None)
+    return lib.hgq_residual_norm_bwd(dy, dh, x, u, gate, None, None, r_u, r_y, 256, du, dgate, dpost, 256, ws, rows, P, C, scale, eps, act, type, None)
+
+
+@pytest.mark.parametrize('kw', [dict(rows=-1), dict(P=0), dict(P=4), dict(C=0), dict(eps=-1.0), dict(eps=math.nan), dict(scale=math.nan), dict(act=2), dict(act=-1), dict(type=3), dict(x=None),
+                                dict(u=None, gate=256)])
+def test_residual_entry_points(kw):
+    _refused(_residual(**kw), b'hgq_residual_norm_fwd')
+    _refused(_residual(fwd=False, **kw), b'hgq_residual_norm_bwd')
+
+
+def test_residual_limits():
+    for kw in (dict(h=None), dict(y=None)):
+        _refused(_residual(**kw), b'null')
+    for kw in (dict(r_u=None), dict(r_y=None), dict(dy=None, dh=None), dict(ws=None), dict(dgate=256), dict(u=None), dict(u=None, du=None)):
+        _refused(_residual(fwd=False, **kw), b'null')
+    for kw in (dict(C=(1 << 28) + 1), dict(rows=1 << 41)):
+        _refused(_residual(**kw), b'hgq_residual_norm_fwd', _lib.ERR_UNSUPPORTED)
+        _refused(_residual(fwd=False, **kw), b'hgq_residual_norm_bwd', _lib.ERR_UNSUPPORTED)
+    assert _residual(rows=0, x=None) == 0
+    assert _lib.load().hgq_residual_norm_bwd_workspace(6, 4, 8, 0) == -1 and _lib.load().hgq_residual_norm_bwd_workspace(0, 1, 8, 0) == 0
+
+
+def test_python_refusals():
+    z, i = torch.zeros(3, 7), torch.zeros(3, 2, dtype=torch.long)
+    with pytest.raises(ValueError, match='GPU'):
+        ops.distill_topk(z, z[:, :2], i)
+    with pytest.raises(ValueError, match='leading axes'):
+        ops.distill_topk(z, z[:2, :2], i)
+    with pytest.raises(ValueError, match='teacher_indices'):
+        ops.distill_topk(z, z[:, :2], i[:, :1])
+    with pytest.raises(ValueError, match='teacher_lse'):
+        ops.distill_topk(z, z[:, :2], i, teacher_lse=z)
+    with pytest.raises(ValueError, match='sample_weight'):
+        ops.distill_topk(z, z[:, :2], i, sample_weight=z[:2, 0])
+    with pytest.raises(ValueError, match='detach'):
+        ops.distill_topk(z, z[:, :2].clone().requires_grad_(True), i)
+    with pytest.raises(TypeError, match='tensor'):
+        ops.distill_topk(3.0, z, i)
+
+    s, t = torch.zeros(1, 2, 3, 4), torch.zeros(4, 2)
+    with pytest.raises(ValueError, match='GPU'):
+        ops.relative_bias(s, t, 9)
+    with pytest.raises(ValueError, match='scores'):
+        ops.relative_bias(s[0, 0], t, 9)
+    with pytest.raises(ValueError, match='buckets, heads'):
+        ops.relative_bias(s, t[0], 9)
+    with pytest.raises(ValueError, match='even'):
+        ops.relative_bias(s, t[:3], 9)
+    with pytest.raises(ValueError, match='at most 128'):
+        ops.relative_bias(s, torch.zeros(130, 2))
+    with pytest.raises(ValueError, match='max_distance'):
+        ops.relative_bias(s, torch.zeros(32, 2), 8)
+    with pytest.raises(ValueError, match='max_distance'):
+        ops.relative_bias(s, t, (1 << 30) + 1)
+    with pytest.raises(ValueError, match='two buckets'):
+        ops.relative_bias(s, t[:2], 9)
+
+    x = torch.zeros(2, 3, 8)
+    with pytest.raises(ValueError, match='GPU'):
+        ops.residual_norm(x, x)
+    with pytest.raises(ValueError, match='GPU'):
+        ops.rms_norm(x)
+    with pytest.raises(ValueError, match='gate_activation'):
+        ops.residual_norm(x, x, gate=x, gate_activation='tanh')
+    with pytest.raises(ValueError, match='negative'):
+        ops.rms_norm(x, epsilon=-1.0)
+    with pytest.raises(ValueError, match='update'):
+        ops.residual_norm(x, x[0])
+    with pytest.raises(ValueError, match='update'):
+        ops.residual_norm(x, None)
+    with pytest.raises(ValueError, match='post_gamma'):
+        ops.residual_norm(x, x, post_gamma=x[0, 0, :3])
+    for gate in (x[0], x[:1, 0], x[:, :2], x[..., :4]):
+        with pytest.raises(ValueError, match='gate'):
+            ops.residual_norm(x, x, gate=gate)
+
+
+@pytest.mark.parametrize('n,far', [(2, 2), (2, 100), (3, 9), (8, 40), (16, 128), (32, 128), (32, 33), (64, 500), (20, 1 << 30)])
+def test_first_distances(n, far):
+    """The definition bucket by bucket, in whole numbers: the bucket of a distance is how many first distances are not above it."""
+    first, h = ops.relative_buckets(n, far), n // 2
+    assert len(first) == n - 1 and list(first) == sorted(first) and first[-1] <= far and list(first[:h]) == list(range(1, h + 1))
+    for b, f in enumerate(first[h:], h + 1):
+        reached = lambda k: k**(n - h) * h**(b - h) >= far**(b - h) * h**(n - h)  # noqa: E731
+        assert reached(f) and not reached(f - 1)
+
+
+def test_registered_for_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        z, i = torch.empty(3, 9, device='cuda'), torch.empty(3, 2, dtype=torch.long, device='cuda')
+        none = torch.empty(0, device='cuda')
+        loss, stats, dz = torch.ops.hgq.distill_topk_fwd(z, z[:, :2], i, none, none, 1.0, True)
+        assert loss.shape == () and stats.shape == (3, 4) and dz.shape == z.shape
+        assert torch.ops.hgq.distill_topk_bwd(loss, z, z[:, :2], i, none, none, stats, 1.0).shape == z.shape
+        s, t = torch.empty(2, 4, 5, 6, device='cuda'), torch.empty(8, 4, device='cuda')
+        assert torch.ops.hgq.relative_bias_fwd(s, t, none, 0, [1, 2, 5], True).shape == s.shape
+        assert torch.ops.hgq.relative_bias_bwd(s, none, 0, [1, 2, 5], True).shape == t.shape
+        x = torch.empty(2, 3, 8, device='cuda')
+        y, h, r = torch.ops.hgq.residual_norm_fwd(x, x, none, none, none, 1, 1.0, 1e-6, 0, True)
+        assert y.shape == h.shape == x.shape and r.shape == (12,)
+        got = torch.ops.hgq.residual_norm_bwd(x, none, x, x, none, none, none, r, 1, 1.0, 1e-6, 0, True, True, False, True, False)
+        assert [tuple(g.shape) for g in got] == [(2, 3, 8), (2, 3, 8), (0,), (8,), (0,)]
