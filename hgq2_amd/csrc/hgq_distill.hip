@@ -57,6 +57,20 @@ __device__ __forceinline__ float exp_t(float d, float k_hi, float k_lo) {
     return fmaf(e, lo * HGQ_LN2, e);
 }
 
+// exp(x) and log(x) of numbers in 64 bits with an error of fp32's rounding: what is large of them - whole powers of two - stays in 64 bits.  (The
+// library's take some hundred instructions in 64 bits, for each row more than the row's own where the vocabulary is small.)
+__device__ __forceinline__ double exp_64(double x) {
+    const double two = x * 1.4426950408889634074, whole = __builtin_rint(two);
+    if (!(two > -1000.0)) return two != two ? two : 0.0;
+    return ldexp((double)__builtin_amdgcn_exp2f((float)(two - whole)), (int)fmin(whole, 1100.0));
+}
+
+__device__ __forceinline__ double log_64(double x) {
+    int e;
+    const float f = (float)frexp(x, &e);  // [0.5, 1)
+    return x > 0.0 && x < INFINITY ? (double)e * 0.69314718055994530942 + (double)(__builtin_amdgcn_logf(f) * 0.69314718f) : x == 0.0 ? (double)-INFINITY : x < 0.0 ? (double)__builtin_nanf("") : x;
+}
+
 // a maximum and the sum of exp((z - maximum) / T)
 struct MaxSum {
     float m, s;
@@ -64,10 +78,25 @@ struct MaxSum {
 
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
+// What is added up over a row: the pass, the list's entries (each once), and the teacher's p and p (log p - z / T).
+struct RowSums {
+    MaxSum pass, list;
+    double p, a;
+};
+
+__device__ __forceinline__ MaxSum team_join(MaxSum v, int width, float k) {
+    const float m = team_max(v.m, width);
+    return {m, team_sum(v.s * __builtin_amdgcn_exp2f((base_of(v.m) - base_of(m)) * k), width)};
+}
+
+__device__ __forceinline__ RowSums team_join(const RowSums &v, int width, float k) {
+    return {team_join(v.pass, width, k), team_join(v.list, width, k), team_sum(v.p, width), team_sum(v.a, width)};
+}
+
 template <int TPR>
 struct Team {  // the threads of one row
     static constexpr int WAVES = TPR > 64 ? TPR / 64 : 1;
-    double *lds;  // WAVES numbers
+    RowSums *lds;  // one for each wavefront
     __device__ __forceinline__ void sync() const {
         if (TPR > 64) {
             __syncthreads();
@@ -76,54 +105,66 @@ struct Team {  // the threads of one row
             __builtin_amdgcn_wave_barrier();
         }
     }
-    template <typename V>
-    __device__ __forceinline__ V sum(V v) const {
-        v = team_sum(v, TPR < 64 ? TPR : 64);
-        if (TPR <= 64) return v;
-        V *at = (V *)lds;
-        if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = team_sum(at[threadIdx.x & (WAVES - 1)], WAVES);
-        __syncthreads();
-        return v;
-    }
     __device__ __forceinline__ float max(float v) const {
         v = team_max(v, TPR < 64 ? TPR : 64);
         if (TPR <= 64) return v;
-        float *at = (float *)lds;
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6].pass.m = v;
+        __syncthreads();
+        return team_max(lds[threadIdx.x & (WAVES - 1)].pass.m, WAVES);
+    }
+    template <typename V>
+    __device__ __forceinline__ V join(V v, float k) const {
+        v = team_join(v, TPR < 64 ? TPR : 64, k);
+        if (TPR <= 64) return v;
+        __syncthreads();  // (max's)
+        V *at = (V *)lds;
         if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = team_max(at[threadIdx.x & (WAVES - 1)], WAVES);
-        __syncthreads();
-        return v;
-    }
-    __device__ __forceinline__ MaxSum join(MaxSum v, float k) const {
-        const float m = max(v.m);
-        return {m, sum(v.s * __builtin_amdgcn_exp2f((base_of(v.m) - base_of(m)) * k))};
+        return team_join(at[threadIdx.x & (WAVES - 1)], WAVES, k);
     }
 };
 
-// z[at ...] with -inf behind `end` and, BITS, where an entry is listed (bits: of the entries from `lo` on)
-template <typename T, bool BITS>
-__device__ __forceinline__ Vec<T> distill_load(const T *z, int at, int end, const uint32_t *bits, int lo) {
-    constexpr int N = Vec<T>::N;
-    const T none = (T)-INFINITY;
-    Vec<T> r;
-    if (at + N <= end) {
-        r = load_vec(z + at);
-    } else {
-        r = load_part(z + at, end - at, none);
+// One access of a row: elements `own` .. of z[at ...] are its own, the first ones may be another thread's once more - a row's last access ends with the row, so
+// that no access is cut (one that may be whole or cut is taken apart where it arrives, and waited for there).  Rows that are shorter than an access
+// (teams of eight) are filled with -inf.
+template <typename T, int TPR>
+struct Piece {
+    static constexpr int N = Vec<T>::N;
+    int at, own;
+    __device__ __forceinline__ Piece(int wanted, int end) {
+        at = TPR > 8 ? min(wanted, end - N) : wanted;
+        own = min(N, wanted - at);
     }
-    if (BITS) {
-        const uint32_t b = at < end ? bits[(at - lo) >> 5] >> ((at - lo) & 31) & ((1 << N) - 1) : 0;
+    __device__ __forceinline__ Vec<T> load(const T *z, int end) const {
+        if (TPR > 8) return load_vec(z + at);
+        return at + N <= end ? load_vec(z + at) : load_part(z + at, end - at, (T)-INFINITY);
+    }
+    // -inf where an entry is listed (bits: of the entries from `lo` on)
+    __device__ __forceinline__ void leave_listed(Vec<T> &r, const uint32_t *bits, int lo, int end) const {
+        if (own == N || at >= end) return;
+        const int first = at - lo;
+        uint32_t b = 0;
+        if (own == 0) {
+            b = bits[first >> 5] >> (first & 31) & ((1 << N) - 1);
+        } else {
+            for (int e = own; e < N; ++e) b |= (bits[(first + e) >> 5] >> ((first + e) & 31) & 1) << e;
+        }
         if (b) {
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (b >> e & 1) r.v[e] = none;
+                if (b >> e & 1) r.v[e] = (T)-INFINITY;
         }
     }
-    return r;
-}
+    __device__ __forceinline__ void store(T *z, const Vec<T> &r, int end) const {
+        if (own == 0 && at + N <= end) {
+            store_vec<T, true>(z + at, r);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (e >= own && at + e < end) z[at + e] = r.v[e];
+        }
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ float most_of(const Vec<T> &r) {
@@ -134,11 +175,16 @@ __device__ __forceinline__ float most_of(const Vec<T> &r) {
 }
 
 template <typename T>
-__device__ __forceinline__ float exp_sum(const Vec<T> &r, float base, const DistillRows &a) {
+__device__ __forceinline__ float exp_sum(const Vec<T> &r, int own, float base, const DistillRows &a) {
     constexpr int N = Vec<T>::N;
     float e[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) e[k] = exp_t<sizeof(T) == 4>((float)r.v[k] - base, a.k_hi, a.k_lo);
+    if (own) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < own) e[k] = 0.0f;
+    }
 #pragma unroll
     for (int w = N / 2; w; w /= 2)
 #pragma unroll
@@ -146,16 +192,29 @@ __device__ __forceinline__ float exp_sum(const Vec<T> &r, float base, const Dist
     return e[0];
 }
 
+constexpr int AHEAD = 4;  // accesses of a thread in flight
+
 // maximum and sum over z[lo, end) as the row is read once: the sum follows the maximum
 template <typename T, int TPR, bool BITS>
 __device__ __forceinline__ MaxSum distill_stream(const T *z, int lo, int end, const uint32_t *bits, int lane, const DistillRows &a) {
     constexpr int N = Vec<T>::N;
     MaxSum r = {-INFINITY, 0.0f};
-    for (int at = lo + lane * N; at < end; at += TPR * N) {
-        const Vec<T> v = distill_load<T, BITS>(z, at, end, bits, lo);
-        const float m = most_of(v);
+    for (int at = lo + lane * N; at < end; at += AHEAD * TPR * N) {
+        Vec<T> v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) v[k] = Piece<T, TPR>(at + k * TPR * N, end).load(z, end);
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (BITS) Piece<T, TPR>(at + k * TPR * N, end).leave_listed(v[k], bits, lo, end);
+            m = fmaxf(m, most_of(v[k]));
+        }
         if (m > r.m) r.s *= __builtin_amdgcn_exp2f((r.m - m) * a.k_hi), r.m = m;
-        r.s += exp_sum(v, base_of(r.m), a);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const Piece<T, TPR> p(at + k * TPR * N, end);
+            if (p.own < N) r.s += exp_sum(v[k], p.own, base_of(r.m), a);
+        }
     }
     return r;
 }
@@ -174,7 +233,7 @@ __device__ __forceinline__ void distill_bits(uint32_t *bits, int lo, int end, co
 // Maximum and sum of part `blockIdx % n_parts` of a row.
 template <typename T, bool REST>
 __global__ __launch_bounds__(256) void distill_parts(const DistillRows a) {
-    __shared__ double lds[4];
+    __shared__ RowSums lds[4];
     extern __shared__ uint32_t distill_lds[];
     const Team<256> team = {lds};
     const int64_t row = blockIdx.x / a.n_parts;
@@ -198,7 +257,7 @@ template <typename T, int TPR, bool REST, int FROM, int HOLD>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const DistillRows a) {
     constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR, N = Vec<T>::N, NV = HOLD ? HOLD / N : 1;
     constexpr bool FINE = sizeof(T) == 4;
-    __shared__ double lds[THREADS / 64];
+    __shared__ RowSums lds[THREADS / 64];
     extern __shared__ uint32_t distill_lds[];
     if (FROM == FROM_STATS && a.leave_unit && *a.upstream == 1.0f) return;  // dz holds this gradient
 
@@ -206,11 +265,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const Dist
     const Team<TPR> team = {lds};
     const int64_t block = FROM == FROM_ROW ? blockIdx.x : blockIdx.x / a.grid_parts, row = block * ROWS + slot;
     const int lo = FROM == FROM_ROW ? 0 : (int)(blockIdx.x - block * a.grid_parts) * a.part, end = FROM == FROM_ROW ? a.V : min(a.V, lo + a.part);
-    const int words = REST && FROM == FROM_ROW ? bit_words(a.V) : 0;
-    double *p = (double *)((char *)distill_lds + slot * (DISTILL_ENTRY * a.K + 4 * words));  // (first the teacher's logits)
-    int *index = (int *)(p + a.K);
-    float *z_list = (float *)(index + a.K);
-    uint32_t *bits = (uint32_t *)(z_list + a.K);
+    const int words = REST && FROM == FROM_ROW ? bit_words(a.V) : 0, lists = (a.K + 3) & ~3;
+    double *p = (double *)((char *)distill_lds + slot * (DISTILL_ENTRY * lists + 4 * words));  // (first the teacher's logits)
+    int *index = (int *)(p + lists);
+    float *z_list = (float *)(index + lists);
+    uint32_t *bits = (uint32_t *)(z_list + lists);
 
     double loss = 0;
     if (row < a.rows) {
@@ -219,67 +278,79 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const Dist
         const double inv_T = 1.0 / a.T;
         const float weight = a.weight ? a.weight[row] : 1.0f;
 
-        // the list
-        float t_most = -INFINITY;
-        for (int k = lane; k < a.K; k += TPR) {
-            const int i = distill_index(a, row * a.K + k);
+        // the list; a thread's first logit is not waited for before the pass
+        float t_most = -INFINITY, z_first = -INFINITY;
+        for (int k = lane; k < lists; k += TPR) {
+            const int i = k < a.K ? distill_index(a, row * a.K + k) : -1;
             const float t = i < 0 ? -INFINITY : distill_logit(a, row * a.K + k);
-            index[k] = i, p[k] = t, z_list[k] = i < 0 ? -INFINITY : (float)z[i];
+            index[k] = i, p[k] = t;
+            if (k == lane && i >= 0) z_first = (float)z[i];
             if (t > t_most || t != t) t_most = t != t ? INFINITY : t;
         }
+        const double lse = REST ? (double)a.lse[row] : 0.0;
         t_most = team.max(t_most);
-        team.sync();
         if (!(t_most > -INFINITY) || weight == 0.0f) {  // no entries, or no weight: no loss, no gradient
-            if (dz)
-                for (int at = lo + lane * N; at < end; at += TPR * N) {
-                    Vec<T> zero;
+            if (dz) {
+                Vec<T> zero;
 #pragma unroll
-                    for (int e = 0; e < N; ++e) zero.v[e] = (T)0.0f;
-                    if (at + N <= end) store_vec(dz + at, zero);
-                    else store_part(dz + at, zero, end - at);
-                }
+                for (int e = 0; e < N; ++e) zero.v[e] = (T)0.0f;
+                for (int at = lo + lane * N; at < end; at += TPR * N) Piece<T, TPR>(at, end).store(dz, zero, end);
+            }
         } else {
-            // maximum and sum of the row
+            RowSums sums = {{-INFINITY, 0.0f}, {-INFINITY, 0.0f}, 0.0, 0.0};
+            MaxSum &r = sums.pass;
             Vec<T> held[NV];
-            MaxSum r = {-INFINITY, 0.0f};
             if (FROM == FROM_PARTS) {
                 for (int c = lane; c < a.n_parts; c += TPR) {
                     const float2 q = a.parts[row * a.n_parts + c];
                     if (q.x > r.m) r.s *= __builtin_amdgcn_exp2f((r.m - q.x) * a.k_hi), r.m = q.x;
                     r.s += q.y * __builtin_amdgcn_exp2f((base_of(q.x) - base_of(r.m)) * a.k_hi);
                 }
-                r = team.join(r, a.k_hi);
             }
             if (FROM == FROM_ROW) {
                 if (REST) distill_bits<T>(bits, 0, a.V, index, a.K, lane, team);
                 if (HOLD) {
 #pragma unroll
                     for (int v = 0; v < NV; ++v)
-                        if (v * TPR * N < a.V) held[v] = distill_load<T, REST>(z, (v * TPR + lane) * N, a.V, bits, 0);
+                        if (v * TPR * N < a.V) held[v] = Piece<T, TPR>((v * TPR + lane) * N, a.V).load(z, a.V);
 #pragma unroll
                     for (int v = 0; v < NV; ++v)
-                        if (v * TPR * N < a.V) r.m = fmaxf(r.m, most_of(held[v]));
-                    r.m = team.max(r.m);
+                        if (v * TPR * N < a.V) {
+                            if (REST) Piece<T, TPR>((v * TPR + lane) * N, a.V).leave_listed(held[v], bits, 0, a.V);
+                            r.m = fmaxf(r.m, most_of(held[v]));
+                        }
 #pragma unroll
                     for (int v = 0; v < NV; ++v)
-                        if (v * TPR * N < a.V) r.s += exp_sum(held[v], base_of(r.m), a);
-                    r.s = team.sum(r.s);
+                        if (v * TPR * N < a.V) r.s += exp_sum(held[v], Piece<T, TPR>((v * TPR + lane) * N, a.V).own, base_of(r.m), a);
                 } else {
-                    r = team.join(distill_stream<T, TPR, REST>(z, 0, a.V, bits, lane, a), a.k_hi);
+                    r = distill_stream<T, TPR, REST>(z, 0, a.V, bits, lane, a);
                 }
             }
+            team.sync();
 
-            // the teacher
-            double log_sum = 0, p_sum = 0, p_rest = 0;
-            if (REST) {
-                log_sum = a.lse[row];
-                for (int k = lane; k < a.K; k += TPR) p_sum += exp(p[k] * inv_T - log_sum);
-                p_sum = team.sum(p_sum);
-            } else {
-                for (int k = lane; k < a.K; k += TPR) p_sum += exp_t<true>((float)p[k] - t_most, a.k_hi, a.k_lo);
-                p_sum = team.sum(p_sum);
-                log_sum = log(p_sum) + (double)t_most * inv_T;
+            // the list: p without its sum (without the teacher's lse), logarithms, and the logits
+            for (int k = lane; k < a.K; k += TPR) {
+                const int i = index[k];
+                const float zk = k == lane ? z_first : i < 0 ? -INFINITY : (float)z[i];
+                const double log_p = REST ? p[k] * inv_T - lse : (p[k] - t_most) * inv_T;
+                const double q = i < 0 ? 0.0 : REST ? exp_64(log_p) : (double)exp_t<true>((float)p[k] - t_most, a.k_hi, a.k_lo);
+                z_list[k] = zk, p[k] = q;
+                sums.p += q;
+                if (q != 0) sums.a += q * (log_p - zk * inv_T);
+                if (REST && FROM != FROM_STATS) {
+                    int before = 0;
+#pragma unroll 4
+                    for (int l = 0; l < lists; l += 4) {
+                        const int4 four = *(const int4 *)(index + l);
+                        before += (four.x == i && l < k) + (four.y == i && l + 1 < k) + (four.z == i && l + 2 < k) + (four.w == i && l + 3 < k);
+                    }
+                    if (i >= 0 && !before) {
+                        if (zk > sums.list.m) sums.list.s *= exp_t<true>(sums.list.m - zk, a.k_hi, a.k_lo), sums.list.m = zk;
+                        sums.list.s += exp_t<true>(zk - base_of(sums.list.m), a.k_hi, a.k_lo);
+                    }
+                }
             }
+            sums = team.join(sums, a.k_hi);
 
             // m, a of the pass and M, b of the list
             float m, pass, M, list;
@@ -287,73 +358,73 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const Dist
                 const float4 s = a.stats[row];
                 m = s.x, pass = s.y, M = s.z, list = s.w;
             } else {
-                m = base_of(r.m);
-                float most = r.m;
-                double total = r.s;
-                if (REST) {  // the whole row: with the list's entries, each once
-                    for (int k = lane; k < a.K; k += TPR) most = fmaxf(most, z_list[k]);
-                    most = team.max(most);
-                    double s = 0;
-                    for (int k = lane; k < a.K; k += TPR) {
-                        const int i = index[k];
-                        bool first = i >= 0;
-                        for (int l = 0; l < k; ++l) first &= index[l] != i;
-                        if (first) s += exp_t<true>(z_list[k] - most, a.k_hi, a.k_lo);
-                    }
-                    const double outside = r.s > 0.0f ? (double)r.s * exp(((double)r.m - most) * inv_T) : (double)r.s;
-                    total = team.sum(s) + outside;
-                    if (r.s > 0.0f) p_rest = fmax(0.0, 1.0 - p_sum);
-                    if (lane == 0 && p_rest > 0) loss = p_rest * (log(p_rest) - (log((double)r.s) + ((double)r.m - most) * inv_T - log(total)));
-                    pass = r.s == 0.0f ? 0.0f : (float)((p_sum + p_rest) * (outside / r.s) / total - p_rest / r.s);
-                    list = (float)((p_sum + p_rest) / total);
+                const float most = REST ? fmaxf(r.m, sums.list.m) : r.m;
+                m = base_of(r.m), M = base_of(most);
+                float total = r.s, p_rest = 0;
+                if (REST) {
+                    // (a side that has nothing has no maximum either)
+                    const float down = r.s == 0.0f ? 0.0f : exp_t<true>(m - M, a.k_hi, a.k_lo);
+                    total = r.s * down + (sums.list.s == 0.0f ? 0.0f : sums.list.s * exp_t<true>(sums.list.m - M, a.k_hi, a.k_lo));
+                    if (r.s > 0.0f) p_rest = (float)fmax(0.0, 1.0 - sums.p);
+                    const float P = (float)sums.p + p_rest;
+                    pass = r.s == 0.0f ? 0.0f : P * down / total - p_rest / r.s;
+                    list = P / total;
                 } else {
-                    pass = list = (float)(1.0 / total);
+                    pass = list = 1.0f / total;
                 }
-                M = base_of(most);
-                const double log_total = log(total);
-                for (int k = lane; k < a.K; k += TPR) {
-                    const double log_p = p[k] * inv_T - log_sum, q = REST ? exp(log_p) : exp_t<true>((float)p[k] - t_most, a.k_hi, a.k_lo) / p_sum;
-                    if (q != 0) loss += q * (log_p - (((double)z_list[k] - M) * inv_T - log_total));
-                    p[k] = q;
+                if (threadIdx.x - slot * TPR < 64) {  // (one wavefront)
+                    if (REST) {
+                        loss = sums.a + sums.p * (M * inv_T + log_64(total));
+                        if (p_rest > 0) loss += p_rest * (log_64((double)p_rest * total / r.s) + ((double)M - m) * inv_T);
+                    } else {
+                        loss = sums.a / sums.p + log_64(total / sums.p) + M * inv_T;
+                    }
+                    loss *= weight * a.scale;
+                    if (a.stats && lane == 0 && lo == 0) a.stats[row] = make_float4(m, pass, M, list);
                 }
-                loss = team.sum(loss) * weight * a.scale;
-                if (a.stats && lane == 0 && lo == 0) a.stats[row] = make_float4(m, pass, M, list);
             }
 
             if (dz) {
-                if (FROM == FROM_STATS)
-                    for (int k = lane; k < a.K; k += TPR) p[k] = REST ? exp(p[k] * inv_T - log_sum) : exp_t<true>((float)p[k] - t_most, a.k_hi, a.k_lo) / p_sum;
                 const float c = (float)(weight * a.scale * inv_T) * (FROM == FROM_STATS ? *a.upstream : 1.0f), ca = c * pass;
+                auto gradient = [&](const Vec<T> &v, int at) {
+                    Vec<T> o;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) o.v[e] = (T)(ca * exp_t<FINE>((float)v.v[e] - m, a.k_hi, a.k_lo));
+                    Piece<T, TPR>(at, end).store(dz, o, end);
+                };
                 if (HOLD) {
 #pragma unroll
-                    for (int v = 0; v < NV; ++v) {
-                        const int at = (v * TPR + lane) * N;
-                        if (v * TPR * N >= a.V) continue;
-                        Vec<T> o;
-#pragma unroll
-                        for (int e = 0; e < N; ++e) o.v[e] = (T)(ca * exp_t<FINE>((float)held[v].v[e] - m, a.k_hi, a.k_lo));
-                        if (at + N <= a.V) store_vec(dz + at, o);
-                        else if (at < a.V) store_part(dz + at, o, a.V - at);
-                    }
+                    for (int v = 0; v < NV; ++v)
+                        if (v * TPR * N < a.V) gradient(held[v], (v * TPR + lane) * N);
                 } else {
-                    for (int at = lo + lane * N; at < end; at += TPR * N) {
-                        const Vec<T> v = distill_load<T, false>(z, at, end, nullptr, 0);
-                        Vec<T> o;
+                    for (int at = lo + lane * N; at < end; at += AHEAD * TPR * N) {
+                        Vec<T> v[AHEAD];
 #pragma unroll
-                        for (int e = 0; e < N; ++e) o.v[e] = (T)(ca * exp_t<FINE>((float)v.v[e] - m, a.k_hi, a.k_lo));
-                        if (at + N <= end) store_vec(dz + at, o);
-                        else store_part(dz + at, o, end - at);
+                        for (int k = 0; k < AHEAD; ++k) v[k] = Piece<T, TPR>(at + k * TPR * N, end).load(z, end);
+#pragma unroll
+                        for (int k = 0; k < AHEAD; ++k) gradient(v[k], at + k * TPR * N);
                     }
                 }
                 // the list's entries, over what the pass wrote there
                 __threadfence_block();
                 team.sync();
+                const float one = REST ? 1.0f : 1.0f / (float)sums.p;
                 for (int k = lane; k < a.K; k += TPR) {
                     const int i = index[k];
                     if (i < lo || i >= end) continue;
-                    double sum = 0;
-                    for (int l = 0; l < a.K; ++l) sum += index[l] == i ? p[l] : 0.0;
-                    dz[i] = (T)(c * (float)(list * (double)exp_t<true>(z_list[k] - M, a.k_hi, a.k_lo) - sum));
+                    int same = 0;
+#pragma unroll 4
+                    for (int l = 0; l < lists; l += 4) {
+                        const int4 four = *(const int4 *)(index + l);
+                        same += (four.x == i) + (four.y == i) + (four.z == i) + (four.w == i);
+                    }
+                    double sum = p[k];
+                    if (same > 1) {  // (in the list's order, so that all of them write the same)
+                        sum = 0;
+                        for (int l = 0; l < a.K; ++l)
+                            if (index[l] == i) sum += p[l];
+                    }
+                    dz[i] = (T)(c * (list * exp_t<true>(z_list[k] - M, a.k_hi, a.k_lo) - (float)sum * one));
                 }
             }
         }
@@ -377,8 +448,10 @@ __global__ __launch_bounds__(1024) void distill_sum(const double *__restrict__ l
     __shared__ double lds[16];
     double s = 0;
     for (int64_t k = threadIdx.x; k < n; k += 1024) s += losses[k];
-    const Team<1024> team = {lds};
-    s = team.sum(s);
+    s = team_sum(s, 64);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = team_sum(lds[threadIdx.x & 15], 16);
     if (threadIdx.x == 0) *loss = (float)s;
 }
 
@@ -388,15 +461,30 @@ constexpr int SPLIT_ROWS = 256;   // rows from which on a row has a workgroup to
 constexpr int SPLIT_PART = 4096;  // entries of a part, at least
 
 struct DistillPlan {
-    int tpr, hold;        // threads per row, elements held
-    int n_parts, part;    // of a row
-    int64_t blocks;       // sums of losses
+    int tpr, hold;      // threads per row, elements held
+    int n_parts, part;  // of a row
+    int64_t blocks;     // sums of losses
 };
 
-DistillPlan distill_plan(int64_t rows, int V, int K, bool rest) {
+// us for the loss with its gradient (without the teacher's lse), and for the loss alone:
+// * 8 and 16 threads: a row costs its list, whatever its length, and a wavefront takes eight or four lists at once (100000 x 100 float32: 16 threads 32 and 22, 64 threads
+//   86 and 66).
+// * A wavefront needs no barrier and has the most rows in flight, but takes long for a long row (16000 x 4000 bfloat16: 65 and 34, 256 threads 81 and 62; 8192 x 10000
+//   float32: 175 and 59, 256 threads 127 and 67; 1000 x 4000 bfloat16: 15 and 11, 256 threads 12 and 11).
+// * Rows that are held save the second read, and cost registers that others' loads would need: up to 64 elements a thread (8192 x 10000 float32: 127, read twice 155;
+//   4096 x 32000 bfloat16 in 128 a thread: 145, read twice 128).
+// * Rows that are read twice find what the first read left in the card's 256 MB cache while those in flight are a part of it: 64 KB a row with eight
+//   workgroups a compute unit, 256 KB with four, two beyond (4096 x 131072 bfloat16: 256 threads 628, 512 507, 1024 484, and with the teacher's lse, whose
+//   list a smaller workgroup waits less for, 622, 521, 650; float32 1242, 1151, 976).  The loss alone reads once (227, 260 and 340 with the lse).
+DistillPlan distill_plan(int64_t rows, int V, int K, bool rest, int size, bool gradient) {
     DistillPlan p = {};
-    p.tpr = V <= 64 && K <= 64 ? 8 : V <= 2048 && K <= 512 ? 64 : V <= 16384 ? 256 : 1024;
-    p.hold = p.tpr == 8 ? 8 : p.tpr == 64 ? 32 : V <= 65536 ? 64 : 0;
+    const int64_t bytes = (int64_t)V * size;
+    if (V <= 64 && K <= 64) p.tpr = 8, p.hold = 8;
+    else if (V <= 256 && K <= 64) p.tpr = 16, p.hold = 16;
+    else if (V <= 2048 && K <= 512) p.tpr = 64, p.hold = 32;
+    else if (rows >= 4096 && K <= 512 && bytes <= (gradient ? 16 << 10 : 64 << 10)) p.tpr = 64, p.hold = 0;
+    else if (gradient && V <= 16384) p.tpr = 256, p.hold = 64;
+    else p.tpr = !gradient || bytes <= 64 << 10 ? 256 : bytes <= 256 << 10 ? 512 : 1024, p.hold = 0;
     p.n_parts = 1, p.part = V;
     int64_t parts = 1;
     if (rows < SPLIT_ROWS && V >= 2 * SPLIT_PART) parts = (2 * SPLIT_ROWS + rows - 1) / rows;
@@ -422,7 +510,7 @@ int check_distill(const char *what, int64_t rows, int64_t V, int64_t K, double T
 }
 
 int64_t lds_of(const DistillRows &a, int tpr, bool bits, int entries) {
-    return (int64_t)(tpr < 256 ? 256 / tpr : 1) * (DISTILL_ENTRY * a.K + (bits ? 4 * bit_words(entries) : 0));
+    return (int64_t)(tpr < 256 ? 256 / tpr : 1) * (DISTILL_ENTRY * ((a.K + 3) & ~3) + (bits ? 4 * bit_words(entries) : 0));
 }
 
 template <typename T, int TPR, bool REST, int FROM, int HOLD>
@@ -447,10 +535,11 @@ int forward(DistillRows a, const DistillPlan &p, float *loss, hipStream_t st) {
         rc = launch<T, 256, REST, FROM_PARTS, 0>(a, a.rows * a.grid_parts, lds_of(a, 256, false, 0), st, what);
     } else {
         const int64_t lds = lds_of(a, p.tpr, REST, a.V);
-        rc = p.tpr == 8     ? launch<T, 8, REST, FROM_ROW, 8>(a, p.blocks, lds, st, what)
-             : p.tpr == 64  ? launch<T, 64, REST, FROM_ROW, 32>(a, p.blocks, lds, st, what)
-             : p.tpr == 256 ? launch<T, 256, REST, FROM_ROW, 64>(a, p.blocks, lds, st, what)
-             : p.hold       ? launch<T, 1024, REST, FROM_ROW, 64>(a, p.blocks, lds, st, what)
+        rc = p.tpr == 8      ? launch<T, 8, REST, FROM_ROW, 8>(a, p.blocks, lds, st, what)
+             : p.tpr == 16  ? launch<T, 16, REST, FROM_ROW, 16>(a, p.blocks, lds, st, what)
+             : p.tpr == 64  ? p.hold ? launch<T, 64, REST, FROM_ROW, 32>(a, p.blocks, lds, st, what) : launch<T, 64, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what)
+             : p.tpr == 256 ? p.hold ? launch<T, 256, REST, FROM_ROW, 64>(a, p.blocks, lds, st, what) : launch<T, 256, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what)
+             : p.tpr == 512 ? launch<T, 512, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what)
                             : launch<T, 1024, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what);
     }
     if (rc) return rc;
@@ -463,9 +552,11 @@ int backward(DistillRows a, const DistillPlan &p, hipStream_t st) {
     const char *what = "hgq_distill_topk_bwd";
     a.grid_parts = p.n_parts, a.part = p.part;
     const int64_t lds = lds_of(a, p.tpr, false, 0), blocks = p.blocks * p.n_parts;
-    return p.tpr == 8     ? launch<T, 8, REST, FROM_STATS, 0>(a, blocks, lds, st, what)
+    return p.tpr == 16    ? launch<T, 16, REST, FROM_STATS, 0>(a, blocks, lds, st, what)
+           : p.tpr == 8   ? launch<T, 8, REST, FROM_STATS, 0>(a, blocks, lds, st, what)
            : p.tpr == 64  ? launch<T, 64, REST, FROM_STATS, 0>(a, blocks, lds, st, what)
            : p.tpr == 256 ? launch<T, 256, REST, FROM_STATS, 0>(a, blocks, lds, st, what)
+           : p.tpr == 512 ? launch<T, 512, REST, FROM_STATS, 0>(a, blocks, lds, st, what)
                           : launch<T, 1024, REST, FROM_STATS, 0>(a, blocks, lds, st, what);
 }
 
@@ -486,8 +577,8 @@ using namespace hgq;
 
 extern "C" int64_t hgq_distill_topk_workspace(int64_t rows, int64_t V, int64_t K, int rest) {
     if (check_distill("hgq_distill_topk_workspace", rows, V, K, 1.0, HGQ_TYPE_F32, HGQ_TYPE_F32, 4)) return -1;
-    const DistillPlan p = distill_plan(rows, (int)V, (int)K, rest);
-    return 2 * p.blocks + (p.n_parts > 1 ? 2 * rows * p.n_parts : 0);
+    const DistillPlan p = distill_plan(rows, (int)V, (int)K, rest, 4, true);
+    return 2 * rows + (p.n_parts > 1 ? 2 * rows * p.n_parts : 0);  // (a sum for each row, at most)
 }
 
 extern "C" int hgq_distill_topk_fwd(const void *z, int64_t z_stride, const void *t, int t_type, const void *index, int index_bytes, const float *lse,
@@ -501,8 +592,8 @@ extern "C" int hgq_distill_topk_fwd(const void *z, int64_t z_stride, const void 
     if (!z || !t || !index || !workspace) return fail(HGQ_ERR_ARG, "%s: null pointer", what);
     if (z_stride < 0) return fail(HGQ_ERR_ARG, "%s: rows of logits must not run backwards", what);
     DistillRows a = arguments(z, z_stride, t, t_type, index, index_bytes, lse, weight, rows, V, K, T);
-    const DistillPlan p = distill_plan(rows, (int)V, (int)K, lse != nullptr);
-    a.stats = (float4 *)stats, a.dz = dz, a.losses = (double *)workspace, a.parts = (float2 *)(workspace + 2 * p.blocks);
+    const DistillPlan p = distill_plan(rows, (int)V, (int)K, lse != nullptr, type == HGQ_TYPE_F32 ? 4 : 2, dz != nullptr);
+    a.stats = (float4 *)stats, a.dz = dz, a.losses = (double *)workspace, a.parts = (float2 *)(workspace + 2 * rows);
     hipStream_t st = (hipStream_t)stream;
     if (lse) return type == HGQ_TYPE_F32 ? forward<float, true>(a, p, loss, st) : type == HGQ_TYPE_BF16 ? forward<__bf16, true>(a, p, loss, st) : forward<_Float16, true>(a, p, loss, st);
     return type == HGQ_TYPE_F32 ? forward<float, false>(a, p, loss, st) : type == HGQ_TYPE_BF16 ? forward<__bf16, false>(a, p, loss, st) : forward<_Float16, false>(a, p, loss, st);
@@ -519,7 +610,7 @@ extern "C" int hgq_distill_topk_bwd(const void *z, int64_t z_stride, const void 
     if (z_stride < 0) return fail(HGQ_ERR_ARG, "%s: rows of logits must not run backwards", what);
     DistillRows a = arguments(z, z_stride, t, t_type, index, index_bytes, lse, weight, rows, V, K, T);
     a.stats = (float4 *)stats, a.dz = dz, a.upstream = upstream, a.leave_unit = holds_unit;
-    const DistillPlan p = distill_plan(rows, (int)V, (int)K, lse != nullptr);
+    const DistillPlan p = distill_plan(rows, (int)V, (int)K, lse != nullptr, type == HGQ_TYPE_F32 ? 4 : 2, true);
     hipStream_t st = (hipStream_t)stream;
     if (lse) return type == HGQ_TYPE_F32 ? backward<float, true>(a, p, st) : type == HGQ_TYPE_BF16 ? backward<__bf16, true>(a, p, st) : backward<_Float16, true>(a, p, st);
     return type == HGQ_TYPE_F32 ? backward<float, false>(a, p, st) : type == HGQ_TYPE_BF16 ? backward<__bf16, false>(a, p, st) : backward<_Float16, false>(a, p, st);

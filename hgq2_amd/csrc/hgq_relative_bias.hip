@@ -13,6 +13,7 @@
 namespace hgq {
 
 constexpr int BIAS_BUCKETS = 128;
+constexpr int ADD_WGS = 2048;
 constexpr int BIAS_NEAR = 4096;  // distances whose bucket a workgroup looks up; beyond, where buckets still change there, it searches
 
 struct BiasShape {
@@ -20,6 +21,8 @@ struct BiasShape {
     int64_t stride_b, stride_h, offset;
     const void *offsets;  // [B] (int32 or int64) or null
     int B, H, S, TS, m, both, wide, near, chunk, chunks, tiles;
+    uint32_t magic, shift;  // of the division by S
+    __device__ __forceinline__ int row_of(int e) const { return (int)((__umulhi((uint32_t)e, magic) + (uint32_t)e) >> shift); }
 };
 
 __device__ __forceinline__ int bucket_of(const BiasShape &s, const int *first, int d) {
@@ -43,58 +46,66 @@ __device__ __forceinline__ int64_t offset_of(const BiasShape &s, int b) {
     return !s.offsets ? s.offset : s.wide ? ((const int64_t *)s.offsets)[b] : (int64_t)((const int32_t *)s.offsets)[b];
 }
 
-// Workgroup: 256 threads, one access each; blocks run over tiles of the plane, heads and runs of the batch.
-template <typename T>
-__global__ __launch_bounds__(256) void relative_bias_add(const T *__restrict__ scores, const float *__restrict__ table, T *__restrict__ out, const BiasShape s) {
-    constexpr int N = Vec<T>::N, AHEAD = 4;
+// A workgroup takes tiles t, t + stride, ... of a head's plane (256 accesses each) and a run of the batch.
+template <typename T, int AHEAD, bool THROUGH, bool TINY>
+__global__ __launch_bounds__(256) void relative_bias_add(const T *__restrict__ scores, const float *__restrict__ table, T *__restrict__ out, int stride, const BiasShape s) {
+    constexpr int N = Vec<T>::N;
     extern __shared__ float by_distance[];  // [2 near + 1], then the first distances
     int *first = (int *)(by_distance + 2 * s.near + 1);
     for (int k = threadIdx.x; k < s.m - 1; k += 256) first[k] = s.first[k];
     __syncthreads();
     int block = blockIdx.x;
-    const int tile = block % s.tiles;
-    block /= s.tiles;
+    const int tile0 = block % stride;
+    block /= stride;
     const int h = block % s.H, b0 = block / s.H * s.chunk, b1 = min(s.B, b0 + s.chunk);
     for (int k = threadIdx.x; k <= 2 * s.near; k += 256) by_distance[k] = table[bucket_of(s, first, k - s.near) * s.H + h];
     __syncthreads();
-    const int e0 = (tile * 256 + (int)threadIdx.x) * N;
-    if (e0 >= s.TS) return;
-    const int i0 = e0 / s.S, j0 = e0 - i0 * s.S, n = min(N, s.TS - e0);
     const bool beyond = s.first[s.m - 2] > s.near;
-    float bias[N];
-    const T *from = scores + b0 * s.stride_b + h * s.stride_h + e0;
-    T *to = out + ((int64_t)b0 * s.H + h) * s.TS + e0;
     const int64_t step = (int64_t)s.H * s.TS;
-    for (int b = b0; b < b1; b += AHEAD) {
-        Vec<T> v[AHEAD];
-        if (n == N) {
+    for (int tile = tile0; tile < s.tiles; tile += stride) {
+        const int at = (tile * 256 + (int)threadIdx.x) * N;
+        if (at >= s.TS) return;
+        const int e0 = TINY ? 0 : min(at, s.TS - N), i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
+        float bias[N];
+        const T *from = scores + b0 * s.stride_b + h * s.stride_h + e0;
+        T *to = out + ((int64_t)b0 * s.H + h) * s.TS + e0;
+        for (int b = b0; b < b1; b += AHEAD) {
+            Vec<T> v[AHEAD];
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a)
-                if (b + a < b1) v[a] = load_vec(from + a * s.stride_b);
-        } else {
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a)
-                if (b + a < b1) v[a] = load_part(from + a * s.stride_b, n, (T)0.0f);
-        }
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            if (b + a >= b1) break;
-            if (b + a == b0 || s.offsets) {
-                const int64_t offset = offset_of(s, b + a);
-                int i = i0, j = j0;
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const int d = distance(i, j, offset);
-                    bias[e] = beyond && abs(d) > s.near ? table[bucket_of(s, first, d) * s.H + h] : by_distance[max(-s.near, min(s.near, d)) + s.near];
-                    if (++j == s.S) j = 0, ++i;
-                }
+            for (int a = 0; a < AHEAD; ++a) {
+                const T *p = from + min(a, b1 - 1 - b) * s.stride_b;
+                if (TINY) v[a] = load_part(p, s.TS, (T)0.0f);
+                else v[a] = load_vec<T, THROUGH>(p);
             }
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[a].v[e] = (T)((float)v[a].v[e] + bias[e]);
-            if (n == N) store_vec(to + a * step, v[a]);
-            else store_part(to + a * step, v[a], n);
+            for (int a = 0; a < AHEAD; ++a) {
+                if (b + a >= b1) break;
+                if (b + a == b0 || s.offsets) {
+                    const int64_t offset = offset_of(s, b + a);
+                    int i = i0, j = j0;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const int d = distance(i, j, offset);
+                        bias[e] = by_distance[max(-s.near, min(s.near, d)) + s.near];
+                        if (++j == s.S) j = 0, ++i;
+                    }
+                    if (beyond) {
+                        i = i0, j = j0;
+                        for (int e = 0; e < N; ++e) {
+                            const int d = distance(i, j, offset);
+                            if (abs(d) > s.near) bias[e] = table[bucket_of(s, first, d) * s.H + h];
+                            if (++j == s.S) j = 0, ++i;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[a].v[e] = (T)((float)v[a].v[e] + bias[e]);
+                // (the last access writes what the one before it writes, once more)
+                if (TINY) store_part(to + a * step, v[a], s.TS);
+                else store_vec<T, THROUGH>(to + a * step, v[a]);
+            }
+            from += AHEAD * s.stride_b, to += AHEAD * step;
         }
-        from += AHEAD * s.stride_b, to += AHEAD * step;
     }
 }
 
@@ -112,10 +123,13 @@ struct BiasRun {
     }
 };
 
-// Workgroup w of a head takes items w, w + parts, ... - an item: a tile of the plane and a run of the batch.  parts [H][parts][n].
-template <typename T>
+// Workgroup w of a head takes items w, w + parts, ... - an item: TILES tiles of the plane and a run of the batch, which is read SEQS sequences at a time (with
+// more than one tile a run has no more than that).  While one such round is added up, the next one's loads are on their way.  parts [H][parts][n].
+// The last access of a plane ends with it, and its first elements are the one before's again: no access is cut (a load that may be either whole or cut is
+// taken apart into elements where it arrives, and waited for there: 357 us instead of 205 at 8 x 16 x 2048 x 2048 bfloat16).  TINY: planes of less than one access.
+template <typename T, int SEQS, int TILES, bool TINY>
 __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ dy, double *__restrict__ part, int parts, const BiasShape s) {
-    constexpr int N = Vec<T>::N, AHEAD = 8;
+    constexpr int N = Vec<T>::N, LOADS = SEQS * TILES;
     extern __shared__ double bias_lds[];
     const int n_buckets = s.both ? 2 * s.m : s.m, threads = blockDim.x;
     int *first = (int *)(bias_lds + n_buckets * threads);
@@ -128,53 +142,99 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
     const bool beyond = s.first[s.m - 2] > s.near;
     const int h = blockIdx.x / parts, w = blockIdx.x - h * parts;
     BiasRun run = {bias_lds, threads, -1, 0.0};
-    for (int64_t item = w; item < (int64_t)s.tiles * s.chunks; item += parts) {
-        const int c = (int)(item / s.tiles), tile = (int)(item - (int64_t)c * s.tiles);
-        const int b0 = c * s.chunk, b1 = min(s.B, b0 + s.chunk), e0 = (tile * threads + (int)threadIdx.x) * N;
-        if (e0 >= s.TS) continue;
-        const int i0 = e0 / s.S, j0 = e0 - i0 * s.S, n = min(N, s.TS - e0);
-        const T *from = dy + b0 * s.stride_b + h * s.stride_h + e0;
-        double sum[N] = {};
-        for (int b = b0; b < b1; b += AHEAD) {  // eight terms pairwise in fp32, their sums in fp64
-            Vec<T> v[AHEAD];
+    const int groups = (s.tiles + TILES - 1) / TILES, rounds = TILES > 1 ? 1 : (s.chunk + SEQS - 1) / SEQS;
+    const int64_t items = (int64_t)groups * s.chunks;
+    double sum[N] = {};
+
+    struct Step {
+        int64_t item;
+        int c, tile, round;
+    };
+    auto step_of = [&](int64_t item) {
+        const int c = (int)(item / groups);
+        return Step{item, c, (int)(item - (int64_t)c * groups) * TILES, 0};
+    };
+    auto after = [&](const Step &k) { return k.round + 1 < rounds ? Step{k.item, k.c, k.tile, k.round + 1} : step_of(k.item + parts); };
+    auto first_of = [&](const Step &k, int t) { return ((int64_t)(k.tile + t) * threads + (int)threadIdx.x) * N; };
+
+    auto ask = [&](const Step &k, Vec<T> *v) {  // beyond the run and the last item: what is there already, once more
+        const int b = min(k.c, s.chunks - 1) * s.chunk + k.round * SEQS, b1 = min(s.B, (min(k.c, s.chunks - 1) + 1) * s.chunk);
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                if (b + a < b1) v[a] = n == N ? load_vec(from + a * s.stride_b) : load_part(from + a * s.stride_b, n, (T)0.0f);
-                else {
+        for (int t = 0; t < TILES; ++t) {
+            const T *from = dy + b * s.stride_b + h * s.stride_h + max((int64_t)0, min(first_of(k, t), (int64_t)s.TS - N));
 #pragma unroll
-                    for (int e = 0; e < N; ++e) v[a].v[e] = (T)0.0f;
+            for (int a = 0; a < SEQS; ++a) {
+                const T *at = from + min(a, b1 - 1 - b) * s.stride_b;
+                if (TINY) v[t * SEQS + a] = load_part(at, s.TS, (T)0.0f);
+                else v[t * SEQS + a] = load_vec(at);
+            }
+        }
+    };
+
+    auto bucket = [&](int d) {
+        int k = near[max(-s.near, min(s.near, d)) + s.near];
+        if (beyond && abs(d) > s.near) k = bucket_of(s, first, d);
+        return k;
+    };
+
+    auto take = [&](const Step &k, const Vec<T> *v) {
+        const int many = min(s.B, (k.c + 1) * s.chunk) - k.c * s.chunk - k.round * SEQS;  // sequences of this round
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {  // up to eight terms pairwise in fp32, their sums in fp64
+                float f[SEQS];
+#pragma unroll
+                for (int a = 0; a < SEQS; ++a) f[a] = a < many ? (float)v[t * SEQS + a].v[e] : 0.0f;
+#pragma unroll
+                for (int d = SEQS / 2; d; d /= 2)
+#pragma unroll
+                    for (int a = 0; a < d; ++a) f[a] += f[a + d];
+                sum[e] += f[0];
+            }
+            if (k.round + 1 < rounds) continue;
+            const int64_t at = first_of(k, t);
+            if (at < s.TS) {
+                const int e0 = TINY ? 0 : min((int)at, s.TS - N), skip = (int)at - e0, n = TINY ? s.TS : N, i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
+                const int64_t offset = offset_of(s, k.c * s.chunk);  // (with offsets of their own, runs are of one sequence)
+                const int d0 = distance(i0, j0, offset), k0 = bucket(d0), k1 = bucket(distance(i0, j0 + N - 1, offset));
+                if (!TINY && j0 + N <= s.S && k0 == k1) {
+                    double all[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) all[e] = e < skip ? 0.0 : sum[e];
+#pragma unroll
+                    for (int d = N / 2; d; d /= 2)
+#pragma unroll
+                        for (int e = 0; e < d; ++e) all[e] += all[e + d];
+                    run.add(k0, all[0]);
+                } else {
+                    int i = i0, j = j0, of[N];
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        of[e] = bucket(distance(i, j, offset));
+                        if (++j == s.S) j = 0, ++i;
+                    }
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (e >= skip && e < n) run.add(of[e], sum[e]);
                 }
             }
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                float f[AHEAD];
-#pragma unroll
-                for (int a = 0; a < AHEAD; ++a) f[a] = (float)v[a].v[e];
-#pragma unroll
-                for (int k = AHEAD / 2; k; k /= 2)
-#pragma unroll
-                    for (int a = 0; a < k; ++a) f[a] += f[a + k];
-                sum[e] += f[0];
-            }
-            from += AHEAD * s.stride_b;
+            for (int e = 0; e < N; ++e) sum[e] = 0;
         }
-        const int64_t offset = offset_of(s, b0);  // (with offsets of their own, runs are of one sequence)
-        auto bucket = [&](int d) { return beyond && abs(d) > s.near ? bucket_of(s, first, d) : (int)near[max(-s.near, min(s.near, d)) + s.near]; };
-        const int d0 = distance(i0, j0, offset), k0 = bucket(d0);
-        if (n == N && j0 + N <= s.S && bucket(distance(i0, j0 + N - 1, offset)) == k0) {
-#pragma unroll
-            for (int k = N / 2; k; k /= 2)
-#pragma unroll
-                for (int e = 0; e < k; ++e) sum[e] += sum[e + k];
-            run.add(k0, sum[0]);
-        } else {
-            int i = i0, j = j0;
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                if (e < n) run.add(bucket(distance(i, j, offset)), sum[e]);
-                if (++j == s.S) j = 0, ++i;
-            }
-        }
+    };
+
+    Vec<T> even[LOADS], odd[LOADS];
+    Step k = step_of(w);
+    ask(k, even);
+    while (k.item < items) {
+        const Step k1 = after(k);
+        ask(k1, odd);
+        take(k, even);
+        if (k1.item >= items) break;
+        k = after(k1);
+        ask(k, even);
+        take(k1, odd);
     }
     run.flush();
     __syncthreads();
@@ -217,6 +277,9 @@ BiasShape bias_shape(int64_t B, int64_t H, int64_t T, int64_t S, const int *firs
     s.B = (int)B, s.H = (int)H, s.S = (int)S, s.TS = (int)(T * S), s.m = m, s.both = both, s.offset = offset, s.offsets = offsets, s.wide = offset_bytes == 8;
     s.stride_b = stride_b, s.stride_h = stride_h;
     s.near = first[m - 2] < BIAS_NEAR ? first[m - 2] : BIAS_NEAR;
+    // e / S = (hi(e magic) + e) >> shift for e < 2^31, with magic = floor(2^32 (2^shift - S) / S) + 1 and 2^shift the first power of two that is not below S
+    while (((int64_t)1 << s.shift) < S) ++s.shift;
+    s.magic = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s.shift) - (uint64_t)S)) / (uint64_t)S + 1);
     return s;
 }
 
@@ -230,34 +293,56 @@ void cut(BiasShape &s, int64_t threads, int N, int64_t wanted) {  // tiles of th
 
 int sums_threads(int n) { return n <= 16 ? 256 : n <= 32 ? 128 : 64; }  // 32 KB of bins up to 64 buckets: five workgroups a compute unit
 
-int sums_parts(const BiasShape &s, int threads) {
-    const int64_t items = (int64_t)s.tiles * s.chunks;
+int sums_parts(const BiasShape &s, int threads, int tiles) {
+    const int64_t items = (int64_t)((s.tiles + tiles - 1) / tiles) * s.chunks;
     int64_t parts = (512 * (256 / threads) + s.H - 1) / s.H;
     return (int)(items < parts ? items : parts);
 }
 
 template <typename T>
+auto add_kernel(const BiasShape &s, bool through) {
+    if (s.TS < Vec<T>::N) return relative_bias_add<T, 4, false, true>;
+    if (s.chunk < 4) return through ? relative_bias_add<T, 1, true, false> : relative_bias_add<T, 1, false, false>;
+    return through ? relative_bias_add<T, 4, true, false> : relative_bias_add<T, 4, false, false>;
+}
+
+template <typename T>
 int add(const void *scores, const float *table, void *out, BiasShape s, hipStream_t st) {
     cut(s, 256, Vec<T>::N, 2048);
-    const int64_t blocks = (int64_t)s.tiles * s.H * s.chunks;
+    // a workgroup's table of biases takes it some 2 us: tiles in turn
+    int64_t stride = ADD_WGS / ((int64_t)s.H * s.chunks) + 1;
+    if (stride > s.tiles) stride = s.tiles;
+    const int64_t blocks = stride * s.H * s.chunks;
     if (blocks * 256 > 0xffffffffLL) return fail(HGQ_ERR_UNSUPPORTED, "hgq_relative_bias_fwd: too many scores");
-    hipLaunchKernelGGL(relative_bias_add<T>, dim3((unsigned)blocks), dim3(256), 4 * (2 * s.near + 1 + BIAS_BUCKETS), st, (const T *)scores, table, (T *)out, s);
+    const bool through = (int64_t)s.B * s.H * s.TS * (int64_t)sizeof(T) * 2 > (int64_t)256 << 20;
+    hipLaunchKernelGGL(add_kernel<T>(s, through), dim3((unsigned)blocks), dim3(256), 4 * (2 * s.near + 1 + BIAS_BUCKETS), st, (const T *)scores, table, (T *)out,
+                       (int)stride, s);
     return check_launch("hgq_relative_bias_fwd");
+}
+
+template <typename T, int SEQS, int TILES, bool TINY>
+int sums_of(const void *dy, double *part, int parts, int threads, const BiasShape &s, hipStream_t st) {
+    const int n = s.both ? 2 * s.m : s.m, lds = 8 * n * threads + 4 * BIAS_BUCKETS + 2 * s.near + 1;
+    // (more than 112 buckets; per device, so it is asked for at every such call)
+    if (lds > 64 << 10 && hipFuncSetAttribute((const void *)relative_bias_sums<T, SEQS, TILES, TINY>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 << 10) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(HGQ_ERR_LAUNCH, "hgq_relative_bias_bwd: cannot reserve LDS");
+    }
+    hipLaunchKernelGGL((relative_bias_sums<T, SEQS, TILES, TINY>), dim3((unsigned)(parts * s.H)), dim3(threads), lds, st, (const T *)dy, part, parts, s);
+    return check_launch("hgq_relative_bias_bwd");
 }
 
 template <typename T>
 int sums(const void *dy, float *dtable, double *part, BiasShape s, hipStream_t st) {
     const int n = s.both ? 2 * s.m : s.m, threads = sums_threads(n);
     cut(s, threads, Vec<T>::N, 1024);
-    const int parts = sums_parts(s, threads);
-    const int lds = 8 * n * threads + 4 * BIAS_BUCKETS + 2 * s.near + 1;
-    // (more than 112 buckets; per device, so it is asked for at every such call)
-    if (lds > 64 << 10 && hipFuncSetAttribute((const void *)relative_bias_sums<T>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 << 10) != hipSuccess) {
-        (void)hipGetLastError();
-        return fail(HGQ_ERR_LAUNCH, "hgq_relative_bias_bwd: cannot reserve LDS");
-    }
-    hipLaunchKernelGGL(relative_bias_sums<T>, dim3((unsigned)(parts * s.H)), dim3(threads), lds, st, (const T *)dy, part, parts, s);
-    int rc = check_launch("hgq_relative_bias_bwd");
+    const int seqs = s.chunk >= 5 ? 8 : s.chunk >= 3 ? 4 : s.chunk, parts = sums_parts(s, threads, 8 / seqs);
+    const bool tiny = s.TS < Vec<T>::N;
+    int rc = (tiny        ? seqs == 8 ? sums_of<T, 8, 1, true> : seqs == 4 ? sums_of<T, 4, 2, true> : seqs == 2 ? sums_of<T, 2, 4, true> : sums_of<T, 1, 8, true>
+              : seqs == 8 ? sums_of<T, 8, 1, false>
+              : seqs == 4 ? sums_of<T, 4, 2, false>
+              : seqs == 2 ? sums_of<T, 2, 4, false>
+                          : sums_of<T, 1, 8, false>)(dy, part, parts, threads, s, st);
     if (rc) return rc;
     hipLaunchKernelGGL(relative_bias_join, dim3((unsigned)((n * s.H + 3) / 4)), dim3(256), 0, st, (const double *)part, parts, dtable, n, s.H);
     return check_launch("hgq_relative_bias_bwd");
