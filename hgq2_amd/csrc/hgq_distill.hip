@@ -155,9 +155,10 @@ struct Piece {
                 if (b >> e & 1) r.v[e] = (T)-INFINITY;
         }
     }
+    template <bool THROUGH>
     __device__ __forceinline__ void store(T *z, const Vec<T> &r, int end) const {
         if (own == 0 && at + N <= end) {
-            store_vec<T, true>(z + at, r);
+            store_vec<T, THROUGH>(z + at, r);
         } else {
 #pragma unroll
             for (int e = 0; e < N; ++e)
@@ -252,8 +253,9 @@ __global__ __launch_bounds__(256) void distill_parts(const DistillRows a) {
 // What the maximum and the sum of a row come from: the row itself, what distill_parts left, or a forward call's numbers
 enum { FROM_ROW, FROM_PARTS, FROM_STATS };
 
-// TPR threads take a row; HOLD elements of it stay in a thread's registers between the sum and the gradient (0: the row is read twice).
-template <typename T, int TPR, bool REST, int FROM, int HOLD>
+// TPR threads take a row; HOLD elements of it stay in a thread's registers between the sum and the gradient (0: the row is read twice).  THROUGH: the gradient goes past the
+// cache, which it leaves to the logits.
+template <typename T, int TPR, bool REST, int FROM, int HOLD, bool THROUGH = false>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const DistillRows a) {
     constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR, N = Vec<T>::N, NV = HOLD ? HOLD / N : 1;
     constexpr bool FINE = sizeof(T) == 4;
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const Dist
                 Vec<T> zero;
 #pragma unroll
                 for (int e = 0; e < N; ++e) zero.v[e] = (T)0.0f;
-                for (int at = lo + lane * N; at < end; at += TPR * N) Piece<T, TPR>(at, end).store(dz, zero, end);
+                for (int at = lo + lane * N; at < end; at += TPR * N) Piece<T, TPR>(at, end).template store<THROUGH>(dz, zero, end);
             }
         } else {
             RowSums sums = {{-INFINITY, 0.0f}, {-INFINITY, 0.0f}, 0.0, 0.0};
@@ -390,7 +392,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const Dist
                     Vec<T> o;
 #pragma unroll
                     for (int e = 0; e < N; ++e) o.v[e] = (T)(ca * exp_t<FINE>((float)v.v[e] - m, a.k_hi, a.k_lo));
-                    Piece<T, TPR>(at, end).store(dz, o, end);
+                    Piece<T, TPR>(at, end).template store<THROUGH>(dz, o, end);
                 };
                 if (HOLD) {
 #pragma unroll
@@ -513,11 +515,11 @@ int64_t lds_of(const DistillRows &a, int tpr, bool bits, int entries) {
     return (int64_t)(tpr < 256 ? 256 / tpr : 1) * (DISTILL_ENTRY * ((a.K + 3) & ~3) + (bits ? 4 * bit_words(entries) : 0));
 }
 
-template <typename T, int TPR, bool REST, int FROM, int HOLD>
+template <typename T, int TPR, bool REST, int FROM, int HOLD, bool THROUGH = false>
 int launch(const DistillRows &a, int64_t blocks, int64_t lds, hipStream_t st, const char *what) {
     constexpr int threads = TPR > 256 ? TPR : 256;
     if (blocks * threads > 0xffffffffLL) return fail(HGQ_ERR_UNSUPPORTED, "%s: too many rows", what);
-    hipLaunchKernelGGL((distill_rows<T, TPR, REST, FROM, HOLD>), dim3((unsigned)blocks), dim3(threads), (size_t)lds, st, a);
+    hipLaunchKernelGGL((distill_rows<T, TPR, REST, FROM, HOLD, THROUGH>), dim3((unsigned)blocks), dim3(threads), (size_t)lds, st, a);
     return check_launch(what);
 }
 
@@ -535,11 +537,15 @@ int forward(DistillRows a, const DistillPlan &p, float *loss, hipStream_t st) {
         rc = launch<T, 256, REST, FROM_PARTS, 0>(a, a.rows * a.grid_parts, lds_of(a, 256, false, 0), st, what);
     } else {
         const int64_t lds = lds_of(a, p.tpr, REST, a.V);
+        const bool through = a.dz && a.rows * a.V * (int64_t)sizeof(T) * 2 > (int64_t)256 << 20;  // logits and gradient are more than the card's cache
         rc = p.tpr == 8      ? launch<T, 8, REST, FROM_ROW, 8>(a, p.blocks, lds, st, what)
              : p.tpr == 16  ? launch<T, 16, REST, FROM_ROW, 16>(a, p.blocks, lds, st, what)
              : p.tpr == 64  ? p.hold ? launch<T, 64, REST, FROM_ROW, 32>(a, p.blocks, lds, st, what) : launch<T, 64, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what)
-             : p.tpr == 256 ? p.hold ? launch<T, 256, REST, FROM_ROW, 64>(a, p.blocks, lds, st, what) : launch<T, 256, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what)
-             : p.tpr == 512 ? launch<T, 512, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what)
+             : p.tpr == 256 ? p.hold      ? launch<T, 256, REST, FROM_ROW, 64>(a, p.blocks, lds, st, what)
+                              : through ? launch<T, 256, REST, FROM_ROW, 0, true>(a, p.blocks, lds, st, what)
+                                        : launch<T, 256, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what)
+             : p.tpr == 512 ? through ? launch<T, 512, REST, FROM_ROW, 0, true>(a, p.blocks, lds, st, what) : launch<T, 512, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what)
+             : through      ? launch<T, 1024, REST, FROM_ROW, 0, true>(a, p.blocks, lds, st, what)
                             : launch<T, 1024, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what);
     }
     if (rc) return rc;

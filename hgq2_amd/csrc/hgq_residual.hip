@@ -26,42 +26,67 @@ struct ResidualRows {
     float *r_u, *r_y;
     float *slices;       // [workgroups][2][C]: dpost, dpre
     float *gate_slices;  // [units][C], or null: dgate is written as it is formed
+    int64_t step_samples, step_rows;         // of a workgroup's step over rows, in samples and rows
+    int64_t samples;                         // rows of a gate for P rows
     int64_t rows, P, units, per_unit, cuts;  // rows; of a gate's row; what a workgroup takes at a time, its rows; units of a sample
     int C, tpr, act, by_sample;
     float scale, eps;
 };
 
-// the threads of a row: neighbouring lanes of a wavefront, or (WIDE) a workgroup
+// The threads of a row: neighbouring lanes of a wavefront, or (WIDE) a workgroup.  Sums of a workgroup take turns with two places in LDS: whoever writes one
+// again is behind the barrier of the sum between.
 template <bool WIDE>
-__device__ __forceinline__ float row_sum(float v, int tpr, float *lds) {
-    if (!WIDE) return team_sum(v, tpr);
-    v = team_sum(v, 64);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    const int waves = tpr >> 6;
-    v = team_sum(lds[threadIdx.x & (waves - 1)], waves);
-    __syncthreads();
-    return v;
-}
+struct RowTeam {
+    int tpr;
+    float (*lds)[16];
+    int turn;
+    __device__ __forceinline__ float sum(float v) {
+        if (!WIDE) return team_sum(v, tpr);
+        v = team_sum(v, 64);
+        float *at = lds[turn ^= 1];
+        if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+        __syncthreads();
+        const int waves = tpr >> 6;
+        return team_sum(at[threadIdx.x & (waves - 1)], waves);
+    }
+};
 
 __device__ __forceinline__ float norm_factor(float sum, int C, float eps) { return 1.0f / sqrtf(sum / (float)C + eps); }
 
 __device__ __forceinline__ float opened(float g, int act) { return act ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269502f)) : g; }
 
-template <typename T>
+// A thread's eight elements of a row.  A row's last access ends with the row: its first elements are the neighbour's again and count as zeros here.  TINY: rows of
+// less than one access.
+template <typename T, bool TINY>
 struct Held {
     static constexpr int N = Vec<T>::N, NV = RES_HELD / N;
-    int at[NV], n[NV];  // this thread's columns
-    __device__ __forceinline__ Held(int lane, int tpr, int C) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) at[v] = (v * tpr + lane) * N, n[v] = max(0, min(N, C - at[v]));
-    }
-    __device__ __forceinline__ void load(float *f, const T *row) const {
+    struct Raw {
+        u32x4 v[NV];
+    };
+    int at[NV], own[NV];  // this thread's columns, and which of the first ones are the neighbour's
+    int C;
+    __device__ __forceinline__ Held(int lane, int tpr, int channels) : C(channels) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const Vec<T> r = n[v] == N ? load_vec(row + at[v]) : load_part(row + at[v], n[v], (T)0.0f);
+            const int wanted = (v * tpr + lane) * N;
+            at[v] = TINY ? wanted : min(wanted, C - N), own[v] = min(N, wanted - at[v]);
+        }
+    }
+    __device__ __forceinline__ Raw ask(const T *row) const {
+        Raw r;
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[v * N + e] = (float)r.v[e];
+        for (int v = 0; v < NV; ++v) {
+            if (TINY) r.v[v] = __builtin_bit_cast(u32x4, load_part(row + at[v], C - at[v], (T)0.0f));
+            else r.v[v] = load_words(row + at[v]);
+        }
+        return r;
+    }
+    __device__ __forceinline__ void take(float *f, const Raw &r) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const Vec<T> w = __builtin_bit_cast(Vec<T>, r.v[v]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[v * N + e] = e < own[v] ? 0.0f : (float)w.v[e];
         }
     }
     __device__ __forceinline__ void store(T *row, const float *f) const {
@@ -70,43 +95,72 @@ struct Held {
             Vec<T> r;
 #pragma unroll
             for (int e = 0; e < N; ++e) r.v[e] = (T)f[v * N + e];
-            if (n[v] == N) store_vec(row + at[v], r);
-            else store_part(row + at[v], r, n[v]);
+            if (!TINY && own[v] == 0) {
+                store_vec(row + at[v], r);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (e >= own[v] && at[v] + e < C) row[at[v] + e] = r.v[e];
+            }
         }
     }
+    __device__ __forceinline__ bool mine(int v, int e) const { return e >= own[v] && at[v] + e < C; }
     __device__ __forceinline__ void vector(float *f, const float *p, float scale) const {  // of channels, times `scale`
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[v * N + e] = e < n[v] ? (p ? p[at[v] + e] : 1.0f) * scale : 0.0f;
+            for (int e = 0; e < N; ++e) f[v * N + e] = p ? p[TINY ? min(at[v] + e, C - 1) : at[v] + e] : 1.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < N; ++e) f[v * N + e] = mine(v, e) ? f[v * N + e] * scale : 0.0f;
     }
 };
 
-enum { NO_UPDATE, NO_GATE, GATED };
+enum { NO_UPDATE, NO_GATE, GATED, GATED_SAMPLES };  // the last: one row of a gate for P rows
 
-template <typename T, int KIND, bool WIDE>
-__global__ __launch_bounds__(WIDE ? 1024 : 256) void residual_fwd(const ResidualRows a) {
-    __shared__ float lds[16];
+template <typename T, int KIND, int THREADS, bool TINY>
+__global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
+    constexpr bool WIDE = THREADS > 256;
+    __shared__ float lds[2][16];
+    using H = Held<T, TINY>;
     const int teams = WIDE ? 1 : 256 / a.tpr, slot = WIDE ? 0 : threadIdx.x / a.tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (a.tpr - 1);
-    const Held<T> held(lane, a.tpr, a.C);
+    const H held(lane, a.tpr, a.C);
+    RowTeam<WIDE> team = {a.tpr, lds, 0};
     float post[RES_HELD], pre[RES_HELD];
     if (KIND != NO_UPDATE) held.vector(post, a.post, a.scale);
     held.vector(pre, a.pre, 1.0f);
-    for (int64_t row = (int64_t)blockIdx.x * teams + slot; row < a.rows; row += (int64_t)gridDim.x * teams) {
+    const int64_t step = (int64_t)gridDim.x * teams;
+    int64_t row = (int64_t)blockIdx.x * teams + slot, sample = 0, position = 0;
+    if (KIND == GATED_SAMPLES) sample = row / a.P, position = row - sample * a.P;
+    typename H::Raw x_raw, u_raw, g_raw;
+    auto ask = [&](int64_t k) {
+        const int64_t base = min(k, a.rows - 1) * a.C;
+        x_raw = held.ask((const T *)a.x + base);
+        if (KIND != NO_UPDATE) u_raw = held.ask((const T *)a.u + base);
+        if (KIND >= GATED) g_raw = held.ask((const T *)a.gate + (KIND == GATED_SAMPLES ? min(sample, a.samples - 1) * a.C : base));
+    };
+    ask(row);
+    for (; row < a.rows; row += step) {
         const int64_t base = row * a.C;
         float y[RES_HELD], u[RES_HELD], g[RES_HELD], s = 0;
-        held.load(y, (const T *)a.x + base);
+        held.take(y, x_raw);
+        if (KIND != NO_UPDATE) held.take(u, u_raw);
+        if (KIND >= GATED) held.take(g, g_raw);
+        if (KIND == GATED_SAMPLES) {
+            sample += a.step_samples, position += a.step_rows;
+            if (position >= a.P) position -= a.P, ++sample;
+        }
+        ask(row + step);  // on its way while this row is worked on
         if (KIND != NO_UPDATE) {
-            held.load(u, (const T *)a.u + base);
-            if (KIND == GATED) held.load(g, (const T *)a.gate + (a.by_sample ? row / a.P * a.C : base));
 #pragma unroll
             for (int e = 0; e < RES_HELD; ++e) s += u[e] * u[e];
-            const float r_u = norm_factor(row_sum<WIDE>(s, a.tpr, lds), a.C, a.eps);
+            const float r_u = norm_factor(team.sum(s), a.C, a.eps);
             s = 0;
 #pragma unroll
             for (int e = 0; e < RES_HELD; ++e) {
                 float b = u[e] * r_u * post[e];
-                if (KIND == GATED) b *= opened(g[e], a.act);
+                if (KIND >= GATED) b *= opened(g[e], a.act);
                 y[e] += b;
             }
             if (a.r_u && lane == 0) a.r_u[row] = r_u;
@@ -114,7 +168,7 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void residual_fwd(const Residual
         }
 #pragma unroll
         for (int e = 0; e < RES_HELD; ++e) s += y[e] * y[e];
-        const float r_y = norm_factor(row_sum<WIDE>(s, a.tpr, lds), a.C, a.eps);
+        const float r_y = norm_factor(team.sum(s), a.C, a.eps);
         if (a.r_y && lane == 0) a.r_y[row] = r_y;
 #pragma unroll
         for (int e = 0; e < RES_HELD; ++e) y[e] *= r_y * pre[e];
@@ -122,107 +176,151 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void residual_fwd(const Residual
     }
 }
 
-template <typename T, int KIND, bool WIDE>
-__global__ __launch_bounds__(WIDE ? 1024 : 256) void residual_bwd(const ResidualRows a) {
-    __shared__ float lds[16];
+template <typename T, int KIND, int THREADS, bool TINY>
+__global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
+    constexpr bool WIDE = THREADS > 256;
+    __shared__ float lds[2][16];
     __shared__ float joined[WIDE ? 1 : 256 * RES_HELD];
+    using H = Held<T, TINY>;
     const int teams = WIDE ? 1 : 256 / a.tpr, slot = WIDE ? 0 : threadIdx.x / a.tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (a.tpr - 1);
-    const Held<T> held(lane, a.tpr, a.C);
+    const H held(lane, a.tpr, a.C);
+    RowTeam<WIDE> team = {a.tpr, lds, 0};
     float post[RES_HELD], pre[RES_HELD], dpost[RES_HELD] = {}, dpre[RES_HELD] = {}, dgate[RES_HELD] = {};
     if (KIND != NO_UPDATE) held.vector(post, a.post, a.scale);
     held.vector(pre, a.pre, 1.0f);
 
     // one row of channels from the teams' sums, in order
     auto leave = [&](const float *f, auto *out) {
+        using Out = std::remove_reference_t<decltype(*out)>;
         if (WIDE) {
 #pragma unroll
-            for (int v = 0; v < Held<T>::NV; ++v)
+            for (int v = 0; v < H::NV; ++v)
 #pragma unroll
-                for (int e = 0; e < Held<T>::N; ++e)
-                    if (e < held.n[v]) out[held.at[v] + e] = (std::remove_reference_t<decltype(*out)>)f[v * Held<T>::N + e];
+                for (int e = 0; e < H::N; ++e)
+                    if (held.mine(v, e)) out[held.at[v] + e] = (Out)f[v * H::N + e];
             return;
         }
         __syncthreads();
-        const int width = a.tpr * RES_HELD;
 #pragma unroll
-        for (int v = 0; v < Held<T>::NV; ++v)
+        for (int v = 0; v < H::NV; ++v)
 #pragma unroll
-            for (int e = 0; e < Held<T>::N; ++e) joined[slot * width + held.at[v] + e] = f[v * Held<T>::N + e];
+            for (int e = 0; e < H::N; ++e)
+                if (held.mine(v, e)) joined[slot * a.C + held.at[v] + e] = f[v * H::N + e];
         __syncthreads();
         for (int c = threadIdx.x; c < a.C; c += 256) {
             float s = 0;
-            for (int t = 0; t < teams; ++t) s += joined[t * width + c];
-            out[c] = (std::remove_reference_t<decltype(*out)>)s;
+            for (int t = 0; t < teams; ++t) s += joined[t * a.C + c];
+            out[c] = (Out)s;
         }
     };
 
-    for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-        const int64_t sample = unit / a.cuts, r0 = sample * a.P + (unit - sample * a.cuts) * a.per_unit, r1 = min(min(r0 + a.per_unit, (sample + 1) * a.P), a.rows);
-        float g[RES_HELD], open[RES_HELD];
-        if (KIND == GATED && a.by_sample) held.load(g, (const T *)a.gate + sample * a.C);
-        for (int64_t row = r0 + slot; row < r1; row += teams) {
-            const int64_t base = row * a.C;
-            float x[RES_HELD], n[RES_HELD], dy[RES_HELD], dh[RES_HELD];
-            held.load(x, (const T *)a.x + base);
-            if (KIND != NO_UPDATE) held.load(n, (const T *)a.u + base);
-            if (KIND == GATED && !a.by_sample) held.load(g, (const T *)a.gate + base);
-            if (a.dy) held.load(dy, (const T *)a.dy + base);
-            if (a.dh) held.load(dh, (const T *)a.dh + base);
-            const float r_u = KIND != NO_UPDATE ? a.r_u[row] : 0.0f, r_y = a.r_y[row];
-            if (KIND != NO_UPDATE) {
+    // where the workgroup stands: rows r .. r + teams - 1 of a unit's rows below r1
+    struct Step {
+        int64_t unit, sample, r, r1;
+    };
+    auto enter = [&](int64_t unit) {
+        const int64_t sample = KIND == GATED_SAMPLES ? unit / a.cuts : 0, r0 = sample * a.P + (unit - sample * a.cuts) * a.per_unit;
+        return Step{unit, sample, r0, min(min(r0 + a.per_unit, (sample + 1) * a.P), a.rows)};
+    };
+    typename H::Raw x_raw, u_raw, g_raw, dy_raw = {}, dh_raw = {};
+    float r_u_next = 0, r_y_next = 0;
+    auto ask = [&](const Step &k) {
+        const int64_t row = min(k.r + slot, a.rows - 1), base = row * a.C;
+        x_raw = held.ask((const T *)a.x + base);
+        if (KIND != NO_UPDATE) u_raw = held.ask((const T *)a.u + base);
+        if (KIND >= GATED) g_raw = held.ask((const T *)a.gate + (KIND == GATED_SAMPLES ? min(k.sample, a.samples - 1) * a.C : base));
+        if (a.dy) dy_raw = held.ask((const T *)a.dy + base);
+        if (a.dh) dh_raw = held.ask((const T *)a.dh + base);
+        if (KIND != NO_UPDATE) r_u_next = a.r_u[row];
+        r_y_next = a.r_y[row];
+    };
+    // Where a gate's row stands for a unit's rows, they add up dx n alone: dgate and dpost are that times factors of the unit.
+    float open[RES_HELD];
+    bool first = true;
+    Step k = enter(blockIdx.x);
+    ask(k);
+    while (k.unit < a.units) {
+        float x[RES_HELD], n[RES_HELD], g[RES_HELD], dy[RES_HELD], dh[RES_HELD];
+        held.take(x, x_raw);
+        if (KIND != NO_UPDATE) held.take(n, u_raw);
+        if (KIND == GATED) held.take(g, g_raw);
+        if (KIND == GATED_SAMPLES && first) {
+            held.take(open, g_raw);
 #pragma unroll
-                for (int e = 0; e < RES_HELD; ++e) {
-                    n[e] *= r_u;
-                    float b = n[e] * post[e];
-                    if (KIND == GATED) open[e] = opened(g[e], a.act), b *= open[e];
-                    x[e] += b;
-                }
-            }
-            if (a.dh) {
-                float s = 0;
+            for (int e = 0; e < RES_HELD; ++e) open[e] = opened(open[e], a.act);
+        }
+        held.take(dy, dy_raw);
+        held.take(dh, dh_raw);
+        const float r_u = r_u_next, r_y = r_y_next;
+        const Step now = k;
+        const bool last = k.r + teams >= k.r1;
+        first = last;
+        if (last) k = enter(k.unit + gridDim.x);
+        else k.r += teams;
+        ask(k);  // on its way while these rows are worked on
+        const bool there = now.r + slot < now.r1;
+        const int64_t base = (now.r + slot) * a.C;
+        if (!there) {
 #pragma unroll
-                for (int e = 0; e < RES_HELD; ++e) {
-                    x[e] *= r_y;  // m
-                    dpre[e] += dh[e] * x[e];
-                    dh[e] *= pre[e];
-                    s += dh[e] * x[e];
-                }
-                s = row_sum<WIDE>(s, a.tpr, lds) / (float)a.C;
-#pragma unroll
-                for (int e = 0; e < RES_HELD; ++e) {
-                    const float d = r_y * (dh[e] - x[e] * s);
-                    dy[e] = a.dy ? dy[e] + d : d;
-                }
-            }
-            if (a.dx) held.store((T *)a.dx + base, dy);
-            if (KIND == NO_UPDATE) continue;
-            float s = 0, dn[RES_HELD];
+            for (int e = 0; e < RES_HELD; ++e) dy[e] = dh[e] = 0;
+        }
+        if (KIND != NO_UPDATE) {
 #pragma unroll
             for (int e = 0; e < RES_HELD; ++e) {
-                const float db = KIND == GATED ? dy[e] * open[e] : dy[e];
-                dpost[e] += db * n[e];
+                n[e] *= r_u;
+                float b = n[e] * post[e];
+                if (KIND == GATED) open[e] = opened(g[e], a.act);
+                if (KIND >= GATED) b *= open[e];
+                x[e] += b;
+            }
+        }
+        float s = 0;
+        if (a.dh) {
+#pragma unroll
+            for (int e = 0; e < RES_HELD; ++e) {
+                x[e] *= r_y;  // m
+                if (there) dpre[e] += dh[e] * x[e];
+                dh[e] *= pre[e];
+                s += dh[e] * x[e];
+            }
+            s = team.sum(s) / (float)a.C;
+#pragma unroll
+            for (int e = 0; e < RES_HELD; ++e) dy[e] += r_y * (dh[e] - x[e] * s);
+        }
+        if (a.dx && there) held.store((T *)a.dx + base, dy);
+        if (KIND != NO_UPDATE) {
+            float dn[RES_HELD];
+            s = 0;
+#pragma unroll
+            for (int e = 0; e < RES_HELD; ++e) {
+                const float db = KIND >= GATED ? dy[e] * open[e] : dy[e];
+                if (there && KIND == GATED_SAMPLES) dgate[e] += dy[e] * n[e];
+                if (there && KIND != GATED_SAMPLES) dpost[e] += db * n[e];
                 dn[e] = db * post[e];
                 s += dn[e] * n[e];
                 if (KIND == GATED) {
-                    float dg = dy[e] * (n[e] * post[e]);
-                    if (a.act) dg *= open[e] * (1.0f - open[e]);
-                    if (a.by_sample) dgate[e] += dg;
-                    else open[e] = dg;
+                    open[e] = dy[e] * (n[e] * post[e]) * (a.act ? open[e] * (1.0f - open[e]) : 1.0f);
                 }
             }
-            if (KIND == GATED && !a.by_sample && a.dgate) held.store((T *)a.dgate + base, open);
+            if (KIND == GATED && a.dgate && there) held.store((T *)a.dgate + base, open);
             if (a.du) {
-                s = row_sum<WIDE>(s, a.tpr, lds) / (float)a.C;
+                s = team.sum(s) / (float)a.C;
 #pragma unroll
                 for (int e = 0; e < RES_HELD; ++e) dn[e] = r_u * (dn[e] - n[e] * s);
-                held.store((T *)a.du + base, dn);
+                if (there) held.store((T *)a.du + base, dn);
             }
-        }
-        if (KIND == GATED && a.by_sample && a.dgate) {
-            if (a.gate_slices) leave(dgate, a.gate_slices + unit * a.C);
-            else leave(dgate, (T *)a.dgate + sample * a.C);
+            if (KIND == GATED_SAMPLES && last) {
 #pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) dgate[e] = 0;
+                for (int e = 0; e < RES_HELD; ++e) {
+                    dpost[e] += dgate[e] * open[e];
+                    dgate[e] *= post[e] * (a.act ? open[e] * (1.0f - open[e]) : 1.0f);
+                }
+                if (!a.dgate) {
+                } else if (a.gate_slices) leave(dgate, a.gate_slices + now.unit * a.C);
+                else leave(dgate, (T *)a.dgate + now.sample * a.C);
+#pragma unroll
+                for (int e = 0; e < RES_HELD; ++e) dgate[e] = 0;
+            }
         }
     }
     if (a.slices) {
@@ -250,7 +348,8 @@ __device__ __forceinline__ float residual_sum_element(const ResidualRows &a, int
 
 template <typename T>
 __global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
-    __shared__ float lds[16];
+    __shared__ float lds[2][16];
+    RowTeam<true> team = {1024, lds, 0};
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t base = row * a.C, gate_base = a.by_sample ? row / a.P * a.C : base;
         float r_u = 0, s = 0;
@@ -259,14 +358,14 @@ __global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
                 const float u = (float)((const T *)a.u)[base + c];
                 s += u * u;
             }
-            r_u = norm_factor(row_sum<true>(s, 1024, lds), a.C, a.eps);
+            r_u = norm_factor(team.sum(s), a.C, a.eps);
             s = 0;
         }
         for (int c = threadIdx.x; c < a.C; c += 1024) {
             const float y = residual_sum_element<T>(a, base, gate_base, c, r_u);
             s += y * y;
         }
-        const float r_y = norm_factor(row_sum<true>(s, 1024, lds), a.C, a.eps);
+        const float r_y = norm_factor(team.sum(s), a.C, a.eps);
         for (int c = threadIdx.x; c < a.C; c += 1024) {
             const float y = residual_sum_element<T>(a, base, gate_base, c, r_u);
             if (a.u) ((T *)a.y)[base + c] = (T)y;
@@ -281,7 +380,8 @@ __global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
 
 template <typename T>
 __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
-    __shared__ float lds[16];
+    __shared__ float lds[2][16];
+    RowTeam<true> team = {1024, lds, 0};
     float *dpost = a.slices ? a.slices + (int64_t)blockIdx.x * 2 * a.C : nullptr, *dpre = dpost ? dpost + a.C : nullptr;
     if (dpost)
         for (int c = threadIdx.x; c < 2 * a.C; c += 1024) dpost[c] = 0;
@@ -296,7 +396,7 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
             if (a.dh) {
                 for (int c = threadIdx.x; c < a.C; c += 1024)
                     s1 += (float)((const T *)a.dh)[base + c] * (a.pre ? a.pre[c] : 1.0f) * (residual_sum_element<T>(a, base, gate_base, c, r_u) * r_y);
-                s1 = row_sum<true>(s1, 1024, lds) / (float)a.C;
+                s1 = team.sum(s1) / (float)a.C;
             }
             auto through = [&](int c, float &dh_m) {  // dx of channel c
                 float d = a.dy ? (float)((const T *)a.dy)[base + c] : 0.0f;
@@ -325,7 +425,7 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
                 }
             }
             if (!a.du) continue;
-            s2 = row_sum<true>(s2, 1024, lds) / (float)a.C;
+            s2 = team.sum(s2) / (float)a.C;
             for (int c = threadIdx.x; c < a.C; c += 1024) {
                 float unused;
                 const float n = (float)((const T *)a.u)[base + c] * r_u, post = (a.post ? a.post[c] : 1.0f) * a.scale;
@@ -336,21 +436,28 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
     }
 }
 
-// out[b][c] = sum over n of in[b][n][c] (rows of `stride` floats), 32 columns and 32 runs of rows a workgroup, joined in fp64
+// out[b][c] = sum over n of in[b][n][c] (columns 0 .. split - 1 to `out`, the others to `more`; either may be null), 16 columns and 64 runs of rows a workgroup, joined in fp64
 template <typename T>
-__global__ __launch_bounds__(1024) void residual_join(const float *__restrict__ in, int64_t n, int C, int64_t stride, T *__restrict__ out) {
-    __shared__ double sums[32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5;
-    const float *from = in + (int64_t)blockIdx.y * n * stride;
+__global__ __launch_bounds__(1024) void residual_join(const float *__restrict__ in, int64_t n, int columns, int split, T *__restrict__ out, T *__restrict__ more) {
+    __shared__ double sums[64][17];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
+    const float *from = in + (int64_t)blockIdx.y * n * columns + min(c, columns - 1);
     double s = 0;
-    if (c < C)
-        for (int64_t k = run; k < n; k += 32) s += from[k * stride + c];
-    sums[run][threadIdx.x & 31] = s;
+    for (int64_t k = run; k < n; k += 64 * 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = k + 64 * j < n ? from[(k + 64 * j) * columns] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    sums[run][threadIdx.x & 15] = s;
     __syncthreads();
-    if (run == 0 && c < C) {
+    if (run == 0 && c < columns) {
         s = 0;
-        for (int r = 0; r < 32; ++r) s += sums[r][threadIdx.x & 31];
-        out[(int64_t)blockIdx.y * C + c] = (T)(float)s;
+#pragma unroll 8
+        for (int r = 0; r < 64; ++r) s += sums[r][threadIdx.x & 15];
+        T *to = c < split ? out : more;
+        if (to) to[(int64_t)blockIdx.y * split + (c < split ? c : c - split)] = (T)(float)s;
     }
 }
 
@@ -395,40 +502,49 @@ ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample) {
 }
 
 template <typename T, int KIND>
-int forward(const ResidualRows &a, const ResidualPlan &p, hipStream_t st) {
-    const int64_t most = 256 * 2048 / p.threads;
-    if (a.C > RES_WIDEST) {
-        hipLaunchKernelGGL((residual_fwd_any<T>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(1024), 0, st, a);
-    } else if (p.tpr > 64) {
-        hipLaunchKernelGGL((residual_fwd<T, KIND, true>), dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(p.tpr), 0, st, a);
-    } else {
-        const int64_t blocks = (a.rows + 256 / p.tpr - 1) / (256 / p.tpr);
-        hipLaunchKernelGGL((residual_fwd<T, KIND, false>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, a);
-    }
+auto residual_fwd_of(const ResidualPlan &p, int C) {
+    constexpr int N = Vec<T>::N;
+    if (C < N) return residual_fwd<T, KIND, 256, true>;
+    if (p.tpr <= 64) return residual_fwd<T, KIND, 256, false>;
+    return p.tpr <= 512 ? residual_fwd<T, KIND, 512, false> : residual_fwd<T, KIND, 1024, false>;
+}
+
+template <typename T, int KIND>
+auto residual_bwd_of(const ResidualPlan &p, int C) {
+    constexpr int N = Vec<T>::N;
+    if (C < N) return residual_bwd<T, KIND, 256, true>;
+    if (p.tpr <= 64) return residual_bwd<T, KIND, 256, false>;
+    return p.tpr <= 512 ? residual_bwd<T, KIND, 512, false> : residual_bwd<T, KIND, 1024, false>;
+}
+
+template <typename T, int KIND>
+int forward(ResidualRows a, const ResidualPlan &p, hipStream_t st) {
+    const bool wide = p.tpr > 64;
+    const int teams = wide ? 1 : 256 / p.tpr, threads = wide ? p.tpr : 256;
+    const int64_t most = 256 * 2048 / p.threads, blocks = (a.rows + teams - 1) / teams, grid = blocks < most ? blocks : most, step = grid * teams;
+    a.step_samples = step / a.P, a.step_rows = step % a.P;
+    if (a.C > RES_WIDEST) hipLaunchKernelGGL((residual_fwd_any<T>), dim3((unsigned)grid), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((residual_fwd_of<T, KIND>(p, a.C)), dim3((unsigned)grid), dim3(threads), 0, st, a);
     return check_launch("hgq_residual_norm_fwd");
 }
 
 template <typename T, int KIND>
 int backward(const ResidualRows &a, const ResidualPlan &p, float *dpost, float *dpre, hipStream_t st) {
     const char *what = "hgq_residual_norm_bwd";
+    const bool wide = p.tpr > 64;
     if (a.C > RES_WIDEST) hipLaunchKernelGGL((residual_bwd_any<T>), dim3(p.grid), dim3(1024), 0, st, a);
-    else if (p.tpr > 64) hipLaunchKernelGGL((residual_bwd<T, KIND, true>), dim3(p.grid), dim3(p.tpr), 0, st, a);
-    else hipLaunchKernelGGL((residual_bwd<T, KIND, false>), dim3(p.grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((residual_bwd_of<T, KIND>(p, a.C)), dim3(p.grid), dim3(wide ? p.tpr : 256), 0, st, a);
     int rc = check_launch(what);
-    const unsigned columns = (unsigned)((a.C + 31) / 32);
-    if (!rc && dpost) {
-        hipLaunchKernelGGL(residual_join<float>, dim3(columns), dim3(1024), 0, st, (const float *)a.slices, (int64_t)p.grid, a.C, (int64_t)2 * a.C, dpost);
-        rc = check_launch(what);
-    }
-    if (!rc && dpre) {
-        hipLaunchKernelGGL(residual_join<float>, dim3(columns), dim3(1024), 0, st, (const float *)a.slices + a.C, (int64_t)p.grid, a.C, (int64_t)2 * a.C, dpre);
+    if (!rc && a.slices) {
+        hipLaunchKernelGGL(residual_join<float>, dim3((unsigned)((2 * (int64_t)a.C + 15) / 16)), dim3(1024), 0, st, (const float *)a.slices, (int64_t)p.grid, 2 * a.C, a.C, dpost, dpre);
         rc = check_launch(what);
     }
     if (!rc && a.gate_slices) {
         const int64_t samples = a.rows / a.P;
         for (int64_t b = 0; b < samples && !rc; b += 65535) {
             const unsigned many = (unsigned)(samples - b < 65535 ? samples - b : 65535);
-            hipLaunchKernelGGL(residual_join<T>, dim3(columns, many), dim3(1024), 0, st, (const float *)a.gate_slices + b * p.cuts * a.C, p.cuts, a.C, (int64_t)a.C, (T *)a.dgate + b * a.C);
+            hipLaunchKernelGGL(residual_join<T>, dim3((unsigned)((a.C + 15) / 16), many), dim3(1024), 0, st, (const float *)a.gate_slices + b * p.cuts * a.C, p.cuts, a.C, a.C, (T *)a.dgate + b * a.C,
+                               (T *)nullptr);
             rc = check_launch(what);
         }
     }
@@ -439,12 +555,12 @@ bool slices_of_gate(const ResidualPlan &p, int C) { return p.cuts > 1 || C > RES
 
 template <typename T>
 auto forward_of(int kind) {
-    return kind == NO_UPDATE ? forward<T, NO_UPDATE> : kind == NO_GATE ? forward<T, NO_GATE> : forward<T, GATED>;
+    return kind == NO_UPDATE ? forward<T, NO_UPDATE> : kind == NO_GATE ? forward<T, NO_GATE> : kind == GATED ? forward<T, GATED> : forward<T, GATED_SAMPLES>;
 }
 
 template <typename T>
 auto backward_of(int kind) {
-    return kind == NO_UPDATE ? backward<T, NO_UPDATE> : kind == NO_GATE ? backward<T, NO_GATE> : backward<T, GATED>;
+    return kind == NO_UPDATE ? backward<T, NO_UPDATE> : kind == NO_GATE ? backward<T, NO_GATE> : kind == GATED ? backward<T, GATED> : backward<T, GATED_SAMPLES>;
 }
 
 }  // namespace
@@ -461,8 +577,8 @@ extern "C" int hgq_residual_norm_fwd(const void *x, const void *u, const void *g
     ResidualRows a = {};
     a.x = x, a.u = u, a.gate = gate, a.post = post, a.pre = pre, a.y = y, a.h = h, a.r_u = u ? r_u : nullptr, a.r_y = r_y;
     const ResidualPlan p = residual_plan(rows, P, (int)C, false);
-    a.rows = rows, a.P = P, a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.scale = scale, a.eps = eps;
-    const int kind = !u ? NO_UPDATE : gate ? GATED : NO_GATE;
+    a.rows = rows, a.P = P, a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.samples = rows / P, a.scale = scale, a.eps = eps;
+    const int kind = !u ? NO_UPDATE : !gate ? NO_GATE : P > 1 ? GATED_SAMPLES : GATED;
     return (type == HGQ_TYPE_F32 ? forward_of<float>(kind) : type == HGQ_TYPE_BF16 ? forward_of<__bf16>(kind) : forward_of<_Float16>(kind))(a, p, (hipStream_t)stream);
 }
 
@@ -491,7 +607,7 @@ extern "C" int hgq_residual_norm_bwd(const void *dy, const void *dh, const void 
     a.r_u = (float *)r_u, a.r_y = (float *)r_y, a.slices = dpost || dpre ? workspace : nullptr;
     a.gate_slices = dgate && P > 1 && slices_of_gate(p, (int)C) ? workspace + 2 * p.grid * C : nullptr;
     a.rows = rows, a.P = P > 1 ? P : rows, a.units = p.units, a.per_unit = p.per_unit, a.cuts = p.cuts;
-    a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1 && gate, a.scale = scale, a.eps = eps;
-    const int kind = !u ? NO_UPDATE : gate ? GATED : NO_GATE;
+    a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1 && gate, a.samples = rows / P, a.scale = scale, a.eps = eps;
+    const int kind = !u ? NO_UPDATE : !gate ? NO_GATE : P > 1 ? GATED_SAMPLES : GATED;
     return (type == HGQ_TYPE_F32 ? backward_of<float>(kind) : type == HGQ_TYPE_BF16 ? backward_of<__bf16>(kind) : backward_of<_Float16>(kind))(a, p, dpost, dpre, st);
 }

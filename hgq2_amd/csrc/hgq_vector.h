@@ -45,6 +45,13 @@ __device__ __forceinline__ void store_vec(T *p, const Vec<T> &r) {
     else *(Words *)p = w;
 }
 
+// the words of an access as they arrive (kept as such until they are used: elements of 16 bits taken apart across a branch are waited for there)
+template <typename T, bool THROUGH = false>
+__device__ __forceinline__ u32x4 load_words(const T *p) {
+    using Words = typename WordsAt<sizeof(T)>::Type;
+    return THROUGH ? __builtin_nontemporal_load((const Words *)p) : *(const Words *)p;
+}
+
 // the first `n` elements of a row's last access (`fill` behind them)
 template <typename T>
 __device__ __forceinline__ Vec<T> load_part(const T *p, int n, T fill) {
