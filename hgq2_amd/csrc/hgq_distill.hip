@@ -26,6 +26,7 @@ struct DistillRows {
     const float *lse, *weight, *upstream;
     float4 *stats;   // m, a, M, b
     double *losses;  // a workgroup's sum each
+    float *loss;     // where there is one workgroup
     float2 *parts;   // maximum and sum of each part of a row
     void *dz;
     int64_t rows, z_stride;
@@ -442,7 +443,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const Dist
                 for (int r = 0; r < ROWS; ++r) loss += sums[r];
             }
         }
-        if (threadIdx.x == 0) a.losses[block] = loss;
+        if (threadIdx.x == 0) {
+            if (a.loss) *a.loss = (float)loss;  // (the only one)
+            else a.losses[block] = loss;
+        }
     }
 }
 
@@ -459,7 +463,7 @@ __global__ __launch_bounds__(1024) void distill_sum(const double *__restrict__ l
 
 namespace {
 
-constexpr int SPLIT_ROWS = 256;   // rows from which on a row has a workgroup to itself
+constexpr int SPLIT_ROWS = 128;   // rows from which on a row has a workgroup to itself (200 x 131072 bfloat16 with gradient: 37 us, in three parts 44)
 constexpr int SPLIT_PART = 4096;  // entries of a part, at least
 
 struct DistillPlan {
@@ -489,7 +493,7 @@ DistillPlan distill_plan(int64_t rows, int V, int K, bool rest, int size, bool g
     else p.tpr = !gradient || bytes <= 64 << 10 ? 256 : bytes <= 256 << 10 ? 512 : 1024, p.hold = 0;
     p.n_parts = 1, p.part = V;
     int64_t parts = 1;
-    if (rows < SPLIT_ROWS && V >= 2 * SPLIT_PART) parts = (2 * SPLIT_ROWS + rows - 1) / rows;
+    if (rows < SPLIT_ROWS && V >= 2 * SPLIT_PART) parts = (512 + rows - 1) / rows;
     if (parts > V / SPLIT_PART) parts = V / SPLIT_PART;
     if (rest && parts < (V + DISTILL_BITS - 1) / DISTILL_BITS) parts = (V + DISTILL_BITS - 1) / DISTILL_BITS;
     if (parts > 1) {
@@ -526,7 +530,7 @@ int launch(const DistillRows &a, int64_t blocks, int64_t lds, hipStream_t st, co
 template <typename T, bool REST>
 int forward(DistillRows a, const DistillPlan &p, float *loss, hipStream_t st) {
     const char *what = "hgq_distill_topk_fwd";
-    a.n_parts = p.n_parts, a.part = p.part;
+    a.n_parts = p.n_parts, a.part = p.part, a.loss = p.blocks == 1 ? loss : nullptr;
     int rc;
     if (p.n_parts > 1) {
         const int64_t blocks = a.rows * p.n_parts;
@@ -548,7 +552,7 @@ int forward(DistillRows a, const DistillPlan &p, float *loss, hipStream_t st) {
              : through      ? launch<T, 1024, REST, FROM_ROW, 0, true>(a, p.blocks, lds, st, what)
                             : launch<T, 1024, REST, FROM_ROW, 0>(a, p.blocks, lds, st, what);
     }
-    if (rc) return rc;
+    if (rc || p.blocks == 1) return rc;
     hipLaunchKernelGGL(distill_sum, dim3(1), dim3(1024), 0, st, (const double *)a.losses, p.blocks, loss);
     return check_launch(what);
 }

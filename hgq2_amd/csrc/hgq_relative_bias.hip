@@ -20,7 +20,7 @@ struct BiasShape {
     int first[BIAS_BUCKETS];  // of buckets 1 .. m - 1
     int64_t stride_b, stride_h, offset;
     const void *offsets;  // [B] (int32 or int64) or null
-    int B, H, S, TS, m, both, wide, near, chunk, chunks, tiles;
+    int B, H, S, TS, m, both, wide, near, chunk, chunks, tiles, align;
     uint32_t magic, shift;  // of the division by S
     __device__ __forceinline__ int row_of(int e) const { return (int)((__umulhi((uint32_t)e, magic) + (uint32_t)e) >> shift); }
 };
@@ -36,14 +36,18 @@ __device__ __forceinline__ int bucket_of(const BiasShape &s, const int *first, i
     return lo + (s.both && d > 0 ? s.m : 0);
 }
 
-// distance of element e of the plane, held within what an int's arithmetic takes
-__device__ __forceinline__ int distance(int i, int j, int64_t offset) {
-    const int64_t d = (int64_t)j - i - offset;
-    return (int)(d < -(1 << 30) ? -(1 << 30) : d > 1 << 30 ? 1 << 30 : d);
+// Offsets beyond all distances that there are (queries and keys: below 2^28, first distances: up to 2^30) are as good as the first such one.
+__device__ __forceinline__ int offset_of(const BiasShape &s, int b) {
+    const int64_t o = !s.offsets ? s.offset : s.wide ? ((const int64_t *)s.offsets)[b] : (int64_t)((const int32_t *)s.offsets)[b];
+    constexpr int64_t far = ((int64_t)1 << 30) + (1 << 28);
+    return (int)(o < -far ? -far : o > far ? far : o);
 }
 
-__device__ __forceinline__ int64_t offset_of(const BiasShape &s, int b) {
-    return !s.offsets ? s.offset : s.wide ? ((const int64_t *)s.offsets)[b] : (int64_t)((const int32_t *)s.offsets)[b];
+// By how many elements a plane's accesses begin early, so that a wavefront's lie in lines of its own (8 x 16 x 2047 x 2047 bfloat16: forward 513 -> 462 us, the table's
+// gradient 265 -> 222 us); s.align: elements of a line, 1 where planes lie there already, or differently in the sequences of a run.
+template <typename T>
+__device__ __forceinline__ int shift_of(const BiasShape &s, const T *plane) {
+    return (int)((uintptr_t)plane / sizeof(T) & (uintptr_t)(s.align - 1));
 }
 
 // A workgroup takes tiles t, t + stride, ... of a head's plane (256 accesses each) and a run of the batch.
@@ -62,10 +66,12 @@ __global__ __launch_bounds__(256) void relative_bias_add(const T *__restrict__ s
     __syncthreads();
     const bool beyond = s.first[s.m - 2] > s.near;
     const int64_t step = (int64_t)s.H * s.TS;
+    const int shift = TINY ? 0 : shift_of(s, out + ((int64_t)b0 * s.H + h) * s.TS);
     for (int tile = tile0; tile < s.tiles; tile += stride) {
-        const int at = (tile * 256 + (int)threadIdx.x) * N;
+        const int at = (tile * 256 + (int)threadIdx.x) * N - shift;
         if (at >= s.TS) return;
-        const int e0 = TINY ? 0 : min(at, s.TS - N), i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
+        if (at + N <= 0) continue;
+        const int e0 = TINY ? 0 : max(0, min(at, s.TS - N)), i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
         float bias[N];
         const T *from = scores + b0 * s.stride_b + h * s.stride_h + e0;
         T *to = out + ((int64_t)b0 * s.H + h) * s.TS + e0;
@@ -81,18 +87,18 @@ __global__ __launch_bounds__(256) void relative_bias_add(const T *__restrict__ s
             for (int a = 0; a < AHEAD; ++a) {
                 if (b + a >= b1) break;
                 if (b + a == b0 || s.offsets) {
-                    const int64_t offset = offset_of(s, b + a);
+                    const int offset = offset_of(s, b + a);
                     int i = i0, j = j0;
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
-                        const int d = distance(i, j, offset);
+                        const int d = j - i - offset;
                         bias[e] = by_distance[max(-s.near, min(s.near, d)) + s.near];
                         if (++j == s.S) j = 0, ++i;
                     }
                     if (beyond) {
                         i = i0, j = j0;
                         for (int e = 0; e < N; ++e) {
-                            const int d = distance(i, j, offset);
+                            const int d = j - i - offset;
                             if (abs(d) > s.near) bias[e] = table[bucket_of(s, first, d) * s.H + h];
                             if (++j == s.S) j = 0, ++i;
                         }
@@ -100,7 +106,7 @@ __global__ __launch_bounds__(256) void relative_bias_add(const T *__restrict__ s
                 }
 #pragma unroll
                 for (int e = 0; e < N; ++e) v[a].v[e] = (T)((float)v[a].v[e] + bias[e]);
-                // (the last access writes what the one before it writes, once more)
+                // (the first and the last access write some of what their neighbour writes, once more)
                 if (TINY) store_part(to + a * step, v[a], s.TS);
                 else store_vec<T, THROUGH>(to + a * step, v[a]);
             }
@@ -134,11 +140,6 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
     const int n_buckets = s.both ? 2 * s.m : s.m, threads = blockDim.x;
     int *first = (int *)(bias_lds + n_buckets * threads);
     uint8_t *near = (uint8_t *)(first + BIAS_BUCKETS);
-    for (int k = threadIdx.x; k < s.m - 1; k += threads) first[k] = s.first[k];
-    for (int k = threadIdx.x; k < n_buckets * threads; k += threads) bias_lds[k] = 0;
-    __syncthreads();
-    for (int k = threadIdx.x; k <= 2 * s.near; k += threads) near[k] = (uint8_t)bucket_of(s, first, k - s.near);
-    __syncthreads();
     const bool beyond = s.first[s.m - 2] > s.near;
     const int h = blockIdx.x / parts, w = blockIdx.x - h * parts;
     BiasRun run = {bias_lds, threads, -1, 0.0};
@@ -148,17 +149,17 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
 
     struct Step {
         int64_t item;
-        int c, tile, round;
+        int c, tile, round, shift, offset;  // (with offsets of their own, runs are of one sequence)
     };
     auto step_of = [&](int64_t item) {
-        const int c = (int)(item / groups);
-        return Step{item, c, (int)(item - (int64_t)c * groups) * TILES, 0};
+        const int c = min((int)(item / groups), s.chunks - 1);
+        return Step{item, c, (int)(item - (int64_t)c * groups) * TILES, 0, TINY ? 0 : shift_of(s, dy + (int64_t)c * s.chunk * s.stride_b + h * s.stride_h), offset_of(s, c * s.chunk)};
     };
-    auto after = [&](const Step &k) { return k.round + 1 < rounds ? Step{k.item, k.c, k.tile, k.round + 1} : step_of(k.item + parts); };
-    auto first_of = [&](const Step &k, int t) { return ((int64_t)(k.tile + t) * threads + (int)threadIdx.x) * N; };
+    auto after = [&](const Step &k) { return k.round + 1 < rounds ? Step{k.item, k.c, k.tile, k.round + 1, k.shift, k.offset} : step_of(k.item + parts); };
+    auto first_of = [&](const Step &k, int t) { return ((int64_t)(k.tile + t) * threads + (int)threadIdx.x) * N - k.shift; };
 
     auto ask = [&](const Step &k, Vec<T> *v) {  // beyond the run and the last item: what is there already, once more
-        const int b = min(k.c, s.chunks - 1) * s.chunk + k.round * SEQS, b1 = min(s.B, (min(k.c, s.chunks - 1) + 1) * s.chunk);
+        const int b = k.c * s.chunk + k.round * SEQS, b1 = min(s.B, (k.c + 1) * s.chunk);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const T *from = dy + b * s.stride_b + h * s.stride_h + max((int64_t)0, min(first_of(k, t), (int64_t)s.TS - N));
@@ -181,42 +182,53 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
         const int many = min(s.B, (k.c + 1) * s.chunk) - k.c * s.chunk - k.round * SEQS;  // sequences of this round
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
+            float f[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {  // up to eight terms pairwise in fp32, their sums in fp64
-                float f[SEQS];
+            for (int e = 0; e < N; ++e) {
+                float g[SEQS];
 #pragma unroll
-                for (int a = 0; a < SEQS; ++a) f[a] = a < many ? (float)v[t * SEQS + a].v[e] : 0.0f;
+                for (int a = 0; a < SEQS; ++a) g[a] = a < many ? (float)v[t * SEQS + a].v[e] : 0.0f;
 #pragma unroll
                 for (int d = SEQS / 2; d; d /= 2)
 #pragma unroll
-                    for (int a = 0; a < d; ++a) f[a] += f[a + d];
-                sum[e] += f[0];
+                    for (int a = 0; a < d; ++a) g[a] += g[a + d];
+                f[e] = g[0];
+                if (TILES == 1) sum[e] += g[0];
             }
             if (k.round + 1 < rounds) continue;
             const int64_t at = first_of(k, t);
-            if (at < s.TS) {
-                const int e0 = TINY ? 0 : min((int)at, s.TS - N), skip = (int)at - e0, n = TINY ? s.TS : N, i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
-                const int64_t offset = offset_of(s, k.c * s.chunk);  // (with offsets of their own, runs are of one sequence)
-                const int d0 = distance(i0, j0, offset), k0 = bucket(d0), k1 = bucket(distance(i0, j0 + N - 1, offset));
+            if (at < s.TS && at + N > 0) {
+                // elements skip .. n - 1 are this access' own
+                const int e0 = TINY ? 0 : max(0, min((int)at, s.TS - N)), skip = max(0, (int)at - e0), n = TINY ? s.TS : N + min(0, (int)at - e0), i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
+                const int d0 = j0 - i0 - k.offset, k0 = bucket(d0), k1 = bucket(d0 + N - 1);
                 if (!TINY && j0 + N <= s.S && k0 == k1) {
                     double all[N];
+                    constexpr int FOLDED = TILES == 1 ? N : N * SEQS / 8 > 1 ? N * SEQS / 8 : 1;  // sums of up to eight terms
+                    if (TILES > 1) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) all[e] = e < skip ? 0.0 : sum[e];
+                        for (int e = 0; e < N; ++e) f[e] = e < skip || e >= n ? 0.0f : f[e];
 #pragma unroll
-                    for (int d = N / 2; d; d /= 2)
+                        for (int d = N / 2; d >= FOLDED; d /= 2)
+#pragma unroll
+                            for (int e = 0; e < d; ++e) f[e] += f[e + d];
+                    }
+#pragma unroll
+                    for (int e = 0; e < FOLDED; ++e) all[e] = TILES > 1 ? (double)f[e] : e < skip || e >= n ? 0.0 : sum[e];
+#pragma unroll
+                    for (int d = FOLDED / 2; d; d /= 2)
 #pragma unroll
                         for (int e = 0; e < d; ++e) all[e] += all[e + d];
                     run.add(k0, all[0]);
                 } else {
-                    int i = i0, j = j0, of[N];
+                    int d = d0, j = j0, of[N];
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
-                        of[e] = bucket(distance(i, j, offset));
-                        if (++j == s.S) j = 0, ++i;
+                        of[e] = bucket(d++);
+                        if (++j == s.S) j = 0, d -= s.S + 1;  // the next query's first key
                     }
 #pragma unroll
                     for (int e = 0; e < N; ++e)
-                        if (e >= skip && e < n) run.add(of[e], sum[e]);
+                        if (e >= skip && e < n) run.add(of[e], TILES > 1 ? (double)f[e] : sum[e]);
                 }
             }
 #pragma unroll
@@ -226,7 +238,12 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
 
     Vec<T> even[LOADS], odd[LOADS];
     Step k = step_of(w);
-    ask(k, even);
+    ask(k, even);  // and the tables meanwhile
+    for (int e = threadIdx.x; e < s.m - 1; e += threads) first[e] = s.first[e];
+    for (int e = threadIdx.x; e < n_buckets * threads; e += threads) bias_lds[e] = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e <= 2 * s.near; e += threads) near[e] = (uint8_t)bucket_of(s, first, e - s.near);
+    __syncthreads();
     while (k.item < items) {
         const Step k1 = after(k);
         ask(k1, odd);
@@ -266,7 +283,7 @@ int check_bias(const char *what, int64_t B, int64_t H, int64_t T, int64_t S, con
     if ((both ? 2 : 1) * (int64_t)m > BIAS_BUCKETS) return fail(HGQ_ERR_UNSUPPORTED, "%s: more than %d buckets", what, BIAS_BUCKETS);
     for (int k = 0; k + 1 < m; ++k)
         if (first[k] < 1 || (k && first[k] < first[k - 1]) || first[k] > 1 << 30) return fail(HGQ_ERR_ARG, "%s: first distances of buckets must rise from 1 on, up to 2^30", what);
-    if (B > INT32_MAX || H > 1 << 20 || T > INT32_MAX || S > INT32_MAX || T * S > INT32_MAX - (1 << 16)) return fail(HGQ_ERR_UNSUPPORTED, "%s: %lld x %lld positions", what, (long long)T, (long long)S);
+    if (B > INT32_MAX || H > 1 << 20 || T >= 1 << 28 || S >= 1 << 28 || T * S > INT32_MAX - (1 << 16)) return fail(HGQ_ERR_UNSUPPORTED, "%s: %lld x %lld positions", what, (long long)T, (long long)S);
     return HGQ_OK;
 }
 
@@ -283,12 +300,21 @@ BiasShape bias_shape(int64_t B, int64_t H, int64_t T, int64_t S, const int *firs
     return s;
 }
 
-void cut(BiasShape &s, int64_t threads, int N, int64_t wanted) {  // tiles of the plane, and runs of the batch for `wanted` workgroups
-    s.tiles = (int)((s.TS + threads * N - 1) / (threads * N));
-    int64_t chunks = s.offsets ? s.B : (wanted + (int64_t)s.tiles * s.H - 1) / ((int64_t)s.tiles * s.H);
+// tiles of the plane, and runs of the batch for `wanted` workgroups; planes lie at `base`, stride_b and stride_h elements apart
+template <typename T>
+void cut(BiasShape &s, int64_t threads, int64_t wanted, const void *base, int64_t stride_b, int64_t stride_h, bool each) {
+    constexpr int N = Vec<T>::N, LINE = 128 / sizeof(T);
+    const int64_t per = threads * N, tiles = (s.TS + per - 1) / per;
+    int64_t chunks = s.offsets ? s.B : (wanted + tiles * s.H - 1) / (tiles * s.H);
     if (chunks > s.B) chunks = s.B;
+    if (each && stride_b % LINE != 0 && s.TS >= 1 << 16) chunks = s.B;
     s.chunk = (int)((s.B + chunks - 1) / chunks);
     s.chunks = (s.B + s.chunk - 1) / s.chunk;
+    const bool there = (uintptr_t)base % 128 == 0 && (s.B == 1 || stride_b % LINE == 0) && (s.H == 1 || stride_h % LINE == 0);
+    s.align = there || s.TS < 2 * LINE ? 1 : LINE;
+    while (s.chunk > 1 && s.align > 1 && stride_b % s.align != 0) s.align /= 2;
+    if (s.align < N) s.align = 1;
+    s.tiles = (int)((s.TS + s.align - 1 + per - 1) / per);
 }
 
 int sums_threads(int n) { return n <= 16 ? 256 : n <= 32 ? 128 : 64; }  // 32 KB of bins up to 64 buckets: five workgroups a compute unit
@@ -308,7 +334,7 @@ auto add_kernel(const BiasShape &s, bool through) {
 
 template <typename T>
 int add(const void *scores, const float *table, void *out, BiasShape s, hipStream_t st) {
-    cut(s, 256, Vec<T>::N, 2048);
+    cut<T>(s, 256, 2048, out, (int64_t)s.H * s.TS, s.TS, true);
     // a workgroup's table of biases takes it some 2 us: tiles in turn
     int64_t stride = ADD_WGS / ((int64_t)s.H * s.chunks) + 1;
     if (stride > s.tiles) stride = s.tiles;
@@ -335,7 +361,7 @@ int sums_of(const void *dy, double *part, int parts, int threads, const BiasShap
 template <typename T>
 int sums(const void *dy, float *dtable, double *part, BiasShape s, hipStream_t st) {
     const int n = s.both ? 2 * s.m : s.m, threads = sums_threads(n);
-    cut(s, threads, Vec<T>::N, 1024);
+    cut<T>(s, threads, 1024, dy, s.stride_b, s.stride_h, false);
     const int seqs = s.chunk >= 5 ? 8 : s.chunk >= 3 ? 4 : s.chunk, parts = sums_parts(s, threads, 8 / seqs);
     const bool tiny = s.TS < Vec<T>::N;
     int rc = (tiny        ? seqs == 8 ? sums_of<T, 8, 1, true> : seqs == 4 ? sums_of<T, 4, 2, true> : seqs == 2 ? sums_of<T, 2, 4, true> : sums_of<T, 1, 8, true>
