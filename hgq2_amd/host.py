@@ -155,5 +155,84 @@ class GroupNormalization(Layer):
         return torch.relu(y) if self.activation == 'relu' else F.silu(y) if self.activation in ('silu', 'swish') else y
 
 
-layers = SimpleNamespace(GroupNormalization=GroupNormalization, MaxPooling2D=MaxPooling2D, AveragePooling2D=AveragePooling2D, Flatten=Flatten,
+class RMSNormalization(Layer):
+    """``keras.layers.RMSNormalization`` over the trailing axis (variable ``scale``): x / sqrt(mean(x^2) + epsilon) * scale.  Full precision, not
+    quantized; inputs are float32, bfloat16 or float16 GPU tensors."""
+
+    def __init__(self, axis=-1, epsilon=1e-6, scale_initializer='ones', **kwargs):
+        super().__init__(**kwargs)
+        if not float(epsilon) >= 0:
+            raise ValueError('RMSNormalization: epsilon must not be negative')
+        self.axis, self.epsilon, self.scale_initializer, self.scale = int(axis), float(epsilon), get_initializer(scale_initializer), None
+
+    def build(self, input_shape):
+        input_shape = tuple(input_shape)
+        if not input_shape or self.axis % len(input_shape) != len(input_shape) - 1:
+            raise NotImplementedError('RMSNormalization: the trailing axis only')
+        self.scale = self.add_weight(shape=(int(input_shape[-1]),), name='scale', initializer=self.scale_initializer)
+        super().build(input_shape)
+
+    def call(self, x, training=None):
+        return ops.rms_norm(x, self.scale, self.epsilon)
+
+    def get_config(self):
+        return {'name': self.name, 'axis': self.axis, 'epsilon': self.epsilon, 'scale_initializer': self.scale_initializer}
+
+
+class ResidualBlocks(Layer):
+    """A stack of blocks that keep their input's shape (a :class:`QMultiHeadAttention`, a ``Sequential`` of dense layers) on a residual stream, with a norm ahead
+    of each and behind each::
+
+        h = norm(x) * gamma_0;   for block k:  x = x + scale * act(gate_k(h)) * norm(block_k(h)) * post_k,   h = norm(x) * gamma_(k + 1)
+
+    and the last h as the output.  Everything between two blocks is one launch each way (:func:`hgq2_amd.ops.residual_norm`); the norms are full precision, the
+    blocks quantize their inputs themselves.  ``gates``: a layer (or ``None``) for each block whose output is ``[batch, ..., channels]``, or one row
+    for each sample ``[batch, channels]``; ``gate_activation`` ``'sigmoid'`` or ``None``."""
+
+    def __init__(self, blocks, gates=None, gate_activation='sigmoid', scale=1.0, epsilon=1e-6, **kwargs):
+        super().__init__(**kwargs)
+        blocks = list(blocks)
+        if not blocks:
+            raise ValueError('ResidualBlocks: at least one block')
+        gates = [None] * len(blocks) if gates is None else list(gates)
+        if len(gates) != len(blocks):
+            raise ValueError(f'ResidualBlocks: {len(blocks)} blocks need as many gates (None for none), got {len(gates)}')
+        if gate_activation not in ops.GATE_ACTIVATIONS:
+            raise ValueError(f'ResidualBlocks: gate_activation must be one of linear, sigmoid; got {gate_activation!r}')
+        if not float(epsilon) >= 0:
+            raise ValueError('ResidualBlocks: epsilon must not be negative')
+        self.blocks = torch.nn.ModuleList(blocks)
+        self.gates = torch.nn.ModuleList([g for g in gates if g is not None])
+        self._gated = [g is not None for g in gates]
+        self.gate_activation, self.scale, self.epsilon = gate_activation, float(scale), float(epsilon)
+
+    def build(self, input_shape):
+        channels = (int(tuple(input_shape)[-1]),)
+        for k in range(len(self.blocks) + 1):
+            self.add_weight(shape=channels, name=f'gamma_{k}', initializer='ones')
+        for k in range(len(self.blocks)):
+            self.add_weight(shape=channels, name=f'post_{k}', initializer='ones')
+        super().build(input_shape)
+
+    @property
+    def same_shape_layers(self):
+        return [*self.blocks, *self.gates]
+
+    def call(self, x, training=None):
+        var = lambda name: getattr(self, f'_var_{name}')  # noqa: E731
+        h = ops.rms_norm(x, var('gamma_0'), self.epsilon)
+        gates = iter(self.gates)
+        for k, (block, gated) in enumerate(zip(self.blocks, self._gated)):
+            gate = next(gates)(h, training=training) if gated else None
+            x, h = ops.residual_norm(x, block(h, training=training), var(f'post_{k}'), var(f'gamma_{k + 1}'), gate, self.gate_activation if gated else None, self.scale,
+                                     self.epsilon)
+        return h
+
+    def get_config(self):
+        gates = iter(self.gates)
+        return {'name': self.name, 'blocks': list(self.blocks), 'gates': [next(gates) if g else None for g in self._gated], 'gate_activation': self.gate_activation,
+                'scale': self.scale, 'epsilon': self.epsilon}
+
+
+layers = SimpleNamespace(GroupNormalization=GroupNormalization, RMSNormalization=RMSNormalization, MaxPooling2D=MaxPooling2D, AveragePooling2D=AveragePooling2D, Flatten=Flatten,
                          GlobalAveragePooling1D=GlobalAveragePooling1D, Layer=Layer)

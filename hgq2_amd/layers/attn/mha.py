@@ -2,6 +2,9 @@
 value with output quantizers, attention_output), scaled dot-product scores, the table softmax, and the EBOPs of the
 two score contractions, for inputs ``[batch, seq..., features]`` of any rank attending over all sequence axes.
 
+With ``relative_buckets`` a learned bias by relative position (a variable ``relative_bias`` ``[buckets, heads]``, no part of the reference's layer) is added to the
+scores ahead of the softmax, whose table scales their sum by 1 / sqrt(key_dim); the contractions and the softmax then run as kernels of their own.
+
 Rank-3 inputs ``[batch, sequence, features]`` take the one-pass attention kernels.  With more sequence axes the
 projections run on the same dense kernels, the two score contractions on the attention contraction kernels over the
 flattened sequence axes, and the softmax over its trailing axes stage by stage."""
@@ -35,8 +38,15 @@ class QMultiHeadAttention(QLayerBase):
                  fuse='none', qkvo_iq_conf=None, qkvo_kq_conf=None, qkvo_bq_conf=None, qkvo_oq_conf=None,
                  softmax_iq_conf=None, softmax_exp_iq_conf=None, softmax_exp_oq_conf=None, softmax_inv_iq_conf=None,
                  softmax_inv_oq_conf=None, softmax_oq_conf=None, stable_softmax=True,
-                 softmax_allow_heterogeneous_table: bool = False, parallelization_factor=-1, **kwargs):
+                 softmax_allow_heterogeneous_table: bool = False, parallelization_factor=-1, relative_buckets: int = 0, relative_max_distance: int = 128,
+                 relative_bidirectional: bool = True, relative_initializer='zeros', **kwargs):
         super().__init__(**kwargs)
+        self._relative = (int(relative_buckets), int(relative_max_distance), bool(relative_bidirectional))
+        self._relative_initializer, self._relative_bias = relative_initializer, None
+        if self._relative[0]:
+            if self._relative[0] < 0 or self._relative[0] > 128 or (relative_bidirectional and self._relative[0] % 2):
+                raise ValueError(f'QMultiHeadAttention: relative_buckets must be at most 128, and even where both directions count; got {relative_buckets}')
+            ops.relative_buckets(self._relative[0] // 2 if relative_bidirectional else self._relative[0], self._relative[1])  # (refuses what cannot be)
         self._attention_axes = None if attention_axes is None else tuple(
             attention_axes if isinstance(attention_axes, (tuple, list)) else (attention_axes,))
         self._num_heads, self._key_dim = int(num_heads), int(key_dim)
@@ -73,6 +83,9 @@ class QMultiHeadAttention(QLayerBase):
                        'stable_softmax': self._stable_softmax,
                        'softmax_allow_heterogeneous_table': self._softmax_allow_heterogeneous_table,
                        'parallelization_factor': self.parallelization_factor})
+        if self._relative[0]:
+            config.update(relative_buckets=self._relative[0], relative_max_distance=self._relative[1], relative_bidirectional=self._relative[2],
+                          relative_initializer=self._relative_initializer)
         return config
 
     def _sub_kwargs(self):
@@ -134,6 +147,10 @@ class QMultiHeadAttention(QLayerBase):
         self._dot_eq, self._combine_eq, scores_rank = attention_equations(out_rank, self._attention_axes)
         q_seq, k_seq = tuple(query_shape[1:-1]), tuple(value_shape[1:-1])
         self._n_seq = len(q_seq)
+        if self._relative[0]:
+            if self._n_seq != 1:
+                raise NotImplementedError('QMultiHeadAttention: relative positions need a single sequence axis')
+            self._relative_bias = self.add_weight(name='relative_bias', shape=(self._relative[0], N), initializer=self._relative_initializer)
         self._T, self._S = math.prod(q_seq), math.prod(k_seq)
         norm_axes = tuple(range(scores_rank - len(self._attention_axes), scores_rank))
         self._softmax = QSoftmax(
@@ -228,7 +245,7 @@ class QMultiHeadAttention(QLayerBase):
         if self._inverse_sqrt_key_dim != 1.0:  # 1 after build: the scale lives in the softmax's exp table
             query = query * self._inverse_sqrt_key_dim
         flat = self._n_seq == 1
-        if FUSED and flat and not need_scores and not (self._dropout and training):
+        if FUSED and flat and self._relative_bias is None and not need_scores and not (self._dropout and training):
             # a boolean mask [1 or B, T, S] and / or the causal rule are applied inside the kernel
             m = attention_mask
             in_kernel = m is None or (m.dim() == 3 and m.dtype == torch.bool and m.shape[0] in (1, query.shape[0])
@@ -247,6 +264,8 @@ class QMultiHeadAttention(QLayerBase):
         q4, k4, v4 = (t.reshape(B, -1, N, t.shape[-1]) for t in (query, key, value))
         own = q4.is_cuda and max(q4.shape[1], k4.shape[1], q4.shape[3], v4.shape[3]) <= ops.ATTN_MAX
         scores = ops.attn_scores(q4, k4) if own else torch.einsum(_DOT_EQ, k4, q4)
+        if self._relative_bias is not None:
+            scores = ops.relative_bias(scores, self._relative_bias, self._relative[1], self._relative[2])
         scores = scores.view((B, N) + q_seq + k_seq)
         mask = None
         if attention_mask is not None:

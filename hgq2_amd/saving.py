@@ -120,7 +120,7 @@ def _registry():
     reg = {name: getattr(layers, name) for name in layers.__all__ if isinstance(getattr(layers, name), type)}
     reg.update({'Sequential': _core.Sequential, 'Quantizer': Quantizer, 'MaxPooling2D': host.MaxPooling2D,
                 'AveragePooling2D': host.AveragePooling2D, 'Flatten': host.Flatten, 'GlobalAveragePooling1D': host.GlobalAveragePooling1D,
-                'GroupNormalization': host.GroupNormalization})
+                'GroupNormalization': host.GroupNormalization, 'RMSNormalization': host.RMSNormalization, 'ResidualBlocks': host.ResidualBlocks})
     return reg
 
 
@@ -216,12 +216,11 @@ def build_for_shape(model, input_shape):
     if isinstance(model, _core.Sequential):
         for layer in model.layers:
             if isinstance(layer, _core.Layer):
-                if not layer.built:
-                    layer.build(shape)
-                    layer.built = True
-                shape = tuple(layer.compute_output_shape(shape))
+                shape = build_for_shape(layer, shape)
         model.built = True
         return shape
+    for layer in getattr(model, 'same_shape_layers', ()):  # layers that it calls on tensors of its input's shape
+        build_for_shape(layer, shape)
     if not model.built:
         model.build(shape)
         model.built = True

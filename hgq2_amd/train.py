@@ -320,13 +320,30 @@ class AdamW(SGD):
         return post
 
 
+def _each(f, y):
+    """``f`` of a batch's targets: of the tensor, or of each of several (``None`` stays)."""
+    return None if y is None else f(y) if isinstance(y, torch.Tensor) else tuple(_each(f, t) for t in y)
+
+
+def _copy_batch(to, y):
+    if isinstance(to, torch.Tensor):
+        to.copy_(y)
+        return
+    if len(to) != len(y) or any((a is None) != (b is None) for a, b in zip(to, y)):
+        raise ValueError('the targets must be as many tensors as the example had')
+    for a, b in zip(to, y):
+        if a is not None:
+            a.copy_(b)
+
+
 class GraphedTrainStep:
     """One training step (forward, loss, backward, optimizer update) captured in a HIP graph.
 
     The step is launch-bound at the layer sizes this package targets (tens of small kernels), so
     the whole sequence is recorded once on a side stream and replayed; inputs are copied into
     static buffers before each replay.  ``loss_fn(outputs, labels)`` must be built from capturable
-    operations (``hgq2_amd.ops.sparse_ce`` is)."""
+    operations (``hgq2_amd.ops.sparse_ce`` is).  The labels are a tensor or a tuple of tensors (and ``None``), as ``loss_fn``
+    takes them."""
 
     def __init__(self, model, loss_fn, optimizer: 'SGD | AdamW', example_x, example_y, warmup: int = 3, overlap: bool = True,
                  warmup_data=None, feed: 'ResidentBatches | None' = None):
@@ -342,7 +359,7 @@ class GraphedTrainStep:
         self.overlap = overlap  # EBOPs launches and the loss sum on a second branch of the graph, beside loss and backward
         self.feed = feed
         self.x = example_x.clone()
-        self.y = example_y.clone()
+        self.y = _each(torch.Tensor.clone, example_y)
         self.total = torch.zeros((), dtype=torch.float32, device=example_x.device)  # with a feed: the sum of the steps' losses
         self.loss = None
         self.warmup_losses = []
@@ -360,7 +377,7 @@ class GraphedTrainStep:
                 if len(warmup_data) < 1:
                     raise ValueError('the recording needs at least one step before it')
                 for wx, wy in warmup_data:
-                    self.x.copy_(wx), self.y.copy_(wy)
+                    self.x.copy_(wx), _copy_batch(self.y, wy)
                     self.warmup_losses.append(self._step().clone())
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
@@ -409,7 +426,7 @@ class GraphedTrainStep:
         if x is not None:
             self.x.copy_(x)
         if y is not None:
-            self.y.copy_(y)
+            _copy_batch(self.y, y)
         ops.touch_state()  # the replayed kernels update the variables
         self.graph.replay()
         return self.loss
@@ -611,14 +628,26 @@ class _FusedStep:
         return self.stack.step(x, y)
 
 
-def train_step_for(model, example_x, example_y, lr: float = 0.01, loss: str = 'sparse_ce', fused: bool | None = None,
+def _distill(outputs, y):
+    logits, indices, *more = y
+    lse, weight = (*more, None, None)[:2]
+    return ops.distill_topk(outputs, logits, indices, teacher_lse=lse, sample_weight=weight)
+
+
+_LOSSES = ('sparse_ce', 'mse', 'distill_topk')
+
+
+def train_step_for(model, example_x, example_y, lr: float = 0.01, loss='sparse_ce', fused: bool | None = None,
                    warmup_data=None, feed=None, warmup: int = 3, optimizer='sgd'):
     """A callable ``step(x, y) -> loss`` that runs one training step of ``model`` on the fastest path that covers it.
 
     A built stack of :class:`QDense` layers trained with mean sparse categorical cross-entropy and within what
     :class:`FusedQDenseStack` checks (widths up to 64, the default quantizer kinds, an LDS plan that fits) runs on the
-    whole-step kernels; every other model, and ``loss='mse'``, runs the per-layer operators replayed from a HIP graph
-    (:class:`GraphedTrainStep` with :class:`SGD`, regularizers folded into the update).  Both paths update the same
+    whole-step kernels; every other model, and every other loss, runs the per-layer operators replayed from a HIP graph
+    (:class:`GraphedTrainStep` with :class:`SGD`, regularizers folded into the update).  ``loss``: ``'sparse_ce'``, ``'mse'``, ``'distill_topk'`` - the targets
+    are a teacher's ``(logits, indices)``, or ``(logits, indices, lse, sample_weight)`` with ``None`` for what there is not
+    (:func:`hgq2_amd.ops.distill_topk`) - or a callable ``loss(outputs, y)`` of capturable operations, such as
+    ``lambda out, y: ops.distill_topk(out, *y, temperature=2.0)``.  Both paths update the same
     variables with the same arithmetic (the whole-step kernels restate the per-layer sequence), so the choice changes
     the time per step and nothing else.  ``fused=False`` forces the per-layer path, ``fused=True`` raises where the
     whole-step path does not apply.  The returned object's ``path`` is ``'fused'`` or ``'layers_graph'``.
@@ -627,8 +656,8 @@ def train_step_for(model, example_x, example_y, lr: float = 0.01, loss: str = 's
     (:class:`AdamW` with ``lr`` and Keras' other defaults) or a callable that makes one of the model's variables, for
     instance ``lambda v: AdamW(v, lr=1e-3, global_clipnorm=1.0, state_bits=8, fold_regularizers=True)``; anything but
     ``'sgd'`` runs the per-layer path, and the returned object's ``opt`` is the optimizer (its ``lr`` may change between steps)."""
-    if loss not in ('sparse_ce', 'mse'):
-        raise ValueError(f"loss must be 'sparse_ce' or 'mse', got {loss!r}")
+    if not callable(loss) and loss not in _LOSSES:
+        raise ValueError(f"loss must be 'sparse_ce', 'mse', 'distill_topk' or a callable, got {loss!r}")
     if not callable(optimizer) and optimizer not in ('sgd', 'adamw'):
         raise ValueError(f"optimizer must be 'sgd', 'adamw' or a callable that makes one of the variables, got {optimizer!r}")
     if fused and optimizer != 'sgd':
@@ -651,7 +680,7 @@ def train_step_for(model, example_x, example_y, lr: float = 0.01, loss: str = 's
                 raise
     elif fused:
         raise ValueError('the fused QDense step computes sparse categorical cross-entropy only')
-    loss_fn = ops.sparse_ce if loss == 'sparse_ce' else ops.mse
+    loss_fn = loss if callable(loss) else _distill if loss == 'distill_topk' else getattr(ops, loss)
     opt = optimizer(model.parameters()) if callable(optimizer) else (AdamW if optimizer == 'adamw' else SGD)(
         model.parameters(), lr=lr, fold_regularizers=True)
     step = GraphedTrainStep(model, loss_fn, opt, example_x, example_y, warmup=warmup, warmup_data=warmup_data, feed=feed)
@@ -670,9 +699,9 @@ def folded_regularizer_loss(model) -> float:
     return total
 
 
-def fit(model, x, y, *, loss: str = 'sparse_ce', lr: float = 0.01, batch_size: int = 1024, epochs: int = 1, callbacks=(),
+def fit(model, x, y, *, loss='sparse_ce', lr: float = 0.01, batch_size: int = 1024, epochs: int = 1, callbacks=(),
         shuffle: bool = True, seed: int | None = None, fused: bool | None = None, optimizer='sgd'):
-    """Train ``model`` on the resident tensors ``x`` / ``y`` (first axis: samples) with plain SGD - or with the ``optimizer`` that
+    """Train ``model`` on the resident tensors ``x`` / ``y`` (first axis: samples; ``y`` may be a tuple of tensors, as ``loss`` takes them) with plain SGD - or with the ``optimizer`` that
     :func:`train_step_for` is given, which makes it once, before the first batch - the way the reference's
     users call ``model.fit`` (reference tests/base.py:313-331; the epoch hooks of src/hgq/utils/sugar/ drive beta from it):
     per epoch the callbacks' ``on_epoch_begin``, the batches in order (shuffled anew per epoch with ``shuffle``; the last
@@ -689,7 +718,8 @@ def fit(model, x, y, *, loss: str = 'sparse_ce', lr: float = 0.01, batch_size: i
     (:func:`folded_regularizer_loss`, of the order of 1e-4 with the default 1e-8 factors) is added to ``logs['loss']``
     once, from the variables as they stand when the epoch ends; the whole-step kernels include it in every step."""
     n = int(x.shape[0])
-    if n < 1 or int(y.shape[0]) != n:
+    several = not isinstance(y, torch.Tensor)  # targets of several tensors: a teacher's logits and indices
+    if n < 1 or any(int(t.shape[0]) != n for t in (y if several else (y,)) if t is not None):
         raise ValueError('x and y must hold the same, non-zero number of samples')
     if not x.is_cuda:
         raise ValueError('fit trains on GPU tensors: the product has no CPU path')
@@ -705,7 +735,7 @@ def fit(model, x, y, *, loss: str = 'sparse_ce', lr: float = 0.01, batch_size: i
     step = None
     history = []
     # a data set of whole 32-bit words per row is fed by a launch inside the recorded step (no copies between replays)
-    feed = ResidentBatches(x, y) if (fused is not True and ResidentBatches.covers(x, y)) else None
+    feed = ResidentBatches(x, y) if (not several and fused is not True and ResidentBatches.covers(x, y)) else None
     for epoch in range(epochs):
         logs: dict = {}
         for cb in callbacks:
@@ -715,9 +745,9 @@ def fit(model, x, y, *, loss: str = 'sparse_ce', lr: float = 0.01, batch_size: i
         def batch(b, size=batch_size):
             lo = b * batch_size
             if order is None:
-                return x[lo:lo + size], y[lo:lo + size]
+                return x[lo:lo + size], _each(lambda t: t[lo:lo + size], y)
             idx = order[lo:lo + size]
-            return x.index_select(0, idx), y.index_select(0, idx)
+            return x.index_select(0, idx), _each(lambda t: t.index_select(0, idx), y)
 
         total = torch.zeros((), dtype=torch.float32, device=x.device)
         first = 0

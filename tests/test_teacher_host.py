@@ -181,3 +181,56 @@ def test_registered_for_fake_tensors():
         assert y.shape == h.shape == x.shape and r.shape == (12,)
         got = torch.ops.hgq.residual_norm_bwd(x, none, x, x, none, none, none, r, 1, 1.0, 1e-6, 0, True, True, False, True, False)
         assert [tuple(g.shape) for g in got] == [(2, 3, 8), (2, 3, 8), (0,), (8,), (0,)]
+
+
+@pytest.fixture
+def cpu_build():
+    from hgq2_amd.core import set_default_device
+
+    set_default_device('cpu')
+    yield
+    set_default_device(None)
+
+
+def test_layers_refuse_what_cannot_be():
+    from hgq2_amd.host import Flatten, ResidualBlocks, RMSNormalization
+    from hgq2_amd.layers import QMultiHeadAttention
+
+    with pytest.raises(ValueError, match='at least one'):
+        ResidualBlocks([])
+    with pytest.raises(ValueError, match='as many gates'):
+        ResidualBlocks([Flatten()], [None, None])
+    with pytest.raises(ValueError, match='gate_activation'):
+        ResidualBlocks([Flatten()], gate_activation='relu')
+    for make in (lambda: ResidualBlocks([Flatten()], epsilon=-1.0), lambda: RMSNormalization(epsilon=math.nan)):
+        with pytest.raises(ValueError, match='epsilon'):
+            make()
+    with pytest.raises(NotImplementedError, match='trailing'):
+        RMSNormalization(axis=1).build((2, 3, 4))
+    for kw in (dict(relative_buckets=7), dict(relative_buckets=130), dict(relative_buckets=-2)):
+        with pytest.raises(ValueError, match='relative_buckets'):
+            QMultiHeadAttention(2, 8, **kw)
+    with pytest.raises(ValueError, match='max_distance'):
+        QMultiHeadAttention(2, 8, relative_buckets=32, relative_max_distance=8)
+    with pytest.raises(ValueError, match="'distill_topk'"):
+        from hgq2_amd.train import train_step_for
+
+        train_step_for(None, None, None, loss='kl')
+
+
+def test_layers_configurations_and_variables(cpu_build):
+    from hgq2_amd.host import ResidualBlocks, RMSNormalization, layers
+    from hgq2_amd.layers import QDense, QMultiHeadAttention
+    from hgq2_amd.saving import build_for_shape, deserialize, serialize, variable_paths
+
+    assert layers.RMSNormalization is RMSNormalization
+    layer = ResidualBlocks([QMultiHeadAttention(2, 8, relative_buckets=9, relative_max_distance=30, relative_bidirectional=False, name='attention'), QDense(16, name='dense')],
+                           [None, QDense(16, name='gate')], scale=0.25, name='blocks')
+    again = deserialize(serialize(layer))
+    for made in (layer, again):
+        build_for_shape(made, (None, 5, 16))
+    paths = variable_paths(layer)
+    assert list(paths) == list(variable_paths(again)) and [tuple(t.shape) for t in paths.values()] == [tuple(t.shape) for t in variable_paths(again).values()]
+    assert tuple(paths['blocks/attention/relative_bias'].shape) == (9, 2) and {f'blocks/{n}' for n in ('gamma_0', 'gamma_1', 'gamma_2', 'post_0', 'post_1', 'gate/kernel')} <= set(paths)
+    assert again._gated == [False, True] and again.scale == 0.25 and again.blocks[0]._relative == (9, 30, False)
+    assert 'relative_buckets' not in QMultiHeadAttention(2, 8).get_config()
