@@ -20,7 +20,7 @@ struct BiasShape {
     int first[BIAS_BUCKETS];  // of buckets 1 .. m - 1
     int64_t stride_b, stride_h, offset;
     const void *offsets;  // [B] (int32 or int64) or null
-    int B, H, S, TS, m, both, wide, near, chunk, chunks, tiles, align;
+    int B, H, S, TS, m, both, wide, near, chunk, chunks, tiles, align, per, groups;  // per: threads for a plane, groups: planes (of other sequences) side by side where it takes few
     uint32_t magic, shift;  // of the division by S
     __device__ __forceinline__ int row_of(int e) const { return (int)((__umulhi((uint32_t)e, magic) + (uint32_t)e) >> shift); }
 };
@@ -66,28 +66,30 @@ __global__ __launch_bounds__(256) void relative_bias_add(const T *__restrict__ s
     __syncthreads();
     const bool beyond = s.first[s.m - 2] > s.near;
     const int64_t step = (int64_t)s.H * s.TS;
+    const int group = threadIdx.x / s.per, thread = threadIdx.x - group * s.per;
     const int shift = TINY ? 0 : shift_of(s, out + ((int64_t)b0 * s.H + h) * s.TS);
     for (int tile = tile0; tile < s.tiles; tile += stride) {
-        const int at = (tile * 256 + (int)threadIdx.x) * N - shift;
-        if (at >= s.TS) return;
+        const int at = (tile * 256 + thread) * N - shift;
+        if (at >= s.TS || group >= s.groups) return;
         if (at + N <= 0) continue;
         const int e0 = TINY ? 0 : max(0, min(at, s.TS - N)), i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
         float bias[N];
-        const T *from = scores + b0 * s.stride_b + h * s.stride_h + e0;
-        T *to = out + ((int64_t)b0 * s.H + h) * s.TS + e0;
-        for (int b = b0; b < b1; b += AHEAD) {
+        const int first_b = b0 + group;
+        for (int b = first_b; b < b1; b += AHEAD * s.groups) {
+            const T *from = scores + b * s.stride_b + h * s.stride_h + e0;
+            T *to = out + ((int64_t)b * s.H + h) * s.TS + e0;
             Vec<T> v[AHEAD];
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
-                const T *p = from + min(a, b1 - 1 - b) * s.stride_b;
+                const T *p = from + min(a * s.groups, b1 - 1 - b) * s.stride_b;
                 if (TINY) v[a] = load_part(p, s.TS, (T)0.0f);
                 else v[a] = load_vec<T, THROUGH>(p);
             }
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
-                if (b + a >= b1) break;
-                if (b + a == b0 || s.offsets) {
-                    const int offset = offset_of(s, b + a);
+                if (b + a * s.groups >= b1) break;
+                if ((a == 0 && b == first_b) || s.offsets) {
+                    const int offset = offset_of(s, b + a * s.groups);
                     int i = i0, j = j0;
 #pragma unroll
                     for (int e = 0; e < N; ++e) {
@@ -107,10 +109,9 @@ __global__ __launch_bounds__(256) void relative_bias_add(const T *__restrict__ s
 #pragma unroll
                 for (int e = 0; e < N; ++e) v[a].v[e] = (T)((float)v[a].v[e] + bias[e]);
                 // (the first and the last access write some of what their neighbour writes, once more)
-                if (TINY) store_part(to + a * step, v[a], s.TS);
-                else store_vec<T, THROUGH>(to + a * step, v[a]);
+                if (TINY) store_part(to + a * s.groups * step, v[a], s.TS);
+                else store_vec<T, THROUGH>(to + a * s.groups * step, v[a]);
             }
-            from += AHEAD * s.stride_b, to += AHEAD * step;
         }
     }
 }
@@ -143,8 +144,9 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
     const bool beyond = s.first[s.m - 2] > s.near;
     const int h = blockIdx.x / parts, w = blockIdx.x - h * parts;
     BiasRun run = {bias_lds, threads, -1, 0.0};
-    const int groups = (s.tiles + TILES - 1) / TILES, rounds = TILES > 1 ? 1 : (s.chunk + SEQS - 1) / SEQS;
-    const int64_t items = (int64_t)groups * s.chunks;
+    const int sets = (s.tiles + TILES - 1) / TILES, rounds = TILES > 1 ? 1 : (s.chunk + SEQS * s.groups - 1) / (SEQS * s.groups);
+    const int group = threadIdx.x / s.per, thread = threadIdx.x - group * s.per;
+    const int64_t items = (int64_t)sets * s.chunks;
     double sum[N] = {};
 
     struct Step {
@@ -152,20 +154,20 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
         int c, tile, round, shift, offset;  // (with offsets of their own, runs are of one sequence)
     };
     auto step_of = [&](int64_t item) {
-        const int c = min((int)(item / groups), s.chunks - 1);
-        return Step{item, c, (int)(item - (int64_t)c * groups) * TILES, 0, TINY ? 0 : shift_of(s, dy + (int64_t)c * s.chunk * s.stride_b + h * s.stride_h), offset_of(s, c * s.chunk)};
+        const int c = min((int)(item / sets), s.chunks - 1);
+        return Step{item, c, (int)(item - (int64_t)c * sets) * TILES, 0, TINY ? 0 : shift_of(s, dy + (int64_t)c * s.chunk * s.stride_b + h * s.stride_h), offset_of(s, c * s.chunk)};
     };
     auto after = [&](const Step &k) { return k.round + 1 < rounds ? Step{k.item, k.c, k.tile, k.round + 1, k.shift, k.offset} : step_of(k.item + parts); };
-    auto first_of = [&](const Step &k, int t) { return ((int64_t)(k.tile + t) * threads + (int)threadIdx.x) * N - k.shift; };
+    auto first_of = [&](const Step &k, int t) { return group >= s.groups ? (int64_t)s.TS : ((int64_t)(k.tile + t) * threads + thread) * N - k.shift; };
 
     auto ask = [&](const Step &k, Vec<T> *v) {  // beyond the run and the last item: what is there already, once more
-        const int b = k.c * s.chunk + k.round * SEQS, b1 = min(s.B, (k.c + 1) * s.chunk);
+        const int b1 = min(s.B, (k.c + 1) * s.chunk), b = min(b1 - 1, k.c * s.chunk + k.round * SEQS * s.groups + group);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const T *from = dy + b * s.stride_b + h * s.stride_h + max((int64_t)0, min(first_of(k, t), (int64_t)s.TS - N));
 #pragma unroll
             for (int a = 0; a < SEQS; ++a) {
-                const T *at = from + min(a, b1 - 1 - b) * s.stride_b;
+                const T *at = from + min(a * s.groups, b1 - 1 - b) * s.stride_b;
                 if (TINY) v[t * SEQS + a] = load_part(at, s.TS, (T)0.0f);
                 else v[t * SEQS + a] = load_vec(at);
             }
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
     };
 
     auto take = [&](const Step &k, const Vec<T> *v) {
-        const int many = min(s.B, (k.c + 1) * s.chunk) - k.c * s.chunk - k.round * SEQS;  // sequences of this round
+        const int left = min(s.B, (k.c + 1) * s.chunk) - (k.c * s.chunk + k.round * SEQS * s.groups + group);  // sequences from this thread's first one on
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             float f[N];
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
             for (int e = 0; e < N; ++e) {
                 float g[SEQS];
 #pragma unroll
-                for (int a = 0; a < SEQS; ++a) g[a] = a < many ? (float)v[t * SEQS + a].v[e] : 0.0f;
+                for (int a = 0; a < SEQS; ++a) g[a] = a * s.groups < left ? (float)v[t * SEQS + a].v[e] : 0.0f;
 #pragma unroll
                 for (int d = SEQS / 2; d; d /= 2)
 #pragma unroll
@@ -255,11 +257,13 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
     }
     run.flush();
     __syncthreads();
-    for (int k = threadIdx.x >> 6; k < n_buckets; k += threads >> 6) {
+    // a team of lanes for each bucket; neighbouring teams begin at neighbouring bins, which lie in other banks
+    const int team = min(64, max(1, threads / (1 << (32 - __clz(n_buckets - 1))))), lane = threadIdx.x & (team - 1);
+    for (int k = threadIdx.x / team; k < n_buckets; k += threads / team) {
         double v = 0;
-        for (int t = threadIdx.x & 63; t < threads; t += 64) v += bias_lds[k * threads + t];
-        v = team_sum(v, 64);
-        if ((threadIdx.x & 63) == 0) part[(int64_t)blockIdx.x * n_buckets + k] = v;
+        for (int t = lane; t < threads; t += team) v += bias_lds[k * threads + ((t + k * team) & (threads - 1))];
+        v = team_sum(v, team);
+        if (lane == 0) part[(int64_t)blockIdx.x * n_buckets + k] = v;
     }
 }
 
@@ -293,25 +297,35 @@ BiasShape bias_shape(int64_t B, int64_t H, int64_t T, int64_t S, const int *firs
     for (int k = 0; k + 1 < m; ++k) s.first[k] = first[k];
     s.B = (int)B, s.H = (int)H, s.S = (int)S, s.TS = (int)(T * S), s.m = m, s.both = both, s.offset = offset, s.offsets = offsets, s.wide = offset_bytes == 8;
     s.stride_b = stride_b, s.stride_h = stride_h;
-    s.near = first[m - 2] < BIAS_NEAR ? first[m - 2] : BIAS_NEAR;
+    // the distances whose bucket is looked up: no more than there are
+    int64_t reach = BIAS_NEAR;
+    if (!offsets && offset > -reach && offset < reach) {
+        const int64_t ahead = S - 1 - offset, behind = T - 1 + offset, most = ahead > behind ? ahead : behind;
+        reach = most < 1 ? 1 : most < reach ? most : reach;
+    }
+    s.near = (int)(first[m - 2] < reach ? first[m - 2] : reach);
     // e / S = (hi(e magic) + e) >> shift for e < 2^31, with magic = floor(2^32 (2^shift - S) / S) + 1 and 2^shift the first power of two that is not below S
     while (((int64_t)1 << s.shift) < S) ++s.shift;
     s.magic = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s.shift) - (uint64_t)S)) / (uint64_t)S + 1);
     return s;
 }
 
-// tiles of the plane, and runs of the batch for `wanted` workgroups; planes lie at `base`, stride_b and stride_h elements apart
+// Tiles of the plane, and runs of the batch for `wanted` workgroups; planes lie at `base`, stride_b and stride_h elements apart.  each: a run's sequences may lie differently
+// (and have offsets of their own).
 template <typename T>
 void cut(BiasShape &s, int64_t threads, int64_t wanted, const void *base, int64_t stride_b, int64_t stride_h, bool each) {
     constexpr int N = Vec<T>::N, LINE = 128 / sizeof(T);
     const int64_t per = threads * N, tiles = (s.TS + per - 1) / per;
-    int64_t chunks = s.offsets ? s.B : (wanted + tiles * s.H - 1) / (tiles * s.H);
-    if (chunks > s.B) chunks = s.B;
+    s.per = s.TS <= threads / 2 * N ? (s.TS + N - 1) / N : (int)threads, s.groups = (int)threads / s.per;
+    const int64_t most = ((int64_t)s.B + s.groups - 1) / s.groups;
+    int64_t chunks = (wanted + tiles * s.H - 1) / (tiles * s.H);
+    if (chunks > most) chunks = most;
+    if (s.offsets && !each) chunks = s.B;
     if (each && stride_b % LINE != 0 && s.TS >= 1 << 16) chunks = s.B;
     s.chunk = (int)((s.B + chunks - 1) / chunks);
     s.chunks = (s.B + s.chunk - 1) / s.chunk;
     const bool there = (uintptr_t)base % 128 == 0 && (s.B == 1 || stride_b % LINE == 0) && (s.H == 1 || stride_h % LINE == 0);
-    s.align = there || s.TS < 2 * LINE ? 1 : LINE;
+    s.align = there || s.groups > 1 || s.TS < 2 * LINE ? 1 : LINE;
     while (s.chunk > 1 && s.align > 1 && stride_b % s.align != 0) s.align /= 2;
     if (s.align < N) s.align = 1;
     s.tiles = (int)((s.TS + s.align - 1 + per - 1) / per);
@@ -328,7 +342,7 @@ int sums_parts(const BiasShape &s, int threads, int tiles) {
 template <typename T>
 auto add_kernel(const BiasShape &s, bool through) {
     if (s.TS < Vec<T>::N) return relative_bias_add<T, 4, false, true>;
-    if (s.chunk < 4) return through ? relative_bias_add<T, 1, true, false> : relative_bias_add<T, 1, false, false>;
+    if ((s.chunk + s.groups - 1) / s.groups < 4) return through ? relative_bias_add<T, 1, true, false> : relative_bias_add<T, 1, false, false>;
     return through ? relative_bias_add<T, 4, true, false> : relative_bias_add<T, 4, false, false>;
 }
 
@@ -361,8 +375,10 @@ int sums_of(const void *dy, double *part, int parts, int threads, const BiasShap
 template <typename T>
 int sums(const void *dy, float *dtable, double *part, BiasShape s, hipStream_t st) {
     const int n = s.both ? 2 * s.m : s.m, threads = sums_threads(n);
-    cut<T>(s, threads, 1024, dy, s.stride_b, s.stride_h, false);
-    const int seqs = s.chunk >= 5 ? 8 : s.chunk >= 3 ? 4 : s.chunk, parts = sums_parts(s, threads, 8 / seqs);
+    // a workgroup's bins and tables take it some 5 us: 16 KB of terms at least
+    const int64_t terms = (int64_t)s.B * s.H * s.TS * sizeof(T) >> 14;
+    cut<T>(s, threads, terms < 1 ? 1 : terms < 1024 ? terms : 1024, dy, s.stride_b, s.stride_h, false);
+    const int each = s.offsets ? 1 : (s.chunk + s.groups - 1) / s.groups, seqs = each >= 5 ? 8 : each >= 3 ? 4 : each, parts = sums_parts(s, threads, 8 / seqs);
     const bool tiny = s.TS < Vec<T>::N;
     int rc = (tiny        ? seqs == 8 ? sums_of<T, 8, 1, true> : seqs == 4 ? sums_of<T, 4, 2, true> : seqs == 2 ? sums_of<T, 2, 4, true> : sums_of<T, 1, 8, true>
               : seqs == 8 ? sums_of<T, 8, 1, false>

@@ -55,8 +55,8 @@ __device__ __forceinline__ float norm_factor(float sum, int C, float eps) { retu
 
 __device__ __forceinline__ float opened(float g, int act) { return act ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269502f)) : g; }
 
-// A thread's eight elements of a row.  A row's last access ends with the row: its first elements are the neighbour's again and count as zeros here.  TINY: rows of
-// less than one access.
+// A thread's eight elements of a row.  A row's last access ends with the row: its first elements are the neighbour's again, which are left out of sums and written
+// twice.  TINY: rows of less than one access.
 template <typename T, bool TINY>
 struct Held {
     static constexpr int N = Vec<T>::N, NV = RES_HELD / N;
@@ -86,7 +86,7 @@ struct Held {
         for (int v = 0; v < NV; ++v) {
             const Vec<T> w = __builtin_bit_cast(Vec<T>, r.v[v]);
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[v * N + e] = e < own[v] ? 0.0f : (float)w.v[e];
+            for (int e = 0; e < N; ++e) f[v * N + e] = (float)w.v[e];
         }
     }
     __device__ __forceinline__ void store(T *row, const float *f) const {
@@ -95,14 +95,18 @@ struct Held {
             Vec<T> r;
 #pragma unroll
             for (int e = 0; e < N; ++e) r.v[e] = (T)f[v * N + e];
-            if (!TINY && own[v] == 0) {
-                store_vec(row + at[v], r);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (e >= own[v] && at[v] + e < C) row[at[v] + e] = r.v[e];
-            }
+            if (TINY) store_part(row + at[v], r, C - at[v]);
+            else if (own[v] < N) store_vec(row + at[v], r);
         }
+    }
+    // the sum of products over this thread's own elements
+    __device__ __forceinline__ float dot(const float *f, const float *g) const {
+        float s = 0;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < N; ++e) s += e < own[v] ? 0.0f : f[v * N + e] * g[v * N + e];
+        return s;
     }
     __device__ __forceinline__ bool mine(int v, int e) const { return e >= own[v] && at[v] + e < C; }
     __device__ __forceinline__ void vector(float *f, const float *p, float scale) const {  // of channels, times `scale`
@@ -111,9 +115,7 @@ struct Held {
 #pragma unroll
             for (int e = 0; e < N; ++e) f[v * N + e] = p ? p[TINY ? min(at[v] + e, C - 1) : at[v] + e] : 1.0f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int e = 0; e < N; ++e) f[v * N + e] = mine(v, e) ? f[v * N + e] * scale : 0.0f;
+        for (int e = 0; e < RES_HELD; ++e) f[e] *= scale;
     }
 };
 
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
     ask(row);
     for (; row < a.rows; row += step) {
         const int64_t base = row * a.C;
-        float y[RES_HELD], u[RES_HELD], g[RES_HELD], s = 0;
+        float y[RES_HELD], u[RES_HELD], g[RES_HELD];
         held.take(y, x_raw);
         if (KIND != NO_UPDATE) held.take(u, u_raw);
         if (KIND >= GATED) held.take(g, g_raw);
@@ -153,10 +155,7 @@ __global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
         }
         ask(row + step);  // on its way while this row is worked on
         if (KIND != NO_UPDATE) {
-#pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) s += u[e] * u[e];
-            const float r_u = norm_factor(team.sum(s), a.C, a.eps);
-            s = 0;
+            const float r_u = norm_factor(team.sum(held.dot(u, u)), a.C, a.eps);
 #pragma unroll
             for (int e = 0; e < RES_HELD; ++e) {
                 float b = u[e] * r_u * post[e];
@@ -166,9 +165,7 @@ __global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
             if (a.r_u && lane == 0) a.r_u[row] = r_u;
             held.store((T *)a.y + base, y);
         }
-#pragma unroll
-        for (int e = 0; e < RES_HELD; ++e) s += y[e] * y[e];
-        const float r_y = norm_factor(team.sum(s), a.C, a.eps);
+        const float r_y = norm_factor(team.sum(held.dot(y, y)), a.C, a.eps);
         if (a.r_y && lane == 0) a.r_y[row] = r_y;
 #pragma unroll
         for (int e = 0; e < RES_HELD; ++e) y[e] *= r_y * pre[e];
@@ -281,30 +278,27 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
                 x[e] *= r_y;  // m
                 if (there) dpre[e] += dh[e] * x[e];
                 dh[e] *= pre[e];
-                s += dh[e] * x[e];
             }
-            s = team.sum(s) / (float)a.C;
+            s = team.sum(held.dot(dh, x)) / (float)a.C;
 #pragma unroll
             for (int e = 0; e < RES_HELD; ++e) dy[e] += r_y * (dh[e] - x[e] * s);
         }
         if (a.dx && there) held.store((T *)a.dx + base, dy);
         if (KIND != NO_UPDATE) {
             float dn[RES_HELD];
-            s = 0;
 #pragma unroll
             for (int e = 0; e < RES_HELD; ++e) {
                 const float db = KIND >= GATED ? dy[e] * open[e] : dy[e];
                 if (there && KIND == GATED_SAMPLES) dgate[e] += dy[e] * n[e];
                 if (there && KIND != GATED_SAMPLES) dpost[e] += db * n[e];
                 dn[e] = db * post[e];
-                s += dn[e] * n[e];
                 if (KIND == GATED) {
                     open[e] = dy[e] * (n[e] * post[e]) * (a.act ? open[e] * (1.0f - open[e]) : 1.0f);
                 }
             }
             if (KIND == GATED && a.dgate && there) held.store((T *)a.dgate + base, open);
             if (a.du) {
-                s = team.sum(s) / (float)a.C;
+                s = team.sum(held.dot(dn, n)) / (float)a.C;
 #pragma unroll
                 for (int e = 0; e < RES_HELD; ++e) dn[e] = r_u * (dn[e] - n[e] * s);
                 if (there) held.store((T *)a.du + base, dn);

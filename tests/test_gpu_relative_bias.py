@@ -71,7 +71,7 @@ def _run(dev, B, H, T, S, n, far, both, dtype, seed, offset=0):
 
 
 # one score; single queries and keys; odd planes; more of the batch than a run, more planes than workgroups; far distances
-SHAPES = [(1, 1, 1, 1), (3, 2, 1, 37), (2, 3, 41, 1), (1, 1, 2, 3), (5, 3, 50, 57), (64, 4, 64, 64), (9, 2, 33, 129), (2, 1, 300, 301), (1, 2, 1, 9001), (700, 1, 3, 5), (1, 5, 517, 259)]
+SHAPES = [(1, 1, 1, 1), (5000, 2, 1, 3), (1500, 3, 8, 8), (333, 2, 5, 13), (3, 2, 1, 37), (2, 3, 41, 1), (1, 1, 2, 3), (5, 3, 50, 57), (64, 4, 64, 64), (9, 2, 33, 129), (2, 1, 300, 301), (1, 2, 1, 9001), (700, 1, 3, 5), (1, 5, 517, 259)]
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
