@@ -470,18 +470,20 @@ struct ResidualPlan {
 };
 
 // by_sample: a unit has rows of one sample, whose gate's gradient it adds up
-ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample) {
+ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample, bool gated) {
     ResidualPlan p;
     p.tpr = 1;
     while (p.tpr * RES_HELD < C && p.tpr < 1024) p.tpr *= 2;
     p.threads = p.tpr > 256 ? p.tpr : 256;
     if (p.tpr > 64) p.threads = p.tpr;
     const int teams = p.tpr > 64 ? 1 : 256 / p.tpr;
-    const int64_t most = 256 * (p.threads >= 1024 ? 1 : 1024 / p.threads);
+    // Workgroups of the backward pass, each with a slice of its own: as many as are resident, fewer where a wavefront holds a row by itself (131072 x 64 float32: 512 39 us, 1024 43,
+    // 2048 48; 45930 x 333 float16 gated: 512 61, 768 58, 1024 64; 32768 x 768 bfloat16: 512 116, 1280 74, 2048 74; 32768 x 4096: 512 328, 1024 340)
+    const int64_t most = 256 * (p.threads >= 1024 ? 1 : p.threads == 512 ? 2 : p.threads == 128 ? 5 : gated ? 3 : 2);
     if (by_sample) {
         const int64_t samples = rows / P;
         p.cuts = samples < most ? (most + samples - 1) / samples : 1;
-        int64_t fewest = 8 * teams;  // rows that pay for a slice
+        const int64_t fewest = 2 * teams;  // rows that pay for a slice
         if (p.cuts > (P + fewest - 1) / fewest) p.cuts = (P + fewest - 1) / fewest;
         p.per_unit = (P + p.cuts - 1) / p.cuts;
         p.cuts = (P + p.per_unit - 1) / p.per_unit;
@@ -515,7 +517,7 @@ template <typename T, int KIND>
 int forward(ResidualRows a, const ResidualPlan &p, hipStream_t st) {
     const bool wide = p.tpr > 64;
     const int teams = wide ? 1 : 256 / p.tpr, threads = wide ? p.tpr : 256;
-    const int64_t most = 256 * 2048 / p.threads, blocks = (a.rows + teams - 1) / teams, grid = blocks < most ? blocks : most, step = grid * teams;
+    const int64_t most = 256 * 2048 / p.threads, blocks = (a.rows + teams - 1) / teams, turns = (blocks + most - 1) / most, grid = (blocks + turns - 1) / turns, step = grid * teams;
     a.step_samples = step / a.P, a.step_rows = step % a.P;
     if (a.C > RES_WIDEST) hipLaunchKernelGGL((residual_fwd_any<T>), dim3((unsigned)grid), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((residual_fwd_of<T, KIND>(p, a.C)), dim3((unsigned)grid), dim3(threads), 0, st, a);
@@ -570,7 +572,7 @@ extern "C" int hgq_residual_norm_fwd(const void *x, const void *u, const void *g
     if (!x || !h || (u && !y) || (gate && !u)) return fail(HGQ_ERR_ARG, "%s: null pointer", what);
     ResidualRows a = {};
     a.x = x, a.u = u, a.gate = gate, a.post = post, a.pre = pre, a.y = y, a.h = h, a.r_u = u ? r_u : nullptr, a.r_y = r_y;
-    const ResidualPlan p = residual_plan(rows, P, (int)C, false);
+    const ResidualPlan p = residual_plan(rows, P, (int)C, false, false);
     a.rows = rows, a.P = P, a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.samples = rows / P, a.scale = scale, a.eps = eps;
     const int kind = !u ? NO_UPDATE : !gate ? NO_GATE : P > 1 ? GATED_SAMPLES : GATED;
     return (type == HGQ_TYPE_F32 ? forward_of<float>(kind) : type == HGQ_TYPE_BF16 ? forward_of<__bf16>(kind) : forward_of<_Float16>(kind))(a, p, (hipStream_t)stream);
@@ -579,8 +581,13 @@ extern "C" int hgq_residual_norm_fwd(const void *x, const void *u, const void *g
 extern "C" int64_t hgq_residual_norm_bwd_workspace(int64_t rows, int64_t P, int64_t C, int type) {
     if (check_residual("hgq_residual_norm_bwd_workspace", rows, P, C, 1.0f, 0.0f, 0, type)) return -1;
     if (rows == 0) return 0;
-    const ResidualPlan p = residual_plan(rows, P, (int)C, P > 1);
-    return 2 * p.grid * C + (P > 1 && slices_of_gate(p, (int)C) ? p.units * C : 0);
+    int64_t most = 0;
+    for (int gated = 0; gated < 2; ++gated) {
+        const ResidualPlan p = residual_plan(rows, P, (int)C, P > 1, gated);
+        const int64_t floats = 2 * p.grid * C + (P > 1 && slices_of_gate(p, (int)C) ? p.units * C : 0);
+        most = floats > most ? floats : most;
+    }
+    return most;
 }
 
 extern "C" int hgq_residual_norm_bwd(const void *dy, const void *dh, const void *x, const void *u, const void *gate, const float *post, const float *pre,
@@ -595,7 +602,7 @@ extern "C" int hgq_residual_norm_bwd(const void *dy, const void *dh, const void 
         return dpre ? fill_f32(dpre, 0.0f, C, st) : HGQ_OK;
     }
     if (!x || !r_y || (u && !r_u) || (!dy && !dh) || !workspace || (gate && !u) || (dgate && !gate) || (!u && (du || dpost))) return fail(HGQ_ERR_ARG, "%s: null pointer", what);
-    const ResidualPlan p = residual_plan(rows, P, (int)C, P > 1);
+    const ResidualPlan p = residual_plan(rows, P, (int)C, P > 1, gate != nullptr);
     ResidualRows a = {};
     a.x = x, a.u = u, a.gate = gate, a.dy = dy, a.dh = dh, a.post = post, a.pre = pre, a.dx = dx, a.du = du, a.dgate = dgate;
     a.r_u = (float *)r_u, a.r_y = (float *)r_y, a.slices = dpost || dpre ? workspace : nullptr;
