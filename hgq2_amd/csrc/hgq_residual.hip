@@ -455,6 +455,18 @@ __global__ __launch_bounds__(1024) void residual_join(const float *__restrict__ 
     }
 }
 
+// the same for few rows, a thread for each column (32 x 4096 columns of 16 rows: 29 us by runs of rows, 5 us so)
+template <typename T>
+__global__ __launch_bounds__(256) void residual_join_few(const float *__restrict__ in, int n, int columns, T *__restrict__ out) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= columns) return;
+    const float *from = in + (int64_t)blockIdx.y * n * columns + c;
+    double s = 0;
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) s += from[(int64_t)k * columns];
+    out[(int64_t)blockIdx.y * columns + c] = (T)(float)s;
+}
+
 namespace {
 
 int check_residual(const char *what, int64_t rows, int64_t P, int64_t C, float scale, float eps, int act, int type) {
@@ -539,8 +551,10 @@ int backward(const ResidualRows &a, const ResidualPlan &p, float *dpost, float *
         const int64_t samples = a.rows / a.P;
         for (int64_t b = 0; b < samples && !rc; b += 65535) {
             const unsigned many = (unsigned)(samples - b < 65535 ? samples - b : 65535);
-            hipLaunchKernelGGL(residual_join<T>, dim3((unsigned)((a.C + 15) / 16), many), dim3(1024), 0, st, (const float *)a.gate_slices + b * p.cuts * a.C, p.cuts, a.C, a.C, (T *)a.dgate + b * a.C,
-                               (T *)nullptr);
+            const float *slices = a.gate_slices + b * p.cuts * a.C;
+            T *dgate = (T *)a.dgate + b * a.C;
+            if (p.cuts <= 64) hipLaunchKernelGGL(residual_join_few<T>, dim3((unsigned)((a.C + 255) / 256), many), dim3(256), 0, st, slices, (int)p.cuts, a.C, dgate);
+            else hipLaunchKernelGGL(residual_join<T>, dim3((unsigned)((a.C + 15) / 16), many), dim3(1024), 0, st, slices, p.cuts, a.C, a.C, dgate, (T *)nullptr);
             rc = check_launch(what);
         }
     }
