@@ -140,14 +140,15 @@ struct Piece {
         if (TPR > 8) return load_vec(z + at);
         return at + N <= end ? load_vec(z + at) : load_part(z + at, end - at, (T)-INFINITY);
     }
-    // -inf where an entry is listed (bits: of the entries from `lo` on)
+    // -inf where an entry is listed (bits: of the entries from `lo` on) or another thread's, whose list this one does not look at
     __device__ __forceinline__ void leave_listed(Vec<T> &r, const uint32_t *bits, int lo, int end) const {
         if (own == N || at >= end) return;
         const int first = at - lo;
-        uint32_t b = 0;
+        uint32_t b;
         if (own == 0) {
             b = bits[first >> 5] >> (first & 31) & ((1 << N) - 1);
         } else {
+            b = (1 << own) - 1;
             for (int e = own; e < N; ++e) b |= (bits[(first + e) >> 5] >> ((first + e) & 31) & 1) << e;
         }
         if (b) {
