@@ -142,7 +142,7 @@ struct Piece {
     }
     // -inf where an entry is listed (bits: of the entries from `lo` on) or another thread's, whose list this one does not look at
     __device__ __forceinline__ void leave_listed(Vec<T> &r, const uint32_t *bits, int lo, int end) const {
-        if (own == N || at >= end) return;
+        if (at >= end) return;
         const int first = at - lo;
         uint32_t b;
         if (own == 0) {
@@ -538,10 +538,12 @@ DistillPlan distill_plan(int64_t rows, int V, int K, bool rest, int size, bool g
 }
 
 int check_distill(const char *what, int64_t rows, int64_t V, int64_t K, double T, int type, int t_type, int index_bytes) {
-    if (rows < 0 || V < 1 || K < 1 || !(T > 0) || T > 3e38) return fail(HGQ_ERR_ARG, "%s: rows %lld, vocabulary %lld, list %lld, temperature %g", what, (long long)rows, (long long)V, (long long)K, T);
+    if (rows < 0 || V < 1 || K < 1 || !(T >= 1e-30 && T <= 1e30)) return fail(HGQ_ERR_ARG, "%s: rows %lld, vocabulary %lld, list %lld, temperature %g", what, (long long)rows, (long long)V, (long long)K, T);
     if (type < HGQ_TYPE_F32 || type > HGQ_TYPE_F16 || t_type < HGQ_TYPE_F32 || t_type > HGQ_TYPE_F16) return fail(HGQ_ERR_ARG, "%s: unknown type", what);
     if (index_bytes != 4 && index_bytes != 8) return fail(HGQ_ERR_ARG, "%s: indices of %d bytes", what, index_bytes);
     if (K > DISTILL_LIST) return fail(HGQ_ERR_UNSUPPORTED, "%s: a list of %lld entries, at most %d", what, (long long)K, DISTILL_LIST);
+    // (teams of eight are the only ones whose accesses may be cut, and the lists of 32 rows have to fit)
+    if (K > 64 && V < 8) return fail(HGQ_ERR_UNSUPPORTED, "%s: a list of %lld entries, at most 64 of a vocabulary of %lld", what, (long long)K, (long long)V);
     if (V > 1 << 30 || rows > (int64_t)1 << 40) return fail(HGQ_ERR_UNSUPPORTED, "%s: %lld rows of %lld entries", what, (long long)rows, (long long)V);
     return HGQ_OK;
 }
