@@ -584,6 +584,7 @@ extern "C" int hgq_residual_norm_fwd(const void *x, const void *u, const void *g
     int rc = check_residual(what, rows, P, C, scale, eps, act, type);
     if (rc || rows == 0) return rc;
     if (!x || !h || (u && !y) || (gate && !u)) return fail(HGQ_ERR_ARG, "%s: null pointer", what);
+    if (!gate) P = 1;
     ResidualRows a = {};
     a.x = x, a.u = u, a.gate = gate, a.post = post, a.pre = pre, a.y = y, a.h = h, a.r_u = u ? r_u : nullptr, a.r_y = r_y;
     const ResidualPlan p = residual_plan(rows, P, (int)C, false, false);
@@ -596,9 +597,10 @@ extern "C" int64_t hgq_residual_norm_bwd_workspace(int64_t rows, int64_t P, int6
     if (check_residual("hgq_residual_norm_bwd_workspace", rows, P, C, 1.0f, 0.0f, 0, type)) return -1;
     if (rows == 0) return 0;
     int64_t most = 0;
-    for (int gated = 0; gated < 2; ++gated) {
-        const ResidualPlan p = residual_plan(rows, P, (int)C, P > 1, gated);
-        const int64_t floats = 2 * p.grid * C + (P > 1 && slices_of_gate(p, (int)C) ? p.units * C : 0);
+    for (int kind = 0; kind < 3; ++kind) {  // no gate, one like x, one for a sample's rows
+        const bool by_sample = kind == 2 && P > 1;
+        const ResidualPlan p = residual_plan(rows, P, (int)C, by_sample, kind > 0);
+        const int64_t floats = 2 * p.grid * C + (by_sample && slices_of_gate(p, (int)C) ? p.units * C : 0);
         most = floats > most ? floats : most;
     }
     return most;
@@ -616,13 +618,14 @@ extern "C" int hgq_residual_norm_bwd(const void *dy, const void *dh, const void 
         return dpre ? fill_f32(dpre, 0.0f, C, st) : HGQ_OK;
     }
     if (!x || !r_y || (u && !r_u) || (!dy && !dh) || !workspace || (gate && !u) || (dgate && !gate) || (!u && (du || dpost))) return fail(HGQ_ERR_ARG, "%s: null pointer", what);
+    if (!gate) P = 1;
     const ResidualPlan p = residual_plan(rows, P, (int)C, P > 1, gate != nullptr);
     ResidualRows a = {};
     a.x = x, a.u = u, a.gate = gate, a.dy = dy, a.dh = dh, a.post = post, a.pre = pre, a.dx = dx, a.du = du, a.dgate = dgate;
     a.r_u = (float *)r_u, a.r_y = (float *)r_y, a.slices = dpost || dpre ? workspace : nullptr;
     a.gate_slices = dgate && P > 1 && slices_of_gate(p, (int)C) ? workspace + 2 * p.grid * C : nullptr;
     a.rows = rows, a.P = P > 1 ? P : rows, a.units = p.units, a.per_unit = p.per_unit, a.cuts = p.cuts;
-    a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1 && gate, a.samples = rows / P, a.scale = scale, a.eps = eps;
+    a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.samples = rows / P, a.scale = scale, a.eps = eps;
     const int kind = !u ? NO_UPDATE : !gate ? NO_GATE : P > 1 ? GATED_SAMPLES : GATED;
     return (type == HGQ_TYPE_F32 ? backward_of<float>(kind) : type == HGQ_TYPE_BF16 ? backward_of<__bf16>(kind) : backward_of<_Float16>(kind))(a, p, dpost, dpre, st);
 }

@@ -331,3 +331,16 @@ def test_recording_beside_a_living_graph_is_refused_and_gradients_are_not_differ
         d.sum().backward()
     with torch.no_grad():
         assert not ops.residual_norm(x, x, pre_gamma=p)[1].requires_grad
+
+
+def test_rows_of_a_gate_that_is_not_there(dev):
+    """The operators take the rows that a gate's row stands for as a number, which says nothing without a gate."""
+    g = torch.Generator().manual_seed(29)
+    none = torch.empty(0, device=dev)
+    for C in (40, 700, 9000):
+        x, u, dy, dh = (torch.randn(24, C, generator=g).to(dev) for _ in range(4))
+        got = []
+        for P in (1, 6):
+            y, h, r = torch.ops.hgq.residual_norm_fwd(x, u, none, none, none, P, 0.5, 1e-6, 0, True)
+            got.append([y, h, r, *torch.ops.hgq.residual_norm_bwd(dy, dh, x, u, none, none, none, r, P, 0.5, 1e-6, 0, True, True, False, True, True)])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
