@@ -287,7 +287,7 @@ int check_bias(const char *what, int64_t B, int64_t H, int64_t T, int64_t S, con
     if ((both ? 2 : 1) * (int64_t)m > BIAS_BUCKETS) return fail(HGQ_ERR_UNSUPPORTED, "%s: more than %d buckets", what, BIAS_BUCKETS);
     for (int k = 0; k + 1 < m; ++k)
         if (first[k] < 1 || (k && first[k] < first[k - 1]) || first[k] > 1 << 30) return fail(HGQ_ERR_ARG, "%s: first distances of buckets must rise from 1 on, up to 2^30", what);
-    if (B > INT32_MAX || H > 1 << 20 || T >= 1 << 28 || S >= 1 << 28 || T * S > INT32_MAX - (1 << 16)) return fail(HGQ_ERR_UNSUPPORTED, "%s: %lld x %lld positions", what, (long long)T, (long long)S);
+    if (B > 1 << 30 || H > 1 << 20 || T >= 1 << 28 || S >= 1 << 28 || T * S > INT32_MAX - (1 << 16)) return fail(HGQ_ERR_UNSUPPORTED, "%s: %lld x %lld positions", what, (long long)T, (long long)S);
     return HGQ_OK;
 }
 

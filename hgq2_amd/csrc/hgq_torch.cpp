@@ -289,7 +289,7 @@ DistillSizes distill_sizes(const Tensor &z, const Tensor &t, const Tensor &index
     TORCH_CHECK_VALUE(t.device() == z.device() && index.device() == z.device(), "logits and the teacher's list must be on one device");
     TORCH_CHECK_VALUE(t.is_contiguous() && index.is_contiguous(), "the teacher's list must be contiguous");
     numbers("teacher_lse", lse, z.size(0), z), numbers("sample_weight", weight, z.size(0), z);
-    TORCH_CHECK_VALUE(T > 0 && std::isfinite(T), "temperature must be positive, got ", T);
+    TORCH_CHECK_VALUE(T >= 1e-30 && T <= 1e30, "temperature must be positive, 1e-30 .. 1e30, got ", T);
     return {z.size(0), z.size(1), t.size(1), type_code(z.scalar_type()), type_code(t.scalar_type()), index.scalar_type() == at::kLong ? 8 : 4};
 }
 

@@ -3580,7 +3580,7 @@ def group_norm(x: Tensor, groups: int, gamma: Tensor | None = None, beta: Tensor
 def distill_topk(logits: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, temperature: float = 1.0, teacher_lse: Tensor | None = None,
                  sample_weight: Tensor | None = None) -> Tensor:
     """Mean loss of a student's ``logits`` ``[..., vocabulary]`` against the ``K`` largest logits that a teacher gave for the same rows:
-    ``teacher_logits`` and ``teacher_indices`` ``[..., K]`` (int32 or int64; K up to 1024).  With ``q = softmax(logits / T)`` a row's loss is
+    ``teacher_logits`` and ``teacher_indices`` ``[..., K]`` (int32 or int64; K up to 1024, up to 64 of a vocabulary below 8).  With ``q = softmax(logits / T)`` a row's loss is
     ``T^2 sum_k p_k (log p_k - log q[i_k])``, the divergence of the student from the teacher times the square of the ``temperature`` T, which keeps the
     gradient's size.  ``p`` is the softmax over the list, or, with ``teacher_lse`` ``[...]`` (float32: the teacher's own ``logsumexp(logits / T)`` over
     everything), its true probabilities; what both have outside the list is then one more entry, ``T^2 p' log(p' / q')``, which counts

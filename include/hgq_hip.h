@@ -1091,14 +1091,14 @@ int hgq_group_norm_bwd(const void *dy, const void *x, const float *gamma, const 
 
 /*
  * Loss of a student's logits against a teacher's top logits (beside the Keras losses that the reference's users train with), row r of
- * z [rows, V] against entries t [rows, K] at indices i [rows, K], temperature T > 0:
+ * z [rows, V] against entries t [rows, K] at indices i [rows, K], temperature T:
  *     q = softmax(z / T);   p_k = softmax(t / T) over the list, or with lse [rows] exp(t_k / T - lse), lse = the teacher's log sum exp(t / T) over its whole vocabulary
  *     loss = (1 / rows) sum_r weight_r T^2 (sum_k p_k log(p_k / q[i_k]) + p' log(p' / q'));   p' = max(0, 1 - sum p), q' outside the list (only with lse, and where q' > 0)
  * z, dz: `type`, t: `t_type` (HGQ_TYPE_*), rows of z `z_stride` elements apart, all else contiguous; indices of 4 or 8 bytes, those that are not in 0 .. V - 1 are
  * missing entries, one that comes twice counts with the sum of both.  lse, weight: NULL for none.  A row without entries, or with the weight 0, has no
  * loss and the gradient 0 (1 / rows stays).  _fwd: loss [1]; stats [rows][4] and dz [rows, V], the gradient for an upstream gradient of one, NULL = not wanted.
  * _bwd: dz for the upstream gradient upstream[0], from stats; holds_unit: dz is what _fwd left, and stays as it is where upstream[0] is 1.
- * workspace: *_workspace(...) floats at a multiple of 8 bytes (-1: bad arguments).  K up to 1024, V up to 2^30.
+ * workspace: *_workspace(...) floats at a multiple of 8 bytes (-1: bad arguments).  K up to 1024 (64 with V < 8), V up to 2^30, T 1e-30 .. 1e30.
  */
 int64_t hgq_distill_topk_workspace(int64_t rows, int64_t V, int64_t K, int rest);
 int hgq_distill_topk_fwd(const void *z, int64_t z_stride, const void *t, int t_type, const void *index, int index_bytes, const float *lse, const float *weight,

@@ -21,7 +21,7 @@ def _distill(fwd=True, z=256, z_stride=9, t=256, t_type=0, index=256, index_byte
     return lib.hgq_distill_topk_bwd(z, z_stride, t, t_type, index, index_bytes, None, None, up, stats, dz, 0, rows, V, K, T, type, None)
 
 
-@pytest.mark.parametrize('kw', [dict(rows=-1), dict(V=0), dict(K=0), dict(T=0.0), dict(T=-1.0), dict(T=math.nan), dict(T=math.inf), dict(type=3), dict(t_type=-1), dict(index_bytes=2),
+@pytest.mark.parametrize('kw', [dict(rows=-1), dict(V=0), dict(K=0), dict(T=0.0), dict(T=-1.0), dict(T=math.nan), dict(T=math.inf), dict(T=1e-31), dict(T=1e31), dict(type=3), dict(t_type=-1), dict(index_bytes=2),
                                 dict(z=None), dict(t=None), dict(index=None), dict(z_stride=-9)])
 def test_distillation_entry_points(kw):
     _refused(_distill(**kw), b'hgq_distill_topk_fwd')
@@ -33,7 +33,7 @@ def test_distillation_limits():
     _refused(_distill(ws=None), b'null')
     for k in ('up', 'stats', 'dz'):
         _refused(_distill(fwd=False, **{k: None}), b'null')
-    for kw in (dict(K=1025), dict(V=(1 << 30) + 1), dict(rows=1 << 41)):
+    for kw in (dict(K=1025), dict(K=65, V=7), dict(V=(1 << 30) + 1), dict(rows=1 << 41)):
         _refused(_distill(**kw), b'hgq_distill_topk_fwd', _lib.ERR_UNSUPPORTED)
         _refused(_distill(fwd=False, **kw), b'hgq_distill_topk_bwd', _lib.ERR_UNSUPPORTED)
         assert _lib.load().hgq_distill_topk_workspace(kw.get('rows', 3), kw.get('V', 9), kw.get('K', 2), 0) == -1
@@ -64,7 +64,7 @@ def test_bias_entry_points(kw):
 
 
 def test_bias_limits():
-    for kw in (dict(first=tuple(range(1, 65))), dict(first=tuple(range(1, 129)), both=0), dict(T=1 << 16, S=1 << 16), dict(B=1 << 31), dict(H=1 << 21)):
+    for kw in (dict(first=tuple(range(1, 65))), dict(first=tuple(range(1, 129)), both=0), dict(T=1 << 16, S=1 << 16), dict(B=(1 << 30) + 1), dict(H=1 << 21)):
         _refused(_bias(**kw), b'hgq_relative_bias_fwd', _lib.ERR_UNSUPPORTED)
         _refused(_bias(fwd=False, **kw), b'hgq_relative_bias_bwd', _lib.ERR_UNSUPPORTED)
     _refused(_bias(out=None), b'null')
