@@ -155,16 +155,18 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
     };
     auto step_of = [&](int64_t item) {
         const int c = min((int)(item / sets), s.chunks - 1);
-        return Step{item, c, (int)(item - (int64_t)c * sets) * TILES, 0, TINY ? 0 : shift_of(s, dy + (int64_t)c * s.chunk * s.stride_b + h * s.stride_h), offset_of(s, c * s.chunk)};
+        return Step{item, c, (int)min(item - (int64_t)c * sets, (int64_t)sets) * TILES, 0, TINY ? 0 : shift_of(s, dy + (int64_t)c * s.chunk * s.stride_b + h * s.stride_h), offset_of(s, c * s.chunk)};
     };
     auto after = [&](const Step &k) { return k.round + 1 < rounds ? Step{k.item, k.c, k.tile, k.round + 1, k.shift, k.offset} : step_of(k.item + parts); };
-    auto first_of = [&](const Step &k, int t) { return group >= s.groups ? (int64_t)s.TS : ((int64_t)(k.tile + t) * threads + thread) * N - k.shift; };
+    // (32 bits hold it: a plane has at most 2^31 - 2^16 elements, and the tiles behind it end less than 2^15 later)
+    auto first_of = [&](const Step &k, int t) { return group >= s.groups ? s.TS : ((k.tile + t) * threads + thread) * N - k.shift; };
 
     auto ask = [&](const Step &k, Vec<T> *v) {  // beyond the run and the last item: what is there already, once more
         const int b1 = min(s.B, (k.c + 1) * s.chunk), b = min(b1 - 1, k.c * s.chunk + k.round * SEQS * s.groups + group);
+        const T *plane = dy + b * s.stride_b + h * s.stride_h;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const T *from = dy + b * s.stride_b + h * s.stride_h + max((int64_t)0, min(first_of(k, t), (int64_t)s.TS - N));
+            const T *from = plane + max(0, min(first_of(k, t), s.TS - N));
 #pragma unroll
             for (int a = 0; a < SEQS; ++a) {
                 const T *at = from + min(a * s.groups, b1 - 1 - b) * s.stride_b;
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
             for (int e = 0; e < N; ++e) {
                 float g[SEQS];
 #pragma unroll
-                for (int a = 0; a < SEQS; ++a) g[a] = a * s.groups < left ? (float)v[t * SEQS + a].v[e] : 0.0f;
+                for (int a = 0; a < SEQS; ++a) g[a] = SEQS == 1 || a * s.groups < left ? (float)v[t * SEQS + a].v[e] : 0.0f;
 #pragma unroll
                 for (int d = SEQS / 2; d; d /= 2)
 #pragma unroll
@@ -198,24 +200,27 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
                 if (TILES == 1) sum[e] += g[0];
             }
             if (k.round + 1 < rounds) continue;
-            const int64_t at = first_of(k, t);
-            if (at < s.TS && at + N > 0) {
+            const int at = first_of(k, t);
+            if (at < s.TS && at > -N && (SEQS > 1 || left > 0)) {
                 // elements skip .. n - 1 are this access' own
-                const int e0 = TINY ? 0 : max(0, min((int)at, s.TS - N)), skip = max(0, (int)at - e0), n = TINY ? s.TS : N + min(0, (int)at - e0), i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
+                const int e0 = TINY ? 0 : max(0, min(at, s.TS - N)), skip = max(0, at - e0), n = TINY ? s.TS : N + min(0, at - e0), i0 = s.row_of(e0), j0 = e0 - i0 * s.S;
                 const int d0 = j0 - i0 - k.offset, k0 = bucket(d0), k1 = bucket(d0 + N - 1);
                 if (!TINY && j0 + N <= s.S && k0 == k1) {
                     double all[N];
                     constexpr int FOLDED = TILES == 1 ? N : N * SEQS / 8 > 1 ? N * SEQS / 8 : 1;  // sums of up to eight terms
-                    if (TILES > 1) {
+                    if (skip > 0 || n < N) {  // (a plane's first or last access)
 #pragma unroll
-                        for (int e = 0; e < N; ++e) f[e] = e < skip || e >= n ? 0.0f : f[e];
+                        for (int e = 0; e < N; ++e)
+                            if (e < skip || e >= n) f[e] = 0.0f, sum[e] = 0.0;
+                    }
+                    if (TILES > 1) {
 #pragma unroll
                         for (int d = N / 2; d >= FOLDED; d /= 2)
 #pragma unroll
                             for (int e = 0; e < d; ++e) f[e] += f[e + d];
                     }
 #pragma unroll
-                    for (int e = 0; e < FOLDED; ++e) all[e] = TILES > 1 ? (double)f[e] : e < skip || e >= n ? 0.0 : sum[e];
+                    for (int e = 0; e < FOLDED; ++e) all[e] = TILES > 1 ? (double)f[e] : sum[e];
 #pragma unroll
                     for (int d = FOLDED / 2; d; d /= 2)
 #pragma unroll
