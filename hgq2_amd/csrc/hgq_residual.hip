@@ -33,21 +33,25 @@ struct ResidualRows {
     float scale, eps;
 };
 
-// The threads of a row: neighbouring lanes of a wavefront, or (WIDE) a workgroup.  Sums of a workgroup take turns with two places in LDS: whoever writes one
-// again is behind the barrier of the sum between.
+// The threads of a row: neighbouring lanes of a wavefront, or (WIDE) a workgroup of as many wavefronts as it needs.  Sums of a workgroup take turns with two places in LDS:
+// whoever writes one again is behind the barrier of the sum between.
 template <bool WIDE>
 struct RowTeam {
     int tpr;
     float (*lds)[16];
-    int turn;
+    int turn, slots;  // wavefronts, up to the next power of two
+    __device__ __forceinline__ RowTeam(int tpr, float (*lds)[16]) : tpr(tpr), lds(lds), turn(0), slots(1) {
+        if (!WIDE) return;
+        while (slots < tpr >> 6) slots *= 2;
+        if (threadIdx.x < 16 && threadIdx.x >= tpr >> 6) lds[0][threadIdx.x] = lds[1][threadIdx.x] = 0.0f;  // (visible behind the first sum's barrier)
+    }
     __device__ __forceinline__ float sum(float v) {
         if (!WIDE) return team_sum(v, tpr);
         v = team_sum(v, 64);
         float *at = lds[turn ^= 1];
         if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
         __syncthreads();
-        const int waves = tpr >> 6;
-        return team_sum(at[threadIdx.x & (waves - 1)], waves);
+        return team_sum(at[threadIdx.x & (slots - 1)], slots);
     }
 };
 
@@ -128,7 +132,7 @@ __global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
     using H = Held<T, TINY>;
     const int teams = WIDE ? 1 : 256 / a.tpr, slot = WIDE ? 0 : threadIdx.x / a.tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (a.tpr - 1);
     const H held(lane, a.tpr, a.C);
-    RowTeam<WIDE> team = {a.tpr, lds, 0};
+    RowTeam<WIDE> team(a.tpr, lds);
     float post[RES_HELD], pre[RES_HELD];
     if (KIND != NO_UPDATE) held.vector(post, a.post, a.scale);
     held.vector(pre, a.pre, 1.0f);
@@ -181,7 +185,7 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
     using H = Held<T, TINY>;
     const int teams = WIDE ? 1 : 256 / a.tpr, slot = WIDE ? 0 : threadIdx.x / a.tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (a.tpr - 1);
     const H held(lane, a.tpr, a.C);
-    RowTeam<WIDE> team = {a.tpr, lds, 0};
+    RowTeam<WIDE> team(a.tpr, lds);
     // What a thread keeps from row to row of its columns' post, pre, dpost and dpre.  With 1024 threads, which have 128 registers each, it lies in LDS, where no other
     // thread looks at it (8192 x 8192 bfloat16, a gate like x: 233 us instead of 330 with 32 registers spilled).
     constexpr bool STASH = THREADS == 1024 && KIND != NO_UPDATE;
@@ -387,7 +391,7 @@ __device__ __forceinline__ float residual_sum_element(const ResidualRows &a, int
 template <typename T>
 __global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
     __shared__ float lds[2][16];
-    RowTeam<true> team = {1024, lds, 0};
+    RowTeam<true> team(1024, lds);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t base = row * a.C, gate_base = a.by_sample ? row / a.P * a.C : base;
         float r_u = 0, s = 0;
@@ -419,7 +423,7 @@ __global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
 template <typename T>
 __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
     __shared__ float lds[2][16];
-    RowTeam<true> team = {1024, lds, 0};
+    RowTeam<true> team(1024, lds);
     float *dpost = a.slices ? a.slices + (int64_t)blockIdx.x * 2 * a.C : nullptr, *dpre = dpost ? dpost + a.C : nullptr;
     if (dpost)
         for (int c = threadIdx.x; c < 2 * a.C; c += 1024) dpost[c] = 0;
@@ -529,13 +533,14 @@ struct ResidualPlan {
 ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample, bool gated) {
     ResidualPlan p;
     p.tpr = 1;
-    while (p.tpr * RES_HELD < C && p.tpr < 1024) p.tpr *= 2;
+    while (p.tpr * RES_HELD < C && p.tpr < 64) p.tpr *= 2;
+    if (p.tpr * RES_HELD < C) p.tpr = C > RES_WIDEST ? 1024 : (C + 64 * RES_HELD - 1) / (64 * RES_HELD) * 64;
     p.threads = p.tpr > 256 ? p.tpr : 256;
     if (p.tpr > 64) p.threads = p.tpr;
     const int teams = p.tpr > 64 ? 1 : 256 / p.tpr;
     // Workgroups of the backward pass, each with a slice of its own: as many as are resident, fewer where a wavefront holds a row by itself (131072 x 64 float32: 512 39 us, 1024 43,
     // 2048 48; 45930 x 333 float16 gated: 512 61, 768 58, 1024 64; 32768 x 768 bfloat16: 512 116, 1280 74, 2048 74; 32768 x 4096: 512 328, 1024 340)
-    const int64_t most = 256 * (p.threads >= 1024 ? 1 : p.threads == 512 ? 2 : p.threads == 128 ? 5 : gated ? 3 : 2);
+    const int64_t most = 256 * (p.threads > 512 ? 1 : p.threads > 256 ? 2 : p.threads == 128 ? 5 : gated ? 3 : 2);
     if (by_sample) {
         const int64_t samples = rows / P;
         p.cuts = samples < most ? (most + samples - 1) / samples : 1;

@@ -127,9 +127,9 @@ def _run(dev, shape, dtype, gate, act, seed, scale=0.75, eps=1e-6, gammas=True):
         assert all(torch.equal(a, b) for a, b in zip(ops.residual_norm(leaves[0], leaves[1], leaves[3], leaves[4], leaves[2], act, scale, eps), (y, h)))
 
 
-# one channel; teams of 1 to 64 threads, of workgroups of 128 to 1024, at their borders; odd rows; rows that no workgroup holds; many and few of them
+# one channel; teams of 1 to 64 threads, of 2 to 16 wavefronts, at their borders; odd rows; rows that no workgroup holds; many and few of them
 SHAPES = [(1, 1), (3, 2), (700, 7), (5, 8), (6, 3, 9), (4, 33), (2, 300, 64), (31, 30, 48), (2, 3, 5, 100), (17, 333), (40, 512), (9, 513), (3, 7, 1000), (12, 1025), (5, 2049), (2, 4, 4096), (3, 4099),
-          (4, 8192), (2, 2, 8193), (3, 9001), (1, 20000), (4000, 16), (300, 1024)]
+          (3, 7000), (4, 8192), (2, 2, 8193), (3, 9001), (1, 20000), (4000, 16), (300, 1024)]
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
@@ -146,6 +146,12 @@ def test_against_64_bits(dev, shape, dtype):
 @pytest.mark.parametrize('shape', [(5, 70, 40), (3, 2, 9, 200), (2, 500, 16), (1500, 3, 24), (2, 40, 1300), (2, 3, 8200), (1, 1, 12)])
 def test_gates(dev, shape, act, gate):
     _run(dev, shape, torch.float32, gate, act, len(shape) * 5 + sum(shape))
+
+
+@pytest.mark.parametrize('gate', ['none', 'element', 'sample'])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_several_rows_of_a_workgroup_that_keeps_its_sums_in_lds(dev, dtype, gate):
+    _run(dev, (2, 300, 4600), dtype, gate, 'sigmoid', 31)
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
