@@ -30,7 +30,7 @@ struct ResidualRows {
     int64_t samples;                         // rows of a gate for P rows
     int64_t rows, P, units, per_unit, cuts;  // rows; of a gate's row; what a workgroup takes at a time, its rows; units of a sample
     int C, tpr, act, by_sample;
-    float scale, eps;
+    float scale, eps, inv_c;
 };
 
 // The threads of a row: neighbouring lanes of a wavefront, or (WIDE) a workgroup of as many wavefronts as it needs.  Sums of a workgroup take turns with two places in LDS:
@@ -55,7 +55,9 @@ struct RowTeam {
     }
 };
 
-__device__ __forceinline__ float norm_factor(float sum, int C, float eps) { return 1.0f / sqrtf(sum / (float)C + eps); }
+// (the hardware's root, a unit in the last place off, and a product with 1 / C: rounded ones are a fifth of a short row's instructions; 1531 x 30 x 333 float16 with a gate: 37 and 57 us
+// with them, 34 and 56 so)
+__device__ __forceinline__ float norm_factor(float sum, float inv_c, float eps) { return __builtin_amdgcn_rsqf(sum * inv_c + eps); }
 
 __device__ __forceinline__ float opened(float g, int act) { return act ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269502f)) : g; }
 
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
         }
         ask(row + step);  // on its way while this row is worked on
         if (KIND != NO_UPDATE) {
-            const float r_u = norm_factor(team.sum(held.dot(u, u)), a.C, a.eps);
+            const float r_u = norm_factor(team.sum(held.dot(u, u)), a.inv_c, a.eps);
 #pragma unroll
             for (int e = 0; e < RES_HELD; ++e) {
                 float b = u[e] * r_u * post[e];
@@ -169,7 +171,7 @@ __global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
             if (a.r_u && lane == 0) a.r_u[row] = r_u;
             held.store((T *)a.y + base, y);
         }
-        const float r_y = norm_factor(team.sum(held.dot(y, y)), a.C, a.eps);
+        const float r_y = norm_factor(team.sum(held.dot(y, y)), a.inv_c, a.eps);
         if (a.r_y && lane == 0) a.r_y[row] = r_y;
 #pragma unroll
         for (int e = 0; e < RES_HELD; ++e) y[e] *= r_y * pre[e];
@@ -320,7 +322,7 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
                 dh[e] *= pre[e];
             }
             keep(DPRE, dpre);
-            s = team.sum(held.dot(dh, x)) / (float)a.C;
+            s = team.sum(held.dot(dh, x)) * a.inv_c;
 #pragma unroll
             for (int e = 0; e < RES_HELD; ++e) dy[e] += r_y * (dh[e] - x[e] * s);
         }
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
             if (KIND != GATED_SAMPLES) keep(DPOST, dpost);
             if (KIND == GATED && a.dgate && there) held.store((T *)a.dgate + base, open);
             if (a.du) {
-                s = team.sum(held.dot(dn, n)) / (float)a.C;
+                s = team.sum(held.dot(dn, n)) * a.inv_c;
 #pragma unroll
                 for (int e = 0; e < RES_HELD; ++e) dn[e] = r_u * (dn[e] - n[e] * s);
                 if (there) held.store((T *)a.du + base, dn);
@@ -400,14 +402,14 @@ __global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
                 const float u = (float)((const T *)a.u)[base + c];
                 s += u * u;
             }
-            r_u = norm_factor(team.sum(s), a.C, a.eps);
+            r_u = norm_factor(team.sum(s), a.inv_c, a.eps);
             s = 0;
         }
         for (int c = threadIdx.x; c < a.C; c += 1024) {
             const float y = residual_sum_element<T>(a, base, gate_base, c, r_u);
             s += y * y;
         }
-        const float r_y = norm_factor(team.sum(s), a.C, a.eps);
+        const float r_y = norm_factor(team.sum(s), a.inv_c, a.eps);
         for (int c = threadIdx.x; c < a.C; c += 1024) {
             const float y = residual_sum_element<T>(a, base, gate_base, c, r_u);
             if (a.u) ((T *)a.y)[base + c] = (T)y;
@@ -438,7 +440,7 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
             if (a.dh) {
                 for (int c = threadIdx.x; c < a.C; c += 1024)
                     s1 += (float)((const T *)a.dh)[base + c] * (a.pre ? a.pre[c] : 1.0f) * (residual_sum_element<T>(a, base, gate_base, c, r_u) * r_y);
-                s1 = team.sum(s1) / (float)a.C;
+                s1 = team.sum(s1) * a.inv_c;
             }
             auto through = [&](int c, float &dh_m) {  // dx of channel c
                 float d = a.dy ? (float)((const T *)a.dy)[base + c] : 0.0f;
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
                 }
             }
             if (!a.du) continue;
-            s2 = team.sum(s2) / (float)a.C;
+            s2 = team.sum(s2) * a.inv_c;
             for (int c = threadIdx.x; c < a.C; c += 1024) {
                 float unused;
                 const float n = (float)((const T *)a.u)[base + c] * r_u, post = (a.post ? a.post[c] : 1.0f) * a.scale;
@@ -637,7 +639,7 @@ extern "C" int hgq_residual_norm_fwd(const void *x, const void *u, const void *g
     ResidualRows a = {};
     a.x = x, a.u = u, a.gate = gate, a.post = post, a.pre = pre, a.y = y, a.h = h, a.r_u = u ? r_u : nullptr, a.r_y = r_y;
     const ResidualPlan p = residual_plan(rows, P, (int)C, false, false);
-    a.rows = rows, a.P = P, a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.samples = rows / P, a.scale = scale, a.eps = eps;
+    a.rows = rows, a.P = P, a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.samples = rows / P, a.scale = scale, a.eps = eps, a.inv_c = (float)(1.0 / (double)C);
     const int kind = !u ? NO_UPDATE : !gate ? NO_GATE : P > 1 ? GATED_SAMPLES : GATED;
     return (type == HGQ_TYPE_F32 ? forward_of<float>(kind) : type == HGQ_TYPE_BF16 ? forward_of<__bf16>(kind) : forward_of<_Float16>(kind))(a, p, (hipStream_t)stream);
 }
@@ -674,7 +676,7 @@ extern "C" int hgq_residual_norm_bwd(const void *dy, const void *dh, const void 
     a.r_u = (float *)r_u, a.r_y = (float *)r_y, a.slices = dpost || dpre ? workspace : nullptr;
     a.gate_slices = dgate && P > 1 && slices_of_gate(p, (int)C) ? workspace + 2 * p.grid * C : nullptr;
     a.rows = rows, a.P = P > 1 ? P : rows, a.units = p.units, a.per_unit = p.per_unit, a.cuts = p.cuts;
-    a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.samples = rows / P, a.scale = scale, a.eps = eps;
+    a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.samples = rows / P, a.scale = scale, a.eps = eps, a.inv_c = (float)(1.0 / (double)C);
     const int kind = !u ? NO_UPDATE : !gate ? NO_GATE : P > 1 ? GATED_SAMPLES : GATED;
     return (type == HGQ_TYPE_F32 ? backward_of<float>(kind) : type == HGQ_TYPE_BF16 ? backward_of<__bf16>(kind) : backward_of<_Float16>(kind))(a, p, dpost, dpre, st);
 }
