@@ -57,7 +57,11 @@ struct RowTeam {
 
 // (the hardware's root, a unit in the last place off, and a product with 1 / C: rounded ones are a fifth of a short row's instructions; 1531 x 30 x 333 float16 with a gate: 37 and 57 us
 // with them, 34 and 56 so)
-__device__ __forceinline__ float norm_factor(float sum, float inv_c, float eps) { return __builtin_amdgcn_rsqf(sum * inv_c + eps); }
+__device__ __forceinline__ float norm_factor(float sum, float inv_c, float eps) {
+    const float square = sum * inv_c + eps;
+    const bool tiny = square < 0x1p-100f;  // (without an epsilon: the root takes numbers below fp32's normal ones for zero)
+    return __builtin_amdgcn_rsqf(tiny ? square * 0x1p100f : square) * (tiny ? 0x1p50f : 1.0f);
+}
 
 __device__ __forceinline__ float opened(float g, int act) { return act ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269502f)) : g; }
 

@@ -255,6 +255,8 @@ def test_rows_of_zeros_and_large_rows(dev):
     assert not y.any() and not h.any()
     y, h = ops.residual_norm(x, x, epsilon=0.0)  # 0 / 0
     assert y.isnan().all() and h.isnan().all()
+    small = torch.full((2, 64), 2.0**-66, device=dev)  # squares below fp32's normal numbers, of a few bits each, here exact
+    assert torch.equal(ops.rms_norm(small, epsilon=0.0), torch.ones_like(small))
     big = torch.full((2, 64), 2.0**15, dtype=torch.float16, device=dev)  # squares beyond fp16
     assert torch.equal(ops.rms_norm(big), torch.ones_like(big))
     x[1, 3] = float('nan')
