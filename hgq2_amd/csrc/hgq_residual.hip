@@ -584,7 +584,8 @@ template <typename T, int KIND>
 int forward(ResidualRows a, const ResidualPlan &p, hipStream_t st) {
     const bool wide = p.tpr > 64;
     const int teams = wide ? 1 : 256 / p.tpr, threads = wide ? p.tpr : 256;
-    const int64_t most = 256 * 2048 / p.threads, blocks = (a.rows + teams - 1) / teams, turns = (blocks + most - 1) / most, grid = (blocks + turns - 1) / turns, step = grid * teams;
+    // five workgroups of 256 a compute unit, what is resident with the most registers (1531 x 30 x 333 float16 with a gate, read anew: 40 us, eight 44; without 33 and 37)
+    const int64_t most = 256 * 1280 / p.threads, blocks = (a.rows + teams - 1) / teams, turns = (blocks + most - 1) / most, grid = (blocks + turns - 1) / turns, step = grid * teams;
     a.step_samples = step / a.P, a.step_rows = step % a.P;
     if (a.C > RES_WIDEST) hipLaunchKernelGGL((residual_fwd_any<T>), dim3((unsigned)grid), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((residual_fwd_of<T, KIND>(p, a.C)), dim3((unsigned)grid), dim3(threads), 0, st, a);
