@@ -584,8 +584,9 @@ template <typename T, int KIND>
 int forward(ResidualRows a, const ResidualPlan &p, hipStream_t st) {
     const bool wide = p.tpr > 64;
     const int teams = wide ? 1 : 256 / p.tpr, threads = wide ? p.tpr : 256;
-    // five workgroups of 256 a compute unit, what is resident with the most registers (1531 x 30 x 333 float16 with a gate, read anew: 40 us, eight 44; without 33 and 37)
-    const int64_t most = 256 * 1280 / p.threads, blocks = (a.rows + teams - 1) / teams, turns = (blocks + most - 1) / most, grid = (blocks + turns - 1) / turns, step = grid * teams;
+    // threads a compute unit, all of them resident: five workgroups of 256 where wavefronts hold rows by themselves (1531 x 30 x 333 float16 with a gate, read anew: 40 us, four
+    // 43, eight 44), 1024 where workgroups do (32768 x 4096 bfloat16 with a gate for samples 213 us, 1280 238, 2048 215; 8192 x 8192 102, 138, 107)
+    const int64_t most = 256 * (wide ? 1024 : 1280) / p.threads, blocks = (a.rows + teams - 1) / teams, turns = (blocks + most - 1) / most, grid = (blocks + turns - 1) / turns, step = grid * teams;
     a.step_samples = step / a.P, a.step_rows = step % a.P;
     if (a.C > RES_WIDEST) hipLaunchKernelGGL((residual_fwd_any<T>), dim3((unsigned)grid), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((residual_fwd_of<T, KIND>(p, a.C)), dim3((unsigned)grid), dim3(threads), 0, st, a);
