@@ -9,6 +9,8 @@
 // are listed (one byte per access of eight entries).  Then every z_j of the pass has the gradient c a exp((z_j - m) / T) with two
 // numbers m, a of its row, an entry of the list c (b exp((z_j - M) / T) - its p), c = w T / rows: the row's four numbers are what a backward call needs.
 // Sums over a row are fp32 of at most 64 terms in a row and pairwise beyond, what is formed of the list's numbers is fp64.
+#include <algorithm>
+
 #include "hgq_device.h"
 #include "hgq_host.h"
 #include "hgq_vector.h"
@@ -496,6 +498,7 @@ namespace {
 
 constexpr int SPLIT_ROWS = 128;   // rows from which on a row has a workgroup to itself (200 x 131072 bfloat16 with gradient: 37 us, in three parts 44)
 constexpr int SPLIT_PART = 4096;  // entries of a part, at least
+constexpr int SPLIT_TERMS = 64;   // terms that a thread adds up one after the other, at most (1000 x 262144 float32 with gradient 556 us, four entries more, in parts, 656)
 
 struct DistillPlan {
     int tpr, hold;      // threads per row, elements held
@@ -527,6 +530,8 @@ DistillPlan distill_plan(int64_t rows, int V, int K, bool rest, int size, bool g
     if (rows < SPLIT_ROWS && V >= 2 * SPLIT_PART) parts = (512 + rows - 1) / rows;
     if (parts > V / SPLIT_PART) parts = V / SPLIT_PART;
     if (rest && parts < (V + DISTILL_BITS - 1) / DISTILL_BITS) parts = (V + DISTILL_BITS - 1) / DISTILL_BITS;
+    const int64_t longest = SPLIT_TERMS * (16 / size);  // entries of a thread
+    if ((parts > 1 || V > longest * p.tpr) && parts < (V + 256 * longest - 1) / (256 * longest)) parts = (V + 256 * longest - 1) / (256 * longest);
     if (parts > 1) {
         p.part = (int)(((V + parts - 1) / parts + 31) / 32 * 32);
         p.n_parts = (V + p.part - 1) / p.part;
@@ -620,8 +625,9 @@ using namespace hgq;
 
 extern "C" int64_t hgq_distill_topk_workspace(int64_t rows, int64_t V, int64_t K, int rest) {
     if (check_distill("hgq_distill_topk_workspace", rows, V, K, 1.0, HGQ_TYPE_F32, HGQ_TYPE_F32, 4)) return -1;
-    const DistillPlan p = distill_plan(rows, (int)V, (int)K, rest, 4, true);
-    return 2 * rows + (p.n_parts > 1 ? 2 * rows * p.n_parts : 0);  // (a sum for each row, at most)
+    int most = 1;
+    for (int kind = 0; kind < 4; ++kind) most = std::max(most, distill_plan(rows, (int)V, (int)K, rest, kind & 1 ? 2 : 4, kind & 2).n_parts);
+    return 2 * rows + (most > 1 ? 2 * rows * most : 0);  // (a sum for each row, at most)
 }
 
 extern "C" int hgq_distill_topk_fwd(const void *z, int64_t z_stride, const void *t, int t_type, const void *index, int index_bytes, const float *lse,

@@ -362,3 +362,43 @@ def test_recording_beside_a_living_graph_is_refused(dev):
         with torch.cuda.graph(graph, stream=side):
             ops.distill_topk(z, t, i)
     assert torch.isfinite(alive)
+
+
+@pytest.mark.parametrize('rest', [False, True])
+@pytest.mark.parametrize('rows,V,dtype', [(130, 300_001, torch.float32), (129, 700_003, torch.bfloat16), (2, 9_000_001, torch.float16)])
+def test_rows_of_many_entries(dev, rows, V, dtype, rest):
+    """Sums stay within their bounds however long a row is: it is cut where a thread would add more than 64 terms.  The same definition, evaluated on the GPU."""
+    from hgq2_amd import ops
+
+    g = torch.Generator(device=dev).manual_seed(V)
+    K, T = 40, 2.0
+    z = (torch.randn(rows, V, generator=g, device=dev) * 4).to(dtype).requires_grad_(True)
+    i = torch.stack([torch.randperm(V, generator=g, device=dev)[:K] for _ in range(rows)])
+    t = torch.randn(rows, K, generator=g, device=dev) * 4 + 40
+    lse = (torch.logsumexp(t.double() / T, 1) + 0.2).float() if rest else None
+    loss = ops.distill_topk(z, t, i, T, lse)
+    (dz,) = torch.autograd.grad(loss, [z])
+    with torch.no_grad():
+        assert abs(float(ops.distill_topk(z, t, i, T, lse)) - float(loss)) <= 2e-5 * abs(float(loss))
+    total, tol = 0.0, 0.0
+    for r in range(rows):
+        zr, tr = z[r].detach().double() / T, t[r].double() / T
+        log_q = zr - torch.logsumexp(zr, 0)
+        q, p = log_q.exp(), (tr - (torch.logsumexp(tr, 0) if lse is None else lse[r].double())).exp()
+        E = (120 + 8 * max(float(zr.max() - zr.min()), float(tr.max() - tr.min()))) * U
+        gap = p.log() - log_q[i[r]]
+        total, tol = total + float((p * gap).sum()), tol + E * float((p * gap.abs() + 2 * p).sum())
+        share, rest_p, q_rest = torch.zeros_like(q), 0.0, 1.0
+        if rest:
+            rest_p = max(0.0, 1.0 - float(p.sum()))
+            share = q.index_fill(0, i[r], 0.0)
+            q_rest = float(share.sum())
+            share /= q_rest
+            total, tol = total + rest_p * math.log(rest_p / q_rest), tol + E * (abs(math.log(rest_p / q_rest)) + 2)
+        at = torch.zeros_like(q).index_add_(0, i[r], p)
+        P, c = float(p.sum()) + rest_p, T / rows
+        want = c * (q * P - at - share * rest_p)
+        bound = c * (2 * E * q * P + 2 * E * at + 2 * E * share * rest_p + E * share + 4 * U * (q + at + share))
+        bound = bound + HALF[dtype] * (want.abs() + bound) + LEAST[dtype]
+        assert ((dz[r].double() - want).abs() <= bound).all(), r
+    assert abs(float(loss) - total * T * T / rows) <= (tol * T * T / rows) + 4 * U * abs(float(loss))
