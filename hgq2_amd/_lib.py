@@ -320,10 +320,13 @@ def _load_host(path):
         return tensors[0].new_empty((), dtype=torch.float32)
 
     @torch.library.register_fake('hgq::distill_topk_fwd')
-    def _(logits, teacher_logits, teacher_indices, teacher_lse, sample_weight, temperature, gradient):
-        rows = logits.shape[0] if gradient else 0
+    def _(logits, teacher_logits, teacher_indices, teacher_lse, sample_weight, temperature):
         number = torch.float32
-        return logits.new_empty((), dtype=number), logits.new_empty((rows, 4), dtype=number), logits.new_empty((rows, logits.shape[1]))
+        return logits.new_empty((), dtype=number), logits.new_empty((logits.shape[0], 4), dtype=number), logits.new_empty(logits.shape)
+
+    @torch.library.register_fake('hgq::distill_topk_loss')
+    def _(logits, teacher_logits, teacher_indices, teacher_lse, sample_weight, temperature):
+        return logits.new_empty((), dtype=torch.float32)
 
     @torch.library.register_fake('hgq::distill_topk_bwd')
     def _(upstream, logits, teacher_logits, teacher_indices, teacher_lse, sample_weight, stats, temperature):
@@ -342,16 +345,20 @@ def _load_host(path):
         return dout.new_empty(((len(first) + 1) * (2 if both else 1), dout.shape[1]), dtype=torch.float32)
 
     @torch.library.register_fake('hgq::residual_norm_fwd')
-    def _(x, update, gate, post_gamma, pre_gamma, gate_rows, scale, epsilon, act, keep):
-        has = update.shape == x.shape
+    def _(x, update, gate, post_gamma, pre_gamma, gate_rows, scale, epsilon, act):
+        has = update is not None and update.shape == x.shape
         rows = x.numel() // x.shape[-1]
-        return (torch.empty_like(x) if has else x.new_empty(0), torch.empty_like(x), x.new_empty((2 if has else 1) * rows if keep else 0, dtype=torch.float32))
+        return (torch.empty_like(x) if has else x.new_empty(0), torch.empty_like(x), x.new_empty((2 if has else 1) * rows, dtype=torch.float32))
+
+    @torch.library.register_fake('hgq::residual_norm_values')
+    def _(x, update, gate, post_gamma, pre_gamma, gate_rows, scale, epsilon, act):
+        return [torch.empty_like(x)] + ([torch.empty_like(x)] if update is not None and update.shape == x.shape else [])
 
     @torch.library.register_fake('hgq::residual_norm_bwd')
     def _(dy, dh, x, update, gate, post_gamma, pre_gamma, r, gate_rows, scale, epsilon, act, need_dx, need_dupdate, need_dgate, need_dpost, need_dpre):
         like = lambda t, need: torch.empty_like(t) if need else x.new_empty(0)  # noqa: E731
         vector = lambda need: x.new_empty(x.shape[-1] if need else 0, dtype=torch.float32)  # noqa: E731
-        return like(x, need_dx), like(x, need_dupdate and update.shape == x.shape), like(gate, need_dgate), vector(need_dpost), vector(need_dpre)
+        return like(x, need_dx), like(x, need_dupdate and update is not None and update.shape == x.shape), like(gate, need_dgate and gate is not None), vector(need_dpost), vector(need_dpre)
 
     return mod
 

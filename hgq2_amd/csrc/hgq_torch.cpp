@@ -242,9 +242,17 @@ void numbers(const char *name, const Tensor &t, int64_t n, const Tensor &like) {
                       " must be a contiguous float32 tensor of ", n, " elements on ", like.device(), ", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
 }
 
+// (0.5 us less than empty_like takes)
+Tensor whole_like(const Tensor &t) { return at::empty(t.sizes(), t.options()); }
+
 bool differentiated(const Tensor &t) { return t.defined() && ((t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined()); }
 
 Tensor plain(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+// What is not given goes without a tensor (an empty one takes 1 us to make); the operators take an empty one for the same.
+using Maybe = std::optional<Tensor>;
+
+Tensor given(const Maybe &t) { return t ? *t : Tensor(); }
 
 // Gradients asked for with create_graph, of any operator: see OnceOnly.
 struct AllOnceOnly : torch::autograd::Function<AllOnceOnly> {
@@ -293,16 +301,27 @@ DistillSizes distill_sizes(const Tensor &z, const Tensor &t, const Tensor &index
     return {z.size(0), z.size(1), t.size(1), type_code(z.scalar_type()), type_code(t.scalar_type()), index.scalar_type() == at::kLong ? 8 : 4};
 }
 
-std::tuple<Tensor, Tensor, Tensor> distill_topk_fwd(const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, double T, bool gradient) {
+// stats and dz: where the gradient is wanted
+Tensor distill_forward(const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, double T, Tensor *stats, Tensor *dz) {
     const DistillSizes s = distill_sizes(z, t, index, lse, weight, T);
     const c10::DeviceGuard guard(z.device());
     const auto options = z.options().dtype(at::kFloat);
-    Tensor loss = at::empty({}, options), stats = at::empty({gradient ? s.rows : 0, 4}, options), dz = at::empty({gradient ? s.rows : 0, s.V}, z.options());
+    Tensor loss = at::empty({}, options);
+    if (stats) *stats = at::empty({s.rows, 4}, options), *dz = at::empty({s.rows, s.V}, z.options());
     const Workspace<float> ws(library().distill_topk_workspace(s.rows, s.V, s.K, lse.numel() > 0));
-    check(lib.distill_topk_fwd(memory(z), z.stride(0), memory(t), s.t_type, memory(index), s.index_bytes, floats(lse), floats(weight), loss.data_ptr<float>(), floats(stats),
-                               memory(dz), ws.get(), s.rows, s.V, s.K, T, s.type, stream_of(z)),
+    check(lib.distill_topk_fwd(memory(z), z.stride(0), memory(t), s.t_type, memory(index), s.index_bytes, floats(lse), floats(weight), loss.data_ptr<float>(),
+                               stats ? floats(*stats) : nullptr, dz ? memory(*dz) : nullptr, ws.get(), s.rows, s.V, s.K, T, s.type, stream_of(z)),
           "hgq_distill_topk_fwd");
+    return loss;
+}
+
+std::tuple<Tensor, Tensor, Tensor> distill_topk_fwd(const Tensor &z, const Tensor &t, const Tensor &index, const Maybe &lse, const Maybe &weight, double T) {
+    Tensor stats, dz, loss = distill_forward(z, t, index, given(lse), given(weight), T, &stats, &dz);
     return {loss, stats, dz};
+}
+
+Tensor distill_topk_loss(const Tensor &z, const Tensor &t, const Tensor &index, const Maybe &lse, const Maybe &weight, double T) {
+    return distill_forward(z, t, index, given(lse), given(weight), T, nullptr, nullptr);
 }
 
 void distill_backward(const Tensor &up, const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, const Tensor &stats, const Tensor &dz, bool holds_unit,
@@ -317,31 +336,27 @@ void distill_backward(const Tensor &up, const Tensor &z, const Tensor &t, const 
           "hgq_distill_topk_bwd");
 }
 
-Tensor distill_topk_bwd(const Tensor &up, const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, const Tensor &stats, double T) {
+Tensor distill_topk_bwd(const Tensor &up, const Tensor &z, const Tensor &t, const Tensor &index, const Maybe &lse, const Maybe &weight, const Tensor &stats, double T) {
     on_gpu("logits", z);
     Tensor dz = at::empty(z.sizes(), z.options());
-    distill_backward(up, z, t, index, lse, weight, stats, dz, false, T);
+    distill_backward(up, z, t, index, given(lse), given(weight), stats, dz, false, T);
     return dz;
 }
 
 // `dz`: the gradient for an upstream of one, which is left as it is where the upstream is one
-void distill_topk_bwd_(const Tensor &up, const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, const Tensor &stats, double T, Tensor dz) {
-    distill_backward(up, z, t, index, lse, weight, stats, dz, true, T);
-}
-
-const auto &distill_op() {
-    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::distill_topk_fwd", "").typed<decltype(distill_topk_fwd)>();
-    return op;
+void distill_topk_bwd_(const Tensor &up, const Tensor &z, const Tensor &t, const Tensor &index, const Maybe &lse, const Maybe &weight, const Tensor &stats, double T, Tensor dz) {
+    distill_backward(up, z, t, index, given(lse), given(weight), stats, dz, true, T);
 }
 
 // The forward pass writes the gradient for an upstream of one while the row is at hand.  The backward pass hands it on where the upstream is one - the
 // kernel that looks at it ends at once - and forms it anew elsewhere, so there is one rounding whatever the upstream (a loss scaled
 // for float16 gets the gradients it was scaled for).  A graph that is kept may be asked again: it gets a tensor of its own each time.
 struct DistillTopk : torch::autograd::Function<DistillTopk> {
-    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &z, const Tensor &t, const Tensor &index, const Tensor &lse, const Tensor &weight, double T) {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &z, const Tensor &t, const Tensor &index, const Maybe &lse, const Maybe &weight, double T) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::distill_topk_fwd", "").typed<decltype(distill_topk_fwd)>();
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [loss, stats, dz] = distill_op().call(z, t, index, lse, weight, T, true);
-        ctx->save_for_backward({z, t, index, lse, weight, stats, dz});
+        auto [loss, stats, dz] = op.call(z, t, index, lse, weight, T);
+        ctx->save_for_backward({z, t, index, given(lse), given(weight), stats, dz});
         ctx->saved_data["T"] = T;
         return loss;
     }
@@ -354,11 +369,12 @@ struct DistillTopk : torch::autograd::Function<DistillTopk> {
         {
             at::AutoDispatchBelowADInplaceOrView below;
             const Tensor up = plain(grads[0]).to(at::kFloat);
+            const Maybe lse = saved[3].defined() ? Maybe(saved[3]) : Maybe(), weight = saved[4].defined() ? Maybe(saved[4]) : Maybe();
             if (torch::autograd::get_current_graph_task_keep_graph()) {
-                out[0] = anew.call(up, saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["T"].toDouble());
+                out[0] = anew.call(up, saved[0], saved[1], saved[2], lse, weight, saved[5], ctx->saved_data["T"].toDouble());
             } else {
                 out[0] = saved[6];
-                over.call(up, saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["T"].toDouble(), out[0]);
+                over.call(up, saved[0], saved[1], saved[2], lse, weight, saved[5], ctx->saved_data["T"].toDouble(), out[0]);
             }
         }
         once_only(out, {grads[0], saved[0]}, "distill_topk");
@@ -381,12 +397,12 @@ Tensor distill_topk(const Tensor &logits, const Tensor &teacher, const Tensor &i
     Tensor z = logits.dim() == 2 ? logits : logits.reshape({rows, V});
     if ((V > 1 && z.stride(1) != 1) || z.stride(0) < 0 || z.is_neg()) z = z.contiguous().resolve_neg();
     const auto flat = [rows](const Tensor &t, int64_t n) { return plain(t.detach()).reshape({rows, n}).contiguous(); };
-    const Tensor none = lse && weight ? Tensor() : at::empty({0}, logits.options().dtype(at::kFloat).requires_grad(false));
-    const Tensor t = flat(teacher, K), i = flat(indices, K), l = lse ? flat(*lse, 1) : none, w = weight ? flat(*weight, 1) : none;
-    // an empty tensor stands for none: with no rows there is nothing that a lse could change
+    const Tensor t = flat(teacher, K), i = flat(indices, K);
+    const Maybe l = lse ? Maybe(flat(*lse, 1)) : Maybe(), w = weight ? Maybe(flat(*weight, 1)) : Maybe();
     if (graph) return DistillTopk::apply(z, t, i, l, w, T);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::distill_topk_loss", "").typed<decltype(distill_topk_loss)>();
     at::AutoDispatchBelowADInplaceOrView below;
-    return std::get<0>(distill_op().call(z, t, i, l, w, T, false));
+    return op.call(z, t, i, l, w, T);
 }
 
 // ---- relative position bias ----------------------------------------------------------------------------------------------
@@ -413,25 +429,27 @@ BiasSizes bias_sizes(const char *name, const Tensor &x, const Tensor &offsets, a
 }
 
 // `first`: the first distances of the buckets of a direction but the nearest
-Tensor relative_bias_fwd(const Tensor &scores, const Tensor &table, const Tensor &offsets, int64_t offset, at::IntArrayRef first, bool both) {
+Tensor relative_bias_fwd(const Tensor &scores, const Tensor &table, const Maybe &each, int64_t offset, at::IntArrayRef first, bool both) {
+    const Tensor offsets = given(each);
     const BiasSizes s = bias_sizes("scores", scores, offsets, first);
     TORCH_CHECK_VALUE(table.scalar_type() == at::kFloat && table.device() == scores.device() && table.is_contiguous() && table.dim() == 2 && table.size(0) == (both ? 2 : 1) * s.m && table.size(1) == s.H,
                       "table must be a contiguous float32 tensor [", (both ? 2 : 1) * s.m, ", ", s.H, "] on ", scores.device(), ", got ", table.scalar_type(), " ", table.sizes(), " on ", table.device());
     const c10::DeviceGuard guard(scores.device());
     Tensor out = at::empty(scores.sizes(), scores.options());
     check(library().relative_bias_fwd(memory(scores), scores.stride(0), scores.stride(1), floats(table), memory(out), s.B, s.H, s.T, s.S, s.first.data(), s.m, both, offset, memory(offsets),
-                                      offsets.scalar_type() == at::kInt ? 4 : 8, s.type, stream_of(scores)),
+                                      offsets.defined() && offsets.scalar_type() == at::kInt ? 4 : 8, s.type, stream_of(scores)),
           "hgq_relative_bias_fwd");
     return out;
 }
 
-Tensor relative_bias_bwd(const Tensor &dy, const Tensor &offsets, int64_t offset, at::IntArrayRef first, bool both) {
+Tensor relative_bias_bwd(const Tensor &dy, const Maybe &each, int64_t offset, at::IntArrayRef first, bool both) {
+    const Tensor offsets = given(each);
     const BiasSizes s = bias_sizes("the scores' gradient", dy, offsets, first);
     const c10::DeviceGuard guard(dy.device());
     Tensor dtable = at::empty({(both ? 2 : 1) * s.m, s.H}, dy.options().dtype(at::kFloat));
     const Workspace<float> ws(library().relative_bias_bwd_workspace(s.B, s.H, s.T, s.S, s.m, both));
     check(lib.relative_bias_bwd(memory(dy), dy.stride(0), dy.stride(1), floats(dtable), ws.get(), s.B, s.H, s.T, s.S, s.first.data(), s.m, both, offset, memory(offsets),
-                                offsets.scalar_type() == at::kInt ? 4 : 8, s.type, stream_of(dy)),
+                                offsets.defined() && offsets.scalar_type() == at::kInt ? 4 : 8, s.type, stream_of(dy)),
           "hgq_relative_bias_bwd");
     return dtable;
 }
@@ -448,9 +466,9 @@ Tensor planes(const Tensor &t) {
 }
 
 struct RelativeBias : torch::autograd::Function<RelativeBias> {
-    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &scores, const Tensor &table, const Tensor &offsets, int64_t offset, std::vector<int64_t> first, bool both) {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &scores, const Tensor &table, const Maybe &offsets, int64_t offset, std::vector<int64_t> first, bool both) {
         at::AutoDispatchBelowADInplaceOrView below;
-        ctx->save_for_backward({offsets});
+        ctx->save_for_backward({given(offsets)});
         ctx->saved_data["offset"] = offset, ctx->saved_data["first"] = first, ctx->saved_data["both"] = both;
         return bias_op().call(scores, table, offsets, offset, first, both);
     }
@@ -461,7 +479,8 @@ struct RelativeBias : torch::autograd::Function<RelativeBias> {
         if (ctx->needs_input_grad(1)) {
             {
                 at::AutoDispatchBelowADInplaceOrView below;
-                table[0] = op.call(planes(grads[0]), ctx->get_saved_variables()[0], ctx->saved_data["offset"].toInt(), ctx->saved_data["first"].toIntVector(), ctx->saved_data["both"].toBool());
+                const Tensor offsets = ctx->get_saved_variables()[0];
+                table[0] = op.call(planes(grads[0]), offsets.defined() ? Maybe(offsets) : Maybe(), ctx->saved_data["offset"].toInt(), ctx->saved_data["first"].toIntVector(), ctx->saved_data["both"].toBool());
             }
             once_only(table, {grads[0]}, "relative_bias");
             out[1] = table[0];
@@ -474,13 +493,13 @@ Tensor relative_bias(const Tensor &scores, const Tensor &table, std::vector<int6
     TORCH_CHECK_VALUE(scores.dim() == 3 || scores.dim() == 4, "scores must be [heads, queries, keys] or [batch, heads, queries, keys], got ", scores.sizes());
     const bool graph = differentiated(scores) || differentiated(table);
     if (graph) accumulates_here("scores", scores), accumulates_here("table", table);
-    const Tensor x = planes(scores.dim() == 3 ? scores.unsqueeze(0) : scores), none = offsets ? *offsets : at::empty({0}, scores.options().dtype(at::kLong).requires_grad(false));
+    const Tensor x = planes(scores.dim() == 3 ? scores.unsqueeze(0) : scores);
     Tensor out;
     if (graph) {
-        out = RelativeBias::apply(x, plain(table.contiguous()), none, offset, first, both);
+        out = RelativeBias::apply(x, plain(table.contiguous()), offsets, offset, first, both);
     } else {
         at::AutoDispatchBelowADInplaceOrView below;
-        out = bias_op().call(x, plain(table.contiguous()), none, offset, first, both);
+        out = bias_op().call(x, plain(table.contiguous()), offsets, offset, first, both);
     }
     return scores.dim() == 3 ? out.squeeze(0) : out;
 }
@@ -505,30 +524,48 @@ ResidualSizes residual_sizes(const Tensor &x, const Tensor &u, const Tensor &gat
     return {rows, C, type_code(x.scalar_type())};
 }
 
-std::tuple<Tensor, Tensor, Tensor> residual_norm_fwd(const Tensor &x, const Tensor &u, const Tensor &gate, const Tensor &post, const Tensor &pre, int64_t P, double scale, double epsilon,
-                                                     int64_t act, bool keep) {
+// y (with an update) and h, and the norms' factors where they are wanted
+void residual_forward(const Tensor &x, const Tensor &u, const Tensor &gate, const Tensor &post, const Tensor &pre, int64_t P, double scale, double epsilon, int64_t act, Tensor &y, Tensor &h,
+                      Tensor *r) {
     const ResidualSizes s = residual_sizes(x, u, gate, post, pre, P);
     const c10::DeviceGuard guard(x.device());
     const bool update = u.sizes() == x.sizes();
-    Tensor y = update ? at::empty_like(x) : at::empty({0}, x.options()), h = at::empty_like(x), r = vector_like(keep ? (update ? 2 : 1) * s.rows : 0, x);
-    float *r_y = floats(r), *r_u = r_y && update ? r_y + s.rows : nullptr;
-    check(library().residual_norm_fwd(memory(x), memory(u), memory(gate), floats(post), floats(pre), memory(y), memory(h), r_u, r_y, s.rows, P, s.C, (float)scale, (float)epsilon, (int)act,
-                                      s.type, stream_of(x)),
+    if (update) y = whole_like(x);
+    h = whole_like(x);
+    if (r) *r = vector_like((update ? 2 : 1) * s.rows, x);
+    float *r_y = r ? floats(*r) : nullptr, *r_u = r_y && update ? r_y + s.rows : nullptr;
+    check(library().residual_norm_fwd(memory(x), memory(u), memory(gate), floats(post), floats(pre), update ? memory(y) : nullptr, memory(h), r_u, r_y, s.rows, P, s.C, (float)scale, (float)epsilon,
+                                      (int)act, s.type, stream_of(x)),
           "hgq_residual_norm_fwd");
-    return {y, h, r};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> residual_norm_bwd(const Tensor &dy, const Tensor &dh, const Tensor &x, const Tensor &u, const Tensor &gate, const Tensor &post, const Tensor &pre,
-                                                                     const Tensor &r, int64_t P, double scale, double epsilon, int64_t act, bool need_dx, bool need_du, bool need_dgate,
+std::tuple<Tensor, Tensor, Tensor> residual_norm_fwd(const Tensor &x, const Maybe &u, const Maybe &gate, const Maybe &post, const Maybe &pre, int64_t P, double scale, double epsilon, int64_t act) {
+    Tensor y, h, r;
+    residual_forward(x, given(u), given(gate), given(post), given(pre), P, scale, epsilon, act, y, h, &r);
+    return {y.defined() ? y : at::empty({0}, x.options()), h, r};
+}
+
+std::vector<Tensor> residual_norm_values(const Tensor &x, const Maybe &u, const Maybe &gate, const Maybe &post, const Maybe &pre, int64_t P, double scale, double epsilon, int64_t act) {
+    Tensor y, h;
+    residual_forward(x, given(u), given(gate), given(post), given(pre), P, scale, epsilon, act, y, h, nullptr);
+    if (!y.defined()) return {h};
+    return {y, h};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> residual_norm_bwd(const Maybe &maybe_dy, const Maybe &maybe_dh, const Tensor &x, const Maybe &maybe_u, const Maybe &maybe_gate,
+                                                                     const Maybe &maybe_post, const Maybe &maybe_pre, const Tensor &r, int64_t P, double scale, double epsilon, int64_t act, bool need_dx, bool need_du, bool need_dgate,
                                                                      bool need_dpost, bool need_dpre) {
+    const Tensor dy = given(maybe_dy), dh = given(maybe_dh), u = given(maybe_u), gate = given(maybe_gate), post = given(maybe_post), pre = given(maybe_pre);
     const ResidualSizes s = residual_sizes(x, u, gate, post, pre, P);
     for (const Tensor *g : {&dy, &dh})
         TORCH_CHECK_VALUE(g->numel() == 0 || (g->sizes() == x.sizes() && g->scalar_type() == x.scalar_type() && g->device() == x.device() && g->is_contiguous()), "gradients must be contiguous and like x");
     const bool update = u.sizes() == x.sizes();
     TORCH_CHECK_VALUE(r.numel() == (update ? 2 : 1) * s.rows && r.scalar_type() == at::kFloat && r.device() == x.device() && r.is_contiguous(), "r must be what the forward call left");
     const c10::DeviceGuard guard(x.device());
-    const Tensor none = at::empty({0}, x.options());
-    Tensor dx = need_dx ? at::empty_like(x) : none, du = need_du && update ? at::empty_like(x) : none, dgate = !need_dgate ? none : s.rows ? at::empty_like(gate) : at::zeros_like(gate), dpost = vector_like(need_dpost ? s.C : 0, x),
+    need_dgate = need_dgate && gate.defined();
+    const bool all = need_dx && need_du && update && need_dgate;
+    const Tensor none = all ? Tensor() : at::empty({0}, x.options());
+    Tensor dx = need_dx ? whole_like(x) : none, du = need_du && update ? whole_like(x) : none, dgate = !need_dgate ? none : s.rows ? whole_like(gate) : at::zeros_like(gate), dpost = vector_like(need_dpost ? s.C : 0, x),
            dpre = vector_like(need_dpre ? s.C : 0, x);
     const Workspace<float> ws(library().residual_norm_bwd_workspace(s.rows, P, s.C, s.type));
     const float *r_y = floats(r), *r_u = r_y && update ? r_y + s.rows : nullptr;
@@ -538,20 +575,16 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> residual_norm_bwd(const Tenso
     return {dx, du, dgate, dpost, dpre};
 }
 
-const auto &residual_op() {
-    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::residual_norm_fwd", "").typed<decltype(residual_norm_fwd)>();
-    return op;
-}
-
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
-    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &u, const Tensor &gate, const Tensor &post, const Tensor &pre, int64_t P,
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Maybe &u, const Maybe &gate, const Maybe &post, const Maybe &pre, int64_t P,
                                                   double scale, double epsilon, int64_t act) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::residual_norm_fwd", "").typed<decltype(residual_norm_fwd)>();
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [y, h, r] = residual_op().call(x, u, gate, post, pre, P, scale, epsilon, act, true);
-        ctx->save_for_backward({x, u, gate, post, pre, r});
+        auto [y, h, r] = op.call(x, u, gate, post, pre, P, scale, epsilon, act);
+        ctx->save_for_backward({x, given(u), given(gate), given(post), given(pre), r});
         ctx->saved_data["P"] = P, ctx->saved_data["scale"] = scale, ctx->saved_data["epsilon"] = epsilon, ctx->saved_data["act"] = act;
         ctx->set_materialize_grads(false);
-        if (u.sizes() != x.sizes()) return {h};
+        if (!u) return {h};
         return {y, h};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads) {
@@ -562,16 +595,18 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         torch::autograd::variable_list out(9);
         const Tensor &gy = update ? grads[0] : Tensor(), &gh = grads[update ? 1 : 0];
         if (!gy.defined() && !gh.defined()) return out;
+        bool need[5];  // (what was not given is no input of the node)
+        for (int k = 0, input = 0; k < 5; ++k) need[k] = saved[k].defined() && ctx->needs_input_grad(input++);
         {
             at::AutoDispatchBelowADInplaceOrView below;
-            const Tensor none = at::empty({0}, x.options().requires_grad(false));
-            const auto given = [&](const Tensor &g) { return g.defined() ? plain(g.contiguous()) : none; };
-            const auto [dx, du, dgate, dpost, dpre] = op.call(given(gy), given(gh), x, saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["P"].toInt(),
-                                                              ctx->saved_data["scale"].toDouble(), ctx->saved_data["epsilon"].toDouble(), ctx->saved_data["act"].toInt(),
-                                                              ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3), ctx->needs_input_grad(4));
+            const auto there = [](const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
+            const auto whole = [](const Tensor &g) { return g.defined() ? Maybe(plain(g.contiguous())) : Maybe(); };
+            const auto [dx, du, dgate, dpost, dpre] = op.call(whole(gy), whole(gh), x, there(saved[1]), there(saved[2]), there(saved[3]), there(saved[4]), saved[5], ctx->saved_data["P"].toInt(),
+                                                              ctx->saved_data["scale"].toDouble(), ctx->saved_data["epsilon"].toDouble(), ctx->saved_data["act"].toInt(), need[0], need[1], need[2],
+                                                              need[3], need[4]);
             const Tensor *all[] = {&dx, &du, &dgate, &dpost, &dpre};
             for (int k = 0; k < 5; ++k)
-                if (ctx->needs_input_grad(k)) out[k] = *all[k];
+                if (need[k]) out[k] = *all[k];
         }
         once_only(out, {gy, gh, saved[0], saved[1], saved[2], saved[3], saved[4]}, "residual_norm");
         return out;
@@ -599,21 +634,22 @@ std::vector<Tensor> residual_norm(const Tensor &x, const std::optional<Tensor> &
         TORCH_CHECK_VALUE(fits, "gate must be like x, [batch, channels] or [channels], got ", gate->sizes(), " for ", x.sizes());
         if (P < 1) P = 1;
     }
-    std::vector<Tensor> inputs = {x};
-    const char *names[] = {"x", "update", "gate", "post_gamma", "pre_gamma"};
+    const char *names[] = {"update", "gate", "post_gamma", "pre_gamma"};
     const std::optional<Tensor> *rest[] = {&u, &gate, &post, &pre};
-    bool graph = differentiated(x), missing = false;
-    for (const auto *t : rest) graph = graph || (*t && differentiated(**t)), missing = missing || !*t;
-    const Tensor none = missing ? at::empty({0}, x.options().dtype(at::kFloat).requires_grad(false)) : Tensor();
-    for (const auto *t : rest) inputs.push_back(*t ? **t : none);
-    if (graph)
-        for (int k = 0; k < 5; ++k) accumulates_here(names[k], inputs[k]);
-    for (Tensor &t : inputs) t = plain(t.contiguous());
-    if (graph) return ResidualNorm::apply(inputs[0], inputs[1], inputs[2], inputs[3], inputs[4], P, scale, epsilon, act);
+    bool graph = differentiated(x);
+    for (const auto *t : rest) graph = graph || (*t && differentiated(**t));
+    if (graph) {
+        accumulates_here("x", x);
+        for (int k = 0; k < 4; ++k)
+            if (*rest[k]) accumulates_here(names[k], **rest[k]);
+    }
+    const auto whole = [](const Maybe &t) { return t ? Maybe(plain(t->contiguous())) : Maybe(); };
+    const Tensor rows_of_x = plain(x.contiguous());
+    const Maybe in_u = whole(u), in_gate = whole(gate), in_post = whole(post), in_pre = whole(pre);
+    if (graph) return ResidualNorm::apply(rows_of_x, in_u, in_gate, in_post, in_pre, P, scale, epsilon, act);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("hgq::residual_norm_values", "").typed<decltype(residual_norm_values)>();
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, h, r] = residual_op().call(inputs[0], inputs[1], inputs[2], inputs[3], inputs[4], P, scale, epsilon, act, false);
-    if (!u) return {h};
-    return {y, h};
+    return op.call(rows_of_x, in_u, in_gate, in_post, in_pre, P, scale, epsilon, act);
 }
 
 // ---- the global norm -------------------------------------------------------------------------------------------------
@@ -826,17 +862,17 @@ TORCH_LIBRARY_FRAGMENT(hgq, m) {
     m.def("group_norm_bwd(Tensor dy, Tensor x, Tensor gamma, Tensor beta, Tensor stats, int groups, int act, bool need_dx, bool need_dgamma, bool need_dbeta) "
           "-> (Tensor, Tensor, Tensor)");
     m.def("global_norm(Tensor[] tensors) -> Tensor");
-    m.def("distill_topk_fwd(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor teacher_lse, Tensor sample_weight, float temperature, bool gradient) "
-          "-> (Tensor, Tensor, Tensor)");
-    m.def("distill_topk_bwd(Tensor upstream, Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor teacher_lse, Tensor sample_weight, Tensor stats, float temperature) "
+    m.def("distill_topk_loss(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor? teacher_lse, Tensor? sample_weight, float temperature) -> Tensor");
+    m.def("distill_topk_fwd(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor? teacher_lse, Tensor? sample_weight, float temperature) -> (Tensor, Tensor, Tensor)");
+    m.def("distill_topk_bwd(Tensor upstream, Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor? teacher_lse, Tensor? sample_weight, Tensor stats, float temperature) "
           "-> Tensor");
-    m.def("distill_topk_bwd_(Tensor upstream, Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor teacher_lse, Tensor sample_weight, Tensor stats, float temperature, "
+    m.def("distill_topk_bwd_(Tensor upstream, Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor? teacher_lse, Tensor? sample_weight, Tensor stats, float temperature, "
           "Tensor(a!) dlogits) -> ()");
-    m.def("relative_bias_fwd(Tensor scores, Tensor table, Tensor offsets, int offset, int[] first, bool both) -> Tensor");
-    m.def("relative_bias_bwd(Tensor dout, Tensor offsets, int offset, int[] first, bool both) -> Tensor");
-    m.def("residual_norm_fwd(Tensor x, Tensor update, Tensor gate, Tensor post_gamma, Tensor pre_gamma, int gate_rows, float scale, float epsilon, int act, bool keep) "
-          "-> (Tensor, Tensor, Tensor)");
-    m.def("residual_norm_bwd(Tensor dy, Tensor dh, Tensor x, Tensor update, Tensor gate, Tensor post_gamma, Tensor pre_gamma, Tensor r, int gate_rows, float scale, float epsilon, int act, "
+    m.def("relative_bias_fwd(Tensor scores, Tensor table, Tensor? offsets, int offset, int[] first, bool both) -> Tensor");
+    m.def("relative_bias_bwd(Tensor dout, Tensor? offsets, int offset, int[] first, bool both) -> Tensor");
+    m.def("residual_norm_values(Tensor x, Tensor? update, Tensor? gate, Tensor? post_gamma, Tensor? pre_gamma, int gate_rows, float scale, float epsilon, int act) -> Tensor[]");
+    m.def("residual_norm_fwd(Tensor x, Tensor? update, Tensor? gate, Tensor? post_gamma, Tensor? pre_gamma, int gate_rows, float scale, float epsilon, int act) -> (Tensor, Tensor, Tensor)");
+    m.def("residual_norm_bwd(Tensor? dy, Tensor? dh, Tensor x, Tensor? update, Tensor? gate, Tensor? post_gamma, Tensor? pre_gamma, Tensor r, int gate_rows, float scale, float epsilon, int act, "
           "bool need_dx, bool need_dupdate, bool need_dgate, bool need_dpost, bool need_dpre) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
@@ -845,11 +881,13 @@ TORCH_LIBRARY_IMPL(hgq, CUDA, m) {
     m.impl("group_norm_fwd", group_norm_fwd);
     m.impl("group_norm_bwd", group_norm_bwd);
     m.impl("global_norm", global_norm);
+    m.impl("distill_topk_loss", distill_topk_loss);
     m.impl("distill_topk_fwd", distill_topk_fwd);
     m.impl("distill_topk_bwd", distill_topk_bwd);
     m.impl("distill_topk_bwd_", distill_topk_bwd_);
     m.impl("relative_bias_fwd", relative_bias_fwd);
     m.impl("relative_bias_bwd", relative_bias_bwd);
+    m.impl("residual_norm_values", residual_norm_values);
     m.impl("residual_norm_fwd", residual_norm_fwd);
     m.impl("residual_norm_bwd", residual_norm_bwd);
 }
@@ -857,11 +895,13 @@ TORCH_LIBRARY_IMPL(hgq, CPU, m) {
     m.impl("group_norm_fwd", group_norm_fwd);
     m.impl("group_norm_bwd", group_norm_bwd);
     m.impl("global_norm", global_norm);
+    m.impl("distill_topk_loss", distill_topk_loss);
     m.impl("distill_topk_fwd", distill_topk_fwd);
     m.impl("distill_topk_bwd", distill_topk_bwd);
     m.impl("distill_topk_bwd_", distill_topk_bwd_);
     m.impl("relative_bias_fwd", relative_bias_fwd);
     m.impl("relative_bias_bwd", relative_bias_bwd);
+    m.impl("residual_norm_values", residual_norm_values);
     m.impl("residual_norm_fwd", residual_norm_fwd);
     m.impl("residual_norm_bwd", residual_norm_bwd);
 }

@@ -349,6 +349,6 @@ def test_rows_of_a_gate_that_is_not_there(dev):
         x, u, dy, dh = (torch.randn(24, C, generator=g).to(dev) for _ in range(4))
         got = []
         for P in (1, 6):
-            y, h, r = torch.ops.hgq.residual_norm_fwd(x, u, none, none, none, P, 0.5, 1e-6, 0, True)
-            got.append([y, h, r, *torch.ops.hgq.residual_norm_bwd(dy, dh, x, u, none, none, none, r, P, 0.5, 1e-6, 0, True, True, False, True, True)])
+            y, h, r = torch.ops.hgq.residual_norm_fwd(x, u, none, none, None, P, 0.5, 1e-6, 0)
+            got.append([y, h, r, *torch.ops.hgq.residual_norm_bwd(dy, dh, x, u, none, none, None, r, P, 0.5, 1e-6, 0, True, True, False, True, True)])
         assert all(torch.equal(a, b) for a, b in zip(*got))

@@ -170,16 +170,19 @@ def test_registered_for_fake_tensors():
     with FakeTensorMode():
         z, i = torch.empty(3, 9, device='cuda'), torch.empty(3, 2, dtype=torch.long, device='cuda')
         none = torch.empty(0, device='cuda')
-        loss, stats, dz = torch.ops.hgq.distill_topk_fwd(z, z[:, :2], i, none, none, 1.0, True)
+        loss, stats, dz = torch.ops.hgq.distill_topk_fwd(z, z[:, :2], i, none, None, 1.0)
         assert loss.shape == () and stats.shape == (3, 4) and dz.shape == z.shape
-        assert torch.ops.hgq.distill_topk_bwd(loss, z, z[:, :2], i, none, none, stats, 1.0).shape == z.shape
+        assert torch.ops.hgq.distill_topk_bwd(loss, z, z[:, :2], i, none, None, stats, 1.0).shape == z.shape
+        assert torch.ops.hgq.distill_topk_loss(z, z[:, :2], i, None, None, 1.0).shape == ()
         s, t = torch.empty(2, 4, 5, 6, device='cuda'), torch.empty(8, 4, device='cuda')
         assert torch.ops.hgq.relative_bias_fwd(s, t, none, 0, [1, 2, 5], True).shape == s.shape
-        assert torch.ops.hgq.relative_bias_bwd(s, none, 0, [1, 2, 5], True).shape == t.shape
+        assert torch.ops.hgq.relative_bias_bwd(s, None, 0, [1, 2, 5], True).shape == t.shape
         x = torch.empty(2, 3, 8, device='cuda')
-        y, h, r = torch.ops.hgq.residual_norm_fwd(x, x, none, none, none, 1, 1.0, 1e-6, 0, True)
+        y, h, r = torch.ops.hgq.residual_norm_fwd(x, x, none, None, None, 1, 1.0, 1e-6, 0)
         assert y.shape == h.shape == x.shape and r.shape == (12,)
-        got = torch.ops.hgq.residual_norm_bwd(x, none, x, x, none, none, none, r, 1, 1.0, 1e-6, 0, True, True, False, True, False)
+        assert [t.shape for t in torch.ops.hgq.residual_norm_values(x, x, None, None, none, 1, 1.0, 1e-6, 0)] == [x.shape] * 2
+        assert [t.shape for t in torch.ops.hgq.residual_norm_values(x, None, None, None, None, 1, 1.0, 1e-6, 0)] == [x.shape]
+        got = torch.ops.hgq.residual_norm_bwd(x, None, x, x, none, none, None, r, 1, 1.0, 1e-6, 0, True, True, False, True, False)
         assert [tuple(g.shape) for g in got] == [(2, 3, 8), (2, 3, 8), (0,), (8,), (0,)]
 
 
