@@ -140,6 +140,23 @@ def test_another_upstream_gradient(dev, up, rest, dtype):
     _run(dev, _inputs(2, 20001, 9, dtype, 5, rest=rest), 2.0, dtype, up)
 
 
+@pytest.mark.parametrize('rows,V,dtype', [(70000, 50, torch.float32), (40000, 200, torch.bfloat16), (9000, 3000, torch.bfloat16), (3000, 20000, torch.float16), (1100, 50000, torch.bfloat16),
+                                          (600, 140000, torch.float32)])
+def test_another_upstream_gradient_of_many_rows(dev, rows, V, dtype):
+    """Every form of a row.  Both gradients have the same number times 1 or 3 / rows: a rounding each of the factor, the product and the result."""
+    from hgq2_amd import ops
+
+    for rest in (False, True):
+        g = torch.Generator(device=dev).manual_seed(rows)
+        z = (torch.randn(rows, V, generator=g, device=dev) * 4).to(dtype).requires_grad_(True)
+        i, t = torch.randint(0, V, (rows, 9), generator=g, device=dev), torch.randn(rows, 9, generator=g, device=dev) * 3
+        lse = torch.logsumexp(t / 2.0, 1) + 0.2 if rest else None
+        (one,) = torch.autograd.grad(ops.distill_topk(z, t, i, 2.0, lse), [z])
+        (three,) = torch.autograd.grad(ops.distill_topk(z, t, i, 2.0, lse) * 3.0, [z])
+        one, three = one.double() * 3, three.double()
+        assert ((one - three).abs() <= (HALF[dtype] + 3 * U) * (one.abs() + three.abs()) + 4 * LEAST[dtype]).all()
+
+
 @pytest.mark.parametrize('rest', [False, True])
 def test_the_same_index_more_than_once(dev, rest):
     z, t, i, lse, w = _inputs(5, 40, 8, torch.float32, 11, rest=rest, missing=False)
