@@ -129,16 +129,20 @@ struct Held {
     }
 };
 
+// rows of less than one access; of a wavefront (257 .. 512 channels), whose addresses are then scalars (1531 x 30 x 333 float16 backward: 72 -> 68 us with a gate, 63 -> 54 without);
+// all others
+enum { TINY_ROWS, WAVE_ROWS, ROWS };
 enum { NO_UPDATE, NO_GATE, GATED, GATED_SAMPLES };  // the last: one row of a gate for P rows
 
-template <typename T, int KIND, int THREADS, bool TINY>
+template <typename T, int KIND, int THREADS, int FORM>
 __global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
-    constexpr bool WIDE = THREADS > 256;
+    constexpr bool WIDE = THREADS > 256, TINY = FORM == TINY_ROWS;
     __shared__ float lds[2][16];
     using H = Held<T, TINY>;
-    const int teams = WIDE ? 1 : 256 / a.tpr, slot = WIDE ? 0 : threadIdx.x / a.tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (a.tpr - 1);
-    const H held(lane, a.tpr, a.C);
-    RowTeam<WIDE> team(a.tpr, lds);
+    const int tpr = FORM == WAVE_ROWS ? 64 : a.tpr, teams = WIDE ? 1 : 256 / tpr;
+    const int slot = WIDE ? 0 : FORM == WAVE_ROWS ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (tpr - 1);
+    const H held(lane, tpr, a.C);
+    RowTeam<WIDE> team(tpr, lds);
     float post[RES_HELD], pre[RES_HELD];
     if (KIND != NO_UPDATE) held.vector(post, a.post, a.scale);
     held.vector(pre, a.pre, 1.0f);
@@ -183,15 +187,16 @@ __global__ __launch_bounds__(THREADS) void residual_fwd(const ResidualRows a) {
     }
 }
 
-template <typename T, int KIND, int THREADS, bool TINY>
+template <typename T, int KIND, int THREADS, int FORM>
 __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
-    constexpr bool WIDE = THREADS > 256;
+    constexpr bool WIDE = THREADS > 256, TINY = FORM == TINY_ROWS;
     __shared__ float lds[2][16];
     __shared__ float joined[WIDE ? 1 : 256 * RES_HELD];
     using H = Held<T, TINY>;
-    const int teams = WIDE ? 1 : 256 / a.tpr, slot = WIDE ? 0 : threadIdx.x / a.tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (a.tpr - 1);
-    const H held(lane, a.tpr, a.C);
-    RowTeam<WIDE> team(a.tpr, lds);
+    const int tpr = FORM == WAVE_ROWS ? 64 : a.tpr, teams = WIDE ? 1 : 256 / tpr;
+    const int slot = WIDE ? 0 : FORM == WAVE_ROWS ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / tpr, lane = WIDE ? threadIdx.x : threadIdx.x & (tpr - 1);
+    const H held(lane, tpr, a.C);
+    RowTeam<WIDE> team(tpr, lds);
     // What a thread keeps from row to row of its columns' post, pre, dpost and dpre.  With 1024 threads, which have 128 registers each, it lies in LDS, where no other
     // thread looks at it (8192 x 8192 bfloat16, a gate like x: 233 us instead of 330 with 32 registers spilled).
     constexpr bool STASH = THREADS == 1024 && KIND != NO_UPDATE;
@@ -567,17 +572,17 @@ ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample, bool 
 template <typename T, int KIND>
 auto residual_fwd_of(const ResidualPlan &p, int C) {
     constexpr int N = Vec<T>::N;
-    if (C < N) return residual_fwd<T, KIND, 256, true>;
-    if (p.tpr <= 64) return residual_fwd<T, KIND, 256, false>;
-    return p.tpr <= 512 ? residual_fwd<T, KIND, 512, false> : residual_fwd<T, KIND, 1024, false>;
+    if (C < N) return residual_fwd<T, KIND, 256, TINY_ROWS>;
+    if (p.tpr <= 64) return p.tpr == 64 ? residual_fwd<T, KIND, 256, WAVE_ROWS> : residual_fwd<T, KIND, 256, ROWS>;
+    return p.tpr <= 512 ? residual_fwd<T, KIND, 512, ROWS> : residual_fwd<T, KIND, 1024, ROWS>;
 }
 
 template <typename T, int KIND>
 auto residual_bwd_of(const ResidualPlan &p, int C) {
     constexpr int N = Vec<T>::N;
-    if (C < N) return residual_bwd<T, KIND, 256, true>;
-    if (p.tpr <= 64) return residual_bwd<T, KIND, 256, false>;
-    return p.tpr <= 512 ? residual_bwd<T, KIND, 512, false> : residual_bwd<T, KIND, 1024, false>;
+    if (C < N) return residual_bwd<T, KIND, 256, TINY_ROWS>;
+    if (p.tpr <= 64) return p.tpr == 64 ? residual_bwd<T, KIND, 256, WAVE_ROWS> : residual_bwd<T, KIND, 256, ROWS>;
+    return p.tpr <= 512 ? residual_bwd<T, KIND, 512, ROWS> : residual_bwd<T, KIND, 1024, ROWS>;
 }
 
 template <typename T, int KIND>
