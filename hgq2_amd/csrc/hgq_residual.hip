@@ -387,45 +387,83 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
     }
 }
 
-// Rows of more channels than a workgroup holds: read again for each of the means, sums over rows in the workgroup's own slice.
+// Rows of more channels than a workgroup holds: read again for each of the means, ANY columns of a thread at a time (all their loads ahead of their stores: 4000 x 12000 bfloat16
+// 201 and 442 us, one by one 250 and 875); sums over rows in the workgroup's own slice.
+constexpr int ANY = 4;
+
 template <typename T>
-__device__ __forceinline__ float residual_sum_element(const ResidualRows &a, int64_t base, int64_t gate_base, int c, float r_u) {
-    float y = (float)((const T *)a.x)[base + c];
-    if (a.u) {
-        float b = (float)((const T *)a.u)[base + c] * r_u * ((a.post ? a.post[c] : 1.0f) * a.scale);
-        if (a.gate) b *= opened((float)((const T *)a.gate)[gate_base + c], a.act);
-        y += b;
+struct AnyRow {
+    const ResidualRows &a;
+    int64_t base, gate_base;
+    float r_u;
+    struct Columns {  // n = norm(u) (without post), open = act(gate), post with the scale
+        float y[ANY], n[ANY], open[ANY], post[ANY], pre[ANY], dy[ANY], dh[ANY];
+    };
+    __device__ __forceinline__ int column(int c, int k) const { return min(c + 1024 * k, a.C - 1); }
+    // (what there is not is read from x: elements of 16 bits loaded in a branch would be waited for there)
+    __device__ __forceinline__ void one(float *f, const void *from, int64_t at, int c) const {
+        const T *p = from ? (const T *)from + at : (const T *)a.x + base;
+        T v[ANY];
+#pragma unroll
+        for (int k = 0; k < ANY; ++k) v[k] = p[column(c, k)];
+#pragma unroll
+        for (int k = 0; k < ANY; ++k) f[k] = from ? (float)v[k] : 0.0f;
     }
-    return y;
-}
+    __device__ __forceinline__ void factor(float *f, const float *from, int c) const {
+#pragma unroll
+        for (int k = 0; k < ANY; ++k) f[k] = from ? from[column(c, k)] : 1.0f;
+    }
+    __device__ __forceinline__ Columns take(int c, bool gradients) const {
+        Columns v;
+        one(v.y, a.x, base, c), one(v.n, a.u, base, c), one(v.open, a.gate, gate_base, c);
+        factor(v.post, a.post, c), factor(v.pre, a.pre, c);
+        if (gradients) one(v.dy, a.dy, base, c), one(v.dh, a.dh, base, c);
+#pragma unroll
+        for (int k = 0; k < ANY; ++k) {
+            v.n[k] *= r_u, v.post[k] *= a.scale, v.open[k] = a.gate ? opened(v.open[k], a.act) : 1.0f;
+            v.y[k] += v.n[k] * v.post[k] * v.open[k];  // (without an update n is zero)
+        }
+        return v;
+    }
+    // dx, with m = norm(y)
+    __device__ __forceinline__ float through(const Columns &v, int k, float r_y, float s1) const { return v.dy[k] + r_y * (v.dh[k] * v.pre[k] - v.y[k] * r_y * s1); }
+};
 
 template <typename T>
 __global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
     __shared__ float lds[2][16];
     RowTeam<true> team(1024, lds);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const int64_t base = row * a.C, gate_base = a.by_sample ? row / a.P * a.C : base;
-        float r_u = 0, s = 0;
+        AnyRow<T> r = {a, row * a.C, a.by_sample ? row / a.P * a.C : row * a.C, 0.0f};
+        float s = 0;
         if (a.u) {
-            for (int c = threadIdx.x; c < a.C; c += 1024) {
-                const float u = (float)((const T *)a.u)[base + c];
-                s += u * u;
+            for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
+                float u[ANY];
+                r.one(u, a.u, r.base, c);
+#pragma unroll
+                for (int k = 0; k < ANY; ++k) s += c + 1024 * k < a.C ? u[k] * u[k] : 0.0f;
             }
-            r_u = norm_factor(team.sum(s), a.inv_c, a.eps);
+            r.r_u = norm_factor(team.sum(s), a.inv_c, a.eps);
             s = 0;
         }
-        for (int c = threadIdx.x; c < a.C; c += 1024) {
-            const float y = residual_sum_element<T>(a, base, gate_base, c, r_u);
-            s += y * y;
+        for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
+            const auto v = r.take(c, false);
+#pragma unroll
+            for (int k = 0; k < ANY; ++k) s += c + 1024 * k < a.C ? v.y[k] * v.y[k] : 0.0f;
         }
         const float r_y = norm_factor(team.sum(s), a.inv_c, a.eps);
-        for (int c = threadIdx.x; c < a.C; c += 1024) {
-            const float y = residual_sum_element<T>(a, base, gate_base, c, r_u);
-            if (a.u) ((T *)a.y)[base + c] = (T)y;
-            ((T *)a.h)[base + c] = (T)(y * (r_y * (a.pre ? a.pre[c] : 1.0f)));
+        for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
+            const auto v = r.take(c, false);
+#pragma unroll
+            for (int k = 0; k < ANY; ++k) {
+                const int at = c + 1024 * k;
+                if (at >= a.C) break;
+                if (a.u) ((T *)a.y)[r.base + at] = (T)v.y[k];
+                ((T *)a.h)[r.base + at] = (T)(v.y[k] * (r_y * v.pre[k]));
+            }
         }
         if (threadIdx.x == 0) {
-            if (a.r_u) a.r_u[row] = r_u;
+            if (a.r_u) a.r_u[row] = r.r_u;
             if (a.r_y) a.r_y[row] = r_y;
         }
     }
@@ -443,47 +481,50 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
         const int64_t sample = unit / a.cuts, r0 = sample * a.P + (unit - sample * a.cuts) * a.per_unit, r1 = min(min(r0 + a.per_unit, (sample + 1) * a.P), a.rows);
         float *dgate = a.by_sample && a.dgate ? a.gate_slices + unit * a.C : nullptr;
         for (int64_t row = r0; row < r1; ++row) {
-            const int64_t base = row * a.C, gate_base = a.by_sample ? sample * a.C : base;
-            const float r_u = a.u ? a.r_u[row] : 0.0f, r_y = a.r_y[row];
+            const AnyRow<T> r = {a, row * a.C, a.by_sample ? sample * a.C : row * a.C, a.u ? a.r_u[row] : 0.0f};
+            const float r_y = a.r_y[row];
             float s1 = 0, s2 = 0;
             if (a.dh) {
-                for (int c = threadIdx.x; c < a.C; c += 1024)
-                    s1 += (float)((const T *)a.dh)[base + c] * (a.pre ? a.pre[c] : 1.0f) * (residual_sum_element<T>(a, base, gate_base, c, r_u) * r_y);
+                for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
+                    const auto v = r.take(c, true);
+#pragma unroll
+                    for (int k = 0; k < ANY; ++k) s1 += c + 1024 * k < a.C ? v.dh[k] * v.pre[k] * (v.y[k] * r_y) : 0.0f;
+                }
                 s1 = team.sum(s1) * a.inv_c;
             }
-            auto through = [&](int c, float &dh_m) {  // dx of channel c
-                float d = a.dy ? (float)((const T *)a.dy)[base + c] : 0.0f;
-                if (a.dh) {
-                    const float m = residual_sum_element<T>(a, base, gate_base, c, r_u) * r_y, dh = (float)((const T *)a.dh)[base + c];
-                    dh_m = dh * m;
-                    d += r_y * (dh * (a.pre ? a.pre[c] : 1.0f) - m * s1);
+            for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
+                const auto v = r.take(c, true);
+                float post[ANY], pre[ANY], gate[ANY];  // the sums so far
+#pragma unroll
+                for (int k = 0; k < ANY; ++k) {
+                    const int at = r.column(c, k);
+                    post[k] = dpost ? dpost[at] : 0.0f, pre[k] = dpre ? dpre[at] : 0.0f, gate[k] = dgate && row > r0 ? dgate[at] : 0.0f;
                 }
-                return d;
-            };
-            for (int c = threadIdx.x; c < a.C; c += 1024) {
-                float dh_m = 0;
-                const float d = through(c, dh_m);
-                if (dpre) dpre[c] += dh_m;
-                if (a.dx) ((T *)a.dx)[base + c] = (T)d;
-                if (!a.u) continue;
-                const float n = (float)((const T *)a.u)[base + c] * r_u, post = (a.post ? a.post[c] : 1.0f) * a.scale;
-                const float open = a.gate ? opened((float)((const T *)a.gate)[gate_base + c], a.act) : 1.0f, db = d * open;
-                if (dpost) dpost[c] += db * n * a.scale;
-                s2 += db * post * n;
-                if (a.dgate) {
-                    float dg = d * (n * post);
-                    if (a.act) dg *= open * (1.0f - open);
-                    if (dgate) dgate[c] = row == r0 ? dg : dgate[c] + dg;
-                    else ((T *)a.dgate)[base + c] = (T)dg;
+#pragma unroll
+                for (int k = 0; k < ANY; ++k) {
+                    const int at = c + 1024 * k;
+                    if (at >= a.C) break;
+                    const float d = r.through(v, k, r_y, s1), db = d * v.open[k];
+                    if (dpre) dpre[at] = pre[k] + v.dh[k] * (v.y[k] * r_y);
+                    if (a.dx) ((T *)a.dx)[r.base + at] = (T)d;
+                    if (!a.u) continue;
+                    if (dpost) dpost[at] = post[k] + db * v.n[k] * a.scale;
+                    s2 += db * v.post[k] * v.n[k];
+                    if (a.dgate) {
+                        float dg = d * (v.n[k] * v.post[k]);
+                        if (a.act) dg *= v.open[k] * (1.0f - v.open[k]);
+                        if (dgate) dgate[at] = gate[k] + dg;
+                        else ((T *)a.dgate)[r.base + at] = (T)dg;
+                    }
                 }
             }
             if (!a.du) continue;
             s2 = team.sum(s2) * a.inv_c;
-            for (int c = threadIdx.x; c < a.C; c += 1024) {
-                float unused;
-                const float n = (float)((const T *)a.u)[base + c] * r_u, post = (a.post ? a.post[c] : 1.0f) * a.scale;
-                const float open = a.gate ? opened((float)((const T *)a.gate)[gate_base + c], a.act) : 1.0f;
-                ((T *)a.du)[base + c] = (T)(r_u * (through(c, unused) * open * post - n * s2));
+            for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
+                const auto v = r.take(c, true);
+#pragma unroll
+                for (int k = 0; k < ANY; ++k)
+                    if (c + 1024 * k < a.C) ((T *)a.du)[r.base + c + 1024 * k] = (T)(r.r_u * (r.through(v, k, r_y, s1) * v.open[k] * v.post[k] - v.n[k] * s2));
             }
         }
     }

@@ -150,8 +150,9 @@ def test_gates(dev, shape, act, gate):
 
 @pytest.mark.parametrize('gate', ['none', 'element', 'sample'])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
-def test_several_rows_of_a_workgroup_that_keeps_its_sums_in_lds(dev, dtype, gate):
+def test_several_rows_of_a_workgroup_that_keeps_its_sums_in_lds_or_memory(dev, dtype, gate):
     _run(dev, (2, 300, 4600), dtype, gate, 'sigmoid', 31)
+    _run(dev, (2, 150, 8300), dtype, gate, None, 32)
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
