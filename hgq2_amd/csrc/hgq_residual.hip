@@ -587,8 +587,7 @@ ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample, bool 
     p.tpr = 1;
     while (p.tpr * RES_HELD < C && p.tpr < 64) p.tpr *= 2;
     if (p.tpr * RES_HELD < C) p.tpr = C > RES_WIDEST ? 1024 : (C + 64 * RES_HELD - 1) / (64 * RES_HELD) * 64;
-    p.threads = p.tpr > 256 ? p.tpr : 256;
-    if (p.tpr > 64) p.threads = p.tpr;
+    p.threads = p.tpr > 64 ? p.tpr : 256;
     const int teams = p.tpr > 64 ? 1 : 256 / p.tpr;
     // Workgroups of the backward pass, each with a slice of its own: as many as are resident, fewer where a wavefront holds a row by itself (131072 x 64 float32: 512 39 us, 1024 43,
     // 2048 48; 45930 x 333 float16 gated: 512 61, 768 58, 1024 64; 32768 x 768 bfloat16: 512 116, 1280 74, 2048 74; 32768 x 4096: 512 328, 1024 340)
@@ -629,22 +628,21 @@ auto residual_bwd_of(const ResidualPlan &p, int C) {
 template <typename T, int KIND>
 int forward(ResidualRows a, const ResidualPlan &p, hipStream_t st) {
     const bool wide = p.tpr > 64;
-    const int teams = wide ? 1 : 256 / p.tpr, threads = wide ? p.tpr : 256;
+    const int teams = wide ? 1 : 256 / p.tpr;
     // threads a compute unit, all of them resident: five workgroups of 256 where wavefronts hold rows by themselves (1531 x 30 x 333 float16 with a gate, read anew: 40 us, four
     // 43, eight 44), 1024 where workgroups do (32768 x 4096 bfloat16 with a gate for samples 213 us, 1280 238, 2048 215; 8192 x 8192 102, 138, 107)
     const int64_t most = 256 * (wide ? 1024 : 1280) / p.threads, blocks = (a.rows + teams - 1) / teams, turns = (blocks + most - 1) / most, grid = (blocks + turns - 1) / turns, step = grid * teams;
     a.step_samples = step / a.P, a.step_rows = step % a.P;
     if (a.C > RES_WIDEST) hipLaunchKernelGGL((residual_fwd_any<T>), dim3((unsigned)grid), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((residual_fwd_of<T, KIND>(p, a.C)), dim3((unsigned)grid), dim3(threads), 0, st, a);
+    else hipLaunchKernelGGL((residual_fwd_of<T, KIND>(p, a.C)), dim3((unsigned)grid), dim3(p.threads), 0, st, a);
     return check_launch("hgq_residual_norm_fwd");
 }
 
 template <typename T, int KIND>
 int backward(const ResidualRows &a, const ResidualPlan &p, float *dpost, float *dpre, hipStream_t st) {
     const char *what = "hgq_residual_norm_bwd";
-    const bool wide = p.tpr > 64;
     if (a.C > RES_WIDEST) hipLaunchKernelGGL((residual_bwd_any<T>), dim3(p.grid), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((residual_bwd_of<T, KIND>(p, a.C)), dim3(p.grid), dim3(wide ? p.tpr : 256), 0, st, a);
+    else hipLaunchKernelGGL((residual_bwd_of<T, KIND>(p, a.C)), dim3(p.grid), dim3(p.threads), 0, st, a);
     int rc = check_launch(what);
     if (!rc && a.slices) {
         hipLaunchKernelGGL(residual_join<float>, dim3((unsigned)((2 * (int64_t)a.C + 15) / 16)), dim3(1024), 0, st, (const float *)a.slices, (int64_t)p.grid, 2 * a.C, a.C, dpost, dpre);
