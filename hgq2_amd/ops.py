@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 import struct
 import threading
 from array import array
@@ -3628,7 +3629,7 @@ def relative_bias(scores: Tensor, table: Tensor, max_distance: int = 128, bidire
     _need(n <= 128, f'at most 128 buckets, got {n}')
     _need(not bidirectional or n % 2 == 0, f'both directions have as many buckets: an even number, got {n}')
     first = relative_buckets(n // 2 if bidirectional else n, int(max_distance))
-    at, each = (0, offset) if isinstance(offset, Tensor) else (int(offset), None)
+    at, each = (0, offset) if isinstance(offset, Tensor) else (operator.index(offset), None)
     _need(-(1 << 62) < at < 1 << 62, 'offset is out of range')
     return _lib.native().relative_bias(scores, table, first, bool(bidirectional), at, each)
 

@@ -133,6 +133,8 @@ def test_python_refusals():
         ops.relative_bias(s, t, (1 << 30) + 1)
     with pytest.raises(ValueError, match='two buckets'):
         ops.relative_bias(s, t[:2], 9)
+    with pytest.raises(TypeError):
+        ops.relative_bias(s, t, 9, offset=2.5)  # (a position is a whole number)
 
     x = torch.zeros(2, 3, 8)
     with pytest.raises(ValueError, match='GPU'):
