@@ -87,9 +87,13 @@ struct RowSums {
     double p, a;
 };
 
+// (a side without entries has the maximum -inf, its factor is exp(-inf) = 0: with a number in place of its -inf the factor overflows beside a low maximum, and
+// zero times that is not a number)
+__device__ __forceinline__ float down_to(float m, float most, float k) { return __builtin_amdgcn_exp2f((m - base_of(most)) * k); }
+
 __device__ __forceinline__ MaxSum team_join(MaxSum v, int width, float k) {
     const float m = team_max(v.m, width);
-    return {m, team_sum(v.s * __builtin_amdgcn_exp2f((base_of(v.m) - base_of(m)) * k), width)};
+    return {m, team_sum(v.s * down_to(v.m, m, k), width)};
 }
 
 __device__ __forceinline__ RowSums team_join(const RowSums &v, int width, float k) {
@@ -346,7 +350,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void distill_rows(const Dist
                 for (int c = lane; c < a.n_parts; c += TPR) {
                     const float2 q = a.parts[row * a.n_parts + c];
                     if (q.x > r.m) r.s *= __builtin_amdgcn_exp2f((r.m - q.x) * a.k_hi), r.m = q.x;
-                    r.s += q.y * __builtin_amdgcn_exp2f((base_of(q.x) - base_of(r.m)) * a.k_hi);
+                    r.s += q.y * down_to(q.x, r.m, a.k_hi);
                 }
             }
             if (!REST || FROM != FROM_ROW) {
