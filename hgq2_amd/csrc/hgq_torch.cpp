@@ -416,13 +416,18 @@ bool whole_planes(const Tensor &t) {
     return t.numel() == 0 || ((t.size(3) == 1 || t.stride(3) == 1) && (t.size(2) == 1 || t.stride(2) == t.size(3)) && t.stride(0) >= 0 && t.stride(1) >= 0);
 }
 
+// one for each of the batch
+void offsets_fit(const Tensor &offsets, int64_t B, c10::Device device) {
+    TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.size(0) == B && offsets.device() == device && offsets.is_contiguous() &&
+                          (offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong),
+                      "offset must be a number, or a contiguous int32 or int64 tensor with one for each of the batch on ", device, ", got ", offsets.scalar_type(), " ", offsets.sizes());
+}
+
 BiasSizes bias_sizes(const char *name, const Tensor &x, const Tensor &offsets, at::IntArrayRef first) {
     on_gpu(name, x);
     TORCH_CHECK_VALUE(x.dim() == 4, name, " must be [batch, heads, queries, keys], got ", x.sizes());
     TORCH_CHECK_VALUE(whole_planes(x), name, ": a head's queries and keys must be contiguous");
-    TORCH_CHECK_VALUE(offsets.numel() == 0 || (offsets.dim() == 1 && offsets.numel() == x.size(0) && offsets.device() == x.device() && offsets.is_contiguous() &&
-                                               (offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong)),
-                      "offset must be a number, or a contiguous int32 or int64 tensor with one for each of the batch on ", x.device(), ", got ", offsets.scalar_type(), " ", offsets.sizes());
+    if (offsets.numel()) offsets_fit(offsets, x.size(0), x.device());
     BiasSizes s = {x.size(0), x.size(1), x.size(2), x.size(3), type_code(x.scalar_type()), (int)first.size() + 1, {}};
     for (const int64_t f : first) s.first.push_back(f > INT32_MAX ? INT32_MAX : (int)f);
     return s;
@@ -491,6 +496,7 @@ struct RelativeBias : torch::autograd::Function<RelativeBias> {
 
 Tensor relative_bias(const Tensor &scores, const Tensor &table, std::vector<int64_t> first, bool both, int64_t offset, const std::optional<Tensor> &offsets) {
     TORCH_CHECK_VALUE(scores.dim() == 3 || scores.dim() == 4, "scores must be [heads, queries, keys] or [batch, heads, queries, keys], got ", scores.sizes());
+    if (offsets) offsets_fit(*offsets, scores.dim() == 4 ? scores.size(0) : 1, scores.device());  // (one without elements is none to the operators, not to a caller)
     const bool graph = differentiated(scores) || differentiated(table);
     if (graph) accumulates_here("scores", scores), accumulates_here("table", table);
     const Tensor x = planes(scores.dim() == 3 ? scores.unsqueeze(0) : scores);

@@ -254,3 +254,13 @@ def test_recording_beside_a_living_graph_is_refused(dev):
         with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
             ops.relative_bias(s, t, 9)
     del living
+
+
+def test_an_offset_for_each_of_no_sequences_and_none_for_some(dev):
+    from hgq2_amd import ops
+
+    table = torch.randn(8, 2, device=dev)
+    none = torch.empty(0, dtype=torch.long, device=dev)
+    assert ops.relative_bias(torch.empty(0, 2, 3, 4, device=dev), table, 9, offset=none).shape == (0, 2, 3, 4)
+    with pytest.raises(ValueError, match='offset must be'):
+        ops.relative_bias(torch.zeros(32, 2, 1, 4, device=dev), table, 9, offset=none)

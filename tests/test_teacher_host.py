@@ -156,6 +156,17 @@ def test_python_refusals():
             ops.residual_norm(x, x, gate=gate)
 
 
+@pytest.mark.parametrize('offset', [torch.empty(0, dtype=torch.long), torch.zeros(2, dtype=torch.long), torch.zeros(4, dtype=torch.int32), torch.zeros((), dtype=torch.long),
+                                    torch.zeros(3, 1, dtype=torch.long), torch.zeros(6, dtype=torch.long)[::2], torch.zeros(3), torch.zeros(3, dtype=torch.int16)])
+def test_offsets_that_are_not_one_for_each_sequence(offset):
+    with pytest.raises(ValueError, match='offset must be'):
+        ops.relative_bias(torch.zeros(3, 2, 3, 4), torch.zeros(4, 2), 9, offset=offset)
+    with pytest.raises(ValueError, match='offset must be'):
+        ops.relative_bias(torch.zeros(2, 3, 4), torch.zeros(4, 2), 9, offset=offset)
+    with pytest.raises(ValueError, match='GPU'):  # (one that is)
+        ops.relative_bias(torch.zeros(3, 2, 3, 4), torch.zeros(4, 2), 9, offset=torch.zeros(3, dtype=torch.long))
+
+
 @pytest.mark.parametrize('n,far', [(2, 2), (2, 100), (3, 9), (8, 40), (16, 128), (32, 128), (32, 33), (64, 500), (20, 1 << 30)])
 def test_first_distances(n, far):
     """The definition bucket by bucket, in whole numbers: the bucket of a distance is how many first distances are not above it."""
