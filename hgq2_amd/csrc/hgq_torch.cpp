@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/hgq_hip.h"
@@ -429,7 +430,7 @@ BiasSizes bias_sizes(const char *name, const Tensor &x, const Tensor &offsets, a
     TORCH_CHECK_VALUE(whole_planes(x), name, ": a head's queries and keys must be contiguous");
     if (offsets.numel()) offsets_fit(offsets, x.size(0), x.device());
     BiasSizes s = {x.size(0), x.size(1), x.size(2), x.size(3), type_code(x.scalar_type()), (int)first.size() + 1, {}};
-    for (const int64_t f : first) s.first.push_back(f > INT32_MAX ? INT32_MAX : (int)f);
+    for (const int64_t f : first) s.first.push_back((int)std::clamp<int64_t>(f, -1, INT32_MAX));  // (what is none stays none)
     return s;
 }
 

@@ -264,3 +264,14 @@ def test_an_offset_for_each_of_no_sequences_and_none_for_some(dev):
     assert ops.relative_bias(torch.empty(0, 2, 3, 4, device=dev), table, 9, offset=none).shape == (0, 2, 3, 4)
     with pytest.raises(ValueError, match='offset must be'):
         ops.relative_bias(torch.zeros(32, 2, 1, 4, device=dev), table, 9, offset=none)
+
+
+@pytest.mark.parametrize('first', [[1, 2, 5 - 2**32], [1 - 2**32, 2, 5], [1, 2, 5 + 2**32], [1, 2, -5]])
+def test_first_distances_of_the_operators_that_are_none(dev, first):
+    from hgq2_amd import _lib
+
+    s, t = torch.zeros(1, 2, 3, 4, device=dev), torch.zeros(8, 2, device=dev)
+    with pytest.raises(_lib.HGQLibraryError, match='first distances'):
+        torch.ops.hgq.relative_bias_fwd(s, t, None, 0, first, True)
+    with pytest.raises(_lib.HGQLibraryError, match='first distances'):
+        torch.ops.hgq.relative_bias_bwd(s, None, 0, first, True)
