@@ -8,7 +8,8 @@
 //
 // Bound by memory.  One pass each way: a row's elements stay in registers, eight a thread, while a team of as many threads as the row needs
 // forms both means; the backward pass forms y again from x (which costs the bytes that y would, and keeps what y's rounding drops).  Sums over rows stay
-// in registers while a workgroup goes from row to row, and leave as one slice per workgroup, added in a fixed order.
+// in registers while a workgroup goes from row to row, and leave in slices, at least one a workgroup and one for 64 rows of a thread, which are joined in 64 bits in a fixed order.
+#include <algorithm>
 #include <type_traits>
 
 #include "hgq_host.h"
@@ -24,12 +25,12 @@ struct ResidualRows {
     const float *post, *pre;
     void *y, *h, *dx, *du, *dgate;
     float *r_u, *r_y;
-    float *slices;       // [workgroups][2][C]: dpost, dpre
+    float *slices;       // [..][2][C]: dpost, dpre; a workgroup's j-th one is j workgroups' number behind its first
     float *gate_slices;  // [units][C], or null: dgate is written as it is formed
     int64_t step_samples, step_rows;         // of a workgroup's step over rows, in samples and rows
     int64_t samples;                         // rows of a gate for P rows
     int64_t rows, P, units, per_unit, cuts;  // rows; of a gate's row; what a workgroup takes at a time, its rows; units of a sample
-    int C, tpr, act, by_sample;
+    int C, tpr, act, by_sample, run;  // run: units that a workgroup adds up in a slice
     float scale, eps, inv_c;
 };
 
@@ -244,15 +245,18 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
                     if (held.mine(v, e)) out[held.at[v] + e] = (Out)f[v * H::N + e];
             return;
         }
+        int at = slot * a.C;
+        asm("" : "+v"(at));  // (places in LDS are worked out here, not kept in registers through the rows)
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < H::NV; ++v)
 #pragma unroll
             for (int e = 0; e < H::N; ++e)
-                if (held.mine(v, e)) joined[slot * a.C + held.at[v] + e] = f[v * H::N + e];
+                if (held.mine(v, e)) joined[at + held.at[v] + e] = f[v * H::N + e];
         __syncthreads();
         for (int c = threadIdx.x; c < a.C; c += 256) {
             float s = 0;
+#pragma unroll 8  // (one read after the other takes 2 us of a launch)
             for (int t = 0; t < teams; ++t) s += joined[t * a.C + c];
             out[c] = (Out)s;
         }
@@ -281,114 +285,123 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
     // Where a gate's row stands for a unit's rows, they add up dx n alone: dgate and dpost are that times factors of the unit.
     float open[RES_HELD];
     bool first = true;
+    int slice = blockIdx.x;
+    int taken = 0;  // units in this slice
     Step k = enter(blockIdx.x);
     ask(k);
-    while (k.unit < a.units) {
-        float x[RES_HELD], n[RES_HELD], g[RES_HELD], dy[RES_HELD], dh[RES_HELD];
-        held.take(x, x_raw);
-        if (KIND != NO_UPDATE) held.take(n, u_raw);
-        if (KIND == GATED) held.take(g, g_raw);
-        if (KIND == GATED_SAMPLES && first) {
-            held.take(open, g_raw);
+    while (k.unit < a.units) {  // a slice
+        bool last;
+        do {
+            float x[RES_HELD], n[RES_HELD], g[RES_HELD], dy[RES_HELD], dh[RES_HELD];
+            held.take(x, x_raw);
+            if (KIND != NO_UPDATE) held.take(n, u_raw);
+            if (KIND == GATED) held.take(g, g_raw);
+            if (KIND == GATED_SAMPLES && first) {
+                held.take(open, g_raw);
 #pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) open[e] = opened(open[e], a.act);
-        }
-        held.take(dy, dy_raw);
-        held.take(dh, dh_raw);
-        const float r_u = r_u_next, r_y = r_y_next;
-        const Step now = k;
-        const bool last = k.r + teams >= k.r1;
-        first = last;
-        if (last) k = enter(k.unit + gridDim.x);
-        else k.r += teams;
-        ask(k);  // on its way while these rows are worked on
-        const bool there = now.r + slot < now.r1;
-        const int64_t base = (now.r + slot) * a.C;
-        if (!there) {
-#pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) dy[e] = dh[e] = 0;
-        }
-        if (KIND != NO_UPDATE) {
-            float post[RES_HELD];
-            recall(POST, post);
-#pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) {
-                n[e] *= r_u;
-                float b = n[e] * post[e];
-                if (KIND == GATED) open[e] = opened(g[e], a.act);
-                if (KIND >= GATED) b *= open[e];
-                x[e] += b;
+                for (int e = 0; e < RES_HELD; ++e) open[e] = opened(open[e], a.act);
             }
-        }
-        float s = 0;
-        if (a.dh) {
-            float pre[RES_HELD], dpre[RES_HELD];
-            recall(PRE, pre), recall(DPRE, dpre);
+            held.take(dy, dy_raw);
+            held.take(dh, dh_raw);
+            const float r_u = r_u_next, r_y = r_y_next;
+            const Step now = k;
+            last = k.r + teams >= k.r1;
+            first = last;
+            if (last) k = enter(k.unit + gridDim.x);
+            else k.r += teams;
+            ask(k);  // on its way while these rows are worked on
+            const bool there = now.r + slot < now.r1;
+            const int64_t base = (now.r + slot) * a.C;
+            if (!there) {
 #pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) {
-                x[e] *= r_y;  // m
-                if (there) dpre[e] += dh[e] * x[e];
-                dh[e] *= pre[e];
+                for (int e = 0; e < RES_HELD; ++e) dy[e] = dh[e] = 0;
             }
-            keep(DPRE, dpre);
-            s = team.sum(held.dot(dh, x)) * a.inv_c;
-#pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) dy[e] += r_y * (dh[e] - x[e] * s);
-        }
-        if (a.dx && there) held.store((T *)a.dx + base, dy);
-        if (KIND != NO_UPDATE) {
-            float dn[RES_HELD], post[RES_HELD], dpost[RES_HELD];
-            recall(POST, post);
-            if (KIND != GATED_SAMPLES) recall(DPOST, dpost);
-#pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) {
-                const float db = KIND >= GATED ? dy[e] * open[e] : dy[e];
-                if (there && KIND == GATED_SAMPLES) dgate[e] += dy[e] * n[e];
-                if (there && KIND != GATED_SAMPLES) dpost[e] += db * n[e];
-                dn[e] = db * post[e];
-                if (KIND == GATED) {
-                    open[e] = dy[e] * (n[e] * post[e]) * (a.act ? open[e] * (1.0f - open[e]) : 1.0f);
-                }
-            }
-            if (KIND != GATED_SAMPLES) keep(DPOST, dpost);
-            if (KIND == GATED && a.dgate && there) held.store((T *)a.dgate + base, open);
-            if (a.du) {
-                s = team.sum(held.dot(dn, n)) * a.inv_c;
-#pragma unroll
-                for (int e = 0; e < RES_HELD; ++e) dn[e] = r_u * (dn[e] - n[e] * s);
-                if (there) held.store((T *)a.du + base, dn);
-            }
-            if (KIND == GATED_SAMPLES && last) {
-                recall(POST, post), recall(DPOST, dpost);
+            if (KIND != NO_UPDATE) {
+                float post[RES_HELD];
+                recall(POST, post);
 #pragma unroll
                 for (int e = 0; e < RES_HELD; ++e) {
-                    dpost[e] += dgate[e] * open[e];
-                    dgate[e] *= post[e] * (a.act ? open[e] * (1.0f - open[e]) : 1.0f);
+                    n[e] *= r_u;
+                    float b = n[e] * post[e];
+                    if (KIND == GATED) open[e] = opened(g[e], a.act);
+                    if (KIND >= GATED) b *= open[e];
+                    x[e] += b;
                 }
-                keep(DPOST, dpost);
-                if (!a.dgate) {
-                } else if (a.gate_slices) leave(dgate, a.gate_slices + now.unit * a.C);
-                else leave(dgate, (T *)a.dgate + now.sample * a.C);
-#pragma unroll
-                for (int e = 0; e < RES_HELD; ++e) dgate[e] = 0;
             }
-        }
-    }
-    if (a.slices) {
-        float *out = a.slices + (int64_t)blockIdx.x * 2 * a.C, f[RES_HELD];
-        if (KIND != NO_UPDATE) {
-            recall(DPOST, f);
+            float s = 0;
+            if (a.dh) {
+                float pre[RES_HELD], dpre[RES_HELD];
+                recall(PRE, pre), recall(DPRE, dpre);
 #pragma unroll
-            for (int e = 0; e < RES_HELD; ++e) f[e] *= a.scale;
-            leave(f, out);
+                for (int e = 0; e < RES_HELD; ++e) {
+                    x[e] *= r_y;  // m
+                    if (there) dpre[e] += dh[e] * x[e];
+                    dh[e] *= pre[e];
+                }
+                keep(DPRE, dpre);
+                s = team.sum(held.dot(dh, x)) * a.inv_c;
+#pragma unroll
+                for (int e = 0; e < RES_HELD; ++e) dy[e] += r_y * (dh[e] - x[e] * s);
+            }
+            if (a.dx && there) held.store((T *)a.dx + base, dy);
+            if (KIND != NO_UPDATE) {
+                float dn[RES_HELD], post[RES_HELD], dpost[RES_HELD];
+                recall(POST, post);
+                if (KIND != GATED_SAMPLES) recall(DPOST, dpost);
+#pragma unroll
+                for (int e = 0; e < RES_HELD; ++e) {
+                    const float db = KIND >= GATED ? dy[e] * open[e] : dy[e];
+                    if (there && KIND == GATED_SAMPLES) dgate[e] += dy[e] * n[e];
+                    if (there && KIND != GATED_SAMPLES) dpost[e] += db * n[e];
+                    dn[e] = db * post[e];
+                    if (KIND == GATED) {
+                        open[e] = dy[e] * (n[e] * post[e]) * (a.act ? open[e] * (1.0f - open[e]) : 1.0f);
+                    }
+                }
+                if (KIND != GATED_SAMPLES) keep(DPOST, dpost);
+                if (KIND == GATED && a.dgate && there) held.store((T *)a.dgate + base, open);
+                if (a.du) {
+                    s = team.sum(held.dot(dn, n)) * a.inv_c;
+#pragma unroll
+                    for (int e = 0; e < RES_HELD; ++e) dn[e] = r_u * (dn[e] - n[e] * s);
+                    if (there) held.store((T *)a.du + base, dn);
+                }
+                if (KIND == GATED_SAMPLES && last) {
+                    recall(POST, post), recall(DPOST, dpost);
+#pragma unroll
+                    for (int e = 0; e < RES_HELD; ++e) {
+                        dpost[e] += dgate[e] * open[e];
+                        dgate[e] *= post[e] * (a.act ? open[e] * (1.0f - open[e]) : 1.0f);
+                    }
+                    keep(DPOST, dpost);
+                    if (!a.dgate) {
+                    } else if (a.gate_slices) leave(dgate, a.gate_slices + now.unit * a.C);
+                    else leave(dgate, (T *)a.dgate + now.sample * a.C);
+#pragma unroll
+                    for (int e = 0; e < RES_HELD; ++e) dgate[e] = 0;
+                }
+            }
+        } while (!last || (++taken < a.run && k.unit < a.units));
+        taken = 0;
+        if (a.slices) {
+            float *out = a.slices + (int64_t)slice * 2 * a.C, f[RES_HELD], none[RES_HELD] = {};
+            if (KIND != NO_UPDATE) {
+                recall(DPOST, f);
+#pragma unroll
+                for (int e = 0; e < RES_HELD; ++e) f[e] *= a.scale;
+                leave(f, out);
+                keep(DPOST, none);
+            }
+            recall(DPRE, f);
+            leave(f, out + a.C);
+            keep(DPRE, none);
+            slice += gridDim.x;
         }
-        recall(DPRE, f);
-        leave(f, out + a.C);
     }
 }
 
 // Rows of more channels than a workgroup holds: read again for each of the means, ANY columns of a thread at a time (all their loads ahead of their stores: 4000 x 12000 bfloat16
-// 201 and 442 us, one by one 250 and 875); sums over rows in the workgroup's own slice.
+// 201 and 442 us, one by one 250 and 875); sums over rows in the workgroup's own slices, means' sums in 64 bits beyond four columns.
 constexpr int ANY = 4;
 
 template <typename T>
@@ -413,6 +426,13 @@ struct AnyRow {
 #pragma unroll
         for (int k = 0; k < ANY; ++k) f[k] = from ? from[column(c, k)] : 1.0f;
     }
+    // the sum of products over these columns: a thread adds up such sums in 64 bits (it has as many as a row is long)
+    __device__ __forceinline__ float dot(const float *f, const float *g, int c) const {
+        float s = 0;
+#pragma unroll
+        for (int k = 0; k < ANY; ++k) s += c + 1024 * k < a.C ? f[k] * g[k] : 0.0f;
+        return s;
+    }
     __device__ __forceinline__ Columns take(int c, bool gradients) const {
         Columns v;
         one(v.y, a.x, base, c), one(v.n, a.u, base, c), one(v.open, a.gate, gate_base, c);
@@ -435,23 +455,21 @@ __global__ __launch_bounds__(1024) void residual_fwd_any(const ResidualRows a) {
     RowTeam<true> team(1024, lds);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         AnyRow<T> r = {a, row * a.C, a.by_sample ? row / a.P * a.C : row * a.C, 0.0f};
-        float s = 0;
+        double s = 0;
         if (a.u) {
             for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
                 float u[ANY];
                 r.one(u, a.u, r.base, c);
-#pragma unroll
-                for (int k = 0; k < ANY; ++k) s += c + 1024 * k < a.C ? u[k] * u[k] : 0.0f;
+                s += r.dot(u, u, c);
             }
-            r.r_u = norm_factor(team.sum(s), a.inv_c, a.eps);
+            r.r_u = norm_factor(team.sum((float)s), a.inv_c, a.eps);
             s = 0;
         }
         for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
             const auto v = r.take(c, false);
-#pragma unroll
-            for (int k = 0; k < ANY; ++k) s += c + 1024 * k < a.C ? v.y[k] * v.y[k] : 0.0f;
+            s += r.dot(v.y, v.y, c);
         }
-        const float r_y = norm_factor(team.sum(s), a.inv_c, a.eps);
+        const float r_y = norm_factor(team.sum((float)s), a.inv_c, a.eps);
         for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
             const auto v = r.take(c, false);
 #pragma unroll
@@ -473,24 +491,29 @@ template <typename T>
 __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
     __shared__ float lds[2][16];
     RowTeam<true> team(1024, lds);
-    float *dpost = a.slices ? a.slices + (int64_t)blockIdx.x * 2 * a.C : nullptr, *dpre = dpost ? dpost + a.C : nullptr;
-    if (dpost)
-        for (int c = threadIdx.x; c < 2 * a.C; c += 1024) dpost[c] = 0;
-    __syncthreads();
+    int slice = blockIdx.x;
+    int taken = 0;  // units in this slice
     for (int64_t unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        if (taken == a.run) taken = 0, slice += gridDim.x;
+        float *dpost = a.slices ? a.slices + (int64_t)slice * 2 * a.C : nullptr, *dpre = dpost ? dpost + a.C : nullptr;
         const int64_t sample = unit / a.cuts, r0 = sample * a.P + (unit - sample * a.cuts) * a.per_unit, r1 = min(min(r0 + a.per_unit, (sample + 1) * a.P), a.rows);
         float *dgate = a.by_sample && a.dgate ? a.gate_slices + unit * a.C : nullptr;
         for (int64_t row = r0; row < r1; ++row) {
             const AnyRow<T> r = {a, row * a.C, a.by_sample ? sample * a.C : row * a.C, a.u ? a.r_u[row] : 0.0f};
             const float r_y = a.r_y[row];
+            const bool fresh = taken == 0 && row == r0;  // (nothing in the slice yet)
             float s1 = 0, s2 = 0;
+            double s = 0;
             if (a.dh) {
                 for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
                     const auto v = r.take(c, true);
+                    float e[ANY], m[ANY];
 #pragma unroll
-                    for (int k = 0; k < ANY; ++k) s1 += c + 1024 * k < a.C ? v.dh[k] * v.pre[k] * (v.y[k] * r_y) : 0.0f;
+                    for (int k = 0; k < ANY; ++k) e[k] = v.dh[k] * v.pre[k], m[k] = v.y[k] * r_y;
+                    s += r.dot(e, m, c);
                 }
-                s1 = team.sum(s1) * a.inv_c;
+                s1 = team.sum((float)s) * a.inv_c;
+                s = 0;
             }
             for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
                 const auto v = r.take(c, true);
@@ -498,8 +521,9 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
 #pragma unroll
                 for (int k = 0; k < ANY; ++k) {
                     const int at = r.column(c, k);
-                    post[k] = dpost ? dpost[at] : 0.0f, pre[k] = dpre ? dpre[at] : 0.0f, gate[k] = dgate && row > r0 ? dgate[at] : 0.0f;
+                    post[k] = dpost && !fresh ? dpost[at] : 0.0f, pre[k] = dpre && !fresh ? dpre[at] : 0.0f, gate[k] = dgate && row > r0 ? dgate[at] : 0.0f;
                 }
+                float among = 0;
 #pragma unroll
                 for (int k = 0; k < ANY; ++k) {
                     const int at = c + 1024 * k;
@@ -509,7 +533,7 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
                     if (a.dx) ((T *)a.dx)[r.base + at] = (T)d;
                     if (!a.u) continue;
                     if (dpost) dpost[at] = post[k] + db * v.n[k] * a.scale;
-                    s2 += db * v.post[k] * v.n[k];
+                    among += db * v.post[k] * v.n[k];
                     if (a.dgate) {
                         float dg = d * (v.n[k] * v.post[k]);
                         if (a.act) dg *= v.open[k] * (1.0f - v.open[k]);
@@ -517,9 +541,10 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
                         else ((T *)a.dgate)[r.base + at] = (T)dg;
                     }
                 }
+                s += among;
             }
             if (!a.du) continue;
-            s2 = team.sum(s2) * a.inv_c;
+            s2 = team.sum((float)s) * a.inv_c;
             for (int c = threadIdx.x; c < a.C; c += 1024 * ANY) {
                 const auto v = r.take(c, true);
 #pragma unroll
@@ -527,6 +552,7 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
                     if (c + 1024 * k < a.C) ((T *)a.du)[r.base + c + 1024 * k] = (T)(r.r_u * (r.through(v, k, r_y, s1) * v.open[k] * v.post[k] - v.n[k] * s2));
             }
         }
+        ++taken;
     }
 }
 
@@ -576,9 +602,11 @@ int check_residual(const char *what, int64_t rows, int64_t P, int64_t C, float s
     return HGQ_OK;
 }
 
+constexpr int RES_TERMS = 64;  // rows that a thread adds up one after the other, at most
+
 struct ResidualPlan {
-    int tpr, threads, grid;
-    int64_t units, per_unit, cuts;
+    int tpr, threads, grid, run;
+    int64_t units, per_unit, cuts, slices;
 };
 
 // by_sample: a unit has rows of one sample, whose gate's gradient it adds up
@@ -597,15 +625,19 @@ ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample, bool 
         p.cuts = samples < most ? (most + samples - 1) / samples : 1;
         const int64_t fewest = 2 * teams;  // rows that pay for a slice
         if (p.cuts > (P + fewest - 1) / fewest) p.cuts = (P + fewest - 1) / fewest;
-        p.per_unit = (P + p.cuts - 1) / p.cuts;
+        p.per_unit = std::min<int64_t>((P + p.cuts - 1) / p.cuts, RES_TERMS * teams);
         p.cuts = (P + p.per_unit - 1) / p.per_unit;
         p.units = samples * p.cuts;
     } else {
         p.per_unit = (rows + most - 1) / most;
-        p.per_unit = (p.per_unit + teams - 1) / teams * teams;
+        p.per_unit = std::min<int64_t>((p.per_unit + teams - 1) / teams * teams, RES_TERMS * teams);
         p.cuts = p.units = (rows + p.per_unit - 1) / p.per_unit;
     }
     p.grid = (int)(p.units < most ? p.units : most);
+    // (of many rows a workgroup leaves several slices: what a thread adds up does not grow with the rows.  A slice takes as much as two rows in fp32, for 64 or more of them.)
+    p.run = (int)(RES_TERMS / ((p.per_unit + teams - 1) / teams));
+    const int64_t turns = (p.units + p.grid - 1) / p.grid, runs = (turns + p.run - 1) / p.run, before = (runs - 1) * p.grid;
+    p.slices = before + std::min<int64_t>(p.grid, p.units - before * p.run);
     return p;
 }
 
@@ -645,7 +677,7 @@ int backward(const ResidualRows &a, const ResidualPlan &p, float *dpost, float *
     else hipLaunchKernelGGL((residual_bwd_of<T, KIND>(p, a.C)), dim3(p.grid), dim3(p.threads), 0, st, a);
     int rc = check_launch(what);
     if (!rc && a.slices) {
-        hipLaunchKernelGGL(residual_join<float>, dim3((unsigned)((2 * (int64_t)a.C + 15) / 16)), dim3(1024), 0, st, (const float *)a.slices, (int64_t)p.grid, 2 * a.C, a.C, dpost, dpre);
+        hipLaunchKernelGGL(residual_join<float>, dim3((unsigned)((2 * (int64_t)a.C + 15) / 16)), dim3(1024), 0, st, (const float *)a.slices, p.slices, 2 * a.C, a.C, dpost, dpre);
         rc = check_launch(what);
     }
     if (!rc && a.gate_slices) {
@@ -701,7 +733,7 @@ extern "C" int64_t hgq_residual_norm_bwd_workspace(int64_t rows, int64_t P, int6
     for (int kind = 0; kind < 3; ++kind) {  // no gate, one like x, one for a sample's rows
         const bool by_sample = kind == 2 && P > 1;
         const ResidualPlan p = residual_plan(rows, P, (int)C, by_sample, kind > 0);
-        const int64_t floats = 2 * p.grid * C + (by_sample && slices_of_gate(p, (int)C) ? p.units * C : 0);
+        const int64_t floats = 2 * p.slices * C + (by_sample && slices_of_gate(p, (int)C) ? p.units * C : 0);
         most = floats > most ? floats : most;
     }
     return most;
@@ -724,8 +756,8 @@ extern "C" int hgq_residual_norm_bwd(const void *dy, const void *dh, const void 
     ResidualRows a = {};
     a.x = x, a.u = u, a.gate = gate, a.dy = dy, a.dh = dh, a.post = post, a.pre = pre, a.dx = dx, a.du = du, a.dgate = dgate;
     a.r_u = (float *)r_u, a.r_y = (float *)r_y, a.slices = dpost || dpre ? workspace : nullptr;
-    a.gate_slices = dgate && P > 1 && slices_of_gate(p, (int)C) ? workspace + 2 * p.grid * C : nullptr;
-    a.rows = rows, a.P = P > 1 ? P : rows, a.units = p.units, a.per_unit = p.per_unit, a.cuts = p.cuts;
+    a.gate_slices = dgate && P > 1 && slices_of_gate(p, (int)C) ? workspace + 2 * p.slices * C : nullptr;
+    a.rows = rows, a.P = P > 1 ? P : rows, a.units = p.units, a.per_unit = p.per_unit, a.cuts = p.cuts, a.run = p.run;
     a.C = (int)C, a.tpr = p.tpr, a.act = act, a.by_sample = P > 1, a.samples = rows / P, a.scale = scale, a.eps = eps, a.inv_c = (float)(1.0 / (double)C);
     const int kind = !u ? NO_UPDATE : !gate ? NO_GATE : P > 1 ? GATED_SAMPLES : GATED;
     return (type == HGQ_TYPE_F32 ? backward_of<float>(kind) : type == HGQ_TYPE_BF16 ? backward_of<__bf16>(kind) : backward_of<_Float16>(kind))(a, p, dpost, dpre, st);
