@@ -61,7 +61,8 @@ __device__ __forceinline__ float exp_t(float d, float k_hi, float k_lo) {
 }
 
 // exp(x) and log(x) of numbers in 64 bits with an error of fp32's rounding: what is large of them - whole powers of two - stays in 64 bits.  (The
-// library's take some hundred instructions in 64 bits, for each row more than the row's own where the vocabulary is small.)
+// library's take some hundred instructions in 64 bits, for each row more than the row's own where the vocabulary is small.  The teacher's lse is a number in fp32, whose own
+// half step moves p by as much.)
 __device__ __forceinline__ double exp_64(double x) {
     const double two = x * 1.4426950408889634074, whole = __builtin_rint(two);
     if (!(two > -1000.0)) return two != two ? two : 0.0;

@@ -336,7 +336,7 @@ void cut(BiasShape &s, int64_t threads, int64_t wanted, const void *base, int64_
     s.tiles = (int)((s.TS + s.align - 1 + per - 1) / per);
 }
 
-int sums_threads(int n) { return n <= 16 ? 256 : n <= 32 ? 128 : 64; }  // 32 KB of bins up to 64 buckets: five workgroups a compute unit
+int sums_threads(int n) { return n <= 16 ? 256 : n <= 32 ? 128 : 64; }  // 32 KB of bins with 16, 32 and 64 buckets: four workgroups a compute unit, three beside the longest table of distances
 
 int sums_parts(const BiasShape &s, int threads, int tiles) {
     const int64_t items = (int64_t)((s.tiles + tiles - 1) / tiles) * s.chunks;

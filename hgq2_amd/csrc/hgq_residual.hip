@@ -56,14 +56,17 @@ struct RowTeam {
     }
 };
 
-// (the hardware's root, a unit in the last place off, and a product with 1 / C: rounded ones are a fifth of a short row's instructions; 1531 x 30 x 333 float16 with a gate: 37 and 57 us
-// with them, 34 and 56 so)
+// (the hardware's root, a unit in the last place off, and a product with 1 / C: with the root refined to half a unit float32 outputs and gradients are no nearer to 64 bits,
+// their errors' mean squares within a tenth either way.  Rounded ones take 1531 x 30 x 333 float16 with a gate forward 33.3 us, these 30.7, 32768 x 1536 bfloat16 91.8 and 89.2; backward no
+// difference.  Times here and below are GPU times of whole calls, joins included, with the same inputs each time unless they are said to be read anew.)
 __device__ __forceinline__ float norm_factor(float sum, float inv_c, float eps) {
     const float square = sum * inv_c + eps;
     const bool tiny = square < 0x1p-100f;  // (without an epsilon: the root takes numbers below fp32's normal ones for zero)
     return __builtin_amdgcn_rsqf(tiny ? square * 0x1p100f : square) * (tiny ? 0x1p50f : 1.0f);
 }
 
+// (the hardware's exponential and reciprocal, a unit each, and an exponent off by |g| 2^-24, which the sigmoid's own slope makes less: 16-bit types do not show it, and float32
+// gradients are nearer to 64 bits than elementary operations get them)
 __device__ __forceinline__ float opened(float g, int act) { return act ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269502f)) : g; }
 
 // A thread's eight elements of a row.  A row's last access ends with the row: its first elements are the neighbour's again, which are left out of sums and written
@@ -130,8 +133,8 @@ struct Held {
     }
 };
 
-// rows of less than one access; of a wavefront (257 .. 512 channels), whose addresses are then scalars (1531 x 30 x 333 float16 backward: 72 -> 68 us with a gate, 63 -> 54 without);
-// all others
+// rows of less than one access; of a wavefront (257 .. 512 channels), whose addresses are then scalars (1531 x 30 x 333 float16 backward, read anew: 65 -> 62 us with a gate, 56 -> 53
+// without; forward 32 -> 31 and 26 -> 25); all others
 enum { TINY_ROWS, WAVE_ROWS, ROWS };
 enum { NO_UPDATE, NO_GATE, GATED, GATED_SAMPLES };  // the last: one row of a gate for P rows
 
@@ -199,7 +202,7 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
     const H held(lane, tpr, a.C);
     RowTeam<WIDE> team(tpr, lds);
     // What a thread keeps from row to row of its columns' post, pre, dpost and dpre.  With 1024 threads, which have 128 registers each, it lies in LDS, where no other
-    // thread looks at it (8192 x 8192 bfloat16, a gate like x: 233 us instead of 330 with 32 registers spilled).
+    // thread looks at it (8192 x 8192 bfloat16, a gate like x: 233 us instead of 330 with 32 registers spilled; float32 with a gate still spills 2, with one for samples 10).
     constexpr bool STASH = THREADS == 1024 && KIND != NO_UPDATE;
     __shared__ float4 stash[STASH ? 4 : 1][RES_HELD / 4][STASH ? THREADS : 1];
     enum { POST, PRE, DPOST, DPRE };
@@ -617,8 +620,10 @@ ResidualPlan residual_plan(int64_t rows, int64_t P, int C, bool by_sample, bool 
     if (p.tpr * RES_HELD < C) p.tpr = C > RES_WIDEST ? 1024 : (C + 64 * RES_HELD - 1) / (64 * RES_HELD) * 64;
     p.threads = p.tpr > 64 ? p.tpr : 256;
     const int teams = p.tpr > 64 ? 1 : 256 / p.tpr;
-    // Workgroups of the backward pass, each with a slice of its own: as many as are resident, fewer where a wavefront holds a row by itself (131072 x 64 float32: 512 39 us, 1024 43,
-    // 2048 48; 45930 x 333 float16 gated: 512 61, 768 58, 1024 64; 32768 x 768 bfloat16: 512 116, 1280 74, 2048 74; 32768 x 4096: 512 328, 1024 340)
+    // Workgroups of the backward pass.  Of two wavefronts: five a compute unit, as are resident (32768 x 768 bfloat16: 512 116 us, 1280 74, 2048 74).  Of three and
+    // four: two, three with a gate, fewer than are resident (with four a compute unit 32768 x 1536 bfloat16 takes 139 instead of 134 us, 16384 x 1536 float32 133 and 131, 32768 x 2048
+    // bfloat16 gated 249 and 240).  Of five to eight two, of more one (32768 x 4096: two 328, four 340).  Where wavefronts hold rows by themselves the same: each has a slice to join (131072 x
+    // 64 float32: two 39, four 43, eight 48; 45930 x 333 float16 gated, read anew: two 66, three 62, four 67).
     const int64_t most = 256 * (p.threads > 512 ? 1 : p.threads > 256 ? 2 : p.threads == 128 ? 5 : gated ? 3 : 2);
     if (by_sample) {
         const int64_t samples = rows / P;
