@@ -258,10 +258,10 @@ __global__ __launch_bounds__(THREADS) void residual_bwd(const ResidualRows a) {
                 if (held.mine(v, e)) joined[at + held.at[v] + e] = f[v * H::N + e];
         __syncthreads();
         for (int c = threadIdx.x; c < a.C; c += 256) {
-            float s = 0;
+            double s = 0;  // (up to 256 teams)
 #pragma unroll 8  // (one read after the other takes 2 us of a launch)
             for (int t = 0; t < teams; ++t) s += joined[t * a.C + c];
-            out[c] = (Out)s;
+            out[c] = (Out)(float)s;
         }
     };
 

@@ -1,8 +1,8 @@
 """Norms around a residual sum: sums do not lose more as rows, or channels beyond what a workgroup holds, become many.
 
 u = 2^-24.  Rows of ones have norms of one (relatively off by 4 u: the mean, the root, the product), so with an upstream gradient c in every place dpost and dpre are
-rows * c and a sample's dgate its rows * c.  A thread adds at most 64 rows one after the other, teams of a workgroup (256 threads over the row's threads) meet one after the
-other, 64 bits join the rest: 64 + teams u; a gate's sums meet once more over a slice's units, at most 64 in all with the rows: 2 u, and the factors 8 u.  c has the property that adding
+rows * c and a sample's dgate its rows * c.  A thread adds at most 64 rows one after the other, 64 bits join teams of a workgroup (256 threads over the
+row's threads) and the rest: 64 u (and one for each team, which they were once allowed); a gate's sums meet once more over a slice's units, at most 64 in all with the rows: 2 u, and the factors 8 u.  c has the property that adding
 it up 512 times in fp32 is off by 128 u, a bias that grows with every further row."""
 
 import pytest
@@ -35,6 +35,22 @@ def test_sums_over_many_rows(dev, batch, positions, channels, gate):
         assert float((grads[1].double() / (positions * C0) - 1).abs().max()) <= tol
     (got,) = torch.autograd.grad(h, [pre], c)
     assert float((got.double() - want).abs().max()) <= tol * want, float((got.double() / want - 1).abs().max()) / U
+
+
+@pytest.mark.parametrize('rows,channels,gate', [(1 << 17, 8, None), (1 << 17, 8, 'sample'), (1 << 17, 3, None), (1 << 16, 16, 'element')])
+def test_sums_of_many_teams(dev, rows, channels, gate):
+    """A row or two a thread, 128 or 256 teams a workgroup, which meet in 64 bits: 2 + 14 u.  Adding this c up 256 times in fp32 is off by 64 u."""
+    from hgq2_amd import ops
+
+    c0 = float.fromhex('0x1.ff73p+0')
+    shape = (2, rows // 2, channels)
+    x, c, post = torch.ones(shape, device=dev), torch.full(shape, c0, device=dev), torch.ones(channels, device=dev, requires_grad=True)
+    g = None if gate is None else torch.ones(shape if gate == 'element' else (2, channels), device=dev, requires_grad=gate == 'sample')
+    y, _ = ops.residual_norm(x, x, post, None, g, None, epsilon=0.0)
+    grads = torch.autograd.grad(y, [post] + ([g] if gate == 'sample' else []), c)
+    assert float((grads[0].double() / (rows * c0) - 1).abs().max()) <= 16 * U
+    if gate == 'sample':
+        assert float((grads[1].double() / (rows // 2 * c0) - 1).abs().max()) <= 16 * U
 
 
 @pytest.mark.parametrize('rows,channels,P,gate', [(70, 8208, 1, None), (700, 40, 1, None), (66000, 8, 2, 'sample'), (40000, 333, 400, 'sample'), (3000, 1000, 3, 'sample')])
