@@ -98,3 +98,15 @@ def test_means_of_very_many_channels(dev, channels):
     assert float((y.double() - (float(x[0, 0]) + 1)).abs().max()) <= 24 * U * (v + 1)
     dx, du = torch.autograd.grad([y, h], [x, u], [dh, dh])
     assert float((dx.double() - C0).abs().max()) <= 2 * 24 * U * C0 and float(du.abs().max()) <= 2 * 40 * U * C0 / v
+
+
+def test_gradients_of_more_gammas_than_a_launch_has_threads_for(dev):
+    """Two rows of ones and twos have norms of one: dgamma is the sum of two upstream gradients, exact."""
+    from hgq2_amd import ops
+
+    channels = (1 << 25) + 37
+    x = torch.tensor([[1.0], [2.0]], device=dev).expand(2, channels).contiguous()
+    gamma = torch.ones(channels, device=dev, requires_grad=True)
+    dh = torch.randint(-8, 9, (2, channels), device=dev).float()
+    (dg,) = torch.autograd.grad(ops.rms_norm(x, gamma, epsilon=0.0), [gamma], dh)
+    assert float((dg.double() - dh.double().sum(0)).abs().max()) <= 40 * U * 16  # (the norms' own: 20 u each)
