@@ -272,9 +272,9 @@ __global__ __launch_bounds__(256) void relative_bias_sums(const T *__restrict__ 
     }
 }
 
-// dtable [n, H] from [H][parts][n]: a wavefront for each of its elements
-__global__ __launch_bounds__(256) void relative_bias_join(const double *__restrict__ part, int parts, float *__restrict__ dtable, int n, int H) {
-    const int at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+// dtable [n, H] from [H][parts][n], elements `from` on: a wavefront for each
+__global__ __launch_bounds__(256) void relative_bias_join(const double *__restrict__ part, int parts, float *__restrict__ dtable, int n, int H, int from) {
+    const int at = from + blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (at >= n * H) return;
     const int k = at / H, h = at - k * H;
     double v = 0;
@@ -391,8 +391,13 @@ int sums(const void *dy, float *dtable, double *part, BiasShape s, hipStream_t s
               : seqs == 2 ? sums_of<T, 2, 4, false>
                           : sums_of<T, 1, 8, false>)(dy, part, parts, threads, s, st);
     if (rc) return rc;
-    hipLaunchKernelGGL(relative_bias_join, dim3((unsigned)((n * s.H + 3) / 4)), dim3(256), 0, st, (const double *)part, parts, dtable, n, s.H);
-    return check_launch("hgq_relative_bias_bwd");
+    constexpr int most = 1 << 25;  // elements of a launch (one of 2^32 threads or more runs some of them, and says nothing)
+    for (int from = 0; from < n * s.H && !rc; from += most) {
+        const int left = n * s.H - from, here = left < most ? left : most;
+        hipLaunchKernelGGL(relative_bias_join, dim3((unsigned)((here + 3) / 4)), dim3(256), 0, st, (const double *)part, parts, dtable, n, s.H, from);
+        rc = check_launch("hgq_relative_bias_bwd");
+    }
+    return rc;
 }
 
 }  // namespace

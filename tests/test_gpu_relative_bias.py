@@ -275,3 +275,16 @@ def test_first_distances_of_the_operators_that_are_none(dev, first):
         torch.ops.hgq.relative_bias_fwd(s, t, None, 0, first, True)
     with pytest.raises(_lib.HGQLibraryError, match='first distances'):
         torch.ops.hgq.relative_bias_bwd(s, None, 0, first, True)
+
+
+def test_a_table_of_more_elements_than_a_launch_has_wavefronts(dev):
+    """2^19 + 9 heads of one score each and 128 buckets: the score's bucket takes its gradient, all else is zero."""
+    from hgq2_amd import ops
+
+    heads = (1 << 19) + 9
+    scores, table = torch.zeros(1, heads, 1, 1, device=dev), torch.zeros(128, heads, device=dev, requires_grad=True)
+    dy = torch.randn(1, heads, 1, 1, device=dev)
+    (dt,) = torch.autograd.grad(ops.relative_bias(scores, table, 128, True, offset=-3), [table], dy)
+    assert torch.equal(dt[64 + 3], dy.view(-1))  # (three ahead: the fourth bucket of that half)
+    dt[64 + 3] = 0
+    assert not dt.any()
