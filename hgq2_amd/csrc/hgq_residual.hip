@@ -559,32 +559,28 @@ __global__ __launch_bounds__(1024) void residual_bwd_any(const ResidualRows a) {
     }
 }
 
-// out[b][c] = sum over n of in[b][n][c] (columns 0 .. split - 1 to `out`, the others to `more`; either may be null), 16 columns and 64 runs of rows a workgroup, joined in fp64
+// out[b][c] = sum over n of in[b][n][c] (columns 0 .. split - 1 to `out`, the others to `more`; either may be null) for columns from `first` on, 16 columns and 64 runs of rows a workgroup, joined in fp64
 template <typename T>
-__global__ __launch_bounds__(1024) void residual_join(const float *__restrict__ in, int64_t n, int columns, int split, T *__restrict__ out, T *__restrict__ more) {
+__global__ __launch_bounds__(1024) void residual_join(const float *__restrict__ in, int64_t n, int columns, int split, T *__restrict__ out, T *__restrict__ more, int first) {
     __shared__ double sums[64][17];
-    const int run = threadIdx.x >> 4;
-    for (int c0 = blockIdx.x * 16; c0 < columns; c0 += (int)gridDim.x * 16) {
-        const int c = c0 + (threadIdx.x & 15);
-        const float *from = in + (int64_t)blockIdx.y * n * columns + min(c, columns - 1);
-        double s = 0;
-        for (int64_t k = run; k < n; k += 64 * 8) {
-            float v[8];
+    const int c = first + blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
+    const float *from = in + (int64_t)blockIdx.y * n * columns + min(c, columns - 1);
+    double s = 0;
+    for (int64_t k = run; k < n; k += 64 * 8) {
+        float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k + 64 * j < n ? from[(k + 64 * j) * columns] : 0.0f;
+        for (int j = 0; j < 8; ++j) v[j] = k + 64 * j < n ? from[(k + 64 * j) * columns] : 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[j];
-        }
-        sums[run][threadIdx.x & 15] = s;
-        __syncthreads();
-        if (run == 0 && c < columns) {
-            s = 0;
+        for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    sums[run][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (run == 0 && c < columns) {
+        s = 0;
 #pragma unroll 8
-            for (int r = 0; r < 64; ++r) s += sums[r][threadIdx.x & 15];
-            T *to = c < split ? out : more;
-            if (to) to[(int64_t)blockIdx.y * split + (c < split ? c : c - split)] = (T)(float)s;
-        }
-        if (c0 + (int)gridDim.x * 16 < columns) __syncthreads();  // (the next columns take the same places)
+        for (int r = 0; r < 64; ++r) s += sums[r][threadIdx.x & 15];
+        T *to = c < split ? out : more;
+        if (to) to[(int64_t)blockIdx.y * split + (c < split ? c : c - split)] = (T)(float)s;
     }
 }
 
@@ -610,8 +606,6 @@ int check_residual(const char *what, int64_t rows, int64_t P, int64_t C, float s
 }
 
 constexpr int RES_TERMS = 64;  // rows that a thread adds up one after the other, at most
-
-constexpr int64_t JOIN_WGS = 1 << 20;  // of 1024 threads: a launch of 2^32 threads or more runs some of them, and says nothing
 
 struct ResidualPlan {
     int tpr, threads, grid, run;
@@ -681,6 +675,18 @@ int forward(ResidualRows a, const ResidualPlan &p, hipStream_t st) {
     return check_launch("hgq_residual_norm_fwd");
 }
 
+template <typename T>
+int join(const float *in, int64_t n, unsigned many, int columns, int split, T *out, T *more, hipStream_t st) {
+    constexpr int most = 1 << 25;  // columns of a launch (one of 2^32 threads or more runs some of them, and says nothing)
+    int rc = HGQ_OK;
+    for (int first = 0; first < columns && !rc; first += most) {
+        const int left = columns - first, here = left < most ? left : most;
+        hipLaunchKernelGGL(residual_join<T>, dim3((unsigned)((here + 15) / 16), many), dim3(1024), 0, st, in, n, columns, split, out, more, first);
+        rc = check_launch("hgq_residual_norm_bwd");
+    }
+    return rc;
+}
+
 template <typename T, int KIND>
 int backward(const ResidualRows &a, const ResidualPlan &p, float *dpost, float *dpre, hipStream_t st) {
     const char *what = "hgq_residual_norm_bwd";
@@ -688,8 +694,7 @@ int backward(const ResidualRows &a, const ResidualPlan &p, float *dpost, float *
     else hipLaunchKernelGGL((residual_bwd_of<T, KIND>(p, a.C)), dim3(p.grid), dim3(p.threads), 0, st, a);
     int rc = check_launch(what);
     if (!rc && a.slices) {
-        hipLaunchKernelGGL(residual_join<float>, dim3((unsigned)std::min((2 * (int64_t)a.C + 15) / 16, JOIN_WGS)), dim3(1024), 0, st, (const float *)a.slices, p.slices, 2 * a.C, a.C, dpost, dpre);
-        rc = check_launch(what);
+        rc = join(a.slices, p.slices, 1, 2 * a.C, a.C, dpost, dpre, st);
     }
     if (!rc && a.gate_slices) {
         const int64_t samples = a.rows / a.P;
@@ -698,8 +703,8 @@ int backward(const ResidualRows &a, const ResidualPlan &p, float *dpost, float *
             const float *slices = a.gate_slices + b * p.cuts * a.C;
             T *dgate = (T *)a.dgate + b * a.C;
             if (p.cuts <= 64) hipLaunchKernelGGL(residual_join_few<T>, dim3((unsigned)((a.C + 255) / 256), many), dim3(256), 0, st, slices, (int)p.cuts, a.C, dgate);
-            else hipLaunchKernelGGL(residual_join<T>, dim3((unsigned)std::min<int64_t>((a.C + 15) / 16, JOIN_WGS), many), dim3(1024), 0, st, slices, p.cuts, a.C, a.C, dgate, (T *)nullptr);
-            rc = check_launch(what);
+            else rc = join(slices, p.cuts, many, a.C, a.C, dgate, (T *)nullptr, st);
+            if (!rc) rc = check_launch(what);
         }
     }
     return rc;
