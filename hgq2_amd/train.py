@@ -322,15 +322,18 @@ class AdamW(SGD):
 
 def _each(f, y):
     """``f`` of a batch's targets: of the tensor, or of each of several (``None`` stays)."""
-    return None if y is None else f(y) if isinstance(y, torch.Tensor) else tuple(_each(f, t) for t in y)
+    return None if y is None else f(y) if isinstance(y, torch.Tensor) else tuple(None if t is None else f(t) for t in y)
 
 
 def _copy_batch(to, y):
     if isinstance(to, torch.Tensor):
         to.copy_(y)
         return
-    if len(to) != len(y) or any((a is None) != (b is None) for a, b in zip(to, y)):
-        raise ValueError('the targets must be as many tensors as the example had')
+    if to is None and y is None:
+        return
+    shape = lambda t: None if t is None else t.shape  # noqa: E731
+    if to is None or not isinstance(y, (tuple, list)) or [shape(t) for t in to] != [shape(t) for t in y]:  # (a copy would repeat what is shorter)
+        raise ValueError('the targets must be as many tensors as the example had, of the same shapes')
     for a, b in zip(to, y):
         if a is not None:
             a.copy_(b)

@@ -167,6 +167,27 @@ def test_offsets_that_are_not_one_for_each_sequence(offset):
         ops.relative_bias(torch.zeros(3, 2, 3, 4), torch.zeros(4, 2), 9, offset=torch.zeros(3, dtype=torch.long))
 
 
+def test_batches_of_several_targets():
+    from hgq2_amd.train import _copy_batch, _each
+
+    example = (torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.long), None)
+    to = _each(torch.Tensor.clone, example)
+    batch = (torch.rand(2, 3), torch.randint(0, 9, (2, 3)), None)
+    _copy_batch(to, list(batch))
+    assert torch.equal(to[0], batch[0]) and torch.equal(to[1], batch[1]) and to[2] is None and not example[0].any()
+    _copy_batch(None, None)
+    kept = _each(torch.Tensor.clone, to)
+    for wrong in (batch[:2], (*batch[:2], torch.rand(2)), (batch[0], None, None), (batch[0][:, :1], *batch[1:]), (batch[0], batch[1][:1], None), torch.rand(3, 2, 3), None):
+        with pytest.raises(ValueError, match='targets'):
+            _copy_batch(to, wrong)
+    with pytest.raises(ValueError, match='targets'):
+        _copy_batch(None, batch)
+    assert torch.equal(to[0], kept[0]) and torch.equal(to[1], kept[1])
+    single = torch.zeros(4)
+    _copy_batch(single, torch.arange(4.0))
+    assert torch.equal(single, torch.arange(4.0))
+
+
 @pytest.mark.parametrize('n,far', [(2, 2), (2, 100), (3, 9), (8, 40), (16, 128), (32, 128), (32, 33), (64, 500), (20, 1 << 30)])
 def test_first_distances(n, far):
     """The definition bucket by bucket, in whole numbers: the bucket of a distance is how many first distances are not above it."""
