@@ -649,7 +649,7 @@ def train_step_for(model, example_x, example_y, lr: float = 0.01, loss='sparse_c
     whole-step kernels; every other model, and every other loss, runs the per-layer operators replayed from a HIP graph
     (:class:`GraphedTrainStep` with :class:`SGD`, regularizers folded into the update).  ``loss``: ``'sparse_ce'``, ``'mse'``, ``'distill_topk'`` - the targets
     are a teacher's ``(logits, indices)``, or ``(logits, indices, lse, sample_weight)`` with ``None`` for what there is not
-    (:func:`hgq2_amd.ops.distill_topk`) - or a callable ``loss(outputs, y)`` of capturable operations, such as
+    (:func:`hgq2_amd.ops.distill_topk`, at temperature 1) - or a callable ``loss(outputs, y)`` of capturable operations, such as
     ``lambda out, y: ops.distill_topk(out, *y, temperature=2.0)``.  Both paths update the same
     variables with the same arithmetic (the whole-step kernels restate the per-layer sequence), so the choice changes
     the time per step and nothing else.  ``fused=False`` forces the per-layer path, ``fused=True`` raises where the
@@ -716,7 +716,7 @@ def fit(model, x, y, *, loss='sparse_ce', lr: float = 0.01, batch_size: int = 10
     every batch is trained on exactly once - and a shorter last batch through the same kernels launched one by one.
     On the replayed path the recorded step fetches its own batch (:class:`ResidentBatches`: the epoch's order lies in
     device memory and a launch at the head of the step gathers the next rows) and adds its loss to a running sum, so a
-    step costs the host one replay call.  The epoch's loss is summed on the device and read once per epoch.  On the per-layer path the MonoL1 terms of the
+    step costs the host one replay call; a ``y`` of several tensors is gathered and copied ahead of each replay instead.  The epoch's loss is summed on the device and read once per epoch.  On the per-layer path the MonoL1 terms of the
     variables are applied inside the update launch and are not part of a step's loss value: their sum
     (:func:`folded_regularizer_loss`, of the order of 1e-4 with the default 1e-8 factors) is added to ``logs['loss']``
     once, from the variables as they stand when the epoch ends; the whole-step kernels include it in every step."""
